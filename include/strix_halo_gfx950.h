@@ -447,6 +447,94 @@ int amd_strix_halo_kernels_quantize(int device_index, uintptr_t stream, const vo
                                     int64_t cols, int64_t ld_x, float inv_scale, int32_t bits, int32_t mode,
                                     void* out, int64_t ld_out);
 
+/* ---- quantized key/value cache ---------------------------------------------
+ * No counterpart in the reference.  A paged cache in int8 or int4: codes
+ * [pages, kv_heads, page_size, head_dim * bits / 8] (contiguous; int4 pairs
+ * along head_dim, the even element in the low nibble) and one bf16 scale for
+ * each row of head_dim codes, [pages, kv_heads, page_size].  The value of a
+ * code is code * scale.  bits 4 or 8, head_dim 64, 128 or 256, page_size a
+ * power of two from 16 to 1024; code pointers on 16 bytes, scales on 8. */
+typedef struct shk_kv_cache {
+  void* key_codes;
+  void* value_codes;
+  void* key_scales;
+  void* value_scales;
+  int64_t pages;
+  int64_t kv_heads;
+  int64_t page_size;
+  int64_t head_dim;
+  int64_t bits;
+} shk_kv_cache;
+
+/* Rows of tokens that go into the cache or come out of it: keys and values
+ * [tokens, kv_heads, head_dim], head_dim contiguous, strides in elements.
+ * Token t goes to slot slots[t] = page * page_size + position in the page. */
+typedef struct shk_kv_rows {
+  void* keys;
+  void* values;
+  int64_t key_token_stride;
+  int64_t key_head_stride;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  int64_t type; /* SHK_SRC_F32, SHK_SRC_F16 or SHK_SRC_BF16 */
+  const void* slots;
+  int64_t slot_bytes; /* 4 or 8: int32 or int64 slots */
+  int64_t tokens;
+} shk_kv_rows;
+
+/* Quantizes rows into their slots.  With Q = 7 (int4) or 127 (int8),
+ *   scale = bf16(fl32(max|x| / Q)),  code = clamp(rint(fl32(x / scale)), -Q, Q)
+ * rounding half to even; a zero scale has zero codes, and a row that holds an
+ * infinity or a NaN has a scale that reads back as NaN throughout.  Slots
+ * outside the cache (negative ones: padding) are skipped; the slots of a call
+ * are distinct. */
+int amd_strix_halo_kernels_kv_write(int device_index, uintptr_t stream, const shk_kv_cache* cache,
+                                    const shk_kv_rows* rows);
+/* code * scale of each slot, rounded once to the rows' type; NaN for slots
+ * outside the cache. */
+int amd_strix_halo_kernels_kv_read(int device_index, uintptr_t stream, const shk_kv_cache* cache,
+                                   const shk_kv_rows* rows);
+
+/* Attention of each sequence's newest `queries` tokens over its cached tokens.
+ * q [batch, queries, heads, head_dim] (head_dim contiguous, strides in
+ * elements, 16-byte aligned rows) f16 or bf16; query head h reads key head
+ * h / (heads / kv_heads).  Sequence b holds lengths[b] tokens in the pages
+ * page_table[b * table_stride ...], its `queries` newest tokens among them;
+ * query t sees the first lengths[b] - queries + t + 1 of them, after the
+ * prefix_length tokens of prefix_pages, which every query sees.
+ * out [batch, queries, heads, head_dim], contiguous, of q's type:
+ *   softmax(scale * q k^T) v;  lse [batch, queries, heads] f32 or null: the
+ * natural logarithm of the sum of exponentials.  A query that sees nothing
+ * gives 0 and -inf.  Lengths past table_pages * page_size count as that, and
+ * a page outside the cache makes its sequence's outputs NaN.
+ * workspace: at least amd_strix_halo_kernels_kv_attention_workspace bytes, on
+ * 16 bytes, not read before it is written. */
+typedef struct shk_kv_attention {
+  const void* q;
+  int64_t q_batch_stride;
+  int64_t q_query_stride;
+  int64_t q_head_stride;
+  int64_t type; /* SHK_SRC_F16 or SHK_SRC_BF16 */
+  int64_t batch;
+  int64_t queries;
+  int64_t heads;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int64_t table_pages; /* pages a row of the table holds */
+  const int32_t* lengths;
+  const int32_t* prefix_pages;
+  int64_t prefix_length;
+  double scale;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+} shk_kv_attention;
+
+int64_t amd_strix_halo_kernels_kv_attention_workspace(const shk_kv_cache* cache, const shk_kv_attention* args);
+int amd_strix_halo_kernels_kv_attention(int device_index, uintptr_t stream, const shk_kv_cache* cache,
+                                        const shk_kv_attention* args);
+
 #ifdef __cplusplus
 }
 #endif

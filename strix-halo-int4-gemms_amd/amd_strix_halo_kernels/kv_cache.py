@@ -1,0 +1,300 @@
+"""Quantized key/value cache of a decoder, and the attention that reads it.
+
+No counterpart in the reference, whose path ends at the GEMMs.  The cache is
+a pool of pages that sequences share; a page holds ``page_size`` tokens of
+every key head as int8 or packed int4 codes with one bf16 scale per row of
+``head_dim`` codes:
+
+    scale = bf16(max|x| / Q)          Q = 7 (int4) or 127 (int8)
+    code  = clamp(round(x / scale), -Q, Q)        value = code * scale
+
+in 32 bits, rounding half to even.  A row of zeros has scale 0 and reads back
+as zeros; a row that holds an infinity or a NaN reads back as NaN.
+
+``kv_cache_write`` quantizes new tokens into their slots, ``kv_cache_read``
+dequantizes slots, and ``kv_cache_attention`` is softmax attention of each
+sequence's newest tokens over its pages, after a prefix that the whole batch
+may share.  All run on the current stream of the tensors' device and read
+nothing back to the host; there is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import Any
+
+from . import kernel_table as kt
+from .native import _check, _device_index, _require_device, _stream_handle, _torch, _verified_library
+
+HEAD_DIMS = (64, 128, 256)
+_I64, _P = ctypes.c_int64, ctypes.c_void_p
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("key_codes", _P), ("value_codes", _P), ("key_scales", _P), ("value_scales", _P), ("pages", _I64),
+                ("kv_heads", _I64), ("page_size", _I64), ("head_dim", _I64), ("bits", _I64)]
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("keys", _P), ("values", _P), ("key_token_stride", _I64), ("key_head_stride", _I64),
+                ("value_token_stride", _I64), ("value_head_stride", _I64), ("type", _I64), ("slots", _P),
+                ("slot_bytes", _I64), ("tokens", _I64)]
+
+
+class _Attention(ctypes.Structure):
+    _fields_ = [("q", _P), ("q_batch_stride", _I64), ("q_query_stride", _I64), ("q_head_stride", _I64),
+                ("type", _I64), ("batch", _I64), ("queries", _I64), ("heads", _I64), ("page_table", _P),
+                ("table_stride", _I64), ("table_pages", _I64), ("lengths", _P), ("prefix_pages", _P),
+                ("prefix_length", _I64), ("scale", ctypes.c_double), ("out", _P), ("lse", _P), ("workspace", _P),
+                ("workspace_bytes", _I64)]
+
+
+@dataclass(frozen=True, eq=False)
+class KVCache:
+    """The tensors of one layer's cache; ``new_kv_cache`` makes them.
+
+    ``key_codes`` and ``value_codes`` are ``[pages, kv_heads, page_size,
+    head_dim]`` int8, or ``[..., head_dim / 2]`` uint8 with int4 pairs along
+    head_dim (the even element in the low nibble, as ``pack_int4_k_major``
+    packs); ``key_scales`` and ``value_scales`` are ``[pages, kv_heads,
+    page_size]`` bf16.  head_dim is 64, 128 or 256, page_size a power of two
+    from 16 to 1024.
+    """
+
+    key_codes: Any
+    value_codes: Any
+    key_scales: Any
+    value_scales: Any
+
+    def __post_init__(self) -> None:
+        torch = _torch()
+        codes = self.key_codes
+        if codes.dtype not in (torch.uint8, torch.int8):
+            raise ValueError(f"key_codes must be int8 codes or packed int4 torch.uint8; got {codes.dtype}")
+        if codes.ndim != 4:
+            raise ValueError("key_codes must have shape (pages, kv_heads, page_size, head_dim or head_dim/2); "
+                             f"got {tuple(codes.shape)}")
+        bits = 4 if codes.dtype == torch.uint8 else 8
+        pages, heads, page_size, row = (int(n) for n in codes.shape)
+        head_dim = row * 8 // bits
+        for name, want_shape, want_dtype in (("value_codes", codes.shape, codes.dtype),
+                                             ("key_scales", codes.shape[:3], torch.bfloat16),
+                                             ("value_scales", codes.shape[:3], torch.bfloat16)):
+            t = getattr(self, name)
+            if tuple(t.shape) != tuple(want_shape) or t.dtype != want_dtype:
+                raise ValueError(f"{name} must have shape {tuple(want_shape)} and dtype {want_dtype}; "
+                                 f"got {tuple(t.shape)} and {t.dtype}")
+        for name in ("key_codes", "value_codes", "key_scales", "value_scales"):
+            t = getattr(self, name)
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+            if t.device != codes.device:
+                raise ValueError(f"{name} is on {t.device}, expected {codes.device}")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}; got {head_dim}")
+        if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 1024; got {page_size}")
+        if not 1 <= heads <= 65535 or pages < 1:
+            raise ValueError(f"the cache needs at least one page and 1 to 65535 heads; got {pages} and {heads}")
+        native = _Cache(codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(),
+                        self.value_scales.data_ptr(), pages, heads, page_size, head_dim, bits)
+        for name, value in (("pages", pages), ("kv_heads", heads), ("page_size", page_size), ("head_dim", head_dim),
+                            ("bits", bits), ("device", codes.device), ("_native", native),
+                            ("_ref", ctypes.addressof(native))):
+            object.__setattr__(self, name, value)
+
+
+def new_kv_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, bits: int = 4,
+                 device: Any = "cuda") -> KVCache:
+    """A zero-filled cache of ``pages`` pages (every row reads back as zeros)."""
+    torch = _torch()
+    if bits not in (4, 8):
+        raise ValueError("bits must be 4 or 8")
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}; got {head_dim}")
+    shape = (pages, kv_heads, page_size)
+    dtype = torch.uint8 if bits == 4 else torch.int8
+    codes = [torch.zeros((*shape, head_dim * bits // 8), dtype=dtype, device=device) for _ in range(2)]
+    scales = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    return KVCache(*codes, *scales)
+
+
+def _row_type(torch: Any, name: str, dtype: Any) -> int:
+    if dtype == torch.bfloat16:
+        return kt.SRC_BF16
+    if dtype == torch.float16:
+        return kt.SRC_F16
+    if dtype == torch.float32:
+        return kt.SRC_F32
+    raise ValueError(f"{name} must have dtype torch.bfloat16, torch.float16 or torch.float32; got {dtype}")
+
+
+def _check_slots(torch: Any, slots: Any, tokens: int | None) -> None:
+    if slots.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"slots must have dtype torch.int64 or torch.int32; got {slots.dtype}")
+    if slots.ndim != 1 or (tokens is not None and slots.shape[0] != tokens):
+        want = "(tokens,)" if tokens is None else f"({tokens},)"
+        raise ValueError(f"slots must have shape {want}; got {tuple(slots.shape)}")
+    if not slots.is_contiguous():
+        raise ValueError("slots must be contiguous")
+
+
+def _rows(keys: Any, values: Any, slots: Any, kind: int, tokens: int) -> _Rows:
+    ks, vs = keys.stride(), values.stride()
+    return _Rows(keys.data_ptr(), values.data_ptr(), ks[0], ks[1], vs[0], vs[1], kind, slots.data_ptr(),
+                 slots.element_size(), tokens)
+
+
+def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream: Any | None = None) -> None:
+    """Quantizes ``keys`` and ``values`` [tokens, kv_heads, head_dim] (bf16,
+    f16 or f32; head_dim contiguous, other strides free) into the cache.
+
+    Token t goes to ``slots[t] = page * page_size + position`` (int64 or
+    int32).  Slots outside the cache, such as -1 for padding, are skipped; the
+    others are distinct.  One pass over memory, no copy of the inputs.
+    """
+    torch = _torch()
+    _require_device(torch, {"cache": cache.key_codes, "keys": keys, "values": values, "slots": slots})
+    kind = _row_type(torch, "keys", keys.dtype)
+    if values.dtype != keys.dtype:
+        raise ValueError(f"values must have the dtype of keys, {keys.dtype}; got {values.dtype}")
+    tokens = int(keys.shape[0]) if keys.ndim else 0
+    shape = (tokens, cache.kv_heads, cache.head_dim)
+    for name, t in (("keys", keys), ("values", values)):
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must have shape {shape} == (tokens, kv_heads, head_dim); got {tuple(t.shape)}")
+        if t.stride(2) != 1:
+            raise ValueError(f"{name} must be contiguous along head_dim")
+    _check_slots(torch, slots, tokens)
+    if tokens == 0:
+        return
+    lib = _verified_library()
+    _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, stream),
+                                                    cache._ref,
+                                                    ctypes.byref(_rows(keys, values, slots, kind, tokens))))
+
+
+def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any | None = None) -> tuple[Any, Any]:
+    """The keys and values of ``slots`` [tokens], dequantized to ``dtype``
+    (bf16, the default, f16 or f32): two [tokens, kv_heads, head_dim]
+    tensors.  Slots outside the cache give NaN."""
+    torch = _torch()
+    _require_device(torch, {"cache": cache.key_codes, "slots": slots})
+    dtype = torch.bfloat16 if dtype is None else dtype
+    kind = _row_type(torch, "the result", dtype)
+    _check_slots(torch, slots, None)
+    tokens = int(slots.shape[0])
+    keys, values = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    if tokens:
+        lib = _verified_library()
+        _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, stream),
+                                                       cache._ref,
+                                                    ctypes.byref(_rows(keys, values, slots, kind, tokens))))
+    return keys, values
+
+
+def kv_cache_attention(
+    q: Any,
+    cache: KVCache,
+    page_table: Any,
+    lengths: Any,
+    *,
+    prefix_pages: Any | None = None,
+    prefix_length: int = 0,
+    softmax_scale: float | None = None,
+    return_lse: bool = False,
+    out: Any | None = None,
+    stream: Any | None = None,
+) -> Any:
+    """Softmax attention of each sequence's newest tokens over its cached ones.
+
+    ``q`` is [batch, heads, head_dim] (one new token a sequence) or [batch,
+    queries, heads, head_dim], bf16 or f16, head_dim contiguous; heads is a
+    multiple of the cache's kv_heads, and query head h reads key head
+    ``h // (heads // kv_heads)``.  Sequence b holds ``lengths[b]`` tokens
+    (int32), the ``queries`` newest among them, in the pages
+    ``page_table[b]`` (int32 [batch, pages]); query t sees the first
+    ``lengths[b] - queries + t + 1``.
+
+    ``prefix_pages`` (int32 [pages]) and ``prefix_length`` name tokens that
+    come before every sequence's own, stored once and read once for the whole
+    batch; every query sees all of them.
+
+    Returns ``softmax(softmax_scale * q k^T) v`` in q's shape and dtype
+    (softmax_scale defaults to 1 / sqrt(head_dim)), and with ``return_lse``
+    also the natural logarithm of each row's sum of exponentials (f32, q's
+    shape without head_dim).  A query that sees nothing gives 0 and -inf.
+    A page outside the cache makes its sequence's outputs NaN.  Scores, the
+    softmax and the sums are f32; products take the codes as they are.
+    """
+    torch = _torch()
+    _require_device(torch, {"cache": cache.key_codes, "q": q, "page_table": page_table, "lengths": lengths,
+                            "prefix_pages": prefix_pages, "out": out})
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q must have dtype torch.bfloat16 or torch.float16; got {q.dtype}")
+    if q.ndim not in (3, 4) or q.shape[-1] != cache.head_dim:
+        raise ValueError(f"q must have shape (batch, heads, {cache.head_dim}) or (batch, queries, heads, "
+                         f"{cache.head_dim}); got {tuple(q.shape)}")
+    shape = q.shape
+    batch, heads = int(shape[0]), int(shape[-2])
+    queries = int(shape[1]) if q.ndim == 4 else 1
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"q's heads must be a multiple of the cache's {cache.kv_heads}; got {heads}")
+    if q.stride(-1) != 1:
+        raise ValueError("q must be contiguous along head_dim")
+    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise ValueError(f"page_table and lengths must have dtype torch.int32; got {page_table.dtype} and "
+                         f"{lengths.dtype}")
+    if page_table.ndim != 2 or page_table.shape[0] != batch:
+        raise ValueError(f"page_table must have shape ({batch}, pages); got {tuple(page_table.shape)}")
+    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        raise ValueError("rows of page_table must be contiguous")
+    if tuple(lengths.shape) != (batch,) or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be contiguous with shape ({batch},); got {tuple(lengths.shape)}")
+    if isinstance(prefix_length, bool) or not isinstance(prefix_length, int) or prefix_length < 0:
+        raise ValueError(f"prefix_length must be a non-negative int; got {prefix_length!r}")
+    if prefix_length:
+        if prefix_pages is None:
+            raise ValueError("prefix_length needs prefix_pages")
+        if prefix_pages.dtype != torch.int32 or prefix_pages.ndim != 1 or not prefix_pages.is_contiguous():
+            raise ValueError("prefix_pages must be a contiguous one-dimensional torch.int32 tensor; got "
+                             f"{prefix_pages.dtype} {tuple(prefix_pages.shape)}")
+        if prefix_pages.shape[0] * cache.page_size < prefix_length:
+            raise ValueError(f"prefix_pages holds {prefix_pages.shape[0] * cache.page_size} tokens; prefix_length is "
+                             f"{prefix_length}")
+    scale = 1.0 / math.sqrt(cache.head_dim) if softmax_scale is None else float(softmax_scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"softmax_scale must be finite; got {softmax_scale}")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous with shape {tuple(shape)} and dtype {q.dtype}; got "
+                         f"{tuple(out.shape)} and {out.dtype}")
+    lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    if batch * queries:
+        strides = q.stride()
+        sb, sq, sh = (strides[0], strides[1], strides[2]) if q.ndim == 4 else (strides[0], 0, strides[1])
+        if q.data_ptr() % 16 or sb % 8 or sq % 8 or sh % 8:
+            # 16-byte reads: rows that do not start on 16 bytes are copied
+            with torch.cuda.stream(stream):
+                q = q.clone(memory_format=torch.contiguous_format)
+            sb, sq, sh = queries * heads * cache.head_dim, heads * cache.head_dim, cache.head_dim
+        kind = kt.SRC_BF16 if q.dtype == torch.bfloat16 else kt.SRC_F16
+        args = _Attention(q.data_ptr(), sb, sq, sh, kind, batch, queries, heads, page_table.data_ptr(),
+                          page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
+                          prefix_pages.data_ptr() if prefix_length else None, prefix_length, scale, out.data_ptr(),
+                          lse.data_ptr() if return_lse else None, None, 0)
+        lib = _verified_library()
+        nbytes = lib.amd_strix_halo_kernels_kv_attention_workspace(cache._ref, ctypes.byref(args))
+        if nbytes < 0:
+            _check(lib, 1)
+        if nbytes:
+            work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            if stream is not None:
+                work.record_stream(stream)
+            args.workspace, args.workspace_bytes = work.data_ptr(), nbytes
+        _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, stream),
+                                                            cache._ref, ctypes.byref(args)))
+    return (out, lse) if return_lse else out

@@ -123,6 +123,15 @@ def _declare(lib: ctypes.CDLL) -> None:
     I64 = ctypes.c_int64
     lib.amd_strix_halo_kernels_quantize.argtypes = [I, U, P, I32, I64, I64, I64, ctypes.c_float, I32, I32, P, I64]
     lib.amd_strix_halo_kernels_quantize.restype = I
+    # the decode operators take their arguments in structs, passed by reference
+    lib.amd_strix_halo_kernels_kv_write.argtypes = [I, U, P, P]
+    lib.amd_strix_halo_kernels_kv_write.restype = I
+    lib.amd_strix_halo_kernels_kv_read.argtypes = [I, U, P, P]
+    lib.amd_strix_halo_kernels_kv_read.restype = I
+    lib.amd_strix_halo_kernels_kv_attention_workspace.argtypes = [P, P]
+    lib.amd_strix_halo_kernels_kv_attention_workspace.restype = I64
+    lib.amd_strix_halo_kernels_kv_attention.argtypes = [I, U, P, P]
+    lib.amd_strix_halo_kernels_kv_attention.restype = I
 
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:

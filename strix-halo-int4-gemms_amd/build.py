@@ -69,12 +69,15 @@ def translation_units() -> list[tuple[str, Path, list[str]]]:
     units.append(("ragged_f6", CSRC / "k_f6ragged.hip", list(DMA_FLAGS)))
     units.append(("ragged_skinny", CSRC / "k_ragskinny.hip", []))
     units.append(("quant", CSRC / "k_quant.hip", []))
+    units.append(("kvcache", CSRC / "k_kvcache.hip", []))
+    units.append(("kvattn", CSRC / "k_kvattn.hip", []))
     for layout in (0, 1, 2, 3):
         units.append((f"ragged_{layout}", CSRC / "k_ragged.hip", [f"-DSHK_LAYOUT={layout}"]))
     for bits in (4, 8):
         for layout in (0, 1, 2):
             units.append((f"skinny_{bits}_{layout}", CSRC / "k_skinny.hip", [f"-DSHK_BITS={bits}", f"-DSHK_LAYOUT={layout}"]))
     units.append(("capi", CSRC / "capi.hip", []))
+    units.append(("capi_decode", CSRC / "capi_decode.hip", []))
     return units
 
 

@@ -8,6 +8,7 @@
 #include <string>
 #include <vector>
 
+#include "shk_capi.h"
 #include "shk_quant.h"
 #include "shk_table.h"
 
@@ -59,6 +60,7 @@ __global__ __launch_bounds__(256) void clear_counters_kernel(int4* p, unsigned n
 
 namespace {
 
+using shk::DeviceGuard;
 using shk::Entry;
 
 thread_local std::string g_last_error;
@@ -129,31 +131,17 @@ const std::vector<Entry>& table() {
   return t;
 }
 
-// Makes `device` current for the duration of a launch and restores the
-// caller's device afterwards.
-class DeviceGuard {
- public:
-  explicit DeviceGuard(int device) {
-    if (hipGetDevice(&prev_) != hipSuccess) prev_ = -1;
-    if (prev_ != device) {
-      err_ = hipSetDevice(device);
-      switched_ = err_ == hipSuccess;
-    }
-  }
-  ~DeviceGuard() {
-    if (switched_ && prev_ >= 0) (void)hipSetDevice(prev_);
-  }
-  hipError_t error() const { return err_; }
-
- private:
-  int prev_ = -1;
-  bool switched_ = false;
-  hipError_t err_ = hipSuccess;
-};
-
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 }  // namespace
+
+namespace shk {
+
+int capi_fail(const std::string& msg) { return fail(msg); }
+int capi_fail_hip(const char* what, hipError_t err) { return fail_hip(what, err); }
+void capi_clear_error() { g_last_error.clear(); }
+
+}  // namespace shk
 
 // Scratch of amd_strix_halo_kernels_launch_gemm_noalloc: the fp6 operand
 // workspace of callers that cannot allocate device memory.  Each device the

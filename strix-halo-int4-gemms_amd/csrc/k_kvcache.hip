@@ -1,0 +1,269 @@
+// Keys and values into the quantized cache (kv_write) and out of it (kv_read).
+//
+// One row (token, head) is head_dim values x, stored as codes c and one scale:
+//   s = bf16(fl32(max|x| / Q)),  c = clamp(rint(fl32(x / s)), -Q, Q),
+// Q = 7 or 127.  Both kernels are one pass over memory: each value and each
+// code is touched once, by the lane that owns 8 consecutive values of a row
+// (16 bytes of a 2-byte type in, 4 or 8 bytes of codes out); head_dim / 8
+// lanes share a row and exchange its maximum.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "shk_common.h"
+#include "shk_kvcache.h"
+
+namespace shk {
+namespace {
+
+struct Rows {
+  const uint8_t* x[2];   // keys, values
+  uint8_t* codes[2];
+  uint16_t* scales[2];
+  long token_stride[2], head_stride[2];
+  const void* slots;
+  long slots_total;      // pages * page_size
+  long rows;             // tokens * kv_heads
+  int slot8, heads, page_shift;
+};
+
+__device__ __forceinline__ long slot_of(const Rows& p, long t) {
+  return p.slot8 ? static_cast<const int64_t*>(p.slots)[t] : static_cast<const int32_t*>(p.slots)[t];
+}
+
+// Row of the cache, counted in rows, of (slot, head).
+__device__ __forceinline__ long cache_row(const Rows& p, long slot, int head) {
+  const long page = slot >> p.page_shift;
+  return (((page * p.heads + head) << p.page_shift) | (slot & ((1L << p.page_shift) - 1)));
+}
+
+template <int TYPE>
+constexpr int kSize = TYPE == SHK_SRC_F32 ? 4 : 2;
+
+__device__ __forceinline__ float half_bits(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
+
+// 8 values starting at element address p; VEC: p is 16-byte aligned.
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load8(const uint8_t* p, float (&v)[8]) {
+  if constexpr (TYPE == SHK_SRC_F32) {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (VEC) {
+        const uint4 w = reinterpret_cast<const uint4*>(p)[i];
+        u[4 * i] = w.x, u[4 * i + 1] = w.y, u[4 * i + 2] = w.z, u[4 * i + 3] = w.w;
+      } else {
+        for (int j = 0; j < 4; ++j) u[4 * i + j] = reinterpret_cast<const uint32_t*>(p)[4 * i + j];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+  } else {
+    uint32_t u[4];
+    if constexpr (VEC) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = TYPE == SHK_SRC_BF16 ? __uint_as_float(u[i] << 16) : half_bits(u[i] & 0xFFFFu);
+      v[2 * i + 1] = TYPE == SHK_SRC_BF16 ? __uint_as_float(u[i] & 0xFFFF0000u) : half_bits(u[i] >> 16);
+    }
+  }
+}
+
+// fl32(x / s) for 8 values.  With inv = fl32(1 / s), q = fl32(x * inv) is
+// within one unit of x / s, its remainder x - q * s is exact in one fused
+// multiply-add, and q + remainder * inv rounds to fl32(x / s) (Markstein's
+// theorem) as long as nothing on the way leaves the normal range.  That
+// holds for the scales between the bounds, where codes matter (|x / s| of 2^-30
+// rounds to 0 either way); rows outside them divide.
+template <int BITS>
+__device__ __forceinline__ void codes8(const float (&v)[8], float s, int (&c)[8]) {
+  constexpr float Q = BITS == 4 ? 7.0f : 127.0f;
+  const bool usable = s > 0.0f && s < __builtin_inff();
+  float q[8];
+  if (s > 0x1p-60f && s < 0x1p60f) {
+    const float inv = 1.0f / s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q0 = v[i] * inv;
+      q[i] = __builtin_fmaf(__builtin_fmaf(-q0, s, v[i]), inv, q0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = v[i] / s;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = __builtin_fminf(__builtin_fmaxf(__builtin_rintf(q[i]), -Q), Q);
+    c[i] = usable ? (int)r : 0;
+  }
+}
+
+template <int TYPE, int BITS, int D, bool VEC>
+__global__ __launch_bounds__(256) void kv_write_kernel(const Rows p) {
+  constexpr int LANES = D / 8;  // of a row
+  const int which = blockIdx.y;
+  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int part = threadIdx.x % LANES;
+  const bool live = row < p.rows;
+  const long t = live ? row / p.heads : 0;
+  const int head = live ? (int)(row - t * p.heads) : 0;
+  long slot = live ? slot_of(p, t) : -1;
+  if (slot >= p.slots_total) slot = -1;
+  float v[8] = {};
+  const long from = t * p.token_stride[which] + head * p.head_stride[which] + part * 8;
+  if (slot >= 0) load8<TYPE, VEC>(p.x[which] + from * kSize<TYPE>, v);
+  // magnitudes as integers: a NaN is larger than an infinity, and both stay
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+  if (slot < 0) return;
+  const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (BITS == 4 ? 7.0f : 127.0f));
+  int c[8];
+  codes8<BITS>(v, __uint_as_float(sb << 16), c);
+  const long out = cache_row(p, slot, head);
+  uint8_t* dst = p.codes[which] + out * (D * BITS / 8) + part * BITS;
+  if constexpr (BITS == 4) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= ((uint32_t)c[i] & 0xFu) << (4 * i);
+    *reinterpret_cast<uint32_t*>(dst) = w;
+  } else {
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo |= ((uint32_t)c[i] & 0xFFu) << (8 * i);
+      hi |= ((uint32_t)c[i + 4] & 0xFFu) << (8 * i);
+    }
+    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+  }
+  if (part == 0) p.scales[which][out] = (uint16_t)sb;
+}
+
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
+  if constexpr (TYPE == SHK_SRC_F32) {
+    float* o = reinterpret_cast<float*>(p);
+    if constexpr (VEC) {
+      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      for (int i = 0; i < 8; ++i) o[i] = v[i];
+    }
+  } else {
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      b[i] = TYPE == SHK_SRC_BF16 ? f32_to_bf16_rne(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(b[0] | (b[1] << 16), b[2] | (b[3] << 16), b[4] | (b[5] << 16),
+                                                b[6] | (b[7] << 16));
+    } else {
+      for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)b[i];
+    }
+  }
+}
+
+template <int TYPE, int BITS, int D, bool VEC>
+__global__ __launch_bounds__(256) void kv_read_kernel(const Rows p) {
+  constexpr int LANES = D / 8;
+  const int which = blockIdx.y;
+  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
+  if (row >= p.rows) return;
+  const int part = threadIdx.x % LANES;
+  const long t = row / p.heads;
+  const int head = (int)(row - t * p.heads);
+  const long slot = slot_of(p, t);
+  float v[8];
+  if (slot >= 0 && slot < p.slots_total) {
+    const long at = cache_row(p, slot, head);
+    const uint8_t* src = p.codes[which] + at * (D * BITS / 8) + part * BITS;
+    const float s = bf16_bits_to_f32(p.scales[which][at]);
+    if constexpr (BITS == 4) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(src);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)((int32_t)(w << (28 - 4 * i)) >> 28) * s;
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(src);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i % 4))) * s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_nanf("");
+  }
+  uint8_t* dst = const_cast<uint8_t*>(p.x[which]) +
+                 (t * p.token_stride[which] + head * p.head_stride[which] + part * 8) * kSize<TYPE>;
+  store8<TYPE, VEC>(dst, v);
+}
+
+template <int TYPE, int BITS, int D, bool VEC>
+hipError_t launch(bool write, const Rows& p, hipStream_t s) {
+  const long blocks = (p.rows * (D / 8) + 255) / 256;
+  if (blocks > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
+  const dim3 grid((unsigned)blocks, 2);
+  if (write) hipLaunchKernelGGL((kv_write_kernel<TYPE, BITS, D, VEC>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((kv_read_kernel<TYPE, BITS, D, VEC>), grid, dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+template <int TYPE, int BITS, int D>
+hipError_t launch_d(bool write, bool vec, const Rows& p, hipStream_t s) {
+  return vec ? launch<TYPE, BITS, D, true>(write, p, s) : launch<TYPE, BITS, D, false>(write, p, s);
+}
+
+template <int TYPE, int BITS>
+hipError_t launch_b(bool write, bool vec, long d, const Rows& p, hipStream_t s) {
+  if (d == 64) return launch_d<TYPE, BITS, 64>(write, vec, p, s);
+  if (d == 128) return launch_d<TYPE, BITS, 128>(write, vec, p, s);
+  return launch_d<TYPE, BITS, 256>(write, vec, p, s);
+}
+
+template <int TYPE>
+hipError_t launch_t(bool write, bool vec, const shk_kv_cache& c, const Rows& p, hipStream_t s) {
+  return c.bits == 4 ? launch_b<TYPE, 4>(write, vec, c.head_dim, p, s)
+                     : launch_b<TYPE, 8>(write, vec, c.head_dim, p, s);
+}
+
+hipError_t rows_launch(bool write, const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s) {
+  Rows p{};
+  p.x[0] = static_cast<const uint8_t*>(r.keys), p.x[1] = static_cast<const uint8_t*>(r.values);
+  p.codes[0] = static_cast<uint8_t*>(c.key_codes), p.codes[1] = static_cast<uint8_t*>(c.value_codes);
+  p.scales[0] = static_cast<uint16_t*>(c.key_scales), p.scales[1] = static_cast<uint16_t*>(c.value_scales);
+  p.token_stride[0] = r.key_token_stride, p.token_stride[1] = r.value_token_stride;
+  p.head_stride[0] = r.key_head_stride, p.head_stride[1] = r.value_head_stride;
+  p.slots = r.slots;
+  p.slots_total = c.pages * c.page_size;
+  p.rows = r.tokens * c.kv_heads;
+  p.slot8 = r.slot_bytes == 8;
+  p.heads = (int)c.kv_heads;
+  p.page_shift = __builtin_ctzl((unsigned long)c.page_size);
+  if (p.rows == 0) return hipSuccess;
+  // 16-byte accesses where every row starts on 16 bytes
+  const long size = r.type == SHK_SRC_F32 ? 4 : 2;
+  const bool vec = ((reinterpret_cast<uintptr_t>(r.keys) | reinterpret_cast<uintptr_t>(r.values) |
+                     (uintptr_t)(size * (r.key_token_stride | r.key_head_stride | r.value_token_stride |
+                                         r.value_head_stride))) & 15) == 0;
+  if (r.type == SHK_SRC_F32) return launch_t<SHK_SRC_F32>(write, vec, c, p, s);
+  if (r.type == SHK_SRC_F16) return launch_t<SHK_SRC_F16>(write, vec, c, p, s);
+  return launch_t<SHK_SRC_BF16>(write, vec, c, p, s);
+}
+
+}  // namespace
+
+hipError_t launch_kv_write(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s) {
+  return rows_launch(true, c, r, s);
+}
+hipError_t launch_kv_read(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s) {
+  return rows_launch(false, c, r, s);
+}
+
+}  // namespace shk

@@ -1,0 +1,417 @@
+"""The quantized key/value cache and the attention over it, on the GPU.
+
+kv_cache_write and kv_cache_read are compared bit for bit with their 64-bit
+definition; kv_cache_attention with float64 attention over the same cached
+values, within bounds derived from its arithmetic (_decode_ref).  Everything
+that no token has been written to holds NaN scales, so a read of masked
+places shows.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import amd_strix_halo_kernels as shk  # noqa: E402
+from tests import _decode_ref as ref  # noqa: E402
+from tests._util import stable_seed  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def _cpu(cache):
+    return tuple(t.cpu() for t in (cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales))
+
+
+def _rows(seed, tokens, heads, dim, dtype):
+    g = torch.Generator().manual_seed(seed)
+    size = torch.exp(3 * torch.randn((2, tokens, heads, 1), generator=g))
+    return (torch.randn((2, tokens, heads, dim), generator=g) * size).to(dtype)
+
+
+def _same_bits(got, want):
+    return got.dtype == want.dtype and torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(
+        torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+# ---------------------------------------------------------------------------
+# Writing and reading
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("tokens,heads,page", [(1, 1, 16), (7, 3, 16), (130, 2, 64), (1025, 8, 128)])
+def test_write_then_read(dtype, bits, dim, tokens, heads, page, device):
+    print(f"case write {dtype} int{bits} {tokens}x{heads}x{dim} page {page}", flush=True)
+    seed = stable_seed("kv", dtype, bits, dim, tokens, heads, page)
+    x = _rows(seed, tokens, heads, dim, DTYPES[dtype])
+    x[0, 0, 0] = 0.0  # a row of zeros
+    pages = -(-tokens // page) + 2
+    cache = shk.new_kv_cache(pages, page, heads, dim, bits=bits, device=device)
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(seed))[:tokens]
+    xd = x.to(device)
+    shk.kv_cache_write(cache, xd[0], xd[1], slots.to(device))
+    for part, rows in (("key", x[0]), ("value", x[1])):
+        codes, scales = ref.quantized_rows(rows, bits)
+        got_codes = getattr(cache, f"{part}_codes").cpu()
+        got_scales = getattr(cache, f"{part}_scales").cpu()
+        want_codes, want_scales = torch.zeros_like(got_codes), torch.zeros_like(got_scales)
+        want_codes[slots // page, :, slots % page] = ref.pack(codes, bits)
+        want_scales[slots // page, :, slots % page] = scales
+        assert torch.equal(got_codes, want_codes) and torch.equal(got_scales, want_scales), part
+    for out in DTYPES.values():
+        got = shk.kv_cache_read(cache, slots.to(device).to(torch.int32), dtype=out)
+        for rows, values in zip(x, got):
+            codes, scales = ref.quantized_rows(rows, bits)
+            want = (codes.double() * scales.double()[..., None]).float().to(out)
+            assert values.shape == want.shape and _same_bits(values.cpu(), want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_of_extremes(bits, device):
+    """Rows whose scale leaves the range the fast quotient is used in, ties,
+    infinities and NaN."""
+    dim = 64
+    rows = torch.zeros((10, 1, dim))
+    rows[0] = 3e38
+    rows[1, 0, ::2] = 1e-38
+    rows[2, 0] = torch.arange(dim) * 2.0**-149  # f32 subnormals: the scale rounds to little or nothing
+    rows[3, 0, 5] = math.inf
+    rows[4, 0, 6] = math.nan
+    rows[5, 0] = (torch.arange(dim) - 32) * 0.5  # ties
+    rows[5, 0, 0] = 7.0 if bits == 4 else 127.0
+    rows[5, 0, 1:16] = torch.arange(15) * 0.5
+    rows[6] = -2.0**-60
+    rows[7, 0] = torch.linspace(-(2.0**70), 2.0**70, dim)
+    rows[8, 0, 0] = -math.inf
+    rows[9, 0] = torch.linspace(-(2.0**-80), 2.0**-81, dim)
+    cache = shk.new_kv_cache(1, 16, 1, dim, bits=bits, device=device)
+    slots = torch.arange(10, device=device)
+    shk.kv_cache_write(cache, rows.to(device), rows.to(device), slots)
+    codes, scales = ref.quantized_rows(rows, bits)
+    assert torch.equal(cache.key_codes.cpu()[0, :, :10].transpose(0, 1), ref.pack(codes, bits))
+    got = shk.kv_cache_read(cache, slots, dtype=torch.float32)[0].cpu()
+    want = (codes.double() * scales.double()[..., None]).float()
+    assert _same_bits(got, want)
+    assert torch.isnan(got[[3, 4, 8]]).all() and torch.isfinite(got[[0, 1, 2, 5, 6, 7, 9]]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_write_strided_and_misaligned_rows(dtype, device):
+    """Slices of a fused projection, a view that starts off 16 bytes, and
+    heads in reverse memory order of tokens."""
+    tokens, heads, dim = 33, 2, 128
+    x = _rows(stable_seed("strided", dtype), tokens, heads, dim, DTYPES[dtype])
+    fused = torch.empty((tokens, 3 * heads * dim + 3), dtype=DTYPES[dtype], device=device)
+    keys = fused[:, 1:1 + heads * dim].view(tokens, heads, dim)
+    values = torch.empty((heads, tokens, dim), dtype=DTYPES[dtype], device=device).transpose(0, 1)
+    keys.copy_(x[0])
+    values.copy_(x[1])
+    cache = shk.new_kv_cache(3, 16, heads, dim, bits=8, device=device)
+    slots = torch.arange(tokens, device=device)
+    shk.kv_cache_write(cache, keys, values, slots)
+    got = shk.kv_cache_read(cache, slots, dtype=torch.float32)
+    for rows, have in zip(x, got):
+        codes, scales = ref.quantized_rows(rows, 8)
+        assert torch.equal(have.cpu(), (codes.double() * scales.double()[..., None]).float())
+
+
+def test_slots_outside_the_cache(device):
+    cache = shk.new_kv_cache(2, 16, 1, 64, bits=4, device=device)
+    x = torch.ones((5, 1, 64), device=device, dtype=torch.bfloat16)
+    slots = torch.tensor([-1, 3, 32, 31, -(2**40)], device=device)
+    shk.kv_cache_write(cache, x, x, slots)
+    assert int((cache.key_scales != 0).sum()) == 2 and int((cache.value_codes != 0).any(dim=-1).sum()) == 2
+    got = shk.kv_cache_read(cache, slots)[0]
+    assert torch.isnan(got[[0, 2, 4]]).all() and torch.equal(got[[1, 3]], x[:2])
+
+
+def test_no_tokens(device):
+    cache = shk.new_kv_cache(1, 16, 2, 64, device=device)
+    none = torch.empty((0, 2, 64), device=device)
+    shk.kv_cache_write(cache, none, none, torch.empty(0, dtype=torch.int64, device=device))
+    keys, values = shk.kv_cache_read(cache, torch.empty(0, dtype=torch.int32, device=device))
+    assert keys.shape == values.shape == (0, 2, 64)
+
+
+# ---------------------------------------------------------------------------
+# Attention
+
+
+def _filled(seed, pages, page, heads, dim, bits, device):
+    """A cache of random rows, every scale NaN until _allow allows it."""
+    g = torch.Generator().manual_seed(seed)
+    most = 7 if bits == 4 else 127
+    codes = [ref.pack(torch.randint(-most, most + 1, (pages, heads, page, dim), generator=g), bits) for _ in range(2)]
+    scales = [((0.3 + torch.rand((pages, heads, page), generator=g)) * 1.2 / most).bfloat16() for _ in range(2)]
+    return codes, scales
+
+
+def _case(seed, lengths, *, queries=1, ratio=4, kv_heads=2, dim=128, bits=4, page=16, prefix=0, dtype="bf16", spare=1,
+          q_gain=2.0, device=None):
+    """q, the cache and its tables; tokens that are not held have NaN scales."""
+    g = torch.Generator().manual_seed(seed)
+    own = [-(-n // page) for n in lengths]
+    shared = -(-prefix // page)
+    total = sum(own) + shared + 1
+    codes, scales = _filled(seed, total, page, kv_heads, dim, bits, device)
+    order = torch.randperm(total, generator=g)
+    keep = torch.zeros((total, page), dtype=torch.bool)
+    # entries past a sequence's tokens are never read
+    table = torch.full((len(lengths), max(own + [0]) + spare), 2**31 - 1, dtype=torch.int32)
+    at = shared
+    for b, n in enumerate(own):
+        table[b, :n] = order[at:at + n]
+        for i in range(n):
+            keep[order[at + i], : min(page, lengths[b] - i * page)] = True
+        at += n
+    for i in range(shared):
+        keep[order[i], : min(page, prefix - i * page)] = True
+    for s in scales:
+        s.masked_fill_(~keep[:, None].expand_as(s), math.nan)
+    q = (q_gain * torch.randn((len(lengths), queries, kv_heads * ratio, dim), generator=g)).to(DTYPES[dtype])
+    cache = shk.KVCache(codes[0].to(device), codes[1].to(device), scales[0].to(device), scales[1].to(device))
+    return q, cache, table, torch.tensor(lengths, dtype=torch.int32), order[:shared].to(torch.int32)
+
+
+def _check(got, lse, q, cache, table, lengths, prefix_pages=None, prefix=0, scale=None):
+    want = ref.attention(q, _cpu(cache), table, lengths, prefix_pages, prefix, scale)
+    tokens = int(lengths.max()) + prefix
+    out_bound, lse_bound = ref.attention_bounds(q.dtype, q.shape[-1], tokens, *want)
+    got, lse = got.cpu().double().reshape(q.shape), lse.cpu().double().reshape(q.shape[:3])
+    assert torch.isfinite(got).all()
+    worst = ((got - want[0]).abs() - out_bound).max()
+    assert worst <= 0, f"out off by {float((got - want[0]).abs().max())}, {float(worst)} over its bound"
+    empty = want[1] == -math.inf
+    assert torch.equal(lse == -math.inf, empty) and (got[empty] == 0).all()
+    assert ((lse - want[1])[~empty].abs() <= lse_bound[~empty]).all()
+
+
+def _attend(q, cache, table, lengths, prefix_pages, prefix, device, **kw):
+    return shk.kv_cache_attention(q.to(device), cache, table.to(device), lengths.to(device), return_lse=True,
+                                  prefix_pages=prefix_pages.to(device) if prefix else None, prefix_length=prefix, **kw)
+
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 129, 300]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64, 1024])
+def test_single_tokens(dtype, bits, dim, page, device):
+    print(f"case attend {dtype} int{bits} dim {dim} page {page}", flush=True)
+    q, cache, table, lengths, _ = _case(stable_seed("one", dtype, bits, dim, page), LENGTHS, dim=dim, bits=bits,
+                                        page=page, dtype=dtype, device=device)
+    out, lse = _attend(q[:, 0], cache, table, lengths, None, 0, device)
+    assert out.shape == q[:, 0].shape and lse.shape == (len(LENGTHS), 8)
+    _check(out, lse, q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("queries,ratio,kv_heads", [(1, 1, 3), (1, 7, 1), (1, 17, 2), (2, 8, 2), (5, 4, 2), (33, 2, 1),
+                                                    (70, 1, 1)])
+@pytest.mark.parametrize("dtype,bits,dim", [("bf16", 4, 128), ("f16", 8, 64), ("bf16", 8, 256)])
+def test_several_queries(queries, ratio, kv_heads, dtype, bits, dim, device):
+    """Newest tokens of a sequence see what was written up to themselves;
+    sequences shorter than the number of queries leave rows empty."""
+    print(f"case attend queries {queries} ratio {ratio} heads {kv_heads} {dtype} int{bits} dim {dim}", flush=True)
+    q, cache, table, lengths, _ = _case(stable_seed("several", queries, ratio, kv_heads, dtype, bits, dim),
+                                        [0, 1, queries, 64, 150], queries=queries, ratio=ratio, kv_heads=kv_heads,
+                                        dtype=dtype, bits=bits, dim=dim, page=32, device=device)
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    _check(out, lse, q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("prefix", [1, 16, 63, 200, 1030])
+@pytest.mark.parametrize("batch,ratio,queries", [(1, 4, 1), (3, 8, 1), (40, 4, 1), (5, 2, 3)])
+@pytest.mark.parametrize("dtype,bits,dim", [("bf16", 4, 128), ("f16", 4, 64), ("bf16", 8, 256), ("f16", 8, 128)])
+def test_shared_prefix(prefix, batch, ratio, queries, dtype, bits, dim, device):
+    print(f"case prefix {prefix} batch {batch} ratio {ratio} queries {queries} {dtype} int{bits} dim {dim}", flush=True)
+    lengths = [(i * 37) % 90 for i in range(batch)]
+    q, cache, table, lengths, pages = _case(stable_seed("prefix", prefix, batch, ratio, queries, dtype, bits, dim),
+                                            lengths, queries=queries, ratio=ratio, dtype=dtype, bits=bits, dim=dim,
+                                            prefix=prefix, device=device)
+    out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+    _check(out, lse, q, cache, table, lengths, pages, prefix)
+
+
+def test_shared_prefix_equals_own_tokens(device):
+    """The prefix in front of each sequence's own pages is the same attention."""
+    q, cache, table, lengths, pages = _case(11, [20, 0, 47], prefix=64, page=16, device=device)
+    out, lse = _attend(q, cache, table, lengths, pages, 64, device)
+    joined = torch.cat((pages.expand(3, -1), table), dim=1)
+    whole, whole_lse = _attend(q, cache, joined, lengths + 64, None, 0, device)
+    assert (out.float() - whole.float()).abs().max() <= 2**-6 and (lse - whole_lse).abs().max() <= 2**-16
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_long_sequences_are_split_and_joined(dtype, bits, device):
+    q, cache, table, lengths, pages = _case(stable_seed("long", dtype, bits), [5003, 1, 0], ratio=4, kv_heads=1,
+                                            bits=bits, dtype=dtype, page=64, prefix=2049, device=device)
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    _check(out, lse, q, cache, table, lengths)
+    out, lse = _attend(q, cache, table, lengths, pages, 2049, device)
+    _check(out, lse, q, cache, table, lengths, pages, 2049)
+
+
+@pytest.mark.parametrize("gain", [0.0, 1e-30, 30.0, 1e4])
+def test_flat_and_peaked_scores(gain, device):
+    """All probabilities equal; and one that is all but 1, with scores in the
+    thousands."""
+    q, cache, table, lengths, _ = _case(77, [1, 40, 333], q_gain=gain, device=device)
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    _check(out, lse, q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_value_scales_far_apart(dtype, device):
+    """Scales of values over many powers of two, the largest at the end."""
+    q, cache, table, lengths, _ = _case(stable_seed("apart", dtype), [500], page=64, dtype=dtype, device=device)
+    at = torch.arange(cache.value_scales.shape[2], device=device)
+    for i in range(8):
+        cache.value_scales[int(table[0, i])] *= (2.0 ** ((i + at / 64) * 2 - 20)).bfloat16()
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    _check(out, lse, q, cache, table, lengths)
+
+
+def test_softmax_scale_and_strides(device):
+    q, cache, table, lengths, _ = _case(5, [90, 33], queries=2, device=device)
+    wide = torch.zeros((2, 2, 3 * q.shape[2], q.shape[3]), dtype=q.dtype, device=device)
+    wide[:, :, 8:16] = q.to(device)
+    tables = torch.zeros((2, 20), dtype=torch.int32, device=device)
+    tables[:, 5:5 + table.shape[1]] = table.to(device)
+    for scale in (0.3, -0.05):
+        out, lse = shk.kv_cache_attention(wide[:, :, 8:16], cache, tables[:, 5:5 + table.shape[1]], lengths.to(device),
+                                          softmax_scale=scale, return_lse=True)
+        _check(out, lse, q, cache, table, lengths, scale=scale)
+    flat = torch.zeros(q.numel() + 3, dtype=q.dtype, device=device)  # rows off 16 bytes
+    off = flat[3:].view(q.shape)
+    off.copy_(q)
+    out, lse = shk.kv_cache_attention(off, cache, table.to(device), lengths.to(device), return_lse=True)
+    _check(out, lse, q, cache, table, lengths)
+
+
+def test_nan_and_infinity_stay_in_their_sequence(device):
+    q, cache, table, lengths, _ = _case(9, [30, 30, 30], kv_heads=1, page=32, device=device)
+    cache.value_scales[int(table[1, 0]), 0, 7] = math.inf
+    cache.value_codes[int(table[1, 0]), 0, 7] = 0
+    cache.key_scales[int(table[2, 0]), 0, 3] = math.nan
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all() and torch.isnan(lse[2]).all()
+    assert torch.isfinite(lse[1]).all()
+    _check(out[:1], lse[:1], q[:1], cache, table[:1], lengths[:1])
+
+
+def test_pages_and_lengths_outside_the_cache(device):
+    q, cache, table, lengths, _ = _case(21, [30, 40, 20], page=16, spare=0, device=device)
+    table[1, 1] = 10**6
+    table[2, 1] = -3
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    assert torch.isnan(out[1:]).all() and torch.isnan(lse[1:]).all()
+    _check(out[:1], lse[:1], q[:1], cache, table[:1], lengths[:1])
+    # a length past the table counts as the whole table, a negative one as 0
+    odd = torch.tensor([16, 4000, -5], dtype=torch.int32)
+    long, _ = _attend(q, cache, table[:1, :1].expand(3, 1), odd, None, 0, device)
+    assert torch.isfinite(long).all() and (long[2] == 0).all()
+
+
+def test_no_sequences_and_no_pages(device):
+    q, cache, table, lengths, _ = _case(3, [4], device=device)
+    out = shk.kv_cache_attention(q[:0].to(device), cache, table[:0].to(device), lengths[:0].to(device))
+    assert out.shape == (0, 1, 8, 128)
+    out, lse = shk.kv_cache_attention(q.to(device), cache, table[:, :0].to(device), lengths.to(device), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_repeated_calls_give_the_same_bits(device):
+    q, cache, table, lengths, pages = _case(31, [700, 90], prefix=500, page=64, device=device)
+    first = _attend(q, cache, table, lengths, pages, 500, device)
+    for _ in range(3):
+        again = _attend(q, cache, table, lengths, pages, 500, device)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_other_stream_and_out(device):
+    q, cache, table, lengths, _ = _case(41, [700, 90], page=64, device=device)
+    qd, td, ld = q.to(device), table.to(device), lengths.to(device)
+    want = shk.kv_cache_attention(qd, cache, td, ld)
+    stream, out = torch.cuda.Stream(device), torch.zeros_like(qd)
+    torch.cuda.synchronize()
+    got = shk.kv_cache_attention(qd, cache, td, ld, out=out, stream=stream)
+    stream.synchronize()
+    assert got is out and torch.equal(out, want)
+
+
+def test_graph_of_a_step(device):
+    """Write and attention captured once; every replay equals the eager step
+    on what the buffers hold then."""
+    heads, dim, page = 2, 128, 16
+    cache = shk.new_kv_cache(8, page, heads, dim, bits=4, device=device)
+    table = torch.arange(8, dtype=torch.int32, device=device).view(2, 4)
+    lengths = torch.zeros(2, dtype=torch.int32, device=device)
+    kv = torch.zeros((2, 2, heads, dim), dtype=torch.bfloat16, device=device)
+    q = torch.zeros((2, 8, dim), dtype=torch.bfloat16, device=device)
+    slots = torch.zeros(2, dtype=torch.int64, device=device)
+    out = torch.zeros_like(q)
+
+    def step():
+        shk.kv_cache_write(cache, kv[0], kv[1], slots)
+        shk.kv_cache_attention(q, cache, table, lengths, out=out)
+
+    lengths.fill_(1)
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream(device).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    g = torch.Generator().manual_seed(1)
+    for t in range(5):
+        kv.copy_(torch.randn(kv.shape, generator=g))
+        q.copy_(torch.randn(q.shape, generator=g))
+        lengths.fill_(t + 1)
+        slots.copy_(torch.tensor([t, 64 + t]))
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        step()
+        assert torch.equal(got, out) and torch.isfinite(got).all()
+        _check(out, shk.kv_cache_attention(q, cache, table, lengths, return_lse=True)[1], q.cpu()[:, None], cache,
+               table.cpu(), lengths.cpu())
+
+
+def test_offsets_past_32_bits(device):
+    """A pool of more than 4 GiB a part: its last pages are written, read and
+    attended over as any others."""
+    heads, dim, page = 8, 256, 1024
+    pages = 2**32 // (heads * dim * page) + 3
+    shape = (pages, heads, page)
+    codes = [torch.empty((*shape, dim), dtype=torch.int8, device=device) for _ in range(2)]
+    scales = [torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    cache = shk.KVCache(*codes, *scales)
+    tokens = 77
+    x = _rows(123, tokens, heads, dim, torch.bfloat16)
+    x /= x.float().abs().amax(dim=-1, keepdim=True).bfloat16()
+    slots = (pages - 1) * page + torch.arange(tokens)
+    xd = x.to(device)
+    shk.kv_cache_write(cache, xd[0], xd[1], slots.to(device))
+    for rows, got in zip(x, shk.kv_cache_read(cache, slots.to(device), dtype=torch.float32)):
+        code, scale = ref.quantized_rows(rows, 8)
+        assert torch.equal(got.cpu(), (code.double() * scale.double()[..., None]).float())
+    q = torch.randn((1, 1, heads, dim), generator=torch.Generator().manual_seed(2)).bfloat16()
+    table, lengths = torch.tensor([[pages - 1]], dtype=torch.int32), torch.tensor([tokens], dtype=torch.int32)
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    last = tuple(t[-1:].cpu() for t in (*codes, *scales))
+    want = ref.attention(q, last, torch.zeros_like(table), lengths)
+    bounds = ref.attention_bounds(q.dtype, dim, tokens, *want)
+    assert ((out.cpu().double() - want[0]).abs() <= bounds[0]).all()
+    assert ((lse.cpu().double() - want[1]).abs() <= bounds[1]).all()
