@@ -69,16 +69,22 @@ def translation_units() -> list[tuple[str, Path, list[str]]]:
     units.append(("ragged_f6", CSRC / "k_f6ragged.hip", list(DMA_FLAGS)))
     units.append(("ragged_skinny", CSRC / "k_ragskinny.hip", []))
     units.append(("quant", CSRC / "k_quant.hip", []))
-    units.append(("kvcache", CSRC / "k_kvcache.hip", []))
-    units.append(("kvattn", CSRC / "k_kvattn.hip", []))
     for layout in (0, 1, 2, 3):
         units.append((f"ragged_{layout}", CSRC / "k_ragged.hip", [f"-DSHK_LAYOUT={layout}"]))
     for bits in (4, 8):
         for layout in (0, 1, 2):
             units.append((f"skinny_{bits}_{layout}", CSRC / "k_skinny.hip", [f"-DSHK_BITS={bits}", f"-DSHK_LAYOUT={layout}"]))
     units.append(("capi", CSRC / "capi.hip", []))
-    units.append(("capi_decode", CSRC / "capi_decode.hip", []))
     return units
+
+
+def decode_units() -> list[tuple[str, Path, list[str]]]:
+    """The decode step's operators: no inline assembly, default scheduler."""
+    return [
+        ("kvcache", CSRC / "k_kvcache.hip", []),
+        ("kvattn", CSRC / "k_kvattn.hip", []),
+        ("capi_decode", CSRC / "capi_decode.hip", []),
+    ]
 
 
 def _compile(unit: tuple[str, Path, list[str]]) -> tuple[str, float, str]:
@@ -94,7 +100,7 @@ def _compile(unit: tuple[str, Path, list[str]]) -> tuple[str, float, str]:
 
 def build(jobs: int | None = None, verbose: bool = True) -> Path:
     BUILD.mkdir(parents=True, exist_ok=True)
-    units = translation_units()
+    units = translation_units() + decode_units()
     jobs = jobs or min(len(units), int(os.environ.get("MAX_JOBS", os.cpu_count() or 4)), 16)
     t0 = time.time()
     with ThreadPoolExecutor(max_workers=jobs) as pool:
