@@ -535,6 +535,48 @@ int64_t amd_strix_halo_kernels_kv_attention_workspace(const shk_kv_cache* cache,
 int amd_strix_halo_kernels_kv_attention(int device_index, uintptr_t stream, const shk_kv_cache* cache,
                                         const shk_kv_attention* args);
 
+/* ---- mixture of experts for a few tokens -----------------------------------
+ * No counterpart in the reference (its ragged dots take quantized activations
+ * sorted by expert).  For each token t, with e = ids[t * top + j],
+ *   y[t] = sum_j share[t * top + j] * down_e(up_e(x[t]) * silu(gate_e(x[t])))
+ * on int4 weights and activations in their own type.  Weights as the ragged
+ * forward takes them, K of a packed byte pair in the low nibble first:
+ * layout NN up_gate [experts, ceil(hidden/2), 2 * inner] with the columns
+ * [up | gate], down [experts, ceil(inner/2), hidden]; NT up_gate [experts,
+ * 2 * inner, ceil(hidden/2)], down [experts, hidden, ceil(inner/2)].  Scales
+ * bf16: group 0 up_gate_scale [experts, 2 * inner], down_scale [experts,
+ * hidden]; group 32 to 256 (a multiple of 32) [experts, ceil(K/group), columns].
+ * Ids outside [0, experts) add nothing.  At most 64 tokens, 1024 pairs and
+ * 1024 experts.  x rows are contiguous (x_stride in elements), out [tokens,
+ * hidden] is contiguous, both of one type.  workspace: at least
+ * amd_strix_halo_kernels_moe_workspace bytes, on 16 bytes, not read before it
+ * is written. */
+typedef struct shk_moe {
+  const void* x;
+  int64_t x_stride;
+  int64_t type; /* SHK_SRC_F16 or SHK_SRC_BF16 */
+  int64_t tokens;
+  int64_t hidden;
+  int64_t inner;
+  int64_t experts;
+  int64_t top;
+  const void* up_gate;
+  const void* up_gate_scale;
+  const void* down;
+  const void* down_scale;
+  int64_t group;
+  int64_t layout; /* SHK_LAYOUT_NN or SHK_LAYOUT_NT */
+  const void* ids;
+  int64_t id_bytes; /* 4 or 8: int32 or int64 ids */
+  const float* share;
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+} shk_moe;
+
+int64_t amd_strix_halo_kernels_moe_workspace(const shk_moe* args);
+int amd_strix_halo_kernels_moe(int device_index, uintptr_t stream, const shk_moe* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,146 @@
+"""The gated mixture-of-experts layer for a few tokens.
+
+No counterpart in the reference, whose ragged dots take int4 activations
+sorted by expert.  ``moe_swiglu_int4`` takes a decode step's tokens as they
+are (bf16 or f16, unsorted, with the router's choices) and the experts' int4
+weights in the layouts of ``ragged_dot_int4``, and runs the whole layer:
+gather, up and gate products, SwiGLU, down product, weighted sum.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any
+
+from . import kernel_table as kt
+from .metadata import SUPPORTED_SUBCHANNELS, GemmLayout, ScaleMode, ScaleSpec
+from .native import _check, _device_index, _require_device, _stream_handle, _torch, _verified_library
+
+MOE_MAX_TOKENS = 64
+MOE_MAX_PAIRS = 1024
+MOE_MAX_EXPERTS = 1024
+_I64, _P = ctypes.c_int64, ctypes.c_void_p
+
+
+class _Moe(ctypes.Structure):
+    _fields_ = [("x", _P), ("x_stride", _I64), ("type", _I64), ("tokens", _I64), ("hidden", _I64), ("inner", _I64),
+                ("experts", _I64), ("top", _I64), ("up_gate", _P), ("up_gate_scale", _P), ("down", _P),
+                ("down_scale", _P), ("group", _I64), ("layout", _I64), ("ids", _P), ("id_bytes", _I64), ("share", _P),
+                ("out", _P), ("workspace", _P), ("workspace_bytes", _I64)]
+
+
+def _require(name: str, tensor: Any, shape: tuple[int, ...], dtype: Any, what: str) -> None:
+    if tuple(tensor.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape} == {what}; got {tuple(tensor.shape)}")
+    if tensor.dtype != dtype:
+        raise ValueError(f"{name} must have dtype {dtype}; got {tensor.dtype}")
+    if not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def moe_swiglu_int4(
+    x: Any,
+    up_gate: Any,
+    down: Any,
+    expert_ids: Any,
+    expert_weights: Any,
+    *,
+    up_gate_scale: Any,
+    down_scale: Any,
+    scale: ScaleSpec = ScaleSpec(ScaleMode.PER_CHANNEL),
+    layout: GemmLayout = GemmLayout.NN,
+    out: Any | None = None,
+    stream: Any | None = None,
+) -> Any:
+    """y[t] = sum_j expert_weights[t, j] * down_e(up_e(x[t]) * silu(gate_e(x[t]))),
+    with e = expert_ids[t, j].
+
+    ``x`` is [tokens, hidden] (bf16 or f16, rows contiguous), ``expert_ids``
+    [tokens, top] (int64 or int32) and ``expert_weights`` [tokens, top] f32,
+    as ``torch.topk`` over a router's probabilities leaves them; ids outside
+    the experts, such as -1 for padding, add nothing.  Weights are packed int4
+    (K in byte pairs) in the layouts of ``ragged_dot_int4``:
+
+    * NN: ``up_gate[E, ceil(hidden/2), 2*inner]`` with the columns [up | gate]
+      of ``fused_swiglu_up_gate``, ``down[E, ceil(inner/2), hidden]``;
+    * NT: ``up_gate[E, 2*inner, ceil(hidden/2)]``, ``down[E, hidden,
+      ceil(inner/2)]``.
+
+    Scales are bf16: per-channel ``up_gate_scale[E, 2*inner]`` and
+    ``down_scale[E, hidden]``, or with subchannel S ``[E, ceil(K/S), columns]``.
+    Activations are not quantized; sums and the value between the products
+    are f32.  Takes up to 64 tokens (larger batches are ``ragged_dot_int4``'s),
+    1024 (token, expert) pairs and 1024 experts.  Returns [tokens, hidden] in
+    x's dtype.  Nothing is read back to the host.
+    """
+    layout = GemmLayout(layout)
+    if layout not in (GemmLayout.NN, GemmLayout.NT):
+        raise ValueError(f"unsupported MoE layout {layout.value}; supported layouts are nn, nt")
+    torch = _torch()
+    _require_device(torch, {"x": x, "up_gate": up_gate, "down": down, "expert_ids": expert_ids,
+                            "expert_weights": expert_weights, "up_gate_scale": up_gate_scale,
+                            "down_scale": down_scale, "out": out})
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"x must have dtype torch.bfloat16 or torch.float16; got {x.dtype}")
+    if x.ndim != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must have shape (tokens, hidden); got {tuple(x.shape)}")
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        raise ValueError("rows of x must be contiguous")
+    tokens, hidden = int(x.shape[0]), int(x.shape[1])
+    if up_gate.ndim != 3 or up_gate.shape[0] < 1:
+        raise ValueError(f"up_gate must have shape (experts, K/2, N) or (experts, N, K/2); got {tuple(up_gate.shape)}")
+    experts = int(up_gate.shape[0])
+    nt = layout is GemmLayout.NT
+    columns = int(up_gate.shape[1 if nt else 2])
+    if columns < 2 or columns % 2:
+        raise ValueError(f"up_gate needs an even number of [up | gate] columns; got {columns}")
+    inner = columns // 2
+    k_up, k_down = (hidden + 1) // 2, (inner + 1) // 2
+    _require("up_gate", up_gate, (experts, columns, k_up) if nt else (experts, k_up, columns), torch.uint8,
+             "(experts, 2*inner, hidden/2)" if nt else "(experts, hidden/2, 2*inner)")
+    _require("down", down, (experts, hidden, k_down) if nt else (experts, k_down, hidden), torch.uint8,
+             "(experts, hidden, inner/2)" if nt else "(experts, inner/2, hidden)")
+    group = 0
+    if scale.mode is ScaleMode.SUBCHANNEL:
+        group = scale.subchannel_size or 0
+        if group not in SUPPORTED_SUBCHANNELS:
+            raise ValueError(f"subchannel_size must be one of {SUPPORTED_SUBCHANNELS}; got {group}")
+    for name, t, k, n in (("up_gate_scale", up_gate_scale, hidden, columns), ("down_scale", down_scale, inner, hidden)):
+        if group:
+            _require(name, t, (experts, -(-k // group), n), torch.bfloat16, "(experts, ceil(K/S), columns)")
+        else:
+            _require(name, t, (experts, n), torch.bfloat16, "(experts, columns)")
+    if expert_ids.ndim != 2 or expert_ids.shape[0] != tokens:
+        raise ValueError(f"expert_ids must have shape ({tokens}, top); got {tuple(expert_ids.shape)}")
+    top = int(expert_ids.shape[1])
+    if expert_ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"expert_ids must have dtype torch.int64 or torch.int32; got {expert_ids.dtype}")
+    _require("expert_weights", expert_weights, (tokens, top), torch.float32, "(tokens, top)")
+    if not expert_ids.is_contiguous():
+        raise ValueError("expert_ids must be contiguous")
+    if tokens > MOE_MAX_TOKENS or tokens * top > MOE_MAX_PAIRS:
+        raise ValueError(f"moe_swiglu_int4 takes up to {MOE_MAX_TOKENS} tokens and {MOE_MAX_PAIRS} (token, expert) "
+                         f"pairs; got {tokens} and {tokens * top}. Larger batches: ragged_dot_int4")
+    if experts > MOE_MAX_EXPERTS:
+        raise ValueError(f"moe_swiglu_int4 takes up to {MOE_MAX_EXPERTS} experts; got {experts}")
+    if out is None:
+        out = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device)
+    else:
+        _require("out", out, (tokens, hidden), x.dtype, "(tokens, hidden)")
+    if tokens == 0:
+        return out
+    args = _Moe(x.data_ptr(), x.stride(0), kt.SRC_BF16 if x.dtype == torch.bfloat16 else kt.SRC_F16, tokens, hidden,
+                inner, experts, top, up_gate.data_ptr(), up_gate_scale.data_ptr(), down.data_ptr(),
+                down_scale.data_ptr(), group, kt.LAYOUT_NT if nt else kt.LAYOUT_NN, expert_ids.data_ptr(),
+                expert_ids.element_size(), expert_weights.data_ptr(), out.data_ptr(), None, 0)
+    lib = _verified_library()
+    nbytes = lib.amd_strix_halo_kernels_moe_workspace(ctypes.byref(args))
+    if nbytes < 0:
+        _check(lib, 1)
+    if nbytes:
+        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        if stream is not None:
+            work.record_stream(stream)
+        args.workspace, args.workspace_bytes = work.data_ptr(), nbytes
+    _check(lib, lib.amd_strix_halo_kernels_moe(_device_index(x), _stream_handle(torch, x, stream), ctypes.byref(args)))
+    return out

@@ -132,6 +132,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.amd_strix_halo_kernels_kv_attention_workspace.restype = I64
     lib.amd_strix_halo_kernels_kv_attention.argtypes = [I, U, P, P]
     lib.amd_strix_halo_kernels_kv_attention.restype = I
+    lib.amd_strix_halo_kernels_moe_workspace.argtypes = [P]
+    lib.amd_strix_halo_kernels_moe_workspace.restype = I64
+    lib.amd_strix_halo_kernels_moe.argtypes = [I, U, P]
+    lib.amd_strix_halo_kernels_moe.restype = I
 
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:

@@ -83,6 +83,7 @@ def decode_units() -> list[tuple[str, Path, list[str]]]:
     return [
         ("kvcache", CSRC / "k_kvcache.hip", []),
         ("kvattn", CSRC / "k_kvattn.hip", []),
+        ("moe", CSRC / "k_moe.hip", []),
         ("capi_decode", CSRC / "capi_decode.hip", []),
     ]
 

@@ -5,6 +5,7 @@
 
 #include "shk_capi.h"
 #include "shk_kvcache.h"
+#include "shk_moe.h"
 
 namespace {
 
@@ -75,6 +76,22 @@ int check_attention(const shk_kv_cache* c, const shk_kv_attention* a) {
   return 0;
 }
 
+int check_moe(const shk_moe* a) {
+  if (a == nullptr) return capi_fail("moe arguments must be non-null");
+  if (a->type != SHK_SRC_F16 && a->type != SHK_SRC_BF16) return capi_fail("x is float16 or bfloat16");
+  if (a->layout != SHK_LAYOUT_NN && a->layout != SHK_LAYOUT_NT) return capi_fail("moe layouts are NN and NT");
+  if (a->group < 0 || a->group > 256 || a->group % 32 != 0)
+    return capi_fail("the scale group is 0 or a multiple of 32 up to 256; got " + std::to_string(a->group));
+  if (a->tokens < 0 || a->tokens > 64)
+    return capi_fail("at most 64 tokens a call; got " + std::to_string(a->tokens));
+  if (a->top < 0 || a->tokens * a->top > 1024) return capi_fail("at most 1024 (token, expert) pairs a call");
+  if (a->experts < 1 || a->experts > 1024) return capi_fail("1 to 1024 experts; got " + std::to_string(a->experts));
+  if (a->hidden < 1 || a->inner < 1 || a->hidden > (1 << 20) || a->inner > (1 << 20))
+    return capi_fail("hidden and inner must be from 1 to 1048576");
+  if (a->id_bytes != 4 && a->id_bytes != 8) return capi_fail("ids are int32 or int64");
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -119,6 +136,38 @@ int amd_strix_halo_kernels_kv_attention(int device_index, uintptr_t stream, cons
     const hipError_t err = shk::launch_kv_attention(*cache, a, reinterpret_cast<hipStream_t>(stream));
     if (err == hipErrorInvalidValue) return capi_fail("too many workgroups for one launch");
     if (err != hipSuccess) return capi_fail_hip("kv_attention launch", err);
+    return 0;
+  });
+}
+
+int64_t amd_strix_halo_kernels_moe_workspace(const shk_moe* args) {
+  int64_t bytes = -1;
+  (void)capi_entry([&] {
+    if (int rc = check_moe(args)) return rc;
+    bytes = shk::moe_workspace(*args);
+    return 0;
+  });
+  return bytes;
+}
+
+int amd_strix_halo_kernels_moe(int device_index, uintptr_t stream, const shk_moe* args) {
+  return capi_entry([&] {
+    if (int rc = check_moe(args)) return rc;
+    const shk_moe& a = *args;
+    if (a.tokens == 0) return 0;
+    if (!a.x || !a.out || !a.up_gate || !a.up_gate_scale || !a.down || !a.down_scale)
+      return capi_fail("x, out, weight and scale pointers must be non-null");
+    if (a.top > 0 && (!a.ids || !a.share)) return capi_fail("ids and share pointers must be non-null");
+    if (!on(a.x, 2) || !on(a.out, 2) || !on(a.up_gate_scale, 2) || !on(a.down_scale, 2) ||
+        !on(a.ids, (uintptr_t)a.id_bytes) || !on(a.share, 4))
+      return capi_fail("x, out, scales, ids and share must be aligned to their elements");
+    const int64_t need = shk::moe_workspace(a);
+    if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need || !on(a.workspace, 16)))
+      return capi_fail("the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
+    shk::DeviceGuard guard(device_index);
+    if (guard.error() != hipSuccess) return capi_fail_hip("hipSetDevice", guard.error());
+    const hipError_t err = shk::launch_moe(a, reinterpret_cast<hipStream_t>(stream));
+    if (err != hipSuccess) return capi_fail_hip("moe launch", err);
     return 0;
   });
 }

@@ -107,3 +107,43 @@ def attention_bounds(dtype, dim, tokens, out, lse, spread, scores, largest):
     under = tokens * 2.0**-37 * largest + 2.0**-25 * (dtype == torch.float16)
     return (half_ulp(dtype) * out.abs() + inside[..., None] * spread + under,
             ds + tokens * 2.0**-23 + 2.0**-22 * (lse.abs() + 1))
+
+
+def moe(x, up_gate, down, ids, share, up_scale, down_scale, group, layout):
+    """(y, bound) of the mixture-of-experts layer in float64 on CPU tensors.
+
+    The bound follows the layer's arithmetic.  A product's terms are exact
+    (activations to 2^-17 of themselves where they carry more than bf16's
+    bits) and summed in f32 with codes offset by 24: off by at most
+    K 2^-24 times the sum of |x| (|v| + 2 * 24 + 1) s.  h inherits that of up
+    and gate (silu's slope is at most 1.1) and 2^-20 of its own; y that of h,
+    a product's again, the f32 sum over the experts, and one rounding.
+    """
+    experts, inner = up_gate.shape[0], up_scale.shape[-1] // 2
+    xd = x.double()
+    y, bound = torch.zeros_like(xd), torch.zeros_like(xd)
+
+    def weight(packed, scale, e, k):
+        codes = unpack(packed[e] if layout == "nt" else packed[e].t().contiguous()).t()[:k].double()
+        s = scale[e].double()
+        s = s.repeat_interleave(group, dim=0)[:k] if group else s.expand(k, -1)
+        return codes * s, (codes.abs() + 49.0) * s.abs(), s.abs()
+
+    def product(v, k, e, packed, scale, extra):
+        """v @ W, and its bound given that of v."""
+        w, wide, s = weight(packed, scale, e, k)
+        return v @ w, extra @ w.abs() + k * 2.0**-24 * (v.abs() @ wide) + 2.0**-17 * (v.abs() @ w.abs())
+
+    for e in range(experts):
+        for t, j in (ids == e).nonzero().tolist():
+            v = xd[t:t + 1]
+            ug, off = product(v, v.shape[1], e, up_gate, up_scale, torch.zeros_like(v))
+            up, gate = ug[:, :inner], ug[:, inner:]
+            sig = torch.sigmoid(gate)
+            h = up * gate * sig
+            off_h = off[:, :inner] * (gate * sig).abs() + 1.1 * up.abs() * off[:, inner:] + 2 * off[:, :inner] * off[:, inner:]
+            z, off_z = product(h, inner, e, down, down_scale, off_h + 2.0**-20 * h.abs())
+            f = float(share[t, j])
+            y[t] += f * z[0]
+            bound[t] += abs(f) * (off_z[0] + ids.shape[1] * 2.0**-23 * z[0].abs())
+    return y, bound + half_ulp(x.dtype) * y.abs() + (2.0**-25 if x.dtype == torch.float16 else 0.0)

@@ -1,0 +1,196 @@
+"""The gated mixture-of-experts layer for a few tokens, on the GPU, against
+the layer in float64 within bounds derived from its arithmetic (_decode_ref)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import amd_strix_halo_kernels as shk  # noqa: E402
+from tests import _decode_ref as ref  # noqa: E402
+from tests._util import spec_of, stable_seed  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _case(seed, tokens, experts, top, hidden, inner, *, group=0, layout="nn", dtype="bf16"):
+    g = torch.Generator().manual_seed(seed)
+
+    def weight(k, n):
+        codes = ref.pack(torch.randint(-8, 8, (experts, n, k + k % 2), generator=g), 4)
+        rows = (experts, n) if not group else (experts, -(-k // group), n)
+        s = ((0.5 + torch.rand(rows, generator=g)) * 0.2 / math.sqrt(k)).bfloat16()
+        return (codes if layout == "nt" else codes.transpose(1, 2).contiguous()), s
+
+    up_gate, up_scale = weight(hidden, 2 * inner)
+    down, down_scale = weight(inner, hidden)
+    x = torch.randn((tokens, hidden), generator=g).to(DTYPES[dtype])
+    ids = torch.stack([torch.randperm(experts, generator=g)[:top] for _ in range(tokens)]) if tokens else torch.zeros(
+        (0, top), dtype=torch.int64)
+    share = torch.rand((tokens, top), generator=g)
+    return [x, up_gate, down, ids, share, up_scale, down_scale, group, layout]
+
+
+def _run(case, device, **kw):
+    x, up_gate, down, ids, share, up_scale, down_scale, group, layout = case
+    d = [t.to(device) for t in (x, up_gate, down, ids, share, up_scale, down_scale)]
+    return shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6], scale=spec_of(group),
+                               layout=shk.GemmLayout(layout), **kw)
+
+
+def _check(got, case):
+    want, bound = ref.moe(*case)
+    off = (got.cpu().double() - want).abs()
+    assert got.dtype == case[0].dtype and torch.isfinite(got).all()
+    assert (off <= bound).all(), f"off by {float(off.max())}, {float((off - bound).max())} over its bound"
+
+
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("group", [0, 32, 64, 128, 256])
+@pytest.mark.parametrize("tokens,experts,top,hidden,inner", [(1, 4, 2, 256, 192), (5, 3, 1, 320, 64), (16, 8, 3, 128, 320),
+                                                             (17, 2, 2, 288, 96), (64, 4, 2, 160, 128)])
+def test_layer(layout, dtype, group, tokens, experts, top, hidden, inner, device):
+    print(f"case moe {layout} {dtype} group {group} {tokens} tokens {experts} experts {hidden}x{inner}", flush=True)
+    case = _case(stable_seed("moe", layout, dtype, group, tokens, experts, top, hidden, inner), tokens, experts, top,
+                 hidden, inner, group=group, layout=layout, dtype=dtype)
+    _check(_run(case, device), case)
+
+
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("hidden,inner", [(1, 1), (2, 3), (7, 65), (33, 31), (65, 130), (257, 127), (130, 66)])
+def test_odd_sizes(layout, group, hidden, inner, device):
+    """Rows of any length and alignment, an odd K whose last nibble is padding
+    (here: any value)."""
+    print(f"case moe odd {layout} group {group} {hidden}x{inner}", flush=True)
+    for dtype in DTYPES:
+        case = _case(stable_seed("odd", layout, group, hidden, inner, dtype), 3, 5, 2, hidden, inner, group=group,
+                     layout=layout, dtype=dtype)
+        _check(_run(case, device), case)
+
+
+def test_experts_with_many_rows_and_none(device):
+    """All tokens through one expert of several, a token twice through the
+    same one, and most experts idle."""
+    case = _case(5, 64, 70, 2, 192, 64)
+    case[3][:] = 69
+    _check(_run(case, device), case)
+    case = _case(6, 1, 1000, 1, 64, 64)
+    case[3][:] = 999
+    _check(_run(case, device), case)
+
+
+def test_many_pairs(device):
+    case = _case(7, 64, 40, 16, 64, 64)
+    _check(_run(case, device), case)
+
+
+def test_ids_outside_the_experts_add_nothing(device):
+    case = _case(8, 6, 4, 2, 128, 64)
+    case[3][0] = -1
+    case[3][1, 0] = 4
+    case[3][2, 1] = -(2**40)
+    case[4][0] = math.nan  # a padded token's share is not read into anything
+    got = _run(case, device)
+    assert (got[0] == 0).all()
+    case[4][0] = 0.0
+    _check(got, case)
+    case[3] = case[3].clamp(-1, 4).to(torch.int32)
+    assert torch.equal(_run(case, device), got)
+
+
+def test_zero_scales_and_strided_x(device):
+    case = _case(9, 4, 3, 2, 256, 128, group=64)
+    case[5][:, 1] = 0.0
+    case[6][:, 0] = 0.0
+    wide = torch.full((4, 600), math.nan, dtype=torch.bfloat16)
+    wide[:, 33:33 + 256] = case[0]
+    got = shk.moe_swiglu_int4(wide.to(device)[:, 33:33 + 256], *(t.to(device) for t in case[1:5]),
+                              up_gate_scale=case[5].to(device), down_scale=case[6].to(device), scale=spec_of(64))
+    _check(got, case)
+
+
+def test_no_tokens_and_no_choices(device):
+    case = _case(10, 0, 3, 2, 64, 64)
+    assert _run(case, device).shape == (0, 64)
+    case = _case(11, 3, 3, 0, 64, 64)
+    case[3], case[4] = torch.zeros((3, 0), dtype=torch.int64), torch.zeros((3, 0))
+    assert (_run(case, device) == 0).all()
+
+
+def test_nan_stays_in_its_token(device):
+    case = _case(12, 3, 2, 2, 128, 64)
+    case[0][1, 5] = math.nan
+    got = _run(case, device)
+    assert torch.isnan(got[1]).all()
+    case[0][1, 5] = 0.0
+    want, bound = ref.moe(*case)
+    off = (got.cpu().double() - want).abs()
+    assert (off[[0, 2]] <= bound[[0, 2]]).all()
+
+
+def test_repeated_calls_streams_and_out(device):
+    case = _case(13, 20, 6, 2, 320, 192)
+    first = _run(case, device)
+    for _ in range(3):
+        assert torch.equal(_run(case, device), first)
+    stream, out = torch.cuda.Stream(device), torch.zeros_like(first)
+    d = [t.to(device) for t in case[:7]]
+    torch.cuda.synchronize()
+    got = shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6], out=out, stream=stream)
+    stream.synchronize()
+    assert got is out and torch.equal(out, first)
+
+
+def test_graph_of_the_layer(device):
+    case = _case(14, 4, 6, 2, 320, 192)
+    d = [t.to(device) for t in case[:7]]
+    out = torch.zeros_like(d[0])
+
+    def step():
+        shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6], out=out)
+
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream(device).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    g = torch.Generator().manual_seed(3)
+    for _ in range(4):
+        case[0] = torch.randn((4, 320), generator=g).bfloat16()
+        case[3] = torch.stack([torch.randperm(6, generator=g)[:2] for _ in range(4)])
+        d[0].copy_(case[0])
+        d[3].copy_(case[3])
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        step()
+        assert torch.equal(got, out)
+        _check(got, case)
+
+
+def test_weights_past_32_bits(device):
+    """The last expert of a weight of more than 4 GiB."""
+    hidden, inner = 512, 16384
+    case = _case(15, 2, 1, 1, hidden, inner)
+    experts = 2**32 // (hidden * inner) + 2
+    up_gate = torch.zeros((experts, hidden // 2, 2 * inner), dtype=torch.uint8, device=device)
+    assert up_gate.numel() > 2**32
+    down = torch.zeros((experts, inner // 2, hidden), dtype=torch.uint8, device=device)
+    up_scale = torch.zeros((experts, 2 * inner), dtype=torch.bfloat16, device=device)
+    down_scale = torch.zeros((experts, hidden), dtype=torch.bfloat16, device=device)
+    for whole, part in ((up_gate, case[1]), (down, case[2]), (up_scale, case[5]), (down_scale, case[6])):
+        whole[-1] = part[0].to(device)
+    ids = torch.full((2, 1), experts - 1, device=device)
+    got = shk.moe_swiglu_int4(case[0].to(device), up_gate, down, ids, case[4].to(device), up_gate_scale=up_scale,
+                              down_scale=down_scale)
+    _check(got, case)
