@@ -545,7 +545,7 @@ int amd_strix_halo_kernels_kv_attention(int device_index, uintptr_t stream, cons
  * [up | gate], down [experts, ceil(inner/2), hidden]; NT up_gate [experts,
  * 2 * inner, ceil(hidden/2)], down [experts, hidden, ceil(inner/2)].  Scales
  * bf16: group 0 up_gate_scale [experts, 2 * inner], down_scale [experts,
- * hidden]; group 32 to 256 (a multiple of 32) [experts, ceil(K/group), columns].
+ * hidden]; group 32, 64, 128 or 256 [experts, ceil(K/group), columns].
  * Ids outside [0, experts) add nothing.  At most 64 tokens, 1024 pairs and
  * 1024 experts.  x rows are contiguous (x_stride in elements), out [tokens,
  * hidden] is contiguous, both of one type.  workspace: at least

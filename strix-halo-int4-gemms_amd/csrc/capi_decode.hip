@@ -80,8 +80,8 @@ int check_moe(const shk_moe* a) {
   if (a == nullptr) return capi_fail("moe arguments must be non-null");
   if (a->type != SHK_SRC_F16 && a->type != SHK_SRC_BF16) return capi_fail("x is float16 or bfloat16");
   if (a->layout != SHK_LAYOUT_NN && a->layout != SHK_LAYOUT_NT) return capi_fail("moe layouts are NN and NT");
-  if (a->group < 0 || a->group > 256 || a->group % 32 != 0)
-    return capi_fail("the scale group is 0 or a multiple of 32 up to 256; got " + std::to_string(a->group));
+  if (a->group != 0 && a->group != 32 && a->group != 64 && a->group != 128 && a->group != 256)
+    return capi_fail("the scale group is 0, 32, 64, 128 or 256; got " + std::to_string(a->group));
   if (a->tokens < 0 || a->tokens > 64)
     return capi_fail("at most 64 tokens a call; got " + std::to_string(a->tokens));
   if (a->top < 0 || a->tokens * a->top > 1024) return capi_fail("at most 1024 (token, expert) pairs a call");

@@ -37,8 +37,15 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 8;
+typedef __attribute__((address_space(1))) const uint8_t* global_bytes;
+typedef __attribute__((address_space(1))) const uint16_t* global_halves;
+typedef uint32_t any_u32 __attribute__((aligned(1)));  // loads of any alignment
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef u2 any_u2 __attribute__((aligned(1)));
+typedef u4 any_u4 __attribute__((aligned(1)));
+
 constexpr int kHalf = 64;          // columns of half a workgroup's tile
+constexpr int kPitch = 2 * kHalf + 4;  // floats of an LDS row of sums: rows start on different banks
 constexpr int kSuper = 128;        // K values a wave loads at a time, four products deep
 constexpr int kMostPairs = 1024;   // (token, expert) pairs of a call
 constexpr int kMostExperts = 1024;
@@ -70,9 +77,9 @@ __device__ __forceinline__ f4 mfma_bf16(b8 a, b8 b, f4 c) {
 
 // The eight codes of a dword, each plus 24, in the order 0 4 1 5 2 6 3 7.
 __device__ __forceinline__ b8 expand(uint32_t w) {
-  w ^= 0x88888888u;
-  return __builtin_bit_cast(b8, u4{((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
-                                   ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u});
+  // 0x41C0: 16, with the nibble's sign bit flipped on the way
+  return __builtin_bit_cast(b8, u4{((w << 3) & 0x00780078u) ^ 0x41C041C0u, ((w >> 1) & 0x00780078u) ^ 0x41C041C0u,
+                                   ((w >> 5) & 0x00780078u) ^ 0x41C041C0u, ((w >> 9) & 0x00780078u) ^ 0x41C041C0u});
 }
 
 // Where a product's codes come from: the expert's matrix, and the end of all
@@ -82,43 +89,69 @@ struct Codes {
   int total, k_packed;  // columns of a row (NN) and bytes of one (NT)
 };
 
-// A uniform address, kept in scalar registers: the compiler would otherwise
-// keep one 64-bit vector address for every load of a piece.
-__device__ __forceinline__ const uint8_t* scalar(const uint8_t* p) {
-  asm("" : "+s"(p));
-  return p;
+// Loads from a uniform address, kept in scalar registers, plus a lane's 32-bit
+// offset: left to itself the compiler keeps one 64-bit vector address for every
+// load of a piece.  The address space is spelled out, since the empty asm hides
+// where the pointer comes from and flat loads cannot be waited for one by one.
+template <typename T>
+__device__ __forceinline__ T load_at(const uint8_t* p, uint32_t mine) {
+  global_bytes q = (global_bytes)p;
+  asm("" : "+s"(q));
+  return *(__attribute__((address_space(1))) const T*)(q + mine);
 }
 
 // 16 dwords of a lane: the codes of 128 K values from k0 for 64 columns from
 // n0, as they are stored.  What lies outside the expert's matrix meets
 // activations of zero or is not stored, so it may be anything.
 template <int LAYOUT>
-__device__ __forceinline__ void load_w(const Codes& s, int k0, int n0, uint32_t (&o)[16]) {
+__device__ __forceinline__ void load_half(const Codes& s, int k0, int n0, uint32_t (&o)[16]) {
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   if constexpr (LAYOUT == SHK_LAYOUT_NT) {  // [n][k_packed]: 16 bytes of the rows 4 c + j
     const uint32_t mine = (uint32_t)(4 * c * s.k_packed + 16 * g);
     const uint8_t* p = s.w + (long)n0 * s.k_packed + k0 / 2;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) __builtin_memcpy(&o[4 * j], scalar(p + (long)j * s.k_packed) + mine, 16);
+    for (int j = 0; j < 4; ++j) {
+      const u4 v = load_at<any_u4>(p + (long)j * s.k_packed, mine);
+      o[4 * j] = v[0], o[4 * j + 1] = v[1], o[4 * j + 2] = v[2], o[4 * j + 3] = v[3];
+    }
   } else {  // [k_packed][n]: four columns of the rows 16 q + 4 g + i
     const uint32_t mine = (uint32_t)(4 * g * s.total + 4 * c);
     const uint8_t* p = s.w + (long)(k0 / 2) * s.total + n0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      __builtin_memcpy(&o[i], scalar(p + (long)(16 * (i / 4) + i % 4) * s.total) + mine, 4);
+    for (int i = 0; i < 16; ++i) o[i] = load_at<any_u32>(p + (long)(16 * (i / 4) + i % 4) * s.total, mine);
+  }
+}
+
+// The codes of 128 K values for the 128 columns of a tile, in two halves of
+// 64 columns from n0 and n1.  WIDE: the halves are one stretch of columns,
+// and a lane's are 8 c + 4 half + j (otherwise 4 c + j of each half).
+template <int LAYOUT, bool WIDE>
+__device__ __forceinline__ void load_w(const Codes& s, int k0, int n0, int n1, uint32_t (&o)[2][16]) {
+  if constexpr (WIDE) {  // [k_packed][n]: eight columns of a row
+    const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
+    const uint32_t mine = (uint32_t)(4 * g * s.total + 8 * c);
+    const uint8_t* p = s.w + (long)(k0 / 2) * s.total + n0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const u2 v = load_at<any_u2>(p + (long)(16 * (i / 4) + i % 4) * s.total, mine);
+      o[0][i] = v[0], o[1][i] = v[1];
+    }
+  } else {
+    load_half<LAYOUT>(s, k0, n0, o[0]);
+    load_half<LAYOUT>(s, k0, n1, o[1]);
   }
 }
 
 // The same where part of it lies past the end of all codes, by way of 16
 // dwords of LDS a lane (few registers; at most the last expert's last pieces).
-template <int LAYOUT>
+template <int LAYOUT, bool WIDE>
 __device__ __forceinline__ void load_w_end(const Codes& s, int k0, int n0, uint32_t* lds, uint32_t (&o)[16]) {
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
 #pragma unroll 1
   for (int i = 0; i < 16; ++i) {
     const uint8_t* p = LAYOUT == SHK_LAYOUT_NT
                            ? s.w + (long)(n0 + 4 * c + i / 4) * s.k_packed + k0 / 2 + 16 * g + 4 * (i % 4)
-                           : s.w + (long)(k0 / 2 + 16 * (i / 4) + 4 * g + i % 4) * s.total + n0 + 4 * c;
+                           : s.w + (long)(k0 / 2 + 16 * (i / 4) + 4 * g + i % 4) * s.total + n0 + (WIDE ? 8 : 4) * c;
     // the last dword there is, shifted to where it would be
     const long over = p - (s.end - 4);
     uint32_t v;
@@ -173,12 +206,12 @@ template <bool FIRST, int TYPE>
 constexpr int kTerms = FIRST && TYPE == SHK_SRC_BF16 ? 1 : 2;
 
 template <bool FIRST, int TYPE>
-__device__ __forceinline__ void load_x(const MoeArgs& a, const uint16_t* row, int k, u4 (&o)[kLoads<FIRST, TYPE>]) {
+__device__ __forceinline__ void load_x(const MoeArgs& a, global_halves row, int k, u4 (&o)[kLoads<FIRST, TYPE>]) {
   if constexpr (FIRST) {
-    __builtin_memcpy(&o[0], row + k, 16);
+    o[0] = *(__attribute__((address_space(1))) const any_u4*)(row + k);
   } else {
-    o[0] = *reinterpret_cast<const u4*>(row + k);
-    o[1] = *reinterpret_cast<const u4*>(row + a.inner_pad + k);
+    o[0] = *(__attribute__((address_space(1))) const u4*)(row + k);
+    o[1] = *(__attribute__((address_space(1))) const u4*)(row + a.inner_pad + k);
   }
 }
 
@@ -204,32 +237,333 @@ __device__ __forceinline__ void terms(const u4 (&u)[kLoads<FIRST, TYPE>], b8 (&t
   }
 }
 
-// One product of the layer.  FIRST: up and gate, h = up * silu(gate) to a.h,
-// the halves of the tile being the same 64 columns of each; otherwise down,
-// 128 columns, to a.part.  RT: row tiles of 16 tokens a pass.
-template <int LAYOUT, bool FIRST, int RT, int TYPE, bool GROUPED>
-__global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
-  constexpr int kPitch = 2 * kHalf + 4;
-  constexpr int kStep = FIRST ? kHalf : 2 * kHalf;  // columns from one workgroup to the next
+// Where the columns of lane group g's sums r start, in the 128 of a tile.
+template <bool WIDE>
+__device__ __forceinline__ int column(int half, int g, int r) {
+  return WIDE ? 32 * g + 8 * r + 4 * half : kHalf * half + 16 * g + 4 * r;
+}
+
+// A workgroup's tile for the pairs list[row0 ..] of an expert, at most 16 * RT
+// of them.
+template <int LAYOUT, bool FIRST, int RT, int TYPE, bool GROUPED, int kWaves>
+__device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const uint16_t* scale, const uint16_t* list,
+                                         int rows, int row0, int n0, int k_first, int k_last, float* red,
+                                         uint32_t* lds_scale) {
   constexpr int kT = kTerms<FIRST, TYPE>, kL = kLoads<FIRST, TYPE>;
-  // the waves' sums, and before them 1024 dwords a wave for what ends in a piece
-  __shared__ __align__(16) float red[kWaves / 2][16 * kPitch];
-  static_assert(sizeof(red) >= kWaves * 4096, "room for the pieces that end");
-  __shared__ uint16_t list[kMostPairs];
-  __shared__ int count[kMostExperts];
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int n1 = n0 + (FIRST ? a.cols : kHalf);  // the second half's first column
+  const __bf16 one = (__bf16)1.0f;
+  const b8 ones = {one, one, one, one, one, one, one, one};
+
+  // columns of a product without a row repeat the last one; they are not stored
+  global_halves src[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int p = list[min(row0 + 16 * t + c, rows - 1)];
+    src[t] = FIRST ? (global_halves)a.x + (p / a.top) * a.x_stride : (global_halves)a.h + (long)p * 2 * a.inner_pad;
+  }
+  f4 acc[RT][8], sum[RT][2], all[RT][GROUPED ? 8 : 1];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    sum[t][0] = sum[t][1] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      acc[t][j] = f4{0, 0, 0, 0};
+      if constexpr (GROUPED) all[t][j] = f4{0, 0, 0, 0};
+    }
+  }
+  uint32_t* lds = reinterpret_cast<uint32_t*>(red) + 1024 * wave;
+  constexpr bool kWide = !FIRST && LAYOUT == SHK_LAYOUT_NN && RT == 1;
+  struct Block {  // 128 K values: the codes of both halves, the activations, and the scales of up to four groups
+    uint32_t w[2][16];
+    u4 x[RT][4][kL];
+    uint32_t sc[GROUPED ? 4 : 1];  // of two columns: the half lane / 32, columns 2 (lane % 32)
+  };
+  // Pieces from before `whole` lie inside the codes, the activations and the
+  // scales.
+  const int sc_n = (lane < 32 ? n0 : n1) + 2 * (lane % 32);
+  auto fits = [&](int k0) {
+    const bool scales = !GROUPED || scale + (long)min((k0 + kSuper - 1) / a.group, a.groups - 1) * s.total + n1 + kHalf <=
+                                        a.scale + (long)a.experts * a.groups * s.total;
+    return scales && inside<LAYOUT>(s, k0, n0) && inside<LAYOUT>(s, k0, n1);
+  };
+  int whole = FIRST ? min(k_last, a.k - kSuper + 1) : k_last;
+  while (whole > k_first && !fits(whole - 1)) whole -= kSuper;
+  const int last = k_first + (max(whole - k_first, 1) - 1) / kSuper * kSuper;  // the last of them
+  auto load_scales = [&](int k0, auto end, Block& b) {
+    if constexpr (GROUPED) {
+      const int count = a.group >= kSuper ? 1 : kSuper / a.group;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < count) {
+          const uint16_t* p = scale + (long)min(k0 / a.group + i, a.groups - 1) * s.total;
+          if constexpr (decltype(end)::value)
+            b.sc[i] = p[min(sc_n, s.total - 1)] | ((uint32_t)p[min(sc_n + 1, s.total - 1)] << 16);
+          else
+            b.sc[i] = load_at<any_u32>(reinterpret_cast<const uint8_t*>(p), 2u * (uint32_t)sc_n);
+        }
+    }
+  };
+  auto load_rows = [&](int k0, u4 (&x)[RT][4][kL]) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) load_x<FIRST, TYPE>(a, src[t], k0 + 32 * q + 8 * g, x[t][q]);
+  };
+  auto load_end = [&](int k0, Block& b) {  // by way of LDS
+    load_scales(k0, std::true_type{}, b);
+    load_w_end<LAYOUT, kWide>(s, k0, n0, lds, b.w[0]);
+    load_w_end<LAYOUT, kWide>(s, k0, kWide ? n0 + 4 : n1, lds, b.w[1]);
+    if constexpr (FIRST) {  // zeros past the end of x
+      uint16_t* h = reinterpret_cast<uint16_t*>(lds) + 8 * lane;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+          const int k = k0 + 32 * (i / 8) + 8 * g + i % 8;
+          h[512 * (i / 8) + i % 8] = k < a.k ? src[t][k] : (uint16_t)0;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) b.x[t][q][0] = *reinterpret_cast<const u4*>(h + 512 * q);
+      }
+    } else {
+      load_rows(k0, b.x);
+    }
+  };
+  auto share_scales = [&](const Block& b) {  // to where the other lanes read them
+    if constexpr (GROUPED) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds_scale[64 * i + lane] = b.sc[i];
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  auto multiply = [&](int k0, auto half, Block& b) {
+    constexpr int kAt = decltype(half)::value;
+    uint32_t(&w)[16] = b.w[kAt];
+    arrange<LAYOUT>(w);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int k = k0 + 32 * q;
+      if (k < k_last) {
+        b8 xt[RT][kT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          terms<FIRST, TYPE>(b.x[t][q], xt[t]);
+#pragma unroll
+          for (int i = 0; i < kT; ++i)
+            if (GROUPED || kAt == 0) sum[t][kAt] = mfma_bf16(ones, xt[t][i], sum[t][kAt]);
+        }
+        uint32_t o[4];
+        step_codes<LAYOUT>(w, q, o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const b8 v = expand(o[j]);
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int i = 0; i < kT; ++i) acc[t][4 * kAt + j] = mfma_bf16(v, xt[t][i], acc[t][4 * kAt + j]);
+        }
+        if constexpr (GROUPED) {
+          if (k + 32 >= k_last || (k + 32) % a.group == 0) {
+            // the group ends: its sums, without the offset, times its scales
+            const uint16_t* sc = reinterpret_cast<const uint16_t*>(lds_scale) + 128 * (k / a.group - k0 / a.group);
+            float f[16];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const u2 v = *reinterpret_cast<const u2*>(sc + column<kWide>(kAt, g, r));
+              f[4 * r] = bf16_bits_to_f32((uint16_t)v[0]), f[4 * r + 1] = __uint_as_float(v[0] & 0xFFFF0000u);
+              f[4 * r + 2] = bf16_bits_to_f32((uint16_t)v[1]), f[4 * r + 3] = __uint_as_float(v[1] & 0xFFFF0000u);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  all[t][4 * kAt + j][r] +=
+                      f[4 * r + j] * (acc[t][4 * kAt + j][r] - 24.0f * sum[t][kAt][r]);
+                acc[t][4 * kAt + j] = f4{0, 0, 0, 0};
+              }
+              sum[t][kAt] = f4{0, 0, 0, 0};
+            }
+          }
+        }
+      }
+    }
+  };
+  constexpr std::integral_constant<int, 0> h0{};
+  constexpr std::integral_constant<int, 1> h1{};
+  // What is loaded ahead is loaded whether it comes or not (the last piece
+  // again): a load that may not happen would have to be waited for as if it
+  // were the latest.
+  int k0 = k_first;
+  if (k0 < whole) {
+    if constexpr (RT == 1 && (kWide || LAYOUT == SHK_LAYOUT_NT)) {
+      // the next 128 K values are on their way while these are multiplied
+      auto load = [&](int k, Block& b) {
+        load_scales(k, std::false_type{}, b);
+        load_w<LAYOUT, kWide>(s, k, n0, n1, b.w);
+        load_rows(k, b.x);
+      };
+      auto use = [&](Block& b) {
+        share_scales(b);
+        multiply(k0, h0, b);
+        multiply(k0, h1, b);
+        return (k0 += kSuper) < whole;
+      };
+      Block b0, b1;
+      load(k0, b0);
+      while (true) {
+        load(min(k0 + kSuper, last), b1);
+        if (!use(b0)) break;
+        load(min(k0 + kSuper, last), b0);
+        if (!use(b1)) break;
+      }
+    } else {
+      // Each half's codes are on their way while the other half is
+      // multiplied: two sets of 32 loads would pass the 63 that can be
+      // counted, and with RT = 2 the registers.  So are the activations where
+      // they take few registers.
+      constexpr bool kAhead = RT * kL == 1 || (RT * kL == 2 && !GROUPED);
+      Block b;
+      if constexpr (kAhead) load_rows(k0, b.x);
+      load_half<LAYOUT>(s, k0, n0, b.w[0]);
+      if constexpr (kAhead) load_half<LAYOUT>(s, k0, n1, b.w[1]);
+      for (; k0 < whole; k0 += kSuper) {
+        const int next = min(k0 + kSuper, last);
+        load_scales(k0, std::false_type{}, b);
+        if constexpr (kAhead) {
+          share_scales(b);
+          multiply(k0, h0, b);
+          u4 x[RT][4][kL];
+          load_rows(next, x);
+          load_half<LAYOUT>(s, next, n0, b.w[0]);
+          multiply(k0, h1, b);
+          load_half<LAYOUT>(s, next, n1, b.w[1]);
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int i = 0; i < kL; ++i) b.x[t][q][i] = x[t][q][i];
+        } else {
+          load_rows(k0, b.x);
+          load_half<LAYOUT>(s, k0, n1, b.w[1]);
+          share_scales(b);
+          multiply(k0, h0, b);
+          load_half<LAYOUT>(s, next, n0, b.w[0]);
+          multiply(k0, h1, b);
+        }
+      }
+    }
+  }
+  for (; k0 < k_last; k0 += kSuper) {
+    Block b;
+    load_end(k0, b);
+    share_scales(b);
+    multiply(k0, h0, b);
+    multiply(k0, h1, b);
+  }
+  // The waves' sums: lane (g, c) holds token c, columns column(half, g, r)
+  // + j.  The second half of the waves hand theirs to the first half.
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    f4 v[8];  // [half][r] over j
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (GROUPED) v[4 * half + r][j] = all[t][4 * half + j][r];
+          else v[4 * half + r][j] = acc[t][4 * half + j][r] - 24.0f * sum[t][0][r];
+        }
+    float* mine = &red[(wave % (kWaves / 2)) * 16 * kPitch + c * kPitch];
+    __syncthreads();
+    if (wave >= kWaves / 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<f4*>(mine + column<kWide>(i / 4, g, i % 4)) = v[i];
+    }
+    __syncthreads();
+    if (wave < kWaves / 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f4* at = reinterpret_cast<f4*>(mine + column<kWide>(i / 4, g, i % 4));
+        *at += v[i];
+      }
+    }
+    __syncthreads();
+    const int here = min(rows - row0 - 16 * t, 16);
+    if constexpr (FIRST) {
+      for (int i = threadIdx.x; i < here * kHalf; i += 64 * kWaves) {
+        const int r = i / kHalf, n = i % kHalf, col = n0 + n;
+        if (col >= a.inner_pad) continue;
+        float h = 0.0f;  // up to inner_pad
+        if (col < a.cols) {
+          float up = 0.0f, gate = 0.0f;
+#pragma unroll
+          for (int q = 0; q < kWaves / 2; ++q) up += red[q * 16 * kPitch + r * kPitch + n], gate += red[q * 16 * kPitch + r * kPitch + kHalf + n];
+          if constexpr (!GROUPED) up *= load_bf16(scale + col), gate *= load_bf16(scale + a.cols + col);
+          h = up * (gate / (1.0f + __expf(-gate)));
+        }
+        // place 2 i + u of an eight holds its element i + 4 u
+        const int at = (col & ~7) | (2 * (col & 3) + ((col >> 2) & 1));
+        const uint32_t hi = f32_to_bf16_rne(h);
+        uint16_t* dst = a.h + (long)list[row0 + 16 * t + r] * 2 * a.inner_pad + at;
+        dst[0] = (uint16_t)hi;
+        dst[a.inner_pad] = (uint16_t)f32_to_bf16_rne(h - bf16_bits_to_f32((uint16_t)hi));
+      }
+    } else {
+      for (int i = threadIdx.x; i < here * 2 * kHalf; i += 64 * kWaves) {
+        const int r = i / (2 * kHalf), n = i % (2 * kHalf), col = n0 + n;
+        if (col >= a.cols) continue;
+        float v2 = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kWaves / 2; ++q) v2 += red[q * 16 * kPitch + r * kPitch + n];
+        if constexpr (!GROUPED) v2 *= load_bf16(scale + col);
+        a.part[(long)list[row0 + 16 * t + r] * a.hidden + col] = v2;
+      }
+    }
+  }
+}
+
+// One product of the layer.  FIRST: up and gate, h = up * silu(gate) to a.h,
+// the halves of the tile being the same 64 columns of each; otherwise down,
+// 128 columns, to a.part.  RT: the most row
+// tiles of 16 tokens a pass over the codes serves.
+template <int LAYOUT, bool FIRST, int RT, int TYPE, bool GROUPED, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
+  constexpr int kStep = FIRST ? kHalf : 2 * kHalf;  // columns from one workgroup to the next
+  // the waves' sums, and before them 1024 dwords a wave for what ends in a piece
+  __shared__ __align__(16) float red[kWaves / 2 * 16 * kPitch];
+  static_assert(sizeof(red) >= kWaves * 4096, "room for the pieces that end");
+  __shared__ uint32_t lds_scale[GROUPED ? kWaves * 256 : 1];  // a wave's four groups of 128 scales
+  __shared__ uint16_t list[kMostPairs];
+  __shared__ int16_t id[kMostPairs];
+  __shared__ int count[kMostExperts];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int pairs = a.tokens * a.top;
+
+  // Workgroups go round the 8 XCDs in turn.  Where a row's piece is half a
+  // cache line (64 columns of NN), neighbouring tiles go to one XCD, which then
+  // fetches the line once: 205 -> 158 us for 14 experts of 2048 x 22016 bytes.
+  // Elsewhere that only narrows an XCD's addresses.
+  constexpr bool kNeighbours = FIRST && LAYOUT == SHK_LAYOUT_NN;
+  const int tile = kNeighbours ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+  if (tile * kStep >= (FIRST ? a.inner_pad : a.cols)) return;
 
   // the blockIdx.y-th expert that is hit, and its pairs in order
   int expert = -1, rank = blockIdx.y, rows = 0;
   if (pairs <= 64) {
     // experts in the order of their first pairs, all in a wave's registers
-    const int id = lane < pairs ? id_of(a, lane) : -1;
-    unsigned long open = __ballot(id >= 0), same = 0;
+    const int mine = lane < pairs ? id_of(a, lane) : -1;
+    unsigned long open = __ballot(mine >= 0), same = 0;
     for (; open != 0; --rank) {
-      const int e = __shfl(id, __builtin_ctzll(open), 64);
-      same = __ballot(id == e);
+      const int e = __shfl(mine, __builtin_ctzll(open), 64);
+      same = __ballot(mine == e);
       if (rank == 0) {
         expert = e;
         break;
@@ -238,32 +572,37 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
     }
     if (expert < 0) return;  // the same for all threads
     rows = __popcll(same);
-    if (wave == 0 && id == expert) list[__popcll(same & ((1ul << lane) - 1))] = (uint16_t)lane;
+    if (wave == 0 && mine == expert) list[__popcll(same & ((1ul << lane) - 1))] = (uint16_t)lane;
   } else {
-    // experts in ascending order, counted in LDS
+    // counted in LDS, those with more than 16 rows first: their workgroups
+    // take longest
     for (int e = threadIdx.x; e < a.experts; e += 64 * kWaves) count[e] = 0;
     __syncthreads();
     for (int p = threadIdx.x; p < pairs; p += 64 * kWaves) {
       const int e = id_of(a, p);
+      id[p] = (int16_t)e;
       if (e >= 0) atomicAdd(&count[e], 1);
     }
     __syncthreads();
-    for (int e0 = 0; e0 < a.experts; e0 += 64) {
-      unsigned long hit = __ballot(e0 + lane < a.experts && count[e0 + lane] > 0);
-      const int here = __popcll(hit);
-      if (rank < here) {
-        for (int i = 0; i < rank; ++i) hit &= hit - 1;
-        expert = e0 + __builtin_ctzll(hit);
-        break;
+    for (int many = 1; many >= 0 && expert < 0; --many) {
+      for (int e0 = 0; e0 < a.experts; e0 += 64) {
+        const int n = e0 + lane < a.experts ? count[e0 + lane] : 0;
+        unsigned long hit = __ballot(n > 0 && (n > 16) == (many != 0));
+        const int here = __popcll(hit);
+        if (rank < here) {
+          for (int i = 0; i < rank; ++i) hit &= hit - 1;
+          expert = e0 + __builtin_ctzll(hit);
+          break;
+        }
+        rank -= here;
       }
-      rank -= here;
     }
     if (expert < 0) return;
     rows = count[expert];
     if (wave == 0) {
       int at = 0;
       for (int p0 = 0; p0 < pairs; p0 += 64) {
-        const bool mine = p0 + lane < pairs && id_of(a, p0 + lane) == expert;
+        const bool mine = p0 + lane < pairs && id[p0 + lane] == expert;
         const unsigned long all = __ballot(mine);
         if (mine) list[at + __popcll(all & ((1ul << lane) - 1))] = (uint16_t)(p0 + lane);
         at += __popcll(all);
@@ -277,7 +616,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   constexpr int kColumns = FIRST ? 2 : 1;
   const Codes s{a.w + (long)expert * kColumns * a.cols * a.k_packed,
                 a.w + (long)a.experts * kColumns * a.cols * a.k_packed, kColumns * a.cols, a.k_packed};
-  const int n0 = blockIdx.x * kStep, n1 = n0 + (FIRST ? a.cols : kHalf);  // the halves' first columns
+  const int n0 = tile * kStep;
   const uint16_t* scale = a.scale + (long)expert * (GROUPED ? a.groups : 1) * s.total;
 
   // this wave's K: whole scale groups, in steps of 32
@@ -285,196 +624,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   const int units = (a.k + unit - 1) / unit, each = (units + kWaves - 1) / kWaves;
   const int k_first = min(a.k, wave * each * unit), k_last = min(a.k, (wave + 1) * each * unit);
 
-  const __bf16 one = (__bf16)1.0f;
-  const b8 ones = {one, one, one, one, one, one, one, one};
-
   for (int row0 = 0; row0 < rows; row0 += 16 * RT) {
     if (row0 > 0) __syncthreads();  // red has been read
-    // columns of a product without a row repeat the last one; they are not stored
-    const uint16_t* src[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int p = list[min(row0 + 16 * t + c, rows - 1)];
-      src[t] = FIRST ? static_cast<const uint16_t*>(a.x) + (p / a.top) * a.x_stride : a.h + (long)p * 2 * a.inner_pad;
-    }
-    f4 acc[RT][8], sum[RT][2], all[RT][GROUPED ? 8 : 1];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      sum[t][0] = sum[t][1] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        acc[t][j] = f4{0, 0, 0, 0};
-        if constexpr (GROUPED) all[t][j] = f4{0, 0, 0, 0};
-      }
-    }
-    uint32_t* lds = reinterpret_cast<uint32_t*>(&red[0][0]) + 1024 * wave;
-    u4 x[RT][4][kL];
-    uint32_t w0[16], w1[16];
-    auto codes = [&](int k0, int n, uint32_t (&w)[16]) {
-      if (inside<LAYOUT>(s, k0, n)) load_w<LAYOUT>(s, k0, n, w);
-      else load_w_end<LAYOUT>(s, k0, n, lds, w);
-    };
-    auto activations = [&](int k0, u4 (&o)[RT][4][kL]) {
-      if (FIRST && k0 + kSuper > a.k) {  // x ends in this piece: zeros past it, by way of LDS
-        uint16_t* h = reinterpret_cast<uint16_t*>(lds) + 8 * lane;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-#pragma unroll 1
-          for (int i = 0; i < 32; ++i) {
-            const int k = k0 + 32 * (i / 8) + 8 * g + i % 8;
-            h[512 * (i / 8) + i % 8] = k < a.k ? src[t][k] : (uint16_t)0;
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) o[t][q][0] = *reinterpret_cast<const u4*>(h + 512 * q);
-        }
-        return;
-      }
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) load_x<FIRST, TYPE>(a, src[t], k0 + 32 * q + 8 * g, o[t][q]);
-    };
-    auto multiply = [&](int k0, auto half, uint32_t (&w)[16]) {
-      constexpr int kAt = decltype(half)::value;
-      arrange<LAYOUT>(w);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int k = k0 + 32 * q;
-        if (k < k_last) {
-          b8 xt[RT][kT];
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            terms<FIRST, TYPE>(x[t][q], xt[t]);
-#pragma unroll
-            for (int i = 0; i < kT; ++i) sum[t][kAt] = mfma_bf16(ones, xt[t][i], sum[t][kAt]);
-          }
-          uint32_t o[4];
-          step_codes<LAYOUT>(w, q, o);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const b8 v = expand(o[j]);
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-              for (int i = 0; i < kT; ++i) acc[t][4 * kAt + j] = mfma_bf16(v, xt[t][i], acc[t][4 * kAt + j]);
-          }
-          if constexpr (GROUPED) {
-            if (k + 32 >= k_last || (k + 32) % a.group == 0) {
-              // the group ends: its sums, without the offset, times its scales
-              const uint16_t* sc = scale + (long)(k / a.group) * s.total;
-              const int n = (kAt ? n1 : n0) + 16 * g;
-              uint16_t f[16];
-              if ((kAt ? n1 : n0) + kHalf <= s.total) {
-                __builtin_memcpy(f, sc + n, 32);
-              } else {
-                uint16_t* h = reinterpret_cast<uint16_t*>(lds) + 16 * lane;
-#pragma unroll 1
-                for (int i = 0; i < 16; ++i) h[i] = sc[min(n + i, s.total - 1)];
-                __builtin_memcpy(f, h, 32);
-              }
-#pragma unroll
-              for (int t = 0; t < RT; ++t) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                  for (int r = 0; r < 4; ++r)
-                    all[t][4 * kAt + j][r] +=
-                        bf16_bits_to_f32(f[4 * r + j]) * (acc[t][4 * kAt + j][r] - 24.0f * sum[t][kAt][r]);
-                  acc[t][4 * kAt + j] = f4{0, 0, 0, 0};
-                }
-                sum[t][kAt] = f4{0, 0, 0, 0};
-              }
-            }
-          }
-        }
-      }
-    };
-    // Each half's codes are on their way while the other half is multiplied;
-    // so are the next activations where two sets of them fit the registers.
-    constexpr bool kAhead = RT * kL == 1;
-    if (k_first < k_last) {
-      if constexpr (kAhead) activations(k_first, x);
-      codes(k_first, n0, w0);
-    }
-    for (int k0 = k_first; k0 < k_last; k0 += kSuper) {
-      const bool more = k0 + kSuper < k_last;
-      if constexpr (!kAhead) activations(k0, x);
-      codes(k0, n1, w1);
-      multiply(k0, std::integral_constant<int, 0>{}, w0);
-      if (more) codes(k0 + kSuper, n0, w0);
-      if constexpr (kAhead) {
-        u4 xn[RT][4][kL];
-        if (more) activations(k0 + kSuper, xn);
-        multiply(k0, std::integral_constant<int, 1>{}, w1);
-        if (more) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) x[0][q][0] = xn[0][q][0];
-        }
-      } else {
-        multiply(k0, std::integral_constant<int, 1>{}, w1);
-      }
-    }
-    // The waves' sums: lane (g, c) holds token c, columns 16 g + 4 r + j of
-    // each half.  Waves 4 to 7 hand theirs to waves 0 to 3 first.
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      f4 v[8];  // [half][r] over j
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (GROUPED) v[4 * half + r][j] = all[t][4 * half + j][r];
-            else v[4 * half + r][j] = acc[t][4 * half + j][r] - 24.0f * sum[t][half][r];
-          }
-      float* mine = &red[wave % (kWaves / 2)][c * kPitch + 16 * g];
-      __syncthreads();
-      if (wave >= kWaves / 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<f4*>(mine + (i / 4) * kHalf + 4 * (i % 4)) = v[i];
-      }
-      __syncthreads();
-      if (wave < kWaves / 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          f4* at = reinterpret_cast<f4*>(mine + (i / 4) * kHalf + 4 * (i % 4));
-          *at += v[i];
-        }
-      }
-      __syncthreads();
-      const int here = min(rows - row0 - 16 * t, 16);
-      if constexpr (FIRST) {
-        for (int i = threadIdx.x; i < here * kHalf; i += 64 * kWaves) {
-          const int r = i / kHalf, n = i % kHalf, col = n0 + n;
-          if (col >= a.inner_pad) continue;
-          float h = 0.0f;  // up to inner_pad
-          if (col < a.cols) {
-            float up = 0.0f, gate = 0.0f;
-#pragma unroll
-            for (int q = 0; q < kWaves / 2; ++q) up += red[q][r * kPitch + n], gate += red[q][r * kPitch + kHalf + n];
-            if constexpr (!GROUPED) up *= load_bf16(scale + col), gate *= load_bf16(scale + a.cols + col);
-            h = up * (gate / (1.0f + __expf(-gate)));
-          }
-          // place 2 i + u of an eight holds its element i + 4 u
-          const int at = (col & ~7) | (2 * (col & 3) + ((col >> 2) & 1));
-          const uint32_t hi = f32_to_bf16_rne(h);
-          uint16_t* dst = a.h + (long)list[row0 + 16 * t + r] * 2 * a.inner_pad + at;
-          dst[0] = (uint16_t)hi;
-          dst[a.inner_pad] = (uint16_t)f32_to_bf16_rne(h - bf16_bits_to_f32((uint16_t)hi));
-        }
-      } else {
-        for (int i = threadIdx.x; i < here * 2 * kHalf; i += 64 * kWaves) {
-          const int r = i / (2 * kHalf), n = i % (2 * kHalf), col = n0 + n;
-          if (col >= a.cols) continue;
-          float v2 = 0.0f;
-#pragma unroll
-          for (int q = 0; q < kWaves / 2; ++q) v2 += red[q][r * kPitch + n];
-          if constexpr (!GROUPED) v2 *= load_bf16(scale + col);
-          a.part[(long)list[row0 + 16 * t + r] * a.hidden + col] = v2;
-        }
-      }
-    }
+    if (RT == 1 || rows - row0 <= 16)
+      moe_rows<LAYOUT, FIRST, 1, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, row0, n0, k_first, k_last, red,
+                                                        lds_scale + 256 * wave);
+    else
+      moe_rows<LAYOUT, FIRST, RT, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, row0, n0, k_first, k_last, red,
+                                                        lds_scale + 256 * wave);
   }
 }
 
@@ -494,14 +651,20 @@ __global__ __launch_bounds__(256) void moe_join(const MoeArgs a) {
 
 template <int LAYOUT, bool FIRST, int TYPE, bool GROUPED>
 void launch_rt(const MoeArgs& a, dim3 grid, hipStream_t s) {
-  constexpr dim3 block(64 * kWaves);
-  if (a.tokens <= 16) hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 1, TYPE, GROUPED>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 2, TYPE, GROUPED>), grid, block, 0, s, a);
+  // Few workgroups: eight waves each, which halves a wave's share of K.  More
+  // than one on each of the 256 CUs: four, which halves the sums to join.
+  if (grid.x * grid.y <= 256 && a.tokens <= 16)
+    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 1, TYPE, GROUPED, 8>), grid, dim3(512), 0, s, a);
+  else if (a.tokens <= 16)
+    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 1, TYPE, GROUPED, 4>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 2, TYPE, GROUPED, 4>), grid, dim3(256), 0, s, a);
 }
 
 template <int LAYOUT, bool FIRST, int TYPE>
 hipError_t launch_product(const MoeArgs& a, unsigned columns, unsigned hit, hipStream_t s) {
-  const dim3 grid((columns + (FIRST ? kHalf : 2 * kHalf) - 1) / (FIRST ? kHalf : 2 * kHalf), hit);
+  constexpr unsigned kStep = FIRST ? kHalf : 2 * kHalf;
+  const dim3 grid(((columns + kStep - 1) / kStep + 7) / 8 * 8, hit);
   if (a.group) launch_rt<LAYOUT, FIRST, TYPE, true>(a, grid, s);
   else launch_rt<LAYOUT, FIRST, TYPE, false>(a, grid, s);
   return hipGetLastError();
