@@ -47,6 +47,8 @@ typedef u4 any_u4 __attribute__((aligned(1)));
 constexpr int kHalf = 64;          // columns of half a workgroup's tile
 constexpr int kPitch = 2 * kHalf + 4;  // floats of an LDS row of sums: rows start on different banks
 constexpr int kSuper = 128;        // K values a wave loads at a time, four products deep
+constexpr int kLargeGroups = 1;    // scale groups of at least a piece
+constexpr int kSmallGroups = 2;    // of 32 or 64
 constexpr int kMostPairs = 1024;   // (token, expert) pairs of a call
 constexpr int kMostExperts = 1024;
 
@@ -245,7 +247,7 @@ __device__ __forceinline__ int column(int half, int g, int r) {
 
 // A workgroup's tile for the pairs list[row0 ..] of an expert, at most 16 * RT
 // of them.
-template <int LAYOUT, bool FIRST, int RT, int TYPE, bool GROUPED, int kWaves>
+template <int LAYOUT, bool FIRST, int RT, int TYPE, int GROUPED, int kWaves>
 __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const uint16_t* scale, const uint16_t* list,
                                          int rows, int row0, int n0, int k_first, int k_last, float* red,
                                          uint32_t* lds_scale) {
@@ -278,7 +280,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   struct Block {  // 128 K values: the codes of both halves, the activations, and the scales of up to four groups
     uint32_t w[2][16];
     u4 x[RT][4][kL];
-    uint32_t sc[GROUPED ? 4 : 1];  // of two columns: the half lane / 32, columns 2 (lane % 32)
+    uint32_t sc[GROUPED == kSmallGroups ? 4 : 1];  // of two columns: the half lane / 32, columns 2 (lane % 32)
   };
   // Pieces from before `whole` lie inside the codes, the activations and the
   // scales.
@@ -293,10 +295,9 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   const int last = k_first + (max(whole - k_first, 1) - 1) / kSuper * kSuper;  // the last of them
   auto load_scales = [&](int k0, auto end, Block& b) {
     if constexpr (GROUPED) {
-      const int count = a.group >= kSuper ? 1 : kSuper / a.group;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < count) {
+      for (int i = 0; i < (GROUPED == kSmallGroups ? 4 : 1); ++i)
+        if (i < 2 || a.group == 32) {
           const uint16_t* p = scale + (long)min(k0 / a.group + i, a.groups - 1) * s.total;
           if constexpr (decltype(end)::value)
             b.sc[i] = p[min(sc_n, s.total - 1)] | ((uint32_t)p[min(sc_n + 1, s.total - 1)] << 16);
@@ -335,61 +336,72 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
     if constexpr (GROUPED) {
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) lds_scale[64 * i + lane] = b.sc[i];
+      for (int i = 0; i < (GROUPED == kSmallGroups ? 4 : 1); ++i) lds_scale[64 * i + lane] = b.sc[i];
       __builtin_amdgcn_wave_barrier();
     }
   };
-  auto multiply = [&](int k0, auto half, Block& b) {
+  // A half's sums of a group that ends, without the offset, times its scales.
+  auto scale_half = [&](auto half, int group) {
     constexpr int kAt = decltype(half)::value;
+    constexpr int kSum = GROUPED == kSmallGroups ? kAt : 0;
+    const uint16_t* sc = reinterpret_cast<const uint16_t*>(lds_scale) + 128 * group;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const u2 v = *reinterpret_cast<const u2*>(sc + column<kWide>(kAt, g, r));
+      const float f[4] = {bf16_bits_to_f32((uint16_t)v[0]), __uint_as_float(v[0] & 0xFFFF0000u),
+                          bf16_bits_to_f32((uint16_t)v[1]), __uint_as_float(v[1] & 0xFFFF0000u)};
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          all[t][4 * kAt + j][r] += f[j] * (acc[t][4 * kAt + j][r] - 24.0f * sum[t][kSum][r]);
+          acc[t][4 * kAt + j][r] = 0.0f;
+        }
+    }
+  };
+  auto multiply = [&](auto half, Block& b) {
+    __builtin_amdgcn_sched_barrier(0);  // what has been asked for ahead stays ahead
+    constexpr int kAt = decltype(half)::value;
+    constexpr int kSum = GROUPED == kSmallGroups ? kAt : 0;
     uint32_t(&w)[16] = b.w[kAt];
     arrange<LAYOUT>(w);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int k = k0 + 32 * q;
-      if (k < k_last) {
-        b8 xt[RT][kT];
+      b8 xt[RT][kT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          terms<FIRST, TYPE>(b.x[t][q], xt[t]);
+      for (int t = 0; t < RT; ++t) {
+        terms<FIRST, TYPE>(b.x[t][q], xt[t]);
 #pragma unroll
-          for (int i = 0; i < kT; ++i)
-            if (GROUPED || kAt == 0) sum[t][kAt] = mfma_bf16(ones, xt[t][i], sum[t][kAt]);
+        for (int i = 0; i < kT; ++i)
+          if (kSum == kAt) sum[t][kSum] = mfma_bf16(ones, xt[t][i], sum[t][kSum]);
+      }
+      uint32_t o[4];
+      step_codes<LAYOUT>(w, q, o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const b8 v = expand(o[j]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int i = 0; i < kT; ++i) acc[t][4 * kAt + j] = mfma_bf16(v, xt[t][i], acc[t][4 * kAt + j]);
+      }
+      if constexpr (GROUPED == kSmallGroups) {
+        if (q % 2 == 1 || a.group == 32) {
+          scale_half(half, 32 * q / a.group);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) sum[t][kAt] = f4{0, 0, 0, 0};
         }
-        uint32_t o[4];
-        step_codes<LAYOUT>(w, q, o);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto finish = [&](int k0) {  // a group of 128 or more ends with this piece
+    if constexpr (GROUPED == kLargeGroups) {
+      if (k0 + kSuper >= k_last || (k0 + kSuper) % a.group == 0) {
+        scale_half(std::integral_constant<int, 0>{}, 0);
+        scale_half(std::integral_constant<int, 1>{}, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const b8 v = expand(o[j]);
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int i = 0; i < kT; ++i) acc[t][4 * kAt + j] = mfma_bf16(v, xt[t][i], acc[t][4 * kAt + j]);
-        }
-        if constexpr (GROUPED) {
-          if (k + 32 >= k_last || (k + 32) % a.group == 0) {
-            // the group ends: its sums, without the offset, times its scales
-            const uint16_t* sc = reinterpret_cast<const uint16_t*>(lds_scale) + 128 * (k / a.group - k0 / a.group);
-            float f[16];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const u2 v = *reinterpret_cast<const u2*>(sc + column<kWide>(kAt, g, r));
-              f[4 * r] = bf16_bits_to_f32((uint16_t)v[0]), f[4 * r + 1] = __uint_as_float(v[0] & 0xFFFF0000u);
-              f[4 * r + 2] = bf16_bits_to_f32((uint16_t)v[1]), f[4 * r + 3] = __uint_as_float(v[1] & 0xFFFF0000u);
-            }
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  all[t][4 * kAt + j][r] +=
-                      f[4 * r + j] * (acc[t][4 * kAt + j][r] - 24.0f * sum[t][kAt][r]);
-                acc[t][4 * kAt + j] = f4{0, 0, 0, 0};
-              }
-              sum[t][kAt] = f4{0, 0, 0, 0};
-            }
-          }
-        }
+        for (int t = 0; t < RT; ++t) sum[t][0] = f4{0, 0, 0, 0};
       }
     }
   };
@@ -409,8 +421,9 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
       };
       auto use = [&](Block& b) {
         share_scales(b);
-        multiply(k0, h0, b);
-        multiply(k0, h1, b);
+        multiply(h0, b);
+        multiply(h1, b);
+        finish(k0);
         return (k0 += kSuper) < whole;
       };
       Block b0, b1;
@@ -436,11 +449,12 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
         load_scales(k0, std::false_type{}, b);
         if constexpr (kAhead) {
           share_scales(b);
-          multiply(k0, h0, b);
+          multiply(h0, b);
           u4 x[RT][4][kL];
           load_rows(next, x);
           load_half<LAYOUT>(s, next, n0, b.w[0]);
-          multiply(k0, h1, b);
+          multiply(h1, b);
+          finish(k0);
           load_half<LAYOUT>(s, next, n1, b.w[1]);
 #pragma unroll
           for (int t = 0; t < RT; ++t)
@@ -452,9 +466,10 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
           load_rows(k0, b.x);
           load_half<LAYOUT>(s, k0, n1, b.w[1]);
           share_scales(b);
-          multiply(k0, h0, b);
+          multiply(h0, b);
           load_half<LAYOUT>(s, next, n0, b.w[0]);
-          multiply(k0, h1, b);
+          multiply(h1, b);
+          finish(k0);
         }
       }
     }
@@ -463,8 +478,9 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
     Block b;
     load_end(k0, b);
     share_scales(b);
-    multiply(k0, h0, b);
-    multiply(k0, h1, b);
+    multiply(h0, b);
+    multiply(h1, b);
+    finish(k0);
   }
   // The waves' sums: lane (g, c) holds token c, columns column(half, g, r)
   // + j.  The second half of the waves hand theirs to the first half.
@@ -533,7 +549,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
 // the halves of the tile being the same 64 columns of each; otherwise down,
 // 128 columns, to a.part.  RT: the most row
 // tiles of 16 tokens a pass over the codes serves.
-template <int LAYOUT, bool FIRST, int RT, int TYPE, bool GROUPED, int kWaves>
+template <int LAYOUT, bool FIRST, int RT, int TYPE, int GROUPED, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   constexpr int kStep = FIRST ? kHalf : 2 * kHalf;  // columns from one workgroup to the next
   // the waves' sums, and before them 1024 dwords a wave for what ends in a piece
@@ -619,8 +635,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   const int n0 = tile * kStep;
   const uint16_t* scale = a.scale + (long)expert * (GROUPED ? a.groups : 1) * s.total;
 
-  // this wave's K: whole scale groups, in steps of 32
-  const int unit = GROUPED ? a.group : 32;
+  // this wave's K: whole pieces and whole scale groups
+  const int unit = GROUPED ? max(a.group, kSuper) : kSuper;
   const int units = (a.k + unit - 1) / unit, each = (units + kWaves - 1) / kWaves;
   const int k_first = min(a.k, wave * each * unit), k_last = min(a.k, (wave + 1) * each * unit);
 
@@ -649,7 +665,7 @@ __global__ __launch_bounds__(256) void moe_join(const MoeArgs a) {
   else static_cast<_Float16*>(a.out)[at] = (_Float16)y;
 }
 
-template <int LAYOUT, bool FIRST, int TYPE, bool GROUPED>
+template <int LAYOUT, bool FIRST, int TYPE, int GROUPED>
 void launch_rt(const MoeArgs& a, dim3 grid, hipStream_t s) {
   // Few workgroups: eight waves each, which halves a wave's share of K.  More
   // than one on each of the 256 CUs: four, which halves the sums to join.
@@ -665,8 +681,9 @@ template <int LAYOUT, bool FIRST, int TYPE>
 hipError_t launch_product(const MoeArgs& a, unsigned columns, unsigned hit, hipStream_t s) {
   constexpr unsigned kStep = FIRST ? kHalf : 2 * kHalf;
   const dim3 grid(((columns + kStep - 1) / kStep + 7) / 8 * 8, hit);
-  if (a.group) launch_rt<LAYOUT, FIRST, TYPE, true>(a, grid, s);
-  else launch_rt<LAYOUT, FIRST, TYPE, false>(a, grid, s);
+  if (a.group >= kSuper) launch_rt<LAYOUT, FIRST, TYPE, kLargeGroups>(a, grid, s);
+  else if (a.group) launch_rt<LAYOUT, FIRST, TYPE, kSmallGroups>(a, grid, s);
+  else launch_rt<LAYOUT, FIRST, TYPE, 0>(a, grid, s);
   return hipGetLastError();
 }
 
