@@ -1,10 +1,19 @@
 // Attention of each sequence's newest tokens over the quantized cache
-// (shk_kvattn.h has the mathematics of a tile).
+// (shk_kvattn.h has the mathematics of a step).
 //
-// A workgroup is one piece of one sequence (or of the shared prefix) for one
-// key head and up to 16 * RT of its query rows; its four waves take every
-// fourth 64 tokens and are joined through LDS.  Pieces of a sequence are
-// joined by kv_join_kernel from their f32 outputs, maxima and sums.
+// kv_stream_kernel serves a sequence's own tokens (and a shared prefix with
+// few query rows).  A workgroup is one key head and up to 16 * RT query rows;
+// its four waves take every fourth 64 tokens, each from memory to its own
+// registers, and are joined through LDS.  The tokens of all sequences are
+// dealt out evenly: in pieces of 256, a workgroup gets the same number of
+// consecutive ones, whichever sequences they belong to.
+//
+// kv_prefix_kernel serves a shared prefix with many query rows (those of all
+// sequences): the four waves have different rows, take the same 64 tokens,
+// and each widens a quarter of them into LDS for all.
+//
+// kv_join_kernel joins the pieces of a row from their f32 outputs, references
+// and sums.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -15,6 +24,8 @@
 namespace shk {
 namespace {
 
+constexpr int kPiece = 4 * kKvTile;  // tokens that a workgroup's waves take at a time
+
 struct AttnArgs {
   const uint16_t* q;
   long q_batch, q_query, q_head;  // strides in elements
@@ -24,15 +35,27 @@ struct AttnArgs {
   long table_stride;
   uint16_t* out;
   float* lse;
-  float* part_o;   // [pieces][rows][D]
-  float2* part_ml; // [pieces][rows]: maximum (in powers of two) and sum
+  // Outputs of pieces and their (reference, sum): own [kv_heads][slots][own
+  // rows], then prefix [splits][kv_heads][batch * own rows].
+  float* part_o;
+  float2* part_ml;
   float scale;
   int type;
   int batch, queries, heads, kv_heads, ratio;
   int pages, page_shift, table_tokens, prefix;
-  int own_splits, prefix_splits;  // pieces of a sequence and of the prefix
-  int own_tiles, prefix_tiles;    // 16 * RT row tiles of a key head
+  int own_groups, own_tiles;        // workgroups of a key head and row tile; row tiles of 16 * RT rows
+  int prefix_splits, prefix_tiles;  // pieces of the prefix; row tiles of its kernel
+  int slots;                        // own_groups + batch
+  int direct;                       // one piece a sequence at most and no prefix: out is written at once
 };
+
+__device__ __forceinline__ int own_rows(const AttnArgs& a) { return a.queries * a.ratio; }
+__device__ __forceinline__ long own_parts(const AttnArgs& a) { return (long)a.kv_heads * a.slots * own_rows(a); }
+__device__ __forceinline__ int tokens_of(const AttnArgs& a, int b) { return min(max(a.lengths[b], 0), a.table_tokens); }
+// Pieces of a sequence; with `direct`, each is one piece, the empty ones too.
+__device__ __forceinline__ int pieces_of(const AttnArgs& a, int tokens) {
+  return a.direct ? 1 : (tokens + kPiece - 1) / kPiece;
+}
 
 template <int D>
 __device__ __forceinline__ void store_row(const AttnArgs& a, long row, int d, f4 v) {
@@ -47,208 +70,433 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
   return m == -__builtin_inff() && !(l != l) ? -__builtin_inff() : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
+// Pieces of the sequences before b.
+__device__ __forceinline__ int pieces_before(const AttnArgs& a, int b) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int b0 = 0; b0 < b; b0 += 64) n += b0 + lane < b ? pieces_of(a, tokens_of(a, b0 + lane)) : 0;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d, 64);
+  return n;
+}
+
+// Query row r of a key head's rows, for one sequence or (b0 < 0) all of them.
+__device__ __forceinline__ void query_row(const AttnArgs& a, int head, int b0, int r, const void*& src, int& query,
+                                          long& out) {
+  const int per = own_rows(a);
+  const int b = b0 < 0 ? r / per : b0, in = b0 < 0 ? r % per : r;
+  query = in / a.ratio;
+  const int h = head * a.ratio + in % a.ratio;
+  src = a.q + b * a.q_batch + query * a.q_query + h * a.q_head;
+  out = ((long)b * a.queries + query) * a.heads + h;
+}
+
+// One piece of a row, from 16 threads (part) of D / 16 values each: to the
+// output where it is the only one, or to the parts.
+template <int D>
+__device__ __forceinline__ void store_piece(const AttnArgs& a, bool direct, long out_row, long part_row, int d, f4 v) {
+  if (direct) store_row<D>(a, out_row, d, v);
+  else *reinterpret_cast<f4*>(a.part_o + part_row * D + d) = v;
+}
+
 template <int BITS, int D, int RT, int TYPE>
-__global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_attention_kernel(const AttnArgs a) {
-  using Tile = KvTile<BITS, D, RT, TYPE>;
+__global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_kernel(const AttnArgs a) {
+  using Rows = KvRows<BITS, D, RT, TYPE>;
   constexpr int kPitch = D + 4;  // floats of an LDS row: the 16 rows start on different banks
-  __shared__ float red_o[4][16 * kPitch];
+  __shared__ __align__(16) float red_o[4][16 * kPitch];
   __shared__ float red_m[4][16], red_l[4][16];
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 
-  // which piece: those of the sequences first, then those of the prefix
+  // which pieces: those of the sequences first, then those of the prefix
   int unit = blockIdx.x;
-  const int own_units = a.batch * a.kv_heads * a.own_tiles * a.own_splits;
+  const int own_units = a.kv_heads * a.own_tiles * a.own_groups;
   const bool shared = unit >= own_units;
   if (shared) unit -= own_units;
-  const int splits = shared ? a.prefix_splits : a.own_splits, tiles = shared ? a.prefix_tiles : a.own_tiles;
-  const int split = unit % splits;
-  unit /= splits;
-  const int tile = unit % tiles;
-  unit /= tiles;
+  const int groups = shared ? a.prefix_splits : a.own_groups, tiles = shared ? a.prefix_tiles : a.own_tiles;
   const int head = unit % a.kv_heads;
-  const int b0 = unit / a.kv_heads;  // 0 for the prefix
-  const int n = shared ? a.prefix : min(max(a.lengths[b0], 0), a.table_tokens);
-  const int piece = shared ? a.own_splits + split : split;
-  const int rows_here = a.queries * a.ratio * (shared ? a.batch : 1);
-
-  KvRow row[RT];
-  long out_row[RT];
-  int limit[RT], least = n;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int r = (tile * RT + t) * 16 + c;
-    row[t].q = nullptr;
-    out_row[t] = -1;
-    limit[t] = n;
-    if (r < rows_here) {
-      const int per = a.queries * a.ratio;
-      const int b = shared ? r / per : b0, in = shared ? r % per : r;
-      const int query = in / a.ratio, h = head * a.ratio + in % a.ratio;
-      row[t].q = a.q + b * a.q_batch + query * a.q_query + h * a.q_head;
-      out_row[t] = ((long)b * a.queries + query) * a.heads + h;
-      if (!shared) limit[t] = max(n - a.queries + query + 1, 0);
-    }
-    least = min(least, limit[t]);
-  }
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) least = min(least, __shfl_xor(least, d, 64));
-  least = __builtin_amdgcn_readfirstlane(least);
-
+  unit /= a.kv_heads;
+  const int tile = unit % tiles, j = unit / tiles;
+  const int total = shared ? pieces_of(a, a.prefix) : __builtin_amdgcn_readfirstlane(pieces_before(a, a.batch));
+  const int each = max((total + groups - 1) / groups, 1);
+  const int first = j * each, end = min(first + each, total);
+  const int rows_here = own_rows(a) * (shared ? a.batch : 1);
   const KvView kv{a.kc, a.vc, a.ks, a.vs, a.pages, a.page_shift, a.kv_heads, head};
-  const int32_t* table = shared ? a.prefix_pages : a.table + b0 * a.table_stride;
-  const int steps = (n + kKvTile - 1) / kKvTile;
-  const int each = (steps + splits - 1) / splits;
-  const int first = split * each, end = min(first + each, steps);
 
-  Tile tl;
-  tl.begin(row, a.scale);
-  for (int i = first + wave; i < end; i += 4) tl.step(kv, table, i * kKvTile, n, limit, least);
-
-  // the waves' outputs, relative to the largest of their maxima
+  int b = 0, before = 0;  // the sequence that holds piece `first`, and the pieces before it
+  if (!shared && first < end) {
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      int n = b0 + lane < a.batch ? pieces_of(a, tokens_of(a, b0 + lane)) : 0;
+      const int own = n;
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const float l = groups_sum(tl.l[t]);
-    if (t > 0) __syncthreads();
-    if (g == 0) red_m[wave][c] = tl.m[t], red_l[wave][c] = tl.bad ? __builtin_nanf("") : l;
-    __syncthreads();
-    float top = red_m[0][c];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, red_m[w][c]);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    const float back = __uint_as_float((uint32_t)tl.ref << 23) * 0x1p-13f * __builtin_amdgcn_exp2f(tl.m[t] - base);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int j = 0; j < Tile::kOut; j += 4)
-        *reinterpret_cast<f4*>(&red_o[wave][c * kPitch + (4 * g + r) * Tile::kOut + j]) =
-            f4{tl.o[t][j][r], tl.o[t][j + 1][r], tl.o[t][j + 2][r], tl.o[t][j + 3][r]} * back;
-    __syncthreads();
-    // 16 threads a row, D / 16 values each
-    const int rr = threadIdx.x / 16, part = threadIdx.x % 16;
-    float rtop = red_m[0][rr];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) rtop = __builtin_fmaxf(rtop, red_m[w][rr]);
-    const float rbase = rtop == -__builtin_inff() ? 0.0f : rtop;
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) sum += red_l[w][rr] * __builtin_amdgcn_exp2f(red_m[w][rr] - rbase);
-    // the row's place in the output, from the lane that holds the row
-    const long at = __shfl(out_row[t], rr, 64);
-    if (at >= 0) {
-      const bool whole = a.own_splits + a.prefix_splits == 1;
-      const float f = !whole ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
-#pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        const int d = (k * 16 + part) * 4;
-        f4 v = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(&red_o[w][rr * kPitch + d]);
-        v *= f;
-        if (whole) store_row<D>(a, at, d, v);
-        else *reinterpret_cast<f4*>(a.part_o + ((long)piece * a.batch * a.queries * a.heads + at) * D + d) = v;
+      for (int d = 1; d < 64; d *= 2) {
+        const int up = __shfl_up(n, d, 64);
+        if (lane >= d) n += up;
       }
-      if (part == 0) {
-        if (!whole) a.part_ml[(long)piece * a.batch * a.queries * a.heads + at] = make_float2(rtop, sum);
-        else if (a.lse != nullptr) a.lse[at] = natural_lse(rtop, sum);
+      const unsigned long past = __ballot(before + n > first);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        b = b0 + at;
+        before += __shfl(n - own, at, 64);
+        break;
+      }
+      before += __shfl(n, 63, 64);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    before = __builtin_amdgcn_readfirstlane(before);
+  }
+  // a sequence without tokens has no piece; a prefix split may have none either
+  for (int piece = first; piece < end || (shared && piece == first); ++b) {
+    const int n = shared ? a.prefix : tokens_of(a, b);
+    const int mine = min(end, before + pieces_of(a, n));  // this sequence's pieces end there
+    if (!shared && mine <= piece) {
+      before += pieces_of(a, n);
+      continue;
+    }
+    const void* src[RT];
+    long out_row[RT];
+    int limit[RT], least = n;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = (tile * RT + t) * 16 + c;
+      src[t] = nullptr;
+      out_row[t] = -1;
+      limit[t] = n;
+      if (r < rows_here) {
+        int query;
+        query_row(a, head, shared ? -1 : b, r, src[t], query, out_row[t]);
+        if (!shared) limit[t] = max(n - a.queries + query + 1, 0);
+      }
+      least = min(least, limit[t]);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) least = min(least, __shfl_xor(least, d, 64));
+    least = __builtin_amdgcn_readfirstlane(least);
+
+    const int32_t* table = shared ? a.prefix_pages : a.table + b * a.table_stride;
+    const int last = (n - 1) >> 4;  // the last block that holds a token; later ones repeat it, masked
+    bool bad = false;
+    Rows rows;
+    rows.begin(src, a.scale);
+    for (int i = 4 * (piece - before) + wave; i < 4 * (mine - before) && i * kKvTile < n; i += 4) {
+      const int t0 = i * kKvTile;
+      KvBlock<BITS, D> blk[4];
+      u2 kss[4], vss[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const long row0 = kv.row_of(table, min(4 * i + x, last), bad);
+        blk[x].load(kv, row0);
+        kss[x] = load_scales(kv.ks, row0);
+        vss[x] = load_scales(kv.vs, row0);
+      }
+      f4 s[RT][4], ks[4], vs[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[t][x] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int st = 0; st < Rows::kSteps; ++st) {
+          const h8 k = blk[x].k_operand(st);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) s[t][x] = mfma_f16(k, rows.q[t][st], s[t][x]);
+        }
+        ks[x] = widen_scales(kss[x]);
+        vs[x] = widen_scales(vss[x]);
+      }
+      int left[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) left[t] = limit[t] - t0;
+      h8 p[RT][2], pl[RT][2];
+      rows.soften(s, ks, vs, t0 + kKvTile > least, left, n - t0, p, pl);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int w = 0; w < Rows::kOut / 4; ++w) {
+          h2 f[4][4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) blk[2 * h + x / 2].v_pairs(w, x % 2, f[x]);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) rows.add(4 * w + jj, join(f[0][jj], f[1][jj], f[2][jj], f[3][jj]), p, pl, h);
+        }
+    }
+
+    // the waves' outputs, relative to the largest of their references
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float l = groups_sum(rows.l[t]);
+      __syncthreads();
+      if (g == 0) red_m[wave][c] = rows.m[t], red_l[wave][c] = bad ? __builtin_nanf("") : l;
+      __syncthreads();
+      float top = red_m[0][c];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, red_m[w][c]);
+      const float back = __builtin_amdgcn_exp2f(rows.m[t] - (top == -__builtin_inff() ? 0.0f : top));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int jj = 0; jj < Rows::kOut; jj += 4)
+          *reinterpret_cast<f4*>(&red_o[wave][c * kPitch + (4 * g + r) * Rows::kOut + jj]) =
+              f4{rows.o[t][jj][r], rows.o[t][jj + 1][r], rows.o[t][jj + 2][r], rows.o[t][jj + 3][r]} * back;
+      __syncthreads();
+      // 16 threads a row, D / 16 values each
+      const int rr = threadIdx.x / 16, part = threadIdx.x % 16;
+      float rtop = red_m[0][rr];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) rtop = __builtin_fmaxf(rtop, red_m[w][rr]);
+      const float rbase = rtop == -__builtin_inff() ? 0.0f : rtop;
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += red_l[w][rr] * __builtin_amdgcn_exp2f(red_m[w][rr] - rbase);
+      const long at = __shfl(out_row[t], rr, 64);  // from the lane that holds the row
+      if (at >= 0) {
+        const int row = (tile * RT + t) * 16 + rr;
+        const long to = shared ? own_parts(a) + ((long)j * a.kv_heads + head) * rows_here + row
+                               : ((long)head * a.slots + j + b) * rows_here + row;
+        const float f = !a.direct ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+          const int d = (k * 16 + part) * 4;
+          f4 v = f4{0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(&red_o[w][rr * kPitch + d]);
+          store_piece<D>(a, a.direct, at, to, d, v * f);
+        }
+        if (part == 0) {
+          if (!a.direct) a.part_ml[to] = make_float2(rtop, sum);
+          else if (a.lse != nullptr) a.lse[at] = natural_lse(rtop, sum);
+        }
       }
     }
+    piece = max(mine, piece + (shared ? 1 : 0));
+    before += pieces_of(a, n);
+    if (shared) break;
   }
 }
 
-// Joins the pieces of a row: 32 lanes a row, D / 32 values each.
+template <int BITS, int D, int RT, int TYPE>
+__global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
+  using Rows = KvRows<BITS, D, RT, TYPE>;
+  using Block = KvBlock<BITS, D>;
+  constexpr int kBuffers = D == 256 ? 1 : 2;  // 64 KB a workgroup: two on a CU
+  constexpr int kSteps = Rows::kSteps, kOut = Rows::kOut;
+  // the products' operands as the lanes read them: K by block and step, V by
+  // 32 tokens and 16 values of head_dim
+  __shared__ h8 lds_k[kBuffers][4][kSteps][64];
+  __shared__ h8 lds_v[kBuffers][2][kOut][64];
+  const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int unit = blockIdx.x;
+  const int head = unit % a.kv_heads;
+  unit /= a.kv_heads;
+  const int split = unit % a.prefix_splits, tile = unit / a.prefix_splits;
+  const int n = a.prefix, rows_here = own_rows(a) * a.batch;
+  const int steps = (n + kKvTile - 1) / kKvTile, each = (steps + a.prefix_splits - 1) / a.prefix_splits;
+  const int first = split * each, end = min(first + each, steps);
+  const KvView kv{a.kc, a.vc, a.ks, a.vs, a.pages, a.page_shift, a.kv_heads, head};
+  const int last = (n - 1) >> 4;
+
+  const void* src[RT];
+  int row[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    row[t] = ((tile * 4 + wave) * RT + t) * 16 + c;
+    src[t] = nullptr;
+    int query;
+    long out;
+    if (row[t] < rows_here) query_row(a, head, -1, row[t], src[t], query, out);
+  }
+  Rows rows;
+  rows.begin(src, a.scale);
+  bool bad = false;
+
+  Block mine;  // this wave's 16 of the 64 tokens
+  u2 kss[4], vss[4];
+  auto load = [&](int step) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const long row0 = kv.row_of(a.prefix_pages, min(4 * step + x, last), bad);
+      kss[x] = load_scales(kv.ks, row0);
+      vss[x] = load_scales(kv.vs, row0);
+    }
+    mine.load(kv, kv.row_of(a.prefix_pages, min(4 * step + wave, last), bad));
+  };
+  if (first < end) load(first);
+  for (int step = first, at = 0; step < end; ++step, at = (at + 1) % kBuffers) {
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) lds_k[at][wave][st][lane] = mine.k_operand(st);
+#pragma unroll
+    for (int w = 0; w < kOut / 4; ++w) {
+      h2 f[2][4];
+      mine.v_pairs(w, 0, f[0]);
+      mine.v_pairs(w, 1, f[1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint2 pair = make_uint2(__builtin_bit_cast(uint32_t, f[0][j]), __builtin_bit_cast(uint32_t, f[1][j]));
+        reinterpret_cast<uint2*>(&lds_v[at][wave / 2][4 * w + j][lane])[wave % 2] = pair;
+      }
+    }
+    f4 ks[4], vs[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) ks[x] = widen_scales(kss[x]), vs[x] = widen_scales(vss[x]);
+    load(min(step + 1, end - 1));  // on its way while this one is multiplied
+    __syncthreads();
+    f4 s[RT][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t][x] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const h8 k = lds_k[at][x][st][lane];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[t][x] = mfma_f16(k, rows.q[t][st], s[t][x]);
+      }
+    }
+    int left[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) left[t] = n - step * kKvTile;
+    h8 p[RT][2], pl[RT][2];
+    rows.soften(s, ks, vs, left[0] < kKvTile, left, left[0], p, pl);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < kOut; ++j) rows.add(j, lds_v[at][h][j][lane], p, pl, h);
+    if constexpr (kBuffers == 1) __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const float l = groups_sum(rows.l[t]);
+    if (row[t] >= rows_here) continue;
+    const long to = own_parts(a) + ((long)split * a.kv_heads + head) * rows_here + row[t];
+    if (g == 0) a.part_ml[to] = make_float2(rows.m[t], bad ? __builtin_nanf("") : l);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < kOut; j += 4)
+        *reinterpret_cast<f4*>(a.part_o + to * D + (4 * g + r) * kOut + j) =
+            f4{rows.o[t][j][r], rows.o[t][j + 1][r], rows.o[t][j + 2][r], rows.o[t][j + 3][r]};
+  }
+}
+
+// Joins the pieces of a row, a wave each: lane p looks at piece p, then all
+// lanes add up the outputs, D / 64 values each.
 template <int D>
 __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
-  const long rows = (long)a.batch * a.queries * a.heads;
-  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / 32;
-  if (row >= rows) return;
-  const int part = threadIdx.x % 32, pieces = a.own_splits + a.prefix_splits;
+  typedef float fv __attribute__((ext_vector_type(D / 64)));
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (row >= (long)a.batch * a.queries * a.heads) return;
+  const int h = (int)(row % a.heads), query = (int)(row / a.heads % a.queries), b = (int)(row / a.heads / a.queries);
+  const int head = h / a.ratio, in = query * a.ratio + h % a.ratio, per = own_rows(a);
+  const int total = pieces_before(a, a.batch), before = pieces_before(a, b), mine = pieces_of(a, tokens_of(a, b));
+  const int each = max((total + a.own_groups - 1) / a.own_groups, 1);
+  const int first = before / each, own = mine == 0 ? 0 : (before + mine - 1) / each - first + 1;
+  const int count = own + a.prefix_splits;
+  const long own_at = ((long)head * a.slots + first + b) * per + in;
+  const long prefix_at = own_parts(a) + (long)head * per * a.batch + (long)b * per + in;
+  const long prefix_step = (long)a.kv_heads * per * a.batch;
+  auto place = [&](int p) { return p < own ? own_at + (long)p * per : prefix_at + (p - own) * prefix_step; };
   float top = -__builtin_inff();
-  for (int s = 0; s < pieces; ++s) top = __builtin_fmaxf(top, a.part_ml[s * rows + row].x);
+  for (int p = lane; p < count; p += 64) top = __builtin_fmaxf(top, a.part_ml[place(p)].x);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d, 64));
   const float base = top == -__builtin_inff() ? 0.0f : top;
   float sum = 0.0f;
-  constexpr int N = D / 32 < 4 ? 1 : D / 128;  // 16-byte pieces of a lane; D = 64: half the lanes
-  f4 v[N] = {};
-  const bool on = part * 4 < D;
-  for (int s = 0; s < pieces; ++s) {
-    const float2 ml = a.part_ml[s * rows + row];
-    if (ml.x == -__builtin_inff() && ml.y == 0.0f) continue;  // nothing seen
-    const float w = __builtin_amdgcn_exp2f(ml.x - base);
-    sum += ml.y * w;
-    if (on) {
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        v[k] += *reinterpret_cast<const f4*>(a.part_o + (s * rows + row) * D + (k * 32 + part) * 4) * w;
+  fv v = {};
+  for (int p0 = 0; p0 < count; p0 += 64) {
+    const int here = min(count - p0, 64);
+    float weight = 0.0f;
+    if (lane < here) {
+      const float2 ml = a.part_ml[place(p0 + lane)];
+      weight = ml.x == -__builtin_inff() && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - base);
+      sum += weight == 0.0f ? 0.0f : ml.y * weight;
     }
+#pragma unroll 8
+    for (int p = 0; p < here; ++p)
+      v += reinterpret_cast<const fv*>(a.part_o + place(p0 + p) * D)[lane] * __shfl(weight, p, 64);
   }
-  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (on) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) store_row<D>(a, row, (k * 32 + part) * 4, v[k] * f);
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+  v *= sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const uint16_t o = a.type == SHK_SRC_BF16 ? (uint16_t)f32_to_bf16_rne(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+    a.out[row * D + lane * (D / 64) + i] = o;
   }
-  if (part == 0 && a.lse != nullptr) a.lse[row] = natural_lse(top, sum);
+  if (lane == 0 && a.lse != nullptr) a.lse[row] = natural_lse(top, sum);
 }
 
 long cdiv(long a, long b) { return (a + b - 1) / b; }
 
-// Pieces of the sequences and of the prefix, and the row tiles' height.
 struct Plan {
-  int rt, own_tiles, prefix_tiles, own_splits, prefix_splits;
+  int rt, prefix_rt;                  // row tiles of a wave in the two kernels
+  bool prefix_kernel;                 // the prefix has a kernel of its own
+  int own_groups, own_tiles, prefix_splits, prefix_tiles;
+  bool direct;
 };
 
 Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
-  const long rows = a.queries * (a.heads / c.kv_heads);
-  Plan p;
-  // two row tiles of 256 columns would not fit the registers
-  p.rt = c.head_dim == 256 ? 1 : rows > 16 || (a.prefix_length > 0 && rows * a.batch > 16) ? 2 : 1;
+  const long rows = a.queries * (a.heads / c.kv_heads), all = rows * a.batch, tokens = a.table_pages * c.page_size;
+  const bool wide = c.head_dim == 256;  // two row tiles of 256 columns would not fit the registers
+  Plan p{};
+  const bool prefix = a.prefix_length > 0;
+  p.prefix_kernel = prefix && all > (wide ? 16 : 32);
+  p.rt = wide || (rows <= 16 && (!prefix || p.prefix_kernel || all <= 16)) ? 1 : 2;
+  p.prefix_rt = wide ? 1 : 2;
   p.own_tiles = (int)cdiv(rows, 16 * p.rt);
-  p.prefix_tiles = a.prefix_length > 0 ? (int)cdiv(rows * a.batch, 16 * p.rt) : 0;
-  const long want = 768;  // workgroups of a launch: three on each of 256 CUs
-  const long own = a.batch * c.kv_heads * p.own_tiles;
-  const long tokens = a.table_pages * c.page_size;
-  p.own_splits = (int)std::max(1L, std::min({cdiv(want, own), cdiv(tokens, 4 * kKvTile), 64L}));
-  p.prefix_splits = 0;
-  if (a.prefix_length > 0)
-    p.prefix_splits = (int)std::max(1L, std::min({cdiv(want, (long)c.kv_heads * p.prefix_tiles),
-                                                  cdiv(a.prefix_length, 4 * kKvTile), 64L}));
+  p.direct = !prefix && tokens <= kPiece;
+  // three workgroups on each of the 256 CUs, two where they hold more
+  const long want = p.rt == 2 || wide ? 512 : 768;
+  p.own_groups = p.direct ? (int)a.batch
+                          : (int)std::max(1L, std::min(want / (c.kv_heads * p.own_tiles), a.batch * cdiv(tokens, kPiece)));
+  if (prefix) {
+    p.prefix_tiles = (int)cdiv(all, p.prefix_kernel ? 64 * p.prefix_rt : 16 * p.rt);
+    p.prefix_splits = (int)std::max(1L, std::min(cdiv(p.prefix_kernel ? 512 : want, c.kv_heads * p.prefix_tiles),
+                                                 cdiv(a.prefix_length, kPiece)));
+  }
   return p;
 }
 
-long part_rows(const shk_kv_attention& a, const Plan& p) {
-  return p.own_splits + p.prefix_splits > 1 ? (p.own_splits + p.prefix_splits) * a.batch * a.queries * a.heads : 0;
-}
-
-template <int BITS, int D, int RT, int TYPE>
-hipError_t launch(const AttnArgs& a, hipStream_t s) {
-  const long per_head = (long)a.batch * a.own_tiles * a.own_splits + (long)a.prefix_tiles * a.prefix_splits;
-  const long units = a.kv_heads * per_head;
-  if (units > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
-  hipLaunchKernelGGL((kv_attention_kernel<BITS, D, RT, TYPE>), dim3((unsigned)units), dim3(256), 0, s, a);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess || a.own_splits + a.prefix_splits == 1) return err;
-  const long rows = (long)a.batch * a.queries * a.heads;
-  hipLaunchKernelGGL((kv_join_kernel<D>), dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, s, a);
-  return hipGetLastError();
+long part_rows(const shk_kv_cache& c, const shk_kv_attention& a, const Plan& p) {
+  const long rows = a.queries * (a.heads / c.kv_heads);
+  return p.direct ? 0 : c.kv_heads * rows * (p.own_groups + a.batch + (long)p.prefix_splits * a.batch);
 }
 
 template <int BITS, int D, int TYPE>
-hipError_t launch_rt(int rt, const AttnArgs& a, hipStream_t s) {
-  if constexpr (D < 256)
-    if (rt == 2) return launch<BITS, D, 2, TYPE>(a, s);
-  return launch<BITS, D, 1, TYPE>(a, s);
+hipError_t launch_kernels(const AttnArgs& a, const Plan& p, hipStream_t s) {
+  const bool shared = a.prefix_splits > 0 && !p.prefix_kernel;
+  const long own = (long)a.kv_heads * a.own_tiles * a.own_groups;
+  const long prefix = (long)a.kv_heads * a.prefix_tiles * a.prefix_splits;
+  const dim3 grid((unsigned)(own + (shared ? prefix : 0))), block(256);
+  if (own + prefix > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
+  if constexpr (D < 256) {
+    if (p.rt == 2) hipLaunchKernelGGL((kv_stream_kernel<BITS, D, 2, TYPE>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((kv_stream_kernel<BITS, D, 1, TYPE>), grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((kv_stream_kernel<BITS, D, 1, TYPE>), grid, block, 0, s, a);
+  }
+  hipError_t err = hipGetLastError();
+  if (err == hipSuccess && p.prefix_kernel) {
+    hipLaunchKernelGGL((kv_prefix_kernel<BITS, D, D == 256 ? 1 : 2, TYPE>), dim3((unsigned)prefix), block, 0, s, a);
+    err = hipGetLastError();
+  }
+  if (err != hipSuccess || a.direct) return err;
+  const long rows = (long)a.batch * a.queries * a.heads;
+  hipLaunchKernelGGL((kv_join_kernel<D>), dim3((unsigned)cdiv(rows, 4)), block, 0, s, a);
+  return hipGetLastError();
 }
 
 template <int BITS, int TYPE>
-hipError_t launch_d(long d, int rt, const AttnArgs& a, hipStream_t s) {
-  if (d == 64) return launch_rt<BITS, 64, TYPE>(rt, a, s);
-  if (d == 128) return launch_rt<BITS, 128, TYPE>(rt, a, s);
-  return launch_rt<BITS, 256, TYPE>(rt, a, s);
+hipError_t launch_d(long d, const AttnArgs& a, const Plan& p, hipStream_t s) {
+  if (d == 64) return launch_kernels<BITS, 64, TYPE>(a, p, s);
+  if (d == 128) return launch_kernels<BITS, 128, TYPE>(a, p, s);
+  return launch_kernels<BITS, 256, TYPE>(a, p, s);
 }
 
 }  // namespace
 
 int64_t kv_attention_workspace(const shk_kv_cache& c, const shk_kv_attention& a) {
-  return part_rows(a, plan_of(c, a)) * (c.head_dim * 4 + 8);
+  return part_rows(c, a, plan_of(c, a)) * (c.head_dim * 4 + 8);
 }
 
 hipError_t launch_kv_attention(const shk_kv_cache& c, const shk_kv_attention& x, hipStream_t s) {
@@ -263,7 +511,7 @@ hipError_t launch_kv_attention(const shk_kv_cache& c, const shk_kv_attention& x,
   a.out = static_cast<uint16_t*>(x.out);
   a.lse = x.lse;
   a.part_o = static_cast<float*>(x.workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows(x, p) * c.head_dim);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows(c, x, p) * c.head_dim);
   a.scale = (float)x.scale;
   a.type = (int)x.type;
   a.batch = (int)x.batch, a.queries = (int)x.queries, a.heads = (int)x.heads, a.kv_heads = (int)c.kv_heads;
@@ -272,13 +520,15 @@ hipError_t launch_kv_attention(const shk_kv_cache& c, const shk_kv_attention& x,
   a.page_shift = __builtin_ctzl((unsigned long)c.page_size);
   a.table_tokens = (int)(x.table_pages * c.page_size);
   a.prefix = (int)x.prefix_length;
-  a.own_splits = p.own_splits, a.prefix_splits = p.prefix_splits;
-  a.own_tiles = p.own_tiles, a.prefix_tiles = p.prefix_tiles;
+  a.own_groups = p.own_groups, a.own_tiles = p.own_tiles;
+  a.prefix_splits = p.prefix_splits, a.prefix_tiles = p.prefix_tiles;
+  a.slots = p.own_groups + a.batch;
+  a.direct = p.direct;
   if (c.bits == 4)
-    return x.type == SHK_SRC_BF16 ? launch_d<4, SHK_SRC_BF16>(c.head_dim, p.rt, a, s)
-                                  : launch_d<4, SHK_SRC_F16>(c.head_dim, p.rt, a, s);
-  return x.type == SHK_SRC_BF16 ? launch_d<8, SHK_SRC_BF16>(c.head_dim, p.rt, a, s)
-                                : launch_d<8, SHK_SRC_F16>(c.head_dim, p.rt, a, s);
+    return x.type == SHK_SRC_BF16 ? launch_d<4, SHK_SRC_BF16>(c.head_dim, a, p, s)
+                                  : launch_d<4, SHK_SRC_F16>(c.head_dim, a, p, s);
+  return x.type == SHK_SRC_BF16 ? launch_d<8, SHK_SRC_BF16>(c.head_dim, a, p, s)
+                                : launch_d<8, SHK_SRC_F16>(c.head_dim, a, p, s);
 }
 
 }  // namespace shk

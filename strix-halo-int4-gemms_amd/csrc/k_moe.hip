@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "shk_common.h"
+#include "shk_loads.h"
 #include "shk_moe.h"
 
 namespace shk {
@@ -35,14 +36,8 @@ namespace {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-typedef __attribute__((address_space(1))) const uint8_t* global_bytes;
 typedef __attribute__((address_space(1))) const uint16_t* global_halves;
-typedef uint32_t any_u32 __attribute__((aligned(1)));  // loads of any alignment
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-typedef u2 any_u2 __attribute__((aligned(1)));
-typedef u4 any_u4 __attribute__((aligned(1)));
 
 constexpr int kHalf = 64;          // columns of half a workgroup's tile
 constexpr int kPitch = 2 * kHalf + 4;  // floats of an LDS row of sums: rows start on different banks
@@ -90,17 +85,6 @@ struct Codes {
   const uint8_t *w, *end;
   int total, k_packed;  // columns of a row (NN) and bytes of one (NT)
 };
-
-// Loads from a uniform address, kept in scalar registers, plus a lane's 32-bit
-// offset: left to itself the compiler keeps one 64-bit vector address for every
-// load of a piece.  The address space is spelled out, since the empty asm hides
-// where the pointer comes from and flat loads cannot be waited for one by one.
-template <typename T>
-__device__ __forceinline__ T load_at(const uint8_t* p, uint32_t mine) {
-  global_bytes q = (global_bytes)p;
-  asm("" : "+s"(q));
-  return *(__attribute__((address_space(1))) const T*)(q + mine);
-}
 
 // 16 dwords of a lane: the codes of 128 K values from k0 for 64 columns from
 // n0, as they are stored.  What lies outside the expert's matrix meets
@@ -302,7 +286,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
           if constexpr (decltype(end)::value)
             b.sc[i] = p[min(sc_n, s.total - 1)] | ((uint32_t)p[min(sc_n + 1, s.total - 1)] << 16);
           else
-            b.sc[i] = load_at<any_u32>(reinterpret_cast<const uint8_t*>(p), 2u * (uint32_t)sc_n);
+            b.sc[i] = load_at<any_u32>(p, 2u * (uint32_t)sc_n);
         }
     }
   };

@@ -1,10 +1,7 @@
-// Attention of a few query rows over a piece of the quantized cache: the
-// streaming tile that the decode kernel runs (k_kvattn.hip).
+// Attention of a few query rows over a piece of the quantized cache: what the
+// streaming kernel and the shared-prefix kernel have in common (k_kvattn.hip).
 //
-// One workgroup of four waves serves one key head and up to 16 * RT query
-// rows (the queries of a sequence that read this key head, or, for a shared
-// prefix, those of all sequences).  A wave takes 64 tokens at a time, 16 by
-// 16 in four blocks i, and keeps everything in registers:
+// Tokens are taken 64 at a time, in four blocks i of 16:
 //
 //   S^T = K q^T   v_mfma_f32_16x16x32_f16, tokens in the rows, query rows in
 //                 the columns: lane (g = lane / 16, c = lane % 16) gets the
@@ -20,33 +17,39 @@
 // score (K) or its probability (V) instead of head_dim values.  q enters as
 // q * 2^-e with its row's largest magnitude in [1, 2): bf16 and f16 values
 // then keep all their bits in f16 down to 2^-14 of the largest one.
-// Probabilities enter as p * (v_scale / 2^ref) * 2^13, ref the exponent of
-// the largest v_scale that the wave has met: at most 2^15, so f16 does not
-// overflow, and normal down to 2^-28 of the largest; for f16 outputs they are split into two f16 terms, because
-// one rounding to 11 bits would be as large as the output's own.
-// Sums, maxima and outputs are f32.
+//
+// A row's probabilities are taken relative to
+//   m = max(score) + exponent(max(v_scale)) - 13,
+// in powers of two and over what the row has met so far, not to the largest
+// score: 2^(score - m) * v_scale is then at most 2^14, so f16 does not
+// overflow and keeps all its bits down to 2^-27 of the largest term, whatever
+// the scales are (an exponent below -80 counts as -80, so that the sum cannot
+// overflow either).  For f16 outputs the term is split into two f16 terms,
+// because one rounding to 11 bits would be as large as the output's own.
+// Maxima, sums and outputs are f32.
 #pragma once
 
 #include "shk_common.h"
 #include "shk_kvcache.h"
+#include "shk_loads.h"
 
 namespace shk {
 
-constexpr int kKvTile = 64;  // tokens of a wave's step
+constexpr int kKvTile = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Two codes that sit in the low bytes / nibbles of a dword's halves, as f16.
-// 0x6400 | n is 1024 + n, exactly; int4 codes come offset by 8 (their sign
-// bits flipped), int8 codes by 128.
+// Two codes that sit in the low bytes / nibbles of a dword's halves, as f16:
+// 0x6400 | n is 1024 + n exactly, n the code with its sign bit flipped (code + 8
+// or + 128), which the exclusive or does on the way.
 __device__ __forceinline__ h2 nib_lo(uint32_t w) {
-  return __builtin_bit_cast(h2, (w & 0x000F000Fu) | 0x64006400u) - (h2)(_Float16)1032.0f;
+  return __builtin_bit_cast(h2, (w & 0x000F000Fu) ^ 0x64086408u) - (h2)(_Float16)1032.0f;
 }
 __device__ __forceinline__ h2 nib_hi(uint32_t w) {  // bits 4..7: 1024 + 16 n, over 16
-  return __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00F000F0u) | 0x64006400u), (h2)(_Float16)0.0625f,
+  return __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00F000F0u) ^ 0x64806480u), (h2)(_Float16)0.0625f,
                                    (h2)(_Float16)-72.0f);
 }
-__device__ __forceinline__ h2 byte_pair(uint32_t w) {  // w = u0 | u1 << 16, u = code + 128
-  return __builtin_bit_cast(h2, w | 0x64006400u) - (h2)(_Float16)1152.0f;
+__device__ __forceinline__ h2 byte_pair(uint32_t w) {  // w = byte | byte << 16
+  return __builtin_bit_cast(h2, w ^ 0x64806480u) - (h2)(_Float16)1152.0f;
 }
 
 __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
@@ -55,13 +58,11 @@ __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
 
 // 8 codes of one row as a product's operand.  int4 codes 0..7 of a dword come
 // in the order 0 4 1 5 2 6 3 7 (kv_order), which q's operand repeats.
-__device__ __forceinline__ h8 codes4(uint32_t w) {
-  w ^= 0x88888888u;
+__device__ __forceinline__ h8 row_codes4(uint32_t w) {
   const uint32_t u = w >> 8;
   return join(nib_lo(w), nib_hi(w), nib_lo(u), nib_hi(u));
 }
-__device__ __forceinline__ h8 codes8(uint32_t lo, uint32_t hi) {
-  lo ^= 0x80808080u, hi ^= 0x80808080u;
+__device__ __forceinline__ h8 row_codes8(uint32_t lo, uint32_t hi) {
   return join(byte_pair(perm_b32(0, lo, 0x0C010C00u)), byte_pair(perm_b32(0, lo, 0x0C030C02u)),
               byte_pair(perm_b32(0, hi, 0x0C010C00u)), byte_pair(perm_b32(0, hi, 0x0C030C02u)));
 }
@@ -88,40 +89,109 @@ struct KvView {  // one key head of the cache
   const uint8_t *kc, *vc;
   const uint16_t *ks, *vs;
   int pages, page_shift, heads, head;
+
+  // First row of a block of 16 tokens; a page outside the cache reads as the
+  // first one and is remembered.
+  __device__ __forceinline__ long row_of(const int32_t* table, int blk, bool& bad) const {
+    int page = __builtin_amdgcn_readfirstlane(table[blk >> (page_shift - 4)]);
+    if ((unsigned)page >= (unsigned)pages) page = 0, bad = true;
+    return (((long)page * heads + head) << page_shift) + ((blk << 4) & ((1 << page_shift) - 1));
+  }
 };
 
-struct KvRow {     // what a lane's query row needs
-  const void* q;   // null: no such row
-  int limit;       // tokens it sees of this piece
+// A lane's share of a block of 16 tokens: 1/4 of the K row of token c, 1/16
+// of the V rows of the tokens 4 g + r.
+template <int BITS, int D>
+struct KvBlock {
+  static constexpr int kRow = D * BITS / 8;              // bytes of a cached row
+  static constexpr int kK = kRow / 16;                   // dwords
+  static constexpr int kV = kRow >= 64 ? kRow / 64 : 1;  // dwords (2 bytes of one at 32)
+  uint32_t k[kK], v[4][kV];
+
+  __device__ __forceinline__ void load(const KvView& kv, long row0) {
+    const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
+    const uint8_t* ks = kv.kc + row0 * kRow;
+    const uint32_t my_k = (uint32_t)(c * kRow + g * (kRow / 4));
+    if constexpr (kK == 2) {
+      const u2 w = load_at<u2>(ks, my_k);
+      k[0] = w[0], k[1] = w[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kK; j += 4) {
+        const u4 w = load_at<u4>(ks + 4 * j, my_k);
+        k[j] = w[0], k[j + 1] = w[1], k[j + 2] = w[2], k[j + 3] = w[3];
+      }
+    }
+    const uint8_t* vs = kv.vc + row0 * kRow;
+    const uint32_t my_v = (uint32_t)(4 * g * kRow + c * (kRow / 16));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (kRow == 32) {
+        v[r][0] = load_at<uint16_t>(vs + r * kRow, my_v);
+      } else if constexpr (kV == 1) {
+        v[r][0] = load_at<uint32_t>(vs + r * kRow, my_v);
+      } else if constexpr (kV == 2) {
+        const u2 w = load_at<u2>(vs + r * kRow, my_v);
+        v[r][0] = w[0], v[r][1] = w[1];
+      } else {
+        const u4 w = load_at<u4>(vs + r * kRow, my_v);
+        v[r][0] = w[0], v[r][1] = w[1], v[r][2] = w[2], v[r][3] = w[3];
+      }
+    }
+  }
+
+  __device__ __forceinline__ h8 k_operand(int step) const {
+    if constexpr (BITS == 4) return row_codes4(k[step]);
+    else return row_codes8(k[2 * step], k[2 * step + 1]);
+  }
+  // V of the tokens 4 g + 2 x and + 1, for head_dim (D / 16) c + 4 w + j: four
+  // values of j at a time.
+  __device__ __forceinline__ void v_pairs(int w, int x, h2 (&f)[4]) const {
+    if constexpr (BITS == 4) {
+      const uint32_t y = perm_b32(v[2 * x + 1][w / 2], v[2 * x][w / 2], w % 2 ? 0x07060302u : 0x05040100u);
+      f[0] = nib_lo(y), f[1] = nib_hi(y), f[2] = nib_lo(y >> 8), f[3] = nib_hi(y >> 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = byte_pair(perm_b32(v[2 * x + 1][w], v[2 * x][w], 0x0C000C00u | (uint32_t)((4 + j) << 16) | (uint32_t)j));
+    }
+  }
 };
 
+// bf16 scales of the tokens 4 g + r of a block.
+__device__ __forceinline__ u2 load_scales(const uint16_t* s, long row0) {
+  return load_at<u2>(s + row0, 8 * ((threadIdx.x & 63) / 16));
+}
+__device__ __forceinline__ f4 widen_scales(u2 w) {
+  return f4{bf16_bits_to_f32((uint16_t)w[0]), __uint_as_float(w[0] & 0xFFFF0000u), bf16_bits_to_f32((uint16_t)w[1]),
+            __uint_as_float(w[1] & 0xFFFF0000u)};
+}
+
+// A wave's query rows (16 * RT, row c of tile t in lane c of every group) and
+// their running softmax.
 template <int BITS, int D, int RT, int TYPE>
-struct KvTile {
-  static constexpr int kRow = D * BITS / 8;       // bytes of a cached row
-  static constexpr int kK = kRow / 16;            // dwords of a lane's share of a K row
-  static constexpr int kV = kRow >= 64 ? kRow / 64 : 1;  // dwords of a lane's share of a V row (2 bytes of one at 32)
+struct KvRows {
   static constexpr int kSteps = D / 32, kOut = D / 16;
   static constexpr bool kSplitP = TYPE == SHK_SRC_F16;
 
   h8 q[RT][kSteps];
-  float qs[RT];  // 2^e of the row, times softmax scale and log2(e)
+  float qs[RT];  // 2^e of the row, times |softmax scale| and log2(e)
   f4 o[RT][kOut];
-  float m[RT], l[RT];
-  int ref;       // biased exponent that v scales are taken relative to
-  bool bad;      // a page outside the cache
+  float m[RT], l[RT];  // reference and sum (the lane's tokens only)
+  uint32_t big;        // bits of the largest v scale met
 
-  // q[c][g * (D / 4) + 8 s + kv_order(i)] for step s.
-  __device__ __forceinline__ void begin(const KvRow (&row)[RT], float scale) {
+  // q[c][g * (D / 4) + 8 s + kv_order(i)] for step s; null rows are zero.
+  __device__ __forceinline__ void begin(const void* const (&row)[RT], float scale) {
     const int g = (threadIdx.x & 63) / 16;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       float v[kSteps][8];
       uint32_t most = 0;
-      const uint4* src = static_cast<const uint4*>(row[t].q) + g * (D / 32);
+      const uint4* src = static_cast<const uint4*>(row[t]) + g * (D / 32);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (row[t].q != nullptr) w = src[s];
+        if (row[t] != nullptr) w = src[s];
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -134,8 +204,8 @@ struct KvTile {
       most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
       // the largest magnitude's exponent, within what both 2^e and 2^-e hold
       const int e = min(max((int)(most >> 23), 1), 253);
-      const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-      qs[t] = __uint_as_float((uint32_t)e << 23) * (scale * kLog2e);
+      const float inv = __builtin_copysignf(__uint_as_float((uint32_t)(254 - e) << 23), scale);
+      qs[t] = __uint_as_float((uint32_t)e << 23) * (__builtin_fabsf(scale) * kLog2e);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -145,118 +215,48 @@ struct KvTile {
 #pragma unroll
       for (int j = 0; j < kOut; ++j) o[t][j] = f4{0, 0, 0, 0};
     }
-    ref = 1;
-    bad = false;
+    big = 0;
   }
 
-  // Tokens [t0, t0 + 64) of a sequence of n (t0 < n, a multiple of 64).
-  __device__ __forceinline__ void step(const KvView& kv, const int32_t* table, int t0, int n, const int (&limit)[RT],
-                                       int least_limit) {
-    const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
-    const int last = (n - 1) >> 4;  // the last block that holds a token; later ones repeat it, masked
-    uint32_t kw[4][kK], vw[16][kV];
-    uint2 ksw[4], vsw[4];
+  // Scores (before the row's factor) of 64 tokens and their scales to the
+  // second product's operands; o shrinks where a row's reference grew.
+  // limit[t]: the row's tokens end there, counted from the step's first;
+  // `ends`: some row's do (uniform); held: the sequence's tokens end there.
+  __device__ __forceinline__ void soften(f4 (&s)[RT][4], const f4 (&ks)[4], f4 (&vs)[4], bool ends,
+                                         const int (&limit)[RT], int held, h8 (&p)[RT][2], h8 (&pl)[RT][2]) {
+    const int g = (threadIdx.x & 63) / 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int blk = min((t0 >> 4) + i, last);
-      int page = table[blk >> (kv.page_shift - 4)];
-      if ((unsigned)page >= (unsigned)kv.pages) page = 0, bad = true;
-      const int in_page = (blk << 4) & ((1 << kv.page_shift) - 1);
-      const long row0 = (((long)page * kv.heads + kv.head) << kv.page_shift) + in_page;
-      const uint32_t* ksrc = reinterpret_cast<const uint32_t*>(kv.kc + (row0 + c) * kRow) + g * kK;
-      if constexpr (kK == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(ksrc);
-        kw[i][0] = w.x, kw[i][1] = w.y;
-      } else {
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int j = 0; j < kK; j += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(ksrc + j);
-          kw[i][j] = w.x, kw[i][j + 1] = w.y, kw[i][j + 2] = w.z, kw[i][j + 3] = w.w;
-        }
-      }
-      ksw[i] = *reinterpret_cast<const uint2*>(kv.ks + row0 + 4 * g);
-      vsw[i] = *reinterpret_cast<const uint2*>(kv.vs + row0 + 4 * g);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint8_t* vsrc = kv.vc + (row0 + 4 * g + r) * kRow + c * (kRow / 16);
-        uint32_t* dst = vw[4 * i + r];
-        if constexpr (kRow == 32) {
-          dst[0] = *reinterpret_cast<const uint16_t*>(vsrc);
-        } else if constexpr (kV == 1) {
-          dst[0] = *reinterpret_cast<const uint32_t*>(vsrc);
-        } else if constexpr (kV == 2) {
-          const uint2 w = *reinterpret_cast<const uint2*>(vsrc);
-          dst[0] = w.x, dst[1] = w.y;
-        } else {
-          const uint4 w = *reinterpret_cast<const uint4*>(vsrc);
-          dst[0] = w.x, dst[1] = w.y, dst[2] = w.z, dst[3] = w.w;
-        }
-      }
-    }
-    float s[RT][4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f4 acc[RT];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) acc[t] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        h8 k;
-        if constexpr (BITS == 4) k = codes4(kw[i][st]);
-        else k = shk::codes8(kw[i][2 * st], kw[i][2 * st + 1]);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = mfma_f16(k, q[t][st], acc[t]);
-      }
-      const float ks[4] = {bf16_bits_to_f32((uint16_t)ksw[i].x), __uint_as_float(ksw[i].x & 0xFFFF0000u),
-                           bf16_bits_to_f32((uint16_t)ksw[i].y), __uint_as_float(ksw[i].y & 0xFFFF0000u)};
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[t][i][r] = acc[t][r] * (ks[r] * qs[t]);
-    }
-    float vs[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vs[i][0] = bf16_bits_to_f32((uint16_t)vsw[i].x), vs[i][1] = __uint_as_float(vsw[i].x & 0xFFFF0000u);
-      vs[i][2] = bf16_bits_to_f32((uint16_t)vsw[i].y), vs[i][3] = __uint_as_float(vsw[i].y & 0xFFFF0000u);
-    }
-    if (t0 + kKvTile > least_limit) {  // some row ends in this step
+      for (int i = 0; i < 4; ++i) s[t][i] *= ks[i];
+    if (ends) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int at = t0 + 16 * i + 4 * g + r;
+          const int at = 16 * i + 4 * g + r;
 #pragma unroll
           for (int t = 0; t < RT; ++t)
             if (at >= limit[t]) s[t][i][r] = -__builtin_inff();
-          if (at >= n) vs[i][r] = 0.0f;  // never written: may hold anything
+          if (at >= held) vs[i][r] = 0.0f;  // never written: may hold anything
         }
     }
-    // exponent of the largest v scale so far
-    uint32_t big = 0;
+    uint32_t most = big;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) big = max(big, __float_as_uint(vs[i][r]));
-    big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
-    big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
-    const int e = max(ref, min((int)((big >> 23) & 0xFF), 253));
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23) * 8192.0f;
-    const float shrink = e == ref ? 1.0f : (e - ref < 127 ? __uint_as_float((uint32_t)(127 - (e - ref)) << 23) : 0.0f);
-    ref = e;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) vs[i][r] *= inv;
-    h8 p[RT][2], pl[RT][2];
+      for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(vs[i][r]));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+    big = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+    const float up = (float)(min(max((int)(big >> 23), 47), 254) - 127 - 13);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      float top = m[t];
+      float top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = __builtin_fmaxf(top, s[t][i][r]);
-      top = groups_max(top);
+      top = __builtin_fmaxf(m[t], groups_max(top) * qs[t] + up);
       const float base = top == -__builtin_inff() ? 0.0f : top;
       const float alpha = __builtin_amdgcn_exp2f(m[t] - base);
       m[t] = top;
@@ -265,7 +265,7 @@ struct KvTile {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float pv = __builtin_amdgcn_exp2f(s[t][i][r] - base);
+          const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i][r], qs[t], -base));
           sum += pv;
           const float w = pv * vs[i][r];
           const _Float16 hi = (_Float16)w;
@@ -273,43 +273,15 @@ struct KvTile {
           if constexpr (kSplitP) pl[t][i / 2][4 * (i % 2) + r] = (_Float16)(w - (float)hi);
         }
       l[t] = l[t] * alpha + sum;
-      const float a = alpha * shrink;
-      if (__any(a != 1.0f)) {
+      if (__any(alpha != 1.0f)) {
 #pragma unroll
-        for (int j = 0; j < kOut; ++j) o[t][j] *= a;
-      }
-    }
-    // O^T += V^T P^T, 32 tokens (blocks 2 h and 2 h + 1) at a time
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if constexpr (BITS == 4) {
-#pragma unroll
-        for (int w = 0; w < (kOut + 3) / 4; ++w) {  // four head_dim values a piece
-          h2 f[4][4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t a = vw[8 * h + 2 * x][w / 2], b = vw[8 * h + 2 * x + 1][w / 2];
-            const uint32_t y = perm_b32(b, a, w % 2 ? 0x07060302u : 0x05040100u) ^ 0x88888888u;
-            f[0][x] = nib_lo(y), f[1][x] = nib_hi(y), f[2][x] = nib_lo(y >> 8), f[3][x] = nib_hi(y >> 8);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) pv_step(4 * w + j, join(f[j][0], f[j][1], f[j][2], f[j][3]), p, pl, h);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kOut; ++j) {
-          h2 f[4];
-          const uint32_t sel = 0x0C000C00u | (uint32_t)((4 + j % 4) << 16) | (uint32_t)(j % 4);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            f[x] = byte_pair(perm_b32(vw[8 * h + 2 * x + 1][j / 4], vw[8 * h + 2 * x][j / 4], sel) ^ 0x00800080u);
-          pv_step(j, join(f[0], f[1], f[2], f[3]), p, pl, h);
-        }
+        for (int j = 0; j < kOut; ++j) o[t][j] *= alpha;
       }
     }
   }
 
-  __device__ __forceinline__ void pv_step(int j, const h8& v, const h8 (&p)[RT][2], const h8 (&pl)[RT][2], int h) {
+  // o^T += V^T P^T for 32 tokens and 16 values of head_dim.
+  __device__ __forceinline__ void add(int j, const h8& v, const h8 (&p)[RT][2], const h8 (&pl)[RT][2], int h) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       o[t][j] = mfma_f16(v, p[t][h], o[t][j]);

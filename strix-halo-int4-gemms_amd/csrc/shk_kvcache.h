@@ -19,7 +19,6 @@ namespace shk {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 hipError_t launch_kv_write(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s);
 hipError_t launch_kv_read(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s);
