@@ -25,6 +25,7 @@ int check_cache(const shk_kv_cache* c) {
     return capi_fail("cache page_size must be a power of two from 16 to 1024; got " + std::to_string(c->page_size));
   if (c->kv_heads < 1 || c->kv_heads > 65535 || c->pages < 1 || c->pages > INT_MAX)
     return capi_fail("cache needs 1 to 65535 heads and 1 to 2147483647 pages");
+  if (c->pages * c->kv_heads > INT_MAX) return capi_fail("the cache holds more than 2147483647 pages of a head");
   if (!c->key_codes || !c->value_codes || !c->key_scales || !c->value_scales)
     return capi_fail("cache pointers must be non-null");
   if (!on(c->key_codes, 16) || !on(c->value_codes, 16)) return capi_fail("cache codes must be aligned to 16 bytes");

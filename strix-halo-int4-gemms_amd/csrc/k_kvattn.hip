@@ -100,7 +100,7 @@ __device__ __forceinline__ void store_piece(const AttnArgs& a, bool direct, long
 }
 
 template <int BITS, int D, int RT, int TYPE>
-__global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
   using Rows = KvRows<BITS, D, RT, TYPE>;
   constexpr int kPitch = D + 4;  // floats of an LDS row: the 16 rows start on different banks
   __shared__ __align__(16) float red_o[4][16 * kPitch];
@@ -117,7 +117,18 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_ke
   const int head = unit % a.kv_heads;
   unit /= a.kv_heads;
   const int tile = unit % tiles, j = unit / tiles;
-  const int total = shared ? pieces_of(a, a.prefix) : __builtin_amdgcn_readfirstlane(pieces_before(a, a.batch));
+  // the pieces of the first 64 sequences, a lane each, and their sums
+  const int tokens0 = !shared && lane < a.batch ? tokens_of(a, lane) : 0;
+  const int pieces0 = !shared && lane < a.batch ? pieces_of(a, tokens0) : 0;
+  int upto0 = pieces0;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int up = __shfl_up(upto0, d, 64);
+    if (lane >= d) upto0 += up;
+  }
+  int total = shared ? pieces_of(a, a.prefix) : __shfl(upto0, 63, 64);
+  if (!shared && a.batch > 64) total = pieces_before(a, a.batch);
+  total = __builtin_amdgcn_readfirstlane(total);
   const int each = max((total + groups - 1) / groups, 1);
   const int first = j * each, end = min(first + each, total);
   const int rows_here = own_rows(a) * (shared ? a.batch : 1);
@@ -125,29 +136,32 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_ke
 
   int b = 0, before = 0;  // the sequence that holds piece `first`, and the pieces before it
   if (!shared && first < end) {
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      int n = b0 + lane < a.batch ? pieces_of(a, tokens_of(a, b0 + lane)) : 0;
-      const int own = n;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int up = __shfl_up(n, d, 64);
-        if (lane >= d) n += up;
-      }
-      const unsigned long past = __ballot(before + n > first);
+    int upto = upto0, own = pieces0;
+    for (int b0 = 0;;) {
+      const unsigned long past = __ballot(before + upto > first);
       if (past != 0) {
         const int at = __builtin_ctzll(past);
         b = b0 + at;
-        before += __shfl(n - own, at, 64);
+        before += __shfl(upto - own, at, 64);
         break;
       }
-      before += __shfl(n, 63, 64);
+      before += __shfl(upto, 63, 64);
+      b0 += 64;
+      own = b0 + lane < a.batch ? pieces_of(a, tokens_of(a, b0 + lane)) : 0;
+      upto = own;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int up = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += up;
+      }
     }
     b = __builtin_amdgcn_readfirstlane(b);
     before = __builtin_amdgcn_readfirstlane(before);
   }
   // a sequence without tokens has no piece; a prefix split may have none either
   for (int piece = first; piece < end || (shared && piece == first); ++b) {
-    const int n = shared ? a.prefix : tokens_of(a, b);
+    const int n = shared ? a.prefix
+                         : (b < 64 ? __builtin_amdgcn_readfirstlane(__shfl(tokens0, b, 64)) : tokens_of(a, b));
     const int mine = min(end, before + pieces_of(a, n));  // this sequence's pieces end there
     if (!shared && mine <= piece) {
       before += pieces_of(a, n);
@@ -178,17 +192,44 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_ke
     bool bad = false;
     Rows rows;
     rows.begin(src, a.scale);
-    for (int i = 4 * (piece - before) + wave; i < 4 * (mine - before) && i * kKvTile < n; i += 4) {
-      const int t0 = i * kKvTile;
+    // A step's V is asked for with the next step's K, so half of the bytes are
+    // always on their way, where the registers hold them.
+    constexpr bool kAhead = D * BITS * RT <= 1024;
+    const int step0 = 4 * (piece - before) + wave, step_end = min(4 * (mine - before), (n + kKvTile - 1) / kKvTile);
+    const int step_last = step0 + (max(step_end - step0, 1) - 1) / 4 * 4;
+    struct Keys {
       KvBlock<BITS, D> blk[4];
-      u2 kss[4], vss[4];
+      u2 scales[4];
+    };
+    long rows_now[4], rows_next[4];  // first rows of the blocks
+    int page[4];                     // and pages of those after
+    auto pages = [&](int i) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const long row0 = kv.row_of(table, min(4 * i + x, last), bad);
-        blk[x].load(kv, row0);
-        kss[x] = load_scales(kv.ks, row0);
-        vss[x] = load_scales(kv.vs, row0);
+      for (int x = 0; x < 4; ++x) page[x] = kv.page_of(table, min(4 * min(i, step_last) + x, last));
+    };
+    auto find_rows = [&](int i, long (&r)[4]) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) r[x] = kv.row_of(page[x], min(4 * min(i, step_last) + x, last), bad);
+    };
+    auto load_keys = [&](const long (&r)[4], Keys& k) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) k.blk[x].load_k(kv, r[x]), k.scales[x] = load_scales(kv.ks, r[x]);
+    };
+    auto step = [&](int i, Keys& now, Keys& next) {
+      u2 vss[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) now.blk[x].load_v(kv, rows_now[x]), vss[x] = load_scales(kv.vs, rows_now[x]);
+      if constexpr (kAhead) {
+        find_rows(i + 4, rows_next);
+        load_keys(rows_next, next);
+      } else {
+        load_keys(rows_now, now);
+        find_rows(i + 4, rows_next);
       }
+      pages(i + 8);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) rows_now[x] = rows_next[x];
+      __builtin_amdgcn_sched_barrier(0);  // what has been asked for stays ahead
       f4 s[RT][4], ks[4], vs[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -196,13 +237,14 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_ke
         for (int t = 0; t < RT; ++t) s[t][x] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < Rows::kSteps; ++st) {
-          const h8 k = blk[x].k_operand(st);
+          const h8 k = now.blk[x].k_operand(st);
 #pragma unroll
           for (int t = 0; t < RT; ++t) s[t][x] = mfma_f16(k, rows.q[t][st], s[t][x]);
         }
-        ks[x] = widen_scales(kss[x]);
+        ks[x] = widen_scales(now.scales[x]);
         vs[x] = widen_scales(vss[x]);
       }
+      const int t0 = i * kKvTile;
       int left[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) left[t] = limit[t] - t0;
@@ -214,10 +256,29 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 2 : 3) void kv_stream_ke
         for (int w = 0; w < Rows::kOut / 4; ++w) {
           h2 f[4][4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) blk[2 * h + x / 2].v_pairs(w, x % 2, f[x]);
+          for (int x = 0; x < 4; ++x) now.blk[2 * h + x / 2].v_pairs(w, x % 2, f[x]);
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) rows.add(4 * w + jj, join(f[0][jj], f[1][jj], f[2][jj], f[3][jj]), p, pl, h);
         }
+    };
+    if (step0 < step_end) {
+      Keys now, next;
+      pages(step0);
+      find_rows(step0, rows_now);
+      if constexpr (kAhead) load_keys(rows_now, now);
+      pages(step0 + 4);
+#pragma unroll 1
+      for (int i = step0; i < step_end; i += 4) {
+        step(i, now, next);
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int w = 0; w < KvBlock<BITS, D>::kK; ++w) now.blk[x].k[w] = next.blk[x].k[w];
+            now.scales[x] = next.scales[x];
+          }
+        }
+      }
     }
 
     // the waves' outputs, relative to the largest of their references
@@ -283,6 +344,8 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
   // 32 tokens and 16 values of head_dim
   __shared__ h8 lds_k[kBuffers][4][kSteps][64];
   __shared__ h8 lds_v[kBuffers][2][kOut][64];
+  __shared__ __align__(16) float lds_s[kBuffers][2][kKvTile];  // scales
+  __shared__ int lds_bad;
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   int unit = blockIdx.x;
@@ -308,17 +371,18 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
   Rows rows;
   rows.begin(src, a.scale);
   bool bad = false;
+  if (threadIdx.x == 0) lds_bad = 0;
 
   Block mine;  // this wave's 16 of the 64 tokens
-  u2 kss[4], vss[4];
+  u2 ksw, vsw;
+  int page = first < end ? kv.page_of(a.prefix_pages, min(4 * first + wave, last)) : 0;
   auto load = [&](int step) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const long row0 = kv.row_of(a.prefix_pages, min(4 * step + x, last), bad);
-      kss[x] = load_scales(kv.ks, row0);
-      vss[x] = load_scales(kv.vs, row0);
-    }
-    mine.load(kv, kv.row_of(a.prefix_pages, min(4 * step + wave, last), bad));
+    const long row0 = kv.row_of(page, min(4 * step + wave, last), bad);
+    mine.load_k(kv, row0);
+    mine.load_v(kv, row0);
+    ksw = load_scales(kv.ks, row0);
+    vsw = load_scales(kv.vs, row0);
+    page = kv.page_of(a.prefix_pages, min(4 * min(step + 1, end - 1) + wave, last));
   };
   if (first < end) load(first);
   for (int step = first, at = 0; step < end; ++step, at = (at + 1) % kBuffers) {
@@ -335,11 +399,18 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
         reinterpret_cast<uint2*>(&lds_v[at][wave / 2][4 * w + j][lane])[wave % 2] = pair;
       }
     }
+    if (c == 0) {
+      *reinterpret_cast<f4*>(&lds_s[at][0][16 * wave + 4 * g]) = widen_scales(ksw);
+      *reinterpret_cast<f4*>(&lds_s[at][1][16 * wave + 4 * g]) = widen_scales(vsw);
+    }
+    load(min(step + 1, end - 1));  // on its way while this one is multiplied; the last one is loaded twice
+    __syncthreads();
     f4 ks[4], vs[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) ks[x] = widen_scales(kss[x]), vs[x] = widen_scales(vss[x]);
-    load(min(step + 1, end - 1));  // on its way while this one is multiplied
-    __syncthreads();
+    for (int x = 0; x < 4; ++x) {
+      ks[x] = *reinterpret_cast<const f4*>(&lds_s[at][0][16 * x + 4 * g]);
+      vs[x] = *reinterpret_cast<const f4*>(&lds_s[at][1][16 * x + 4 * g]);
+    }
     f4 s[RT][4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -363,6 +434,10 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
       for (int j = 0; j < kOut; ++j) rows.add(j, lds_v[at][h][j][lane], p, pl, h);
     if constexpr (kBuffers == 1) __syncthreads();
   }
+  __syncthreads();  // lds_bad has been cleared; a page outside the cache is every row's
+  if (bad && lane == 0) lds_bad = 1;
+  __syncthreads();
+  bad = lds_bad != 0;
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const float l = groups_sum(rows.l[t]);
@@ -378,17 +453,27 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
   }
 }
 
-// Joins the pieces of a row, a wave each: lane p looks at piece p, then all
-// lanes add up the outputs, D / 64 values each.
+// Joins the pieces of a row, a workgroup each: lane p of every wave looks at
+// piece p, then wave w adds up the outputs of the pieces w, w + 4, ..., D / 64
+// values a lane.
 template <int D>
 __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
   typedef float fv __attribute__((ext_vector_type(D / 64)));
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  if (row >= (long)a.batch * a.queries * a.heads) return;
+  __shared__ fv part[4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const long row = blockIdx.x;
   const int h = (int)(row % a.heads), query = (int)(row / a.heads % a.queries), b = (int)(row / a.heads / a.queries);
   const int head = h / a.ratio, in = query * a.ratio + h % a.ratio, per = own_rows(a);
-  const int total = pieces_before(a, a.batch), before = pieces_before(a, b), mine = pieces_of(a, tokens_of(a, b));
+  // pieces before the sequence, its own, and all
+  int before = 0, total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int n = b0 + lane < a.batch ? pieces_of(a, tokens_of(a, b0 + lane)) : 0;
+    total += n;
+    before += b0 + lane < b ? n : 0;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d, 64), before += __shfl_xor(before, d, 64);
+  const int mine = pieces_of(a, tokens_of(a, b));
   const int each = max((total + a.own_groups - 1) / a.own_groups, 1);
   const int first = before / each, own = mine == 0 ? 0 : (before + mine - 1) / each - first + 1;
   const int count = own + a.prefix_splits;
@@ -404,25 +489,38 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
   float sum = 0.0f;
   fv v = {};
   for (int p0 = 0; p0 < count; p0 += 64) {
-    const int here = min(count - p0, 64);
     float weight = 0.0f;
-    if (lane < here) {
+    if (p0 + lane < count) {
       const float2 ml = a.part_ml[place(p0 + lane)];
       weight = ml.x == -__builtin_inff() && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - base);
       sum += weight == 0.0f ? 0.0f : ml.y * weight;
     }
-#pragma unroll 8
-    for (int p = 0; p < here; ++p)
-      v += reinterpret_cast<const fv*>(a.part_o + place(p0 + p) * D)[lane] * __shfl(weight, p, 64);
+    const int here = min(count - p0, 64);
+    for (int p = wave; p < here; p += 32) {  // eight loads at a time
+      fv o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        o[i] = reinterpret_cast<const fv*>(a.part_o + place(p0 + min(p + 4 * i, here - 1)) * D)[lane];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __shfl(weight, min(p + 4 * i, here - 1), 64);
+        if (p + 4 * i < here && w != 0.0f) v += o[i] * w;
+      }
+    }
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-  v *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  part[wave][lane] = v;
+  __syncthreads();
+  if (wave != 0) return;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const uint16_t o = a.type == SHK_SRC_BF16 ? (uint16_t)f32_to_bf16_rne(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
-    a.out[row * D + lane * (D / 64) + i] = o;
-  }
+  for (int w = 1; w < 4; ++w) v += part[w][lane];
+  v *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t o[D / 64];
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+    o[i] = a.type == SHK_SRC_BF16 ? (uint16_t)f32_to_bf16_rne(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+  __builtin_memcpy(a.out + row * D + lane * (D / 64), o, sizeof(o));
   if (lane == 0 && a.lse != nullptr) a.lse[row] = natural_lse(top, sum);
 }
 
@@ -446,7 +544,7 @@ Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
   p.own_tiles = (int)cdiv(rows, 16 * p.rt);
   p.direct = !prefix && tokens <= kPiece;
   // three workgroups on each of the 256 CUs, two where they hold more
-  const long want = p.rt == 2 || wide ? 512 : 768;
+  const long want = 512;
   p.own_groups = p.direct ? (int)a.batch
                           : (int)std::max(1L, std::min(want / (c.kv_heads * p.own_tiles), a.batch * cdiv(tokens, kPiece)));
   if (prefix) {
@@ -482,7 +580,7 @@ hipError_t launch_kernels(const AttnArgs& a, const Plan& p, hipStream_t s) {
   }
   if (err != hipSuccess || a.direct) return err;
   const long rows = (long)a.batch * a.queries * a.heads;
-  hipLaunchKernelGGL((kv_join_kernel<D>), dim3((unsigned)cdiv(rows, 4)), block, 0, s, a);
+  hipLaunchKernelGGL((kv_join_kernel<D>), dim3((unsigned)rows), block, 0, s, a);
   return hipGetLastError();
 }
 

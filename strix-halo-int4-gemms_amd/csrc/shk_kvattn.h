@@ -90,12 +90,14 @@ struct KvView {  // one key head of the cache
   const uint16_t *ks, *vs;
   int pages, page_shift, heads, head;
 
-  // First row of a block of 16 tokens; a page outside the cache reads as the
-  // first one and is remembered.
-  __device__ __forceinline__ long row_of(const int32_t* table, int blk, bool& bad) const {
-    int page = __builtin_amdgcn_readfirstlane(table[blk >> (page_shift - 4)]);
+  // The page of a block of 16 tokens, asked for a step before it is needed.
+  __device__ __forceinline__ int page_of(const int32_t* table, int blk) const { return table[blk >> (page_shift - 4)]; }
+  // The block's first row; a page outside the cache reads as the first one
+  // and is remembered.
+  __device__ __forceinline__ long row_of(int page, int blk, bool& bad) const {
+    page = __builtin_amdgcn_readfirstlane(page);
     if ((unsigned)page >= (unsigned)pages) page = 0, bad = true;
-    return (((long)page * heads + head) << page_shift) + ((blk << 4) & ((1 << page_shift) - 1));
+    return ((long)(page * heads + head) << page_shift) + ((blk << 4) & ((1 << page_shift) - 1));
   }
 };
 
@@ -108,7 +110,7 @@ struct KvBlock {
   static constexpr int kV = kRow >= 64 ? kRow / 64 : 1;  // dwords (2 bytes of one at 32)
   uint32_t k[kK], v[4][kV];
 
-  __device__ __forceinline__ void load(const KvView& kv, long row0) {
+  __device__ __forceinline__ void load_k(const KvView& kv, long row0) {
     const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
     const uint8_t* ks = kv.kc + row0 * kRow;
     const uint32_t my_k = (uint32_t)(c * kRow + g * (kRow / 4));
@@ -118,23 +120,26 @@ struct KvBlock {
     } else {
 #pragma unroll
       for (int j = 0; j < kK; j += 4) {
-        const u4 w = load_at<u4>(ks + 4 * j, my_k);
+        const u4 w = load_at<u4>(ks, my_k, 4 * j);
         k[j] = w[0], k[j + 1] = w[1], k[j + 2] = w[2], k[j + 3] = w[3];
       }
     }
+  }
+  __device__ __forceinline__ void load_v(const KvView& kv, long row0) {
+    const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
     const uint8_t* vs = kv.vc + row0 * kRow;
     const uint32_t my_v = (uint32_t)(4 * g * kRow + c * (kRow / 16));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if constexpr (kRow == 32) {
-        v[r][0] = load_at<uint16_t>(vs + r * kRow, my_v);
+        v[r][0] = load_at<uint16_t>(vs, my_v, r * kRow);
       } else if constexpr (kV == 1) {
-        v[r][0] = load_at<uint32_t>(vs + r * kRow, my_v);
+        v[r][0] = load_at<uint32_t>(vs, my_v, r * kRow);
       } else if constexpr (kV == 2) {
-        const u2 w = load_at<u2>(vs + r * kRow, my_v);
+        const u2 w = load_at<u2>(vs, my_v, r * kRow);
         v[r][0] = w[0], v[r][1] = w[1];
       } else {
-        const u4 w = load_at<u4>(vs + r * kRow, my_v);
+        const u4 w = load_at<u4>(vs, my_v, r * kRow);
         v[r][0] = w[0], v[r][1] = w[1], v[r][2] = w[2], v[r][3] = w[3];
       }
     }

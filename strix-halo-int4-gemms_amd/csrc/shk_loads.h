@@ -16,12 +16,13 @@ typedef uint32_t any_u32 __attribute__((aligned(1)));  // of any alignment
 typedef u2 any_u2 __attribute__((aligned(1)));
 typedef u4 any_u4 __attribute__((aligned(1)));
 
+// `offset` goes into the instruction: loads near each other share an address.
 template <typename T>
-__device__ __forceinline__ T load_at(const void* p, uint32_t mine) {
+__device__ __forceinline__ T load_at(const void* p, uint32_t mine, int offset = 0) {
   typedef __attribute__((address_space(1))) const uint8_t* global_bytes;
   global_bytes q = (global_bytes)p;
   asm("" : "+s"(q));
-  return *(__attribute__((address_space(1))) const T*)(q + mine);
+  return *(__attribute__((address_space(1))) const T*)(q + mine + offset);
 }
 
 }  // namespace shk
