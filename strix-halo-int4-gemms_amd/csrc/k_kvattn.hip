@@ -102,6 +102,10 @@ __device__ __forceinline__ void store_piece(const AttnArgs& a, bool direct, long
 template <int BITS, int D, int RT, int TYPE>
 __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
   using Rows = KvRows<BITS, D, RT, TYPE>;
+  // blocks of 16 tokens a wave takes at a time: half of the usual four where
+  // they would not fit the registers
+  constexpr int NB = D * RT >= 256 ? 2 : 4;
+  constexpr int kStep = 16 * NB, kPer = kPiece / kStep;
   constexpr int kPitch = D + 4;  // floats of an LDS row: the 16 rows start on different banks
   __shared__ __align__(16) float red_o[4][16 * kPitch];
   __shared__ float red_m[4][16], red_l[4][16];
@@ -194,31 +198,31 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
     rows.begin(src, a.scale);
     // A step's V is asked for with the next step's K, so half of the bytes are
     // always on their way, where the registers hold them.
-    constexpr bool kAhead = D * BITS * RT <= 1024;
-    const int step0 = 4 * (piece - before) + wave, step_end = min(4 * (mine - before), (n + kKvTile - 1) / kKvTile);
+    constexpr bool kAhead = D * BITS * RT * NB <= 4096;
+    const int step0 = kPer * (piece - before) + wave, step_end = min(kPer * (mine - before), (n + kStep - 1) / kStep);
     const int step_last = step0 + (max(step_end - step0, 1) - 1) / 4 * 4;
     struct Keys {
-      KvBlock<BITS, D> blk[4];
-      u2 scales[4];
+      KvBlock<BITS, D> blk[NB];
+      u2 scales[NB];
     };
-    long rows_now[4], rows_next[4];  // first rows of the blocks
-    int page[4];                     // and pages of those after
+    long rows_now[NB], rows_next[NB];  // first rows of the blocks
+    int page[NB];                    // and pages of those after
     auto pages = [&](int i) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) page[x] = kv.page_of(table, min(4 * min(i, step_last) + x, last));
+      for (int x = 0; x < NB; ++x) page[x] = kv.page_of(table, min(NB * min(i, step_last) + x, last));
     };
-    auto find_rows = [&](int i, long (&r)[4]) {
+    auto find_rows = [&](int i, long (&r)[NB]) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) r[x] = kv.row_of(page[x], min(4 * min(i, step_last) + x, last), bad);
+      for (int x = 0; x < NB; ++x) r[x] = kv.row_of(page[x], min(NB * min(i, step_last) + x, last), bad);
     };
-    auto load_keys = [&](const long (&r)[4], Keys& k) {
+    auto load_keys = [&](const long (&r)[NB], Keys& k) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) k.blk[x].load_k(kv, r[x]), k.scales[x] = load_scales(kv.ks, r[x]);
+      for (int x = 0; x < NB; ++x) k.blk[x].load_k(kv, r[x]), k.scales[x] = load_scales(kv.ks, r[x]);
     };
     auto step = [&](int i, Keys& now, Keys& next) {
-      u2 vss[4];
+      u2 vss[NB];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) now.blk[x].load_v(kv, rows_now[x]), vss[x] = load_scales(kv.vs, rows_now[x]);
+      for (int x = 0; x < NB; ++x) now.blk[x].load_v(kv, rows_now[x]), vss[x] = load_scales(kv.vs, rows_now[x]);
       if constexpr (kAhead) {
         find_rows(i + 4, rows_next);
         load_keys(rows_next, next);
@@ -228,11 +232,11 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
       }
       pages(i + 8);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) rows_now[x] = rows_next[x];
+      for (int x = 0; x < NB; ++x) rows_now[x] = rows_next[x];
       __builtin_amdgcn_sched_barrier(0);  // what has been asked for stays ahead
-      f4 s[RT][4], ks[4], vs[4];
+      f4 s[RT][NB], ks[NB], vs[NB];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
+      for (int x = 0; x < NB; ++x) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) s[t][x] = f4{0, 0, 0, 0};
 #pragma unroll
@@ -244,21 +248,21 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
         ks[x] = widen_scales(now.scales[x]);
         vs[x] = widen_scales(vss[x]);
       }
-      const int t0 = i * kKvTile;
+      const int t0 = i * kStep;
       int left[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) left[t] = limit[t] - t0;
-      h8 p[RT][2], pl[RT][2];
-      rows.soften(s, ks, vs, t0 + kKvTile > least, left, n - t0, p, pl);
+      h8 p[RT][NB / 2], pl[RT][NB / 2];
+      rows.template soften<NB>(s, ks, vs, t0 + kStep > least, left, n - t0, p, pl);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < NB / 2; ++h)
 #pragma unroll
         for (int w = 0; w < Rows::kOut / 4; ++w) {
           h2 f[4][4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) now.blk[2 * h + x / 2].v_pairs(w, x % 2, f[x]);
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) rows.add(4 * w + jj, join(f[0][jj], f[1][jj], f[2][jj], f[3][jj]), p, pl, h);
+          for (int jj = 0; jj < 4; ++jj) rows.template add<NB / 2>(4 * w + jj, join(f[0][jj], f[1][jj], f[2][jj], f[3][jj]), p, pl, h);
         }
     };
     if (step0 < step_end) {
@@ -272,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
         step(i, now, next);
         if constexpr (kAhead) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < NB; ++x) {
 #pragma unroll
             for (int w = 0; w < KvBlock<BITS, D>::kK; ++w) now.blk[x].k[w] = next.blk[x].k[w];
             now.scales[x] = next.scales[x];
@@ -427,11 +431,11 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) left[t] = n - step * kKvTile;
     h8 p[RT][2], pl[RT][2];
-    rows.soften(s, ks, vs, left[0] < kKvTile, left, left[0], p, pl);
+    rows.template soften<4>(s, ks, vs, left[0] < kKvTile, left, left[0], p, pl);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < kOut; ++j) rows.add(j, lds_v[at][h][j][lane], p, pl, h);
+      for (int j = 0; j < kOut; ++j) rows.template add<2>(j, lds_v[at][h][j][lane], p, pl, h);
     if constexpr (kBuffers == 1) __syncthreads();
   }
   __syncthreads();  // lds_bad has been cleared; a page outside the cache is every row's

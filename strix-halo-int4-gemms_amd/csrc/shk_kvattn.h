@@ -21,7 +21,7 @@
 // A row's probabilities are taken relative to
 //   m = max(score) + exponent(max(v_scale)) - 13,
 // in powers of two and over what the row has met so far, not to the largest
-// score: 2^(score - m) * v_scale is then at most 2^14, so f16 does not
+// score: 2^(score - m) * v_scale is then at most 2^15, so f16 does not
 // overflow and keeps all its bits down to 2^-27 of the largest term, whatever
 // the scales are (an exponent below -80 counts as -80, so that the sum cannot
 // overflow either).  For f16 outputs the term is split into two f16 terms,
@@ -75,14 +75,29 @@ __device__ __forceinline__ f4 mfma_f16(h8 a, h8 b, f4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Largest / sum over the four lane groups (lanes c, c + 16, c + 32, c + 48).
+// Combines the four lane groups (lanes c, c + 16, c + 32, c + 48).  A register
+// swapped with itself gives the even rows of 16 lanes twice and the odd ones
+// twice (then the halves), at the speed of a VALU operation: a shuffle by way of
+// LDS is waited for three times a step.
+template <typename F>
+__device__ __forceinline__ uint32_t groups(uint32_t v, F f) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = f(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return f(b[0], b[1]);
+}
+__device__ __forceinline__ uint32_t groups_most(uint32_t v) {
+  return groups(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
 __device__ __forceinline__ float groups_max(float v) {
-  v = __builtin_fmaxf(v, __shfl_xor(v, 16, 64));
-  return __builtin_fmaxf(v, __shfl_xor(v, 32, 64));
+  return __uint_as_float(groups(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__builtin_fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
 }
 __device__ __forceinline__ float groups_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  return __uint_as_float(groups(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 
 struct KvView {  // one key head of the cache
@@ -205,8 +220,7 @@ struct KvRows {
           most = max(most, __float_as_uint(v[s][i]) & 0x7FFFFFFFu);
         }
       }
-      most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
-      most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+      most = groups_most(most);
       // the largest magnitude's exponent, within what both 2^e and 2^-e hold
       const int e = min(max((int)(most >> 23), 1), 253);
       const float inv = __builtin_copysignf(__uint_as_float((uint32_t)(254 - e) << 23), scale);
@@ -223,20 +237,24 @@ struct KvRows {
     big = 0;
   }
 
-  // Scores (before the row's factor) of 64 tokens and their scales to the
-  // second product's operands; o shrinks where a row's reference grew.
+  // Scores (before the row's factor) of 16 * NB tokens and their scales to the
+  // second product's operands; o shrinks where a row's reference grew.  It
+  // grows only past twice its value, which the 13 leaves room for: the shrink
+  // runs in few steps instead of nearly all.
   // limit[t]: the row's tokens end there, counted from the step's first;
   // `ends`: some row's do (uniform); held: the sequence's tokens end there.
-  __device__ __forceinline__ void soften(f4 (&s)[RT][4], const f4 (&ks)[4], f4 (&vs)[4], bool ends,
-                                         const int (&limit)[RT], int held, h8 (&p)[RT][2], h8 (&pl)[RT][2]) {
+  template <int NB>
+  __device__ __forceinline__ void soften(f4 (&s)[RT][NB], const f4 (&ks)[NB], f4 (&vs)[NB], bool ends,
+                                         const int (&limit)[RT], int held, h8 (&p)[RT][NB / 2],
+                                         h8 (&pl)[RT][NB / 2]) {
     const int g = (threadIdx.x & 63) / 16;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[t][i] *= ks[i];
+      for (int i = 0; i < NB; ++i) s[t][i] *= ks[i];
     if (ends) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int at = 16 * i + 4 * g + r;
@@ -248,26 +266,26 @@ struct KvRows {
     }
     uint32_t most = big;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(vs[i][r]));
-    most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
-    big = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+    big = groups_most(most);
     const float up = (float)(min(max((int)(big >> 23), 47), 254) - 127 - 13);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       float top = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = __builtin_fmaxf(top, s[t][i][r]);
-      top = __builtin_fmaxf(m[t], groups_max(top) * qs[t] + up);
+      top = groups_max(top) * qs[t] + up;
+      top = top > m[t] + 1.0f ? top : m[t];
       const float base = top == -__builtin_inff() ? 0.0f : top;
       const float alpha = __builtin_amdgcn_exp2f(m[t] - base);
       m[t] = top;
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i][r], qs[t], -base));
@@ -286,7 +304,8 @@ struct KvRows {
   }
 
   // o^T += V^T P^T for 32 tokens and 16 values of head_dim.
-  __device__ __forceinline__ void add(int j, const h8& v, const h8 (&p)[RT][2], const h8 (&pl)[RT][2], int h) {
+  template <int NH>
+  __device__ __forceinline__ void add(int j, const h8& v, const h8 (&p)[RT][NH], const h8 (&pl)[RT][NH], int h) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       o[t][j] = mfma_f16(v, p[t][h], o[t][j]);
