@@ -20,8 +20,8 @@ nothing back to the host; there is no CPU path.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import Any
 
@@ -29,26 +29,14 @@ from . import kernel_table as kt
 from .native import _check, _device_index, _require_device, _stream_handle, _torch, _verified_library
 
 HEAD_DIMS = (64, 128, 256)
-_I64, _P = ctypes.c_int64, ctypes.c_void_p
 
 
-class _Cache(ctypes.Structure):
-    _fields_ = [("key_codes", _P), ("value_codes", _P), ("key_scales", _P), ("value_scales", _P), ("pages", _I64),
-                ("kv_heads", _I64), ("page_size", _I64), ("head_dim", _I64), ("bits", _I64)]
-
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("keys", _P), ("values", _P), ("key_token_stride", _I64), ("key_head_stride", _I64),
-                ("value_token_stride", _I64), ("value_head_stride", _I64), ("type", _I64), ("slots", _P),
-                ("slot_bytes", _I64), ("tokens", _I64)]
-
-
-class _Attention(ctypes.Structure):
-    _fields_ = [("q", _P), ("q_batch_stride", _I64), ("q_query_stride", _I64), ("q_head_stride", _I64),
-                ("type", _I64), ("batch", _I64), ("queries", _I64), ("heads", _I64), ("page_table", _P),
-                ("table_stride", _I64), ("table_pages", _I64), ("lengths", _P), ("prefix_pages", _P),
-                ("prefix_length", _I64), ("scale", ctypes.c_double), ("out", _P), ("lse", _P), ("workspace", _P),
-                ("workspace_bytes", _I64)]
+# The structs of include/strix_halo_gfx950.h, field by field; every field is 8
+# bytes (pointers and int64 alike, one double), so packing them is a tenth of
+# the time that filling ctypes.Structure takes.
+_CACHE = struct.Struct("=9q")
+_ROWS = struct.Struct("=10q")
+_ATTENTION = struct.Struct("=14qd4q")
 
 
 @dataclass(frozen=True, eq=False)
@@ -98,11 +86,10 @@ class KVCache:
             raise ValueError(f"page_size must be a power of two from 16 to 1024; got {page_size}")
         if not 1 <= heads <= 65535 or pages < 1:
             raise ValueError(f"the cache needs at least one page and 1 to 65535 heads; got {pages} and {heads}")
-        native = _Cache(codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(),
-                        self.value_scales.data_ptr(), pages, heads, page_size, head_dim, bits)
+        native = _CACHE.pack(codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(),
+                             self.value_scales.data_ptr(), pages, heads, page_size, head_dim, bits)
         for name, value in (("pages", pages), ("kv_heads", heads), ("page_size", page_size), ("head_dim", head_dim),
-                            ("bits", bits), ("device", codes.device), ("_native", native),
-                            ("_ref", ctypes.addressof(native))):
+                            ("bits", bits), ("device", codes.device), ("_native", native), ("_workspaces", {})):
             object.__setattr__(self, name, value)
 
 
@@ -132,7 +119,7 @@ def _row_type(torch: Any, name: str, dtype: Any) -> int:
 
 
 def _check_slots(torch: Any, slots: Any, tokens: int | None) -> None:
-    if slots.dtype not in (torch.int64, torch.int32):
+    if slots.dtype != torch.int64 and slots.dtype != torch.int32:
         raise ValueError(f"slots must have dtype torch.int64 or torch.int32; got {slots.dtype}")
     if slots.ndim != 1 or (tokens is not None and slots.shape[0] != tokens):
         want = "(tokens,)" if tokens is None else f"({tokens},)"
@@ -141,10 +128,21 @@ def _check_slots(torch: Any, slots: Any, tokens: int | None) -> None:
         raise ValueError("slots must be contiguous")
 
 
-def _rows(keys: Any, values: Any, slots: Any, kind: int, tokens: int) -> _Rows:
+def _rows(keys: Any, values: Any, slots: Any, kind: int, tokens: int) -> bytes:
     ks, vs = keys.stride(), values.stride()
-    return _Rows(keys.data_ptr(), values.data_ptr(), ks[0], ks[1], vs[0], vs[1], kind, slots.data_ptr(),
-                 slots.element_size(), tokens)
+    return _ROWS.pack(keys.data_ptr(), values.data_ptr(), ks[0], ks[1], vs[0], vs[1], kind, slots.data_ptr(),
+                      slots.element_size(), tokens)
+
+
+def _check_devices(cache: KVCache, **tensors: Any) -> None:
+    index = cache.key_codes.get_device()
+    for t in tensors.values():
+        if t is not None and t.get_device() != index:
+            break
+    else:
+        if index >= 0:
+            return
+    _require_device(_torch(), {"cache": cache.key_codes, **tensors})  # says what is wrong
 
 
 def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream: Any | None = None) -> None:
@@ -156,14 +154,14 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
     others are distinct.  One pass over memory, no copy of the inputs.
     """
     torch = _torch()
-    _require_device(torch, {"cache": cache.key_codes, "keys": keys, "values": values, "slots": slots})
+    _check_devices(cache, keys=keys, values=values, slots=slots)
     kind = _row_type(torch, "keys", keys.dtype)
     if values.dtype != keys.dtype:
         raise ValueError(f"values must have the dtype of keys, {keys.dtype}; got {values.dtype}")
     tokens = int(keys.shape[0]) if keys.ndim else 0
     shape = (tokens, cache.kv_heads, cache.head_dim)
     for name, t in (("keys", keys), ("values", values)):
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} must have shape {shape} == (tokens, kv_heads, head_dim); got {tuple(t.shape)}")
         if t.stride(2) != 1:
             raise ValueError(f"{name} must be contiguous along head_dim")
@@ -172,8 +170,7 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
         return
     lib = _verified_library()
     _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, stream),
-                                                    cache._ref,
-                                                    ctypes.byref(_rows(keys, values, slots, kind, tokens))))
+                                                    cache._native, _rows(keys, values, slots, kind, tokens)))
 
 
 def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any | None = None) -> tuple[Any, Any]:
@@ -181,17 +178,18 @@ def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any 
     (bf16, the default, f16 or f32): two [tokens, kv_heads, head_dim]
     tensors.  Slots outside the cache give NaN."""
     torch = _torch()
-    _require_device(torch, {"cache": cache.key_codes, "slots": slots})
+    _check_devices(cache, slots=slots)
     dtype = torch.bfloat16 if dtype is None else dtype
     kind = _row_type(torch, "the result", dtype)
     _check_slots(torch, slots, None)
     tokens = int(slots.shape[0])
-    keys, values = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    shape = (tokens, cache.kv_heads, cache.head_dim)
+    keys = torch.empty(shape, dtype=dtype, device=cache.device)
+    values = torch.empty_like(keys)
     if tokens:
         lib = _verified_library()
         _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, stream),
-                                                       cache._ref,
-                                                    ctypes.byref(_rows(keys, values, slots, kind, tokens))))
+                                                       cache._native, _rows(keys, values, slots, kind, tokens)))
     return keys, values
 
 
@@ -230,9 +228,8 @@ def kv_cache_attention(
     softmax and the sums are f32; products take the codes as they are.
     """
     torch = _torch()
-    _require_device(torch, {"cache": cache.key_codes, "q": q, "page_table": page_table, "lengths": lengths,
-                            "prefix_pages": prefix_pages, "out": out})
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    _check_devices(cache, q=q, page_table=page_table, lengths=lengths, prefix_pages=prefix_pages, out=out)
+    if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
         raise ValueError(f"q must have dtype torch.bfloat16 or torch.float16; got {q.dtype}")
     if q.ndim not in (3, 4) or q.shape[-1] != cache.head_dim:
         raise ValueError(f"q must have shape (batch, heads, {cache.head_dim}) or (batch, queries, heads, "
@@ -251,7 +248,7 @@ def kv_cache_attention(
         raise ValueError(f"page_table must have shape ({batch}, pages); got {tuple(page_table.shape)}")
     if page_table.stride(1) != 1 and page_table.shape[1] > 1:
         raise ValueError("rows of page_table must be contiguous")
-    if tuple(lengths.shape) != (batch,) or not lengths.is_contiguous():
+    if lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError(f"lengths must be contiguous with shape ({batch},); got {tuple(lengths.shape)}")
     if isinstance(prefix_length, bool) or not isinstance(prefix_length, int) or prefix_length < 0:
         raise ValueError(f"prefix_length must be a non-negative int; got {prefix_length!r}")
@@ -268,11 +265,11 @@ def kv_cache_attention(
     if not math.isfinite(scale):
         raise ValueError(f"softmax_scale must be finite; got {softmax_scale}")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"out must be contiguous with shape {tuple(shape)} and dtype {q.dtype}; got "
                          f"{tuple(out.shape)} and {out.dtype}")
-    lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty(shape[:-1], dtype=torch.float32) if return_lse else None
     if batch * queries:
         strides = q.stride()
         sb, sq, sh = (strides[0], strides[1], strides[2]) if q.ndim == 4 else (strides[0], 0, strides[1])
@@ -282,19 +279,30 @@ def kv_cache_attention(
                 q = q.clone(memory_format=torch.contiguous_format)
             sb, sq, sh = queries * heads * cache.head_dim, heads * cache.head_dim, cache.head_dim
         kind = kt.SRC_BF16 if q.dtype == torch.bfloat16 else kt.SRC_F16
-        args = _Attention(q.data_ptr(), sb, sq, sh, kind, batch, queries, heads, page_table.data_ptr(),
-                          page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-                          prefix_pages.data_ptr() if prefix_length else None, prefix_length, scale, out.data_ptr(),
-                          lse.data_ptr() if return_lse else None, None, 0)
+        table_pages = page_table.shape[1]
+
+        def args(work: Any, nbytes: int) -> bytes:
+            return _ATTENTION.pack(q.data_ptr(), sb, sq, sh, kind, batch, queries, heads, page_table.data_ptr(),
+                                   page_table.stride(0), table_pages, lengths.data_ptr(),
+                                   prefix_pages.data_ptr() if prefix_length else 0, prefix_length, scale,
+                                   out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                                   work.data_ptr() if nbytes else 0, nbytes)
+
         lib = _verified_library()
-        nbytes = lib.amd_strix_halo_kernels_kv_attention_workspace(cache._ref, ctypes.byref(args))
-        if nbytes < 0:
-            _check(lib, 1)
+        # the workspace's size is a function of the sizes alone
+        key = (batch, queries, heads, table_pages, prefix_length)
+        nbytes = cache._workspaces.get(key)
+        if nbytes is None:
+            nbytes = lib.amd_strix_halo_kernels_kv_attention_workspace(cache._native, args(None, 0))
+            if nbytes < 0:
+                _check(lib, 1)
+            if len(cache._workspaces) < 4096:
+                cache._workspaces[key] = nbytes
+        work = None
         if nbytes:
-            work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            work = q.new_empty(nbytes, dtype=torch.uint8)
             if stream is not None:
                 work.record_stream(stream)
-            args.workspace, args.workspace_bytes = work.data_ptr(), nbytes
         _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, stream),
-                                                            cache._ref, ctypes.byref(args)))
+                                                            cache._native, args(work, nbytes)))
     return (out, lse) if return_lse else out

@@ -9,7 +9,7 @@ gather, up and gate products, SwiGLU, down product, weighted sum.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Any
 
 from . import kernel_table as kt
@@ -19,18 +19,14 @@ from .native import _check, _device_index, _require_device, _stream_handle, _tor
 MOE_MAX_TOKENS = 64
 MOE_MAX_PAIRS = 1024
 MOE_MAX_EXPERTS = 1024
-_I64, _P = ctypes.c_int64, ctypes.c_void_p
 
 
-class _Moe(ctypes.Structure):
-    _fields_ = [("x", _P), ("x_stride", _I64), ("type", _I64), ("tokens", _I64), ("hidden", _I64), ("inner", _I64),
-                ("experts", _I64), ("top", _I64), ("up_gate", _P), ("up_gate_scale", _P), ("down", _P),
-                ("down_scale", _P), ("group", _I64), ("layout", _I64), ("ids", _P), ("id_bytes", _I64), ("share", _P),
-                ("out", _P), ("workspace", _P), ("workspace_bytes", _I64)]
+# shk_moe of include/strix_halo_gfx950.h: every field is 8 bytes
+_MOE = struct.Struct("=20q")
 
 
 def _require(name: str, tensor: Any, shape: tuple[int, ...], dtype: Any, what: str) -> None:
-    if tuple(tensor.shape) != shape:
+    if tensor.shape != shape:
         raise ValueError(f"{name} must have shape {shape} == {what}; got {tuple(tensor.shape)}")
     if tensor.dtype != dtype:
         raise ValueError(f"{name} must have dtype {dtype}; got {tensor.dtype}")
@@ -77,10 +73,13 @@ def moe_swiglu_int4(
     if layout not in (GemmLayout.NN, GemmLayout.NT):
         raise ValueError(f"unsupported MoE layout {layout.value}; supported layouts are nn, nt")
     torch = _torch()
-    _require_device(torch, {"x": x, "up_gate": up_gate, "down": down, "expert_ids": expert_ids,
-                            "expert_weights": expert_weights, "up_gate_scale": up_gate_scale,
-                            "down_scale": down_scale, "out": out})
-    if x.dtype not in (torch.bfloat16, torch.float16):
+    index = x.get_device()
+    for t in (up_gate, down, expert_ids, expert_weights, up_gate_scale, down_scale, x if out is None else out):
+        if index < 0 or t.get_device() != index:
+            _require_device(torch, {"x": x, "up_gate": up_gate, "down": down, "expert_ids": expert_ids,
+                                    "expert_weights": expert_weights, "up_gate_scale": up_gate_scale,
+                                    "down_scale": down_scale, "out": out})  # says what is wrong
+    if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
         raise ValueError(f"x must have dtype torch.bfloat16 or torch.float16; got {x.dtype}")
     if x.ndim != 2 or x.shape[1] < 1:
         raise ValueError(f"x must have shape (tokens, hidden); got {tuple(x.shape)}")
@@ -113,7 +112,7 @@ def moe_swiglu_int4(
     if expert_ids.ndim != 2 or expert_ids.shape[0] != tokens:
         raise ValueError(f"expert_ids must have shape ({tokens}, top); got {tuple(expert_ids.shape)}")
     top = int(expert_ids.shape[1])
-    if expert_ids.dtype not in (torch.int64, torch.int32):
+    if expert_ids.dtype != torch.int64 and expert_ids.dtype != torch.int32:
         raise ValueError(f"expert_ids must have dtype torch.int64 or torch.int32; got {expert_ids.dtype}")
     _require("expert_weights", expert_weights, (tokens, top), torch.float32, "(tokens, top)")
     if not expert_ids.is_contiguous():
@@ -124,23 +123,21 @@ def moe_swiglu_int4(
     if experts > MOE_MAX_EXPERTS:
         raise ValueError(f"moe_swiglu_int4 takes up to {MOE_MAX_EXPERTS} experts; got {experts}")
     if out is None:
-        out = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
         _require("out", out, (tokens, hidden), x.dtype, "(tokens, hidden)")
     if tokens == 0:
         return out
-    args = _Moe(x.data_ptr(), x.stride(0), kt.SRC_BF16 if x.dtype == torch.bfloat16 else kt.SRC_F16, tokens, hidden,
-                inner, experts, top, up_gate.data_ptr(), up_gate_scale.data_ptr(), down.data_ptr(),
-                down_scale.data_ptr(), group, kt.LAYOUT_NT if nt else kt.LAYOUT_NN, expert_ids.data_ptr(),
-                expert_ids.element_size(), expert_weights.data_ptr(), out.data_ptr(), None, 0)
+    # h as two bf16 terms with rows of whole 128s, and f32 results, for each pair
+    nbytes = 4 * tokens * top * (-(-inner // 128) * 128 + hidden)
+    work = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    if stream is not None and nbytes:
+        work.record_stream(stream)
+    args = _MOE.pack(x.data_ptr(), x.stride(0), kt.SRC_BF16 if x.dtype == torch.bfloat16 else kt.SRC_F16, tokens,
+                     hidden, inner, experts, top, up_gate.data_ptr(), up_gate_scale.data_ptr(), down.data_ptr(),
+                     down_scale.data_ptr(), group, kt.LAYOUT_NT if nt else kt.LAYOUT_NN, expert_ids.data_ptr(),
+                     expert_ids.element_size(), expert_weights.data_ptr(), out.data_ptr(),
+                     work.data_ptr() if nbytes else 0, nbytes)
     lib = _verified_library()
-    nbytes = lib.amd_strix_halo_kernels_moe_workspace(ctypes.byref(args))
-    if nbytes < 0:
-        _check(lib, 1)
-    if nbytes:
-        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        if stream is not None:
-            work.record_stream(stream)
-        args.workspace, args.workspace_bytes = work.data_ptr(), nbytes
-    _check(lib, lib.amd_strix_halo_kernels_moe(_device_index(x), _stream_handle(torch, x, stream), ctypes.byref(args)))
+    _check(lib, lib.amd_strix_halo_kernels_moe(index, _stream_handle(torch, x, stream), args))
     return out

@@ -3,8 +3,6 @@ Python argument checks, and the C ABI's own before it touches the device."""
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -76,13 +74,13 @@ def lib():
 def _native_cache(**kw):
     f = {"key_codes": FAKE, "value_codes": FAKE, "key_scales": FAKE, "value_scales": FAKE, "pages": 4, "kv_heads": 2,
          "page_size": 16, "head_dim": 64, "bits": 4} | kw
-    return kv_cache._Cache(**f)
+    return kv_cache._CACHE.pack(*(v or 0 for v in f.values()))
 
 
 def _native_rows(**kw):
     f = {"keys": FAKE, "values": FAKE, "key_token_stride": 128, "key_head_stride": 64, "value_token_stride": 128,
          "value_head_stride": 64, "type": kt.SRC_BF16, "slots": FAKE, "slot_bytes": 8, "tokens": 3} | kw
-    return kv_cache._Rows(**f)
+    return kv_cache._ROWS.pack(*(v or 0 for v in f.values()))
 
 
 def _native_attention(**kw):
@@ -90,7 +88,7 @@ def _native_attention(**kw):
          "queries": 1, "heads": 4, "page_table": FAKE, "table_stride": 4, "table_pages": 4, "lengths": FAKE,
          "prefix_pages": None, "prefix_length": 0, "scale": 0.125, "out": FAKE, "lse": None, "workspace": None,
          "workspace_bytes": 0} | kw
-    return kv_cache._Attention(**f)
+    return kv_cache._ATTENTION.pack(*(v or 0 for v in f.values()))
 
 
 CACHE_FAULTS = [({"bits": 5}, "bits must be 4 or 8"), ({"head_dim": 80}, "head_dim must be"),
@@ -102,14 +100,14 @@ CACHE_FAULTS = [({"bits": 5}, "bits must be 4 or 8"), ({"head_dim": 80}, "head_d
 @pytest.mark.parametrize("kw,match", CACHE_FAULTS)
 def test_c_abi_refuses_caches(lib, kw, match):
     cache = _native_cache(**kw)
-    for call in (lambda: lib.amd_strix_halo_kernels_kv_write(0, 0, ctypes.byref(cache), ctypes.byref(_native_rows())),
-                 lambda: lib.amd_strix_halo_kernels_kv_read(0, 0, ctypes.byref(cache), ctypes.byref(_native_rows())),
-                 lambda: lib.amd_strix_halo_kernels_kv_attention(0, 0, ctypes.byref(cache),
-                                                                 ctypes.byref(_native_attention()))):
+    for call in (lambda: lib.amd_strix_halo_kernels_kv_write(0, 0, cache, _native_rows()),
+                 lambda: lib.amd_strix_halo_kernels_kv_read(0, 0, cache, _native_rows()),
+                 lambda: lib.amd_strix_halo_kernels_kv_attention(0, 0, cache,
+                                                                 _native_attention())):
         assert call() == 1
         assert match in lib.amd_strix_halo_kernels_last_error().decode()
     args = _native_attention()
-    assert lib.amd_strix_halo_kernels_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(args)) == -1
+    assert lib.amd_strix_halo_kernels_kv_attention_workspace(cache, args) == -1
 
 
 @pytest.mark.parametrize("kw,match", [({"type": kt.SRC_I8}, "row type"), ({"slot_bytes": 2}, "int32 or int64"),
@@ -117,7 +115,7 @@ def test_c_abi_refuses_caches(lib, kw, match):
                                       ({"slots": None}, "non-null")])
 def test_c_abi_refuses_rows(lib, kw, match):
     cache, rows = _native_cache(), _native_rows(**kw)
-    assert lib.amd_strix_halo_kernels_kv_write(0, 0, ctypes.byref(cache), ctypes.byref(rows)) == 1
+    assert lib.amd_strix_halo_kernels_kv_write(0, 0, cache, rows) == 1
     assert match in lib.amd_strix_halo_kernels_last_error().decode()
 
 
@@ -132,15 +130,15 @@ def test_c_abi_refuses_rows(lib, kw, match):
 ])
 def test_c_abi_refuses_attention(lib, kw, match):
     args = _native_attention(**kw)
-    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, ctypes.byref(_native_cache()), ctypes.byref(args)) == 1
+    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, _native_cache(), args) == 1
     assert match in lib.amd_strix_halo_kernels_last_error().decode()
 
 
 def test_c_abi_null_structs_and_empty_calls(lib):
     cache, rows, args = _native_cache(), _native_rows(tokens=0), _native_attention(batch=0)
-    assert lib.amd_strix_halo_kernels_kv_write(0, 0, None, ctypes.byref(rows)) == 1
-    assert lib.amd_strix_halo_kernels_kv_read(0, 0, ctypes.byref(cache), None) == 1
-    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, ctypes.byref(cache), None) == 1
-    assert lib.amd_strix_halo_kernels_kv_write(0, 0, ctypes.byref(cache), ctypes.byref(rows)) == 0
-    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, ctypes.byref(cache), ctypes.byref(args)) == 0
-    assert lib.amd_strix_halo_kernels_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(args)) == 0
+    assert lib.amd_strix_halo_kernels_kv_write(0, 0, None, rows) == 1
+    assert lib.amd_strix_halo_kernels_kv_read(0, 0, cache, None) == 1
+    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, cache, None) == 1
+    assert lib.amd_strix_halo_kernels_kv_write(0, 0, cache, rows) == 0
+    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, cache, args) == 0
+    assert lib.amd_strix_halo_kernels_kv_attention_workspace(cache, args) == 0

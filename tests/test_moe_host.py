@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -39,7 +37,7 @@ def _args(**kw):
     f = {"x": FAKE, "x_stride": 64, "type": kt.SRC_BF16, "tokens": 2, "hidden": 64, "inner": 32, "experts": 4, "top": 2,
          "up_gate": FAKE, "up_gate_scale": FAKE, "down": FAKE, "down_scale": FAKE, "group": 0, "layout": kt.LAYOUT_NN,
          "ids": FAKE, "id_bytes": 8, "share": FAKE, "out": FAKE, "workspace": FAKE, "workspace_bytes": 1 << 20} | kw
-    return moe._Moe(**f)
+    return moe._MOE.pack(*(v or 0 for v in f.values()))
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -49,16 +47,16 @@ def _args(**kw):
     ({"hidden": 0}, "hidden and inner"), ({"inner": 2**21}, "hidden and inner"), ({"id_bytes": 2}, "int32 or int64"),
     ({"x": None}, "non-null"), ({"down_scale": None}, "non-null"), ({"ids": None}, "non-null"),
     ({"share": FAKE + 2}, "aligned to their elements"), ({"x": FAKE + 1}, "aligned to their elements"),
-    ({"workspace": None}, "workspace must hold"), ({"workspace_bytes": 1535}, "workspace must hold 1536 bytes"),
+    ({"workspace": None}, "workspace must hold"), ({"workspace_bytes": 3071}, "workspace must hold 3072 bytes"),
     ({"workspace": FAKE + 4}, "aligned to 16"),
 ])
 def test_c_abi_refusals(lib, kw, match):
-    assert lib.amd_strix_halo_kernels_moe(0, 0, ctypes.byref(_args(**kw))) == 1
+    assert lib.amd_strix_halo_kernels_moe(0, 0, _args(**kw)) == 1
     assert match in lib.amd_strix_halo_kernels_last_error().decode()
 
 
 def test_c_abi_null_struct_and_no_tokens(lib):
     assert lib.amd_strix_halo_kernels_moe(0, 0, None) == 1
     assert lib.amd_strix_halo_kernels_moe_workspace(None) == -1
-    assert lib.amd_strix_halo_kernels_moe(0, 0, ctypes.byref(_args(tokens=0))) == 0
-    assert lib.amd_strix_halo_kernels_moe_workspace(ctypes.byref(_args())) == 1536
+    assert lib.amd_strix_halo_kernels_moe(0, 0, _args(tokens=0)) == 0
+    assert lib.amd_strix_halo_kernels_moe_workspace(_args()) == 3072
