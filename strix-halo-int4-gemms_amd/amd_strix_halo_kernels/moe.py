@@ -128,16 +128,17 @@ def moe_swiglu_int4(
         _require("out", out, (tokens, hidden), x.dtype, "(tokens, hidden)")
     if tokens == 0:
         return out
-    # h as two bf16 terms with rows of whole 128s, and f32 results, for each pair
-    nbytes = 4 * tokens * top * (-(-inner // 128) * 128 + hidden)
-    work = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    if stream is not None and nbytes:
+    # h as two bf16 terms with rows of whole 128s, and f32 results, for each
+    # pair; a counter for each 128 columns of the output
+    nbytes = 4 * (tokens * top * (-(-inner // 128) * 128 + hidden) + -(-hidden // 128))
+    work = x.new_empty(nbytes, dtype=torch.uint8)
+    if stream is not None:
         work.record_stream(stream)
     args = _MOE.pack(x.data_ptr(), x.stride(0), kt.SRC_BF16 if x.dtype == torch.bfloat16 else kt.SRC_F16, tokens,
                      hidden, inner, experts, top, up_gate.data_ptr(), up_gate_scale.data_ptr(), down.data_ptr(),
                      down_scale.data_ptr(), group, kt.LAYOUT_NT if nt else kt.LAYOUT_NN, expert_ids.data_ptr(),
                      expert_ids.element_size(), expert_weights.data_ptr(), out.data_ptr(),
-                     work.data_ptr() if nbytes else 0, nbytes)
+                     work.data_ptr(), nbytes)
     lib = _verified_library()
     _check(lib, lib.amd_strix_halo_kernels_moe(index, _stream_handle(torch, x, stream), args))
     return out

@@ -56,11 +56,13 @@ struct MoeArgs {
   const float* share;
   uint16_t* h;             // [pairs][high, low][inner_pad]: bf16 terms, eights in the order of expand
   float* part;             // [pairs][hidden]
+  int* arrived;            // a counter for each tile of the down product
   void* out;
   int k, k_packed, cols;   // this product's K, its bytes, and columns (of up alone)
   int group, groups;       // scale group (0: per channel) and groups of K
-  int tokens, top, experts, hidden, inner, inner_pad;
+  int tokens, top, experts, hidden, inner, inner_pad, tiles;
   int type, id8;
+  int joined;              // the down product adds up the pairs itself
 };
 
 __device__ __forceinline__ int id_of(const MoeArgs& a, int p) {
@@ -523,10 +525,36 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
 #pragma unroll
         for (int q = 0; q < kWaves / 2; ++q) v2 += red[q * 16 * kPitch + r * kPitch + n];
         if constexpr (!GROUPED) v2 *= load_bf16(scale + col);
-        a.part[(long)list[row0 + 16 * t + r] * a.hidden + col] = v2;
+        __hip_atomic_store(a.part + (long)list[row0 + 16 * t + r] * a.hidden + col, v2, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
+}
+
+// y[t, n] = sum_j share[t, j] * part[t, j][n], in the order of j.
+__device__ __forceinline__ void join_value(const MoeArgs& a, int t, int n) {
+  float y = 0.0f;
+  for (int j = 0; j < a.top; ++j) {
+    const int p = t * a.top + j;
+    if (id_of(a, p) >= 0)
+      y += a.share[p] * __hip_atomic_load(a.part + (long)p * a.hidden + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  const long at = (long)t * a.hidden + n;
+  if (a.type == SHK_SRC_BF16) static_cast<uint16_t*>(a.out)[at] = (uint16_t)f32_to_bf16_rne(y);
+  else static_cast<_Float16*>(a.out)[at] = (_Float16)y;
+}
+
+// The 128 columns from n0, by one workgroup.
+template <int kWaves>
+__device__ __forceinline__ void join_tile(const MoeArgs& a, int n0) {
+  for (int i = threadIdx.x; i < a.tokens * 2 * kHalf; i += 64 * kWaves)
+    if (n0 + i % (2 * kHalf) < a.hidden) join_value(a, i / (2 * kHalf), n0 + i % (2 * kHalf));
+}
+
+__global__ __launch_bounds__(256) void moe_join(const MoeArgs a) {
+  const long at = (long)blockIdx.x * 256 + threadIdx.x;
+  if (at < (long)a.tokens * a.hidden) join_value(a, (int)(at / a.hidden), (int)(at % a.hidden));
 }
 
 // One product of the layer.  FIRST: up and gate, h = up * silu(gate) to a.h,
@@ -553,26 +581,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   // Elsewhere that only narrows an XCD's addresses.
   constexpr bool kNeighbours = FIRST && LAYOUT == SHK_LAYOUT_NN;
   const int tile = kNeighbours ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+  if (FIRST && blockIdx.y == 0)  // the down product counts from zero
+    for (int i = blockIdx.x * 64 * kWaves + threadIdx.x; i < a.tiles; i += gridDim.x * 64 * kWaves) a.arrived[i] = 0;
   if (tile * kStep >= (FIRST ? a.inner_pad : a.cols)) return;
 
   // the blockIdx.y-th expert that is hit, and its pairs in order
-  int expert = -1, rank = blockIdx.y, rows = 0;
+  int expert = -1, rank = blockIdx.y, rows = 0, hits = 0;  // hits: experts that are hit
   if (pairs <= 64) {
     // experts in the order of their first pairs, all in a wave's registers
     const int mine = lane < pairs ? id_of(a, lane) : -1;
     unsigned long open = __ballot(mine >= 0), same = 0;
-    for (; open != 0; --rank) {
+    for (; open != 0; ++hits) {
       const int e = __shfl(mine, __builtin_ctzll(open), 64);
-      same = __ballot(mine == e);
-      if (rank == 0) {
-        expert = e;
-        break;
-      }
-      open &= ~same;
+      const unsigned long all = __ballot(mine == e);
+      if (hits == rank) expert = e, same = all;
+      open &= ~all;
     }
-    if (expert < 0) return;  // the same for all threads
     rows = __popcll(same);
-    if (wave == 0 && mine == expert) list[__popcll(same & ((1ul << lane) - 1))] = (uint16_t)lane;
+    if (wave == 0 && expert >= 0 && mine == expert) list[__popcll(same & ((1ul << lane) - 1))] = (uint16_t)lane;
   } else {
     // counted in LDS, those with more than 16 rows first: their workgroups
     // take longest
@@ -584,22 +610,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
       if (e >= 0) atomicAdd(&count[e], 1);
     }
     __syncthreads();
-    for (int many = 1; many >= 0 && expert < 0; --many) {
+    for (int many = 1; many >= 0; --many) {
       for (int e0 = 0; e0 < a.experts; e0 += 64) {
         const int n = e0 + lane < a.experts ? count[e0 + lane] : 0;
         unsigned long hit = __ballot(n > 0 && (n > 16) == (many != 0));
         const int here = __popcll(hit);
-        if (rank < here) {
-          for (int i = 0; i < rank; ++i) hit &= hit - 1;
+        if (rank >= hits && rank < hits + here) {
+          for (int i = hits; i < rank; ++i) hit &= hit - 1;
           expert = e0 + __builtin_ctzll(hit);
-          break;
         }
-        rank -= here;
+        hits += here;
       }
     }
-    if (expert < 0) return;
-    rows = count[expert];
-    if (wave == 0) {
+    rows = expert < 0 ? 0 : count[expert];
+    if (wave == 0 && expert >= 0) {
       int at = 0;
       for (int p0 = 0; p0 < pairs; p0 += 64) {
         const bool mine = p0 + lane < pairs && id[p0 + lane] == expert;
@@ -611,6 +635,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   }
   expert = __builtin_amdgcn_readfirstlane(expert);
   rows = __builtin_amdgcn_readfirstlane(rows);
+  hits = __builtin_amdgcn_readfirstlane(hits);
+  if constexpr (!FIRST)
+    if (a.joined && hits == 0 && blockIdx.y == 0) join_tile<kWaves>(a, tile * kStep);  // no token asks for any expert
+  if (expert < 0) return;  // the same for all threads
   __syncthreads();
 
   constexpr int kColumns = FIRST ? 2 : 1;
@@ -633,20 +661,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
       moe_rows<LAYOUT, FIRST, RT, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, row0, n0, k_first, k_last, red,
                                                         lds_scale + 256 * wave);
   }
-}
-
-// y[t] = sum_j share[t, j] * part[t, j], in the order of j.
-__global__ __launch_bounds__(256) void moe_join(const MoeArgs a) {
-  const long at = (long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (long)a.tokens * a.hidden) return;
-  const int t = (int)(at / a.hidden), n = (int)(at - (long)t * a.hidden);
-  float y = 0.0f;
-  for (int j = 0; j < a.top; ++j) {
-    const int p = t * a.top + j;
-    if (id_of(a, p) >= 0) y += a.share[p] * a.part[(long)p * a.hidden + n];
+  if (!FIRST && a.joined) {
+    // The last workgroup of a tile adds up its pairs.  Results are written and
+    // read with device scope, which the XCDs' caches see without being
+    // flushed; each workgroup's have arrived before it counts itself.
+    __shared__ int last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+      last = __hip_atomic_fetch_add(a.arrived + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == hits - 1;
+    __syncthreads();
+    if (last) join_tile<kWaves>(a, tile * kStep);
   }
-  if (a.type == SHK_SRC_BF16) static_cast<uint16_t*>(a.out)[at] = (uint16_t)f32_to_bf16_rne(y);
-  else static_cast<_Float16*>(a.out)[at] = (_Float16)y;
 }
 
 template <int LAYOUT, bool FIRST, int TYPE, int GROUPED>
@@ -671,16 +697,10 @@ hipError_t launch_product(const MoeArgs& a, unsigned columns, unsigned hit, hipS
   return hipGetLastError();
 }
 
-hipError_t launch_join(const MoeArgs& a, hipStream_t s) {
-  const long values = (long)a.tokens * a.hidden;
-  hipLaunchKernelGGL(moe_join, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, s, a);
-  return hipGetLastError();
-}
-
 template <int LAYOUT>
 hipError_t launch_layout(const shk_moe& x, MoeArgs a, hipStream_t s) {
-  const unsigned hit = (unsigned)std::min(x.tokens * x.top, x.experts);
-  if (hit == 0) return launch_join(a, s);
+  // with no pairs the down product still writes the zeros
+  const unsigned hit = (unsigned)std::max(1L, (long)std::min(x.tokens * x.top, x.experts));
   a.w = static_cast<const uint8_t*>(x.up_gate);
   a.scale = static_cast<const uint16_t*>(x.up_gate_scale);
   a.k = a.hidden, a.k_packed = (a.hidden + 1) / 2, a.cols = a.inner;
@@ -694,7 +714,10 @@ hipError_t launch_layout(const shk_moe& x, MoeArgs a, hipStream_t s) {
   a.k = a.inner, a.k_packed = (a.inner + 1) / 2, a.cols = a.hidden;
   a.groups = a.group ? (a.k + a.group - 1) / a.group : 1;
   err = launch_product<LAYOUT, false, SHK_SRC_BF16>(a, (unsigned)a.cols, hit, s);
-  return err != hipSuccess ? err : launch_join(a, s);
+  if (err != hipSuccess || a.joined) return err;
+  const long values = (long)a.tokens * a.hidden;
+  hipLaunchKernelGGL(moe_join, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -702,7 +725,11 @@ hipError_t launch_layout(const shk_moe& x, MoeArgs a, hipStream_t s) {
 // h's rows are whole pieces of 128 K values, the rest zero.
 static long inner_pad(const shk_moe& a) { return (a.inner + kSuper - 1) / kSuper * kSuper; }
 
-int64_t moe_workspace(const shk_moe& a) { return a.tokens * a.top * (inner_pad(a) + a.hidden) * 4; }
+static long down_tiles(const shk_moe& a) { return (a.hidden + 2 * kHalf - 1) / (2 * kHalf); }
+
+int64_t moe_workspace(const shk_moe& a) {
+  return a.tokens * a.top * (inner_pad(a) + a.hidden) * 4 + down_tiles(a) * 4;
+}
 
 hipError_t launch_moe(const shk_moe& x, hipStream_t s) {
   MoeArgs a{};
@@ -711,11 +738,17 @@ hipError_t launch_moe(const shk_moe& x, hipStream_t s) {
   a.share = x.share;
   a.h = static_cast<uint16_t*>(x.workspace);
   a.part = static_cast<float*>(x.workspace) + x.tokens * x.top * inner_pad(x);
+  a.arrived = reinterpret_cast<int*>(a.part + x.tokens * x.top * x.hidden);
+  a.tiles = (int)down_tiles(x);
   a.out = x.out;
   a.group = (int)x.group;
   a.tokens = (int)x.tokens, a.top = (int)x.top, a.experts = (int)x.experts;
   a.hidden = (int)x.hidden, a.inner = (int)x.inner, a.inner_pad = (int)inner_pad(x);
   a.type = (int)x.type;
+  // One workgroup a tile adds few pairs sooner than another launch starts; with
+  // many it would keep all others waiting (96 pairs: 29 us of the down product
+  // became 50, where the launch is 4).
+  a.joined = x.tokens * x.top <= 16;
   return x.layout == SHK_LAYOUT_NT ? launch_layout<SHK_LAYOUT_NT>(x, a, s) : launch_layout<SHK_LAYOUT_NN>(x, a, s);
 }
 

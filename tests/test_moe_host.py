@@ -47,7 +47,7 @@ def _args(**kw):
     ({"hidden": 0}, "hidden and inner"), ({"inner": 2**21}, "hidden and inner"), ({"id_bytes": 2}, "int32 or int64"),
     ({"x": None}, "non-null"), ({"down_scale": None}, "non-null"), ({"ids": None}, "non-null"),
     ({"share": FAKE + 2}, "aligned to their elements"), ({"x": FAKE + 1}, "aligned to their elements"),
-    ({"workspace": None}, "workspace must hold"), ({"workspace_bytes": 3071}, "workspace must hold 3072 bytes"),
+    ({"workspace": None}, "workspace must hold"), ({"workspace_bytes": 3075}, "workspace must hold 3076 bytes"),
     ({"workspace": FAKE + 4}, "aligned to 16"),
 ])
 def test_c_abi_refusals(lib, kw, match):
@@ -59,4 +59,4 @@ def test_c_abi_null_struct_and_no_tokens(lib):
     assert lib.amd_strix_halo_kernels_moe(0, 0, None) == 1
     assert lib.amd_strix_halo_kernels_moe_workspace(None) == -1
     assert lib.amd_strix_halo_kernels_moe(0, 0, _args(tokens=0)) == 0
-    assert lib.amd_strix_halo_kernels_moe_workspace(_args()) == 3072
+    assert lib.amd_strix_halo_kernels_moe_workspace(_args()) == 3076
