@@ -49,6 +49,7 @@ int rows_entry(bool write, int device_index, uintptr_t stream, const shk_kv_cach
     if (int rc = check_cache(cache)) return rc;
     if (int rc = check_rows(rows)) return rc;
     if (rows->tokens == 0) return 0;
+    if (rows->tokens > INT_MAX / cache->kv_heads) return capi_fail("too many tokens for one launch");
     shk::DeviceGuard guard(device_index);
     if (guard.error() != hipSuccess) return capi_fail_hip("hipSetDevice", guard.error());
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -23,12 +23,18 @@ struct Rows {
   long token_stride[2], head_stride[2];
   const void* slots;
   long slots_total;      // pages * page_size
-  long rows;             // tokens * kv_heads
-  int slot8, heads, page_shift;
+  unsigned rows;         // tokens * kv_heads
+  unsigned heads;
+  int slot8, page_shift;
 };
 
+// Rows of a lane, each of keys and of values.
+constexpr int kWriteRows = 1, kReadRows = 2;
+
+// The slot of a token, -1 outside the cache.
 __device__ __forceinline__ long slot_of(const Rows& p, long t) {
-  return p.slot8 ? static_cast<const int64_t*>(p.slots)[t] : static_cast<const int32_t*>(p.slots)[t];
+  const long slot = p.slot8 ? static_cast<const int64_t*>(p.slots)[t] : static_cast<const int32_t*>(p.slots)[t];
+  return slot >= 0 && slot < p.slots_total ? slot : -1;
 }
 
 // Row of the cache, counted in rows, of (slot, head).
@@ -108,108 +114,139 @@ __device__ __forceinline__ void codes8(const float (&v)[8], float s, int (&c)[8]
 template <int TYPE, int BITS, int D, bool VEC>
 __global__ __launch_bounds__(256) void kv_write_kernel(const Rows p) {
   constexpr int LANES = D / 8;  // of a row
-  const int which = blockIdx.y;
-  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
   const int part = threadIdx.x % LANES;
-  const bool live = row < p.rows;
-  const long t = live ? row / p.heads : 0;
-  const int head = live ? (int)(row - t * p.heads) : 0;
-  long slot = live ? slot_of(p, t) : -1;
-  if (slot >= p.slots_total) slot = -1;
-  float v[8] = {};
-  const long from = t * p.token_stride[which] + head * p.head_stride[which] + part * 8;
-  if (slot >= 0) load8<TYPE, VEC>(p.x[which] + from * kSize<TYPE>, v);
-  // magnitudes as integers: a NaN is larger than an infinity, and both stay
-  uint32_t most = 0;
+  const unsigned first = blockIdx.x * (256 / LANES * kWriteRows) + threadIdx.x / LANES;
+  long slot[kWriteRows];
+  unsigned head[kWriteRows];
+  float v[kWriteRows][2][8] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < kWriteRows; ++i) {
+    const unsigned row = first + i * (256 / LANES), t = row / p.heads;
+    head[i] = row - t * p.heads;
+    slot[i] = row < p.rows ? slot_of(p, t) : -1;
 #pragma unroll
-  for (int d = 1; d < LANES; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
-  if (slot < 0) return;
-  const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (BITS == 4 ? 7.0f : 127.0f));
-  int c[8];
-  codes8<BITS>(v, __uint_as_float(sb << 16), c);
-  const long out = cache_row(p, slot, head);
-  uint8_t* dst = p.codes[which] + out * (D * BITS / 8) + part * BITS;
-  if constexpr (BITS == 4) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= ((uint32_t)c[i] & 0xFu) << (4 * i);
-    *reinterpret_cast<uint32_t*>(dst) = w;
-  } else {
-    uint32_t lo = 0, hi = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo |= ((uint32_t)c[i] & 0xFFu) << (8 * i);
-      hi |= ((uint32_t)c[i + 4] & 0xFFu) << (8 * i);
-    }
-    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    for (int which = 0; which < 2; ++which)
+      if (slot[i] >= 0)
+        load8<TYPE, VEC>(p.x[which] + ((long)t * p.token_stride[which] + head[i] * p.head_stride[which] + part * 8) *
+                                          kSize<TYPE>, v[i][which]);
   }
-  if (part == 0) p.scales[which][out] = (uint16_t)sb;
+#pragma unroll
+  for (int i = 0; i < kWriteRows; ++i)
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      // magnitudes as integers: a NaN is larger than an infinity, and both stay
+      uint32_t most = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[i][which][e]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int d = 1; d < LANES; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+      if (slot[i] < 0) continue;
+      const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (BITS == 4 ? 7.0f : 127.0f));
+      int c[8];
+      codes8<BITS>(v[i][which], __uint_as_float(sb << 16), c);
+      const long out = cache_row(p, slot[i], head[i]);
+      uint8_t* dst = p.codes[which] + out * (D * BITS / 8) + part * BITS;
+      if constexpr (BITS == 4) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w |= ((uint32_t)c[e] & 0xFu) << (4 * e);
+        *reinterpret_cast<uint32_t*>(dst) = w;
+      } else {
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo |= ((uint32_t)c[e] & 0xFFu) << (8 * e);
+          hi |= ((uint32_t)c[e + 4] & 0xFFu) << (8 * e);
+        }
+        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      }
+      if (part == 0) p.scales[which][out] = (uint16_t)sb;
+    }
 }
 
-template <int TYPE, bool VEC>
+// Streamed past the caches: what is read back is used by another kernel.
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void stream16(void* p, v4u v) { __builtin_nontemporal_store(v, static_cast<v4u*>(p)); }
+
+// Eight values at element address p.  FINITE: none is a NaN.
+template <int TYPE, bool VEC, bool FINITE>
 __device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
+  uint32_t o[TYPE == SHK_SRC_F32 ? 8 : 4];
   if constexpr (TYPE == SHK_SRC_F32) {
-    float* o = reinterpret_cast<float*>(p);
-    if constexpr (VEC) {
-      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      for (int i = 0; i < 8; ++i) o[i] = v[i];
-    }
-  } else {
-    uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      b[i] = TYPE == SHK_SRC_BF16 ? f32_to_bf16_rne(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(b[0] | (b[1] << 16), b[2] | (b[3] << 16), b[4] | (b[5] << 16),
-                                                b[6] | (b[7] << 16));
-    } else {
-      for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)b[i];
+    for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (TYPE == SHK_SRC_F16)
+        o[i] = __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) << 16);
+      else if constexpr (FINITE) o[i] = pack_bf16x2_nonan(v[2 * i], v[2 * i + 1]);
+      else o[i] = f32_to_bf16_rne(v[2 * i]) | (f32_to_bf16_rne(v[2 * i + 1]) << 16);
     }
+  }
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (TYPE == SHK_SRC_F32 ? 2 : 1); ++i)
+      stream16(p + 16 * i, v4u{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]});
+  } else {
+    __builtin_memcpy(__builtin_assume_aligned(p, 2), o, sizeof(o));
   }
 }
 
 template <int TYPE, int BITS, int D, bool VEC>
 __global__ __launch_bounds__(256) void kv_read_kernel(const Rows p) {
   constexpr int LANES = D / 8;
-  const int which = blockIdx.y;
-  const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
-  if (row >= p.rows) return;
   const int part = threadIdx.x % LANES;
-  const long t = row / p.heads;
-  const int head = (int)(row - t * p.heads);
-  const long slot = slot_of(p, t);
-  float v[8];
-  if (slot >= 0 && slot < p.slots_total) {
-    const long at = cache_row(p, slot, head);
-    const uint8_t* src = p.codes[which] + at * (D * BITS / 8) + part * BITS;
-    const float s = bf16_bits_to_f32(p.scales[which][at]);
-    if constexpr (BITS == 4) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(src);
+  const unsigned first = blockIdx.x * (256 / LANES * kReadRows) + threadIdx.x / LANES;
+  unsigned t[kReadRows], head[kReadRows];
+  long slot[kReadRows];
+  uint2 w[kReadRows][2] = {};
+  float scale[kReadRows][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)((int32_t)(w << (28 - 4 * i)) >> 28) * s;
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(src);
+  for (int i = 0; i < kReadRows; ++i) {
+    const unsigned row = first + i * (256 / LANES);
+    t[i] = row / p.heads;
+    head[i] = row - t[i] * p.heads;
+    slot[i] = row < p.rows ? slot_of(p, t[i]) : -1;
+    const long at = slot[i] >= 0 ? cache_row(p, slot[i], head[i]) : 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i % 4))) * s;
+    for (int which = 0; which < 2; ++which) {
+      scale[i][which] = __builtin_nanf("");
+      if (slot[i] < 0) continue;
+      const uint8_t* src = p.codes[which] + at * (D * BITS / 8) + part * BITS;
+      if constexpr (BITS == 4) w[i][which].x = *reinterpret_cast<const uint32_t*>(src);
+      else w[i][which] = *reinterpret_cast<const uint2*>(src);
+      scale[i][which] = bf16_bits_to_f32(p.scales[which][at]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __builtin_nanf("");
   }
-  uint8_t* dst = const_cast<uint8_t*>(p.x[which]) +
-                 (t * p.token_stride[which] + head * p.head_stride[which] + part * 8) * kSize<TYPE>;
-  store8<TYPE, VEC>(dst, v);
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    if (first + i * (256 / LANES) >= p.rows) continue;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint2 u = w[i][which];
+        const int code = BITS == 4 ? (int32_t)(u.x << (28 - 4 * e)) >> 28 : (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e % 4)));
+        v[e] = (float)code * scale[i][which];
+      }
+      uint8_t* dst = const_cast<uint8_t*>(p.x[which]) +
+                     ((long)t[i] * p.token_stride[which] + head[i] * p.head_stride[which] + part * 8) * kSize<TYPE>;
+      // an infinite scale makes NaN of a zero code
+      if (__builtin_fabsf(scale[i][which]) < __builtin_inff()) store8<TYPE, VEC, true>(dst, v);
+      else store8<TYPE, VEC, false>(dst, v);
+    }
+  }
 }
 
 template <int TYPE, int BITS, int D, bool VEC>
 hipError_t launch(bool write, const Rows& p, hipStream_t s) {
-  const long blocks = (p.rows * (D / 8) + 255) / 256;
+  const long kPer = 256 / (D / 8) * (write ? kWriteRows : kReadRows);  // rows of a workgroup
+  const long blocks = (p.rows + kPer - 1) / kPer;
   if (blocks > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
-  const dim3 grid((unsigned)blocks, 2);
+  const dim3 grid((unsigned)blocks);
   if (write) hipLaunchKernelGGL((kv_write_kernel<TYPE, BITS, D, VEC>), grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((kv_read_kernel<TYPE, BITS, D, VEC>), grid, dim3(256), 0, s, p);
   return hipGetLastError();
@@ -242,9 +279,9 @@ hipError_t rows_launch(bool write, const shk_kv_cache& c, const shk_kv_rows& r, 
   p.head_stride[0] = r.key_head_stride, p.head_stride[1] = r.value_head_stride;
   p.slots = r.slots;
   p.slots_total = c.pages * c.page_size;
-  p.rows = r.tokens * c.kv_heads;
+  p.rows = (unsigned)(r.tokens * c.kv_heads);
   p.slot8 = r.slot_bytes == 8;
-  p.heads = (int)c.kv_heads;
+  p.heads = (unsigned)c.kv_heads;
   p.page_shift = __builtin_ctzl((unsigned long)c.page_size);
   if (p.rows == 0) return hipSuccess;
   // 16-byte accesses where every row starts on 16 bytes
