@@ -70,6 +70,13 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
   return m == -__builtin_inff() && !(l != l) ? -__builtin_inff() : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
+// The first of `total` pieces that workgroup j of `spread` takes, and the
+// workgroup that takes a piece.
+__device__ __forceinline__ int share(int j, int total, int spread) { return (int)((long)j * total / spread); }
+__device__ __forceinline__ int taker(int piece, int total, int spread) {
+  return (int)(((long)(piece + 1) * spread - 1) / total);
+}
+
 // Pieces of the sequences before b.
 __device__ __forceinline__ int pieces_before(const AttnArgs& a, int b) {
   const int lane = threadIdx.x & 63;
@@ -133,8 +140,8 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
   int total = shared ? pieces_of(a, a.prefix) : __shfl(upto0, 63, 64);
   if (!shared && a.batch > 64) total = pieces_before(a, a.batch);
   total = __builtin_amdgcn_readfirstlane(total);
-  const int each = max((total + groups - 1) / groups, 1);
-  const int first = j * each, end = min(first + each, total);
+  const int spread = max(min(groups, total), 1);  // workgroups with a piece
+  const int first = j < spread ? share(j, total, spread) : total, end = j < spread ? share(j + 1, total, spread) : total;
   const int rows_here = own_rows(a) * (shared ? a.batch : 1);
   const KvView kv{a.kc, a.vc, a.ks, a.vs, a.pages, a.page_shift, a.kv_heads, head};
 
@@ -478,8 +485,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d, 64), before += __shfl_xor(before, d, 64);
   const int mine = pieces_of(a, tokens_of(a, b));
-  const int each = max((total + a.own_groups - 1) / a.own_groups, 1);
-  const int first = before / each, own = mine == 0 ? 0 : (before + mine - 1) / each - first + 1;
+  const int spread = max(min(a.own_groups, total), 1);
+  const int first = mine == 0 ? 0 : taker(before, total, spread);
+  const int own = mine == 0 ? 0 : taker(before + mine - 1, total, spread) - first + 1;
   const int count = own + a.prefix_splits;
   const long own_at = ((long)head * a.slots + first + b) * per + in;
   const long prefix_at = own_parts(a) + (long)head * per * a.batch + (long)b * per + in;
