@@ -106,21 +106,38 @@ __device__ __forceinline__ void store_piece(const AttnArgs& a, bool direct, long
   else *reinterpret_cast<f4*>(a.part_o + part_row * D + d) = v;
 }
 
+// The LDS of a workgroup of either kind.
+template <int D>
+struct StreamShared {
+  static constexpr int kPitch = D + 4;  // floats of a row: the 16 rows start on different banks
+  float o[4][16 * kPitch];              // the waves' outputs, references and sums
+  float m[4][16], l[4][16];
+};
+template <int D>
+struct PrefixShared {
+  static constexpr int kBuffers = D == 256 ? 1 : 2;  // 64 KB a workgroup: two on a CU
+  // the products' operands as the lanes read them: K by block and step, V by
+  // 32 tokens and 16 values of head_dim
+  h8 k[kBuffers][4][D / 32][64];
+  h8 v[kBuffers][2][D / 16][64];
+  float scale[kBuffers][2][kKvTile];
+  int bad;
+};
+
 template <int BITS, int D, int RT, int TYPE>
-__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
+__device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, StreamShared<D>& lds) {
   using Rows = KvRows<BITS, D, RT, TYPE>;
   // blocks of 16 tokens a wave takes at a time: half of the usual four where
   // they would not fit the registers
   constexpr int NB = D * RT >= 256 ? 2 : 4;
   constexpr int kStep = 16 * NB, kPer = kPiece / kStep;
-  constexpr int kPitch = D + 4;  // floats of an LDS row: the 16 rows start on different banks
-  __shared__ __align__(16) float red_o[4][16 * kPitch];
-  __shared__ float red_m[4][16], red_l[4][16];
+  constexpr int kPitch = StreamShared<D>::kPitch;
+  auto &red_o = lds.o;
+  auto &red_m = lds.m, &red_l = lds.l;
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 
   // which pieces: those of the sequences first, then those of the prefix
-  int unit = blockIdx.x;
   const int own_units = a.kv_heads * a.own_tiles * a.own_groups;
   const bool shared = unit >= own_units;
   if (shared) unit -= own_units;
@@ -346,20 +363,17 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
 }
 
 template <int BITS, int D, int RT, int TYPE>
-__global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
+__device__ __forceinline__ void prefix_pieces(const AttnArgs& a, int unit, PrefixShared<D>& lds) {
   using Rows = KvRows<BITS, D, RT, TYPE>;
   using Block = KvBlock<BITS, D>;
-  constexpr int kBuffers = D == 256 ? 1 : 2;  // 64 KB a workgroup: two on a CU
+  constexpr int kBuffers = PrefixShared<D>::kBuffers;
   constexpr int kSteps = Rows::kSteps, kOut = Rows::kOut;
-  // the products' operands as the lanes read them: K by block and step, V by
-  // 32 tokens and 16 values of head_dim
-  __shared__ h8 lds_k[kBuffers][4][kSteps][64];
-  __shared__ h8 lds_v[kBuffers][2][kOut][64];
-  __shared__ __align__(16) float lds_s[kBuffers][2][kKvTile];  // scales
-  __shared__ int lds_bad;
+  auto &lds_k = lds.k;
+  auto &lds_v = lds.v;
+  auto &lds_s = lds.scale;
+  int &lds_bad = lds.bad;
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  int unit = blockIdx.x;
   const int head = unit % a.kv_heads;
   unit /= a.kv_heads;
   const int split = unit % a.prefix_splits, tile = unit / a.prefix_splits;
@@ -462,6 +476,25 @@ __global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
         *reinterpret_cast<f4*>(a.part_o + to * D + (4 * g + r) * kOut + j) =
             f4{rows.o[t][j][r], rows.o[t][j + 1][r], rows.o[t][j + 2][r], rows.o[t][j + 3][r]};
   }
+}
+
+template <int BITS, int D, int RT, int TYPE>
+__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const AttnArgs a) {
+  __shared__ __align__(16) StreamShared<D> lds;
+  stream_pieces<BITS, D, RT, TYPE>(a, blockIdx.x, lds);
+}
+
+// The prefix's workgroups and those of the sequences' own tokens in one
+// launch: the latter fill the CUs that the former leave.
+template <int BITS, int D, int PREFIX_RT, int RT, int TYPE>
+__global__ __launch_bounds__(256, 2) void kv_prefix_kernel(const AttnArgs a) {
+  __shared__ __align__(16) union {
+    PrefixShared<D> prefix;
+    StreamShared<D> stream;
+  } lds;
+  const int units = a.kv_heads * a.prefix_tiles * a.prefix_splits;
+  if ((int)blockIdx.x < units) prefix_pieces<BITS, D, PREFIX_RT, TYPE>(a, blockIdx.x, lds.prefix);
+  else stream_pieces<BITS, D, RT, TYPE>(a, blockIdx.x - units, lds.stream);
 }
 
 // Joins the pieces of a row, a workgroup each: lane p of every wave looks at
@@ -572,28 +605,26 @@ long part_rows(const shk_kv_cache& c, const shk_kv_attention& a, const Plan& p) 
   return p.direct ? 0 : c.kv_heads * rows * (p.own_groups + a.batch + (long)p.prefix_splits * a.batch);
 }
 
-template <int BITS, int D, int TYPE>
-hipError_t launch_kernels(const AttnArgs& a, const Plan& p, hipStream_t s) {
-  const bool shared = a.prefix_splits > 0 && !p.prefix_kernel;
+template <int BITS, int D, int RT, int TYPE>
+hipError_t launch_rt(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const long own = (long)a.kv_heads * a.own_tiles * a.own_groups;
   const long prefix = (long)a.kv_heads * a.prefix_tiles * a.prefix_splits;
-  const dim3 grid((unsigned)(own + (shared ? prefix : 0))), block(256);
   if (own + prefix > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
-  if constexpr (D < 256) {
-    if (p.rt == 2) hipLaunchKernelGGL((kv_stream_kernel<BITS, D, 2, TYPE>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv_stream_kernel<BITS, D, 1, TYPE>), grid, block, 0, s, a);
-  } else {
-    hipLaunchKernelGGL((kv_stream_kernel<BITS, D, 1, TYPE>), grid, block, 0, s, a);
-  }
-  hipError_t err = hipGetLastError();
-  if (err == hipSuccess && p.prefix_kernel) {
-    hipLaunchKernelGGL((kv_prefix_kernel<BITS, D, D == 256 ? 1 : 2, TYPE>), dim3((unsigned)prefix), block, 0, s, a);
-    err = hipGetLastError();
-  }
+  const dim3 grid((unsigned)(own + prefix)), block(256);
+  if (p.prefix_kernel) hipLaunchKernelGGL((kv_prefix_kernel<BITS, D, D == 256 ? 1 : 2, RT, TYPE>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((kv_stream_kernel<BITS, D, RT, TYPE>), grid, block, 0, s, a);
+  const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.direct) return err;
   const long rows = (long)a.batch * a.queries * a.heads;
   hipLaunchKernelGGL((kv_join_kernel<D>), dim3((unsigned)rows), block, 0, s, a);
   return hipGetLastError();
+}
+
+template <int BITS, int D, int TYPE>
+hipError_t launch_kernels(const AttnArgs& a, const Plan& p, hipStream_t s) {
+  if constexpr (D < 256)
+    if (p.rt == 2) return launch_rt<BITS, D, 2, TYPE>(a, p, s);
+  return launch_rt<BITS, D, 1, TYPE>(a, p, s);
 }
 
 template <int BITS, int TYPE>
