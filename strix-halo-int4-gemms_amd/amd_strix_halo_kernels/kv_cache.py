@@ -14,8 +14,10 @@ as zeros; a row that holds an infinity or a NaN reads back as NaN.
 ``kv_cache_write`` quantizes new tokens into their slots, ``kv_cache_read``
 dequantizes slots, and ``kv_cache_attention`` is softmax attention of each
 sequence's newest tokens over its pages, after a prefix that the whole batch
-may share.  All run on the current stream of the tensors' device and read
-nothing back to the host; there is no CPU path.
+may share.  All run on the current stream of the tensors' device, or on
+``stream`` (which is then the current one for the call, its allocations
+included), and read nothing back to the host.  There is no CPU path and no
+gradient.
 """
 
 from __future__ import annotations
@@ -26,7 +28,7 @@ from dataclasses import dataclass
 from typing import Any
 
 from . import kernel_table as kt
-from .native import _check, _device_index, _require_device, _stream_handle, _torch, _verified_library
+from .native import _check, _device_index, _on_stream, _require_device, _stream_handle, _torch, _verified_library
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -155,6 +157,9 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
     """
     torch = _torch()
     _check_devices(cache, keys=keys, values=values, slots=slots)
+    if stream is not None:
+        with _on_stream(torch, keys, stream):
+            return kv_cache_write(cache, keys, values, slots)
     kind = _row_type(torch, "keys", keys.dtype)
     if values.dtype != keys.dtype:
         raise ValueError(f"values must have the dtype of keys, {keys.dtype}; got {values.dtype}")
@@ -169,7 +174,7 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
     if tokens == 0:
         return
     lib = _verified_library()
-    _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, stream),
+    _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, None),
                                                     cache._native, _rows(keys, values, slots, kind, tokens)))
 
 
@@ -179,6 +184,9 @@ def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any 
     tensors.  Slots outside the cache give NaN."""
     torch = _torch()
     _check_devices(cache, slots=slots)
+    if stream is not None:
+        with _on_stream(torch, slots, stream):
+            return kv_cache_read(cache, slots, dtype=dtype)
     dtype = torch.bfloat16 if dtype is None else dtype
     kind = _row_type(torch, "the result", dtype)
     _check_slots(torch, slots, None)
@@ -188,7 +196,7 @@ def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any 
     values = torch.empty_like(keys)
     if tokens:
         lib = _verified_library()
-        _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, stream),
+        _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, None),
                                                        cache._native, _rows(keys, values, slots, kind, tokens)))
     return keys, values
 
@@ -229,6 +237,11 @@ def kv_cache_attention(
     """
     torch = _torch()
     _check_devices(cache, q=q, page_table=page_table, lengths=lengths, prefix_pages=prefix_pages, out=out)
+    if stream is not None:
+        with _on_stream(torch, q, stream):
+            return kv_cache_attention(q, cache, page_table, lengths, prefix_pages=prefix_pages,
+                                      prefix_length=prefix_length, softmax_scale=softmax_scale,
+                                      return_lse=return_lse, out=out)
     if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
         raise ValueError(f"q must have dtype torch.bfloat16 or torch.float16; got {q.dtype}")
     if q.ndim not in (3, 4) or q.shape[-1] != cache.head_dim:
@@ -275,8 +288,7 @@ def kv_cache_attention(
         sb, sq, sh = (strides[0], strides[1], strides[2]) if q.ndim == 4 else (strides[0], 0, strides[1])
         if q.data_ptr() % 16 or sb % 8 or sq % 8 or sh % 8:
             # 16-byte reads: rows that do not start on 16 bytes are copied
-            with torch.cuda.stream(stream):
-                q = q.clone(memory_format=torch.contiguous_format)
+            q = q.clone(memory_format=torch.contiguous_format)
             sb, sq, sh = queries * heads * cache.head_dim, heads * cache.head_dim, cache.head_dim
         kind = kt.SRC_BF16 if q.dtype == torch.bfloat16 else kt.SRC_F16
         table_pages = page_table.shape[1]
@@ -298,11 +310,7 @@ def kv_cache_attention(
                 _check(lib, 1)
             if len(cache._workspaces) < 4096:
                 cache._workspaces[key] = nbytes
-        work = None
-        if nbytes:
-            work = q.new_empty(nbytes, dtype=torch.uint8)
-            if stream is not None:
-                work.record_stream(stream)
-        _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, stream),
+        work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, None),
                                                             cache._native, args(work, nbytes)))
     return (out, lse) if return_lse else out

@@ -14,7 +14,7 @@ from typing import Any
 
 from . import kernel_table as kt
 from .metadata import SUPPORTED_SUBCHANNELS, GemmLayout, ScaleMode, ScaleSpec
-from .native import _check, _device_index, _require_device, _stream_handle, _torch, _verified_library
+from .native import _check, _device_index, _on_stream, _require_device, _stream_handle, _torch, _verified_library
 
 MOE_MAX_TOKENS = 64
 MOE_MAX_PAIRS = 1024
@@ -67,7 +67,9 @@ def moe_swiglu_int4(
     Activations are not quantized; sums and the value between the products
     are f32.  Takes up to 64 tokens (larger batches are ``ragged_dot_int4``'s),
     1024 (token, expert) pairs and 1024 experts.  Returns [tokens, hidden] in
-    x's dtype.  Nothing is read back to the host.
+    x's dtype.  Runs on the current stream, or on ``stream`` (which is then the
+    current one for the call, its allocations included); nothing is read back
+    to the host, and there is no gradient.
     """
     layout = GemmLayout(layout)
     if layout not in (GemmLayout.NN, GemmLayout.NT):
@@ -79,6 +81,10 @@ def moe_swiglu_int4(
             _require_device(torch, {"x": x, "up_gate": up_gate, "down": down, "expert_ids": expert_ids,
                                     "expert_weights": expert_weights, "up_gate_scale": up_gate_scale,
                                     "down_scale": down_scale, "out": out})  # says what is wrong
+    if stream is not None:
+        with _on_stream(torch, x, stream):
+            return moe_swiglu_int4(x, up_gate, down, expert_ids, expert_weights, up_gate_scale=up_gate_scale,
+                                   down_scale=down_scale, scale=scale, layout=layout, out=out)
     if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
         raise ValueError(f"x must have dtype torch.bfloat16 or torch.float16; got {x.dtype}")
     if x.ndim != 2 or x.shape[1] < 1:
@@ -120,6 +126,8 @@ def moe_swiglu_int4(
     if tokens > MOE_MAX_TOKENS or tokens * top > MOE_MAX_PAIRS:
         raise ValueError(f"moe_swiglu_int4 takes up to {MOE_MAX_TOKENS} tokens and {MOE_MAX_PAIRS} (token, expert) "
                          f"pairs; got {tokens} and {tokens * top}. Larger batches: ragged_dot_int4")
+    if up_gate.numel() < 4 or down.numel() < 4:
+        raise ValueError("up_gate and down must hold at least 4 bytes each")
     if experts > MOE_MAX_EXPERTS:
         raise ValueError(f"moe_swiglu_int4 takes up to {MOE_MAX_EXPERTS} experts; got {experts}")
     if out is None:
@@ -132,13 +140,11 @@ def moe_swiglu_int4(
     # pair; a counter for each 128 columns of the output
     nbytes = 4 * (tokens * top * (-(-inner // 128) * 128 + hidden) + -(-hidden // 128))
     work = x.new_empty(nbytes, dtype=torch.uint8)
-    if stream is not None:
-        work.record_stream(stream)
     args = _MOE.pack(x.data_ptr(), x.stride(0), kt.SRC_BF16 if x.dtype == torch.bfloat16 else kt.SRC_F16, tokens,
                      hidden, inner, experts, top, up_gate.data_ptr(), up_gate_scale.data_ptr(), down.data_ptr(),
                      down_scale.data_ptr(), group, kt.LAYOUT_NT if nt else kt.LAYOUT_NN, expert_ids.data_ptr(),
                      expert_ids.element_size(), expert_weights.data_ptr(), out.data_ptr(),
                      work.data_ptr(), nbytes)
     lib = _verified_library()
-    _check(lib, lib.amd_strix_halo_kernels_moe(index, _stream_handle(torch, x, stream), args))
+    _check(lib, lib.amd_strix_halo_kernels_moe(index, _stream_handle(torch, x, None), args))
     return out

@@ -224,6 +224,15 @@ def _stream_handle(torch: Any, tensor: Any, stream: Any | None) -> int:
     return int(torch.cuda.current_stream(tensor.device).cuda_stream)
 
 
+def _on_stream(torch: Any, tensor: Any, stream: Any) -> Any:
+    """`stream` as the current one: what a call allocates then belongs to it,
+    and no block comes back that the caller's own stream still works on."""
+    index = getattr(stream, "device_index", None)
+    if index is not None and index != tensor.get_device():
+        raise ValueError(f"stream is on cuda:{index}, expected {tensor.device}")
+    return torch.cuda.stream(stream)
+
+
 def _device_index(tensor: Any) -> int:
     index = tensor.device.index
     return 0 if index is None else int(index)

@@ -83,7 +83,8 @@ def decode_units() -> list[tuple[str, Path, list[str]]]:
     return [
         ("kvcache", CSRC / "k_kvcache.hip", []),
         ("kvattn", CSRC / "k_kvattn.hip", []),
-        ("moe", CSRC / "k_moe.hip", []),
+        ("moe_nn", CSRC / "k_moe.hip", ["-DSHK_LAYOUT=0"]),
+        ("moe_nt", CSRC / "k_moe.hip", ["-DSHK_LAYOUT=1"]),
         ("capi_decode", CSRC / "capi_decode.hip", []),
     ]
 

@@ -90,6 +90,9 @@ int check_moe(const shk_moe* a) {
   if (a->experts < 1 || a->experts > 1024) return capi_fail("1 to 1024 experts; got " + std::to_string(a->experts));
   if (a->hidden < 1 || a->inner < 1 || a->hidden > (1 << 20) || a->inner > (1 << 20))
     return capi_fail("hidden and inner must be from 1 to 1048576");
+  // codes are read a dword at a time, the last one from the matrix's end
+  if (a->experts * 2 * a->inner * ((a->hidden + 1) / 2) < 4 || a->experts * a->hidden * ((a->inner + 1) / 2) < 4)
+    return capi_fail("up_gate and down must hold at least 4 bytes each");
   if (a->id_bytes != 4 && a->id_bytes != 8) return capi_fail("ids are int32 or int64");
   return 0;
 }
@@ -168,7 +171,8 @@ int amd_strix_halo_kernels_moe(int device_index, uintptr_t stream, const shk_moe
       return capi_fail("the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
     shk::DeviceGuard guard(device_index);
     if (guard.error() != hipSuccess) return capi_fail_hip("hipSetDevice", guard.error());
-    const hipError_t err = shk::launch_moe(a, reinterpret_cast<hipStream_t>(stream));
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const hipError_t err = a.layout == SHK_LAYOUT_NT ? shk::launch_moe_nt(a, s) : shk::launch_moe_nn(a, s);
     if (err != hipSuccess) return capi_fail_hip("moe launch", err);
     return 0;
   });

@@ -158,7 +158,8 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
   if (!shared && a.batch > 64) total = pieces_before(a, a.batch);
   total = __builtin_amdgcn_readfirstlane(total);
   const int spread = max(min(groups, total), 1);  // workgroups with a piece
-  const int first = j < spread ? share(j, total, spread) : total, end = j < spread ? share(j + 1, total, spread) : total;
+  const int first = j < spread ? share(j, total, spread) : total;
+  const int end = j < spread ? share(j + 1, total, spread) : total;
   const int rows_here = own_rows(a) * (shared ? a.batch : 1);
   const KvView kv{a.kc, a.vc, a.ks, a.vs, a.pages, a.page_shift, a.kv_heads, head};
 
@@ -286,7 +287,8 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
 #pragma unroll
           for (int x = 0; x < 4; ++x) now.blk[2 * h + x / 2].v_pairs(w, x % 2, f[x]);
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) rows.template add<NB / 2>(4 * w + jj, join(f[0][jj], f[1][jj], f[2][jj], f[3][jj]), p, pl, h);
+          for (int jj = 0; jj < 4; ++jj)
+            rows.template add<NB / 2>(4 * w + jj, join(f[0][jj], f[1][jj], f[2][jj], f[3][jj]), p, pl, h);
         }
     };
     if (step0 < step_end) {
@@ -591,7 +593,8 @@ Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
   // three workgroups on each of the 256 CUs, two where they hold more
   const long want = 512;
   p.own_groups = p.direct ? (int)a.batch
-                          : (int)std::max(1L, std::min(want / (c.kv_heads * p.own_tiles), a.batch * cdiv(tokens, kPiece)));
+                          : (int)std::max(1L, std::min(want / (c.kv_heads * p.own_tiles),
+                                                       a.batch * cdiv(tokens, kPiece)));
   if (prefix) {
     p.prefix_tiles = (int)cdiv(all, p.prefix_kernel ? 64 * p.prefix_rt : 16 * p.rt);
     p.prefix_splits = (int)std::max(1L, std::min(cdiv(p.prefix_kernel ? 512 : want, c.kv_heads * p.prefix_tiles),
@@ -611,7 +614,8 @@ hipError_t launch_rt(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const long prefix = (long)a.kv_heads * a.prefix_tiles * a.prefix_splits;
   if (own + prefix > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
   const dim3 grid((unsigned)(own + prefix)), block(256);
-  if (p.prefix_kernel) hipLaunchKernelGGL((kv_prefix_kernel<BITS, D, D == 256 ? 1 : 2, RT, TYPE>), grid, block, 0, s, a);
+  if (p.prefix_kernel)
+    hipLaunchKernelGGL((kv_prefix_kernel<BITS, D, D == 256 ? 1 : 2, RT, TYPE>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((kv_stream_kernel<BITS, D, RT, TYPE>), grid, block, 0, s, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.direct) return err;

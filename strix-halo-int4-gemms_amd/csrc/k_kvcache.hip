@@ -229,7 +229,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const Rows p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint2 u = w[i][which];
-        const int code = BITS == 4 ? (int32_t)(u.x << (28 - 4 * e)) >> 28 : (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e % 4)));
+        const int code = BITS == 4 ? (int32_t)(u.x << (28 - 4 * e)) >> 28
+                                   : (int8_t)((e < 4 ? u.x : u.y) >> (8 * (e % 4)));
         v[e] = (float)code * scale[i][which];
       }
       uint8_t* dst = const_cast<uint8_t*>(p.x[which]) +

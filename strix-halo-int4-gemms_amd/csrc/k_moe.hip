@@ -31,6 +31,10 @@
 #include "shk_loads.h"
 #include "shk_moe.h"
 
+#ifndef SHK_LAYOUT
+#error "SHK_LAYOUT must be defined: the weights' layout, 0 NN or 1 NT"
+#endif
+
 namespace shk {
 namespace {
 
@@ -39,9 +43,9 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 typedef __attribute__((address_space(1))) const uint16_t* global_halves;
 
-constexpr int kHalf = 64;          // columns of half a workgroup's tile
+constexpr int kHalf = kMoeColumns / 2;  // columns of half a workgroup's tile
 constexpr int kPitch = 2 * kHalf + 4;  // floats of an LDS row of sums: rows start on different banks
-constexpr int kSuper = 128;        // K values a wave loads at a time, four products deep
+constexpr int kSuper = kMoePiece;        // K values a wave loads at a time, four products deep
 constexpr int kLargeGroups = 1;    // scale groups of at least a piece
 constexpr int kSmallGroups = 2;    // of 32 or 64
 constexpr int kMostPairs = 1024;   // (token, expert) pairs of a call
@@ -272,7 +276,8 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   // scales.
   const int sc_n = (lane < 32 ? n0 : n1) + 2 * (lane % 32);
   auto fits = [&](int k0) {
-    const bool scales = !GROUPED || scale + (long)min((k0 + kSuper - 1) / a.group, a.groups - 1) * s.total + n1 + kHalf <=
+    const int last = GROUPED ? min((k0 + kSuper - 1) / a.group, a.groups - 1) : 0;
+    const bool scales = !GROUPED || scale + (long)last * s.total + n1 + kHalf <=
                                         a.scale + (long)a.experts * a.groups * s.total;
     return scales && inside<LAYOUT>(s, k0, n0) && inside<LAYOUT>(s, k0, n1);
   };
@@ -506,7 +511,10 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
         if (col < a.cols) {
           float up = 0.0f, gate = 0.0f;
 #pragma unroll
-          for (int q = 0; q < kWaves / 2; ++q) up += red[q * 16 * kPitch + r * kPitch + n], gate += red[q * 16 * kPitch + r * kPitch + kHalf + n];
+          for (int q = 0; q < kWaves / 2; ++q) {
+            up += red[q * 16 * kPitch + r * kPitch + n];
+            gate += red[q * 16 * kPitch + r * kPitch + kHalf + n];
+          }
           if constexpr (!GROUPED) up *= load_bf16(scale + col), gate *= load_bf16(scale + a.cols + col);
           h = up * (gate / (1.0f + __expf(-gate)));
         }
@@ -707,8 +715,8 @@ hipError_t launch_product(const MoeArgs& a, unsigned columns, unsigned hit, hipS
   return hipGetLastError();
 }
 
-template <int LAYOUT>
-hipError_t launch_layout(const shk_moe& x, MoeArgs a, hipStream_t s) {
+hipError_t launch_layer(const shk_moe& x, MoeArgs a, hipStream_t s) {
+  constexpr int LAYOUT = SHK_LAYOUT;
   // with no pairs the down product still writes the zeros
   const unsigned hit = (unsigned)std::max(1L, (long)std::min(x.tokens * x.top, x.experts));
   a.w = static_cast<const uint8_t*>(x.up_gate);
@@ -732,34 +740,29 @@ hipError_t launch_layout(const shk_moe& x, MoeArgs a, hipStream_t s) {
 
 }  // namespace
 
-// h's rows are whole pieces of 128 K values, the rest zero.
-static long inner_pad(const shk_moe& a) { return (a.inner + kSuper - 1) / kSuper * kSuper; }
-
-static long down_tiles(const shk_moe& a) { return (a.hidden + 2 * kHalf - 1) / (2 * kHalf); }
-
-int64_t moe_workspace(const shk_moe& a) {
-  return a.tokens * a.top * (inner_pad(a) + a.hidden) * 4 + down_tiles(a) * 4;
-}
-
-hipError_t launch_moe(const shk_moe& x, hipStream_t s) {
+#if SHK_LAYOUT == 0  // SHK_LAYOUT_NN
+hipError_t launch_moe_nn(const shk_moe& x, hipStream_t s) {
+#else
+hipError_t launch_moe_nt(const shk_moe& x, hipStream_t s) {
+#endif
   MoeArgs a{};
   a.x = x.x, a.x_stride = x.x_stride;
   a.ids = x.ids, a.id8 = x.id_bytes == 8;
   a.share = x.share;
   a.h = static_cast<uint16_t*>(x.workspace);
-  a.part = static_cast<float*>(x.workspace) + x.tokens * x.top * inner_pad(x);
+  a.part = static_cast<float*>(x.workspace) + x.tokens * x.top * moe_inner_pad(x);
   a.arrived = reinterpret_cast<int*>(a.part + x.tokens * x.top * x.hidden);
-  a.tiles = (int)down_tiles(x);
+  a.tiles = (int)moe_down_tiles(x);
   a.out = x.out;
   a.group = (int)x.group;
   a.tokens = (int)x.tokens, a.top = (int)x.top, a.experts = (int)x.experts;
-  a.hidden = (int)x.hidden, a.inner = (int)x.inner, a.inner_pad = (int)inner_pad(x);
+  a.hidden = (int)x.hidden, a.inner = (int)x.inner, a.inner_pad = (int)moe_inner_pad(x);
   a.type = (int)x.type;
   // One workgroup a tile adds few pairs sooner than another launch starts; with
   // many it would keep all others waiting (96 pairs: 29 us of the down product
   // became 50, where the launch is 4).
   a.joined = x.tokens * x.top <= 16;
-  return x.layout == SHK_LAYOUT_NT ? launch_layout<SHK_LAYOUT_NT>(x, a, s) : launch_layout<SHK_LAYOUT_NN>(x, a, s);
+  return launch_layer(x, a, s);
 }
 
 }  // namespace shk

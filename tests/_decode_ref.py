@@ -141,7 +141,8 @@ def moe(x, up_gate, down, ids, share, up_scale, down_scale, group, layout):
             up, gate = ug[:, :inner], ug[:, inner:]
             sig = torch.sigmoid(gate)
             h = up * gate * sig
-            off_h = off[:, :inner] * (gate * sig).abs() + 1.1 * up.abs() * off[:, inner:] + 2 * off[:, :inner] * off[:, inner:]
+            off_h = off[:, :inner] * (gate * sig).abs() + 1.1 * up.abs() * off[:, inner:]
+            off_h = off_h + 2 * off[:, :inner] * off[:, inner:]
             z, off_z = product(h, inner, e, down, down_scale, off_h + 2.0**-20 * h.abs())
             f = float(share[t, j])
             y[t] += f * z[0]

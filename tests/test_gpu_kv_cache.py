@@ -349,6 +349,34 @@ def test_other_stream_and_out(device):
     assert got is out and torch.equal(out, want)
 
 
+def _after_a_long_wait(device, sizes, call):
+    """Runs `call` on another stream while this one still has to read blocks
+    of these sizes that it has given back, and checks what it reads."""
+    stream = torch.cuda.Stream(device)
+    torch.cuda.synchronize()
+    blocks = [torch.full((n,), 7, dtype=torch.uint8, device=device) for n in sizes for _ in range(4)]
+    torch.cuda._sleep(20_000_000)
+    copies = [b.clone() for b in blocks]
+    del blocks
+    got = call(stream)
+    torch.cuda.synchronize()
+    assert all((c == 7).all() for c in copies)
+    return got
+
+
+def test_other_stream_takes_no_block_of_this_one(device):
+    q, cache, table, lengths, _ = _case(43, [700, 90], page=64, device=device)
+    qd, td, ld = q.to(device), table.to(device), lengths.to(device)
+    shifted = torch.empty(qd.numel() + 1, dtype=qd.dtype, device=device)[1:].view(qd.shape).copy_(qd)  # is copied
+    slots = torch.arange(90, device=device)
+    want, read = shk.kv_cache_attention(qd, cache, td, ld), shk.kv_cache_read(cache, slots)
+    sizes = [2 * q.numel(), 2 * read[0].numel()]
+    got = _after_a_long_wait(device, sizes, lambda s: (shk.kv_cache_attention(shifted, cache, td, ld, stream=s),
+                                                       shk.kv_cache_read(cache, slots, stream=s)))
+    assert torch.equal(got[0], want)
+    assert torch.equal(got[1][0], read[0]) and torch.equal(got[1][1], read[1])
+
+
 def test_graph_of_a_step(device):
     """Write and attention captured once; every replay equals the eager step
     on what the buffers hold then."""

@@ -53,7 +53,8 @@ def _check(got, case):
 @pytest.mark.parametrize("layout", ["nn", "nt"])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("group", [0, 32, 64, 128, 256])
-@pytest.mark.parametrize("tokens,experts,top,hidden,inner", [(1, 4, 2, 256, 192), (5, 3, 1, 320, 64), (16, 8, 3, 128, 320),
+@pytest.mark.parametrize("tokens,experts,top,hidden,inner", [(1, 4, 2, 256, 192), (5, 3, 1, 320, 64),
+                                                             (16, 8, 3, 128, 320),
                                                              (17, 2, 2, 288, 96), (64, 4, 2, 160, 128)])
 def test_layer(layout, dtype, group, tokens, experts, top, hidden, inner, device):
     print(f"case moe {layout} {dtype} group {group} {tokens} tokens {experts} experts {hidden}x{inner}", flush=True)
@@ -146,6 +147,22 @@ def test_repeated_calls_streams_and_out(device):
     got = shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6], out=out, stream=stream)
     stream.synchronize()
     assert got is out and torch.equal(out, first)
+
+
+def test_other_stream_takes_no_block_of_this_one(device):
+    case = _case(15, 20, 6, 2, 320, 192)
+    want = _run(case, device)
+    d = [t.to(device) for t in case[:7]]
+    stream = torch.cuda.Stream(device)
+    work = 4 * (20 * 2 * (256 + 320) + 3)
+    torch.cuda.synchronize()
+    blocks = [torch.full((n,), 7, dtype=torch.uint8, device=device) for n in (2 * want.numel(), work) for _ in range(4)]
+    torch.cuda._sleep(20_000_000)
+    copies = [b.clone() for b in blocks]
+    del blocks
+    got = shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6], stream=stream)
+    torch.cuda.synchronize()
+    assert all((c == 7).all() for c in copies) and torch.equal(got, want)
 
 
 def test_graph_of_the_layer(device):

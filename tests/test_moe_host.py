@@ -41,10 +41,11 @@ def _args(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    ({"type": kt.SRC_F32}, "float16 or bfloat16"), ({"layout": kt.LAYOUT_TN}, "NN and NT"), ({"group": 48}, "scale group"),
-    ({"group": 512}, "scale group"), ({"tokens": 65}, "64 tokens"), ({"tokens": -1}, "64 tokens"),
+    ({"type": kt.SRC_F32}, "float16 or bfloat16"), ({"layout": kt.LAYOUT_TN}, "NN and NT"),
+    ({"group": 48}, "scale group"), ({"group": 512}, "scale group"), ({"tokens": 65}, "64 tokens"), ({"tokens": -1}, "64 tokens"),
     ({"top": 513}, "1024 (token, expert) pairs"), ({"experts": 0}, "1024 experts"), ({"experts": 1025}, "1024 experts"),
-    ({"hidden": 0}, "hidden and inner"), ({"inner": 2**21}, "hidden and inner"), ({"id_bytes": 2}, "int32 or int64"),
+    ({"hidden": 1, "inner": 1, "experts": 1}, "at least 4 bytes"), ({"hidden": 0}, "hidden and inner"),
+    ({"inner": 2**21}, "hidden and inner"), ({"id_bytes": 2}, "int32 or int64"),
     ({"x": None}, "non-null"), ({"down_scale": None}, "non-null"), ({"ids": None}, "non-null"),
     ({"share": FAKE + 2}, "aligned to their elements"), ({"x": FAKE + 1}, "aligned to their elements"),
     ({"workspace": None}, "workspace must hold"), ({"workspace_bytes": 3075}, "workspace must hold 3076 bytes"),
