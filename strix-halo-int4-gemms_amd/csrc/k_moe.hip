@@ -5,10 +5,14 @@
 //   y[t] = sum_j share[t, j] * (h[t, j] D_e)
 //
 // Few tokens reach an expert, so the layer is the time to stream the weights
-// of the experts that are hit: each is read once, and each pass over it
-// serves all its rows.  Two products share one body (moe_product): a
-// workgroup takes 64 columns (of up and of gate, or of down) of one expert,
-// its eight waves a slice of K each, joined through LDS.
+// of the experts that are hit.  Two products share one body (moe_product): a
+// workgroup takes 16 pairs of one expert and 128 columns (64 of up and of
+// gate, or 128 of down), its waves a slice of K each, joined through LDS.  An
+// expert with more than 16 pairs has a workgroup for each 16 of them, side by
+// side: all but the first find the codes in the caches.  (Two tiles of 16 in
+// one workgroup take twice the registers for the sums and leave fewer
+// workgroups: 253 us instead of 240 for 122 pairs of 16 experts of 4096 x
+// 11008, 90 instead of 53 for 306 pairs of 16 experts of 320 x 4320.)
 //
 // Products are v_mfma_f32_16x16x32_bf16 with the weights in the rows and the
 // tokens in the columns.  A code v enters as v + 24, which one shift and one
@@ -50,6 +54,8 @@ constexpr int kLargeGroups = 1;    // scale groups of at least a piece
 constexpr int kSmallGroups = 2;    // of 32 or 64
 constexpr int kMostPairs = 1024;   // (token, expert) pairs of a call
 constexpr int kMostExperts = 1024;
+
+constexpr int kRows = 16;          // pairs of a workgroup, the columns of a product
 
 struct MoeArgs {
   const void* x;
@@ -134,21 +140,29 @@ __device__ __forceinline__ void load_w(const Codes& s, int k0, int n0, int n1, u
   }
 }
 
-// The same where part of it lies past the end of all codes, by way of 16
-// dwords of LDS a lane (few registers; at most the last expert's last pieces).
+// The same where part of it lies past the end of all codes (at most the last
+// expert's last pieces), by way of 16 dwords of LDS a lane: few registers, and
+// eight loads at a time.
 template <int LAYOUT, bool WIDE>
 __device__ __forceinline__ void load_w_end(const Codes& s, int k0, int n0, uint32_t* lds, uint32_t (&o)[16]) {
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
 #pragma unroll 1
-  for (int i = 0; i < 16; ++i) {
-    const uint8_t* p = LAYOUT == SHK_LAYOUT_NT
-                           ? s.w + (long)(n0 + 4 * c + i / 4) * s.k_packed + k0 / 2 + 16 * g + 4 * (i % 4)
-                           : s.w + (long)(k0 / 2 + 16 * (i / 4) + 4 * g + i % 4) * s.total + n0 + (WIDE ? 8 : 4) * c;
-    // the last dword there is, shifted to where it would be
-    const long over = p - (s.end - 4);
-    uint32_t v;
-    __builtin_memcpy(&v, over > 0 ? s.end - 4 : p, 4);
-    lds[i * 64 + lane] = over <= 0 ? v : (over < 4 ? v >> (8 * over) : 0u);
+  for (int i0 = 0; i0 < 16; i0 += 8) {
+    uint32_t v[8];
+    long over[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u;
+      const uint8_t* p = LAYOUT == SHK_LAYOUT_NT
+                             ? s.w + (long)(n0 + 4 * c + i / 4) * s.k_packed + k0 / 2 + 16 * g + 4 * (i % 4)
+                             : s.w + (long)(k0 / 2 + 16 * (i / 4) + 4 * g + i % 4) * s.total + n0 + (WIDE ? 8 : 4) * c;
+      // the last dword there is, shifted to where it would be
+      over[u] = p - (s.end - 4);
+      v[u] = *(__attribute__((address_space(1))) const any_u32*)(s.end - 4 + min(over[u], 0l));
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      lds[(i0 + u) * 64 + lane] = over[u] <= 0 ? v[u] : (over[u] < 4 ? v[u] >> (8 * over[u]) : 0u);
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = lds[i * 64 + lane];
@@ -235,11 +249,10 @@ __device__ __forceinline__ int column(int half, int g, int r) {
   return WIDE ? 32 * g + 8 * r + 4 * half : kHalf * half + 16 * g + 4 * r;
 }
 
-// A workgroup's tile for the pairs list[row0 ..] of an expert, at most 16 * RT
-// of them.
-template <int LAYOUT, bool FIRST, int RT, int TYPE, int GROUPED, int kWaves>
+// A workgroup's tile for the first `rows` pairs of the list, at most 16.
+template <int LAYOUT, bool FIRST, int TYPE, int GROUPED, int kWaves>
 __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const uint16_t* scale, const uint16_t* list,
-                                         int rows, int row0, int n0, int k_first, int k_last, float* red,
+                                         int rows, int n0, int k_first, int k_last, float* red,
                                          uint32_t* lds_scale) {
   constexpr int kT = kTerms<FIRST, TYPE>, kL = kLoads<FIRST, TYPE>;
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
@@ -249,27 +262,21 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   const b8 ones = {one, one, one, one, one, one, one, one};
 
   // columns of a product without a row repeat the last one; they are not stored
-  global_halves src[RT];
+  const int pair = list[min(c, rows - 1)];
+  const global_halves src = FIRST ? (global_halves)a.x + (pair / a.top) * a.x_stride
+                                  : (global_halves)a.h + (long)pair * 2 * a.inner_pad;
+  f4 acc[8], sum[2], all[GROUPED ? 8 : 1];
+  sum[0] = sum[1] = f4{0, 0, 0, 0};
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int p = list[min(row0 + 16 * t + c, rows - 1)];
-    src[t] = FIRST ? (global_halves)a.x + (p / a.top) * a.x_stride : (global_halves)a.h + (long)p * 2 * a.inner_pad;
-  }
-  f4 acc[RT][8], sum[RT][2], all[RT][GROUPED ? 8 : 1];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    sum[t][0] = sum[t][1] = f4{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      acc[t][j] = f4{0, 0, 0, 0};
-      if constexpr (GROUPED) all[t][j] = f4{0, 0, 0, 0};
-    }
+  for (int j = 0; j < 8; ++j) {
+    acc[j] = f4{0, 0, 0, 0};
+    if constexpr (GROUPED) all[j] = f4{0, 0, 0, 0};
   }
   uint32_t* lds = reinterpret_cast<uint32_t*>(red) + 1024 * wave;
-  constexpr bool kWide = !FIRST && LAYOUT == SHK_LAYOUT_NN && RT == 1;
+  constexpr bool kWide = !FIRST && LAYOUT == SHK_LAYOUT_NN;
   struct Block {  // 128 K values: the codes of both halves, the activations, and the scales of up to four groups
     uint32_t w[2][16];
-    u4 x[RT][4][kL];
+    u4 x[4][kL];
     uint32_t sc[GROUPED == kSmallGroups ? 4 : 1];  // of two columns: the half lane / 32, columns 2 (lane % 32)
   };
   // Pieces from before `whole` lie inside the codes, the activations and the
@@ -297,11 +304,9 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
         }
     }
   };
-  auto load_rows = [&](int k0, u4 (&x)[RT][4][kL]) {
+  auto load_rows = [&](int k0, u4 (&x)[4][kL]) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) load_x<FIRST, TYPE>(a, src[t], k0 + 32 * q + 8 * g, x[t][q]);
+    for (int q = 0; q < 4; ++q) load_x<FIRST, TYPE>(a, src, k0 + 32 * q + 8 * g, x[q]);
   };
   auto load_end = [&](int k0, Block& b) {  // by way of LDS
     load_scales(k0, std::true_type{}, b);
@@ -309,16 +314,17 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
     load_w_end<LAYOUT, kWide>(s, k0, kWide ? n0 + 4 : n1, lds, b.w[1]);
     if constexpr (FIRST) {  // zeros past the end of x
       uint16_t* h = reinterpret_cast<uint16_t*>(lds) + 8 * lane;
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
 #pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-          const int k = k0 + 32 * (i / 8) + 8 * g + i % 8;
-          h[512 * (i / 8) + i % 8] = k < a.k ? src[t][k] : (uint16_t)0;
-        }
+      for (int q = 0; q < 4; q += 2) {
+        uint16_t v[16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) b.x[t][q][0] = *reinterpret_cast<const u4*>(h + 512 * q);
+        for (int i = 0; i < 16; ++i) v[i] = src[min(k0 + 32 * (q + i / 8) + 8 * g + i % 8, a.k - 1)];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          h[512 * (q + i / 8) + i % 8] = k0 + 32 * (q + i / 8) + 8 * g + i % 8 < a.k ? v[i] : (uint16_t)0;
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) b.x[q][0] = *reinterpret_cast<const u4*>(h + 512 * q);
     } else {
       load_rows(k0, b.x);
     }
@@ -341,13 +347,10 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
       const u2 v = *reinterpret_cast<const u2*>(sc + column<kWide>(kAt, g, r));
       const float f[4] = {bf16_bits_to_f32((uint16_t)v[0]), __uint_as_float(v[0] & 0xFFFF0000u),
                           bf16_bits_to_f32((uint16_t)v[1]), __uint_as_float(v[1] & 0xFFFF0000u)};
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          all[t][4 * kAt + j][r] += f[j] * (acc[t][4 * kAt + j][r] - 24.0f * sum[t][kSum][r]);
-          acc[t][4 * kAt + j][r] = 0.0f;
-        }
+      for (int j = 0; j < 4; ++j) {
+        all[4 * kAt + j][r] += f[j] * (acc[4 * kAt + j][r] - 24.0f * sum[kSum][r]);
+        acc[4 * kAt + j][r] = 0.0f;
+      }
     }
   };
   auto multiply = [&](auto half, Block& b) {
@@ -358,29 +361,23 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
     arrange<LAYOUT>(w);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      b8 xt[RT][kT];
+      b8 xt[kT];
+      terms<FIRST, TYPE>(b.x[q], xt);
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        terms<FIRST, TYPE>(b.x[t][q], xt[t]);
-#pragma unroll
-        for (int i = 0; i < kT; ++i)
-          if (kSum == kAt) sum[t][kSum] = mfma_bf16(ones, xt[t][i], sum[t][kSum]);
-      }
+      for (int i = 0; i < kT; ++i)
+        if (kSum == kAt) sum[kSum] = mfma_bf16(ones, xt[i], sum[kSum]);
       uint32_t o[4];
       step_codes<LAYOUT>(w, q, o);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const b8 v = expand(o[j]);
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int i = 0; i < kT; ++i) acc[t][4 * kAt + j] = mfma_bf16(v, xt[t][i], acc[t][4 * kAt + j]);
+        for (int i = 0; i < kT; ++i) acc[4 * kAt + j] = mfma_bf16(v, xt[i], acc[4 * kAt + j]);
       }
       if constexpr (GROUPED == kSmallGroups) {
         if (q % 2 == 1 || a.group == 32) {
           scale_half(half, 32 * q / a.group);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) sum[t][kAt] = f4{0, 0, 0, 0};
+          sum[kAt] = f4{0, 0, 0, 0};
         }
       }
     }
@@ -391,8 +388,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
       if (k0 + kSuper >= k_last || (k0 + kSuper) % a.group == 0) {
         scale_half(std::integral_constant<int, 0>{}, 0);
         scale_half(std::integral_constant<int, 1>{}, 0);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) sum[t][0] = f4{0, 0, 0, 0};
+        sum[0] = f4{0, 0, 0, 0};
       }
     }
   };
@@ -403,7 +399,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   // were the latest.
   int k0 = k_first;
   if (k0 < whole) {
-    if constexpr (RT == 1 && (kWide || LAYOUT == SHK_LAYOUT_NT)) {
+    if constexpr (kWide || LAYOUT == SHK_LAYOUT_NT) {
       // the next 128 K values are on their way while these are multiplied
       auto load = [&](int k, Block& b) {
         load_scales(k, std::false_type{}, b);
@@ -427,41 +423,26 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
       }
     } else {
       // Each half's codes are on their way while the other half is
-      // multiplied: two sets of 32 loads would pass the 63 that can be
-      // counted, and with RT = 2 the registers.  So are the activations where
-      // they take few registers.
-      constexpr bool kAhead = RT * kL == 1 || (RT * kL == 2 && !GROUPED);
+      // multiplied: two sets of 32 loads would pass the 63 that can be counted.
       Block b;
-      if constexpr (kAhead) load_rows(k0, b.x);
+      load_rows(k0, b.x);
       load_half<LAYOUT>(s, k0, n0, b.w[0]);
-      if constexpr (kAhead) load_half<LAYOUT>(s, k0, n1, b.w[1]);
+      load_half<LAYOUT>(s, k0, n1, b.w[1]);
       for (; k0 < whole; k0 += kSuper) {
         const int next = min(k0 + kSuper, last);
         load_scales(k0, std::false_type{}, b);
-        if constexpr (kAhead) {
-          share_scales(b);
-          multiply(h0, b);
-          u4 x[RT][4][kL];
-          load_rows(next, x);
-          load_half<LAYOUT>(s, next, n0, b.w[0]);
-          multiply(h1, b);
-          finish(k0);
-          load_half<LAYOUT>(s, next, n1, b.w[1]);
+        share_scales(b);
+        multiply(h0, b);
+        u4 x[4][kL];
+        load_rows(next, x);
+        load_half<LAYOUT>(s, next, n0, b.w[0]);
+        multiply(h1, b);
+        finish(k0);
+        load_half<LAYOUT>(s, next, n1, b.w[1]);
 #pragma unroll
-          for (int t = 0; t < RT; ++t)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int i = 0; i < kL; ++i) b.x[t][q][i] = x[t][q][i];
-        } else {
-          load_rows(k0, b.x);
-          load_half<LAYOUT>(s, k0, n1, b.w[1]);
-          share_scales(b);
-          multiply(h0, b);
-          load_half<LAYOUT>(s, next, n0, b.w[0]);
-          multiply(h1, b);
-          finish(k0);
-        }
+          for (int i = 0; i < kL; ++i) b.x[q][i] = x[q][i];
       }
     }
   }
@@ -475,67 +456,63 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   }
   // The waves' sums: lane (g, c) holds token c, columns column(half, g, r)
   // + j.  The second half of the waves hand theirs to the first half.
+  f4 v[8];  // [half][r] over j
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    f4 v[8];  // [half][r] over j
+  for (int half = 0; half < 2; ++half)
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (GROUPED) v[4 * half + r][j] = all[4 * half + j][r];
+        else v[4 * half + r][j] = acc[4 * half + j][r] - 24.0f * sum[0][r];
+      }
+  float* mine = &red[(wave % (kWaves / 2)) * 16 * kPitch + c * kPitch];
+  __syncthreads();
+  if (wave >= kWaves / 2) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (GROUPED) v[4 * half + r][j] = all[t][4 * half + j][r];
-          else v[4 * half + r][j] = acc[t][4 * half + j][r] - 24.0f * sum[t][0][r];
-        }
-    float* mine = &red[(wave % (kWaves / 2)) * 16 * kPitch + c * kPitch];
-    __syncthreads();
-    if (wave >= kWaves / 2) {
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<f4*>(mine + column<kWide>(i / 4, g, i % 4)) = v[i];
+  }
+  __syncthreads();
+  if (wave < kWaves / 2) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *reinterpret_cast<f4*>(mine + column<kWide>(i / 4, g, i % 4)) = v[i];
+    for (int i = 0; i < 8; ++i) {
+      f4* at = reinterpret_cast<f4*>(mine + column<kWide>(i / 4, g, i % 4));
+      *at += v[i];
     }
-    __syncthreads();
-    if (wave < kWaves / 2) {
+  }
+  __syncthreads();
+  if constexpr (FIRST) {
+    for (int i = threadIdx.x; i < rows * kHalf; i += 64 * kWaves) {
+      const int r = i / kHalf, n = i % kHalf, col = n0 + n;
+      if (col >= a.inner_pad) continue;
+      float h = 0.0f;  // up to inner_pad
+      if (col < a.cols) {
+        float up = 0.0f, gate = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f4* at = reinterpret_cast<f4*>(mine + column<kWide>(i / 4, g, i % 4));
-        *at += v[i];
-      }
-    }
-    __syncthreads();
-    const int here = min(rows - row0 - 16 * t, 16);
-    if constexpr (FIRST) {
-      for (int i = threadIdx.x; i < here * kHalf; i += 64 * kWaves) {
-        const int r = i / kHalf, n = i % kHalf, col = n0 + n;
-        if (col >= a.inner_pad) continue;
-        float h = 0.0f;  // up to inner_pad
-        if (col < a.cols) {
-          float up = 0.0f, gate = 0.0f;
-#pragma unroll
-          for (int q = 0; q < kWaves / 2; ++q) {
-            up += red[q * 16 * kPitch + r * kPitch + n];
-            gate += red[q * 16 * kPitch + r * kPitch + kHalf + n];
-          }
-          if constexpr (!GROUPED) up *= load_bf16(scale + col), gate *= load_bf16(scale + a.cols + col);
-          h = up * (gate / (1.0f + __expf(-gate)));
+        for (int q = 0; q < kWaves / 2; ++q) {
+          up += red[q * 16 * kPitch + r * kPitch + n];
+          gate += red[q * 16 * kPitch + r * kPitch + kHalf + n];
         }
-        // place 2 i + u of an eight holds its element i + 4 u
-        const int at = (col & ~7) | (2 * (col & 3) + ((col >> 2) & 1));
-        const uint32_t hi = f32_to_bf16_rne(h);
-        uint16_t* dst = a.h + (long)list[row0 + 16 * t + r] * 2 * a.inner_pad + at;
-        dst[0] = (uint16_t)hi;
-        dst[a.inner_pad] = (uint16_t)f32_to_bf16_rne(h - bf16_bits_to_f32((uint16_t)hi));
+        if constexpr (!GROUPED) up *= load_bf16(scale + col), gate *= load_bf16(scale + a.cols + col);
+        h = up * (gate / (1.0f + __expf(-gate)));
       }
-    } else {
-      for (int i = threadIdx.x; i < here * 2 * kHalf; i += 64 * kWaves) {
-        const int r = i / (2 * kHalf), n = i % (2 * kHalf), col = n0 + n;
-        if (col >= a.cols) continue;
-        float v2 = 0.0f;
+      // place 2 i + u of an eight holds its element i + 4 u
+      const int at = (col & ~7) | (2 * (col & 3) + ((col >> 2) & 1));
+      const uint32_t hi = f32_to_bf16_rne(h);
+      uint16_t* dst = a.h + (long)list[r] * 2 * a.inner_pad + at;
+      dst[0] = (uint16_t)hi;
+      dst[a.inner_pad] = (uint16_t)f32_to_bf16_rne(h - bf16_bits_to_f32((uint16_t)hi));
+    }
+  } else {
+    for (int i = threadIdx.x; i < rows * 2 * kHalf; i += 64 * kWaves) {
+      const int r = i / (2 * kHalf), n = i % (2 * kHalf), col = n0 + n;
+      if (col >= a.cols) continue;
+      float v2 = 0.0f;
 #pragma unroll
-        for (int q = 0; q < kWaves / 2; ++q) v2 += red[q * 16 * kPitch + r * kPitch + n];
-        if constexpr (!GROUPED) v2 *= load_bf16(scale + col);
-        __hip_atomic_store(a.part + (long)list[row0 + 16 * t + r] * a.hidden + col, v2, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-      }
+      for (int q = 0; q < kWaves / 2; ++q) v2 += red[q * 16 * kPitch + r * kPitch + n];
+      if constexpr (!GROUPED) v2 *= load_bf16(scale + col);
+      __hip_atomic_store(a.part + (long)list[r] * a.hidden + col, v2, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
     }
   }
 }
@@ -567,16 +544,15 @@ __global__ __launch_bounds__(256) void moe_join(const MoeArgs a) {
 
 // One product of the layer.  FIRST: up and gate, h = up * silu(gate) to a.h,
 // the halves of the tile being the same 64 columns of each; otherwise down,
-// 128 columns, to a.part.  RT: the most row
-// tiles of 16 tokens a pass over the codes serves.
-template <int LAYOUT, bool FIRST, int RT, int TYPE, int GROUPED, int kWaves>
+// 128 columns, to a.part.
+template <int LAYOUT, bool FIRST, int TYPE, int GROUPED, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   constexpr int kStep = FIRST ? kHalf : 2 * kHalf;  // columns from one workgroup to the next
   // the waves' sums, and before them 1024 dwords a wave for what ends in a piece
   __shared__ __align__(16) float red[kWaves / 2 * 16 * kPitch];
   static_assert(sizeof(red) >= kWaves * 4096, "room for the pieces that end");
   __shared__ uint32_t lds_scale[GROUPED ? kWaves * 256 : 1];  // a wave's four groups of 128 scales
-  __shared__ uint16_t list[kMostPairs];
+  __shared__ uint16_t list[kRows];
   __shared__ int16_t id[kMostPairs];
   __shared__ int count[kMostExperts];
   const int lane = threadIdx.x & 63;
@@ -593,23 +569,27 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
     for (int i = blockIdx.x * 64 * kWaves + threadIdx.x; i < a.tiles; i += gridDim.x * 64 * kWaves) a.arrived[i] = 0;
   if (tile * kStep >= (FIRST ? a.inner_pad : a.cols)) return;
 
-  // the blockIdx.y-th expert that is hit, and its pairs in order
-  int expert = -1, rank = blockIdx.y, rows = 0, hits = 0;  // hits: experts that are hit
+  // The pairs of each expert that is hit are dealt out in order, kRows at a
+  // time: this workgroup's are the blockIdx.y-th.  `row0` counts the expert's
+  // pairs before them, `shares` all such parts.
+  int expert = -1, rank = blockIdx.y, row0 = 0, rows = 0, shares = 0;
   if (pairs <= 64) {
     // experts in the order of their first pairs, all in a wave's registers
     const int mine = lane < pairs ? id_of(a, lane) : -1;
     unsigned long open = __ballot(mine >= 0), same = 0;
-    for (; open != 0; ++hits) {
+    while (open != 0) {
       const int e = __shfl(mine, __builtin_ctzll(open), 64);
       const unsigned long all = __ballot(mine == e);
-      if (hits == rank) expert = e, same = all;
+      const int before = rank - shares, here = (__popcll(all) + kRows - 1) / kRows;
+      if (before >= 0 && before < here) expert = e, same = all, row0 = kRows * before;
+      shares += here;
       open &= ~all;
     }
-    rows = __popcll(same);
-    if (wave == 0 && expert >= 0 && mine == expert) list[__popcll(same & ((1ul << lane) - 1))] = (uint16_t)lane;
+    rows = __popcll(same) - row0;
+    const int at = __popcll(same & ((1ul << lane) - 1)) - row0;
+    if (wave == 0 && expert >= 0 && mine == expert && at >= 0 && at < kRows) list[at] = (uint16_t)lane;
   } else {
-    // counted in LDS, those with more than 16 rows first: their workgroups
-    // take longest
+    // counted in LDS
     for (int e = threadIdx.x; e < a.experts; e += 64 * kWaves) count[e] = 0;
     __syncthreads();
     for (int p = threadIdx.x; p < pairs; p += 64 * kWaves) {
@@ -618,34 +598,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
       if (e >= 0) atomicAdd(&count[e], 1);
     }
     __syncthreads();
-    for (int many = 1; many >= 0; --many) {
-      for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int n = e0 + lane < a.experts ? count[e0 + lane] : 0;
-        unsigned long hit = __ballot(n > 0 && (n > 16) == (many != 0));
-        const int here = __popcll(hit);
-        if (rank >= hits && rank < hits + here) {
-          for (int i = hits; i < rank; ++i) hit &= hit - 1;
-          expert = e0 + __builtin_ctzll(hit);
-        }
-        hits += here;
+    for (int e0 = 0; e0 < a.experts; e0 += 64) {
+      const int n = e0 + lane < a.experts ? count[e0 + lane] : 0, here = (n + kRows - 1) / kRows;
+      int upto = here;  // with the lanes before
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(upto, d, 64);
+        upto += lane >= d ? v : 0;
       }
+      const int before = rank - shares - (upto - here);
+      const unsigned long at = __ballot(before >= 0 && before < here);
+      if (at != 0) {
+        const int l = __builtin_ctzll(at);
+        expert = e0 + l, row0 = kRows * __shfl(before, l, 64), rows = __shfl(n, l, 64) - row0;
+      }
+      shares += __shfl(upto, 63, 64);
     }
-    rows = expert < 0 ? 0 : count[expert];
     if (wave == 0 && expert >= 0) {
-      int at = 0;
-      for (int p0 = 0; p0 < pairs; p0 += 64) {
+      int at = -row0;
+      for (int p0 = 0; p0 < pairs && at < kRows; p0 += 64) {
         const bool mine = p0 + lane < pairs && id[p0 + lane] == expert;
         const unsigned long all = __ballot(mine);
-        if (mine) list[at + __popcll(all & ((1ul << lane) - 1))] = (uint16_t)(p0 + lane);
+        const int to = at + __popcll(all & ((1ul << lane) - 1));
+        if (mine && to >= 0 && to < kRows) list[to] = (uint16_t)(p0 + lane);
         at += __popcll(all);
       }
     }
   }
   expert = __builtin_amdgcn_readfirstlane(expert);
-  rows = __builtin_amdgcn_readfirstlane(rows);
-  hits = __builtin_amdgcn_readfirstlane(hits);
+  rows = __builtin_amdgcn_readfirstlane(min(rows, kRows));
+  shares = __builtin_amdgcn_readfirstlane(shares);
   if constexpr (!FIRST)
-    if (a.joined && hits == 0 && blockIdx.y == 0) join_tile<kWaves>(a, tile * kStep);  // no token asks for any expert
+    if (a.joined && shares == 0 && blockIdx.y == 0) join_tile<kWaves>(a, tile * kStep);  // no token asks for any expert
   if (expert < 0) return;  // the same for all threads
   __syncthreads();
 
@@ -660,15 +644,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   const int units = (a.k + unit - 1) / unit, each = (units + kWaves - 1) / kWaves;
   const int k_first = min(a.k, wave * each * unit), k_last = min(a.k, (wave + 1) * each * unit);
 
-  for (int row0 = 0; row0 < rows; row0 += 16 * RT) {
-    if (row0 > 0) __syncthreads();  // red has been read
-    if (RT == 1 || rows - row0 <= 16)
-      moe_rows<LAYOUT, FIRST, 1, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, row0, n0, k_first, k_last, red,
-                                                        lds_scale + 256 * wave);
-    else
-      moe_rows<LAYOUT, FIRST, RT, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, row0, n0, k_first, k_last, red,
-                                                        lds_scale + 256 * wave);
-  }
+  moe_rows<LAYOUT, FIRST, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, n0, k_first, k_last, red,
+                                                 lds_scale + 256 * wave);
   if (!FIRST && a.joined) {
     // The last workgroup of a tile adds up its pairs.  Results are written and
     // read with device scope, which the XCDs' caches see without being
@@ -677,48 +654,45 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0)
-      last = __hip_atomic_fetch_add(a.arrived + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == hits - 1;
+      last = __hip_atomic_fetch_add(a.arrived + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == shares - 1;
     __syncthreads();
     if (last) join_tile<kWaves>(a, tile * kStep);
   }
 }
 
 template <int LAYOUT, bool FIRST, int TYPE, int GROUPED>
-void launch_rt(const MoeArgs& a, dim3 grid, hipStream_t s) {
+void launch_waves(const MoeArgs& a, dim3 grid, hipStream_t s) {
   // A workgroup's waves share K.  Few workgroups (at most one on each of the
-  // 256 CUs): eight, the shortest way through.  Otherwise every wave's start
-  // and end count, and a wave should have about 1024 K values: two waves, or
-  // four for a long K, whose workgroups would otherwise be few and uneven.
+  // 256 CUs): eight, the shortest way through.  Many: every wave's start and
+  // end count, and a wave should have about 1024 K values: two waves.  Four in
+  // between, and for a long K, whose workgroups would otherwise be uneven.
   // Measured, us for up and gate / down with 2, 4, 8 waves: 41 experts of
   // 2048 x 1408 36 / 27, 43 / 30, 60 / 39; 14 of 4096 x 11008 146 / 117, 145 / 106.
-  if (a.tokens <= 16) {
-    if (grid.x * grid.y <= 256)
-      hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 1, TYPE, GROUPED, 8>), grid, dim3(512), 0, s, a);
-    else if (a.k < 4096)
-      hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 1, TYPE, GROUPED, 2>), grid, dim3(128), 0, s, a);
-    else
-      hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 1, TYPE, GROUPED, 4>), grid, dim3(256), 0, s, a);
-  } else if (a.k < 4096) {
-    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 2, TYPE, GROUPED, 2>), grid, dim3(128), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, 2, TYPE, GROUPED, 4>), grid, dim3(256), 0, s, a);
-  }
+  // The layer of 32 pairs of 16 experts of 2048 x 1408 (up to 384 workgroups)
+  // with 2 and 4 waves: 37, 29.
+  if (grid.x * grid.y <= 256)
+    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 8>), grid, dim3(512), 0, s, a);
+  else if (a.k < 4096 && grid.x * grid.y > 1024)
+    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 2>), grid, dim3(128), 0, s, a);
+  else
+    hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 4>), grid, dim3(256), 0, s, a);
 }
 
 template <int LAYOUT, bool FIRST, int TYPE>
 hipError_t launch_product(const MoeArgs& a, unsigned columns, unsigned hit, hipStream_t s) {
   constexpr unsigned kStep = FIRST ? kHalf : 2 * kHalf;
   const dim3 grid(((columns + kStep - 1) / kStep + 7) / 8 * 8, hit);
-  if (a.group >= kSuper) launch_rt<LAYOUT, FIRST, TYPE, kLargeGroups>(a, grid, s);
-  else if (a.group) launch_rt<LAYOUT, FIRST, TYPE, kSmallGroups>(a, grid, s);
-  else launch_rt<LAYOUT, FIRST, TYPE, 0>(a, grid, s);
+  if (a.group >= kSuper) launch_waves<LAYOUT, FIRST, TYPE, kLargeGroups>(a, grid, s);
+  else if (a.group) launch_waves<LAYOUT, FIRST, TYPE, kSmallGroups>(a, grid, s);
+  else launch_waves<LAYOUT, FIRST, TYPE, 0>(a, grid, s);
   return hipGetLastError();
 }
 
 hipError_t launch_layer(const shk_moe& x, MoeArgs a, hipStream_t s) {
   constexpr int LAYOUT = SHK_LAYOUT;
   // with no pairs the down product still writes the zeros
-  const unsigned hit = (unsigned)std::max(1L, (long)std::min(x.tokens * x.top, x.experts));
+  const long pairs = x.tokens * x.top, most = std::min(pairs, (long)x.experts);
+  const unsigned hit = (unsigned)std::max(1L, most + (pairs - most) / 16);
   a.w = static_cast<const uint8_t*>(x.up_gate);
   a.scale = static_cast<const uint16_t*>(x.up_gate_scale);
   a.k = a.hidden, a.k_packed = (a.hidden + 1) / 2, a.cols = a.inner;
