@@ -221,6 +221,16 @@ __device__ __forceinline__ void load_x(const MoeArgs& a, global_halves row, int 
   }
 }
 
+// Eight 16-bit values without the first n (none for n <= 0), zeros behind.
+__device__ __forceinline__ u4 drop(u4 v, int n) {
+  n = max(n, 0);
+  if (n & 1) v = u4{perm_b32(v[1], v[0], 0x05040302u), perm_b32(v[2], v[1], 0x05040302u),
+                    perm_b32(v[3], v[2], 0x05040302u), v[3] >> 16};
+  if (n & 2) v = u4{v[1], v[2], v[3], 0};
+  if (n & 4) v = u4{v[2], v[3], 0, 0};
+  return n < 8 ? v : u4{0, 0, 0, 0};
+}
+
 // As bf16 terms in the order 0 4 1 5 2 6 3 7.
 template <bool FIRST, int TYPE>
 __device__ __forceinline__ void terms(const u4 (&u)[kLoads<FIRST, TYPE>], b8 (&t)[kTerms<FIRST, TYPE>]) {
@@ -308,23 +318,31 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
 #pragma unroll
     for (int q = 0; q < 4; ++q) load_x<FIRST, TYPE>(a, src, k0 + 32 * q + 8 * g, x[q]);
   };
-  auto load_end = [&](int k0, Block& b) {  // by way of LDS
+  auto load_end = [&](int k0, Block& b) {
     load_scales(k0, std::true_type{}, b);
-    load_w_end<LAYOUT, kWide>(s, k0, n0, lds, b.w[0]);
-    load_w_end<LAYOUT, kWide>(s, k0, kWide ? n0 + 4 : n1, lds, b.w[1]);
+    if (inside<LAYOUT>(s, k0, n0) && inside<LAYOUT>(s, k0, n1)) {
+      load_w<LAYOUT, kWide>(s, k0, n0, n1, b.w);
+    } else {
+      load_w_end<LAYOUT, kWide>(s, k0, n0, lds, b.w[0]);
+      load_w_end<LAYOUT, kWide>(s, k0, kWide ? n0 + 4 : n1, lds, b.w[1]);
+    }
     if constexpr (FIRST) {  // zeros past the end of x
-      uint16_t* h = reinterpret_cast<uint16_t*>(lds) + 8 * lane;
+      if (a.k >= 8) {
+        // the last eight values there are, shifted to where they would be
+#pragma unroll
+        for (int q = 0; q < 4; ++q) load_x<FIRST, TYPE>(a, src, min(k0 + 32 * q + 8 * g, a.k - 8), b.x[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) b.x[q][0] = drop(b.x[q][0], k0 + 32 * q + 8 * g - (a.k - 8));
+      } else {
+        uint16_t* h = reinterpret_cast<uint16_t*>(lds) + 8 * lane;
 #pragma unroll 1
-      for (int q = 0; q < 4; q += 2) {
-        uint16_t v[16];
+        for (int i = 0; i < 32; ++i) {
+          const int k = k0 + 32 * (i / 8) + 8 * g + i % 8;
+          h[512 * (i / 8) + i % 8] = k < a.k ? src[k] : (uint16_t)0;
+        }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = src[min(k0 + 32 * (q + i / 8) + 8 * g + i % 8, a.k - 1)];
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          h[512 * (q + i / 8) + i % 8] = k0 + 32 * (q + i / 8) + 8 * g + i % 8 < a.k ? v[i] : (uint16_t)0;
+        for (int q = 0; q < 4; ++q) b.x[q][0] = *reinterpret_cast<const u4*>(h + 512 * q);
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) b.x[q][0] = *reinterpret_cast<const u4*>(h + 512 * q);
     } else {
       load_rows(k0, b.x);
     }

@@ -5,13 +5,15 @@ against the eager one."""
 from __future__ import annotations
 
 import importlib.util
+from pathlib import Path
 
 import pytest
-import torch
 
-import _decode_ref as ref
-from conftest import ROOT
+torch = pytest.importorskip("torch")
 
+from tests import _decode_ref as ref  # noqa: E402
+
+ROOT = Path(__file__).resolve().parents[1]
 pytestmark = pytest.mark.gpu
 
 SMALL = dict(hidden=256, heads=8, kv_heads=2, head_dim=64, experts=4, inner=96, top=2, batch=16, most=64, page=16)

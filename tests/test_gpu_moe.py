@@ -76,6 +76,20 @@ def test_odd_sizes(layout, group, hidden, inner, device):
         _check(_run(case, device), case)
 
 
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+def test_every_end_of_a_row(layout, device):
+    """hidden takes every residue of eight values; rows past x's are not read."""
+    for hidden in range(137, 153):
+        case = _case(stable_seed("end", layout, hidden), 5, 3, 2, hidden, 70, layout=layout, dtype="f16")
+        wide = torch.full((5, hidden + 3), math.nan, dtype=torch.float16)
+        wide[:, :hidden] = case[0]
+        case[0] = wide[:, :hidden]
+        x = wide.to(device)[:, :hidden]
+        d = [t.to(device) for t in case[1:7]]
+        got = shk.moe_swiglu_int4(x, *d[:4], up_gate_scale=d[4], down_scale=d[5], layout=shk.GemmLayout(layout))
+        _check(got, case)
+
+
 def test_experts_with_many_rows_and_none(device):
     """All tokens through one expert of several, a token twice through the
     same one, and most experts idle."""
