@@ -547,7 +547,7 @@ int amd_strix_halo_kernels_kv_attention(int device_index, uintptr_t stream, cons
  * bf16: group 0 up_gate_scale [experts, 2 * inner], down_scale [experts,
  * hidden]; group 32, 64, 128 or 256 [experts, ceil(K/group), columns].
  * Ids outside [0, experts) add nothing.  At most 64 tokens, 1024 pairs and
- * 1024 experts.  x rows are contiguous (x_stride in elements), out [tokens,
+ * 1024 experts; up_gate and down of at least 4 bytes each.  x rows are contiguous (x_stride in elements), out [tokens,
  * hidden] is contiguous, both of one type.  workspace: at least
  * amd_strix_halo_kernels_moe_workspace bytes, on 16 bytes, not read before it
  * is written. */

@@ -86,7 +86,7 @@ int check_moe(const shk_moe* a) {
     return capi_fail("the scale group is 0, 32, 64, 128 or 256; got " + std::to_string(a->group));
   if (a->tokens < 0 || a->tokens > 64)
     return capi_fail("at most 64 tokens a call; got " + std::to_string(a->tokens));
-  if (a->top < 0 || a->tokens * a->top > 1024) return capi_fail("at most 1024 (token, expert) pairs a call");
+  if (a->top < 0 || (a->tokens > 0 && a->top > 1024 / a->tokens)) return capi_fail("at most 1024 (token, expert) pairs a call");
   if (a->experts < 1 || a->experts > 1024) return capi_fail("1 to 1024 experts; got " + std::to_string(a->experts));
   if (a->hidden < 1 || a->inner < 1 || a->hidden > (1 << 20) || a->inner > (1 << 20))
     return capi_fail("hidden and inner must be from 1 to 1048576");

@@ -5,7 +5,14 @@
 // Q = 7 or 127.  Both kernels are one pass over memory: each value and each
 // code is touched once, by the lane that owns 8 consecutive values of a row
 // (16 bytes of a 2-byte type in, 4 or 8 bytes of codes out); head_dim / 8
-// lanes share a row and exchange its maximum.
+// lanes share a row and exchange its maximum.  Keys and values go side by side,
+// so a lane has two rows on their way (write) or four (read).
+//
+// Bound by memory.  Measured with 8 heads of 128, bf16: 8191 tokens to int8,
+// 50.7 MB, 14.0 us (3.6 TB/s; about 4 us of it are the launch's start and end,
+// which is all that a few tokens take); 65536 tokens from int4, 338 MB of which
+// 268 are stores, 88 us (3.9 TB/s, where a copy of 2 GiB runs at 4.9).  Stores
+// past the caches: 114 -> 88 us.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

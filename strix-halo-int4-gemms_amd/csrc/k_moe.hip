@@ -14,6 +14,13 @@
 // workgroups: 253 us instead of 240 for 122 pairs of 16 experts of 4096 x
 // 11008, 90 instead of 53 for 306 pairs of 16 experts of 320 x 4320.)
 //
+// Measured: 61 tokens over 16 experts (14 are hit) of 4096 x 11008, 949 MB of
+// codes: up and gate 151 us, down 85, 4.0 TB/s together; the same loads without
+// the products take 110 and 60.  16 tokens over 64 experts (41 hit) of 2048 x
+// 1408 in groups of 128: 35 and 26 us for 183 MB, where a wave has eight pieces
+// and its start (the pairs of its expert) and end (the sums of the waves) are
+// half of it.  One token through two experts: 9 and 11 us, all latency.
+//
 // Products are v_mfma_f32_16x16x32_bf16 with the weights in the rows and the
 // tokens in the columns.  A code v enters as v + 24, which one shift and one
 // and-or make of two nibbles: with n = v + 8 (the sign bit flipped), bf16's
