@@ -269,7 +269,7 @@ __device__ __forceinline__ int column(int half, int g, int r) {
 // A workgroup's tile for the first `rows` pairs of the list, at most 16.
 template <int LAYOUT, bool FIRST, int TYPE, int GROUPED, int kWaves>
 __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const uint16_t* scale, const uint16_t* list,
-                                         int rows, int n0, int k_first, int k_last, float* red,
+                                         int rows, int n0, int k_first, int k_last, int k_step, float* red,
                                          uint32_t* lds_scale) {
   constexpr int kT = kTerms<FIRST, TYPE>, kL = kLoads<FIRST, TYPE>;
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
@@ -307,7 +307,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
   };
   int whole = FIRST ? min(k_last, a.k - kSuper + 1) : k_last;
   while (whole > k_first && !fits(whole - 1)) whole -= kSuper;
-  const int last = k_first + (max(whole - k_first, 1) - 1) / kSuper * kSuper;  // the last of them
+  const int last = k_first + (max(whole - k_first, 1) - 1) / k_step * k_step;  // the last of them
   auto load_scales = [&](int k0, auto end, Block& b) {
     if constexpr (GROUPED) {
 #pragma unroll
@@ -436,14 +436,14 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
         multiply(h0, b);
         multiply(h1, b);
         finish(k0);
-        return (k0 += kSuper) < whole;
+        return (k0 += k_step) < whole;
       };
       Block b0, b1;
       load(k0, b0);
       while (true) {
-        load(min(k0 + kSuper, last), b1);
+        load(min(k0 + k_step, last), b1);
         if (!use(b0)) break;
-        load(min(k0 + kSuper, last), b0);
+        load(min(k0 + k_step, last), b0);
         if (!use(b1)) break;
       }
     } else {
@@ -453,8 +453,8 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
       load_rows(k0, b.x);
       load_half<LAYOUT>(s, k0, n0, b.w[0]);
       load_half<LAYOUT>(s, k0, n1, b.w[1]);
-      for (; k0 < whole; k0 += kSuper) {
-        const int next = min(k0 + kSuper, last);
+      for (; k0 < whole; k0 += k_step) {
+        const int next = min(k0 + k_step, last);
         load_scales(k0, std::false_type{}, b);
         share_scales(b);
         multiply(h0, b);
@@ -471,7 +471,7 @@ __device__ __forceinline__ void moe_rows(const MoeArgs& a, const Codes& s, const
       }
     }
   }
-  for (; k0 < k_last; k0 += kSuper) {
+  for (; k0 < k_last; k0 += k_step) {
     Block b;
     load_end(k0, b);
     share_scales(b);
@@ -664,12 +664,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   const int n0 = tile * kStep;
   const uint16_t* scale = a.scale + (long)expert * (GROUPED ? a.groups : 1) * s.total;
 
-  // this wave's K: whole pieces and whole scale groups
+  // This wave's K: whole pieces and whole scale groups.  A piece is half a
+  // cache line of NT's rows: there the waves take pieces in turn, so that both
+  // halves are asked for at about the same time.
+  const bool turns = LAYOUT == SHK_LAYOUT_NT && a.group <= kSuper;
   const int unit = GROUPED ? max(a.group, kSuper) : kSuper;
   const int units = (a.k + unit - 1) / unit, each = (units + kWaves - 1) / kWaves;
-  const int k_first = min(a.k, wave * each * unit), k_last = min(a.k, (wave + 1) * each * unit);
+  const int k_first = turns ? wave * kSuper : min(a.k, wave * each * unit);
+  const int k_last = turns ? a.k : min(a.k, (wave + 1) * each * unit), k_step = turns ? kWaves * kSuper : kSuper;
 
-  moe_rows<LAYOUT, FIRST, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, n0, k_first, k_last, red,
+  moe_rows<LAYOUT, FIRST, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, n0, k_first, k_last, k_step, red,
                                                  lds_scale + 256 * wave);
   if (!FIRST && a.joined) {
     // The last workgroup of a tile adds up its pairs.  Results are written and
