@@ -1,8 +1,8 @@
 // Attention of each sequence's newest tokens over the quantized cache
 // (shk_kvattn.h has the mathematics of a step).
 //
-// kv_stream_kernel serves a sequence's own tokens (and a shared prefix with
-// few query rows).  A workgroup is one key head and up to 16 * RT query rows;
+// kv_stream_kernel serves a sequence's own tokens (and a shared prefix with up
+// to 64 query rows over the batch).  A workgroup is one key head and up to 16 * RT query rows;
 // its four waves take every fourth 64 tokens, each from memory to its own
 // registers, and are joined through LDS.  The tokens of all sequences are
 // dealt out evenly: in pieces of 256, a workgroup gets the same number of
@@ -600,8 +600,17 @@ Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
   const bool wide = c.head_dim == 256;  // two row tiles of 256 columns would not fit the registers
   Plan p{};
   const bool prefix = a.prefix_length > 0;
-  p.prefix_kernel = prefix && all > (wide ? 16 : 32);
-  p.rt = wide || (rows <= 16 && (!prefix || p.prefix_kernel || all <= 16)) ? 1 : 2;
+  // The prefix's own kernel widens a token once for up to 128 rows, the
+  // streaming one once for 16 * rt but without barriers.  Us with the one / the
+  // other after 2000 and 32768 shared tokens, int4: 64 rows of 128 20 / 17 and
+  // 45 / 41, 96 rows 22 / 22 and 50 / 63; of 256 23 / 21 and 56 / 58, 25 / 27 and
+  // 74 / 93; 256 rows of 128 after 65536 tokens 121 / 145.
+  p.prefix_kernel = prefix && all > 64;
+  // Two row tiles read a sequence's tokens once for 32 rows: 24 sequences of up
+  // to 8000 tokens with 32 rows 61 us instead of 68.  Rows that are few in a
+  // sequence but many over the batch take two tiles for a short prefix too
+  // long (64 rows: 19 us, with one tile 17; a long one 38 and 41).
+  p.rt = wide || rows <= 16 ? 1 : 2;
   p.prefix_rt = wide ? 1 : 2;
   p.own_tiles = (int)cdiv(rows, 16 * p.rt);
   p.direct = !prefix && tokens <= kPiece;
