@@ -607,9 +607,9 @@ Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
   // 74 / 93; 256 rows of 128 after 65536 tokens 121 / 145.
   p.prefix_kernel = prefix && all > 64;
   // Two row tiles read a sequence's tokens once for 32 rows: 24 sequences of up
-  // to 8000 tokens with 32 rows 61 us instead of 68.  Rows that are few in a
-  // sequence but many over the batch take two tiles for a short prefix too
-  // long (64 rows: 19 us, with one tile 17; a long one 38 and 41).
+  // to 8000 tokens with 32 rows 61 us instead of 68.  Where only the batch has
+  // more than 16 rows, two tiles for its prefix gain after a long one (64 rows
+  // 38 us, with one tile 41) what they lose after a short one (19 and 17).
   p.rt = wide || rows <= 16 ? 1 : 2;
   p.prefix_rt = wide ? 1 : 2;
   p.own_tiles = (int)cdiv(rows, 16 * p.rt);
@@ -620,7 +620,7 @@ Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
                                                        a.batch * cdiv(tokens, kPiece)));
   if (prefix) {
     p.prefix_tiles = (int)cdiv(all, p.prefix_kernel ? 64 * p.prefix_rt : 16 * p.rt);
-    p.prefix_splits = (int)std::max(1L, std::min(cdiv(p.prefix_kernel ? 512 : want, c.kv_heads * p.prefix_tiles),
+    p.prefix_splits = (int)std::max(1L, std::min(cdiv(want, c.kv_heads * p.prefix_tiles),
                                                  cdiv(a.prefix_length, kPiece)));
   }
   return p;
