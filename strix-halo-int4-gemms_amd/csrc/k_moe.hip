@@ -19,7 +19,7 @@
 // the products take 110 and 60.  16 tokens over 64 experts (41 hit) of 2048 x
 // 1408 in groups of 128: 35 and 26 us for 183 MB, where a wave has eight pieces
 // and its start (the pairs of its expert) and end (the sums of the waves) are
-// half of it.  One token through two experts: 9 and 11 us, all latency.
+// half of it.  One token through two experts: 10 us each, all latency.
 //
 // Products are v_mfma_f32_16x16x32_bf16 with the weights in the rows and the
 // tokens in the columns.  A code v enters as v + 24, which one shift and one
