@@ -88,11 +88,26 @@ class KVCache:
             raise ValueError(f"page_size must be a power of two from 16 to 1024; got {page_size}")
         if not 1 <= heads <= 65535 or pages < 1:
             raise ValueError(f"the cache needs at least one page and 1 to 65535 heads; got {pages} and {heads}")
-        native = _CACHE.pack(codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(),
-                             self.value_scales.data_ptr(), pages, heads, page_size, head_dim, bits)
+        at = self._addresses()
+        packed = _CACHE.pack(*at, pages, heads, page_size, head_dim, bits)
         for name, value in (("pages", pages), ("kv_heads", heads), ("page_size", page_size), ("head_dim", head_dim),
-                            ("bits", bits), ("device", codes.device), ("_native", native), ("_workspaces", {})):
+                            ("bits", bits), ("device", codes.device), ("_packed", (at, packed)), ("_workspaces", {})):
             object.__setattr__(self, name, value)
+
+    def __reduce__(self) -> Any:
+        # copies and loaded caches are made of their own tensors
+        return KVCache, (self.key_codes, self.value_codes, self.key_scales, self.value_scales)
+
+    def _addresses(self) -> tuple[int, int, int, int]:
+        return (self.key_codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(),
+                self.value_scales.data_ptr())
+
+    @property
+    def _native(self) -> bytes:
+        """shk_kv_cache, at the addresses that the tensors have now."""
+        if self._packed[0] != self._addresses():
+            self.__post_init__()  # a tensor was given other memory: all checks again
+        return self._packed[1]
 
 
 def new_kv_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, bits: int = 4,
@@ -156,6 +171,7 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
     others are distinct.  One pass over memory, no copy of the inputs.
     """
     torch = _torch()
+    native = cache._native  # first: the sizes that follow are the tensors' own
     _check_devices(cache, keys=keys, values=values, slots=slots)
     if stream is not None:
         with _on_stream(torch, keys, stream):
@@ -174,8 +190,8 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
     if tokens == 0:
         return
     lib = _verified_library()
-    _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, None),
-                                                    cache._native, _rows(keys, values, slots, kind, tokens)))
+    _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, None), native,
+                                                    _rows(keys, values, slots, kind, tokens)))
 
 
 def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any | None = None) -> tuple[Any, Any]:
@@ -183,6 +199,7 @@ def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any 
     (bf16, the default, f16 or f32): two [tokens, kv_heads, head_dim]
     tensors.  Slots outside the cache give NaN."""
     torch = _torch()
+    native = cache._native  # first: the sizes that follow are the tensors' own
     _check_devices(cache, slots=slots)
     if stream is not None:
         with _on_stream(torch, slots, stream):
@@ -196,8 +213,8 @@ def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any 
     values = torch.empty_like(keys)
     if tokens:
         lib = _verified_library()
-        _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, None),
-                                                       cache._native, _rows(keys, values, slots, kind, tokens)))
+        _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, None), native,
+                                                       _rows(keys, values, slots, kind, tokens)))
     return keys, values
 
 
@@ -236,6 +253,7 @@ def kv_cache_attention(
     softmax and the sums are f32; products take the codes as they are.
     """
     torch = _torch()
+    native = cache._native  # first: the sizes that follow are the tensors' own
     _check_devices(cache, q=q, page_table=page_table, lengths=lengths, prefix_pages=prefix_pages, out=out)
     if stream is not None:
         with _on_stream(torch, q, stream):
@@ -305,12 +323,12 @@ def kv_cache_attention(
         key = (batch, queries, heads, table_pages, prefix_length)
         nbytes = cache._workspaces.get(key)
         if nbytes is None:
-            nbytes = lib.amd_strix_halo_kernels_kv_attention_workspace(cache._native, args(None, 0))
+            nbytes = lib.amd_strix_halo_kernels_kv_attention_workspace(native, args(None, 0))
             if nbytes < 0:
                 _check(lib, 1)
             if len(cache._workspaces) < 4096:
                 cache._workspaces[key] = nbytes
         work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, None),
-                                                            cache._native, args(work, nbytes)))
+        _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, None), native,
+                                                            args(work, nbytes)))
     return (out, lse) if return_lse else out

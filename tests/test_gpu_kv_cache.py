@@ -9,6 +9,7 @@ places shows.
 
 from __future__ import annotations
 
+import copy
 import math
 
 import pytest
@@ -130,6 +131,20 @@ def test_slots_outside_the_cache(device):
     assert int((cache.key_scales != 0).sum()) == 2 and int((cache.value_codes != 0).any(dim=-1).sum()) == 2
     got = shk.kv_cache_read(cache, slots)[0]
     assert torch.isnan(got[[0, 2, 4]]).all() and torch.equal(got[[1, 3]], x[:2])
+
+
+def test_a_copy_is_written_alone(device):
+    """A prompt's cache is copied, and both go on differently."""
+    cache = shk.new_kv_cache(2, 16, 1, 64, bits=8, device=device)
+    x = torch.ones((3, 1, 64), device=device, dtype=torch.bfloat16)
+    slots = torch.arange(3, device=device)
+    shk.kv_cache_write(cache, x, x, slots)
+    fork = copy.deepcopy(cache)
+    shk.kv_cache_write(fork, 2 * x[:1], 2 * x[:1], slots[:1])
+    shk.kv_cache_write(cache, 3 * x[1:2], 3 * x[1:2], slots[1:2])
+    for c, want in ((cache, [1, 3, 1]), (fork, [2, 1, 1])):
+        keys, _ = shk.kv_cache_read(c, slots)
+        assert keys[:, 0].amax(dim=-1).tolist() == keys[:, 0].amin(dim=-1).tolist() == want
 
 
 def test_no_tokens(device):

@@ -3,6 +3,10 @@ Python argument checks, and the C ABI's own before it touches the device."""
 
 from __future__ import annotations
 
+import copy
+import io
+import pickle
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -52,6 +56,46 @@ def test_cache_tensor_refusals():
     ):
         with pytest.raises(ValueError, match=match):
             shk.KVCache(**{**parts, name: bad})
+
+
+PARTS = ("key_codes", "value_codes", "key_scales", "value_scales")
+
+
+def _saved(c):
+    f = io.BytesIO()
+    torch.save(c, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c)), _saved, copy.copy])
+def test_copies_pass_their_own_memory(how):
+    """What reaches the library are the addresses and sizes of the copy's own
+    tensors; only a shallow copy shares the original's."""
+    c = _cache(bits=8, head_dim=128)
+    c._workspaces[(1, 1, 2, 1, 0)] = 64
+    d = how(c)
+    own = tuple(getattr(d, n).data_ptr() for n in PARTS)
+    assert kv_cache._CACHE.unpack(d._native) == (*own, 4, 2, 16, 128, 8)
+    assert (own == tuple(getattr(c, n).data_ptr() for n in PARTS)) == (how is copy.copy)
+    assert (d.pages, d.kv_heads, d.page_size, d.head_dim, d.bits, d.device) == (4, 2, 16, 128, 8, c.device)
+    assert d._workspaces is not c._workspaces
+
+
+def test_memory_that_a_tensor_was_given_later():
+    c = _cache()
+    c.key_scales.data = torch.zeros_like(c.key_scales)
+    assert kv_cache._CACHE.unpack(c._native)[:4] == tuple(getattr(c, n).data_ptr() for n in PARTS)
+    c.value_codes.data = torch.zeros((3, 2, 16, 32), dtype=torch.uint8)
+    with pytest.raises(ValueError, match="value_codes must have shape"):
+        c._native
+    c = _cache()
+    for n in PARTS:  # more heads in all of them: the next call checks its arguments against those
+        t = getattr(c, n)
+        t.data = torch.zeros((4, 5, *t.shape[2:]), dtype=t.dtype)
+    with pytest.raises(RuntimeError, match="CUDA/HIP"):
+        shk.kv_cache_read(c, torch.arange(3))
+    assert c.kv_heads == 5
 
 
 def test_calls_need_the_device():
