@@ -553,9 +553,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
   for (int p0 = 0; p0 < count; p0 += 64) {
     float weight = 0.0f;
     if (p0 + lane < count) {
+      // A piece of NaN keys has reference -inf, so a weight of 0 does not mean
+      // that it says nothing: 0 times its NaN sum and outputs stays NaN.
       const float2 ml = a.part_ml[place(p0 + lane)];
-      weight = ml.x == -__builtin_inff() && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - base);
-      sum += weight == 0.0f ? 0.0f : ml.y * weight;
+      weight = __builtin_amdgcn_exp2f(ml.x - base);
+      sum += ml.y * weight;
     }
     const int here = min(count - p0, 64);
     for (int p = wave; p < here; p += 32) {  // eight loads at a time
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float w = __shfl(weight, min(p + 4 * i, here - 1), 64);
-        if (p + 4 * i < here && w != 0.0f) v += o[i] * w;
+        if (p + 4 * i < here) v += o[i] * w;
       }
     }
   }

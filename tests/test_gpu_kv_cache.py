@@ -324,6 +324,75 @@ def test_nan_and_infinity_stay_in_their_sequence(device):
     _check(out[:1], lse[:1], q[:1], cache, table[:1], lengths[:1])
 
 
+def _first_page_unused(cache, *tables):
+    """Swaps the page that no table names with page 0, which bad page numbers
+    are read as."""
+    named = torch.cat([t.flatten() for t in tables])
+    unused = next(i for i in range(cache.pages) if not (named == i).any())
+    for t in tables:
+        t[t == 0] = unused
+    for part in (cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales):
+        part[[0, unused]] = part[[unused, 0]]
+
+
+# own tokens alone; after a prefix of few rows and of many
+WHERE = {"own": (3, 1, 0), "prefix": (3, 1, 600), "many rows": (3, 6, 600)}
+
+
+@pytest.mark.parametrize("where", list(WHERE))
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
+def test_nan_in_one_of_several_pieces(where, dtype, dim, device):
+    """A piece in which all visible keys are NaN, one NaN key among the pieces
+    that weigh nothing, and queries of NaN: NaN there, and nowhere else."""
+    batch, queries, prefix = WHERE[where]
+    for gain in (2.0, 1e4):  # at the second, most pieces' weights underflow
+        q, cache, table, lengths, pages = _case(stable_seed("pieces", where, dtype, dim), [257, 700, 513],
+                                                queries=queries, page=64, dim=dim, dtype=dtype, prefix=prefix,
+                                                q_gain=gain, device=device)
+        cache.key_scales[int(table[0, 4]), :, 0] = math.nan  # the newest token, alone in its piece
+        q[2] = math.nan
+        out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+        assert torch.isnan(out[0, -1]).all() and torch.isnan(lse[0, -1]).all()
+        assert torch.isnan(out[2]).all() and torch.isnan(lse[2]).all()
+        _check(out[1:2], lse[1:2], q[1:2], cache, table[1:2], lengths[1:2], pages, prefix)
+        cache.key_scales[int(table[0, 4]), :, 0] = 0.01
+        for piece in range(3):
+            at = int(table[1, 4 * piece + 1])
+            kept = cache.key_scales[at, 1, 5].clone()
+            cache.key_scales[at, 1, 5] = math.nan
+            out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+            assert torch.isnan(out[1, :, 4:]).all() and torch.isnan(lse[1, :, 4:]).all()
+            assert torch.isfinite(out[1, :, :4]).all() and torch.isfinite(lse[1, :, :4]).all()
+            cache.key_scales[at, 1, 5] = kept
+        _check(out[:1], lse[:1], q[:1], cache, table[:1], lengths[:1], pages, prefix)
+
+
+@pytest.mark.parametrize("where", list(WHERE))
+@pytest.mark.parametrize("gain", [2.0, 1e4])
+def test_page_outside_the_cache_in_one_of_several_pieces(where, gain, device):
+    """Whichever piece the page is in, whatever the page read instead holds,
+    and however little the piece weighs."""
+    batch, queries, prefix = WHERE[where]
+    q, cache, table, lengths, pages = _case(stable_seed("bad page", where), [700, 0, 90], queries=queries, page=64,
+                                            prefix=prefix, q_gain=gain, spare=0, device=device)
+    _first_page_unused(cache, table, pages)
+    for hold in (math.nan, 1e-3):
+        cache.key_scales[0] = cache.value_scales[0] = hold
+        for i in range(11):
+            bad = table.clone()
+            bad[0, i] = -1 if i % 2 else cache.pages
+            if i >= 4 and i % 4 == 0:
+                bad[0, i:i + 4] = 10**9  # a whole piece
+            out, lse = _attend(q, cache, bad, lengths, pages, prefix, device)
+            assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all(), i
+            _check(out[1:], lse[1:], q[1:], cache, table[1:], lengths[1:], pages, prefix)
+        for i in range(-(-prefix // 64)):
+            bad = pages.clone()
+            bad[i] = -5
+            out, lse = _attend(q, cache, table, lengths, bad, prefix, device)
+            assert torch.isnan(out).all() and torch.isnan(lse).all(), i
+
+
 def test_pages_and_lengths_outside_the_cache(device):
     q, cache, table, lengths, _ = _case(21, [30, 40, 20], page=16, spare=0, device=device)
     table[1, 1] = 10**6
