@@ -293,7 +293,7 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
 #pragma unroll
       for (int t = 0; t < RT; ++t) left[t] = limit[t] - t0;
       h8 p[RT][NB / 2], pl[RT][NB / 2];
-      rows.template soften<NB>(s, ks, vs, t0 + kStep > least, left, n - t0, p, pl);
+      rows.template soften<NB>(s, ks, vs, t0 + kStep > least, left, p, pl);
 #pragma unroll
       for (int h = 0; h < NB / 2; ++h)
 #pragma unroll
@@ -469,7 +469,7 @@ __device__ __forceinline__ void prefix_pieces(const AttnArgs& a, int unit, Prefi
 #pragma unroll
     for (int t = 0; t < RT; ++t) left[t] = n - step * kKvTile;
     h8 p[RT][2], pl[RT][2];
-    rows.template soften<4>(s, ks, vs, left[0] < kKvTile, left, left[0], p, pl);
+    rows.template soften<4>(s, ks, vs, left[0] < kKvTile, left, p, pl);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll

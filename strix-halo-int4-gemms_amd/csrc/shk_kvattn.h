@@ -198,7 +198,7 @@ struct KvRows {
   float qs[RT];  // 2^e of the row, times |softmax scale| and log2(e)
   f4 o[RT][kOut];
   float m[RT], l[RT];  // reference and sum (the lane's tokens only)
-  uint32_t big;        // bits of the largest v scale met
+  uint32_t big[RT];    // bits of the largest v scale that the row has seen
 
   // q[c][g * (D / 4) + 8 s + kv_order(i)] for step s; null rows are zero.
   __device__ __forceinline__ void begin(const void* const (&row)[RT], float scale) {
@@ -231,10 +231,10 @@ struct KvRows {
         for (int i = 0; i < 8; ++i) q[t][s][i] = (_Float16)(v[s][kv_order<BITS>(i)] * inv);
       m[t] = -__builtin_inff();
       l[t] = 0.0f;
+      big[t] = 0;
 #pragma unroll
       for (int j = 0; j < kOut; ++j) o[t][j] = f4{0, 0, 0, 0};
     }
-    big = 0;
   }
 
   // Scores (before the row's factor) of 16 * NB tokens and their scales to the
@@ -242,37 +242,44 @@ struct KvRows {
   // grows only past twice its value, which the 13 leaves room for: the shrink
   // runs in few steps instead of nearly all.
   // limit[t]: the row's tokens end there, counted from the step's first;
-  // `ends`: some row's do (uniform); held: the sequence's tokens end there.
+  // `ends`: some row's do (uniform).  What a row does not see may hold
+  // anything, NaN too: it stays out of the row's scores, largest scale and
+  // products.
   template <int NB>
-  __device__ __forceinline__ void soften(f4 (&s)[RT][NB], const f4 (&ks)[NB], f4 (&vs)[NB], bool ends,
-                                         const int (&limit)[RT], int held, h8 (&p)[RT][NB / 2],
-                                         h8 (&pl)[RT][NB / 2]) {
+  __device__ __forceinline__ void soften(f4 (&s)[RT][NB], const f4 (&ks)[NB], const f4 (&vs)[NB], bool ends,
+                                         const int (&limit)[RT], h8 (&p)[RT][NB / 2], h8 (&pl)[RT][NB / 2]) {
     const int g = (threadIdx.x & 63) / 16;
+    auto unseen = [&](int t, int i, int r) { return 16 * i + 4 * g + r >= limit[t]; };
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int i = 0; i < NB; ++i) s[t][i] *= ks[i];
     if (ends) {
 #pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (unseen(t, i, r)) s[t][i][r] = -__builtin_inff();
+            most = max(most, unseen(t, i, r) ? 0u : __float_as_uint(vs[i][r]));
+          }
+        big[t] = max(big[t], groups_most(most));
+      }
+    } else {
+      uint32_t most = 0;
+#pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int at = 16 * i + 4 * g + r;
+        for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(vs[i][r]));
+      most = groups_most(most);
 #pragma unroll
-          for (int t = 0; t < RT; ++t)
-            if (at >= limit[t]) s[t][i][r] = -__builtin_inff();
-          if (at >= held) vs[i][r] = 0.0f;  // never written: may hold anything
-        }
+      for (int t = 0; t < RT; ++t) big[t] = max(big[t], most);
     }
-    uint32_t most = big;
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(vs[i][r]));
-    big = groups_most(most);
-    const float up = (float)(min(max((int)(big >> 23), 47), 254) - 127 - 13);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+      const float up = (float)(min(max((int)(big[t] >> 23), 47), 254) - 127 - 13);
       float top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -295,6 +302,16 @@ struct KvRows {
           p[t][i / 2][4 * (i % 2) + r] = hi;
           if constexpr (kSplitP) pl[t][i / 2][4 * (i % 2) + r] = (_Float16)(w - (float)hi);
         }
+      if (ends) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (unseen(t, i, r)) {  // 0 times a scale that may be NaN
+              p[t][i / 2][4 * (i % 2) + r] = (_Float16)0.0f;
+              if constexpr (kSplitP) pl[t][i / 2][4 * (i % 2) + r] = (_Float16)0.0f;
+            }
+      }
       l[t] = l[t] * alpha + sum;
       if (__any(alpha != 1.0f)) {
 #pragma unroll

@@ -324,6 +324,25 @@ def test_nan_and_infinity_stay_in_their_sequence(device):
     _check(out[:1], lse[:1], q[:1], cache, table[:1], lengths[:1])
 
 
+@pytest.mark.parametrize("queries,ratio", [(2, 1), (5, 2), (6, 4)])
+@pytest.mark.parametrize("dtype,bits,dim", [("bf16", 4, 128), ("f16", 8, 64), ("bf16", 8, 256), ("f16", 4, 128)])
+def test_values_that_a_query_must_not_see(queries, ratio, dtype, bits, dim, device):
+    """The newest token's value is NaN, infinite or larger than all others by
+    far: earlier queries give what they give without it."""
+    q, cache, table, lengths, _ = _case(stable_seed("unseen", queries, ratio, dtype, bits, dim), [40, 300, 705, 1, 64],
+                                        queries=queries, ratio=ratio, bits=bits, dim=dim, dtype=dtype, page=32,
+                                        device=device)
+    for scale in (math.nan, math.inf, 2.0**60):
+        for b, n in enumerate(lengths.tolist()):
+            cache.value_scales[int(table[b, (n - 1) // 32]), :, (n - 1) % 32] = scale
+        out, lse = _attend(q, cache, table, lengths, None, 0, device)
+        _check(out[:, :-1], lse[:, :-1], q[:, :-1], cache, table, lengths - 1)
+        if scale != 2.0**60:
+            assert not torch.isfinite(out[:, -1]).any() and torch.isfinite(lse[:, -1]).all()
+        elif dtype == "bf16":
+            _check(out[:, -1:], lse[:, -1:], q[:, -1:], cache, table, lengths)
+
+
 def _first_page_unused(cache, *tables):
     """Swaps the page that no table names with page 0, which bad page numbers
     are read as."""
