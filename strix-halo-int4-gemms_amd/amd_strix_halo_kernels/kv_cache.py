@@ -293,8 +293,8 @@ def kv_cache_attention(
             raise ValueError(f"prefix_pages holds {prefix_pages.shape[0] * cache.page_size} tokens; prefix_length is "
                              f"{prefix_length}")
     scale = 1.0 / math.sqrt(cache.head_dim) if softmax_scale is None else float(softmax_scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"softmax_scale must be finite; got {softmax_scale}")
+    if not abs(scale) < 2.0**128 - 2.0**103:  # what rounds to a finite f32
+        raise ValueError(f"softmax_scale must be finite in 32 bits; got {softmax_scale}")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():

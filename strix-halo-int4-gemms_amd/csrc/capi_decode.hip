@@ -1,6 +1,7 @@
 // C ABI of the decode step's operators: argument validation and launches.
 // Declarations are in include/strix_halo_gfx950.h.
 #include <climits>
+#include <cmath>
 #include <string>
 
 #include "shk_capi.h"
@@ -73,6 +74,8 @@ int check_attention(const shk_kv_cache* c, const shk_kv_attention* a) {
     return capi_fail("too many query rows for one launch");
   if (a->table_pages < 0 || (__int128)a->table_pages * c->page_size > INT_MAX - 64)
     return capi_fail("a sequence holds at most 2147483583 tokens");
+  if (!std::isfinite((float)a->scale))
+    return capi_fail("the softmax scale must be finite in 32 bits; got " + std::to_string(a->scale));
   if (a->prefix_length < 0 || a->prefix_length > INT_MAX - 64)
     return capi_fail("prefix_length must be from 0 to 2147483583; got " + std::to_string(a->prefix_length));
   return 0;

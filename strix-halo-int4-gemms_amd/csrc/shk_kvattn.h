@@ -224,7 +224,9 @@ struct KvRows {
       // the largest magnitude's exponent, within what both 2^e and 2^-e hold
       const int e = min(max((int)(most >> 23), 1), 253);
       const float inv = __builtin_copysignf(__uint_as_float((uint32_t)(254 - e) << 23), scale);
-      qs[t] = __uint_as_float((uint32_t)e << 23) * (__builtin_fabsf(scale) * kLog2e);
+      // Never 0, which would make NaN of a masked -inf: a scale of 0, or one
+      // that a row of zeros leaves no bits of, is as flat at the smallest f32.
+      qs[t] = __builtin_fmaxf(__uint_as_float((uint32_t)e << 23) * (__builtin_fabsf(scale) * kLog2e), 0x1p-149f);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll

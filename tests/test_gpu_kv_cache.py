@@ -313,6 +313,26 @@ def test_softmax_scale_and_strides(device):
     _check(out, lse, q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-60, 1e-44, -1e-30])
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 256)])
+def test_flat_softmax_scales(scale, dtype, dim, device):
+    """A scale of zero, or one that a row of zeros leaves no bits of: every
+    visible token counts the same."""
+    q, cache, table, lengths, pages = _case(stable_seed("flat", dtype, dim), [1, 40, 333, 0], queries=3, dim=dim,
+                                            dtype=dtype, prefix=70, device=device)
+    q[1] = 0.0
+    for prefix in (0, 70):
+        out, lse = _attend(q, cache, table, lengths, pages, prefix, device, softmax_scale=scale)
+        _check(out, lse, q, cache, table, lengths, pages if prefix else None, prefix, scale=scale)
+
+
+def test_softmax_scales_that_are_refused(device):
+    q, cache, table, lengths, _ = _case(6, [20], device=device)
+    for scale in (math.nan, math.inf, -math.inf, 2.0**128 - 2.0**103, 1e300):
+        with pytest.raises(ValueError, match="finite in 32 bits"):
+            _attend(q, cache, table, lengths, None, 0, device, softmax_scale=scale)
+
+
 def test_nan_and_infinity_stay_in_their_sequence(device):
     q, cache, table, lengths, _ = _case(9, [30, 30, 30], kv_heads=1, page=32, device=device)
     cache.value_scales[int(table[1, 0]), 0, 7] = math.inf

@@ -171,6 +171,8 @@ def test_c_abi_refuses_rows(lib, kw, match):
     ({"page_table": None}, "page_table pointer"), ({"q": FAKE + 2}, "aligned to 16"),
     ({"q_head_stride": 65}, "aligned to 16"), ({"out": FAKE + 2}, "out must be aligned"),
     ({"table_pages": 4096}, "workspace must hold"),
+    ({"scale": float("nan")}, "finite in 32 bits"), ({"scale": float("-inf")}, "finite in 32 bits"),
+    ({"scale": 3.5e38}, "finite in 32 bits"),
 ])
 def test_c_abi_refuses_attention(lib, kw, match):
     args = _native_attention(**kw)
