@@ -19,7 +19,7 @@
 // then keep all their bits in f16 down to 2^-14 of the largest one.
 //
 // A row's probabilities are taken relative to
-//   m = max(score) + exponent(max(v_scale)) - 13,
+//   m = max(score) + exponent(max |v_scale|) - 13,
 // in powers of two and over what the row has met so far, not to the largest
 // score: 2^(score - m) * v_scale is then at most 2^15, so f16 does not
 // overflow and keeps all its bits down to 2^-27 of the largest term, whatever
@@ -98,6 +98,11 @@ __device__ __forceinline__ float groups_sum(float v) {
   return __uint_as_float(groups(__float_as_uint(v), [](uint32_t a, uint32_t b) {
     return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
   }));
+}
+
+// max(a, |b|), a NaN where b is one: two of them are one instruction.
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_elementwise_maximum(a, __builtin_fabsf(b));
 }
 
 struct KvView {  // one key head of the cache
@@ -198,7 +203,7 @@ struct KvRows {
   float qs[RT];  // 2^e of the row, times |softmax scale| and log2(e)
   f4 o[RT][kOut];
   float m[RT], l[RT];  // reference and sum (the lane's tokens only)
-  uint32_t big[RT];    // bits of the largest v scale that the row has seen
+  uint32_t big[RT];    // bits of the largest |v scale| that the row has seen
 
   // q[c][g * (D / 4) + 8 s + kv_order(i)] for step s; null rows are zero.
   __device__ __forceinline__ void begin(const void* const (&row)[RT], float scale) {
@@ -259,25 +264,25 @@ struct KvRows {
     if (ends) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        uint32_t most = 0;
+        float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (unseen(t, i, r)) s[t][i][r] = -__builtin_inff();
-            most = max(most, unseen(t, i, r) ? 0u : __float_as_uint(vs[i][r]));
+            most = larger(most, unseen(t, i, r) ? 0.0f : vs[i][r]);
           }
-        big[t] = max(big[t], groups_most(most));
+        big[t] = max(big[t], groups_most(__float_as_uint(most)));
       }
     } else {
-      uint32_t most = 0;
+      float most = 0.0f;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(vs[i][r]));
-      most = groups_most(most);
+        for (int r = 0; r < 4; ++r) most = larger(most, vs[i][r]);
+      const uint32_t bits = groups_most(__float_as_uint(most));
 #pragma unroll
-      for (int t = 0; t < RT; ++t) big[t] = max(big[t], most);
+      for (int t = 0; t < RT; ++t) big[t] = max(big[t], bits);
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {

@@ -333,6 +333,22 @@ def test_softmax_scales_that_are_refused(device):
             _attend(q, cache, table, lengths, None, 0, device, softmax_scale=scale)
 
 
+@pytest.mark.parametrize("dtype,bits,dim", [("bf16", 4, 128), ("f16", 8, 64), ("bf16", 8, 256)])
+def test_scales_below_zero(dtype, bits, dim, device):
+    """Scales of any sign, zeros of either sign among them, count as they
+    read back."""
+    q, cache, table, lengths, pages = _case(stable_seed("signs", dtype, bits, dim), [1, 40, 600], queries=2, dim=dim,
+                                            bits=bits, dtype=dtype, prefix=70, page=32, device=device)
+    g = torch.Generator().manual_seed(4)
+    for s in (cache.key_scales, cache.value_scales):
+        s *= torch.tensor([1.0, -1.0, 0.0, -0.0])[torch.randint(0, 4, s.shape, generator=g)].to(s)
+    out, lse = _attend(q, cache, table, lengths, pages, 70, device)
+    _check(out, lse, q, cache, table, lengths, pages, 70)
+    cache.value_scales.abs_().neg_()
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    _check(out, lse, q, cache, table, lengths)
+
+
 def test_nan_and_infinity_stay_in_their_sequence(device):
     q, cache, table, lengths, _ = _case(9, [30, 30, 30], kv_heads=1, page=32, device=device)
     cache.value_scales[int(table[1, 0]), 0, 7] = math.inf
