@@ -286,7 +286,10 @@ struct KvRows {
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const float up = (float)(min(max((int)(big[t] >> 23), 47), 254) - 127 - 13);
+      // an infinite or NaN scale needs no room: its outputs are not finite
+      // whatever the reference, and the row's sum keeps its bits
+      const int e = big[t] < 0x7F800000u ? max((int)(big[t] >> 23), 47) : 47;
+      const float up = (float)(e - 127 - 13);
       float top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < NB; ++i)

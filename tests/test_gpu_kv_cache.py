@@ -349,6 +349,21 @@ def test_scales_below_zero(dtype, bits, dim, device):
     _check(out, lse, q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_lse_beside_bad_values(dtype, bad, device):
+    """The sum of exponentials does not depend on the values."""
+    q, cache, table, lengths, _ = _case(stable_seed("lse", dtype), [300, 1500], page=64, q_gain=4.0, dtype=dtype,
+                                        device=device)
+    for b in range(2):
+        cache.value_scales[int(table[b, 0]), :, 9] = bad
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    assert not torch.isfinite(out).any()
+    want = ref.attention(q, _cpu(cache), table, lengths)
+    bound = ref.attention_bounds(q.dtype, 128, 1500, *want)[1]
+    assert ((lse.cpu().double() - want[1]).abs() <= bound).all()
+
+
 def test_nan_and_infinity_stay_in_their_sequence(device):
     q, cache, table, lengths, _ = _case(9, [30, 30, 30], kv_heads=1, page=32, device=device)
     cache.value_scales[int(table[1, 0]), 0, 7] = math.inf
