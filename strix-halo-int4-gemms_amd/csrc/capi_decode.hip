@@ -50,12 +50,11 @@ int rows_entry(bool write, int device_index, uintptr_t stream, const shk_kv_cach
     if (int rc = check_cache(cache)) return rc;
     if (int rc = check_rows(rows)) return rc;
     if (rows->tokens == 0) return 0;
-    if (rows->tokens > INT_MAX / cache->kv_heads) return capi_fail("too many tokens for one launch");
+    if (rows->tokens > shk::kv_rows_most(write, *cache)) return capi_fail("too many tokens for one launch");
     shk::DeviceGuard guard(device_index);
     if (guard.error() != hipSuccess) return capi_fail_hip("hipSetDevice", guard.error());
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const hipError_t err = write ? shk::launch_kv_write(*cache, *rows, s) : shk::launch_kv_read(*cache, *rows, s);
-    if (err == hipErrorInvalidValue) return capi_fail("too many tokens for one launch");
     if (err != hipSuccess) return capi_fail_hip(write ? "kv_write launch" : "kv_read launch", err);
     return 0;
   });
@@ -72,12 +71,17 @@ int check_attention(const shk_kv_cache* c, const shk_kv_attention* a) {
   if (a->batch > INT_MAX || a->queries > INT_MAX || a->heads > INT_MAX ||
       (__int128)a->batch * a->queries * a->heads > INT_MAX / 32)
     return capi_fail("too many query rows for one launch");
-  if (a->table_pages < 0 || (__int128)a->table_pages * c->page_size > INT_MAX - 64)
-    return capi_fail("a sequence holds at most 2147483583 tokens");
+  // tokens are counted in 32 bits, and rounded up to pieces of 256 there
+  constexpr int64_t most = INT_MAX - 256;
+  if (a->table_pages < 0 || (__int128)a->table_pages * c->page_size > most)
+    return capi_fail("a sequence holds at most 2147483391 tokens");
+  if ((__int128)a->batch * ((a->table_pages * c->page_size + 255) / 256) > most)
+    return capi_fail("too many tokens in the page table");
   if (!std::isfinite((float)a->scale))
     return capi_fail("the softmax scale must be finite in 32 bits; got " + std::to_string(a->scale));
-  if (a->prefix_length < 0 || a->prefix_length > INT_MAX - 64)
-    return capi_fail("prefix_length must be from 0 to 2147483583; got " + std::to_string(a->prefix_length));
+  if (a->prefix_length < 0 || a->prefix_length > most)
+    return capi_fail("prefix_length must be from 0 to 2147483391; got " + std::to_string(a->prefix_length));
+  if (a->batch * a->queries > 0 && !shk::kv_attention_fits(*c, *a)) return capi_fail("too many query rows for one launch");
   return 0;
 }
 
@@ -142,7 +146,6 @@ int amd_strix_halo_kernels_kv_attention(int device_index, uintptr_t stream, cons
     shk::DeviceGuard guard(device_index);
     if (guard.error() != hipSuccess) return capi_fail_hip("hipSetDevice", guard.error());
     const hipError_t err = shk::launch_kv_attention(*cache, a, reinterpret_cast<hipStream_t>(stream));
-    if (err == hipErrorInvalidValue) return capi_fail("too many workgroups for one launch");
     if (err != hipSuccess) return capi_fail_hip("kv_attention launch", err);
     return 0;
   });

@@ -597,6 +597,7 @@ struct Plan {
   bool direct;
 };
 
+// For at least one query row.
 Plan plan_of(const shk_kv_cache& c, const shk_kv_attention& a) {
   const long rows = a.queries * (a.heads / c.kv_heads), all = rows * a.batch, tokens = a.table_pages * c.page_size;
   const bool wide = c.head_dim == 256;  // two row tiles of 256 columns would not fit the registers
@@ -637,7 +638,6 @@ template <int BITS, int D, int RT, int TYPE>
 hipError_t launch_rt(const AttnArgs& a, const Plan& p, hipStream_t s) {
   const long own = (long)a.kv_heads * a.own_tiles * a.own_groups;
   const long prefix = (long)a.kv_heads * a.prefix_tiles * a.prefix_splits;
-  if (own + prefix > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
   const dim3 grid((unsigned)(own + prefix)), block(256);
   if (p.prefix_kernel)
     hipLaunchKernelGGL((kv_prefix_kernel<BITS, D, D == 256 ? 1 : 2, RT, TYPE>), grid, block, 0, s, a);
@@ -667,6 +667,13 @@ hipError_t launch_d(long d, const AttnArgs& a, const Plan& p, hipStream_t s) {
 
 int64_t kv_attention_workspace(const shk_kv_cache& c, const shk_kv_attention& a) {
   return part_rows(c, a, plan_of(c, a)) * (c.head_dim * 4 + 8);
+}
+
+bool kv_attention_fits(const shk_kv_cache& c, const shk_kv_attention& a) {
+  const Plan p = plan_of(c, a);
+  const long first = c.kv_heads * ((long)p.own_tiles * p.own_groups + (long)p.prefix_tiles * p.prefix_splits);
+  const long join = p.direct ? 0 : a.batch * a.queries * a.heads;  // a workgroup a row
+  return std::max(first, join) <= kMostWorkgroups;
 }
 
 hipError_t launch_kv_attention(const shk_kv_cache& c, const shk_kv_attention& x, hipStream_t s) {

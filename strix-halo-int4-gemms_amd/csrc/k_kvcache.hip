@@ -16,6 +16,8 @@
 // what is written does not (f32 values read past them: 295 -> 333 us).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <climits>
 #include <cstdint>
 
 #include "shk_common.h"
@@ -255,12 +257,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const Rows p) {
   }
 }
 
+long rows_of_workgroup(bool write, long d) { return 256 / (d / 8) * (write ? kWriteRows : kReadRows); }
+
 template <int TYPE, int BITS, int D, bool VEC>
 hipError_t launch(bool write, const Rows& p, hipStream_t s) {
-  const long kPer = 256 / (D / 8) * (write ? kWriteRows : kReadRows);  // rows of a workgroup
-  const long blocks = (p.rows + kPer - 1) / kPer;
-  if (blocks > 0x7FFFFF) return hipErrorInvalidValue;  // a launch holds fewer than 2^32 work-items
-  const dim3 grid((unsigned)blocks);
+  const long kPer = rows_of_workgroup(write, D);
+  const dim3 grid((unsigned)((p.rows + kPer - 1) / kPer));
   if (write) hipLaunchKernelGGL((kv_write_kernel<TYPE, BITS, D, VEC>), grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((kv_read_kernel<TYPE, BITS, D, VEC>), grid, dim3(256), 0, s, p);
   return hipGetLastError();
@@ -309,6 +311,11 @@ hipError_t rows_launch(bool write, const shk_kv_cache& c, const shk_kv_rows& r, 
 }
 
 }  // namespace
+
+int64_t kv_rows_most(bool write, const shk_kv_cache& c) {
+  // rows are counted in 32 bits
+  return std::min(kMostWorkgroups * rows_of_workgroup(write, c.head_dim), (int64_t)INT_MAX) / c.kv_heads;
+}
 
 hipError_t launch_kv_write(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s) {
   return rows_launch(true, c, r, s);

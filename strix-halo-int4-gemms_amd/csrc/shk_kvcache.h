@@ -20,6 +20,11 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
+// A launch holds fewer than 2^32 work-items: the tokens of a write or read, and
+// whether an attention's query rows fit.
+constexpr int64_t kMostWorkgroups = 0xFFFFFF;  // of 256
+int64_t kv_rows_most(bool write, const shk_kv_cache& c);
+bool kv_attention_fits(const shk_kv_cache& c, const shk_kv_attention& a);
 hipError_t launch_kv_write(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s);
 hipError_t launch_kv_read(const shk_kv_cache& c, const shk_kv_rows& r, hipStream_t s);
 int64_t kv_attention_workspace(const shk_kv_cache& c, const shk_kv_attention& a);

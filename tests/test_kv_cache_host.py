@@ -180,6 +180,43 @@ def test_c_abi_refuses_attention(lib, kw, match):
     assert match in lib.amd_strix_halo_kernels_last_error().decode()
 
 
+@pytest.mark.parametrize("kw,match", [
+    # 32-bit counts of tokens and pieces
+    ({"table_pages": (2**31 - 256) // 16}, "at most 2147483391 tokens"),
+    ({"prefix_pages": FAKE, "prefix_length": 2**31 - 256}, "prefix_length must be from 0 to 2147483391"),
+    ({"batch": 2**12, "table_pages": 2**27 - 256}, "too many tokens in the page table"),
+    # a launch of 2^32 work-items or more, of the join and of the first kernel
+    ({"batch": 2**21, "heads": 8, "table_pages": 17}, "too many query rows for one launch"),
+    ({"batch": 2**23, "heads": 2}, "too many query rows for one launch"),
+])
+def test_c_abi_refuses_attention_past_its_counts(lib, kw, match):
+    args = _native_attention(**kw)
+    assert lib.amd_strix_halo_kernels_kv_attention(0, 0, _native_cache(), args) == 1
+    assert match in lib.amd_strix_halo_kernels_last_error().decode()
+    assert lib.amd_strix_halo_kernels_kv_attention_workspace(_native_cache(), args) == -1
+    assert match in lib.amd_strix_halo_kernels_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [
+    {"table_pages": (2**31 - 257) // 16}, {"prefix_pages": FAKE, "prefix_length": 2**31 - 257},
+    {"batch": 2**21 - 1, "heads": 8, "table_pages": 17}, {"batch": 2**21, "heads": 8, "table_pages": 16},
+    {"batch": 2**23 - 1, "heads": 2},
+    {"batch": 0, "table_pages": 100, "prefix_pages": FAKE, "prefix_length": 100}, {"queries": 0, "table_pages": 100},
+])
+def test_attention_up_to_its_counts(lib, kw):
+    assert lib.amd_strix_halo_kernels_kv_attention_workspace(_native_cache(), _native_attention(**kw)) >= 0
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_c_abi_refuses_rows_past_a_launch(lib, head_dim):
+    """16777215 workgroups of 2048 values written, of 4096 read; rows in 32 bits."""
+    cache = _native_cache(head_dim=head_dim, kv_heads=3)
+    for call, values in ((lib.amd_strix_halo_kernels_kv_write, 2048), (lib.amd_strix_halo_kernels_kv_read, 4096)):
+        most = min(16777215 * (values // head_dim), 2**31 - 1) // 3
+        assert call(0, 0, cache, _native_rows(tokens=most + 1)) == 1
+        assert "too many tokens for one launch" in lib.amd_strix_halo_kernels_last_error().decode()
+
+
 def test_c_abi_null_structs_and_empty_calls(lib):
     cache, rows, args = _native_cache(), _native_rows(tokens=0), _native_attention(batch=0)
     assert lib.amd_strix_halo_kernels_kv_write(0, 0, None, rows) == 1
