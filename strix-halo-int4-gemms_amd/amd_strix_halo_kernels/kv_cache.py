@@ -17,7 +17,8 @@ sequence's newest tokens over its pages, after a prefix that the whole batch
 may share.  All run on the current stream of the tensors' device, or on
 ``stream`` (which is then the current one for the call, its allocations
 included), and read nothing back to the host.  There is no CPU path and no
-gradient.
+gradient: what is written into a cache is cut from its graph, and asking the
+attention's outputs for a gradient raises.
 """
 
 from __future__ import annotations
@@ -28,7 +29,16 @@ from dataclasses import dataclass
 from typing import Any
 
 from . import kernel_table as kt
-from .native import _check, _device_index, _on_stream, _require_device, _stream_handle, _torch, _verified_library
+from .native import (
+    _check,
+    _device_index,
+    _no_gradient,
+    _on_stream,
+    _require_device,
+    _stream_handle,
+    _torch,
+    _verified_library,
+)
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -265,7 +275,7 @@ def kv_cache_attention(
     if q.ndim not in (3, 4) or q.shape[-1] != cache.head_dim:
         raise ValueError(f"q must have shape (batch, heads, {cache.head_dim}) or (batch, queries, heads, "
                          f"{cache.head_dim}); got {tuple(q.shape)}")
-    shape = q.shape
+    given, shape = q, q.shape
     batch, heads = int(shape[0]), int(shape[-2])
     queries = int(shape[1]) if q.ndim == 4 else 1
     if heads == 0 or heads % cache.kv_heads:
@@ -331,4 +341,7 @@ def kv_cache_attention(
         work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, None), native,
                                                             args(work, nbytes)))
+    if given.requires_grad:
+        out = _no_gradient(torch, "kv_cache_attention", out, given)
+        lse = _no_gradient(torch, "kv_cache_attention", lse, given) if return_lse else None
     return (out, lse) if return_lse else out

@@ -14,7 +14,15 @@ from typing import Any
 
 from . import kernel_table as kt
 from .metadata import SUPPORTED_SUBCHANNELS, GemmLayout, ScaleMode, ScaleSpec
-from .native import _check, _device_index, _on_stream, _require_device, _stream_handle, _torch, _verified_library
+from .native import (
+    _check,
+    _no_gradient,
+    _on_stream,
+    _require_device,
+    _stream_handle,
+    _torch,
+    _verified_library,
+)
 
 MOE_MAX_TOKENS = 64
 MOE_MAX_PAIRS = 1024
@@ -69,7 +77,7 @@ def moe_swiglu_int4(
     1024 (token, expert) pairs and 1024 experts.  Returns [tokens, hidden] in
     x's dtype.  Runs on the current stream, or on ``stream`` (which is then the
     current one for the call, its allocations included); nothing is read back
-    to the host, and there is no gradient.
+    to the host, and there is no gradient (asking the result for one raises).
     """
     layout = GemmLayout(layout)
     if layout not in (GemmLayout.NN, GemmLayout.NT):
@@ -134,8 +142,9 @@ def moe_swiglu_int4(
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
         _require("out", out, (tokens, hidden), x.dtype, "(tokens, hidden)")
+    wanting = (x, expert_weights, up_gate_scale, down_scale)
     if tokens == 0:
-        return out
+        return _no_gradient(torch, "moe_swiglu_int4", out, *wanting)
     # h as two bf16 terms with rows of whole 128s, and f32 results, for each
     # pair; a counter for each 128 columns of the output
     nbytes = 4 * (tokens * top * (-(-inner // 128) * 128 + hidden) + -(-hidden // 128))
@@ -147,4 +156,4 @@ def moe_swiglu_int4(
                      work.data_ptr(), nbytes)
     lib = _verified_library()
     _check(lib, lib.amd_strix_halo_kernels_moe(index, _stream_handle(torch, x, None), args))
-    return out
+    return _no_gradient(torch, "moe_swiglu_int4", out, *wanting)

@@ -233,6 +233,31 @@ def _on_stream(torch: Any, tensor: Any, stream: Any) -> Any:
     return torch.cuda.stream(stream)
 
 
+@functools.lru_cache(maxsize=None)
+def _no_gradient_function() -> Any:
+    class NoGradient(_torch().autograd.Function):
+        @staticmethod
+        def forward(ctx: Any, name: str, out: Any, *inputs: Any) -> Any:
+            ctx.name = name
+            ctx.mark_dirty(out)
+            return out
+
+        @staticmethod
+        def backward(ctx: Any, grad: Any) -> Any:
+            raise RuntimeError(f"{ctx.name} has no gradient; call it under torch.no_grad() or detach its inputs")
+
+    return NoGradient
+
+
+def _no_gradient(torch: Any, name: str, out: Any, *inputs: Any) -> Any:
+    """`out` of a call that has no backward pass.  Where one of its inputs asks
+    for a gradient, asking `out` for it raises instead of leaving it out."""
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in inputs):
+        return out
+    # an alias: a buffer that the caller reuses does not gather the graphs of its calls
+    return _no_gradient_function().apply(name, out.detach(), *inputs)
+
+
 def _device_index(tensor: Any) -> int:
     index = tensor.device.index
     return 0 if index is None else int(index)

@@ -484,6 +484,26 @@ def test_no_sequences_and_no_pages(device):
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
+def test_no_gradient_is_said(device):
+    """Outputs are the same bits; asking them for a gradient raises, and a
+    reused buffer keeps no graph."""
+    q, cache, table, lengths, _ = _case(51, [30, 9], device=device)
+    want = _attend(q, cache, table, lengths, None, 0, device)
+    qd = q.to(device).requires_grad_()
+    x = torch.ones((1, 2, 128), device=device, requires_grad=True)
+    shk.kv_cache_write(cache, x, x, torch.tensor([-1], device=device))
+    out = torch.empty_like(qd)
+    for kw in ({}, {"out": out}):
+        got = _attend(qd, cache, table, lengths, None, 0, device, **kw)
+        for g, w in zip(got, want):
+            assert torch.equal(g, w)
+            with pytest.raises(RuntimeError, match="kv_cache_attention has no gradient"):
+                g.sum().backward()
+    assert not out.requires_grad and torch.equal(out, want[0])
+    with torch.no_grad():
+        assert _attend(qd, cache, table, lengths, None, 0, device, out=out)[0] is out
+
+
 def test_repeated_calls_give_the_same_bits(device):
     q, cache, table, lengths, pages = _case(31, [700, 90], prefix=500, page=64, device=device)
     first = _attend(q, cache, table, lengths, pages, 500, device)

@@ -150,6 +150,21 @@ def test_nan_stays_in_its_token(device):
     assert (off[[0, 2]] <= bound[[0, 2]]).all()
 
 
+@pytest.mark.parametrize("which", [0, 4, 5, 6])
+def test_no_gradient_is_said(which, device):
+    for tokens in (3, 0):
+        case = _case(17, tokens, 2, 2, 128, 64)
+        d = [t.to(device) for t in case[:7]]
+        d[which].requires_grad_()
+        got = shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6])
+        if tokens:
+            _check(got.detach(), case)
+        with pytest.raises(RuntimeError, match="moe_swiglu_int4 has no gradient"):
+            got.sum().backward()
+        with torch.no_grad():
+            assert not shk.moe_swiglu_int4(*d[:5], up_gate_scale=d[5], down_scale=d[6]).requires_grad
+
+
 def test_repeated_calls_streams_and_out(device):
     case = _case(13, 20, 6, 2, 320, 192)
     first = _run(case, device)
