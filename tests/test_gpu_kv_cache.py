@@ -276,6 +276,63 @@ def test_long_sequences_are_split_and_joined(dtype, bits, device):
     _check(out, lse, q, cache, table, lengths, pages, 2049)
 
 
+def _pieces_each(kv_heads, tiles, lengths):
+    """The most pieces of 256 tokens that a workgroup of the sequences' own
+    tokens takes: they are dealt out over 512 workgroups."""
+    total = sum(-(-n // 256) for n in lengths)
+    return -(-total // max(1, 512 // (kv_heads * tiles)))
+
+
+UNEVEN = [3000, 0, 5000, 257, 1, 9000, 256, 3333]
+
+
+@pytest.mark.parametrize("kv_heads,ratio,queries,lengths,least", [
+    (16, 1, 1, UNEVEN, 3),                 # across sequences, an empty and a short one among them
+    (64, 1, 3, [3000, 0, 2, 700, 2049], 3),
+    (16, 6, 3, [3000, 40, 5000], 2),       # two row tiles
+    (64, 1, 1, [5003], 3),                 # one sequence's pieces alone
+])
+@pytest.mark.parametrize("dtype,bits,dim", [("bf16", 4, 64), ("f16", 4, 128), ("bf16", 8, 128), ("f16", 8, 256)])
+def test_workgroups_with_several_pieces(kv_heads, ratio, queries, lengths, least, dtype, bits, dim, device):
+    """Several pieces a workgroup, of one sequence and of sequences that follow
+    each other."""
+    print(f"case pieces {kv_heads} heads ratio {ratio} queries {queries} {dtype} int{bits} dim {dim}", flush=True)
+    tiles = -(-queries * ratio // (16 if dim == 256 or queries * ratio <= 16 else 32))
+    assert _pieces_each(kv_heads, tiles, lengths) >= least
+    q, cache, table, lengths, _ = _case(stable_seed("several pieces", kv_heads, ratio, queries, dtype, bits, dim),
+                                        lengths, queries=queries, ratio=ratio, kv_heads=kv_heads, bits=bits, dim=dim,
+                                        dtype=dtype, page=64, device=device)
+    out, lse = _attend(q, cache, table, lengths, None, 0, device)
+    _check(out, lse, q, cache, table, lengths)
+
+
+@pytest.mark.parametrize("batch", [65, 130])
+@pytest.mark.parametrize("kv_heads,dim,prefix", [(2, 128, 0), (32, 64, 0), (2, 128, 300), (32, 64, 300)])
+def test_more_sequences_than_a_wave_has_lanes(batch, kv_heads, dim, prefix, device):
+    """Empty sequences at either end and past the 64th."""
+    lengths = [(i * 97) % 401 * (i % 5 > 0) for i in range(batch)]
+    lengths[64:66] = [0, 700]
+    lengths = lengths[:batch - 1] + [0] if batch > 65 else lengths[:64] + [700]
+    q, cache, table, lengths, pages = _case(stable_seed("many", batch, kv_heads, dim, prefix), lengths, ratio=2,
+                                            kv_heads=kv_heads, dim=dim, prefix=prefix, page=32, device=device)
+    out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+    _check(out, lse, q, cache, table, lengths, pages if prefix else None, prefix)
+
+
+@pytest.mark.parametrize("batch,kv_heads,dtype,bits,dim", [
+    (3, 64, "bf16", 4, 128), (3, 64, "f16", 8, 64), (3, 64, "bf16", 8, 256),  # the streaming kernel
+    (20, 64, "bf16", 4, 128), (20, 64, "f16", 8, 64), (20, 64, "bf16", 8, 256),  # the prefix's own
+])
+def test_workgroups_with_several_pieces_of_a_prefix(batch, kv_heads, dtype, bits, dim, device):
+    prefix = 5003
+    assert -(-prefix // 256) >= 2 * -(-512 // kv_heads)  # pieces a workgroup, one row tile
+    q, cache, table, lengths, pages = _case(stable_seed("prefix pieces", batch, kv_heads, dtype, bits, dim),
+                                            [(i * 37) % 90 for i in range(batch)], kv_heads=kv_heads, bits=bits,
+                                            dim=dim, dtype=dtype, prefix=prefix, page=64, device=device)
+    out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+    _check(out, lse, q, cache, table, lengths, pages, prefix)
+
+
 @pytest.mark.parametrize("gain", [0.0, 1e-30, 30.0, 1e4])
 def test_flat_and_peaked_scores(gain, device):
     """All probabilities equal; and one that is all but 1, with scores in the
@@ -474,6 +531,55 @@ def test_pages_and_lengths_outside_the_cache(device):
     odd = torch.tensor([16, 4000, -5], dtype=torch.int32)
     long, _ = _attend(q, cache, table[:1, :1].expand(3, 1), odd, None, 0, device)
     assert torch.isfinite(long).all() and (long[2] == 0).all()
+
+
+def _refusal(match, call, **kw):
+    with pytest.raises((ValueError, RuntimeError), match=match):
+        call(**kw)
+
+
+def test_refusals_of_attention(device):
+    q, cache, table, lengths, pages = _case(7, [20, 30], prefix=40, device=device)
+    good = {"q": q.to(device), "cache": cache, "page_table": table.to(device), "lengths": lengths.to(device),
+            "prefix_pages": pages.to(device), "prefix_length": 40}
+    wide = torch.zeros((2, 1, 8, 256), dtype=q.dtype, device=device)
+    for name, bad, match in (
+        ("q", good["q"].float(), "torch.bfloat16 or torch.float16"), ("q", good["q"][..., :64], "q must have shape"),
+        ("q", good["q"][0, 0], "q must have shape"), ("q", good["q"][:, :, :7], "multiple of the cache's 2"),
+        ("q", wide[..., ::2], "contiguous along head_dim"), ("q", q, "CUDA/HIP"),
+        ("page_table", good["page_table"].long(), "torch.int32"),
+        ("page_table", good["page_table"][:1], "page_table must have shape"),
+        ("page_table", good["page_table"].t().contiguous().t(), "rows of page_table must be contiguous"),
+        ("lengths", good["lengths"].long(), "torch.int32"),
+        ("lengths", good["lengths"][:1], "lengths must be contiguous"),
+        ("lengths", good["lengths"].expand(2, 2), "lengths must be contiguous"), ("lengths", lengths, "CUDA/HIP"),
+        ("prefix_length", 49, "prefix_pages holds 48 tokens"), ("prefix_length", -1, "non-negative"),
+        ("prefix_length", True, "non-negative"), ("prefix_pages", None, "needs prefix_pages"),
+        ("prefix_pages", good["prefix_pages"].long(), "torch.int32"),
+        ("prefix_pages", good["prefix_pages"][::2], "contiguous one-dimensional"),
+        ("out", torch.empty_like(good["q"]).float(), "out must be contiguous"),
+        ("out", torch.empty((2, 1, 8, 256), dtype=q.dtype, device=device)[..., :128], "out must be contiguous"),
+        ("out", torch.empty(2048 + 1, dtype=q.dtype, device=device)[1:].view(q.shape), "out must be aligned to 8"),
+    ):
+        _refusal(match, shk.kv_cache_attention, **{**good, name: bad})
+    shk.kv_cache_attention(**good)
+
+
+def test_refusals_of_rows(device):
+    cache = shk.new_kv_cache(2, 16, 2, 64, device=device)
+    x, slots = torch.ones((3, 2, 64), device=device), torch.arange(3, device=device)
+    good = {"cache": cache, "keys": x, "values": x, "slots": slots}
+    for name, bad, match in (
+        ("keys", x.double(), "keys must have dtype"), ("values", x.half(), "values must have the dtype of keys"),
+        ("keys", x[:, :1], "keys must have shape"), ("values", x[:2], "values must have shape"),
+        ("keys", torch.ones((3, 64, 2), device=device).transpose(1, 2), "contiguous along head_dim"),
+        ("slots", slots.float(), "slots must have dtype"), ("slots", slots[:2], "slots must have shape"),
+        ("slots", torch.arange(6, device=device)[::2], "slots must be contiguous"), ("keys", x.cpu(), "CUDA/HIP"),
+    ):
+        _refusal(match, shk.kv_cache_write, **{**good, name: bad})
+    for kw, match in (({"dtype": torch.int8}, "the result must have dtype"),
+                      ({"slots": slots[None]}, "slots must have shape"), ({"slots": slots.cpu()}, "CUDA/HIP")):
+        _refusal(match, shk.kv_cache_read, **{"cache": cache, "slots": slots, **kw})
 
 
 def test_no_sequences_and_no_pages(device):

@@ -76,6 +76,79 @@ def test_odd_sizes(layout, group, hidden, inner, device):
         _check(_run(case, device), case)
 
 
+def _waves(grid, k):
+    """Waves of a product's workgroups, which share K."""
+    return 8 if grid <= 256 else 2 if k < 4096 and grid > 1024 else 4
+
+
+def _up(n, to):
+    return -(-n // to) * to
+
+
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+@pytest.mark.parametrize("group", [0, 64, 128, 256])
+@pytest.mark.parametrize("tokens,top,experts,hidden,inner,waves", [
+    (54, 1, 54, 808, 1290, (2, 4)), (33, 2, 60, 2600, 810, (4, 2)), (33, 2, 60, 4200, 1290, (4, 2)),
+    (2, 2, 3, 3208, 200, (8, 8)), (2, 2, 3, 200, 3208, (8, 8))])
+def test_several_pieces_of_k_a_wave(layout, group, tokens, top, experts, hidden, inner, waves, device):
+    """Each number of waves, with three pieces of 128 or more for each in one of
+    the two products, and an end that is none.  Most choices are padding."""
+    print(f"case moe waves {waves} {layout} group {group} {hidden}x{inner}", flush=True)
+    pairs = tokens * top
+    most = min(pairs, experts)
+    hit = most + (pairs - most) // 16
+    grids = _up(-(-_up(inner, 128) // 64), 8) * hit, _up(-(-hidden // 128), 8) * hit
+    assert waves == (_waves(grids[0], hidden), _waves(grids[1], inner))
+    dtype = "f16" if group == 64 else "bf16"
+    case = _case(stable_seed("waves", layout, group, hidden, inner), tokens, 3, min(top, 2), hidden, inner, group=group,
+                 layout=layout, dtype=dtype)
+    g = torch.Generator().manual_seed(hidden + group)
+    ids = torch.full((tokens, top), -1)
+    ids.view(-1)[torch.randperm(pairs, generator=g)[:12]] = torch.randint(0, experts, (12,), generator=g)[:pairs]
+    if pairs > 40:
+        ids[:19, 0] = experts - 1  # two workgroups' rows
+    case[3], case[4] = ids, torch.rand((tokens, top), generator=g)
+    whole = [case[i][torch.arange(experts) % 3] for i in (1, 2, 5, 6)]
+    x, share = case[0].to(device), case[4].to(device)
+    got = shk.moe_swiglu_int4(x, whole[0].to(device), whole[1].to(device), ids.to(device), share,
+                              up_gate_scale=whole[2].to(device), down_scale=whole[3].to(device), scale=spec_of(group),
+                              layout=shk.GemmLayout(layout))
+    # the three experts that all others repeat
+    case[3] = torch.where(ids >= 0, ids % 3, ids)
+    _check(got, case)
+
+
+def test_refusals(device):
+    x, up_gate, down, ids, share, up_scale, down_scale, _, _ = _case(3, 3, 4, 2, 64, 32)
+    good = {n: t.to(device) for n, t in (("x", x), ("up_gate", up_gate), ("down", down), ("expert_ids", ids),
+                                         ("expert_weights", share), ("up_gate_scale", up_scale),
+                                         ("down_scale", down_scale))}
+    for name, bad, match in (
+        ("x", good["x"].float(), "x must have dtype"), ("x", good["x"][0], "x must have shape"),
+        ("x", good["x"].t().contiguous().t(), "rows of x must be contiguous"), ("x", x, "CUDA/HIP"),
+        ("up_gate", good["up_gate"][..., :63], "even number"),
+        ("up_gate", good["up_gate"][:, :31], "up_gate must have shape"),
+        ("up_gate", good["up_gate"][0], "up_gate must have shape"), ("down", good["down"][:3], "down must have shape"),
+        ("down", good["down"].to(torch.int8), "down must have dtype"),
+        ("down", good["down"].transpose(1, 2).contiguous().transpose(1, 2), "down must be contiguous"),
+        ("up_gate_scale", good["up_gate_scale"].float(), "up_gate_scale must have dtype"),
+        ("down_scale", good["down_scale"][:, :63], "down_scale must have shape"),
+        ("expert_ids", good["expert_ids"][:2], "expert_ids must have shape"),
+        ("expert_ids", good["expert_ids"].float(), "expert_ids must have dtype"),
+        ("expert_ids", good["expert_ids"].t().contiguous().t(), "expert_ids must be contiguous"),
+        ("expert_weights", good["expert_weights"].half(), "expert_weights must have dtype"),
+        ("out", torch.empty_like(good["x"]).half(), "out must have dtype"),
+        ("scale", spec_of(32), "up_gate_scale must have shape"),
+        ("layout", shk.GemmLayout.NT, "up_gate must have shape|even number"),
+    ):
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            shk.moe_swiglu_int4(**{**good, name: bad})
+    case = _case(3, 65, 4, 2, 64, 32)
+    with pytest.raises(ValueError, match="up to 64 tokens"):
+        _run(case, device)
+    shk.moe_swiglu_int4(**good)
+
+
 @pytest.mark.parametrize("layout", ["nn", "nt"])
 def test_every_end_of_a_row(layout, device):
     """hidden takes every residue of eight values; rows past x's are not read."""
