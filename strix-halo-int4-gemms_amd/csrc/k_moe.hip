@@ -676,9 +676,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_product(const MoeArgs a) {
   moe_rows<LAYOUT, FIRST, TYPE, GROUPED, kWaves>(a, s, scale, list, rows, n0, k_first, k_last, k_step, red,
                                                  lds_scale + 256 * wave);
   if (!FIRST && a.joined) {
-    // The last workgroup of a tile adds up its pairs.  Results are written and
-    // read with device scope, which the XCDs' caches see without being
-    // flushed; each workgroup's have arrived before it counts itself.
+    // The last workgroup of a tile adds up its pairs, in a fixed order.  This
+    // rests on gfx942's memory model as LLVM's AMDGPU guide states it, which
+    // gfx950 shares: a device-scope store (sc1) has reached the level that all
+    // XCDs see once vmcnt counts it off, and a device-scope load (sc1) takes
+    // nothing older from its own caches.  Every wave waits for its stores
+    // before the barrier, so they are there before thread 0 counts the
+    // workgroup, and the last one's loads come after its count.  A release and
+    // acquire count would also write back and invalidate the caches
+    // (buffer_wbl2, buffer_inv), for ordinary stores and loads, of which none
+    // is shared here: 16 pairs of 64 experts of 4096 x 1408 53.6 us instead of
+    // 47.5.
     __shared__ int last;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
