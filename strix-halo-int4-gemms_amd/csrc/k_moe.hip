@@ -701,15 +701,30 @@ template <int LAYOUT, bool FIRST, int TYPE, int GROUPED>
 void launch_waves(const MoeArgs& a, dim3 grid, hipStream_t s) {
   // A workgroup's waves share K.  Few workgroups (at most one on each of the
   // 256 CUs): eight, the shortest way through.  Many: every wave's start and
-  // end count, and a wave should have about 1024 K values: two waves.  Four in
-  // between, and for a long K, whose workgroups would otherwise be uneven.
-  // Measured, us for up and gate / down with 2, 4, 8 waves: 41 experts of
-  // 2048 x 1408 36 / 27, 43 / 30, 60 / 39; 14 of 4096 x 11008 146 / 117, 145 / 106.
-  // The layer of 32 pairs of 16 experts of 2048 x 1408 (up to 384 workgroups)
-  // with 2 and 4 waves: 37, 29.
+  // end count, and two waves halve them, until K is so long that workgroups
+  // become uneven.  Without scale groups to add up in between, up and gate
+  // come to that sooner.  Four waves in between and for a long K.
+  // The layer of 16 tokens, 6 of 64 experts, us with two / four waves for
+  // up and gate (inner 2560 up to hidden 2048, 1408 from 2816):
+  //   hidden             512    1088   1536   2048    2816    3584     4096
+  //   NN, bf16         43/45   71/73  78/78  92/93   74/70   97/91  105/98
+  //   NN, f16          44/47   74/75  81/80  96/94   79/72  103/93
+  //   NT, bf16         48/53   82/84  86/86  98/96   80/76  103/97
+  //   NT, f16          52/53   88/86  93/89  106/100 77/78  100/100
+  //   NN, groups of 128 (inner 1408)  53/58          73/79   98/101
+  //   NT, groups of 128 (inner 1408)  57/61  64/67   80/82  103/103 113/110
+  // and for down (hidden 2816):
+  //   inner              704    1408   2816
+  //   NN               60/63   74/79  125/130
+  //   NT, groups of 128 61/66  80/83  139/142
+  // 14 experts of 4096 x 11008, down: 117, 106.  Eight waves for 41 experts of
+  // 2048 x 1408 60 / 39 us for up and gate / down, with four 43 / 30.  The layer
+  // of 32 pairs of 16 experts of 2048 x 1408 (up to 384 workgroups) with two and
+  // four waves: 37, 29.
+  constexpr int kTwoBelow = FIRST && !GROUPED ? 1536 : 4096;
   if (grid.x * grid.y <= 256)
     hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 8>), grid, dim3(512), 0, s, a);
-  else if (a.k < 4096 && grid.x * grid.y > 1024)
+  else if (a.k < kTwoBelow && grid.x * grid.y > 1024)
     hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 2>), grid, dim3(128), 0, s, a);
   else
     hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 4>), grid, dim3(256), 0, s, a);

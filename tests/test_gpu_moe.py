@@ -76,9 +76,9 @@ def test_odd_sizes(layout, group, hidden, inner, device):
         _check(_run(case, device), case)
 
 
-def _waves(grid, k):
+def _waves(grid, k, two_below):
     """Waves of a product's workgroups, which share K."""
-    return 8 if grid <= 256 else 2 if k < 4096 and grid > 1024 else 4
+    return 8 if grid <= 256 else 2 if k < two_below and grid > 1024 else 4
 
 
 def _up(n, to):
@@ -98,7 +98,7 @@ def test_several_pieces_of_k_a_wave(layout, group, tokens, top, experts, hidden,
     most = min(pairs, experts)
     hit = most + (pairs - most) // 16
     grids = _up(-(-_up(inner, 128) // 64), 8) * hit, _up(-(-hidden // 128), 8) * hit
-    assert waves == (_waves(grids[0], hidden), _waves(grids[1], inner))
+    assert waves == (_waves(grids[0], hidden, 4096 if group else 1536), _waves(grids[1], inner, 4096))
     dtype = "f16" if group == 64 else "bf16"
     case = _case(stable_seed("waves", layout, group, hidden, inner), tokens, 3, min(top, 2), hidden, inner, group=group,
                  layout=layout, dtype=dtype)
