@@ -31,11 +31,10 @@ from typing import Any
 from . import kernel_table as kt
 from .native import (
     _check,
-    _device_index,
+    _current_stream,
     _no_gradient,
     _on_stream,
     _require_device,
-    _stream_handle,
     _torch,
     _verified_library,
 )
@@ -98,26 +97,26 @@ class KVCache:
             raise ValueError(f"page_size must be a power of two from 16 to 1024; got {page_size}")
         if not 1 <= heads <= 65535 or pages < 1:
             raise ValueError(f"the cache needs at least one page and 1 to 65535 heads; got {pages} and {heads}")
-        at = self._addresses()
+        where = (codes.data_ptr, self.value_codes.data_ptr, self.key_scales.data_ptr, self.value_scales.data_ptr)
+        at = tuple(address() for address in where)
         packed = _CACHE.pack(*at, pages, heads, page_size, head_dim, bits)
         for name, value in (("pages", pages), ("kv_heads", heads), ("page_size", page_size), ("head_dim", head_dim),
-                            ("bits", bits), ("device", codes.device), ("_packed", (at, packed)), ("_workspaces", {})):
+                            ("bits", bits), ("device", codes.device), ("_packed", (where, at, packed)),
+                            ("_workspaces", {})):
             object.__setattr__(self, name, value)
 
     def __reduce__(self) -> Any:
         # copies and loaded caches are made of their own tensors
         return KVCache, (self.key_codes, self.value_codes, self.key_scales, self.value_scales)
 
-    def _addresses(self) -> tuple[int, int, int, int]:
-        return (self.key_codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(),
-                self.value_scales.data_ptr())
-
     @property
     def _native(self) -> bytes:
         """shk_kv_cache, at the addresses that the tensors have now."""
-        if self._packed[0] != self._addresses():
-            self.__post_init__()  # a tensor was given other memory: all checks again
-        return self._packed[1]
+        (kc, vc, ks, vs), at, packed = self._packed
+        if (kc(), vc(), ks(), vs()) == at:
+            return packed
+        self.__post_init__()  # a tensor was given other memory: all checks again
+        return self._packed[2]
 
 
 def new_kv_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, *, bits: int = 4,
@@ -200,7 +199,8 @@ def kv_cache_write(cache: KVCache, keys: Any, values: Any, slots: Any, *, stream
     if tokens == 0:
         return
     lib = _verified_library()
-    _check(lib, lib.amd_strix_halo_kernels_kv_write(_device_index(keys), _stream_handle(torch, keys, None), native,
+    index = keys.get_device()
+    _check(lib, lib.amd_strix_halo_kernels_kv_write(index, _current_stream(torch, index), native,
                                                     _rows(keys, values, slots, kind, tokens)))
 
 
@@ -223,7 +223,8 @@ def kv_cache_read(cache: KVCache, slots: Any, *, dtype: Any = None, stream: Any 
     values = torch.empty_like(keys)
     if tokens:
         lib = _verified_library()
-        _check(lib, lib.amd_strix_halo_kernels_kv_read(_device_index(keys), _stream_handle(torch, keys, None), native,
+        index = keys.get_device()
+        _check(lib, lib.amd_strix_halo_kernels_kv_read(index, _current_stream(torch, index), native,
                                                        _rows(keys, values, slots, kind, tokens)))
     return keys, values
 
@@ -339,7 +340,8 @@ def kv_cache_attention(
             if len(cache._workspaces) < 4096:
                 cache._workspaces[key] = nbytes
         work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _check(lib, lib.amd_strix_halo_kernels_kv_attention(_device_index(q), _stream_handle(torch, q, None), native,
+        index = q.get_device()
+        _check(lib, lib.amd_strix_halo_kernels_kv_attention(index, _current_stream(torch, index), native,
                                                             args(work, nbytes)))
     if given.requires_grad:
         out = _no_gradient(torch, "kv_cache_attention", out, given)

@@ -16,10 +16,10 @@ from . import kernel_table as kt
 from .metadata import SUPPORTED_SUBCHANNELS, GemmLayout, ScaleMode, ScaleSpec
 from .native import (
     _check,
+    _current_stream,
     _no_gradient,
     _on_stream,
     _require_device,
-    _stream_handle,
     _torch,
     _verified_library,
 )
@@ -155,5 +155,5 @@ def moe_swiglu_int4(
                      expert_ids.element_size(), expert_weights.data_ptr(), out.data_ptr(),
                      work.data_ptr(), nbytes)
     lib = _verified_library()
-    _check(lib, lib.amd_strix_halo_kernels_moe(index, _stream_handle(torch, x, None), args))
+    _check(lib, lib.amd_strix_halo_kernels_moe(index, _current_stream(torch, index), args))
     return _no_gradient(torch, "moe_swiglu_int4", out, *wanting)

@@ -218,10 +218,14 @@ def _torch() -> Any:
 def _stream_handle(torch: Any, tensor: Any, stream: Any | None) -> int:
     if stream is not None:
         return int(stream.cuda_stream)
+    return _current_stream(torch, _device_index(tensor))
+
+
+def _current_stream(torch: Any, index: int) -> int:
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is not None:  # the handle alone, without building a Stream object per call
-        return int(raw(_device_index(tensor)))
-    return int(torch.cuda.current_stream(tensor.device).cuda_stream)
+        return int(raw(index))
+    return int(torch.cuda.current_stream(index).cuda_stream)
 
 
 def _on_stream(torch: Any, tensor: Any, stream: Any) -> Any:
