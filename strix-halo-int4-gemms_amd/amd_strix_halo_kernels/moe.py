@@ -73,8 +73,8 @@ def moe_swiglu_int4(
     Scales are bf16: per-channel ``up_gate_scale[E, 2*inner]`` and
     ``down_scale[E, hidden]``, or with subchannel S ``[E, ceil(K/S), columns]``.
     Activations are not quantized; sums and the value between the products
-    are f32.  Takes up to 64 tokens (larger batches are ``ragged_dot_int4``'s),
-    1024 (token, expert) pairs and 1024 experts.  Returns [tokens, hidden] in
+    are f32.  Takes up to 64 tokens (``ragged_dot_int4`` takes more, quantized
+    and sorted by expert), 1024 (token, expert) pairs and 1024 experts.  Returns [tokens, hidden] in
     x's dtype.  Runs on the current stream, or on ``stream`` (which is then the
     current one for the call, its allocations included); nothing is read back
     to the host, and there is no gradient (asking the result for one raises).
@@ -133,7 +133,8 @@ def moe_swiglu_int4(
         raise ValueError("expert_ids must be contiguous")
     if tokens > MOE_MAX_TOKENS or tokens * top > MOE_MAX_PAIRS:
         raise ValueError(f"moe_swiglu_int4 takes up to {MOE_MAX_TOKENS} tokens and {MOE_MAX_PAIRS} (token, expert) "
-                         f"pairs; got {tokens} and {tokens * top}. Larger batches: ragged_dot_int4")
+                         f"pairs; got {tokens} and {tokens * top}. ragged_dot_int4 takes more, quantized and sorted by "
+                         "expert")
     if up_gate.numel() < 4 or down.numel() < 4:
         raise ValueError("up_gate and down must hold at least 4 bytes each")
     if experts > MOE_MAX_EXPERTS:

@@ -2,9 +2,9 @@
 // (shk_kvattn.h has the mathematics of a step).
 //
 // kv_stream_kernel serves a sequence's own tokens (and a shared prefix with up
-// to 64 query rows over the batch).  A workgroup is one key head and up to 16 * RT query rows;
-// its four waves take every fourth 64 tokens, each from memory to its own
-// registers, and are joined through LDS.  The tokens of all sequences are
+// to 64 query rows over the batch).  A workgroup is one key head and up to
+// 16 * RT query rows; its four waves take every fourth step of 16 * NB tokens,
+// each from memory to its own registers, and are joined through LDS.  The tokens of all sequences are
 // dealt out evenly: in pieces of 256, a workgroup gets the same number of
 // consecutive ones, whichever sequences they belong to.
 //
@@ -16,19 +16,27 @@
 // and sums.
 //
 // What bounds them, measured with 8 key heads of 128, four query heads each:
-// * 4 sequences of up to 131072 tokens, int4 (317 MB): stream 74 us, 4.3 TB/s
-//   of the 6.2 that a sum over memory reads at; the operands are made of 4-bit
-//   codes in as many instructions as the products take, and neither waits long.
-// * 32 sequences of up to 4096 tokens, int8 (134 MB): stream 36 us, join 6.
+// * 4 sequences of up to 131072 tokens, int4 (317 MB): stream 73 us, 4.3 TB/s
+//   of the 6.2 that a sum over memory reads at.  The vector unit, which widens
+//   the codes and does the softmax, is busy half of the time, the matrix unit
+//   a tenth.
+// * 32 sequences of up to 4096 tokens, int8 (134 MB): stream 35 us, join 6.
 //   A wave has four to eight steps, so its start (page numbers, then scales
 //   and keys) and its end are a third of it.
-// * 1 sequence of 1001 tokens: stream 9 us, join 4, two dependent launches; the
-//   host needs 13 to prepare them.
+// * 1 sequence of 1001 tokens: stream 8 us with 32 workgroups, join 5, two
+//   dependent launches; the host needs 13 to prepare them.
+// * 8 sequences of up to 6000 tokens with 40 rows of each of 2 key heads of 256,
+//   int8 (30 MB): stream 30 us, join 6.  Rows are tiles of 16, so three
+//   workgroups each fetch and widen the same tokens (94 MB), and the int8 heads
+//   of 256 spill 10 to 15 vector registers (44 to 60 bytes of scratch a lane).
 // * 64 sequences after a shared prefix of 65536 tokens, int4 (69 Gflop, 80 MB):
-//   119 us, 580 Tflop/s.  Each 64 tokens are widened once for 128 rows; the
-//   softmax (an exponential, a scale and a rounding for every score) takes the
-//   vector unit as long as the products take the matrix unit, and a wave does
-//   them in turn.
+//   119 us, 580 Tflop/s.  Each 64 tokens are widened once for 128 rows, twice
+//   for the 256 rows there are, and every wave reads them all from LDS for its
+//   32.  Vector unit busy 54%, matrix unit 23, LDS 25: a wave does widening,
+//   products and softmax in turn, two waves share a SIMD, and barriers keep
+//   them in step.
+// All forms of both kernels spill 21 to 98 scalar registers into lanes of
+// vector registers, most of them between the steps' addresses and page numbers.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -143,7 +151,7 @@ template <int BITS, int D, int RT, int TYPE>
 __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, StreamShared<D>& lds) {
   using Rows = KvRows<BITS, D, RT, TYPE>;
   // blocks of 16 tokens a wave takes at a time: half of the usual four where
-  // they would not fit the registers
+  // two row tiles or 256 columns take the registers (int8 at 256 spills even so)
   constexpr int NB = D * RT >= 256 ? 2 : 4;
   constexpr int kStep = 16 * NB, kPer = kPiece / kStep;
   constexpr int kPitch = StreamShared<D>::kPitch;
@@ -237,8 +245,7 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
     Rows rows;
     rows.begin(src, a.scale);
     // A step's V is asked for with the next step's K, so half of the bytes are
-    // always on their way, where the registers hold them.
-    constexpr bool kAhead = D * BITS * RT * NB <= 4096;
+    // always on their way.
     const int step0 = kPer * (piece - before) + wave, step_end = min(kPer * (mine - before), (n + kStep - 1) / kStep);
     const int step_last = step0 + (max(step_end - step0, 1) - 1) / 4 * 4;
     struct Keys {
@@ -263,13 +270,8 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
       u2 vss[NB];
 #pragma unroll
       for (int x = 0; x < NB; ++x) now.blk[x].load_v(kv, rows_now[x]), vss[x] = load_scales(kv.vs, rows_now[x]);
-      if constexpr (kAhead) {
-        find_rows(i + 4, rows_next);
-        load_keys(rows_next, next);
-      } else {
-        load_keys(rows_now, now);
-        find_rows(i + 4, rows_next);
-      }
+      find_rows(i + 4, rows_next);
+      load_keys(rows_next, next);
       pages(i + 8);
 #pragma unroll
       for (int x = 0; x < NB; ++x) rows_now[x] = rows_next[x];
@@ -310,18 +312,16 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
       Keys now, next;
       pages(step0);
       find_rows(step0, rows_now);
-      if constexpr (kAhead) load_keys(rows_now, now);
+      load_keys(rows_now, now);
       pages(step0 + 4);
 #pragma unroll 1
       for (int i = step0; i < step_end; i += 4) {
         step(i, now, next);
-        if constexpr (kAhead) {
 #pragma unroll
-          for (int x = 0; x < NB; ++x) {
+        for (int x = 0; x < NB; ++x) {
 #pragma unroll
-            for (int w = 0; w < KvBlock<BITS, D>::kK; ++w) now.blk[x].k[w] = next.blk[x].k[w];
-            now.scales[x] = next.scales[x];
-          }
+          for (int w = 0; w < KvBlock<BITS, D>::kK; ++w) now.blk[x].k[w] = next.blk[x].k[w];
+          now.scales[x] = next.scales[x];
         }
       }
     }

@@ -19,7 +19,8 @@
 // the products take 110 and 60.  16 tokens over 64 experts (41 hit) of 2048 x
 // 1408 in groups of 128: 35 and 26 us for 183 MB, where a wave has eight pieces
 // and its start (the pairs of its expert) and end (the sums of the waves) are
-// half of it.  One token through two experts: 10 us each, all latency.
+// half of it.  One token through two experts: 10 us each, with 48 and 32
+// workgroups on 256 CUs: ids, codes and the waves' join behind each other.
 //
 // Products are v_mfma_f32_16x16x32_bf16 with the weights in the rows and the
 // tokens in the columns.  A code v enters as v + 24, which one shift and one
@@ -717,10 +718,13 @@ void launch_waves(const MoeArgs& a, dim3 grid, hipStream_t s) {
   //   inner              704    1408   2816
   //   NN               60/63   74/79  125/130
   //   NT, groups of 128 61/66  80/83  139/142
-  // 14 experts of 4096 x 11008, down: 117, 106.  Eight waves for 41 experts of
-  // 2048 x 1408 60 / 39 us for up and gate / down, with four 43 / 30.  The layer
-  // of 32 pairs of 16 experts of 2048 x 1408 (up to 384 workgroups) with two and
-  // four waves: 37, 29.
+  // With two / four / eight for one of the products, up and gate then down:
+  //   16 tokens, 6 of 64 experts of 2048 x 1408, NT, groups of 128
+  //                                   64 / 68 / 81       64 / 66 / 75
+  //   61 tokens, 2 of 16 experts of 4096 x 11008, NN
+  //                                   241 / 234 / 274    250 / 234 / 240
+  //   16 tokens, 2 of 16 experts of 2048 x 1408 (408 and 272 workgroups), NN
+  //                                   33 / 29 / 32       32 / 29 / 30
   constexpr int kTwoBelow = FIRST && !GROUPED ? 1536 : 4096;
   if (grid.x * grid.y <= 256)
     hipLaunchKernelGGL((moe_product<LAYOUT, FIRST, TYPE, GROUPED, 8>), grid, dim3(512), 0, s, a);

@@ -22,9 +22,13 @@
 //   m = max(score) + exponent(max |v_scale|) - 13,
 // in powers of two and over what the row has met so far, not to the largest
 // score: 2^(score - m) * v_scale is then at most 2^15, so f16 does not
-// overflow and keeps all its bits down to 2^-27 of the largest term, whatever
-// the scales are (an exponent below -80 counts as -80, so that the sum cannot
-// overflow either).  For f16 outputs the term is split into two f16 terms,
+// overflow and keeps all its bits down to 2^-27 of the largest probability
+// times the largest scale.  The two need not be one token's: where they are
+// not, the error is small beside the largest |v|, not beside the output.  An
+// exponent below -80 counts as -80, so that the sum cannot overflow either.
+// Sums are joined in f32, and what lies below 2^-126 of a reference is lost:
+// nothing that counts as long as the largest scales of a row's pieces lie
+// within 2^126 of each other, so up to 2^46 beside values of zero.  For f16 outputs the term is split into two f16 terms,
 // because one rounding to 11 bits would be as large as the output's own.
 // Maxima, sums and outputs are f32.
 #pragma once
