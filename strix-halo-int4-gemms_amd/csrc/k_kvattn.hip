@@ -352,7 +352,10 @@ __device__ __forceinline__ void stream_pieces(const AttnArgs& a, int unit, Strea
       const float rbase = rtop == -__builtin_inff() ? 0.0f : rtop;
       float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sum += red_l[w][rr] * __builtin_amdgcn_exp2f(red_m[w][rr] - rbase);
+      for (int w = 0; w < 4; ++w) {
+        const float half = half_weight(red_m[w][rr] - rbase);
+        sum += red_l[w][rr] * half * half;
+      }
       const long at = __shfl(out_row[t], rr, 64);  // from the lane that holds the row
       if (at >= 0) {
         const int row = (tile * RT + t) * 16 + rr;
@@ -556,8 +559,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttnArgs a) {
       // A piece of NaN keys has reference -inf, so a weight of 0 does not mean
       // that it says nothing: 0 times its NaN sum and outputs stays NaN.
       const float2 ml = a.part_ml[place(p0 + lane)];
-      weight = __builtin_amdgcn_exp2f(ml.x - base);
-      sum += ml.y * weight;
+      const float half = half_weight(ml.x - base);
+      weight = half * half;
+      sum += ml.y * half * half;
     }
     const int here = min(count - p0, 64);
     for (int p = wave; p < here; p += 32) {  // eight loads at a time

@@ -26,9 +26,8 @@
 // times the largest scale.  The two need not be one token's: where they are
 // not, the error is small beside the largest |v|, not beside the output.  An
 // exponent below -80 counts as -80, so that the sum cannot overflow either.
-// Sums are joined in f32, and what lies below 2^-126 of a reference is lost:
-// nothing that counts as long as the largest scales of a row's pieces lie
-// within 2^126 of each other, so up to 2^46 beside values of zero.  For f16 outputs the term is split into two f16 terms,
+// Probabilities below 2^-126 of a reference are lost: a row's sum keeps its
+// bits for scales up to 2^100, and 12 of them for the largest there are.  For f16 outputs the term is split into two f16 terms,
 // because one rounding to 11 bits would be as large as the output's own.
 // Maxima, sums and outputs are f32.
 #pragma once
@@ -108,6 +107,10 @@ __device__ __forceinline__ float groups_sum(float v) {
 __device__ __forceinline__ float larger(float a, float b) {
   return __builtin_elementwise_maximum(a, __builtin_fabsf(b));
 }
+
+// 2^(x / 2).  References may lie up to 207 apart, which 2^x does not hold; a
+// sum that is large by as much is weighted with this twice.
+__device__ __forceinline__ float half_weight(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
 
 struct KvView {  // one key head of the cache
   const uint8_t *kc, *vc;
@@ -302,7 +305,7 @@ struct KvRows {
       top = groups_max(top) * qs[t] + up;
       top = top > m[t] + 1.0f ? top : m[t];
       const float base = top == -__builtin_inff() ? 0.0f : top;
-      const float alpha = __builtin_amdgcn_exp2f(m[t] - base);
+      const float half = half_weight(m[t] - base);
       m[t] = top;
       float sum = 0.0f;
 #pragma unroll
@@ -326,10 +329,10 @@ struct KvRows {
               if constexpr (kSplitP) pl[t][i / 2][4 * (i % 2) + r] = (_Float16)0.0f;
             }
       }
-      l[t] = l[t] * alpha + sum;
-      if (__any(alpha != 1.0f)) {
+      l[t] = l[t] * half * half + sum;
+      if (__any(half != 1.0f)) {
 #pragma unroll
-        for (int j = 0; j < kOut; ++j) o[t][j] *= alpha;
+        for (int j = 0; j < kOut; ++j) o[t][j] *= half * half;
       }
     }
   }

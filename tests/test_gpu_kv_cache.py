@@ -353,6 +353,24 @@ def test_value_scales_far_apart(dtype, device):
     _check(out, lse, q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("big", [2.0**50, 2.0**90])
+@pytest.mark.parametrize("prefix", [0, 600])
+@pytest.mark.parametrize("dim,bits", [(128, 4), (256, 8)])
+def test_large_values_beside_rows_of_zeros(big, prefix, dim, bits, device):
+    """Tokens whose values are zeros keep their share of the sum, whether large
+    values come before them, after them or in another piece."""
+    q, cache, table, lengths, pages = _case(stable_seed("zeros", prefix, dim, bits), [40, 700, 700, 200], page=64,
+                                            q_gain=0.1, dim=dim, bits=bits, prefix=prefix, device=device)
+    held = ~torch.isnan(cache.value_scales)
+    cache.value_scales[held] = 0.0
+    for b, at in ((0, 20), (1, 3), (2, 650), (3, 199)):
+        cache.value_scales[int(table[b, at // 64]), :, at % 64] = big
+    if prefix:
+        cache.value_scales[int(pages[4]), :, 7] = big / 4
+    out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+    _check(out, lse, q, cache, table, lengths, pages if prefix else None, prefix)
+
+
 def test_softmax_scale_and_strides(device):
     q, cache, table, lengths, _ = _case(5, [90, 33], queries=2, device=device)
     wide = torch.zeros((2, 2, 3 * q.shape[2], q.shape[3]), dtype=q.dtype, device=device)
