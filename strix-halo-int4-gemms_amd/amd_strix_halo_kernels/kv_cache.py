@@ -259,9 +259,11 @@ def kv_cache_attention(
     Returns ``softmax(softmax_scale * q k^T) v`` in q's shape and dtype
     (softmax_scale defaults to 1 / sqrt(head_dim)), and with ``return_lse``
     also the natural logarithm of each row's sum of exponentials (f32, q's
-    shape without head_dim).  A query that sees nothing gives 0 and -inf.
-    A page outside the cache makes its sequence's outputs NaN.  Scores, the
-    softmax and the sums are f32; products take the codes as they are.
+    shape without head_dim).  A query that sees nothing gives 0 and -inf, and
+    what it does not see may hold anything.  A length past the table counts as
+    the whole table, a negative one as 0; a page outside the cache makes its
+    sequence's outputs NaN.  Scores, the softmax and the sums are f32; products
+    take the codes as they are.
     """
     torch = _torch()
     native = cache._native  # first: the sizes that follow are the tensors' own

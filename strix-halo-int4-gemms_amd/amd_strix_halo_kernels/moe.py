@@ -42,6 +42,12 @@ def _require(name: str, tensor: Any, shape: tuple[int, ...], dtype: Any, what: s
         raise ValueError(f"{name} must be contiguous")
 
 
+def _outputs(torch: Any, out: Any, a: Any, b: Any, c: Any, d: Any) -> Any:
+    if a.requires_grad or b.requires_grad or c.requires_grad or d.requires_grad:
+        return _no_gradient(torch, "moe_swiglu_int4", out, a, b, c, d)
+    return out
+
+
 def moe_swiglu_int4(
     x: Any,
     up_gate: Any,
@@ -143,9 +149,8 @@ def moe_swiglu_int4(
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
         _require("out", out, (tokens, hidden), x.dtype, "(tokens, hidden)")
-    wanting = (x, expert_weights, up_gate_scale, down_scale)
     if tokens == 0:
-        return _no_gradient(torch, "moe_swiglu_int4", out, *wanting)
+        return _outputs(torch, out, x, expert_weights, up_gate_scale, down_scale)
     # h as two bf16 terms with rows of whole 128s, and f32 results, for each
     # pair; a counter for each 128 columns of the output
     nbytes = 4 * (tokens * top * (-(-inner // 128) * 128 + hidden) + -(-hidden // 128))
@@ -157,4 +162,4 @@ def moe_swiglu_int4(
                      work.data_ptr(), nbytes)
     lib = _verified_library()
     _check(lib, lib.amd_strix_halo_kernels_moe(index, _current_stream(torch, index), args))
-    return _no_gradient(torch, "moe_swiglu_int4", out, *wanting)
+    return _outputs(torch, out, x, expert_weights, up_gate_scale, down_scale)

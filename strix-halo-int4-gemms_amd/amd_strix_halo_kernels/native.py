@@ -254,9 +254,9 @@ def _no_gradient_function() -> Any:
 
 
 def _no_gradient(torch: Any, name: str, out: Any, *inputs: Any) -> Any:
-    """`out` of a call that has no backward pass.  Where one of its inputs asks
-    for a gradient, asking `out` for it raises instead of leaving it out."""
-    if not torch.is_grad_enabled() or not any(t.requires_grad for t in inputs):
+    """`out` of a call that has no backward pass, one of whose inputs asks for a
+    gradient: asking `out` for it raises instead of leaving it out."""
+    if not torch.is_grad_enabled():
         return out
     # an alias: a buffer that the caller reuses does not gather the graphs of its calls
     return _no_gradient_function().apply(name, out.detach(), *inputs)
