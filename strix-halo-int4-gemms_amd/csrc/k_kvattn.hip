@@ -16,7 +16,7 @@
 // and sums.
 //
 // What bounds them, measured with 8 key heads of 128, four query heads each:
-// * 4 sequences of up to 131072 tokens, int4 (317 MB): stream 73 us, 4.3 TB/s
+// * 4 sequences of up to 131072 tokens, int4 (317 MB): stream 70 us, 4.5 TB/s
 //   of the 6.2 that a sum over memory reads at.  The vector unit, which widens
 //   the codes and does the softmax, is busy half of the time, the matrix unit
 //   a tenth.
@@ -26,16 +26,16 @@
 // * 1 sequence of 1001 tokens: stream 8 us with 32 workgroups, join 5, two
 //   dependent launches; the host needs 13 to prepare them.
 // * 8 sequences of up to 6000 tokens with 40 rows of each of 2 key heads of 256,
-//   int8 (30 MB): stream 30 us, join 6.  Rows are tiles of 16, so three
+//   int8 (30 MB): stream 27 us, join 6.  Rows are tiles of 16, so three
 //   workgroups each fetch and widen the same tokens (94 MB), and the int8 heads
-//   of 256 spill 10 to 15 vector registers (44 to 60 bytes of scratch a lane).
+//   of 256 spill 4 to 8 vector registers (20 to 36 bytes of scratch a lane).
 // * 64 sequences after a shared prefix of 65536 tokens, int4 (69 Gflop, 80 MB):
-//   119 us, 580 Tflop/s.  Each 64 tokens are widened once for 128 rows, twice
+//   115 us, 600 Tflop/s.  Each 64 tokens are widened once for 128 rows, twice
 //   for the 256 rows there are, and every wave reads them all from LDS for its
-//   32.  Vector unit busy 54%, matrix unit 23, LDS 25: a wave does widening,
+//   32.  Vector unit busy 54%, matrix unit 24, LDS 26: a wave does widening,
 //   products and softmax in turn, two waves share a SIMD, and barriers keep
 //   them in step.
-// All forms of both kernels spill 21 to 98 scalar registers into lanes of
+// All forms of both kernels spill 12 to 98 scalar registers into lanes of
 // vector registers, most of them between the steps' addresses and page numbers.
 #include <hip/hip_runtime.h>
 

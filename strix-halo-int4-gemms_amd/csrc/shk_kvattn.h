@@ -260,7 +260,7 @@ struct KvRows {
   // anything, NaN too: it stays out of the row's scores, largest scale and
   // products.
   template <int NB>
-  __device__ __forceinline__ void soften(f4 (&s)[RT][NB], const f4 (&ks)[NB], const f4 (&vs)[NB], bool ends,
+  __device__ __forceinline__ void soften(f4 (&s)[RT][NB], const f4 (&ks)[NB], f4 (&vs)[NB], bool ends,
                                          const int (&limit)[RT], h8 (&p)[RT][NB / 2], h8 (&pl)[RT][NB / 2]) {
     const int g = (threadIdx.x & 63) / 16;
     auto unseen = [&](int t, int i, int r) { return 16 * i + 4 * g + r >= limit[t]; };
@@ -276,8 +276,10 @@ struct KvRows {
         for (int i = 0; i < NB; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
+            const float v = unseen(t, i, r) ? 0.0f : vs[i][r];
             if (unseen(t, i, r)) s[t][i][r] = -__builtin_inff();
-            most = larger(most, unseen(t, i, r) ? 0.0f : vs[i][r]);
+            if constexpr (RT == 1) vs[i][r] = v;
+            most = larger(most, v);
           }
         big[t] = max(big[t], groups_most(__float_as_uint(most)));
       }
@@ -319,7 +321,7 @@ struct KvRows {
           p[t][i / 2][4 * (i % 2) + r] = hi;
           if constexpr (kSplitP) pl[t][i / 2][4 * (i % 2) + r] = (_Float16)(w - (float)hi);
         }
-      if (ends) {
+      if (RT > 1 && ends) {  // a scale that one tile sees and another does not
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
