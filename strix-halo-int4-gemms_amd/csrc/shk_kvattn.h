@@ -27,9 +27,9 @@
 // not, the error is small beside the largest |v|, not beside the output.  An
 // exponent below -80 counts as -80, so that the sum cannot overflow either.
 // Probabilities below 2^-126 of a reference are lost: a row's sum keeps its
-// bits for scales up to 2^100, and 12 of them for the largest there are.  For f16 outputs the term is split into two f16 terms,
-// because one rounding to 11 bits would be as large as the output's own.
-// Maxima, sums and outputs are f32.
+// bits for scales up to 2^100, and 12 of them for the largest there are.  For
+// f16 outputs the term is split into two f16 terms, because one rounding to 11
+// bits would be as large as the output's own.  Maxima, sums and outputs are f32.
 #pragma once
 
 #include "shk_common.h"
