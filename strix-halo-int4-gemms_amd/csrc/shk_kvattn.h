@@ -316,7 +316,11 @@ struct KvRows {
         for (int r = 0; r < 4; ++r) {
           const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i][r], qs[t], -base));
           sum += pv;
-          const float w = pv * vs[i][r];
+          float w = pv * vs[i][r];
+          // w as rounded to f32 for both terms: otherwise one use of hi is made
+          // by v_fma_mixlo_f16, which rounds the product once, and where w lies
+          // between two f16 values the terms are of different ones
+          if constexpr (kSplitP) asm("" : "+v"(w));
           const _Float16 hi = (_Float16)w;
           p[t][i / 2][4 * (i % 2) + r] = hi;
           if constexpr (kSplitP) pl[t][i / 2][4 * (i % 2) + r] = (_Float16)(w - (float)hi);

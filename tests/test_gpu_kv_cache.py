@@ -353,6 +353,18 @@ def test_value_scales_far_apart(dtype, device):
     _check(out, lse, q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("dim,bits,ratio,prefix", [(64, 4, 7, 0), (128, 8, 7, 0), (256, 4, 7, 0), (128, 4, 20, 0),
+                                                   (64, 8, 7, 10)])
+def test_f16_probabilities_keep_both_terms(dim, bits, ratio, prefix, device):
+    """The two f16 terms of a probability are of one rounding: with small scores
+    the bound is a fraction of what a term off by its last bit does."""
+    q, cache, table, lengths, pages = _case(stable_seed("terms", dim, bits, ratio, prefix), [10] * 300, ratio=ratio,
+                                            kv_heads=3, dim=dim, bits=bits, dtype="f16", prefix=prefix, q_gain=0.02,
+                                            page=64, device=device)
+    out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+    _check(out, lse, q, cache, table, lengths, pages if prefix else None, prefix)
+
+
 @pytest.mark.parametrize("big", [2.0**50, 2.0**90])
 @pytest.mark.parametrize("prefix", [0, 600])
 @pytest.mark.parametrize("dim,bits", [(128, 4), (256, 8)])
