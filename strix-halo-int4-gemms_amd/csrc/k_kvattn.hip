@@ -89,8 +89,12 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, long row, int d, f4
   *reinterpret_cast<uint2*>(a.out + row * D + d) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
 }
 
+// The power of two of l goes off against the one in m first: log2(l) would
+// round to that of the value scales, up to 2^-18.
 __device__ __forceinline__ float natural_lse(float m, float l) {
-  return m == -__builtin_inff() && !(l != l) ? -__builtin_inff() : (m + __log2f(l)) * 0.6931471805599453f;
+  const float whole = m + (float)__builtin_amdgcn_frexp_expf(l);
+  const float lse = (whole + __log2f(__builtin_amdgcn_frexp_mantf(l))) * 0.6931471805599453f;
+  return m == -__builtin_inff() && !(l != l) ? m : lse;
 }
 
 // The first of `total` pieces that workgroup j of `spread` takes, and the

@@ -353,6 +353,17 @@ def test_value_scales_far_apart(dtype, device):
     _check(out, lse, q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("value", [0.0, 2.0**-70, 1.0, 2.0**90])
+@pytest.mark.parametrize("prefix", [0, 3])
+def test_lse_of_equal_scores(value, prefix, device):
+    """The logarithm of the number of tokens, whatever the values' size."""
+    q, cache, table, lengths, pages = _case(stable_seed("equal"), list(range(1, 18)), prefix=prefix, q_gain=0.0,
+                                            page=64, device=device)
+    cache.value_scales[~torch.isnan(cache.value_scales)] = value
+    out, lse = _attend(q, cache, table, lengths, pages, prefix, device)
+    _check(out, lse, q, cache, table, lengths, pages if prefix else None, prefix)
+
+
 @pytest.mark.parametrize("dim,bits,ratio,prefix", [(64, 4, 7, 0), (128, 8, 7, 0), (256, 4, 7, 0), (128, 4, 20, 0),
                                                    (64, 8, 7, 10)])
 def test_f16_probabilities_keep_both_terms(dim, bits, ratio, prefix, device):
