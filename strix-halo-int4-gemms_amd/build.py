@@ -79,7 +79,7 @@ def translation_units() -> list[tuple[str, Path, list[str]]]:
 
 
 def decode_units() -> list[tuple[str, Path, list[str]]]:
-    """The decode step's operators: no inline assembly, default scheduler."""
+    """The decode step's operators, with the default scheduler."""
     return [
         ("kvcache", CSRC / "k_kvcache.hip", []),
         ("kvattn", CSRC / "k_kvattn.hip", []),
