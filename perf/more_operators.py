@@ -1,0 +1,621 @@
+"""The operators of a step that verifies drafted tokens, as cases that can be timed.
+
+Beside the cached attention, a step of a serving loop that drafts tokens runs
+
+* ``plan``: pages and slots of the new tokens, and the pages of sequences that
+  ended back to the pool, on the device (``kv_pages_step``);
+* ``linear`` and ``weight_grad``: products in 8-bit floating point with a scale
+  for each block of 128 (``quantize_fp8``, ``mm_fp8``): activations times a
+  layer's weights, and the gradient of those weights, which a layer that is
+  trained in these types needs; ``quantize`` times the conversion alone;
+* ``rotate``: the norm of each query and key head and its rotation by
+  position, in one pass (``rotate_qk``), the keys, with their values, into the
+  quantized cache where the case says so;
+* ``verify``: which drafted tokens the target's probabilities keep, and the
+  token that follows them (``verify_draft``).
+
+A case is a dict of plain values:
+
+* linear: ``tokens``, ``inputs`` (K), ``outputs`` (N), ``dtype`` of what goes in
+  and comes out; weight_grad: the same, its result ``outputs`` x ``inputs`` in
+  float32, the output's gradient in e5m2 where ``wide`` is true;
+* quantize: ``tokens``, ``inputs``, ``rows`` (1 or 128 rows that share a scale),
+  ``transpose``, ``dtype``;
+* rotate: ``tokens``, ``heads``, ``kv_heads``, ``head_dim``, ``rotated`` (values of
+  a head that turn), ``interleaved``, ``norm``, ``scaling`` (none, linear, ntk,
+  yarn), ``first`` (the first position), ``bits`` (0: keys come out, else the
+  cache's bits), ``page``, ``dtype``;
+* plan: ``batch``, ``new`` (most new tokens of a sequence), ``length`` (most
+  cached tokens), ``page``, ``ends`` (some sequences end), ``few`` (the pool
+  runs out of pages);
+* verify: ``batch``, ``drafts``, ``vocab``, ``dtype`` of the probabilities,
+  ``greedy`` (the draft has no probabilities).
+"""
+
+import math
+import os
+import random
+import sys
+
+import torch
+
+sys.path.insert(0, os.path.abspath("strix-halo-int4-gemms_amd"))
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+BLOCK = 128  # values of K that share a scale, and rows of a weight
+E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
+LARGEST = {E4M3: 448.0, E5M2: 57344.0}
+
+
+# ---------------------------------------------------------------------------
+# Cases
+
+
+def _linear(name, tokens, inputs, outputs, *, dtype="bf16", op="linear", wide=False):
+    case = {"op": op, "tokens": tokens, "inputs": inputs, "outputs": outputs, "dtype": dtype, "wide": wide}
+    return {"name": name, **case} if name else case
+
+
+def _quantize(name, tokens, inputs, *, rows=1, transpose=False, dtype="bf16"):
+    case = {"op": "quantize", "tokens": tokens, "inputs": inputs, "rows": rows, "transpose": transpose, "dtype": dtype}
+    return {"name": name, **case} if name else case
+
+
+def _rotate(name, tokens, *, heads=32, kv_heads=8, head_dim=128, rotated=None, interleaved=False, norm=True,
+            scaling="none", first=0, bits=0, page=64, dtype="bf16"):
+    case = {"op": "rotate", "tokens": tokens, "heads": heads, "kv_heads": kv_heads, "head_dim": head_dim,
+            "rotated": rotated or head_dim, "interleaved": interleaved, "norm": norm, "scaling": scaling,
+            "first": first, "bits": bits, "page": page, "dtype": dtype}
+    return {"name": name, **case} if name else case
+
+
+def _plan(name, batch, new, length, *, page=64, ends=False, few=False):
+    case = {"op": "plan", "batch": batch, "new": new, "length": length, "page": page, "ends": ends, "few": few}
+    return {"name": name, **case} if name else case
+
+
+def _verify(name, batch, drafts, vocab, *, dtype="f32", greedy=False):
+    case = {"op": "verify", "batch": batch, "drafts": drafts, "vocab": vocab, "dtype": dtype, "greedy": greedy}
+    return {"name": name, **case} if name else case
+
+
+def listed():
+    return [
+        # A decode step's batch through one projection: the weights are
+        # streamed once.
+        _linear("linear_step", 16, 4096, 11008),
+        # A chunk of a prompt, of an odd length, through a narrow projection.
+        _linear("linear_chunk", 333, 2048, 1408, dtype="f16"),
+        # A long prompt, or a training step's forward.
+        _linear("linear_prompt", 4096, 4096, 11008),
+        # The weights' gradient of such a step over a ragged number of tokens;
+        # the output's gradient needs e5m2's range.
+        _linear("weight_grad", 8111, 4096, 4096, op="weight_grad", wide=True),
+        # A layer's weights after an update, for the product that gives the
+        # input's gradient.
+        _quantize("quantize_weights", 11008, 4096, rows=128, transpose=True),
+        # Five drafted tokens and one of each of four sequences: normed,
+        # rotated, and the keys and values into the int4 cache.
+        _rotate("rotate_step", 24, first=1500, bits=4),
+        # A long prompt's queries and keys.
+        _rotate("rotate_prompt", 8191),
+        # Part of each head in pairs side by side, no norm, at far positions
+        # of a context that was stretched eightfold.
+        _rotate("rotate_far", 2050, heads=16, kv_heads=2, head_dim=256, rotated=64, interleaved=True, norm=False,
+                scaling="yarn", first=250000, dtype="f16"),
+        # Every step: drafts and one token of each of 64 sequences, some of
+        # which end.
+        _plan("plan_step", 64, 6, 4000, ends=True),
+        # Many prompts arrive at once, and the pool has too few pages.
+        _plan("plan_prompts", 500, 300, 2000, page=16, ends=True, few=True),
+        # One user, five drafted tokens.
+        _verify("verify_one", 1, 5, 32000),
+        # A busy server's step over a large vocabulary.
+        _verify("verify_batch", 61, 5, 131072),
+    ]
+
+
+def _log(rng, lo, hi, step=1):
+    """A multiple of `step` in [lo, hi], spread over the logarithm."""
+    v = math.exp(rng.uniform(math.log(lo), math.log(hi)))
+    return min(hi // step, max(-(-lo // step), round(v / step))) * step
+
+
+def draw(rng):
+    op = rng.choices(["linear", "weight_grad", "quantize", "rotate", "plan", "verify"], [30, 10, 10, 20, 14, 16])[0]
+    dtype = rng.choice(["bf16", "bf16", "f16", "f32"])
+    if op in ("linear", "weight_grad"):
+        inputs, outputs = _log(rng, 64, 14336, rng.choice([1, 16, 128])), _log(rng, 64, 14336, rng.choice([1, 16, 128]))
+        tokens = _log(rng, 1, max(1, min(8192, 4096 * 4096 * 11008 // (inputs * outputs))))
+        return _linear("", tokens, inputs, outputs, dtype=dtype, op=op, wide=op != "linear" and rng.random() < 0.5)
+    if op == "quantize":
+        inputs = _log(rng, 64, 14336, rng.choice([1, 16, 128]))
+        return _quantize("", _log(rng, 1, 11008 * 4096 // max(4096, inputs)), inputs, rows=rng.choice([1, 128]),
+                         transpose=rng.random() < 0.5, dtype=dtype)
+    if op == "rotate":
+        head_dim, kv_heads = rng.choice([64, 64, 80, 96, 128, 128, 192, 256]), rng.choice([1, 2, 4, 8, 8, 16])
+        heads = kv_heads * rng.choice([1, 2, 4, 4, 7, 8])
+        most = 8191 * 40 * 128 // ((heads + kv_heads) * head_dim * (2 if dtype == "f32" else 1))
+        bits = rng.choice([0, 0, 4, 8]) if head_dim in (64, 128, 256) else 0
+        return _rotate("", _log(rng, 1, min(8191, most) // (2 if bits else 1)), heads=heads, kv_heads=kv_heads,
+                       head_dim=head_dim, rotated=rng.choice([head_dim, head_dim, head_dim // 2, 16]),
+                       interleaved=rng.random() < 0.4, norm=rng.random() < 0.6,
+                       scaling=rng.choice(["none", "none", "linear", "ntk", "yarn"]),
+                       first=rng.choice([0, _log(rng, 1, 1000000)]), bits=bits, page=rng.choice([16, 32, 64, 128]),
+                       dtype=dtype)
+    if op == "plan":
+        batch = _log(rng, 1, 1024)
+        return _plan("", batch, _log(rng, 1, max(1, min(4096, 150000 // batch))),
+                     _log(rng, 1, max(1, min(65536, 2000000 // batch))), page=rng.choice([16, 32, 64, 128]),
+                     ends=rng.random() < 0.5, few=rng.random() < 0.3)
+    batch, vocab = _log(rng, 1, 128), _log(rng, 300, 131072)
+    drafts = rng.choice([1, 2, 3, 4, 5, 5, 8])
+    while batch * (drafts + 1) * vocab > 61 * 6 * 131072:
+        vocab //= 2
+    return _verify("", batch, drafts, vocab, dtype=dtype, greedy=rng.random() < 0.25)
+
+
+# ---------------------------------------------------------------------------
+# Inputs
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+def _activations(gen, rows, cols, dtype, spread=1.0):
+    """Normalised activations (or gradients) with a few large channels, rows of uneven size."""
+    x = torch.randn((rows, cols), device="cuda", generator=gen)
+    x[:, :: 61] *= 8.0
+    return (x * torch.exp(spread * torch.randn((rows, 1), device="cuda", generator=gen))).to(dtype)
+
+
+def _prepare_linear(case, gen):
+    tokens, k, n, dtype = case["tokens"], case["inputs"], case["outputs"], DTYPES[case["dtype"]]
+    state = {"x": _activations(gen, tokens, k, dtype, 0.3), "dtype": dtype, "wide": case["wide"]}
+    if case["op"] == "weight_grad":
+        # of the size that a loss averaged over the tokens leaves
+        state["grad"] = (_activations(gen, tokens, n, torch.float32, 2.0) * 1e-3).to(dtype)
+        return state
+    w = torch.randn((n, k), device="cuda", generator=gen) * 110.0
+    state["weights"] = w.clamp(-448.0, 448.0).to(E4M3)
+    state["scales"] = (0.5 + torch.rand((_blocks(n), _blocks(k)), device="cuda", generator=gen)) / (110.0 * k**0.5)
+    return state
+
+
+def _prepare_quantize(case, gen):
+    return {"x": _activations(gen, case["tokens"], case["inputs"], DTYPES[case["dtype"]]), "rows": case["rows"],
+            "transpose": case["transpose"]}
+
+
+def _frequencies(case):
+    """Radians a position of each pair that turns, and what cosines and sines
+    are multiplied by."""
+    half, base, factor, trained = case["rotated"] // 2, 10000.0, 8.0, 32768
+    if case["scaling"] == "ntk":  # the slowest pair is slowed by the factor, the fastest not at all
+        base *= factor ** (half / max(1, half - 1))
+    plain = [base ** (-i / half) for i in range(half)]
+    if case["scaling"] == "linear":
+        return [f / factor for f in plain], 1.0
+    if case["scaling"] != "yarn":
+        return plain, 1.0
+
+    def pair(turns):  # the pair that turns so often over the trained context
+        return half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)
+
+    low, high = max(0, math.floor(pair(32.0))), min(half - 1, math.ceil(pair(1.0)))
+    slow = [min(1.0, max(0.0, (i - low) / max(1e-3, high - low))) for i in range(half)]
+    return [f * (1 - s) + f / factor * s for f, s in zip(plain, slow)], 0.1 * math.log(factor) + 1.0
+
+
+def _prepare_rotate(case, gen):
+    tokens, dim, dtype, page = case["tokens"], case["head_dim"], DTYPES[case["dtype"]], case["page"]
+    heads, kv_heads = case["heads"], case["kv_heads"]
+    # queries, keys and values as one projection leaves them
+    qkv = torch.randn((tokens, heads + 2 * kv_heads, dim), device="cuda", generator=gen)
+    qkv[:, :, : dim // 16] *= 5.0
+    qkv = qkv.to(dtype)
+    frequencies, amplitude = _frequencies(case)
+    # prompts and drafts side by side: positions run on in pieces
+    at = torch.arange(tokens, device="cuda")
+    state = {"q": qkv[:, :heads], "k": qkv[:, heads:heads + kv_heads], "v": qkv[:, heads + kv_heads:],
+             "positions": case["first"] + at % 700 + 3 * (at // 700), "rotated": case["rotated"],
+             "interleaved": case["interleaved"], "frequencies": frequencies, "amplitude": amplitude,
+             "bits": case["bits"], "dtype": dtype, "norms": None, "eps": 1e-6}
+    if case["norm"]:
+        norms = 0.5 + torch.rand((2, dim), device="cuda", generator=gen)
+        state["norms"] = norms.to(dtype)
+    if case["bits"]:
+        pages = -(-tokens // page) + 3
+        order = torch.randperm(pages, device="cuda", generator=gen)
+        state["slots"] = order[at // page] * page + at % page
+        shape, width = (pages, kv_heads, page), dim * case["bits"] // 8
+        codes = torch.uint8 if case["bits"] == 4 else torch.int8
+        state["pool"] = {part + kind: torch.zeros((*shape, width) if kind == "_codes" else shape,
+                                                  dtype=codes if kind == "_codes" else torch.bfloat16, device="cuda")
+                         for part in ("key", "value") for kind in ("_codes", "_scales")}
+    if own:
+        import amd_strix_halo_kernels as shk
+
+        state["rotary"] = shk.new_rotary(frequencies, amplitude=amplitude, interleaved=case["interleaved"],
+                                         device="cuda")
+        if case["bits"]:
+            state["cache"] = shk.KVCache(**state["pool"])  # over the same tensors
+    return state
+
+
+def _prepare_plan(case, gen):
+    batch, page = case["batch"], case["page"]
+    width = -(-(case["length"] + case["new"]) // page) + 1
+    lengths = (torch.rand(batch, device="cuda", generator=gen) * (case["length"] + 1)).int().clamp(max=case["length"])
+    new = 1 + (torch.rand(batch, device="cuda", generator=gen) * case["new"]).int().clamp(max=case["new"] - 1)
+    if case["ends"]:  # a negative number of new tokens: the sequence ended
+        new[torch.rand(batch, device="cuda", generator=gen) < 0.15] = -1
+    # drafts that were not kept leave a page more than the length asks for
+    owned = (lengths + page - 1) // page + (torch.rand(batch, device="cuda", generator=gen) < 0.1).int()
+    total = int(owned.sum())
+    spare = 3 + (batch * (-(-case["new"] // page)) // (4 if case["few"] else 1))
+    order = torch.randperm(batch * width + spare, device="cuda", generator=gen).int()
+    table = torch.zeros((batch, width), dtype=torch.int32, device="cuda")
+    held = torch.arange(width, device="cuda") < owned[:, None]
+    table[held] = order[:total]
+    free = torch.zeros(batch * width + spare, dtype=torch.int32, device="cuda")
+    free[:spare] = order[batch * width:]
+    # all of it in one buffer, which a pass starts from
+    parts = {"page_table": table, "lengths": lengths, "owned": owned.int(), "free_pages": free,
+             "free_count": torch.tensor([spare], dtype=torch.int32, device="cuda")}
+    start = torch.cat([t.flatten() for t in parts.values()])
+    state = {"page": page, "new": new, "capacity": batch * case["new"], "start": start,
+             "shapes": {name: tuple(t.shape) for name, t in parts.items()}}
+    if own:
+        import amd_strix_halo_kernels as shk
+
+        state["now"] = start.clone()
+        state["handle"] = shk.KVPages(page_size=page, **_pages(state["now"], state["shapes"]))
+    return state
+
+
+def _pages(flat, shapes):
+    """The tensors of a page pool, as views of one buffer."""
+    sizes = [math.prod(shape) for shape in shapes.values()]
+    return {name: part.view(shapes[name]) for name, part in zip(shapes, flat.split(sizes))}
+
+
+def _prepare_verify(case, gen):
+    batch, drafts, vocab, dtype = case["batch"], case["drafts"], case["vocab"], DTYPES[case["dtype"]]
+    logits = 3.0 * torch.randn((batch, drafts + 1, vocab), device="cuda", generator=gen)
+    target = torch.softmax(logits, dim=-1)
+    # a draft model that is right for the most part
+    near = torch.softmax(logits[:, :drafts] + 0.7 * torch.randn((batch, drafts, vocab), device="cuda", generator=gen),
+                         dim=-1)
+    tokens = torch.multinomial(near.flatten(0, 1), 1, generator=gen).view(batch, drafts)
+    if case["greedy"]:
+        tokens = near.argmax(dim=-1)
+    return {"target": target.to(dtype), "draft": None if case["greedy"] else near.to(dtype), "tokens": tokens,
+            "uniforms": torch.rand((batch, drafts + 1), device="cuda", generator=gen)}
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    how = {"quantize": _prepare_quantize, "rotate": _prepare_rotate, "plan": _prepare_plan,
+           "verify": _prepare_verify}.get(case["op"], _prepare_linear)
+    return {"op": case["op"], **how(case, gen)}
+
+
+# ---------------------------------------------------------------------------
+# One pass
+
+
+def run(state):
+    return (_run_own if own else _run_plain)(state)
+
+
+def _run_own(state):
+    import amd_strix_halo_kernels as shk
+
+    op = state["op"]
+    if op == "linear":
+        codes, scales = shk.quantize_fp8(state["x"])
+        return shk.mm_fp8(codes, state["weights"], a_scale=scales, b_scale=state["scales"], out_dtype=state["dtype"])
+    if op == "weight_grad":
+        g, gs = shk.quantize_fp8(state["grad"], transpose=True, dtype=E5M2 if state["wide"] else E4M3)
+        x, xs = shk.quantize_fp8(state["x"], transpose=True)
+        return shk.mm_fp8(g, x, a_scale=gs, b_scale=xs, out_dtype=torch.float32)
+    if op == "quantize":
+        codes, scales = shk.quantize_fp8(state["x"], block_rows=state["rows"], transpose=state["transpose"])
+        return codes.to(torch.bfloat16), scales
+    if op == "rotate":
+        q_weight, k_weight = state["norms"] if state["norms"] is not None else (None, None)
+        how = {"q_weight": q_weight, "k_weight": k_weight, "eps": state["eps"]}
+        if not state["bits"]:
+            return shk.rotate_qk(state["q"], state["k"], state["positions"], state["rotary"], **how)
+        q = shk.rotate_qk(state["q"], state["k"], state["positions"], state["rotary"], cache=state["cache"],
+                          values=state["v"], slots=state["slots"], **how)
+        return q, *shk.kv_cache_read(state["cache"], state["slots"], dtype=state["dtype"])
+    if op == "plan":
+        state["now"].copy_(state["start"])  # a step changes the pool: every pass starts from the same
+        step = shk.kv_pages_step(state["handle"], state["new"], state["capacity"])
+        return {"slots": step.slots, "positions": step.positions, "sequences": step.sequences, "starts": step.starts,
+                **_pages(state["now"], state["shapes"])}
+    return shk.verify_draft(state["target"], state["draft"], state["tokens"], state["uniforms"])
+
+
+def _run_plain(state):
+    return {"linear": _plain_linear, "weight_grad": _plain_weight_grad, "quantize": _plain_quantize,
+            "rotate": _plain_rotate, "plan": _plain_plan, "verify": _plain_verify}[state["op"]](state)
+
+
+def _plain_codes(x, rows=1, kind=E4M3):
+    """Codes (as float32 values) and scales of x: of each block of `rows` rows
+    and 128 columns, the largest magnitude over the type's largest value."""
+    r, c = x.shape
+    pad = torch.nn.functional.pad(x.float(), (0, -c % BLOCK, 0, -r % rows))
+    pad = pad.reshape(-1, rows, _blocks(c), BLOCK)
+    scales = pad.abs().amax(dim=(1, 3)) / torch.full((), LARGEST[kind], device=x.device)
+    wide = scales[:, None, :, None]
+    codes = torch.where(wide > 0, pad / wide, 0.0).clamp(-LARGEST[kind], LARGEST[kind])
+    return codes.to(kind).float().reshape(-1, _blocks(c) * BLOCK)[:r, :c], scales
+
+
+def _spread(scales, rows, shape):
+    """Scales of blocks of rows x 128, one for each value of `shape`."""
+    return scales.repeat_interleave(rows, 0)[: shape[0]].repeat_interleave(BLOCK, 1)[:, : shape[1]]
+
+
+def _plain_linear(state):
+    codes, scales = _plain_codes(state["x"])
+    w = state["weights"].float() * _spread(state["scales"], BLOCK, state["weights"].shape)
+    return ((codes * _spread(scales, 1, codes.shape)) @ w.t()).to(state["dtype"])
+
+
+def _plain_weight_grad(state):
+    g, gs = _plain_codes(state["grad"].t(), kind=E5M2 if state["wide"] else E4M3)
+    x, xs = _plain_codes(state["x"].t())
+    return (g * _spread(gs, 1, g.shape)) @ (x * _spread(xs, 1, x.shape)).t()
+
+
+def _plain_quantize(state):
+    x = state["x"].t() if state["transpose"] else state["x"]
+    codes, scales = _plain_codes(x, rows=state["rows"])
+    return codes.to(torch.bfloat16), scales
+
+
+def _plain_turned(state, x, weight, cos, sin):
+    """A head's norm and rotation in 32 bits; [tokens, heads, head_dim]."""
+    x = x.float()
+    if weight is not None:
+        x = x * torch.rsqrt(x.square().mean(dim=-1, keepdim=True) + state["eps"]) * weight.float()
+    n = state["rotated"]
+    if state["interleaved"]:
+        a, b = x[..., 0:n:2], x[..., 1:n:2]
+        turned = torch.stack((a * cos - b * sin, b * cos + a * sin), dim=-1).flatten(-2)
+    else:
+        a, b = x[..., : n // 2], x[..., n // 2:n]
+        turned = torch.cat((a * cos - b * sin, b * cos + a * sin), dim=-1)
+    return torch.cat((turned, x[..., n:]), dim=-1).to(state["dtype"])
+
+
+def _pack(codes):
+    codes = codes.to(torch.uint8) & 15
+    return codes[..., 0::2] | (codes[..., 1::2] << 4)
+
+
+def _unpack(packed):
+    return torch.stack(((packed << 4).view(torch.int8) >> 4, packed.view(torch.int8) >> 4), dim=-1).flatten(-2)
+
+
+def _plain_rotate(state):
+    # angles of far positions need 64 bits
+    turn = torch.tensor(state["frequencies"], dtype=torch.float64, device="cuda")
+    angle = (state["positions"].double()[:, None] * turn)[:, None]
+    cos = (torch.cos(angle) * state["amplitude"]).float()
+    sin = (torch.sin(angle) * state["amplitude"]).float()
+    q_weight, k_weight = state["norms"] if state["norms"] is not None else (None, None)
+    q = _plain_turned(state, state["q"], q_weight, cos, sin)
+    k = _plain_turned(state, state["k"], k_weight, cos, sin)
+    if not state["bits"]:
+        return q, k
+    pool, bits, slots = state["pool"], state["bits"], state["slots"]
+    page, most = pool["key_scales"].shape[2], 7 if bits == 4 else 127
+    at, offset = slots // page, slots % page
+    x = torch.stack((k, state["v"])).float()
+    largest = x.abs().amax(dim=-1)
+    scales = (largest / torch.full_like(largest, most)).to(torch.bfloat16)
+    wide = scales.float()[..., None]
+    codes = torch.where(wide > 0, torch.round(x / wide), 0.0).clamp(-most, most).to(torch.int8)
+    codes = _pack(codes) if bits == 4 else codes
+    back = []
+    for i, part in enumerate(("key", "value")):
+        pool[part + "_codes"][at, :, offset] = codes[i]
+        pool[part + "_scales"][at, :, offset] = scales[i]
+        stored = pool[part + "_codes"][at, :, offset]
+        stored = (_unpack(stored) if bits == 4 else stored).float()
+        back.append((stored * pool[part + "_scales"][at, :, offset].float()[..., None]).to(state["dtype"]))
+    return q, *back
+
+
+def _plain_plan(state):
+    page, new, device = state["page"], state["new"].long(), state["new"].device
+    pages = _pages(state["start"].clone(), state["shapes"])
+    table, lengths, owned = pages["page_table"], pages["lengths"].long(), pages["owned"].long()
+    free, count = pages["free_pages"], pages["free_count"].long()
+    batch, width = table.shape
+    ended = new < 0
+    # pages of ended sequences go on top of the free ones, in order
+    column = torch.arange(width, device=device)
+    back = torch.where(ended, owned, 0)
+    given = (column < back[:, None]).nonzero()
+    free[count + torch.arange(given.shape[0], device=device)] = table[given[:, 0], given[:, 1]]
+    count = count + given.shape[0]
+    lengths, owned = torch.where(ended, 0, lengths), torch.where(ended, 0, owned)
+    # what each sequence asks for, in order; one that does not fit gets none
+    new = new.clamp(min=0)
+    starts = torch.cat((new.new_zeros(1), new.cumsum(0)))
+    total = (lengths + new + page - 1) // page
+    fits = total <= width
+    asks = torch.where(fits, (total - owned).clamp(min=0), 0)
+    upto = asks.cumsum(0)
+    fits &= (asks == 0) | (upto <= count)
+    gets = torch.where(fits, asks, 0)
+    fresh = (column >= owned[:, None]) & (column < (owned + gets)[:, None])
+    index = count - 1 - ((upto - asks)[:, None] + column - owned[:, None])
+    table = torch.where(fresh, free[index.clamp(min=0)], table)
+    # tokens in order of their sequences
+    at = torch.arange(state["capacity"], device=device)
+    which = torch.searchsorted(starts[1:].contiguous(), at, right=True)
+    real = at < starts[-1]
+    which = which.clamp(max=batch - 1)
+    position = lengths[which] + at - starts[which]
+    slot = table[which, (position // page).clamp(max=width - 1)].long() * page + position % page
+    return {"slots": torch.where(real & fits[which], slot, -1), "positions": torch.where(real, position, 0).int(),
+            "sequences": torch.where(real, which, -1).int(), "starts": starts.int(), "page_table": table,
+            "lengths": torch.where(fits, lengths + new, lengths).int(), "owned": (owned + gets).int(),
+            "free_pages": free, "free_count": (count - gets.sum()).int()}
+
+
+def _plain_verify(state):
+    p, tokens, u = state["target"].double(), state["tokens"], state["uniforms"].double()
+    batch, drafts = tokens.shape
+    at = tokens[..., None]
+    px = p[:, :drafts].gather(-1, at)[..., 0]
+    qx = torch.ones_like(px) if state["draft"] is None else state["draft"].gather(-1, at)[..., 0].double()
+    keeps = u[:, :drafts] * qx < px
+    kept = keeps.long().cumprod(dim=1).sum(dim=1)
+    row = torch.arange(batch, device=p.device)
+    # what is left of the target where the draft was wrong; all of it after the last draft
+    last = p[row, kept]
+    wrong, turn = kept < drafts, kept.clamp(max=drafts - 1)
+    if state["draft"] is None:
+        gone = torch.zeros_like(last).scatter_(1, tokens[row, turn][:, None], math.inf)
+    else:
+        gone = state["draft"][row, turn].double()
+    rest = torch.where(wrong[:, None], (last - gone).clamp(min=0.0), last)
+    rest = torch.where(rest.sum(dim=1, keepdim=True) > 0, rest, last)
+    upto = rest.cumsum(dim=1)
+    token = (upto <= u[:, drafts:] * upto[:, -1:]).sum(dim=1)
+    place = torch.arange(drafts + 1, device=p.device)
+    out = torch.where(place < kept[:, None], torch.nn.functional.pad(tokens, (0, 1)), -1)
+    out = torch.where(place == kept[:, None], token[:, None], out)
+    return out, kept.int()
+
+
+# ---------------------------------------------------------------------------
+# The work of a pass, and its values in 64 bits
+
+
+def _size(dtype):
+    return 4 if dtype == "f32" else 2
+
+
+def work(case):
+    op = case["op"]
+    if op in ("linear", "weight_grad", "quantize"):
+        t, k, size = case["tokens"], case["inputs"], _size(case["dtype"])
+        if op == "quantize":
+            blocks = _blocks(t) * _blocks(k) if case["rows"] == 128 else \
+                k * _blocks(t) if case["transpose"] else t * _blocks(k)
+            return {"bytes": t * k * (size + 1) + 4 * blocks, "flops": 0}
+        n = case["outputs"]
+        if op == "linear":
+            return {"bytes": size * t * (k + n) + n * k + 4 * _blocks(n) * _blocks(k), "flops": 2 * t * n * k}
+        return {"bytes": size * t * (k + n) + 4 * n * k, "flops": 2 * t * n * k}
+    if op == "rotate":
+        size, dim = _size(case["dtype"]), case["head_dim"]
+        q, k = (case["tokens"] * case[name] * dim for name in ("heads", "kv_heads"))
+        values = 2 * (q + k) * size + 8 * case["tokens"]
+        if case["bits"]:
+            # keys and values in, rows of the cache out, and all of it back once
+            rows = 2 * k * case["bits"] // 8 + 2 * 2 * k // dim
+            values = 2 * q * size + 4 * k * size + 2 * rows + 24 * case["tokens"]
+        return {"bytes": values, "flops": 6 * (q + k)}
+    if op == "plan":
+        batch, tokens = case["batch"], case["batch"] * case["new"]
+        return {"bytes": 16 * tokens + 24 * batch + 8 * (tokens // case["page"]), "flops": 0}
+    rows = 1 if case["greedy"] else 2
+    return {"bytes": case["batch"] * rows * case["vocab"] * _size(case["dtype"]), "flops": case["batch"] * case["vocab"]}
+
+
+def exact(case, seed):
+    op = case["op"]
+    if op in ("plan", "verify"):  # whole numbers
+        return None
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    if op == "rotate":
+        return _exact_rotate(case, gen)
+    if op == "quantize":
+        state = _prepare_quantize(case, gen)
+        x = state["x"].t() if state["transpose"] else state["x"]
+        codes, scales = _exact_codes(x, state["rows"], E4M3)
+        return codes, scales
+    state = _prepare_linear(case, gen)
+    if op == "weight_grad":
+        g, x = (_exact_values(state[name].t(), kind)
+                for name, kind in (("grad", E5M2 if case["wide"] else E4M3), ("x", E4M3)))
+        return g @ x.t()
+    return _exact_values(state["x"], E4M3) @ _exact_scaled(state["weights"].double(), state["scales"], BLOCK).t()
+
+
+def _exact_codes(x, rows, kind):
+    """Block by block of columns.  A block's scale is its largest magnitude over
+    the type's largest value, rounded to 32 bits; a code is the value over its
+    scale, rounded to 32 bits and from there to 8, ties to even."""
+    x = x.double()
+    codes, scales = torch.empty_like(x), []
+    most = LARGEST[kind]
+    bits, least = (3, -6) if kind is E4M3 else (2, -14)
+    for c in range(0, x.shape[1], BLOCK):
+        part = x[:, c:c + BLOCK]
+        top = part.abs().amax(dim=1)
+        if rows > 1:
+            top = torch.stack([piece.max() for piece in top.split(rows)])
+        scale = (top / most).float().double()
+        scales.append(scale)
+        wide = scale.repeat_interleave(rows)[: x.shape[0], None]
+        y = torch.where(wide > 0, part / wide, 0.0).float().double().clamp(-most, most)
+        step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0**-60))).clamp(min=least) - bits)
+        codes[:, c:c + BLOCK] = torch.round(y / step) * step
+    return codes, torch.stack(scales, dim=1)
+
+
+def _exact_scaled(codes, scales, rows):
+    out = torch.empty_like(codes)
+    for i in range(scales.shape[1]):
+        wide = scales[:, i].double().repeat_interleave(rows)[: codes.shape[0], None]
+        out[:, i * BLOCK:(i + 1) * BLOCK] = codes[:, i * BLOCK:(i + 1) * BLOCK] * wide
+    return out
+
+
+def _exact_values(x, kind):
+    codes, scales = _exact_codes(x, 1, kind)
+    return _exact_scaled(codes, scales, 1)
+
+
+def _exact_rotate(case, gen):
+    state = _prepare_rotate(case, gen)
+    frequencies, amplitude = _frequencies(case)
+    half, n = case["rotated"] // 2, case["rotated"]
+    angle = state["positions"].double()[:, None, None] * torch.tensor(frequencies, dtype=torch.float64, device="cuda")
+    turn = torch.polar(torch.full_like(angle, amplitude), angle)
+
+    def turned(x, which):
+        x = x.double()
+        if state["norms"] is not None:
+            x = x / torch.sqrt((x * x).sum(dim=-1, keepdim=True) / x.shape[-1] + state["eps"])
+            x = x * state["norms"][which].double()
+        first, second = (slice(0, n, 2), slice(1, n, 2)) if case["interleaved"] else (slice(0, half), slice(half, n))
+        z = torch.complex(x[..., first].contiguous(), x[..., second].contiguous()) * turn
+        out = x.clone()
+        out[..., first], out[..., second] = z.real, z.imag
+        return out
+
+    def stored(x):
+        most = 7 if case["bits"] == 4 else 127
+        x = x.to(state["dtype"]).double()
+        scale = (x.abs().amax(dim=-1, keepdim=True) / most).float().bfloat16().double()
+        code = (x / scale).float().double().round().clamp(-most, most)
+        return torch.where(scale > 0, code, 0.0) * scale
+
+    q, k = turned(state["q"], 0), turned(state["k"], 1)
+    return (q, stored(k), stored(state["v"])) if case["bits"] else (q, k)
