@@ -117,6 +117,8 @@ extern "C" {
 #define SHK_SRC_F16 1
 #define SHK_SRC_BF16 2
 #define SHK_SRC_I8 3
+#define SHK_FP8_E4M3 0
+#define SHK_FP8_E5M2 1
 
 /* Outputs of amd_strix_halo_kernels_quantize. */
 #define SHK_QUANT_CODES 0     /* int8 codes, rows x cols */
@@ -576,6 +578,77 @@ typedef struct shk_moe {
 
 int64_t amd_strix_halo_kernels_moe_workspace(const shk_moe* args);
 int amd_strix_halo_kernels_moe(int device_index, uintptr_t stream, const shk_moe* args);
+
+/* ---- products in 8-bit floating point --------------------------------------
+ * No counterpart in the reference.  Operands are e4m3 (OCP: no infinities,
+ * largest value 448) or e5m2 (largest 57344) codes with one f32 scale for each
+ * block of 128 values of K; the value of a code is code * scale.
+ *
+ * Conversion: x is [rows, cols] of a type SHK_SRC_*, rows contiguous, stride in
+ * elements.  With transpose the operand is x^T, [cols, rows], else x; a block is
+ * block_rows (1 or 128) rows of the operand by 128 of its columns:
+ *   scale = fl32(max|x| / L),  code = fp8(clamp(fl32(x / scale), -L, L))
+ * rounding half to even, L the type's largest value.  A block of zeros has scale
+ * 0 and zero codes; one that holds an infinity or a NaN has that as its scale
+ * and zero codes, so that what it enters becomes NaN.  Row r of the codes starts
+ * at codes + r * code_pitch (bytes); the scale of block (i, j) is
+ * scales[i * scale_row_stride + j * scale_block_stride].  Bytes of the pitch
+ * behind a row are left as they are. */
+typedef struct shk_fp8_quantize {
+  const void* x;
+  int64_t type; /* SHK_SRC_F32, SHK_SRC_F16 or SHK_SRC_BF16 */
+  int64_t rows;
+  int64_t cols;
+  int64_t x_stride;
+  int64_t transpose;
+  int64_t block_rows;
+  int64_t kind; /* SHK_FP8_E4M3 or SHK_FP8_E5M2 */
+  void* codes;
+  int64_t code_pitch;
+  float* scales;
+  int64_t scale_row_stride;
+  int64_t scale_block_stride;
+} shk_fp8_quantize;
+
+int amd_strix_halo_kernels_fp8_quantize(int device_index, uintptr_t stream, const shk_fp8_quantize* args);
+
+/* out[i, j] = sum over the blocks b of K of
+ *   a_scale[i, b] * b_scale[j / b_rows, b] * sum_{k in b} a[i, k] * b[j, k]
+ * with a [m, k] and b [n, k] in rows of a_pitch and b_pitch bytes, scales at
+ * row * row_stride + block * block_stride (elements, not negative), b_rows 1 or
+ * 128.  The inner sum is the matrix unit's (f32), the outer one f32, rounded once
+ * to out_type (SHK_SRC_*; rows of out contiguous, out_stride in elements).
+ * k = 0 gives zeros.  k up to 8388607; each scale tensor spans less than 2^31
+ * bytes.  Operands are best on 16 bytes with pitches of whole 16s: others are
+ * copied into the workspace first.  workspace: at least
+ * amd_strix_halo_kernels_fp8_mm_workspace bytes, on 16 bytes, not read before it
+ * is written. */
+typedef struct shk_fp8_mm {
+  const void* a;
+  int64_t a_pitch;
+  int64_t a_kind; /* SHK_FP8_* */
+  const void* b;
+  int64_t b_pitch;
+  int64_t b_kind;
+  const float* a_scale;
+  int64_t a_scale_row_stride;
+  int64_t a_scale_block_stride;
+  const float* b_scale;
+  int64_t b_scale_row_stride;
+  int64_t b_scale_block_stride;
+  int64_t b_rows;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  void* out;
+  int64_t out_stride;
+  int64_t out_type;
+  void* workspace;
+  int64_t workspace_bytes;
+} shk_fp8_mm;
+
+int64_t amd_strix_halo_kernels_fp8_mm_workspace(const shk_fp8_mm* args);
+int amd_strix_halo_kernels_fp8_mm(int device_index, uintptr_t stream, const shk_fp8_mm* args);
 
 #ifdef __cplusplus
 }

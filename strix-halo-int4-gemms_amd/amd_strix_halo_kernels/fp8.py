@@ -1,0 +1,186 @@
+"""Products in 8-bit floating point with a scale for each block of 128 values.
+
+No counterpart in the reference, whose GEMMs are int4 and int8.  An operand is
+e4m3 or e5m2 codes with one f32 scale for each block of 128 values along K, of
+one row (activations, gradients) or of 128 rows (weights):
+
+    scale = max|x| / L            L = 448 (e4m3) or 57344 (e5m2)
+    code  = fp8(clamp(x / scale, -L, L))        value = code * scale
+
+``quantize_fp8`` makes codes and scales of a tensor or of its transpose, and
+``mm_fp8`` multiplies two of them.  The three products of a linear layer
+``y = x w^T`` are one kernel, fed along its K:
+
+    y  = mm_fp8(*q(x), *q(w, block_rows=128))
+    dx = mm_fp8(*q(dy), *q(w, block_rows=128, transpose=True))
+    dw = mm_fp8(*q(dy, transpose=True), *q(x, transpose=True))
+
+(q for ``quantize_fp8``, its codes and scales passed as a and a_scale, b and
+b_scale).  Both run on the current stream of the tensors' device, or on
+``stream`` (which is then the current one for the call, its allocations
+included), and read nothing back to the host.  There is no CPU path, and asking
+a result for a gradient raises: the products above are the gradients.
+"""
+
+from __future__ import annotations
+
+import struct
+from typing import Any
+
+from . import kernel_table as kt
+from .native import (
+    _check,
+    _current_stream,
+    _no_gradient,
+    _on_stream,
+    _require_device,
+    _torch,
+    _verified_library,
+)
+
+FP8_BLOCK = 128
+
+# the structs of include/strix_halo_gfx950.h: every field is 8 bytes
+_QUANTIZE = struct.Struct("=13q")
+_MM = struct.Struct("=21q")
+
+
+def _kind(torch: Any, name: str, dtype: Any) -> int:
+    if dtype == torch.float8_e4m3fn:
+        return kt.FP8_E4M3
+    if dtype == torch.float8_e5m2:
+        return kt.FP8_E5M2
+    raise ValueError(f"{name} must have dtype torch.float8_e4m3fn or torch.float8_e5m2; got {dtype}")
+
+
+def _value_type(torch: Any, name: str, dtype: Any) -> int:
+    if dtype == torch.bfloat16:
+        return kt.SRC_BF16
+    if dtype == torch.float16:
+        return kt.SRC_F16
+    if dtype == torch.float32:
+        return kt.SRC_F32
+    raise ValueError(f"{name} must have dtype torch.bfloat16, torch.float16 or torch.float32; got {dtype}")
+
+
+def quantize_fp8(x: Any, *, block_rows: int = 1, transpose: bool = False, dtype: Any = None,
+                 stream: Any | None = None) -> tuple[Any, Any]:
+    """Codes and scales of ``x`` [rows, cols] (bf16, f16 or f32; contiguous
+    along either axis), or of its transpose.
+
+    Returns ``(codes, scales)`` of the operand, x or x^T, [R, C]: codes [R, C]
+    in ``dtype`` (``torch.float8_e4m3fn``, the default, or
+    ``torch.float8_e5m2``), each row on 16 bytes, and f32 scales
+    [ceil(R / block_rows), ceil(C / 128)] (stored with the blocks of one row
+    ``ceil(R / block_rows)`` apart), ``block_rows`` 1 or 128.  A block of zeros
+    has scale 0; one that holds an infinity or a NaN has that as its scale and
+    zero codes, so that what it is multiplied with becomes NaN.
+    """
+    torch = _torch()
+    if x.get_device() < 0:
+        _require_device(torch, {"x": x})
+    if stream is not None:
+        with _on_stream(torch, x, stream):
+            return quantize_fp8(x, block_rows=block_rows, transpose=transpose, dtype=dtype)
+    dtype = torch.float8_e4m3fn if dtype is None else dtype
+    kind, source = _kind(torch, "the result", dtype), _value_type(torch, "x", x.dtype)
+    if block_rows not in (1, FP8_BLOCK):
+        raise ValueError(f"block_rows must be 1 or {FP8_BLOCK}; got {block_rows}")
+    if x.ndim != 2:
+        raise ValueError(f"x must have shape (rows, cols); got {tuple(x.shape)}")
+    rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape  # of the operand
+    turn, given = bool(transpose), x
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        if x.stride(0) != 1 and x.shape[0] > 1:
+            raise ValueError("x must be contiguous along rows or columns")
+        x, turn = x.t(), not turn
+    pitch = -(-cols // 16) * 16
+    codes = torch.empty((rows, pitch), dtype=dtype, device=x.device)
+    scales = torch.empty((-(-cols // FP8_BLOCK), -(-rows // block_rows)), dtype=torch.float32, device=x.device)
+    if rows and cols:
+        stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+        lib = _verified_library()
+        index = x.get_device()
+        _check(lib, lib.amd_strix_halo_kernels_fp8_quantize(
+            index, _current_stream(torch, index),
+            _QUANTIZE.pack(x.data_ptr(), source, x.shape[0], x.shape[1], stride, turn, block_rows, kind,
+                           codes.data_ptr(), pitch, scales.data_ptr(), 1, scales.shape[1])))
+    codes, scales = codes[:, :cols], scales.t()
+    if given.requires_grad:
+        scales = _no_gradient(torch, "quantize_fp8", scales, given)
+    return codes, scales
+
+
+def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None, out: Any | None = None,
+           stream: Any | None = None) -> Any:
+    """``out[m, n] = sum_k (a * a_scale)[m, k] (b * b_scale)[n, k]`` of fp8
+    codes, K along the rows of both.
+
+    ``a`` is [M, K] and ``b`` [N, K] (``torch.float8_e4m3fn`` or
+    ``torch.float8_e5m2`` each; rows contiguous, any pitch), ``a_scale`` [M,
+    ceil(K / 128)] and ``b_scale`` [ceil(N / 128), ceil(K / 128)] (a weight's
+    blocks) or [N, ceil(K / 128)], f32 of any strides.  Returns [M, N] in
+    ``out_dtype`` (bf16, the default, f16 or f32).  Sums are f32: inside a
+    block of K by the matrix unit, over the blocks in order of K, or, where few
+    tiles share a long K, in order of its parts; rounded once at the end.
+    Operands whose rows do not all start on 16 bytes are copied first; the codes
+    of ``quantize_fp8`` do.
+    """
+    torch = _torch()
+    index = a.get_device()
+    for t in (b, a_scale, b_scale, a if out is None else out):
+        if index < 0 or t.get_device() != index:
+            _require_device(torch, {"a": a, "b": b, "a_scale": a_scale, "b_scale": b_scale, "out": out})
+    if stream is not None:
+        with _on_stream(torch, a, stream):
+            return mm_fp8(a, b, a_scale=a_scale, b_scale=b_scale, out_dtype=out_dtype, out=out)
+    a_kind, b_kind = _kind(torch, "a", a.dtype), _kind(torch, "b", b.dtype)
+    if a.ndim != 2 or b.ndim != 2 or a.shape[1] != b.shape[1]:
+        raise ValueError(f"a and b must have shapes (M, K) and (N, K); got {tuple(a.shape)} and {tuple(b.shape)}")
+    m, k = a.shape
+    n = b.shape[0]
+    if k > 1 and (a.stride(1) != 1 or b.stride(1) != 1):
+        raise ValueError("rows of a and b must be contiguous")
+    blocks = -(-k // FP8_BLOCK)
+    for name, t in (("a_scale", a_scale), ("b_scale", b_scale)):
+        if t.dtype != torch.float32:
+            raise ValueError(f"{name} must have dtype torch.float32; got {t.dtype}")
+    if a_scale.shape != (m, blocks):
+        raise ValueError(f"a_scale must have shape {(m, blocks)} == (M, ceil(K/128)); got {tuple(a_scale.shape)}")
+    if b_scale.shape == (-(-n // FP8_BLOCK), blocks):
+        b_rows = FP8_BLOCK
+    elif b_scale.shape == (n, blocks):
+        b_rows = 1
+    else:
+        raise ValueError(f"b_scale must have shape {(-(-n // FP8_BLOCK), blocks)} == (ceil(N/128), ceil(K/128)) or "
+                         f"{(n, blocks)} == (N, ceil(K/128)); got {tuple(b_scale.shape)}")
+    if out is None:
+        out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        out_type = _value_type(torch, "the result", out_dtype)
+        out = a.new_empty((m, n), dtype=out_dtype)
+    else:
+        out_type = _value_type(torch, "out", out.dtype)
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out must have dtype {out_dtype}; got {out.dtype}")
+        if out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+            raise ValueError(f"out must have shape {(m, n)} and contiguous rows; got {tuple(out.shape)}")
+    if m and n:
+        a_pitch, b_pitch = a.stride(0) if m > 1 else k, b.stride(0) if n > 1 else k
+
+        def args(work: Any, nbytes: int) -> bytes:
+            return _MM.pack(a.data_ptr(), a_pitch, a_kind, b.data_ptr(), b_pitch, b_kind, a_scale.data_ptr(),
+                            *a_scale.stride(), b_scale.data_ptr(), *b_scale.stride(), b_rows, m, n, k, out.data_ptr(),
+                            out.stride(0) if m > 1 else n, out_type, work.data_ptr() if nbytes else 0, nbytes)
+
+        lib = _verified_library()
+        packed = args(None, 0)
+        nbytes = lib.amd_strix_halo_kernels_fp8_mm_workspace(packed)
+        if nbytes < 0:
+            _check(lib, 1)
+        if nbytes:
+            work = a.new_empty(nbytes, dtype=torch.uint8)
+            packed = args(work, nbytes)
+        _check(lib, lib.amd_strix_halo_kernels_fp8_mm(index, _current_stream(torch, index), packed))
+    if a_scale.requires_grad or b_scale.requires_grad:
+        return _no_gradient(torch, "mm_fp8", out, a_scale, b_scale)
+    return out

@@ -76,6 +76,9 @@ SRC_F32 = 0
 SRC_F16 = 1
 SRC_BF16 = 2
 SRC_I8 = 3
+# 8-bit floating-point codes
+FP8_E4M3 = 0
+FP8_E5M2 = 1
 QUANT_CODES = 0
 QUANT_PACK_COLS = 1
 QUANT_PACK_ROWS = 2

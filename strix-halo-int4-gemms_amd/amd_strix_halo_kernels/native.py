@@ -136,6 +136,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.amd_strix_halo_kernels_moe_workspace.restype = I64
     lib.amd_strix_halo_kernels_moe.argtypes = [I, U, P]
     lib.amd_strix_halo_kernels_moe.restype = I
+    lib.amd_strix_halo_kernels_fp8_quantize.argtypes = [I, U, P]
+    lib.amd_strix_halo_kernels_fp8_quantize.restype = I
+    lib.amd_strix_halo_kernels_fp8_mm_workspace.argtypes = [P]
+    lib.amd_strix_halo_kernels_fp8_mm_workspace.restype = I64
+    lib.amd_strix_halo_kernels_fp8_mm.argtypes = [I, U, P]
+    lib.amd_strix_halo_kernels_fp8_mm.restype = I
 
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:

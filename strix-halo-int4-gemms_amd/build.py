@@ -86,6 +86,9 @@ def decode_units() -> list[tuple[str, Path, list[str]]]:
         ("moe_nn", CSRC / "k_moe.hip", ["-DSHK_LAYOUT=0"]),
         ("moe_nt", CSRC / "k_moe.hip", ["-DSHK_LAYOUT=1"]),
         ("capi_decode", CSRC / "capi_decode.hip", []),
+        ("fp8", CSRC / "k_fp8.hip", []),
+        ("fp8quant", CSRC / "k_fp8quant.hip", []),
+        ("capi_fp8", CSRC / "capi_fp8.hip", []),
     ]
 
 

@@ -1,0 +1,378 @@
+// Products of 8-bit floating-point operands with a scale for each block of 128
+// values of K:
+//   out[i, j] = sum_b sa[i, b] sb[j, b] (sum_{k in b} a[i, k] b[j, k]).
+//
+// The 8-bit matrix unit (v_mfma_f32_16x16x128_f8f6f4, one block of K) does not
+// add its exact products as f32 sums do: of eight neighbours along K it keeps
+// each to 2^-13 of the power of two of the largest, cut towards zero (measured
+// with two products; neighbours of other eights, and f16's unit, keep 2^-23).
+// Over real rows that is about 2e-5 of a result, 5e-5 where some channels are
+// large: below the rounding of a bf16 or f16 result, above that of an f32 one.
+// f32 results are therefore taken through the f16 unit, where each code is exact.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "shk_common.h"
+#include "shk_dma.h"
+#include "shk_fp8.h"
+
+namespace shk {
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+struct Product {
+  const uint8_t* a;
+  const uint8_t* b;
+  long a_pitch, b_pitch;
+  const float* sa;
+  const float* sb;
+  long sa_row, sa_block, sb_row, sb_block;  // elements
+  void* out;
+  long out_stride;
+  float* partial;   // [splits][m][n] where splits > 1
+  int m, n, k;
+  int tiles_m, tiles_n;
+  int splits, per_split;  // blocks of K
+  int out_type, b_shift;  // rows of b >> b_shift: its row of scales
+  int aligned;            // rows of out start on 16 bytes
+};
+
+template <int BM_, int BN_, int WM_, int WN_, int P_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, P = P_;
+  static constexpr int NW = WM * WN, THREADS = 64 * NW;
+  static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // MFMA tiles of a wave
+  static constexpr int SA = (BM + 63) / 64 * 64;              // scales of a stage, whole DMAs
+  static constexpr int DATA = (BM + BN) * 128;
+  static constexpr int STAGE = DATA + (SA + BN) * 4;
+  static constexpr int LOADS = (BM + BN) / 8;                 // 1 KiB DMAs of a stage
+  static constexpr int PER_WAVE = (LOADS + NW - 1) / NW;
+  static constexpr int SCALES = (SA + BN) / 64;               // 256-byte DMAs of a stage
+  static constexpr int SCALES_PER_WAVE = (SCALES + NW - 1) / NW;
+  static constexpr int ISSUED = PER_WAVE + SCALES_PER_WAVE;   // by a wave and stage
+  static_assert(BM % 16 == 0 && BN % 64 == 0 && P * STAGE <= 160 * 1024, "");
+};
+
+template <int KIND_A, int KIND_B>
+__device__ __forceinline__ v4f mfma128(const v8i& b, const v8i& a) {
+  // rows of the result are b's, columns a's
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, v4f{0.f, 0.f, 0.f, 0.f}, KIND_B, KIND_A, 0, 0, 0, 0);
+}
+
+// Eight codes of one operand as f16, which holds every one of them exactly.
+template <int KIND>
+__device__ __forceinline__ v8h widen(int lo, int hi) {
+  v2h h[4];
+  if constexpr (KIND == SHK_FP8_E4M3) {
+    h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+    h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+    h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+    h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  } else {  // the upper bytes of f16
+    h[0] = __builtin_bit_cast(v2h, perm_b32(0u, lo, 0x010C000Cu));
+    h[1] = __builtin_bit_cast(v2h, perm_b32(0u, lo, 0x030C020Cu));
+    h[2] = __builtin_bit_cast(v2h, perm_b32(0u, hi, 0x010C000Cu));
+    h[3] = __builtin_bit_cast(v2h, perm_b32(0u, hi, 0x030C020Cu));
+  }
+  return v8h{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
+
+template <int KIND>
+struct Wide {
+  v8h part[4];
+  __device__ __forceinline__ explicit Wide(const v8i& f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[i] = widen<KIND>(f[2 * i], f[2 * i + 1]);
+  }
+};
+
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ void store_value(const Product& p, long at, float v) {
+  if (p.out_type == SHK_SRC_F32) static_cast<float*>(p.out)[at] = v;
+  else if (p.out_type == SHK_SRC_BF16) static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16_rne(v);
+  else static_cast<_Float16*>(p.out)[at] = (_Float16)v;
+}
+
+template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
+__global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Product p) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x;
+  const int m0 = tile % p.tiles_m * T::BM, n0 = tile / p.tiles_m * T::BN;
+  const int first = blockIdx.y * p.per_split;
+  const int blocks = (p.k + 127) >> 7;
+  const int count = min(p.per_split, blocks - first);
+
+  // where this wave's pieces of a stage come from
+  const int rows_a = min(T::BM, p.m - m0), rows_b = min(T::BN, p.n - n0);
+  const long row_bytes = (p.k + 15) & ~15;
+  const v4i ra = buffer_words(p.a + (long)m0 * p.a_pitch, (unsigned long long)((rows_a - 1) * p.a_pitch + row_bytes));
+  const v4i rb = buffer_words(p.b + (long)n0 * p.b_pitch, (unsigned long long)((rows_b - 1) * p.b_pitch + row_bytes));
+  const int s0 = n0 >> p.b_shift, s_rows = ((n0 + rows_b - 1) >> p.b_shift) - s0 + 1;
+  const v4i rsa = buffer_words(p.sa + (long)m0 * p.sa_row,
+                               (unsigned long long)(((rows_a - 1) * p.sa_row + (blocks - 1) * p.sa_block + 1) * 4));
+  const v4i rsb = buffer_words(p.sb + (long)s0 * p.sb_row,
+                               (unsigned long long)(((s_rows - 1) * p.sb_row + (blocks - 1) * p.sb_block + 1) * 4));
+  uint32_t voff[T::PER_WAVE], to[T::PER_WAVE], soff_s[T::SCALES_PER_WAVE], to_s[T::SCALES_PER_WAVE];
+  bool of_a[T::PER_WAVE], s_of_a[T::SCALES_PER_WAVE];
+#pragma unroll
+  for (int c = 0; c < T::PER_WAVE; ++c) {
+    const int piece = min(wave * T::PER_WAVE + c, T::LOADS - 1);
+    of_a[c] = piece < T::BM / 8;
+    const int row = (of_a[c] ? piece : piece - T::BM / 8) * 8 + lane / 8;
+    const int unit = (lane & 7) ^ (row & 7);
+    voff[c] = of_a[c] ? (uint32_t)(min(row, rows_a - 1) * p.a_pitch) + 16 * unit
+                      : (uint32_t)(min(row, rows_b - 1) * p.b_pitch) + 16 * unit;
+    to[c] = piece * 1024;
+  }
+#pragma unroll
+  for (int c = 0; c < T::SCALES_PER_WAVE; ++c) {
+    const int piece = min(wave * T::SCALES_PER_WAVE + c, T::SCALES - 1);
+    s_of_a[c] = piece < T::SA / 64;
+    const int row = (s_of_a[c] ? piece : piece - T::SA / 64) * 64 + lane;
+    soff_s[c] = s_of_a[c] ? (uint32_t)(min(row, rows_a - 1) * p.sa_row * 4)
+                          : (uint32_t)((((n0 + min(row, rows_b - 1)) >> p.b_shift) - s0) * p.sb_row * 4);
+    to_s[c] = T::DATA + piece * 256;
+  }
+  const uint32_t base = lds_address(lds);
+  auto issue = [&](int kb, int slot) {
+    const uint32_t at = base + slot * T::STAGE;
+#pragma unroll
+    for (int c = 0; c < T::PER_WAVE; ++c)
+      lds_dma16(of_a[c] ? ra : rb, voff[c], (uint32_t)kb * 128u, at + to[c]);
+#pragma unroll
+    for (int c = 0; c < T::SCALES_PER_WAVE; ++c)
+      lds_dma4(s_of_a[c] ? rsa : rsb, soff_s[c], (uint32_t)kb * (uint32_t)((s_of_a[c] ? p.sa_block : p.sb_block) * 4),
+               at + to_s[c]);
+  };
+
+  v4f acc[T::MT][T::NT];
+#pragma unroll
+  for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  const int wm = wave % T::WM, wn = wave / T::WM;
+  const int row_in = lane & 15, group = lane >> 4;
+  // fragment of this lane: units `group` and `group + 4` of its row
+  const uint32_t frag = row_in * 128 + 16 * (group ^ (row_in & 7));
+  const uint32_t a_at = wm * T::MT * 2048 + frag, b_at = T::BM * 128 + wn * T::NT * 2048 + frag;
+  const uint32_t sa_at = T::DATA + (wm * T::MT * 16 + row_in) * 4;
+  const uint32_t sb_at = T::DATA + (T::SA + wn * T::NT * 16 + (BROW ? group * 4 : 0)) * 4;
+
+#pragma unroll
+  for (int s = 0; s < T::P - 1; ++s)
+    if (s < count) issue(first + s, s);
+  int slot = 0;
+  for (int i = 0; i < count; ++i) {
+    if (i + T::P - 2 < count) wait_vmcnt<(T::P - 2) * T::ISSUED>();
+    else wait_vmcnt<0>();
+    stage_barrier();
+    if (i + T::P - 1 < count) issue(first + i + T::P - 1, slot == 0 ? T::P - 1 : slot - 1);
+    uint8_t* st = lds + slot * T::STAGE;
+    const int left = p.k - (first + i) * 128;
+    if (left < 128) {  // K ends in this block: zeros behind it
+      for (int u = threadIdx.x; u < (T::BM + T::BN) * 8; u += T::THREADS) {
+        const int row = u >> 3, unit = (u & 7) ^ (row & 7), keep = left - unit * 16;
+        if (keep >= 16) continue;
+        uint32_t* w = reinterpret_cast<uint32_t*>(st + u * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int bytes = keep - 4 * e;
+          w[e] = bytes <= 0 ? 0u : bytes >= 4 ? w[e] : w[e] & ((1u << (8 * bytes)) - 1u);
+        }
+      }
+      stage_barrier();
+    }
+    auto fragment = [&](uint32_t at) {
+      const v4i lo = *reinterpret_cast<const v4i*>(st + at);
+      const v4i hi = *reinterpret_cast<const v4i*>(st + (at ^ 64u));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    v8i fb[T::NT];
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j) fb[j] = fragment(b_at + j * 2048);
+    float sb = 0.f;
+    v4f sbv[T::NT];
+    if constexpr (BROW) {
+#pragma unroll
+      for (int j = 0; j < T::NT; ++j) sbv[j] = *reinterpret_cast<const v4f*>(st + sb_at + j * 64);
+    } else {
+      sb = *reinterpret_cast<const float*>(st + sb_at);
+    }
+#pragma unroll
+    for (int x = 0; x < T::MT; ++x) {
+      const v8i fa = fragment(a_at + x * 2048);
+      float s = *reinterpret_cast<const float*>(st + sa_at + x * 64);
+      if constexpr (!BROW) s *= sb;
+#pragma unroll
+      for (int j = 0; j < T::NT; ++j) {
+        v4f t;
+        if constexpr (WIDE) {
+          const Wide<KIND_A> wa(fa);
+          const Wide<KIND_B> wb(fb[j]);
+          t = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb.part[i], wa.part[i], t, 0, 0, 0);
+        } else {
+          t = mfma128<KIND_A, KIND_B>(fb[j], fa);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[x][j][r] = __builtin_fmaf(t[r], BROW ? s * sbv[j][r] : s, acc[x][j][r]);
+      }
+    }
+    slot = slot == T::P - 1 ? 0 : slot + 1;
+  }
+
+#pragma unroll
+  for (int x = 0; x < T::MT; ++x) {
+    const int m = m0 + (wm * T::MT + x) * 16 + row_in;
+    if (m >= p.m) continue;
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j) {
+      const int n = n0 + (wn * T::NT + j) * 16 + group * 4;
+      if (p.splits > 1) {
+        float* at = p.partial + ((long)blockIdx.y * p.m + m) * p.n + n;
+        for (int r = 0; r < 4; ++r)
+          if (n + r < p.n) at[r] = acc[x][j][r];
+      } else {
+        for (int r = 0; r < 4; ++r)
+          if (n + r < p.n) store_value(p, (long)m * p.out_stride + n + r, acc[x][j][r]);
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void fp8_join_kernel(const Product p) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, all = (long)p.m * p.n;
+  if (i >= all) return;
+  float v = 0.f;
+  for (int s = 0; s < p.splits; ++s) v += p.partial[s * all + i];
+  store_value(p, i / p.n * p.out_stride + i % p.n, v);
+}
+
+// Rows to a pitch of whole 16 bytes.
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* src, long pitch, int k, uint8_t* dst, long to) {
+  const long row = blockIdx.y + (long)blockIdx.z * 65535;
+  for (int c = blockIdx.x * 256 + threadIdx.x; c < k; c += gridDim.x * 256) dst[row * to + c] = src[row * pitch + c];
+}
+
+struct Plan {
+  int bm, bn, splits, per_split;
+  bool copy_a, copy_b;
+  long pitch;              // of the copies
+  int64_t at_b, at_partial, bytes;
+};
+
+bool loose(const void* x, int64_t pitch, int64_t rows) {
+  return reinterpret_cast<uintptr_t>(x) % 16 != 0 || (rows > 1 && pitch % 16 != 0);
+}
+
+Plan plan_of(const shk_fp8_mm& a) {
+  Plan r{};
+  const int blocks = (int)((a.k + 127) / 128);
+  if (a.m <= 16) r.bm = 16, r.bn = 64;
+  else if (a.m <= 32) r.bm = 32, r.bn = 64;
+  else if (a.m <= 64) r.bm = 64, r.bn = 64;
+  else if (((a.m + 255) / 256) * ((a.n + 255) / 256) >= 192) r.bm = 256, r.bn = 256;
+  else r.bm = 128, r.bn = 128;
+  const int64_t tiles = ((a.m + r.bm - 1) / r.bm) * ((a.n + r.bn - 1) / r.bn);
+  const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, tiles));
+  r.splits = (int)std::min<int64_t>(want, std::max(1, blocks / 4));
+  r.per_split = std::max(1, (blocks + r.splits - 1) / r.splits);
+  r.splits = std::max(1, (blocks + r.per_split - 1) / r.per_split);
+  r.copy_a = loose(a.a, a.a_pitch, a.m), r.copy_b = loose(a.b, a.b_pitch, a.n);
+  r.pitch = (a.k + 15) & ~15L;
+  r.at_b = r.copy_a ? a.m * r.pitch : 0;
+  r.at_partial = r.at_b + (r.copy_b ? a.n * r.pitch : 0);
+  r.bytes = r.at_partial + (r.splits > 1 ? (int64_t)r.splits * a.m * a.n * 4 : 0);
+  return r;
+}
+
+template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
+hipError_t launch(Product& p, hipStream_t s) {
+  p.tiles_m = (p.m + T::BM - 1) / T::BM, p.tiles_n = (p.n + T::BN - 1) / T::BN;
+  constexpr int bytes = T::P * T::STAGE;
+  static const hipError_t set = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(fp8_product_kernel<T, KIND_A, KIND_B, BROW, WIDE>),
+      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (set != hipSuccess) return set;
+  hipLaunchKernelGGL((fp8_product_kernel<T, KIND_A, KIND_B, BROW, WIDE>), dim3(p.tiles_m * p.tiles_n, p.splits),
+                     dim3(T::THREADS), bytes, s, p);
+  return hipGetLastError();
+}
+
+template <class T, int KIND_A, int KIND_B>
+hipError_t launch_rows(Product& p, hipStream_t s) {
+  const bool rows = p.b_shift == 0;
+  if (p.out_type == SHK_SRC_F32)
+    return rows ? launch<T, KIND_A, KIND_B, true, true>(p, s) : launch<T, KIND_A, KIND_B, false, true>(p, s);
+  return rows ? launch<T, KIND_A, KIND_B, true, false>(p, s) : launch<T, KIND_A, KIND_B, false, false>(p, s);
+}
+
+template <class T>
+hipError_t launch_kinds(Product& p, bool e5_a, bool e5_b, hipStream_t s) {
+  if (e5_a) return e5_b ? launch_rows<T, 1, 1>(p, s) : launch_rows<T, 1, 0>(p, s);
+  return e5_b ? launch_rows<T, 0, 1>(p, s) : launch_rows<T, 0, 0>(p, s);
+}
+
+hipError_t copy_rows(const void* src, long pitch, long rows, int k, uint8_t* dst, long to, hipStream_t s) {
+  for (long done = 0; done < rows; done += 65535) {
+    const long part = std::min(65535L, rows - done);
+    hipLaunchKernelGGL(fp8_rows_kernel, dim3((unsigned)std::min(64, (k + 255) / 256), (unsigned)part), dim3(256), 0, s,
+                       static_cast<const uint8_t*>(src) + done * pitch, pitch, k, dst + done * to, to);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+int64_t fp8_mm_workspace(const shk_fp8_mm& a) { return a.m * a.n == 0 ? 0 : plan_of(a).bytes; }
+
+hipError_t launch_fp8_mm(const shk_fp8_mm& a, hipStream_t s) {
+  if (a.m * a.n == 0) return hipSuccess;
+  const Plan r = plan_of(a);
+  uint8_t* work = static_cast<uint8_t*>(a.workspace);
+  Product p{};
+  p.a = static_cast<const uint8_t*>(a.a), p.b = static_cast<const uint8_t*>(a.b);
+  p.a_pitch = a.a_pitch, p.b_pitch = a.b_pitch;
+  if (r.copy_a) {
+    if (hipError_t e = copy_rows(a.a, a.a_pitch, a.m, (int)a.k, work, r.pitch, s)) return e;
+    p.a = work, p.a_pitch = r.pitch;
+  }
+  if (r.copy_b) {
+    if (hipError_t e = copy_rows(a.b, a.b_pitch, a.n, (int)a.k, work + r.at_b, r.pitch, s)) return e;
+    p.b = work + r.at_b, p.b_pitch = r.pitch;
+  }
+  p.sa = a.a_scale, p.sb = a.b_scale;
+  p.sa_row = a.a_scale_row_stride, p.sa_block = a.a_scale_block_stride;
+  p.sb_row = a.b_scale_row_stride, p.sb_block = a.b_scale_block_stride;
+  p.out = a.out, p.out_stride = a.out_stride, p.out_type = (int)a.out_type;
+  p.partial = reinterpret_cast<float*>(work + r.at_partial);
+  p.m = (int)a.m, p.n = (int)a.n, p.k = (int)a.k;
+  p.splits = r.splits, p.per_split = r.per_split;
+  p.b_shift = a.b_rows == 128 ? 7 : 0;
+  const bool e5_a = a.a_kind == SHK_FP8_E5M2, e5_b = a.b_kind == SHK_FP8_E5M2;
+  hipError_t e;
+  if (r.bm == 16) e = launch_kinds<Tile<16, 64, 1, 4, 6>>(p, e5_a, e5_b, s);
+  else if (r.bm == 32) e = launch_kinds<Tile<32, 64, 1, 4, 6>>(p, e5_a, e5_b, s);
+  else if (r.bm == 64) e = launch_kinds<Tile<64, 64, 2, 2, 4>>(p, e5_a, e5_b, s);
+  else if (r.bm == 128) e = launch_kinds<Tile<128, 128, 2, 2, 2>>(p, e5_a, e5_b, s);
+  else e = launch_kinds<Tile<256, 256, 2, 4, 2>>(p, e5_a, e5_b, s);
+  if (e != hipSuccess || p.splits == 1) return e;
+  hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)(((long)p.m * p.n + 255) / 256)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace shk

@@ -1,0 +1,272 @@
+// Values to 8-bit floating point with a scale for each block of 128:
+//   s = fl32(max|x| / L),  c = fp8(clamp(fl32(x / s), -L, L)),
+// L = 448 (e4m3) or 57344 (e5m2).  One pass over memory: a block's values stay
+// in registers between the maximum and the codes.
+//
+// fp8_rows: blocks of one row by 128 columns; 16 lanes hold one, 8 values each.
+// fp8_tile: a workgroup holds 128 rows by 128 columns, a thread 8 rows by 8
+// columns; for blocks of 128 x 128, and for the operand x^T, whose blocks of one
+// row are x's columns.  Transposed codes pass through LDS in units of 8 bytes
+// (8 rows of one column), unit u of column c at c * 128 + 8 * (u ^ (c / 8)), so
+// that neither side meets a bank twice in a step.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "shk_common.h"
+#include "shk_fp8.h"
+
+namespace shk {
+namespace {
+
+struct Convert {
+  const uint8_t* x;
+  long rows, cols, stride;  // elements
+  uint8_t* codes;
+  long pitch;
+  float* scales;
+  long s_row, s_block;
+};
+
+template <int TYPE>
+constexpr int kSize = TYPE == SHK_SRC_F32 ? 4 : 2;
+
+template <int TYPE>
+__device__ __forceinline__ float value_of(const uint8_t* x, long i) {
+  if constexpr (TYPE == SHK_SRC_F32) return reinterpret_cast<const float*>(x)[i];
+  const uint16_t h = reinterpret_cast<const uint16_t*>(x)[i];
+  return TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+}
+
+// x[at .. at + 8); `count` of them lie inside.  VEC: on 16 bytes if all do.
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load8(const uint8_t* x, long at, long count, float (&v)[8]) {
+  if (VEC && count >= 8) {
+    const uint4* src = reinterpret_cast<const uint4*>(x + at * kSize<TYPE>);
+    uint32_t u[kSize<TYPE> * 2];
+#pragma unroll
+    for (int i = 0; i < kSize<TYPE> / 2; ++i) {
+      const uint4 w = src[i];
+      u[4 * i] = w.x, u[4 * i + 1] = w.y, u[4 * i + 2] = w.z, u[4 * i + 3] = w.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (TYPE == SHK_SRC_F32) {
+        v[e] = __uint_as_float(u[e]);
+      } else {
+        const uint16_t h = (uint16_t)(u[e / 2] >> (16 * (e % 2)));
+        v[e] = TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < count ? value_of<TYPE>(x, at + e) : 0.f;
+}
+
+// Magnitudes compare as integers: a NaN is larger than an infinity, and stays.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+template <int KIND>
+constexpr float kLargest = KIND == SHK_FP8_E4M3 ? 448.f : 57344.f;
+
+template <int KIND>
+__device__ __forceinline__ float scale_of(uint32_t most) { return __uint_as_float(most) / kLargest<KIND>; }
+
+// fl32(x / s) by a reciprocal, its product and one exact remainder (Markstein's
+// theorem) where no step leaves the normal range, else by division; what
+// underflows on the way rounds to a code of 0 either way.
+template <int KIND>
+__device__ __forceinline__ void codes8(const float (&v)[8], float s, float inv, bool plain, uint32_t (&w)[2]) {
+  const bool usable = s > 0.f && s < __builtin_inff();
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float r;
+    if (plain) {
+      const float q0 = v[e] * inv;
+      r = __builtin_fmaf(__builtin_fmaf(-q0, s, v[e]), inv, q0);
+    } else {
+      r = v[e] / s;
+    }
+    q[e] = usable ? __builtin_fminf(__builtin_fmaxf(r, -kLargest<KIND>), kLargest<KIND>) : 0.f;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int u = 0;
+    if constexpr (KIND == SHK_FP8_E4M3) {
+      u = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h], q[4 * h + 1], u, false);
+      u = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h + 2], q[4 * h + 3], u, true);
+    } else {
+      u = __builtin_amdgcn_cvt_pk_bf8_f32(q[4 * h], q[4 * h + 1], u, false);
+      u = __builtin_amdgcn_cvt_pk_bf8_f32(q[4 * h + 2], q[4 * h + 3], u, true);
+    }
+    w[h] = (uint32_t)u;
+  }
+}
+
+__device__ __forceinline__ bool normal_scale(float s) { return s > 0x1p-60f && s < 0x1p60f; }
+
+// `count` of 8 bytes; VEC: on 8 bytes.
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t* to, const uint32_t (&w)[2], long count) {
+  if (VEC && count >= 8) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < count) to[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+}
+
+template <int TYPE, int KIND, bool VEC>
+__global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
+  const long blocks = (p.cols + 127) / 128;
+  const long unit = (long)blockIdx.x * 16 + threadIdx.x / 16;
+  const int part = threadIdx.x % 16;
+  if (unit >= p.rows * blocks) return;  // all 16 lanes of a block
+  const long row = unit / blocks, block = unit - row * blocks;
+  const long at = block * 128 + part * 8;
+  float v[8];
+  load8<TYPE, VEC>(p.x, row * p.stride + at, p.cols - at, v);
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e]));
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+  const float s = scale_of<KIND>(most);
+  uint32_t w[2];
+  codes8<KIND>(v, s, 1.f / s, normal_scale(s), w);
+  if (at < p.cols) store8<VEC>(p.codes + row * p.pitch + at, w, p.cols - at);
+  if (part == 0) p.scales[row * p.s_row + block * p.s_block] = s;
+}
+
+template <int TYPE, int KIND, bool VEC, bool TURN, bool WHOLE>  // WHOLE: one scale for the tile
+__global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
+  __shared__ __align__(16) uint8_t lds[TURN ? 128 * 128 : 16];
+  __shared__ uint32_t tops[4][128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int cg = threadIdx.x % 16, rg = threadIdx.x / 16;
+  const long c0 = (long)blockIdx.x * 128, r0 = (long)blockIdx.y * 128;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const long row = r0 + rg * 8 + i, at = c0 + cg * 8;
+    load8<TYPE, VEC>(p.x, row * p.stride + at, row < p.rows ? p.cols - at : 0, v[i]);
+  }
+  uint32_t top[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    top[e] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[e] = max(top[e], magnitude(v[i][e]));
+    top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 16, 64));
+    top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 32, 64));
+  }
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top[0] = max(top[0], top[e]);
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], d, 64));
+    if (lane == 0) tops[wave][0] = top[0];
+  } else if (lane < 16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tops[wave][cg * 8 + e] = top[e];
+  }
+  __syncthreads();
+  float s[8], inv[8];
+  bool plain = true;
+#pragma unroll
+  for (int e = 0; e < (WHOLE ? 1 : 8); ++e) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) t = max(t, tops[w][WHOLE ? 0 : cg * 8 + e]);
+    s[e] = scale_of<KIND>(t);
+    inv[e] = 1.f / s[e];
+    plain &= normal_scale(s[e]);
+  }
+  if constexpr (WHOLE) {
+    if (threadIdx.x == 0)
+      p.scales[TURN ? blockIdx.x * p.s_row + blockIdx.y * p.s_block : blockIdx.y * p.s_row + blockIdx.x * p.s_block] = s[0];
+  } else if (rg == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c0 + cg * 8 + e < p.cols) p.scales[(c0 + cg * 8 + e) * p.s_row + blockIdx.y * p.s_block] = s[e];
+  }
+  if constexpr (!TURN) {
+    static_assert(TURN || WHOLE, "blocks of one row are fp8_rows'");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long row = r0 + rg * 8 + i, at = c0 + cg * 8;
+      uint32_t w[2];
+      codes8<KIND>(v[i], s[0], inv[0], plain, w);
+      if (row < p.rows && at < p.cols) store8<VEC>(p.codes + row * p.pitch + at, w, p.cols - at);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float column[8] = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
+      uint32_t w[2];
+      const float se = s[WHOLE ? 0 : e];
+      codes8<KIND>(column, se, inv[WHOLE ? 0 : e], WHOLE ? plain : normal_scale(se), w);
+      *reinterpret_cast<uint2*>(lds + (cg * 8 + e) * 128 + 8 * (rg ^ cg)) = make_uint2(w[0], w[1]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+      const int c = pass * 32 + threadIdx.x / 8, piece = threadIdx.x % 8, g = c / 8;
+      uint4 w = *reinterpret_cast<const uint4*>(lds + c * 128 + 16 * (piece ^ (g >> 1)));
+      if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+      const long out = c0 + c, at = r0 + piece * 16, count = p.rows - at;
+      if (out >= p.cols || count <= 0) continue;
+      uint8_t* to = p.codes + out * p.pitch + at;
+      if (count >= 16 && ((reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.pitch) & 15) == 0) {
+        *reinterpret_cast<uint4*>(to) = w;
+      } else {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (e < count) to[e] = (uint8_t)(u[e / 4] >> (8 * (e % 4)));
+      }
+    }
+  }
+}
+
+template <int TYPE, int KIND, bool VEC>
+hipError_t launch(const Convert& p, bool turn, bool whole, hipStream_t s) {
+  if (!turn && !whole) {
+    const long units = p.rows * ((p.cols + 127) / 128);
+    hipLaunchKernelGGL((fp8_rows<TYPE, KIND, VEC>), dim3((unsigned)((units + 15) / 16)), dim3(256), 0, s, p);
+  } else {
+    const dim3 grid((unsigned)((p.cols + 127) / 128), (unsigned)((p.rows + 127) / 128));
+    if (!turn) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, VEC, false, true>), grid, dim3(256), 0, s, p);
+    else if (whole) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, VEC, true, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((fp8_tile<TYPE, KIND, VEC, true, false>), grid, dim3(256), 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t launch_type(const Convert& p, bool e5, bool vec, bool turn, bool whole, hipStream_t s) {
+  if (e5) return vec ? launch<TYPE, SHK_FP8_E5M2, true>(p, turn, whole, s) : launch<TYPE, SHK_FP8_E5M2, false>(p, turn, whole, s);
+  return vec ? launch<TYPE, SHK_FP8_E4M3, true>(p, turn, whole, s) : launch<TYPE, SHK_FP8_E4M3, false>(p, turn, whole, s);
+}
+
+}  // namespace
+
+hipError_t launch_fp8_quantize(const shk_fp8_quantize& a, hipStream_t s) {
+  if (a.rows * a.cols == 0) return hipSuccess;
+  const Convert p{static_cast<const uint8_t*>(a.x), a.rows, a.cols, a.x_stride, static_cast<uint8_t*>(a.codes),
+                  a.code_pitch, a.scales, a.scale_row_stride, a.scale_block_stride};
+  // 16-byte loads of x, and 8-byte stores of the codes that lie as x does
+  const long size = a.type == SHK_SRC_F32 ? 4 : 2;
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(size * a.x_stride)) & 15) == 0 &&
+                   (a.transpose || ((reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.code_pitch) & 7) == 0);
+  const bool e5 = a.kind == SHK_FP8_E5M2, turn = a.transpose != 0, whole = a.block_rows == 128;
+  if (a.type == SHK_SRC_F32) return launch_type<SHK_SRC_F32>(p, e5, vec, turn, whole, s);
+  if (a.type == SHK_SRC_F16) return launch_type<SHK_SRC_F16>(p, e5, vec, turn, whole, s);
+  return launch_type<SHK_SRC_BF16>(p, e5, vec, turn, whole, s);
+}
+
+}  // namespace shk
