@@ -650,6 +650,143 @@ typedef struct shk_fp8_mm {
 int64_t amd_strix_halo_kernels_fp8_mm_workspace(const shk_fp8_mm* args);
 int amd_strix_halo_kernels_fp8_mm(int device_index, uintptr_t stream, const shk_fp8_mm* args);
 
+/* ---- query and key heads: norm and rotation by position ---------------------
+ * No counterpart in the reference.  For each token t and head row x of q [tokens,
+ * heads, head_dim] and k [tokens, kv_heads, head_dim] (head_dim contiguous, even,
+ * up to 256, strides in elements):
+ *   n = x * w / sqrt(mean(x^2) + eps)      (n = x where the weights are null)
+ * and, with c_i + j s_i = amplitude * exp(j * positions[t] * 2 pi * turns[i]),
+ * pair i of the first `rotated` values becomes (a c_i - b s_i, b c_i + a s_i):
+ * its values are 2i and 2i + 1 (interleaved) or i and i + rotated / 2.  The other
+ * values stay n.  Angles are reduced in 64 bits; the rest is f32, rounded once.
+ * Outputs go to q_out and k_out (which may be q and k with their strides).  With
+ * a cache, k_out is null and the keys, rounded to their type, go with `values`
+ * [tokens, kv_heads, head_dim] into slots[t], as amd_strix_halo_kernels_kv_write
+ * puts them there; head_dim and kv_heads are then the cache's. */
+typedef struct shk_rotate {
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const void* k;
+  int64_t k_token_stride;
+  int64_t k_head_stride;
+  int64_t type; /* SHK_SRC_F32, SHK_SRC_F16 or SHK_SRC_BF16 */
+  int64_t tokens;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t rotated;
+  int64_t interleaved;
+  const void* positions;
+  int64_t position_bytes; /* 4 or 8: int32 or int64 */
+  const double* turns;    /* rotated / 2 */
+  double amplitude;
+  const void* q_weight; /* head_dim values of weight_type each; both or none */
+  const void* k_weight;
+  int64_t weight_type;
+  double eps;
+  void* q_out;
+  int64_t q_out_token_stride;
+  int64_t q_out_head_stride;
+  void* k_out;
+  int64_t k_out_token_stride;
+  int64_t k_out_head_stride;
+  const void* values;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  const void* slots;
+  int64_t slot_bytes;
+} shk_rotate;
+
+/* cache is null where k_out is not. */
+int amd_strix_halo_kernels_rotate(int device_index, uintptr_t stream, const shk_kv_cache* cache,
+                                  const shk_rotate* args);
+
+/* ---- pages of a step ---------------------------------------------------------
+ * No counterpart in the reference.  Sequence b holds lengths[b] tokens and owns
+ * the first owned[b] pages of its row of page_table [batch, width] (contiguous);
+ * free_pages[0 .. *free_count) is a stack of unused pages, of free_total places.
+ * A step takes new_tokens[b] tokens of each sequence, in order of b:
+ *  1. A negative number ends the sequence: its pages go onto the stack, sequence
+ *     after sequence, and its length and pages become 0.
+ *  2. The others' tokens are numbered through, starts[b] = sum of new_tokens
+ *     before b (starts has batch + 1 values).  Sequence b then asks for
+ *     ceil((lengths[b] + new_tokens[b]) / page_size) - owned[b] pages.  One that
+ *     would pass its row of the table, or whose tokens pass `capacity`, asks for
+ *     none and is refused.
+ *  3. In order of b, asks are served from the top of the stack while all asks up
+ *     to b fit; one that asks for pages past that is refused.
+ *  4. Token i of [0, capacity): sequences[i] its sequence, positions[i] =
+ *     lengths[b] + i - starts[b] with the length before the step, slots[i] =
+ *     page * page_size + position in the page, -1 for a refused sequence.  Behind
+ *     the last token sequences is -1, slots -1, positions 0.
+ *  5. lengths, owned, page_table, free_pages and free_count are updated, and
+ *     taken[b] is the number of tokens that sequence b got places for.
+ * ticket is one zero int32, left zero; steps of one pool follow each other. */
+typedef struct shk_kv_plan {
+  int32_t* page_table;
+  int64_t batch; /* up to 4096 */
+  int64_t width;
+  int32_t* lengths;
+  int32_t* owned;
+  int32_t* free_pages;
+  int64_t free_total;
+  int32_t* free_count;
+  int64_t page_size; /* a power of two from 16 to 1024 */
+  const int32_t* new_tokens;
+  int64_t capacity;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* sequences;
+  int32_t* starts;
+  int32_t* taken;
+  int32_t* ticket;
+} shk_kv_plan;
+
+int amd_strix_halo_kernels_kv_plan(int device_index, uintptr_t stream, const shk_kv_plan* args);
+
+/* ---- drafted tokens ----------------------------------------------------------
+ * No counterpart in the reference.  tokens [batch, drafts] were drafted with the
+ * probabilities draft [batch, drafts, vocab] (null: each was certain), and target
+ * [batch, drafts + 1, vocab] are the target's after each of them (vocabulary
+ * contiguous, strides in elements; the probabilities need not add up to 1).
+ * Draft i is kept while uniforms[b, i] * draft[b, i, token] < target[b, i, token]
+ * (of counts[b] drafts where counts is not null, else of all).  With kept drafts,
+ * the next token is the first t with
+ *   w_0 + .. + w_t > uniforms[b, drafts] * (w_0 + .. + w_{vocab-1}),
+ * w = max(target - draft, 0) of the first draft that was not kept (target alone
+ * where these are all 0), or target after the last draft; NaN and negative
+ * weights count as 0, and where no weight is left the token is -1.  Sums are 64
+ * bits.  out [batch, drafts + 1] (int64) holds the kept drafts, the next token,
+ * then -1; kept [batch].  Where lengths is not null, lengths[b] loses the drafts
+ * that were not kept.  Draft tokens outside the vocabulary are not kept.
+ * workspace: at least amd_strix_halo_kernels_verify_workspace bytes, on 16 bytes,
+ * not read before it is written. */
+typedef struct shk_verify {
+  const void* target;
+  int64_t target_batch_stride;
+  int64_t target_row_stride;
+  const void* draft;
+  int64_t draft_batch_stride;
+  int64_t draft_row_stride;
+  int64_t type; /* SHK_SRC_F32, SHK_SRC_F16 or SHK_SRC_BF16 */
+  int64_t batch;
+  int64_t drafts; /* up to 64 */
+  int64_t vocab;
+  const void* tokens;
+  int64_t token_bytes; /* 4 or 8 */
+  const float* uniforms; /* [batch, drafts + 1] */
+  const int32_t* counts;
+  int64_t* out;
+  int32_t* kept;
+  int32_t* lengths;
+  void* workspace;
+  int64_t workspace_bytes;
+} shk_verify;
+
+int64_t amd_strix_halo_kernels_verify_workspace(const shk_verify* args);
+int amd_strix_halo_kernels_verify(int device_index, uintptr_t stream, const shk_verify* args);
+
 #ifdef __cplusplus
 }
 #endif

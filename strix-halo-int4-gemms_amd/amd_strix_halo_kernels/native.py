@@ -142,6 +142,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.amd_strix_halo_kernels_fp8_mm_workspace.restype = I64
     lib.amd_strix_halo_kernels_fp8_mm.argtypes = [I, U, P]
     lib.amd_strix_halo_kernels_fp8_mm.restype = I
+    lib.amd_strix_halo_kernels_rotate.argtypes = [I, U, P, P]
+    lib.amd_strix_halo_kernels_rotate.restype = I
+    lib.amd_strix_halo_kernels_kv_plan.argtypes = [I, U, P]
+    lib.amd_strix_halo_kernels_kv_plan.restype = I
+    lib.amd_strix_halo_kernels_verify_workspace.argtypes = [P]
+    lib.amd_strix_halo_kernels_verify_workspace.restype = I64
+    lib.amd_strix_halo_kernels_verify.argtypes = [I, U, P]
+    lib.amd_strix_halo_kernels_verify.restype = I
 
 
 def load_dispatch_library(path: str | Path | None = None) -> ctypes.CDLL:

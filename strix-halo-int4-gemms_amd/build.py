@@ -89,6 +89,10 @@ def decode_units() -> list[tuple[str, Path, list[str]]]:
         ("fp8", CSRC / "k_fp8.hip", []),
         ("fp8quant", CSRC / "k_fp8quant.hip", []),
         ("capi_fp8", CSRC / "capi_fp8.hip", []),
+        ("rotate", CSRC / "k_rotate.hip", []),
+        ("kvplan", CSRC / "k_kvplan.hip", []),
+        ("verify", CSRC / "k_verify.hip", []),
+        ("capi_step", CSRC / "capi_step.hip", []),
     ]
 
 

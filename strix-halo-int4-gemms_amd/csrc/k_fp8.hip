@@ -104,7 +104,7 @@ __device__ __forceinline__ void store_value(const Product& p, long at, float v) 
 
 template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
 __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Product p) {
-  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ __align__(16) uint8_t lds[T::P * T::STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x;
   const int m0 = tile % p.tiles_m * T::BM, n0 = tile / p.tiles_m * T::BN;
@@ -302,13 +302,8 @@ Plan plan_of(const shk_fp8_mm& a) {
 template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
 hipError_t launch(Product& p, hipStream_t s) {
   p.tiles_m = (p.m + T::BM - 1) / T::BM, p.tiles_n = (p.n + T::BN - 1) / T::BN;
-  constexpr int bytes = T::P * T::STAGE;
-  static const hipError_t set = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(fp8_product_kernel<T, KIND_A, KIND_B, BROW, WIDE>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (set != hipSuccess) return set;
   hipLaunchKernelGGL((fp8_product_kernel<T, KIND_A, KIND_B, BROW, WIDE>), dim3(p.tiles_m * p.tiles_n, p.splits),
-                     dim3(T::THREADS), bytes, s, p);
+                     dim3(T::THREADS), 0, s, p);
   return hipGetLastError();
 }
 

@@ -22,6 +22,7 @@
 
 #include "shk_common.h"
 #include "shk_kvcache.h"
+#include "shk_kvrows.h"
 
 namespace shk {
 namespace {
@@ -45,80 +46,6 @@ constexpr int kWriteRows = 1, kReadRows = 2;
 __device__ __forceinline__ long slot_of(const Rows& p, long t) {
   const long slot = p.slot8 ? static_cast<const int64_t*>(p.slots)[t] : static_cast<const int32_t*>(p.slots)[t];
   return slot >= 0 && slot < p.slots_total ? slot : -1;
-}
-
-// Row of the cache, counted in rows, of (slot, head).
-__device__ __forceinline__ long cache_row(const Rows& p, long slot, int head) {
-  const long page = slot >> p.page_shift;
-  return (((page * p.heads + head) << p.page_shift) | (slot & ((1L << p.page_shift) - 1)));
-}
-
-template <int TYPE>
-constexpr int kSize = TYPE == SHK_SRC_F32 ? 4 : 2;
-
-__device__ __forceinline__ float half_bits(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
-
-// 8 values starting at element address p; VEC: p is 16-byte aligned.
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void load8(const uint8_t* p, float (&v)[8]) {
-  if constexpr (TYPE == SHK_SRC_F32) {
-    uint32_t u[8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (VEC) {
-        const uint4 w = reinterpret_cast<const uint4*>(p)[i];
-        u[4 * i] = w.x, u[4 * i + 1] = w.y, u[4 * i + 2] = w.z, u[4 * i + 3] = w.w;
-      } else {
-        for (int j = 0; j < 4; ++j) u[4 * i + j] = reinterpret_cast<const uint32_t*>(p)[4 * i + j];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
-  } else {
-    uint32_t u[4];
-    if constexpr (VEC) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
-    } else {
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = TYPE == SHK_SRC_BF16 ? __uint_as_float(u[i] << 16) : half_bits(u[i] & 0xFFFFu);
-      v[2 * i + 1] = TYPE == SHK_SRC_BF16 ? __uint_as_float(u[i] & 0xFFFF0000u) : half_bits(u[i] >> 16);
-    }
-  }
-}
-
-// fl32(x / s) for 8 values.  With inv = fl32(1 / s), q = fl32(x * inv) is
-// within one unit of x / s, its remainder x - q * s is exact in one fused
-// multiply-add, and q + remainder * inv rounds to fl32(x / s) (Markstein's
-// theorem) as long as nothing on the way leaves the normal range.  That
-// holds for the scales between the bounds, where codes matter (|x / s| of 2^-30
-// rounds to 0 either way); rows outside them divide.
-template <int BITS>
-__device__ __forceinline__ void codes8(const float (&v)[8], float s, int (&c)[8]) {
-  constexpr float Q = BITS == 4 ? 7.0f : 127.0f;
-  const bool usable = s > 0.0f && s < __builtin_inff();
-  float q[8];
-  if (s > 0x1p-60f && s < 0x1p60f) {
-    const float inv = 1.0f / s;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q0 = v[i] * inv;
-      q[i] = __builtin_fmaf(__builtin_fmaf(-q0, s, v[i]), inv, q0);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] / s;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float r = __builtin_fminf(__builtin_fmaxf(__builtin_rintf(q[i]), -Q), Q);
-    c[i] = usable ? (int)r : 0;
-  }
 }
 
 template <int TYPE, int BITS, int D, bool VEC>
@@ -154,22 +81,9 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const Rows p) {
       const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (BITS == 4 ? 7.0f : 127.0f));
       int c[8];
       codes8<BITS>(v[i][which], __uint_as_float(sb << 16), c);
-      const long out = cache_row(p, slot[i], head[i]);
+      const long out = cache_row(slot[i], head[i], p.heads, p.page_shift);
       uint8_t* dst = p.codes[which] + out * (D * BITS / 8) + part * BITS;
-      if constexpr (BITS == 4) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w |= ((uint32_t)c[e] & 0xFu) << (4 * e);
-        *reinterpret_cast<uint32_t*>(dst) = w;
-      } else {
-        uint32_t lo = 0, hi = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          lo |= ((uint32_t)c[e] & 0xFFu) << (8 * e);
-          hi |= ((uint32_t)c[e + 4] & 0xFFu) << (8 * e);
-        }
-        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-      }
+      store_codes<BITS>(dst, c);
       if (part == 0) p.scales[which][out] = (uint16_t)sb;
     }
 }
@@ -220,7 +134,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const Rows p) {
     t[i] = row / p.heads;
     head[i] = row - t[i] * p.heads;
     slot[i] = row < p.rows ? slot_of(p, t[i]) : -1;
-    const long at = slot[i] >= 0 ? cache_row(p, slot[i], head[i]) : 0;
+    const long at = slot[i] >= 0 ? cache_row(slot[i], head[i], p.heads, p.page_shift) : 0;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       scale[i][which] = __builtin_nanf("");
