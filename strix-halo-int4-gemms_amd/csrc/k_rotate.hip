@@ -83,187 +83,284 @@ __device__ __forceinline__ float rounded(float v) {
   else return (float)(_Float16)v;
 }
 
-// VEC: every row starts on 16 bytes and is whole 8s, and so is `half` if pairs
-// lie apart.
-template <int TYPE, int LANES, bool VEC, bool APART, int ROUNDS>
-__global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
-  constexpr int PER = 256 / LANES;  // rows of a round
-  extern __shared__ float2 angles[];
-  const int part = threadIdx.x % LANES, first_value = part * 8;
-  const unsigned start = blockIdx.x * (PER * ROUNDS), mine = start + threadIdx.x / LANES;
-  const bool inside = first_value < p.dim;
-  const int count = min(8, p.dim - first_value);
-  float v[ROUNDS][8], w[ROUNDS][8];
-  unsigned token[ROUNDS], head[ROUNDS];
-  int kind[ROUNDS];
-#pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) {
-    const unsigned row = mine + i * PER;
-    token[i] = row / p.per_token;
-    const unsigned h = row - token[i] * p.per_token;
-    kind[i] = row >= p.rows || !inside ? -1 : h < p.heads ? 0 : h < p.heads + p.kv_heads ? 1 : 2;
-    head[i] = kind[i] == 0 ? h : kind[i] == 1 ? h - p.heads : h - p.heads - p.kv_heads;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = w[i][e] = 0.f;
-    if (kind[i] < 0) continue;
-    const uint8_t* x = p.x[kind[i]] + ((long)token[i] * p.token_stride[kind[i]] + (long)head[i] * p.head_stride[kind[i]]) *
-                                          kSize<TYPE>;
-    if constexpr (VEC) {
-      load8<TYPE, true>(x + first_value * kSize<TYPE>, v[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < count) v[i][e] = element<TYPE>(x, first_value + e);
-    }
-    if (APART && kind[i] < 2 && first_value < p.rotated) {
-      if constexpr (VEC) {
-        load8<TYPE, true>(x + (first_value < p.half ? first_value + p.half : first_value - p.half) * kSize<TYPE>, w[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int at = first_value + e;
-          if (at < p.rotated) w[i][e] = element<TYPE>(x, at < p.half ? at + p.half : at - p.half);
-        }
-      }
-    }
-  }
-  const unsigned last = min(start + PER * ROUNDS, p.rows) - 1, token0 = start / p.per_token;
-  const unsigned tokens = last / p.per_token - token0 + 1;
+// The angles of the tokens that a workgroup meets, cosines and sines apart, and
+// both norms' weights, in LDS.
+struct Shared {
+  float* cosines;  // [tokens][half]
+  float* sines;
+  float* weights;  // [2][dim]
+};
+
+__device__ __forceinline__ Shared shared_parts(float* lds, const Rotate& p, unsigned tokens) {
+  return Shared{lds, lds + tokens * p.half, lds + 2 * tokens * p.half};
+}
+
+__device__ __forceinline__ void fill_shared(const Shared& s, const Rotate& p, unsigned token0, unsigned tokens) {
   for (unsigned i = threadIdx.x; i < tokens * p.half; i += 256) {
     const unsigned t = i / p.half;
     const long at = token0 + t;
     const double position = p.position8 ? (double)static_cast<const int64_t*>(p.positions)[at]
                                         : (double)static_cast<const int32_t*>(p.positions)[at];
-    float2 cs = turned(position * p.turns[i - t * p.half]);
-    cs.x *= p.amplitude, cs.y *= p.amplitude;
-    angles[i] = cs;
+    const float2 cs = turned(position * p.turns[i - t * p.half]);
+    s.cosines[i] = cs.x * p.amplitude, s.sines[i] = cs.y * p.amplitude;
   }
-  __syncthreads();
+  if (p.weight[0] != nullptr)
+    for (int i = threadIdx.x; i < 2 * p.dim; i += 256)
+      s.weights[i] = i < p.dim ? weight_of(p, 0, i) : weight_of(p, 1, i - p.dim);
+}
+
+// A row of one round: which head of which token.
+struct Place {
+  unsigned token, head;
+  int kind;  // 0 query, 1 key, 2 value, -1 none
+};
+
+__device__ __forceinline__ Place place_of(const Rotate& p, unsigned row, bool inside) {
+  Place r;
+  r.token = row / p.per_token;
+  const unsigned h = row - r.token * p.per_token;
+  r.kind = row >= p.rows || !inside ? -1 : h < p.heads ? 0 : h < p.heads + p.kv_heads ? 1 : 2;
+  r.head = r.kind == 0 ? h : r.kind == 1 ? h - p.heads : h - p.heads - p.kv_heads;
+  return r;
+}
+
+// The quantized row of a key or value, as kv_write_kernel makes it: a NaN is
+// larger than an infinity, and both stay.
+template <int TYPE, int LANES>
+__device__ __forceinline__ void into_cache(const Rotate& p, const Place& r, int part, float (&v)[8]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = rounded<TYPE>(v[e]);
+    most = max(most, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+  }
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+  const long slot = p.slot8 ? static_cast<const int64_t*>(p.slots)[r.token] : static_cast<const int32_t*>(p.slots)[r.token];
+  if (slot < 0 || slot >= p.slots_total) return;
+  const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (p.bits == 4 ? 7.0f : 127.0f));
+  const long at = cache_row(slot, r.head, p.kv_heads, p.page_shift);
+  uint8_t* dst = p.codes[r.kind - 1] + at * (p.dim * p.bits / 8) + part * p.bits;
+  int c[8];
+  if (p.bits == 4) {
+    codes8<4>(v, __uint_as_float(sb << 16), c);
+    store_codes<4>(dst, c);
+  } else {
+    codes8<8>(v, __uint_as_float(sb << 16), c);
+    store_codes<8>(dst, c);
+  }
+  if (part == 0) p.scales[r.kind - 1][at] = (uint16_t)sb;
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  // v_cvt_pk_bf16_f32 leaves a quiet NaN one, and arithmetic makes no other
+  if constexpr (TYPE == SHK_SRC_BF16) return pack_bf16x2_nonan(a, b);
+  return __builtin_bit_cast(uint16_t, (_Float16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16);
+}
+
+// Eight floats of LDS, on 16 bytes.
+__device__ __forceinline__ void read8(const float* from, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+// Rows on 16 bytes whose values, turning ones and (APART) half of them are whole
+// 8s: a lane turns with all its values or none, and its partners are one load.
+template <int TYPE, int LANES, bool APART, int ROUNDS>
+__global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
+  constexpr int PER = 256 / LANES;  // rows of a round
+  extern __shared__ __align__(16) float lds[];
+  const int part = threadIdx.x % LANES, first = part * 8;
+  const unsigned start = blockIdx.x * (PER * ROUNDS), mine = start + threadIdx.x / LANES;
+  const bool inside = first < p.dim, turning = first < p.rotated, low = first < p.half;
+  const int partner = APART ? (low ? first + p.half : first - p.half) : 0;
+  Place place[ROUNDS];
+  float v[ROUNDS][8], w[APART ? ROUNDS : 1][8];
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
-    const bool turns = kind[i] == 0 || kind[i] == 1;
-    const int which = kind[i] == 1;
-    if (p.weight[0] != nullptr) {  // of both or of none
+    place[i] = place_of(p, mine + i * PER, inside);
+    const Place& r = place[i];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    if (r.kind < 0) continue;
+    const uint8_t* x = p.x[r.kind] + ((long)r.token * p.token_stride[r.kind] + (long)r.head * p.head_stride[r.kind]) *
+                                         kSize<TYPE>;
+    load8<TYPE, true>(x + first * kSize<TYPE>, v[i]);
+    if constexpr (APART)
+      if (r.kind < 2 && turning) load8<TYPE, true>(x + partner * kSize<TYPE>, w[i]);
+  }
+  const unsigned last = min(start + PER * ROUNDS, p.rows) - 1, token0 = start / p.per_token;
+  const unsigned tokens = last / p.per_token - token0 + 1;
+  const Shared s = shared_parts(lds, p, tokens);
+  fill_shared(s, p, token0, tokens);
+  __syncthreads();
+  const bool norm = p.weight[0] != nullptr;
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const Place& r = place[i];
+    const bool head = r.kind == 0 || r.kind == 1;
+    float scale = 1.f;
+    if (norm) {
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[i][e], v[i][e], sum);
 #pragma unroll
       for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d, 64);
-      const float scale = 1.f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
-      if (turns) {
+      scale = 1.f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
+      if (head) {
+        float weight[8];
+        read8(s.weights + (r.kind == 1 ? p.dim : 0) + first, weight);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int at = first_value + e;
-          if (VEC || e < count) v[i][e] = v[i][e] * scale * weight_of(p, which, at);
-          if (APART && at < p.rotated)
-            w[i][e] = w[i][e] * scale * weight_of(p, which, at < p.half ? at + p.half : at - p.half);
-        }
+        for (int e = 0; e < 8; ++e) v[i][e] *= scale * weight[e];
       }
     }
-    if (turns) {
-      const float2* cs = angles + (token[i] - token0) * p.half;
+    if (head && turning) {
+      float c[8], n[8];
+      const float* angles = s.cosines + (r.token - token0) * p.half;
+      const long sines = s.sines - s.cosines;
       if constexpr (APART) {
+        const float* at = angles + (low ? first : partner);
+        read8(at, c);
+        read8(at + sines, n);
+        float weight[8];
+        if (norm) {
+          read8(s.weights + (r.kind == 1 ? p.dim : 0) + partner, weight);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int at = first_value + e;
-          if (at >= p.rotated) continue;
-          const bool low = at < p.half;
-          const float2 c = cs[low ? at : at - p.half];
-          v[i][e] = __builtin_fmaf(v[i][e], c.x, (low ? -w[i][e] : w[i][e]) * c.y);
+          for (int e = 0; e < 8; ++e) weight[e] = 1.f;
         }
+        const float turn = low ? -scale : scale;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(w[i][e] * (turn * weight[e]), n[e], v[i][e] * c[e]);
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const int at = first_value + e;
-          if (at >= p.rotated) continue;
-          const float2 c = cs[at / 2];
-          const float a = v[i][e], b = v[i][e + 1];
-          v[i][e] = __builtin_fmaf(a, c.x, -b * c.y);
-          v[i][e + 1] = __builtin_fmaf(b, c.x, a * c.y);
-        }
-      }
-    }
-    if (kind[i] >= 1 && p.bits != 0) {
-      // as kv_write_kernel does: a NaN is larger than an infinity, and both stay
-      uint32_t most = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[i][e] = rounded<TYPE>(v[i][e]);
-        most = max(most, __float_as_uint(v[i][e]) & 0x7FFFFFFFu);
-      }
-#pragma unroll
-      for (int d = 1; d < LANES; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
-      const long slot = p.slot8 ? static_cast<const int64_t*>(p.slots)[token[i]]
-                                : static_cast<const int32_t*>(p.slots)[token[i]];
-      if (slot < 0 || slot >= p.slots_total) continue;
-      const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (p.bits == 4 ? 7.0f : 127.0f));
-      const long at = cache_row(slot, head[i], p.kv_heads, p.page_shift);
-      uint8_t* dst = p.codes[kind[i] - 1] + at * (p.dim * p.bits / 8) + part * p.bits;
-      int c[8];
-      if (p.bits == 4) {
-        codes8<4>(v[i], __uint_as_float(sb << 16), c);
-        store_codes<4>(dst, c);
-      } else {
-        codes8<8>(v[i], __uint_as_float(sb << 16), c);
-        store_codes<8>(dst, c);
-      }
-      if (part == 0) p.scales[kind[i] - 1][at] = (uint16_t)sb;
-    } else if (kind[i] >= 0) {
-      uint8_t* out = p.out[which] + ((long)token[i] * p.out_token_stride[which] + (long)head[i] * p.out_head_stride[which] +
-                                     first_value) * kSize<TYPE>;
-      uint32_t u[TYPE == SHK_SRC_F32 ? 8 : 4];
-      if constexpr (TYPE == SHK_SRC_F32) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(v[i][e]);
-      } else {
+        const float4 cc = *reinterpret_cast<const float4*>(angles + first / 2);
+        const float4 nn = *reinterpret_cast<const float4*>(angles + sines + first / 2);
+        c[0] = cc.x, c[1] = cc.y, c[2] = cc.z, c[3] = cc.w;
+        n[0] = nn.x, n[1] = nn.y, n[2] = nn.z, n[3] = nn.w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (TYPE == SHK_SRC_BF16)
-            u[e] = f32_to_bf16_rne(v[i][2 * e]) | (f32_to_bf16_rne(v[i][2 * e + 1]) << 16);
-          else
-            u[e] = __builtin_bit_cast(uint16_t, (_Float16)v[i][2 * e]) |
-                   ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[i][2 * e + 1]) << 16);
+          const float a = v[i][2 * e], b = v[i][2 * e + 1];
+          v[i][2 * e] = __builtin_fmaf(-b, n[e], a * c[e]);
+          v[i][2 * e + 1] = __builtin_fmaf(a, n[e], b * c[e]);
         }
       }
-      if constexpr (VEC) {
-#pragma unroll
-        for (int e = 0; e < (TYPE == SHK_SRC_F32 ? 2 : 1); ++e)
-          reinterpret_cast<uint4*>(out)[e] = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+    }
+    if (r.kind >= 1 && p.bits != 0) {
+      into_cache<TYPE, LANES>(p, r, part, v[i]);
+    } else if (r.kind >= 0) {
+      uint8_t* out = p.out[r.kind] + ((long)r.token * p.out_token_stride[r.kind] +
+                                      (long)r.head * p.out_head_stride[r.kind] + first) * kSize<TYPE>;
+      if constexpr (TYPE == SHK_SRC_F32) {
+        reinterpret_cast<float4*>(out)[0] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+        reinterpret_cast<float4*>(out)[1] = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e >= count) continue;
-          if constexpr (TYPE == SHK_SRC_F32) reinterpret_cast<uint32_t*>(out)[e] = u[e];
-          else reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)(u[e / 2] >> (16 * (e % 2)));
-        }
+        *reinterpret_cast<uint4*>(out) = make_uint4(pack2<TYPE>(v[i][0], v[i][1]), pack2<TYPE>(v[i][2], v[i][3]),
+                                                    pack2<TYPE>(v[i][4], v[i][5]), pack2<TYPE>(v[i][6], v[i][7]));
       }
     }
   }
 }
 
-template <int TYPE, int LANES, bool VEC, bool APART, int ROUNDS>
+// Any strides, sizes and alignment: value by value.
+template <int TYPE, int LANES, bool APART>
+__global__ __launch_bounds__(256) void rotate_any_kernel(const Rotate p) {
+  constexpr int PER = 256 / LANES;
+  extern __shared__ __align__(16) float lds[];
+  const int part = threadIdx.x % LANES, first = part * 8, count = min(8, p.dim - first);
+  const unsigned start = blockIdx.x * PER;
+  const Place r = place_of(p, start + threadIdx.x / LANES, count > 0);
+  const bool head = r.kind == 0 || r.kind == 1, norm = p.weight[0] != nullptr;
+  float v[8] = {}, w[8] = {};
+  if (r.kind >= 0) {
+    const uint8_t* x = p.x[r.kind] + ((long)r.token * p.token_stride[r.kind] + (long)r.head * p.head_stride[r.kind]) *
+                                         kSize<TYPE>;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = first + e;
+      if (e < count) v[e] = element<TYPE>(x, at);
+      if (APART && head && at < p.rotated) w[e] = element<TYPE>(x, at < p.half ? at + p.half : at - p.half);
+    }
+  }
+  const unsigned last = min(start + PER, p.rows) - 1, token0 = start / p.per_token;
+  const unsigned tokens = last / p.per_token - token0 + 1;
+  const Shared s = shared_parts(lds, p, tokens);
+  fill_shared(s, p, token0, tokens);
+  __syncthreads();
+  float scale = 1.f;
+  if (norm) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d, 64);
+    scale = 1.f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
+  }
+  if (head) {
+    const float* weight = s.weights + (r.kind == 1 ? p.dim : 0);
+    const unsigned angles = (r.token - token0) * p.half;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (norm && e < count) v[e] *= scale * weight[first + e];
+#pragma unroll
+    for (int e = 0; e < 8; e += APART ? 1 : 2) {
+      const int at = first + e;
+      if (at >= p.rotated) continue;
+      if constexpr (APART) {
+        const bool low = at < p.half;
+        const int pair = low ? at : at - p.half;
+        const float turn = (low ? -scale : scale) * (norm ? weight[low ? at + p.half : pair] : 1.f);
+        v[e] = __builtin_fmaf(w[e] * turn, s.sines[angles + pair], v[e] * s.cosines[angles + pair]);
+      } else {
+        const float c = s.cosines[angles + at / 2], n = s.sines[angles + at / 2], a = v[e], b = v[e + 1];
+        v[e] = __builtin_fmaf(-b, n, a * c);
+        v[e + 1] = __builtin_fmaf(a, n, b * c);
+      }
+    }
+  }
+  if (r.kind >= 1 && p.bits != 0) {
+    into_cache<TYPE, LANES>(p, r, part, v);
+  } else if (r.kind >= 0) {
+    uint8_t* out = p.out[r.kind] + ((long)r.token * p.out_token_stride[r.kind] +
+                                    (long)r.head * p.out_head_stride[r.kind] + first) * kSize<TYPE>;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e >= count) continue;
+      if constexpr (TYPE == SHK_SRC_F32) reinterpret_cast<float*>(out)[e] = v[e];
+      else reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)pack2<TYPE>(v[e], 0.f);
+    }
+  }
+}
+
+// LDS of a workgroup of `rows` rows: angles of the tokens that it can meet, weights.
+unsigned shared_bytes(const Rotate& p, unsigned rows) {
+  const unsigned tokens = (rows + p.per_token - 2) / p.per_token + 1;
+  return (2 * tokens * p.half + (p.weight[0] != nullptr ? 2 * p.dim : 0)) * sizeof(float);
+}
+
+template <int TYPE, int LANES, bool APART, int ROUNDS>
 hipError_t launch(const Rotate& p, hipStream_t s) {
   constexpr unsigned PER = 256 / LANES * ROUNDS;
-  // tokens that a workgroup can meet
-  const unsigned tokens = (PER + p.per_token - 2) / p.per_token + 1;
-  hipLaunchKernelGGL((rotate_kernel<TYPE, LANES, VEC, APART, ROUNDS>), dim3((p.rows + PER - 1) / PER), dim3(256),
-                     tokens * p.half * sizeof(float2), s, p);
+  hipLaunchKernelGGL((rotate_kernel<TYPE, LANES, APART, ROUNDS>), dim3((p.rows + PER - 1) / PER), dim3(256),
+                     shared_bytes(p, PER), s, p);
   return hipGetLastError();
 }
 
-template <int TYPE, int LANES, bool VEC>
-hipError_t launch_pairs(const Rotate& p, bool apart, hipStream_t s) {
-  // one round while that leaves CUs idle, else four, whose loads go out together
-  const bool few = !VEC || p.rows <= 256u * (256 / LANES) * 4;
-  if constexpr (VEC) {
-    if (!few) return apart ? launch<TYPE, LANES, VEC, true, 4>(p, s) : launch<TYPE, LANES, VEC, false, 4>(p, s);
+template <int TYPE, int LANES, bool APART>
+hipError_t launch_pairs(const Rotate& p, bool vec, hipStream_t s) {
+  constexpr unsigned PER = 256 / LANES;
+  if (!vec) {
+    hipLaunchKernelGGL((rotate_any_kernel<TYPE, LANES, APART>), dim3((p.rows + PER - 1) / PER), dim3(256),
+                       shared_bytes(p, PER), s, p);
+    return hipGetLastError();
   }
-  return apart ? launch<TYPE, LANES, VEC, true, 1>(p, s) : launch<TYPE, LANES, VEC, false, 1>(p, s);
+  // one round while that leaves CUs idle, else four, whose loads go out together
+  return p.rows <= 256 * PER * 4 ? launch<TYPE, LANES, APART, 1>(p, s) : launch<TYPE, LANES, APART, 4>(p, s);
 }
 
 template <int TYPE, int LANES>
 hipError_t launch_vec(const Rotate& p, bool vec, bool apart, hipStream_t s) {
-  return vec ? launch_pairs<TYPE, LANES, true>(p, apart, s) : launch_pairs<TYPE, LANES, false>(p, apart, s);
+  return apart ? launch_pairs<TYPE, LANES, true>(p, vec, s) : launch_pairs<TYPE, LANES, false>(p, vec, s);
 }
 
 template <int TYPE>
@@ -309,7 +406,7 @@ hipError_t launch_rotate(const shk_kv_cache* c, const shk_rotate& a, hipStream_t
     all |= (uintptr_t)(size * (a.k_out_token_stride | a.k_out_head_stride));
   }
   const bool apart = a.interleaved == 0;
-  const bool vec = (all & 15) == 0 && a.head_dim % 8 == 0 && (!apart || p.half % 8 == 0);
+  const bool vec = (all & 15) == 0 && a.head_dim % 8 == 0 && a.rotated % (apart ? 16 : 8) == 0;
   if (a.type == SHK_SRC_F32) return launch_type<SHK_SRC_F32>(p, vec, apart, s);
   if (a.type == SHK_SRC_F16) return launch_type<SHK_SRC_F16>(p, vec, apart, s);
   return launch_type<SHK_SRC_BF16>(p, vec, apart, s);

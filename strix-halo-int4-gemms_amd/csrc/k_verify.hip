@@ -10,7 +10,7 @@
 // Bound by the one row of each kind that a sequence reads, or by two launches.
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
+#include <climits>
 #include <cstdint>
 
 #include "shk_common.h"
@@ -20,21 +20,53 @@ namespace shk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPieces = 256;  // at most, of a row
+constexpr int kPieces = 256;           // at most, of a row
+constexpr int kPiece = kThreads * 8;   // values of a step of a workgroup
 
 struct Pieces {
-  int count, size;  // size: values of a piece, whole 8s
+  int count, size;  // size: values of a piece, whole steps
 };
 
 struct Sum {
   double left, all;  // of max(target - draft, 0), of target
 };
 
+// What verify_sums leaves for verify_draw: kept drafts of each sequence, then the
+// sums of its pieces.
+__host__ __device__ constexpr long kept_bytes(long batch) { return (batch * 4 + 15) / 16 * 16; }
+
 template <int TYPE>
 __device__ __forceinline__ float value_of(const void* x, long i) {
   if constexpr (TYPE == SHK_SRC_F32) return static_cast<const float*>(x)[i];
   const uint16_t h = static_cast<const uint16_t*>(x)[i];
   return TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+}
+
+// Values [at, at + 8) of a row, those from `count` on as 0.  VEC: on 16 bytes.
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load8(const void* x, long at, long count, float (&v)[8]) {
+  if (VEC && count >= 8) {
+    constexpr int SIZE = TYPE == SHK_SRC_F32 ? 4 : 2;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * SIZE);
+    uint32_t u[SIZE * 2];
+#pragma unroll
+    for (int i = 0; i < SIZE / 2; ++i) {
+      const uint4 w = src[i];
+      u[4 * i] = w.x, u[4 * i + 1] = w.y, u[4 * i + 2] = w.z, u[4 * i + 3] = w.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (TYPE == SHK_SRC_F32) {
+        v[e] = __uint_as_float(u[e]);
+      } else {
+        const uint16_t h = (uint16_t)(u[e / 2] >> (16 * (e % 2)));
+        v[e] = TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < count ? value_of<TYPE>(x, at + e) : 0.f;
 }
 
 __device__ __forceinline__ long token_of(const shk_verify& p, long i) {
@@ -78,15 +110,20 @@ __device__ __forceinline__ Row row_of(const shk_verify& p, long b, int kept) {
   return r;
 }
 
-// Weights of value t; NaN and negative ones count as 0.
-template <int TYPE>
-__device__ __forceinline__ Sum weight_at(const shk_verify& p, const Row& r, long t) {
-  Sum w;
-  w.all = __builtin_fmax((double)value_of<TYPE>(p.target, r.target + t), 0.0);
-  w.left = w.all;
-  if (r.draft >= 0) w.left = __builtin_fmax(w.all - (double)value_of<TYPE>(p.draft, r.draft + t), 0.0);
-  else if (t == r.certain) w.left = 0.0;
-  return w;
+// Weights of values [t, t + 8); NaN and negative ones count as 0.
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void weights8(const shk_verify& p, const Row& r, long t, Sum (&w)[8]) {
+  const long count = p.vocab - t;
+  float have[8], gone[8];
+  load8<TYPE, VEC>(p.target, r.target + t, count, have);
+  if (r.draft >= 0) {
+    load8<TYPE, VEC>(p.draft, r.draft + t, count, gone);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    w[e].all = __builtin_fmaxf(have[e], 0.f);
+    w[e].left = r.draft >= 0 ? __builtin_fmax(w[e].all - (double)gone[e], 0.0) : t + e == r.certain ? 0.0 : w[e].all;
+  }
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -95,98 +132,110 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-template <int TYPE>
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, const Pieces pieces) {
-  __shared__ double parts[2][kThreads / 64];
+  __shared__ Sum parts[kThreads / 64];
   const long b = blockIdx.y;
-  const Row r = row_of(p, b, kept_of<TYPE>(p, b));
+  const int kept = kept_of<TYPE>(p, b);
+  const Row r = row_of(p, b, kept);
   const long from = (long)blockIdx.x * pieces.size, to = min(from + pieces.size, (long)p.vocab);
   Sum mine{0.0, 0.0};
-  for (long t = from + threadIdx.x; t < to; t += kThreads) {
-    const Sum w = weight_at<TYPE>(p, r, t);
-    mine.left += w.left, mine.all += w.all;
+  for (long t = from + threadIdx.x * 8; t < to; t += kPiece) {
+    Sum w[8];
+    weights8<TYPE, VEC>(p, r, t, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine.left += w[e].left, mine.all += w[e].all;
   }
   mine.left = wave_sum(mine.left), mine.all = wave_sum(mine.all);
-  if ((threadIdx.x & 63) == 0) parts[0][threadIdx.x >> 6] = mine.left, parts[1][threadIdx.x >> 6] = mine.all;
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = mine;
   __syncthreads();
   if (threadIdx.x == 0) {
-    Sum s{0.0, 0.0};
-    for (int w = 0; w < kThreads / 64; ++w) s.left += parts[0][w], s.all += parts[1][w];
-    static_cast<Sum*>(p.workspace)[b * pieces.count + blockIdx.x] = s;
+    Sum s = parts[0];
+    for (int w = 1; w < kThreads / 64; ++w) s.left += parts[w].left, s.all += parts[w].all;
+    uint8_t* work = static_cast<uint8_t*>(p.workspace);
+    reinterpret_cast<Sum*>(work + kept_bytes(p.batch))[b * pieces.count + blockIdx.x] = s;
+    if (blockIdx.x == 0) reinterpret_cast<int32_t*>(work)[b] = kept;
   }
 }
 
-// Inclusive sum over the workgroup's threads.
-__device__ __forceinline__ double group_inclusive(double v, double (&parts)[kThreads / 64]) {
+// Inclusive sums over the workgroup's threads, of both weights.
+__device__ __forceinline__ Sum group_inclusive(Sum v, Sum (&parts)[kThreads / 64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const double o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
+    const Sum o{__shfl_up(v.left, d, 64), __shfl_up(v.all, d, 64)};
+    if (lane >= d) v.left += o.left, v.all += o.all;
   }
-  __syncthreads();
   if (lane == 63) parts[wave] = v;
   __syncthreads();
-  double before = 0.0;
-  for (int w = 0; w < wave; ++w) before += parts[w];
-  return before + v;
+  Sum before{0.0, 0.0};
+  for (int w = 0; w < wave; ++w) before.left += parts[w].left, before.all += parts[w].all;
+  return Sum{before.left + v.left, before.all + v.all};
 }
 
-template <int TYPE>
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, const Pieces pieces) {
-  __shared__ double parts[kThreads / 64], before_piece, total_all;
-  __shared__ int piece, passes, holds;
+  __shared__ Sum parts[2][kThreads / 64], total;
+  __shared__ double before;
+  __shared__ int piece, passes, holds, holds_here;
   const long b = blockIdx.x;
-  const int kept = kept_of<TYPE>(p, b);
+  const uint8_t* work = static_cast<const uint8_t*>(p.workspace);
+  const int kept = reinterpret_cast<const int32_t*>(work)[b];
   const Row r = row_of(p, b, kept);
-  const Sum* sums = static_cast<const Sum*>(p.workspace) + b * pieces.count;
+  const Sum* sums = reinterpret_cast<const Sum*>(work + kept_bytes(p.batch)) + b * pieces.count;
   const Sum mine = (int)threadIdx.x < pieces.count ? sums[threadIdx.x] : Sum{0.0, 0.0};
-  const double left = group_inclusive(mine.left, parts), all = group_inclusive(mine.all, parts);
-  if (threadIdx.x == 0) piece = passes = kThreads, holds = -1;
-  if (threadIdx.x == kThreads - 1) before_piece = left, total_all = all;
+  const Sum upto = group_inclusive(mine, parts[0]);
+  if (threadIdx.x == 0) piece = passes = INT_MAX, holds = holds_here = -1;
+  if (threadIdx.x == kThreads - 1) total = upto;
   __syncthreads();
-  const bool rest = before_piece > 0.0;
-  const double total = rest ? before_piece : total_all, upto = rest ? left : all, own = rest ? mine.left : mine.all;
-  const double share = (double)p.uniforms[b * (p.drafts + 1) + p.drafts] * total;
-  __syncthreads();
+  const bool rest = total.left > 0.0;
+  const double share = (double)p.uniforms[b * (p.drafts + 1) + p.drafts] * (rest ? total.left : total.all);
+  const double run = rest ? upto.left : upto.all, own = rest ? mine.left : mine.all;
   // the first piece whose running sum passes the share; the last that holds
   // anything where a share of the whole sum, or more, was asked for
   if (own > 0.0) {
-    if (upto > share) atomicMin(&piece, (int)threadIdx.x);
+    if (run > share) atomicMin(&piece, (int)threadIdx.x);
     atomicMax(&holds, (int)threadIdx.x);
   }
   __syncthreads();
   const int at = piece < kThreads ? piece : holds;
-  if ((int)threadIdx.x == at) before_piece = upto - own;
+  if ((int)threadIdx.x == at) before = run - own;
   __syncthreads();
   long token = -1;
   if (at >= 0) {
-    double run = before_piece;
+    double carry = before;
     const long from = (long)at * pieces.size, to = min(from + pieces.size, (long)p.vocab);
-    int best = -1, most = -1;  // offsets in the piece
-    for (long base = from; base < to && best < 0; base += kThreads) {
-      const long t = base + threadIdx.x;
-      double w = 0.0;
-      if (t < to) {
-        const Sum s = weight_at<TYPE>(p, r, t);
-        w = rest ? s.left : s.all;
+    for (long base = from; base < to; base += kPiece) {
+      const long t = base + threadIdx.x * 8;
+      Sum w[8], sum{0.0, 0.0};
+      weights8<TYPE, VEC>(p, r, t, w);
+      double values[8], mass = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        values[e] = t + e < to ? (rest ? w[e].left : w[e].all) : 0.0;
+        mass += values[e];
       }
-      const double sum = run + group_inclusive(w, parts);
-      if (threadIdx.x == 0) passes = kThreads, holds = -1;
-      __syncthreads();
-      if (w > 0.0) {
-        if (sum > share) atomicMin(&passes, (int)threadIdx.x);
-        atomicMax(&holds, (int)threadIdx.x);
+      sum.left = mass;
+      const double through = carry + group_inclusive(sum, parts[1]).left;
+      double upto_e = through - mass;
+      int first = -1, last = -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        upto_e += values[e];
+        if (values[e] > 0.0) {
+          last = (int)(t - from) + e;
+          if (first < 0 && upto_e > share) first = last;
+        }
       }
-      if (threadIdx.x == kThreads - 1) before_piece = sum;
+      if (first >= 0) atomicMin(&passes, first);
+      if (last >= 0) atomicMax(&holds_here, last);
+      if (threadIdx.x == kThreads - 1) before = through;
       __syncthreads();
-      if (passes < kThreads) best = (int)(base - from) + passes;
-      if (holds >= 0) most = (int)(base - from) + holds;
-      run = before_piece;
-      __syncthreads();
+      if (passes != INT_MAX) break;
+      carry = before;
     }
     // rounding can leave the running sum of a piece just below its own sum
-    token = from + (best >= 0 ? best : most);
+    token = from + (passes != INT_MAX ? passes : holds_here);
   }
   for (int i = threadIdx.x; i <= (int)p.drafts; i += kThreads)
     p.out[b * (p.drafts + 1) + i] = i < kept ? token_of(p, b * p.drafts + i) : i == kept ? token : -1;
@@ -197,29 +246,40 @@ __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, cons
 }
 
 Pieces pieces_of(const shk_verify& a) {
-  // enough workgroups for the chip, pieces of at least 2048 values
-  const long want = std::min<long>(kPieces, std::max<long>(1, 1024 / std::max<int64_t>(1, a.batch)));
-  long size = std::max<long>(2048, ((a.vocab + want - 1) / want + 7) / 8 * 8);
-  return Pieces{(int)((a.vocab + size - 1) / size), (int)size};
+  // one step each, more where a row has more steps than a workgroup threads
+  const long steps = (a.vocab + kPiece - 1) / kPiece, each = (steps + kPieces - 1) / kPieces;
+  return Pieces{(int)((steps + each - 1) / each), (int)(each * kPiece)};
+}
+
+template <int TYPE, bool VEC>
+hipError_t launch(const shk_verify& a, hipStream_t s) {
+  const Pieces pieces = pieces_of(a);
+  hipLaunchKernelGGL((verify_sums<TYPE, VEC>), dim3(pieces.count, (unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
+  if (hipError_t e = hipGetLastError()) return e;
+  hipLaunchKernelGGL((verify_draw<TYPE, VEC>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
+  return hipGetLastError();
 }
 
 template <int TYPE>
-hipError_t launch(const shk_verify& a, hipStream_t s) {
-  const Pieces pieces = pieces_of(a);
-  hipLaunchKernelGGL((verify_sums<TYPE>), dim3(pieces.count, (unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
-  if (hipError_t e = hipGetLastError()) return e;
-  hipLaunchKernelGGL((verify_draw<TYPE>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
-  return hipGetLastError();
+hipError_t launch_type(const shk_verify& a, hipStream_t s) {
+  // 16-byte loads where every row starts on 16 bytes
+  const uintptr_t size = TYPE == SHK_SRC_F32 ? 4 : 2;
+  uintptr_t all = reinterpret_cast<uintptr_t>(a.target) | size * (uintptr_t)(a.target_batch_stride | a.target_row_stride);
+  if (a.draft != nullptr)
+    all |= reinterpret_cast<uintptr_t>(a.draft) | size * (uintptr_t)(a.draft_batch_stride | a.draft_row_stride);
+  return all % 16 == 0 ? launch<TYPE, true>(a, s) : launch<TYPE, false>(a, s);
 }
 
 }  // namespace
 
-int64_t verify_workspace(const shk_verify& a) { return a.batch * pieces_of(a).count * (int64_t)sizeof(Sum); }
+int64_t verify_workspace(const shk_verify& a) {
+  return kept_bytes(a.batch) + a.batch * pieces_of(a).count * (int64_t)sizeof(Sum);
+}
 
 hipError_t launch_verify(const shk_verify& a, hipStream_t s) {
-  if (a.type == SHK_SRC_F32) return launch<SHK_SRC_F32>(a, s);
-  if (a.type == SHK_SRC_F16) return launch<SHK_SRC_F16>(a, s);
-  return launch<SHK_SRC_BF16>(a, s);
+  if (a.type == SHK_SRC_F32) return launch_type<SHK_SRC_F32>(a, s);
+  if (a.type == SHK_SRC_F16) return launch_type<SHK_SRC_F16>(a, s);
+  return launch_type<SHK_SRC_BF16>(a, s);
 }
 
 }  // namespace shk
