@@ -87,6 +87,9 @@ def decode_units() -> list[tuple[str, Path, list[str]]]:
         ("moe_nt", CSRC / "k_moe.hip", ["-DSHK_LAYOUT=1"]),
         ("capi_decode", CSRC / "capi_decode.hip", []),
         ("fp8", CSRC / "k_fp8.hip", []),
+        ("fp8big", CSRC / "k_fp8big.hip", []),
+        ("fp8wide", CSRC / "k_fp8wide.hip", []),
+        ("fp8few", CSRC / "k_fp8few.hip", []),
         ("fp8quant", CSRC / "k_fp8quant.hip", []),
         ("capi_fp8", CSRC / "capi_fp8.hip", []),
         ("rotate", CSRC / "k_rotate.hip", []),

@@ -14,34 +14,13 @@
 #include <algorithm>
 #include <cstdint>
 
-#include "shk_common.h"
-#include "shk_dma.h"
 #include "shk_fp8.h"
+#include "shk_fp8product.h"
+#include "shk_fp8wide.h"
 
 namespace shk {
 namespace {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-struct Product {
-  const uint8_t* a;
-  const uint8_t* b;
-  long a_pitch, b_pitch;
-  const float* sa;
-  const float* sb;
-  long sa_row, sa_block, sb_row, sb_block;  // elements
-  void* out;
-  long out_stride;
-  float* partial;   // [splits][m][n] where splits > 1
-  int m, n, k;
-  int tiles_m, tiles_n;
-  int splits, per_split;  // blocks of K
-  int out_type, b_shift;  // rows of b >> b_shift: its row of scales
-  int aligned;            // rows of out start on 16 bytes
-};
 
 template <int BM_, int BN_, int WM_, int WN_, int P_>
 struct Tile {
@@ -59,55 +38,17 @@ struct Tile {
   static_assert(BM % 16 == 0 && BN % 64 == 0 && P * STAGE <= 160 * 1024, "");
 };
 
-template <int KIND_A, int KIND_B>
-__device__ __forceinline__ v4f mfma128(const v8i& b, const v8i& a) {
-  // rows of the result are b's, columns a's
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, v4f{0.f, 0.f, 0.f, 0.f}, KIND_B, KIND_A, 0, 0, 0, 0);
-}
-
-// Eight codes of one operand as f16, which holds every one of them exactly.
-template <int KIND>
-__device__ __forceinline__ v8h widen(int lo, int hi) {
-  v2h h[4];
-  if constexpr (KIND == SHK_FP8_E4M3) {
-    h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
-    h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
-    h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
-    h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
-  } else {  // the upper bytes of f16
-    h[0] = __builtin_bit_cast(v2h, perm_b32(0u, lo, 0x010C000Cu));
-    h[1] = __builtin_bit_cast(v2h, perm_b32(0u, lo, 0x030C020Cu));
-    h[2] = __builtin_bit_cast(v2h, perm_b32(0u, hi, 0x010C000Cu));
-    h[3] = __builtin_bit_cast(v2h, perm_b32(0u, hi, 0x030C020Cu));
-  }
-  return v8h{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-}
-
-template <int KIND>
-struct Wide {
-  v8h part[4];
-  __device__ __forceinline__ explicit Wide(const v8i& f) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) part[i] = widen<KIND>(f[2 * i], f[2 * i + 1]);
-  }
-};
-
 __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-__device__ __forceinline__ void store_value(const Product& p, long at, float v) {
-  if (p.out_type == SHK_SRC_F32) static_cast<float*>(p.out)[at] = v;
-  else if (p.out_type == SHK_SRC_BF16) static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16_rne(v);
-  else static_cast<_Float16*>(p.out)[at] = (_Float16)v;
-}
-
 template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
-__global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Product p) {
+__global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Product p) {
   __shared__ __align__(16) uint8_t lds[T::P * T::STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = blockIdx.x;
-  const int m0 = tile % p.tiles_m * T::BM, n0 = tile / p.tiles_m * T::BN;
+  int tm, tn;
+  tile_of(p, 1024 / T::BM, tm, tn);
+  const int m0 = tm * T::BM, n0 = tn * T::BN;
   const int first = blockIdx.y * p.per_split;
   const int blocks = (p.k + 127) >> 7;
   const int count = min(p.per_split, blocks - first);
@@ -169,69 +110,92 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Product p
   const uint32_t sa_at = T::DATA + (wm * T::MT * 16 + row_in) * 4;
   const uint32_t sb_at = T::DATA + (T::SA + wn * T::NT * 16 + (BROW ? group * 4 : 0)) * 4;
 
-#pragma unroll
-  for (int s = 0; s < T::P - 1; ++s)
-    if (s < count) issue(first + s, s);
-  int slot = 0;
-  for (int i = 0; i < count; ++i) {
-    if (i + T::P - 2 < count) wait_vmcnt<(T::P - 2) * T::ISSUED>();
-    else wait_vmcnt<0>();
-    stage_barrier();
-    if (i + T::P - 1 < count) issue(first + i + T::P - 1, slot == 0 ? T::P - 1 : slot - 1);
-    uint8_t* st = lds + slot * T::STAGE;
-    const int left = p.k - (first + i) * 128;
-    if (left < 128) {  // K ends in this block: zeros behind it
-      for (int u = threadIdx.x; u < (T::BM + T::BN) * 8; u += T::THREADS) {
-        const int row = u >> 3, unit = (u & 7) ^ (row & 7), keep = left - unit * 16;
-        if (keep >= 16) continue;
-        uint32_t* w = reinterpret_cast<uint32_t*>(st + u * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int bytes = keep - 4 * e;
-          w[e] = bytes <= 0 ? 0u : bytes >= 4 ? w[e] : w[e] & ((1u << (8 * bytes)) - 1u);
-        }
-      }
-      stage_barrier();
-    }
+  struct Stage {
+    v8i a[T::MT], b[T::NT];
+    float sa[T::MT];
+    v4f sb[BROW ? T::NT : 1];
+  };
+  auto read = [&](int slot, Stage& f) {
+    const uint8_t* st = lds + slot * T::STAGE;
     auto fragment = [&](uint32_t at) {
-      const v4i lo = *reinterpret_cast<const v4i*>(st + at);
-      const v4i hi = *reinterpret_cast<const v4i*>(st + (at ^ 64u));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_shufflevector(*reinterpret_cast<const v4i*>(st + at), *reinterpret_cast<const v4i*>(st + (at ^ 64u)),
+                                     0, 1, 2, 3, 4, 5, 6, 7);
     };
-    v8i fb[T::NT];
 #pragma unroll
-    for (int j = 0; j < T::NT; ++j) fb[j] = fragment(b_at + j * 2048);
-    float sb = 0.f;
-    v4f sbv[T::NT];
-    if constexpr (BROW) {
-#pragma unroll
-      for (int j = 0; j < T::NT; ++j) sbv[j] = *reinterpret_cast<const v4f*>(st + sb_at + j * 64);
-    } else {
-      sb = *reinterpret_cast<const float*>(st + sb_at);
-    }
+    for (int j = 0; j < T::NT; ++j) f.b[j] = fragment(b_at + j * 2048);
 #pragma unroll
     for (int x = 0; x < T::MT; ++x) {
-      const v8i fa = fragment(a_at + x * 2048);
-      float s = *reinterpret_cast<const float*>(st + sa_at + x * 64);
-      if constexpr (!BROW) s *= sb;
+      f.a[x] = fragment(a_at + x * 2048);
+      f.sa[x] = *reinterpret_cast<const float*>(st + sa_at + x * 64);
+    }
+    if constexpr (BROW) {
+#pragma unroll
+      for (int j = 0; j < T::NT; ++j) f.sb[j] = *reinterpret_cast<const v4f*>(st + sb_at + j * 64);
+    } else {
+      f.sb[0][0] = *reinterpret_cast<const float*>(st + sb_at);
+    }
+  };
+  auto multiply = [&](const Stage& f) {
+#pragma unroll
+    for (int x = 0; x < T::MT; ++x) {
+      const float s = BROW ? f.sa[x] : f.sa[x] * f.sb[0][0];
 #pragma unroll
       for (int j = 0; j < T::NT; ++j) {
-        v4f t;
-        if constexpr (WIDE) {
-          const Wide<KIND_A> wa(fa);
-          const Wide<KIND_B> wb(fb[j]);
-          t = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb.part[i], wa.part[i], t, 0, 0, 0);
-        } else {
-          t = mfma128<KIND_A, KIND_B>(fb[j], fa);
-        }
+        const v4f t = product128<KIND_A, KIND_B, WIDE>(f.b[j], f.a[x]);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[x][j][r] = __builtin_fmaf(t[r], BROW ? s * sbv[j][r] : s, acc[x][j][r]);
+          acc[x][j][r] = __builtin_fmaf(t[r], BROW ? s * f.sb[j][r] : s, acc[x][j][r]);
       }
     }
-    slot = slot == T::P - 1 ? 0 : slot + 1;
+  };
+  // zeros behind K in its last stage
+  auto clear_tail = [&](int i, int slot) {
+    const int left = p.k - (first + i) * 128;
+    if (left >= 128) return;
+    uint8_t* st = lds + slot * T::STAGE;
+    for (int u = threadIdx.x; u < (T::BM + T::BN) * 8; u += T::THREADS) {
+      const int row = u >> 3, unit = (u & 7) ^ (row & 7), keep = left - unit * 16;
+      if (keep >= 16) continue;
+      uint32_t* w = reinterpret_cast<uint32_t*>(st + u * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int bytes = keep - 4 * e;
+        w[e] = bytes <= 0 ? 0u : bytes >= 4 ? w[e] : w[e] & ((1u << (8 * bytes)) - 1u);
+      }
+    }
+    stage_barrier();
+  };
+
+#pragma unroll
+  for (int s = 0; s < T::P; ++s)
+    if (s < count) issue(first + s, s);
+  if (count > 0) {
+    if (T::P <= count) wait_vmcnt<(T::P - 1) * T::ISSUED>();
+    else wait_vmcnt<0>();
+    stage_barrier();
+    clear_tail(0, 0);
+  }
+  // Stage i + 1 is read while stage i is multiplied.  The barrier of a stage says
+  // that stage i + 1 has come and that every wave has read stage i, whose slot
+  // then takes stage i + P.
+  Stage even, odd;
+  int slot = 0;
+  auto step = [&](int i, const Stage& now, Stage& next) {
+    if (i + 1 < count) {
+      if (i + T::P - 1 < count) wait_vmcnt<(T::P - 2) * T::ISSUED>();
+      else wait_vmcnt<0>();
+      stage_barrier();
+      if (i + T::P < count) issue(first + i + T::P, slot);
+      slot = slot == T::P - 1 ? 0 : slot + 1;
+      clear_tail(i + 1, slot);
+      read(slot, next);
+    }
+    multiply(now);
+  };
+  if (count > 0) read(0, even);
+  for (int i = 0; i < count; i += 2) {
+    step(i, even, odd);
+    if (i + 1 < count) step(i + 1, odd, even);
   }
 
 #pragma unroll
@@ -246,14 +210,13 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Product p
         for (int r = 0; r < 4; ++r)
           if (n + r < p.n) at[r] = acc[x][j][r];
       } else {
-        for (int r = 0; r < 4; ++r)
-          if (n + r < p.n) store_value(p, (long)m * p.out_stride + n + r, acc[x][j][r]);
+        store_four(p, m, n, acc[x][j]);
       }
     }
   }
 }
 
-__global__ __launch_bounds__(256) void fp8_join_kernel(const Product p) {
+__global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8Product p) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x, all = (long)p.m * p.n;
   if (i >= all) return;
   float v = 0.f;
@@ -267,8 +230,11 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* src, long 
   for (int c = blockIdx.x * 256 + threadIdx.x; c < k; c += gridDim.x * 256) dst[row * to + c] = src[row * pitch + c];
 }
 
+enum Kind { kFew, kTile64, kTile128, kBig, kWide };
+
 struct Plan {
-  int bm, bn, splits, per_split;
+  Kind kind;
+  int splits, per_split;
   bool copy_a, copy_b;
   long pitch;              // of the copies
   int64_t at_b, at_partial, bytes;
@@ -278,17 +244,37 @@ bool loose(const void* x, int64_t pitch, int64_t rows) {
   return reinterpret_cast<uintptr_t>(x) % 16 != 0 || (rows > 1 && pitch % 16 != 0);
 }
 
+// Which kernel takes a call, by what a stage (a block of K) costs each of them
+// with all CUs busy, measured: 64 x 64 tiles 0.62 us for 512 workgroups, 64 x 128
+// 0.95 us for 512, 256 x 256 1.45 us for 256.  f32 results: 64 x 64 0.8 to 0.95,
+// 128 x 128 1.4 for 256 workgroups and 2.2 for 512.
+//  * Up to 32 rows b is streamed past them: 16 x 11008 x 4096 in 11.7 us, by 64 x
+//    64 tiles in 18.  Up to 64 rows where 16 columns a workgroup leave each CU one:
+//    64 x 4096 x 4096 in 12.6 us (tiles: 15.9), but 64 x 11008 x 4096 in 20.3 (17.5).
+//  * One round of 64 x 64 tiles: 333 x 1408 x 2048 in 9.8 us, by 64 x 128 in 13.5;
+//    512 x 4096 x 4096 in 20.7 and 24.4.
+//  * Else the cheaper of the larger ones: 1024 x 4096 x 4096 in 30.5 by 64 x 128 and
+//    43 by 256 x 256, 4096 x 4096 x 4096 in 110 and 65.  f32: 128 x 128 from more
+//    than half a workgroup a CU on, 1024 x 4096 x 4096 in 49 us (64 x 64: 61).
+// K is cut where tiles leave half the CUs idle, into parts of at least 8 stages, so
+// that the join (about 4 us) is less than what it saves: 64 x 512 x 14336.
 Plan plan_of(const shk_fp8_mm& a) {
   Plan r{};
   const int blocks = (int)((a.k + 127) / 128);
-  if (a.m <= 16) r.bm = 16, r.bn = 64;
-  else if (a.m <= 32) r.bm = 32, r.bn = 64;
-  else if (a.m <= 64) r.bm = 64, r.bn = 64;
-  else if (((a.m + 255) / 256) * ((a.n + 255) / 256) >= 192) r.bm = 256, r.bn = 256;
-  else r.bm = 128, r.bn = 128;
-  const int64_t tiles = ((a.m + r.bm - 1) / r.bm) * ((a.n + r.bn - 1) / r.bn);
-  const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, tiles));
-  r.splits = (int)std::min<int64_t>(want, std::max(1, blocks / 4));
+  const bool wide = a.out_type == SHK_SRC_F32;
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
+  const int64_t small = tiles(64, 64);
+  if (a.m <= 32 || (a.m <= 64 && a.n <= 4096)) {
+    r.kind = kFew;
+  } else if (wide) {
+    r.kind = tiles(128, 128) > 128 ? kWide : kTile64;
+  } else if (small <= 512) {
+    r.kind = kTile64;
+  } else {
+    const double tile128 = 0.95 * ((tiles(64, 128) + 511) / 512), big = 1.45 * ((tiles(256, 256) + 255) / 256);
+    r.kind = big < tile128 ? kBig : kTile128;
+  }
+  r.splits = r.kind == kTile64 && small <= 128 ? (int)std::max<int64_t>(1, std::min<int64_t>(256 / small, blocks / 8)) : 1;
   r.per_split = std::max(1, (blocks + r.splits - 1) / r.splits);
   r.splits = std::max(1, (blocks + r.per_split - 1) / r.per_split);
   r.copy_a = loose(a.a, a.a_pitch, a.m), r.copy_b = loose(a.b, a.b_pitch, a.n);
@@ -300,23 +286,28 @@ Plan plan_of(const shk_fp8_mm& a) {
 }
 
 template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
-hipError_t launch(Product& p, hipStream_t s) {
+hipError_t launch(Fp8Product& p, hipStream_t s) {
   p.tiles_m = (p.m + T::BM - 1) / T::BM, p.tiles_n = (p.n + T::BN - 1) / T::BN;
   hipLaunchKernelGGL((fp8_product_kernel<T, KIND_A, KIND_B, BROW, WIDE>), dim3(p.tiles_m * p.tiles_n, p.splits),
                      dim3(T::THREADS), 0, s, p);
   return hipGetLastError();
 }
 
+// 64 x 64 tiles take f32 results too.
+typedef Tile<64, 64, 2, 2, 4> Tile64;
+typedef Tile<64, 128, 2, 2, 3> Tile128;
+
 template <class T, int KIND_A, int KIND_B>
-hipError_t launch_rows(Product& p, hipStream_t s) {
+hipError_t launch_rows(Fp8Product& p, hipStream_t s) {
   const bool rows = p.b_shift == 0;
-  if (p.out_type == SHK_SRC_F32)
-    return rows ? launch<T, KIND_A, KIND_B, true, true>(p, s) : launch<T, KIND_A, KIND_B, false, true>(p, s);
+  if constexpr (T::BN == 64)
+    if (p.out_type == SHK_SRC_F32)
+      return rows ? launch<T, KIND_A, KIND_B, true, true>(p, s) : launch<T, KIND_A, KIND_B, false, true>(p, s);
   return rows ? launch<T, KIND_A, KIND_B, true, false>(p, s) : launch<T, KIND_A, KIND_B, false, false>(p, s);
 }
 
 template <class T>
-hipError_t launch_kinds(Product& p, bool e5_a, bool e5_b, hipStream_t s) {
+hipError_t launch_kinds(Fp8Product& p, bool e5_a, bool e5_b, hipStream_t s) {
   if (e5_a) return e5_b ? launch_rows<T, 1, 1>(p, s) : launch_rows<T, 1, 0>(p, s);
   return e5_b ? launch_rows<T, 0, 1>(p, s) : launch_rows<T, 0, 0>(p, s);
 }
@@ -339,7 +330,7 @@ hipError_t launch_fp8_mm(const shk_fp8_mm& a, hipStream_t s) {
   if (a.m * a.n == 0) return hipSuccess;
   const Plan r = plan_of(a);
   uint8_t* work = static_cast<uint8_t*>(a.workspace);
-  Product p{};
+  Fp8Product p{};
   p.a = static_cast<const uint8_t*>(a.a), p.b = static_cast<const uint8_t*>(a.b);
   p.a_pitch = a.a_pitch, p.b_pitch = a.b_pitch;
   if (r.copy_a) {
@@ -359,12 +350,13 @@ hipError_t launch_fp8_mm(const shk_fp8_mm& a, hipStream_t s) {
   p.splits = r.splits, p.per_split = r.per_split;
   p.b_shift = a.b_rows == 128 ? 7 : 0;
   const bool e5_a = a.a_kind == SHK_FP8_E5M2, e5_b = a.b_kind == SHK_FP8_E5M2;
+  p.aligned = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (p.out_type == SHK_SRC_F32 ? 4 : 2))) % 16 == 0;
   hipError_t e;
-  if (r.bm == 16) e = launch_kinds<Tile<16, 64, 1, 4, 6>>(p, e5_a, e5_b, s);
-  else if (r.bm == 32) e = launch_kinds<Tile<32, 64, 1, 4, 6>>(p, e5_a, e5_b, s);
-  else if (r.bm == 64) e = launch_kinds<Tile<64, 64, 2, 2, 4>>(p, e5_a, e5_b, s);
-  else if (r.bm == 128) e = launch_kinds<Tile<128, 128, 2, 2, 2>>(p, e5_a, e5_b, s);
-  else e = launch_kinds<Tile<256, 256, 2, 4, 2>>(p, e5_a, e5_b, s);
+  if (r.kind == kFew) e = launch_fp8_few(p, e5_a, e5_b, s);
+  else if (r.kind == kTile64) e = launch_kinds<Tile64>(p, e5_a, e5_b, s);
+  else if (r.kind == kTile128) e = launch_kinds<Tile128>(p, e5_a, e5_b, s);
+  else if (r.kind == kBig) e = launch_fp8_big(p, e5_a, e5_b, s);
+  else e = launch_fp8_wide(p, e5_a, e5_b, s);
   if (e != hipSuccess || p.splits == 1) return e;
   hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)(((long)p.m * p.n + 255) / 256)), dim3(256), 0, s, p);
   return hipGetLastError();

@@ -1,0 +1,156 @@
+// 8-bit floating-point products with few rows of a (a decode step's tokens): b is
+// streamed from memory once.
+//
+// A workgroup holds 16 * NT columns of the result (rows of b) and all rows of a.
+// Its eight waves take K's blocks in turn, so that together they read runs of 1
+// KiB of each row of b, and nothing is shared while they do: a wave loads both
+// operands' fragments straight into registers, one block ahead, multiplies a block
+// with one MFMA for each 16 x 16 results, and folds it into its own f32 sums.
+// Behind the loop the eight sums are added in LDS, in order of the waves.
+// K is not cut over workgroups: 16 rows of b keep a CU's share of the memory rate
+// busy, and a sum over workgroups would be another launch.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "shk_fp8product.h"
+#include "shk_fp8wide.h"
+
+namespace shk {
+namespace {
+
+constexpr int kWaves = 8;
+
+// Units `group` and `group + 4` of a block of a row; what lies behind K is zero.
+__device__ __forceinline__ v8i load_block(const uint8_t* row, int kb, int group, int k) {
+  const uint8_t* at = row + (long)kb * 128 + 16 * group;
+  const int left = k - kb * 128 - 16 * group;  // values from `at` on
+  v4i lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
+  if (left >= 80) {
+    lo = *reinterpret_cast<const v4i*>(at);
+    hi = *reinterpret_cast<const v4i*>(at + 64);
+  } else {
+    // rows start on 16 bytes, so a unit that holds a value of the row lies in its pitch
+    if (left > 0) lo = *reinterpret_cast<const v4i*>(at);
+    if (left > 64) hi = *reinterpret_cast<const v4i*>(at + 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = left - 4 * e, m = n - 64;
+      lo[e] = n <= 0 ? 0 : n >= 4 ? lo[e] : lo[e] & ((1 << (8 * n)) - 1);
+      hi[e] = m <= 0 ? 0 : m >= 4 ? hi[e] : hi[e] & ((1 << (8 * m)) - 1);
+    }
+  }
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <int MT, int NT, int KIND_A, int KIND_B, bool BROW, bool WIDE>
+__global__ __launch_bounds__(64 * kWaves) void fp8_few_kernel(const Fp8Product p) {
+  __shared__ v4f sums[kWaves][MT * NT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row_in = lane & 15, group = lane >> 4, n0 = blockIdx.x * 16 * NT;
+  const int blocks = (p.k + 127) >> 7;
+  const uint8_t *a[MT], *b[NT];
+  const float* sa[MT];
+#pragma unroll
+  for (int x = 0; x < MT; ++x) {
+    const long m = min(x * 16 + row_in, p.m - 1);
+    a[x] = p.a + m * p.a_pitch, sa[x] = p.sa + m * p.sa_row;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) b[j] = p.b + (long)min(n0 + j * 16 + row_in, p.n - 1) * p.b_pitch;
+
+  struct Block {
+    v8i a[MT], b[NT];
+    float sa[MT];
+    float sb[NT][BROW ? 4 : 1];
+  };
+  auto load = [&](int kb, Block& f) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) f.b[j] = load_block(b[j], kb, group, p.k);
+#pragma unroll
+    for (int x = 0; x < MT; ++x) f.a[x] = load_block(a[x], kb, group, p.k), f.sa[x] = sa[x][kb * p.sa_block];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < (BROW ? 4 : 1); ++r) {
+        const int n = BROW ? min(n0 + j * 16 + group * 4 + r, p.n - 1) : min(n0 + j * 16, p.n - 1) >> 7;
+        f.sb[j][r] = p.sb[n * p.sb_row + kb * p.sb_block];
+      }
+  };
+  v4f acc[MT][NT];
+#pragma unroll
+  for (int x = 0; x < MT; ++x)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[x][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  Block next;
+  if (wave < blocks) load(wave, next);
+  for (int kb = wave; kb < blocks; kb += kWaves) {
+    const Block now = next;
+    if (kb + kWaves < blocks) load(kb + kWaves, next);
+#pragma unroll
+    for (int x = 0; x < MT; ++x)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const v4f t = product128<KIND_A, KIND_B, WIDE>(now.b[j], now.a[x]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[x][j][r] = __builtin_fmaf(t[r], now.sa[x] * now.sb[j][BROW ? r : 0], acc[x][j][r]);
+      }
+  }
+#pragma unroll
+  for (int x = 0; x < MT; ++x)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sums[wave][x * NT + j][lane] = acc[x][j];
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < MT * NT; t += kWaves) {
+    const int tile = t + wave;
+    if (tile >= MT * NT) continue;
+    v4f v = sums[0][tile][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += sums[w][tile][lane];
+    const int m = tile / NT * 16 + row_in, n = n0 + tile % NT * 16 + group * 4;
+    if (m < p.m) store_four(p, m, n, v);
+  }
+}
+
+template <int MT, int NT, int KIND_A, int KIND_B, bool WIDE>
+hipError_t launch(const Fp8Product& p, hipStream_t s) {
+  const dim3 grid((p.n + 16 * NT - 1) / (16 * NT)), group(64 * kWaves);
+  if (p.b_shift == 0) hipLaunchKernelGGL((fp8_few_kernel<MT, NT, KIND_A, KIND_B, true, WIDE>), grid, group, 0, s, p);
+  else hipLaunchKernelGGL((fp8_few_kernel<MT, NT, KIND_A, KIND_B, false, WIDE>), grid, group, 0, s, p);
+  return hipGetLastError();
+}
+
+template <int MT, int NT, int KIND_A, int KIND_B>
+hipError_t launch_wide(const Fp8Product& p, hipStream_t s) {
+  return p.out_type == SHK_SRC_F32 ? launch<MT, NT, KIND_A, KIND_B, true>(p, s) : launch<MT, NT, KIND_A, KIND_B, false>(p, s);
+}
+
+template <int MT, int NT>
+hipError_t launch_columns(const Fp8Product& p, bool e5_a, bool e5_b, hipStream_t s) {
+  if (e5_a) return e5_b ? launch_wide<MT, NT, 1, 1>(p, s) : launch_wide<MT, NT, 1, 0>(p, s);
+  return e5_b ? launch_wide<MT, NT, 0, 1>(p, s) : launch_wide<MT, NT, 0, 0>(p, s);
+}
+
+// As many columns a workgroup as leave each CU one, four times 16 at most: what a
+// CU can have on its way is limited (41 GB/s each, measured), and every workgroup
+// reads all of a.  16 x 11008 x 4096: 11.7 us with 48 columns (230 workgroups),
+// 16 with 16 or 32.
+template <int MT>
+hipError_t launch_rows(const Fp8Product& p, bool e5_a, bool e5_b, hipStream_t s) {
+  if (p.n <= 4096) return launch_columns<MT, 1>(p, e5_a, e5_b, s);
+  if (p.n <= 8192) return launch_columns<MT, 2>(p, e5_a, e5_b, s);
+  if (p.n <= 12288) return launch_columns<MT, 3>(p, e5_a, e5_b, s);
+  return launch_columns<MT, 4>(p, e5_a, e5_b, s);
+}
+
+}  // namespace
+
+hipError_t launch_fp8_few(Fp8Product& p, bool e5_a, bool e5_b, hipStream_t s) {
+  return p.m <= 16 ? launch_rows<1>(p, e5_a, e5_b, s) : p.m <= 32 ? launch_rows<2>(p, e5_a, e5_b, s)
+                                                                 : launch_columns<4, 1>(p, e5_a, e5_b, s);
+}
+
+}  // namespace shk

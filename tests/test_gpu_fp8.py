@@ -47,7 +47,8 @@ def _check(got, a, b, sa, sb):
 # every tile, its edges and its neighbours; K below, at and past a block
 SIZES = [(1, 1, 1), (1, 64, 128), (1, 4097, 640), (5, 100, 300), (16, 1000, 2048), (17, 130, 129), (32, 640, 1024),
          (33, 257, 127), (64, 512, 4096), (65, 128, 256), (128, 128, 128), (200, 333, 1000), (257, 500, 144),
-         (1, 7, 16384), (70, 1, 130)]
+         (1, 7, 16384), (70, 1, 130), (40, 5000, 300), (20, 5000, 200), (16, 9000, 260), (64, 13000, 130), (70, 90, 5000),
+         (100, 500, 4200)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -59,12 +60,45 @@ def test_product(device, m, n, k, b_rows):
     _check(got, a, b, sa, sb)
 
 
+# tiles of 64 x 128, of 256 x 256 (K of no whole block, one, an odd and an even
+# number, with and without an end), and the f32 results' own of 128 x 128
+LARGE = [(1000, 3000, 200), (2500, 2700, 100), (2600, 2560, 128), (2500, 2505, 384), (2304, 2568, 300),
+         (2400, 2512, 256), (4100, 1300, 777)]
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("b_rows", [1, 128])
-@pytest.mark.parametrize("m,n,k", [(3000, 4000, 400), (2700, 5000, 130), (4096, 4096, 256)])
-def test_large_tiles(device, m, n, k, b_rows):
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_tiles(device, m, n, k, b_rows, out_dtype):
+    """Rows and columns of every tile and its edges: sampled rows against the definition, and all
+    of them against the same rows multiplied few at a time."""
     a, b, sa, sb = _case(_gen("large", m, n, k, b_rows), m, n, k, b_rows)
-    got = shk.mm_fp8(a.to(device), b.to(device), a_scale=sa.to(device), b_scale=sb.to(device), out_dtype=F32)
-    _check(got, a, b, sa, sb)
+    dev = [t.to(device) for t in (a, b, sa, sb)]
+    got = shk.mm_fp8(*dev[:2], a_scale=dev[2], b_scale=dev[3], out_dtype=out_dtype)
+    rows = torch.unique(torch.cat((torch.arange(0, m, 97), torch.tensor([0, 15, 16, 63, 64, 127, 128, 255, 256, m - 1]))))
+    _check(got[rows.to(device)], a[rows], b, sa[rows], sb)
+    wide = [shk.mm_fp8(dev[0][i:i + 32], dev[1], a_scale=dev[2][i:i + 32], b_scale=dev[3], out_dtype=F32)
+            for i in range(0, m, 32)]
+    off = (got.double() - torch.cat(wide).double()).abs().amax(dim=1).cpu()
+    size = torch.cat(wide).double().abs().amax(dim=1).cpu()
+    assert bool((off <= 0.02 * size + 1e-6).all())  # a misplaced row or value would be off by its size
+
+
+def test_large_calls_repeat_their_bits(device):
+    a, b, sa, sb = (t.to(device) for t in _case(_gen("overlap"), 2500, 2510, 640))
+    first = shk.mm_fp8(a, b, a_scale=sa, b_scale=sb)
+    for _ in range(3):
+        assert torch.equal(shk.mm_fp8(a, b, a_scale=sa, b_scale=sb), first)
+
+
+@pytest.mark.parametrize("a_kind,b_kind", [(E4M3, E5M2), (E5M2, E4M3), (E5M2, E5M2)])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(1000, 3000, 200), (2500, 2700, 300)])
+def test_large_types(device, m, n, k, out_dtype, a_kind, b_kind):
+    a, b, sa, sb = _case(_gen("large types", m, out_dtype, a_kind, b_kind), m, n, k, 128, a_kind, b_kind)
+    got = shk.mm_fp8(a.to(device), b.to(device), a_scale=sa.to(device), b_scale=sb.to(device), out_dtype=out_dtype)
+    rows = torch.arange(0, m, 61)
+    _check(got[rows.to(device)], a[rows], b, sa[rows], sb)
 
 
 @pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
