@@ -40,6 +40,10 @@ from .native import (
 
 FP8_BLOCK = 128
 
+# bytes of workspace by what they follow from: sizes, the result's type, and
+# whether the operands' rows start on 16 bytes
+_WORKSPACES: dict[tuple, int] = {}
+
 # the structs of include/strix_halo_gfx950.h: every field is 8 bytes
 _QUANTIZE = struct.Struct("=13q")
 _MM = struct.Struct("=21q")
@@ -105,7 +109,7 @@ def quantize_fp8(x: Any, *, block_rows: int = 1, transpose: bool = False, dtype:
             index, _current_stream(torch, index),
             _QUANTIZE.pack(x.data_ptr(), source, x.shape[0], x.shape[1], stride, turn, block_rows, kind,
                            codes.data_ptr(), pitch, scales.data_ptr(), 1, scales.shape[1])))
-    codes, scales = codes[:, :cols], scales.t()
+    codes, scales = codes if pitch == cols else codes[:, :cols], scales.t()
     if given.requires_grad:
         scales = _no_gradient(torch, "quantize_fp8", scales, given)
     return codes, scales
@@ -166,21 +170,26 @@ def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None,
             raise ValueError(f"out must have shape {(m, n)} and contiguous rows; got {tuple(out.shape)}")
     if m and n:
         a_pitch, b_pitch = a.stride(0) if m > 1 else k, b.stride(0) if n > 1 else k
-
-        def args(work: Any, nbytes: int) -> bytes:
-            return _MM.pack(a.data_ptr(), a_pitch, a_kind, b.data_ptr(), b_pitch, b_kind, a_scale.data_ptr(),
-                            *a_scale.stride(), b_scale.data_ptr(), *b_scale.stride(), b_rows, m, n, k, out.data_ptr(),
-                            out.stride(0) if m > 1 else n, out_type, work.data_ptr() if nbytes else 0, nbytes)
-
+        a_at, b_at = a.data_ptr(), b.data_ptr()
         lib = _verified_library()
-        packed = args(None, 0)
-        nbytes = lib.amd_strix_halo_kernels_fp8_mm_workspace(packed)
-        if nbytes < 0:
-            _check(lib, 1)
-        if nbytes:
-            work = a.new_empty(nbytes, dtype=torch.uint8)
-            packed = args(work, nbytes)
-        _check(lib, lib.amd_strix_halo_kernels_fp8_mm(index, _current_stream(torch, index), packed))
+
+        def args(at: int, nbytes: int) -> bytes:
+            return _MM.pack(a_at, a_pitch, a_kind, b_at, b_pitch, b_kind, a_scale.data_ptr(), *a_scale.stride(),
+                            b_scale.data_ptr(), *b_scale.stride(), b_rows, m, n, k, out.data_ptr(),
+                            out.stride(0) if m > 1 else n, out_type, at, nbytes)
+
+        key = (m, n, k, out_type, (a_at | (a_pitch if m > 1 else 0)) % 16 == 0,
+               (b_at | (b_pitch if n > 1 else 0)) % 16 == 0)
+        nbytes = _WORKSPACES.get(key)
+        if nbytes is None:
+            nbytes = lib.amd_strix_halo_kernels_fp8_mm_workspace(args(0, 0))
+            if nbytes < 0:
+                _check(lib, 1)
+            if len(_WORKSPACES) < 4096:
+                _WORKSPACES[key] = nbytes
+        work = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _check(lib, lib.amd_strix_halo_kernels_fp8_mm(index, _current_stream(torch, index),
+                                                      args(work.data_ptr() if nbytes else 0, nbytes)))
     if a_scale.requires_grad or b_scale.requires_grad:
         return _no_gradient(torch, "mm_fp8", out, a_scale, b_scale)
     return out

@@ -21,6 +21,8 @@ MOST_DRAFTS = 63
 # shk_verify of include/strix_halo_gfx950.h: every field is 8 bytes
 _VERIFY = struct.Struct("=19q")
 
+_WORKSPACES: dict[tuple, int] = {}  # bytes, by batch and vocabulary
+
 
 def verify_draft(
     target: Any,
@@ -96,16 +98,21 @@ def verify_draft(
     out = torch.empty((batch, drafts + 1), dtype=torch.int64, device=target.device)
     kept = torch.empty(batch, dtype=torch.int32, device=target.device)
     if batch:
-        def args(work: Any, nbytes: int) -> bytes:
+        def args(at: int, nbytes: int) -> bytes:
             return _VERIFY.pack(target.data_ptr(), target.stride(0), target.stride(1), *d_at, kind, batch, drafts,
                                 vocab, tokens.data_ptr(), tokens.element_size(), uniforms.data_ptr(),
                                 0 if counts is None else counts.data_ptr(), out.data_ptr(), kept.data_ptr(),
-                                0 if lengths is None else lengths.data_ptr(), work.data_ptr() if nbytes else 0, nbytes)
+                                0 if lengths is None else lengths.data_ptr(), at, nbytes)
 
         lib = _verified_library()
-        nbytes = lib.amd_strix_halo_kernels_verify_workspace(args(None, 0))
-        if nbytes < 0:
-            _check(lib, 1)
+        nbytes = _WORKSPACES.get((batch, vocab))
+        if nbytes is None:
+            nbytes = lib.amd_strix_halo_kernels_verify_workspace(args(0, 0))
+            if nbytes < 0:
+                _check(lib, 1)
+            if len(_WORKSPACES) < 4096:
+                _WORKSPACES[batch, vocab] = nbytes
         work = torch.empty(nbytes, dtype=torch.uint8, device=target.device)
-        _check(lib, lib.amd_strix_halo_kernels_verify(index, _current_stream(torch, index), args(work, nbytes)))
+        _check(lib, lib.amd_strix_halo_kernels_verify(index, _current_stream(torch, index),
+                                                      args(work.data_ptr(), nbytes)))
     return out, kept

@@ -15,6 +15,7 @@
 
 #include "shk_common.h"
 #include "shk_kvrows.h"
+#include "shk_loads.h"
 #include "shk_step.h"
 
 namespace shk {
@@ -30,6 +31,8 @@ struct Rotate {
   const double* turns;
   float amplitude, eps;
   unsigned rows, per_token;  // per_token: heads + kv_heads, and kv_heads more with a cache
+  unsigned inverse[2];       // floor(2^64 / per_token) + 1, low half first
+  float per_dim;             // 1 / dim
   unsigned heads, kv_heads;
   int dim, half, rotated;
   int position8, weight_type;
@@ -95,18 +98,53 @@ __device__ __forceinline__ Shared shared_parts(float* lds, const Rotate& p, unsi
   return Shared{lds, lds + tokens * p.half, lds + 2 * tokens * p.half};
 }
 
-__device__ __forceinline__ void fill_shared(const Shared& s, const Rotate& p, unsigned token0, unsigned tokens) {
-  for (unsigned i = threadIdx.x; i < tokens * p.half; i += 256) {
-    const unsigned t = i / p.half;
-    const long at = token0 + t;
-    const double position = p.position8 ? (double)static_cast<const int64_t*>(p.positions)[at]
-                                        : (double)static_cast<const int32_t*>(p.positions)[at];
-    const float2 cs = turned(position * p.turns[i - t * p.half]);
+// What a thread brings to them: asked for before the rows, since loads return in
+// order, and worked out while the rows are on their way.  `angle` and `weight`:
+// those that it begins with, of every 256.
+struct Asked {
+  double position, turns;
+  float weight;
+  int angles, angle, weights;  // numbers of angles and weights, and the first angle
+};
+
+__device__ __forceinline__ double position_of(const Rotate& p, long token) {
+  return p.position8 ? (double)static_cast<const int64_t*>(p.positions)[token]
+                     : (double)static_cast<const int32_t*>(p.positions)[token];
+}
+
+__device__ __forceinline__ Asked ask_shared(const Rotate& p, unsigned token0, unsigned tokens) {
+  Asked r{0.0, 0.0, 0.f, (int)tokens * p.half, (int)threadIdx.x, p.weight[0] != nullptr ? 2 * p.dim : 0};
+  if (r.angle < r.angles) {
+    const int t = r.angle / p.half;
+    r.position = position_of(p, (long)token0 + t);
+    r.turns = p.turns[r.angle - t * p.half];
+  }
+  if ((int)threadIdx.x < r.weights) r.weight = weight_of(p, (int)threadIdx.x >= p.dim, (int)threadIdx.x % p.dim);
+  return r;
+}
+
+__device__ __forceinline__ void fill_shared(const Shared& s, const Rotate& p, unsigned token0, const Asked& r) {
+  for (int i = r.angle; i < r.angles; i += 256) {
+    double angle = r.position * r.turns;
+    if (i != r.angle) {
+      const int t = i / p.half;
+      angle = position_of(p, (long)token0 + t) * p.turns[i - t * p.half];
+    }
+    const float2 cs = turned(angle);
     s.cosines[i] = cs.x * p.amplitude, s.sines[i] = cs.y * p.amplitude;
   }
-  if (p.weight[0] != nullptr)
-    for (int i = threadIdx.x; i < 2 * p.dim; i += 256)
-      s.weights[i] = i < p.dim ? weight_of(p, 0, i) : weight_of(p, 1, i - p.dim);
+  for (int i = threadIdx.x; i < r.weights; i += 256)
+    s.weights[i] = i < 256 ? r.weight : weight_of(p, i >= p.dim, i >= p.dim ? i - p.dim : i);
+}
+
+// row / per_token, the upper half of row * inverse: exact for every 32-bit row.
+__device__ __forceinline__ unsigned token_of(const Rotate& p, unsigned row) {
+  return (unsigned)(((unsigned long long)row * p.inverse[1] + __umulhi(row, p.inverse[0])) >> 32);
+}
+
+// 1 / sqrt(mean + eps), to 2^-23.
+__device__ __forceinline__ float norm_of(const Rotate& p, float sum) {
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(sum, p.per_dim, p.eps));
 }
 
 // A row of one round: which head of which token.
@@ -117,7 +155,7 @@ struct Place {
 
 __device__ __forceinline__ Place place_of(const Rotate& p, unsigned row, bool inside) {
   Place r;
-  r.token = row / p.per_token;
+  r.token = token_of(p, row);
   const unsigned h = row - r.token * p.per_token;
   r.kind = row >= p.rows || !inside ? -1 : h < p.heads ? 0 : h < p.heads + p.kv_heads ? 1 : 2;
   r.head = r.kind == 0 ? h : r.kind == 1 ? h - p.heads : h - p.heads - p.kv_heads;
@@ -165,6 +203,13 @@ __device__ __forceinline__ void read8(const float* from, float (&v)[8]) {
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+// PAST: past the caches, for more than they hold until it is read again.
+template <bool PAST>
+__device__ __forceinline__ void store16(uint8_t* to, u4 v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<u4*>(to));
+  else *reinterpret_cast<u4*>(to) = v;
+}
+
 // Rows on 16 bytes whose values, turning ones and (APART) half of them are whole
 // 8s: a lane turns with all its values or none, and its partners are one load.
 template <int TYPE, int LANES, bool APART, int ROUNDS>
@@ -175,6 +220,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
   const unsigned start = blockIdx.x * (PER * ROUNDS), mine = start + threadIdx.x / LANES;
   const bool inside = first < p.dim, turning = first < p.rotated, low = first < p.half;
   const int partner = APART ? (low ? first + p.half : first - p.half) : 0;
+  const unsigned last = min(start + PER * ROUNDS, p.rows) - 1, token0 = token_of(p, start);
+  const unsigned tokens = token_of(p, last) - token0 + 1;
+  const Asked asked = ask_shared(p, token0, tokens);
   Place place[ROUNDS];
   float v[ROUNDS][8], w[APART ? ROUNDS : 1][8];
 #pragma unroll
@@ -190,10 +238,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
     if constexpr (APART)
       if (r.kind < 2 && turning) load8<TYPE, true>(x + partner * kSize<TYPE>, w[i]);
   }
-  const unsigned last = min(start + PER * ROUNDS, p.rows) - 1, token0 = start / p.per_token;
-  const unsigned tokens = last / p.per_token - token0 + 1;
   const Shared s = shared_parts(lds, p, tokens);
-  fill_shared(s, p, token0, tokens);
+  fill_shared(s, p, token0, asked);
   __syncthreads();
   const bool norm = p.weight[0] != nullptr;
 #pragma unroll
@@ -207,7 +253,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
       for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[i][e], v[i][e], sum);
 #pragma unroll
       for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d, 64);
-      scale = 1.f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
+      scale = norm_of(p, sum);
       if (head) {
         float weight[8];
         read8(s.weights + (r.kind == 1 ? p.dim : 0) + first, weight);
@@ -252,11 +298,13 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
       uint8_t* out = p.out[r.kind] + ((long)r.token * p.out_token_stride[r.kind] +
                                       (long)r.head * p.out_head_stride[r.kind] + first) * kSize<TYPE>;
       if constexpr (TYPE == SHK_SRC_F32) {
-        reinterpret_cast<float4*>(out)[0] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
-        reinterpret_cast<float4*>(out)[1] = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          store16<(ROUNDS > 1)>(out + 16 * e, u4{__float_as_uint(v[i][4 * e]), __float_as_uint(v[i][4 * e + 1]),
+                                                 __float_as_uint(v[i][4 * e + 2]), __float_as_uint(v[i][4 * e + 3])});
       } else {
-        *reinterpret_cast<uint4*>(out) = make_uint4(pack2<TYPE>(v[i][0], v[i][1]), pack2<TYPE>(v[i][2], v[i][3]),
-                                                    pack2<TYPE>(v[i][4], v[i][5]), pack2<TYPE>(v[i][6], v[i][7]));
+        store16<(ROUNDS > 1)>(out, u4{pack2<TYPE>(v[i][0], v[i][1]), pack2<TYPE>(v[i][2], v[i][3]),
+                                      pack2<TYPE>(v[i][4], v[i][5]), pack2<TYPE>(v[i][6], v[i][7])});
       }
     }
   }
@@ -282,10 +330,10 @@ __global__ __launch_bounds__(256) void rotate_any_kernel(const Rotate p) {
       if (APART && head && at < p.rotated) w[e] = element<TYPE>(x, at < p.half ? at + p.half : at - p.half);
     }
   }
-  const unsigned last = min(start + PER, p.rows) - 1, token0 = start / p.per_token;
-  const unsigned tokens = last / p.per_token - token0 + 1;
+  const unsigned last = min(start + PER, p.rows) - 1, token0 = token_of(p, start);
+  const unsigned tokens = token_of(p, last) - token0 + 1;
   const Shared s = shared_parts(lds, p, tokens);
-  fill_shared(s, p, token0, tokens);
+  fill_shared(s, p, token0, ask_shared(p, token0, tokens));
   __syncthreads();
   float scale = 1.f;
   if (norm) {
@@ -294,7 +342,7 @@ __global__ __launch_bounds__(256) void rotate_any_kernel(const Rotate p) {
     for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
 #pragma unroll
     for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d, 64);
-    scale = 1.f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
+    scale = norm_of(p, sum);
   }
   if (head) {
     const float* weight = s.weights + (r.kind == 1 ? p.dim : 0);
@@ -354,8 +402,10 @@ hipError_t launch_pairs(const Rotate& p, bool vec, hipStream_t s) {
                        shared_bytes(p, PER), s, p);
     return hipGetLastError();
   }
-  // one round while that leaves CUs idle, else four, whose loads go out together
-  return p.rows <= 256 * PER * 4 ? launch<TYPE, LANES, APART, 1>(p, s) : launch<TYPE, LANES, APART, 4>(p, s);
+  // one round while that leaves CUs idle, else two, whose loads go out together
+  // (8191 tokens of 40 heads of 128: 51 us with two, 55 with one, 60 with four,
+  // whose registers halve the waves; 43 with stores past the caches)
+  return p.rows <= 256 * PER * 4 ? launch<TYPE, LANES, APART, 1>(p, s) : launch<TYPE, LANES, APART, 2>(p, s);
 }
 
 template <int TYPE, int LANES>
@@ -389,6 +439,9 @@ hipError_t launch_rotate(const shk_kv_cache* c, const shk_rotate& a, hipStream_t
   p.heads = (unsigned)a.heads, p.kv_heads = (unsigned)a.kv_heads;
   p.per_token = p.heads + p.kv_heads * (c != nullptr ? 2 : 1);
   p.rows = (unsigned)a.tokens * p.per_token;
+  const unsigned long long inverse = ~0ULL / p.per_token + 1;  // per_token is 2 or more, 2^64 - 1 divides alike
+  p.inverse[0] = (unsigned)inverse, p.inverse[1] = (unsigned)(inverse >> 32);
+  p.per_dim = 1.f / (float)a.head_dim;
   p.dim = (int)a.head_dim, p.rotated = (int)a.rotated, p.half = p.rotated / 2;
   uintptr_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
                   reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_out) |
