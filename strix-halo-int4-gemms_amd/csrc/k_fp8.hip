@@ -224,10 +224,22 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8Product p) {
   store_value(p, i / p.n * p.out_stride + i % p.n, v);
 }
 
-// Rows to a pitch of whole 16 bytes.
-__global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* src, long pitch, int k, uint8_t* dst, long to) {
-  const long row = blockIdx.y + (long)blockIdx.z * 65535;
-  for (int c = blockIdx.x * 256 + threadIdx.x; c < k; c += gridDim.x * 256) dst[row * to + c] = src[row * pitch + c];
+// Rows to a pitch of whole 16 bytes, a piece of 16 a thread.
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* src, long pitch, int k, uint8_t* dst, long to, long pieces) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= pieces) return;
+  const long each = to / 16, row = i / each;
+  const int c = (int)(i - row * each) * 16;
+  const uint8_t* from = src + row * pitch + c;
+  u4 v{0, 0, 0, 0};
+  if (c + 16 <= k) {
+    v = *reinterpret_cast<const any_u4*>(from);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (c + e < k) v[e / 4] |= (uint32_t)from[e] << (8 * (e % 4));
+  }
+  *reinterpret_cast<u4*>(dst + row * to + c) = v;
 }
 
 enum Kind { kFew, kTile64, kTile128, kBig, kWide };
@@ -277,7 +289,8 @@ Plan plan_of(const shk_fp8_mm& a) {
   r.splits = r.kind == kTile64 && small <= 128 ? (int)std::max<int64_t>(1, std::min<int64_t>(256 / small, blocks / 8)) : 1;
   r.per_split = std::max(1, (blocks + r.splits - 1) / r.splits);
   r.splits = std::max(1, (blocks + r.per_split - 1) / r.per_split);
-  r.copy_a = loose(a.a, a.a_pitch, a.m), r.copy_b = loose(a.b, a.b_pitch, a.n);
+  // the copies to LDS are of whole 16 bytes; loads to registers are not
+  r.copy_a = r.kind != kFew && loose(a.a, a.a_pitch, a.m), r.copy_b = r.kind != kFew && loose(a.b, a.b_pitch, a.n);
   r.pitch = (a.k + 15) & ~15L;
   r.at_b = r.copy_a ? a.m * r.pitch : 0;
   r.at_partial = r.at_b + (r.copy_b ? a.n * r.pitch : 0);
@@ -313,13 +326,10 @@ hipError_t launch_kinds(Fp8Product& p, bool e5_a, bool e5_b, hipStream_t s) {
 }
 
 hipError_t copy_rows(const void* src, long pitch, long rows, int k, uint8_t* dst, long to, hipStream_t s) {
-  for (long done = 0; done < rows; done += 65535) {
-    const long part = std::min(65535L, rows - done);
-    hipLaunchKernelGGL(fp8_rows_kernel, dim3((unsigned)std::min(64, (k + 255) / 256), (unsigned)part), dim3(256), 0, s,
-                       static_cast<const uint8_t*>(src) + done * pitch, pitch, k, dst + done * to, to);
-    if (hipError_t e = hipGetLastError()) return e;
-  }
-  return hipSuccess;
+  const long pieces = rows * (to / 16);
+  hipLaunchKernelGGL(fp8_rows_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s,
+                     static_cast<const uint8_t*>(src), pitch, k, dst, to, pieces);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -350,7 +360,6 @@ hipError_t launch_fp8_mm(const shk_fp8_mm& a, hipStream_t s) {
   p.splits = r.splits, p.per_split = r.per_split;
   p.b_shift = a.b_rows == 128 ? 7 : 0;
   const bool e5_a = a.a_kind == SHK_FP8_E5M2, e5_b = a.b_kind == SHK_FP8_E5M2;
-  p.aligned = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (p.out_type == SHK_SRC_F32 ? 4 : 2))) % 16 == 0;
   hipError_t e;
   if (r.kind == kFew) e = launch_fp8_few(p, e5_a, e5_b, s);
   else if (r.kind == kTile64) e = launch_kinds<Tile64>(p, e5_a, e5_b, s);

@@ -224,16 +224,15 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     const int r = k * 8 + lane / 8, u = lane & 7, m = m0 + wm * 128 + r, n = n0 + wn * 64 + u * 8;
-    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * 128 + 16 * (u ^ (r & 7)));
+    const u4 v = *reinterpret_cast<const u4*>(mine + r * 128 + 16 * (u ^ (r & 7)));
     if (m >= p.m) continue;
     uint16_t* at = static_cast<uint16_t*>(p.out) + (long)m * p.out_stride + n;
-    if (p.aligned && n + 8 <= p.n) {
-      *reinterpret_cast<uint4*>(at) = v;
+    if (n + 8 <= p.n) {
+      *reinterpret_cast<any_u4*>(at) = v;  // of any alignment, as store_four's
     } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (n + e < p.n) at[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+        if (n + e < p.n) at[e] = (uint16_t)(v[e / 2] >> (16 * (e % 2)));
     }
   }
 }

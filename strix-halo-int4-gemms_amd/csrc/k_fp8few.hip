@@ -22,26 +22,29 @@ namespace {
 
 constexpr int kWaves = 8;
 
-// Units `group` and `group + 4` of a block of a row; what lies behind K is zero.
-__device__ __forceinline__ v8i load_block(const uint8_t* row, int kb, int group, int k) {
-  const uint8_t* at = row + (long)kb * 128 + 16 * group;
-  const int left = k - kb * 128 - 16 * group;  // values from `at` on
-  v4i lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
-  if (left >= 80) {
-    lo = *reinterpret_cast<const v4i*>(at);
-    hi = *reinterpret_cast<const v4i*>(at + 64);
-  } else {
-    // rows start on 16 bytes, so a unit that holds a value of the row lies in its pitch
-    if (left > 0) lo = *reinterpret_cast<const v4i*>(at);
-    if (left > 64) hi = *reinterpret_cast<const v4i*>(at + 64);
+// Units `group` and `group + 4` of a block of a row.
+__device__ __forceinline__ v8i load_block(const uint8_t* at) {
+  return __builtin_shufflevector(__builtin_bit_cast(v4i, *reinterpret_cast<const any_u4*>(at)),
+                                 __builtin_bit_cast(v4i, *reinterpret_cast<const any_u4*>(at + 64)), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The same where `left` bytes of the row are left from `at` on; zeros behind them.
+__device__ __forceinline__ v8i load_end(const uint8_t* at, int left) {
+  v8i v{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = left - 4 * e, m = n - 64;
-      lo[e] = n <= 0 ? 0 : n >= 4 ? lo[e] : lo[e] & ((1 << (8 * n)) - 1);
-      hi[e] = m <= 0 ? 0 : m >= 4 ? hi[e] : hi[e] & ((1 << (8 * m)) - 1);
+  for (int h = 0; h < 2; ++h, left -= 64, at += 64) {
+    if (left >= 16) {
+      const u4 u = *reinterpret_cast<const any_u4*>(at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * h + e] = (int)u[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll 1
+        for (int byte = 0; byte < min(4, left - 4 * e); ++byte) v[4 * h + e] |= (int)at[4 * e + byte] << (8 * byte);
     }
   }
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return v;
 }
 
 template <int MT, int NT, int KIND_A, int KIND_B, bool BROW, bool WIDE>
@@ -49,27 +52,25 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_few_kernel(const Fp8Product p
   __shared__ v4f sums[kWaves][MT * NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row_in = lane & 15, group = lane >> 4, n0 = blockIdx.x * 16 * NT;
-  const int blocks = (p.k + 127) >> 7;
+  const int whole = p.k >> 7, left = (p.k & 127) - 16 * group;  // left: of the last block, from this lane's bytes on
   const uint8_t *a[MT], *b[NT];
   const float* sa[MT];
 #pragma unroll
   for (int x = 0; x < MT; ++x) {
     const long m = min(x * 16 + row_in, p.m - 1);
-    a[x] = p.a + m * p.a_pitch, sa[x] = p.sa + m * p.sa_row;
+    a[x] = p.a + m * p.a_pitch + 16 * group, sa[x] = p.sa + m * p.sa_row;
   }
 #pragma unroll
-  for (int j = 0; j < NT; ++j) b[j] = p.b + (long)min(n0 + j * 16 + row_in, p.n - 1) * p.b_pitch;
+  for (int j = 0; j < NT; ++j) b[j] = p.b + (long)min(n0 + j * 16 + row_in, p.n - 1) * p.b_pitch + 16 * group;
 
   struct Block {
     v8i a[MT], b[NT];
     float sa[MT];
     float sb[NT][BROW ? 4 : 1];
   };
-  auto load = [&](int kb, Block& f) {
+  auto load_scales = [&](int kb, Block& f) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) f.b[j] = load_block(b[j], kb, group, p.k);
-#pragma unroll
-    for (int x = 0; x < MT; ++x) f.a[x] = load_block(a[x], kb, group, p.k), f.sa[x] = sa[x][kb * p.sa_block];
+    for (int x = 0; x < MT; ++x) f.sa[x] = sa[x][kb * p.sa_block];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -78,25 +79,43 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_few_kernel(const Fp8Product p
         f.sb[j][r] = p.sb[n * p.sb_row + kb * p.sb_block];
       }
   };
+  auto load = [&](int kb, Block& f) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) f.b[j] = load_block(b[j] + kb * 128);
+#pragma unroll
+    for (int x = 0; x < MT; ++x) f.a[x] = load_block(a[x] + kb * 128);
+    load_scales(kb, f);
+  };
   v4f acc[MT][NT];
 #pragma unroll
   for (int x = 0; x < MT; ++x)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[x][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  Block next;
-  if (wave < blocks) load(wave, next);
-  for (int kb = wave; kb < blocks; kb += kWaves) {
-    const Block now = next;
-    if (kb + kWaves < blocks) load(kb + kWaves, next);
+  auto multiply = [&](const Block& f) {
 #pragma unroll
     for (int x = 0; x < MT; ++x)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const v4f t = product128<KIND_A, KIND_B, WIDE>(now.b[j], now.a[x]);
+        const v4f t = product128<KIND_A, KIND_B, WIDE>(f.b[j], f.a[x]);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[x][j][r] = __builtin_fmaf(t[r], now.sa[x] * now.sb[j][BROW ? r : 0], acc[x][j][r]);
+          acc[x][j][r] = __builtin_fmaf(t[r], f.sa[x] * f.sb[j][BROW ? r : 0], acc[x][j][r]);
       }
+  };
+  Block next;
+  if (wave < whole) load(wave, next);
+  for (int kb = wave; kb < whole; kb += kWaves) {
+    const Block now = next;
+    if (kb + kWaves < whole) load(kb + kWaves, next);
+    multiply(now);
+  }
+  if ((p.k & 127) != 0 && whole % kWaves == wave) {  // K ends in a block
+#pragma unroll
+    for (int j = 0; j < NT; ++j) next.b[j] = load_end(b[j] + whole * 128, left);
+#pragma unroll
+    for (int x = 0; x < MT; ++x) next.a[x] = load_end(a[x] + whole * 128, left);
+    load_scales(whole, next);
+    multiply(next);
   }
 #pragma unroll
   for (int x = 0; x < MT; ++x)

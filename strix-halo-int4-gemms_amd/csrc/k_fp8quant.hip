@@ -16,6 +16,7 @@
 
 #include "shk_common.h"
 #include "shk_fp8.h"
+#include "shk_loads.h"
 
 namespace shk {
 namespace {
@@ -39,23 +40,21 @@ __device__ __forceinline__ float value_of(const uint8_t* x, long i) {
   return TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
-// x[at .. at + 8); `count` of them lie inside.  VEC: on 16 bytes if all do.
-template <int TYPE, bool VEC>
+// x[at .. at + 8); `count` of them lie inside.  Whole ones come in vectors, of any
+// alignment.
+template <int TYPE>
 __device__ __forceinline__ void load8(const uint8_t* x, long at, long count, float (&v)[8]) {
-  if (VEC && count >= 8) {
-    const uint4* src = reinterpret_cast<const uint4*>(x + at * kSize<TYPE>);
-    uint32_t u[kSize<TYPE> * 2];
+  if (count >= 8) {
+    const any_u4* src = reinterpret_cast<const any_u4*>(x + at * kSize<TYPE>);
+    u4 u[kSize<TYPE> / 2];
 #pragma unroll
-    for (int i = 0; i < kSize<TYPE> / 2; ++i) {
-      const uint4 w = src[i];
-      u[4 * i] = w.x, u[4 * i + 1] = w.y, u[4 * i + 2] = w.z, u[4 * i + 3] = w.w;
-    }
+    for (int i = 0; i < kSize<TYPE> / 2; ++i) u[i] = src[i];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (TYPE == SHK_SRC_F32) {
-        v[e] = __uint_as_float(u[e]);
+        v[e] = __uint_as_float(u[e / 4][e % 4]);
       } else {
-        const uint16_t h = (uint16_t)(u[e / 2] >> (16 * (e % 2)));
+        const uint16_t h = (uint16_t)(u[0][e / 2] >> (16 * (e % 2)));
         v[e] = TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
       }
     }
@@ -108,11 +107,10 @@ __device__ __forceinline__ void codes8(const float (&v)[8], float s, float inv, 
 
 __device__ __forceinline__ bool normal_scale(float s) { return s > 0x1p-60f && s < 0x1p60f; }
 
-// `count` of 8 bytes; VEC: on 8 bytes.
-template <bool VEC>
+// The first `count` of 8 bytes.
 __device__ __forceinline__ void store8(uint8_t* to, const uint32_t (&w)[2], long count) {
-  if (VEC && count >= 8) {
-    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+  if (count >= 8) {
+    *reinterpret_cast<any_u2*>(to) = u2{w[0], w[1]};
     return;
   }
 #pragma unroll
@@ -120,7 +118,7 @@ __device__ __forceinline__ void store8(uint8_t* to, const uint32_t (&w)[2], long
     if (e < count) to[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
 }
 
-template <int TYPE, int KIND, bool VEC>
+template <int TYPE, int KIND>
 __global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
   const long blocks = (p.cols + 127) / 128;
   const long unit = (long)blockIdx.x * 16 + threadIdx.x / 16;
@@ -129,7 +127,7 @@ __global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
   const long row = unit / blocks, block = unit - row * blocks;
   const long at = block * 128 + part * 8;
   float v[8];
-  load8<TYPE, VEC>(p.x, row * p.stride + at, p.cols - at, v);
+  load8<TYPE>(p.x, row * p.stride + at, p.cols - at, v);
   uint32_t most = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e]));
@@ -138,11 +136,11 @@ __global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
   const float s = scale_of<KIND>(most);
   uint32_t w[2];
   codes8<KIND>(v, s, 1.f / s, normal_scale(s), w);
-  if (at < p.cols) store8<VEC>(p.codes + row * p.pitch + at, w, p.cols - at);
+  if (at < p.cols) store8(p.codes + row * p.pitch + at, w, p.cols - at);
   if (part == 0) p.scales[row * p.s_row + block * p.s_block] = s;
 }
 
-template <int TYPE, int KIND, bool VEC, bool TURN, bool WHOLE>  // WHOLE: one scale for the tile
+template <int TYPE, int KIND, bool TURN, bool WHOLE>  // WHOLE: one scale for the tile
 __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
   __shared__ __align__(16) uint8_t lds[TURN ? 128 * 128 : 16];
   __shared__ uint32_t tops[4][128];
@@ -153,7 +151,7 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const long row = r0 + rg * 8 + i, at = c0 + cg * 8;
-    load8<TYPE, VEC>(p.x, row * p.stride + at, row < p.rows ? p.cols - at : 0, v[i]);
+    load8<TYPE>(p.x, row * p.stride + at, row < p.rows ? p.cols - at : 0, v[i]);
   }
   uint32_t top[8];
 #pragma unroll
@@ -201,7 +199,7 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
       const long row = r0 + rg * 8 + i, at = c0 + cg * 8;
       uint32_t w[2];
       codes8<KIND>(v[i], s[0], inv[0], plain, w);
-      if (row < p.rows && at < p.cols) store8<VEC>(p.codes + row * p.pitch + at, w, p.cols - at);
+      if (row < p.rows && at < p.cols) store8(p.codes + row * p.pitch + at, w, p.cols - at);
     }
   } else {
 #pragma unroll
@@ -221,8 +219,8 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
       const long out = c0 + c, at = r0 + piece * 16, count = p.rows - at;
       if (out >= p.cols || count <= 0) continue;
       uint8_t* to = p.codes + out * p.pitch + at;
-      if (count >= 16 && ((reinterpret_cast<uintptr_t>(p.codes) | (uintptr_t)p.pitch) & 15) == 0) {
-        *reinterpret_cast<uint4*>(to) = w;
+      if (count >= 16) {
+        *reinterpret_cast<any_u4*>(to) = u4{w.x, w.y, w.z, w.w};
       } else {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -233,24 +231,23 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
   }
 }
 
-template <int TYPE, int KIND, bool VEC>
+template <int TYPE, int KIND>
 hipError_t launch(const Convert& p, bool turn, bool whole, hipStream_t s) {
   if (!turn && !whole) {
     const long units = p.rows * ((p.cols + 127) / 128);
-    hipLaunchKernelGGL((fp8_rows<TYPE, KIND, VEC>), dim3((unsigned)((units + 15) / 16)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fp8_rows<TYPE, KIND>), dim3((unsigned)((units + 15) / 16)), dim3(256), 0, s, p);
   } else {
     const dim3 grid((unsigned)((p.cols + 127) / 128), (unsigned)((p.rows + 127) / 128));
-    if (!turn) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, VEC, false, true>), grid, dim3(256), 0, s, p);
-    else if (whole) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, VEC, true, true>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((fp8_tile<TYPE, KIND, VEC, true, false>), grid, dim3(256), 0, s, p);
+    if (!turn) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, false, true>), grid, dim3(256), 0, s, p);
+    else if (whole) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, true, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((fp8_tile<TYPE, KIND, true, false>), grid, dim3(256), 0, s, p);
   }
   return hipGetLastError();
 }
 
 template <int TYPE>
-hipError_t launch_type(const Convert& p, bool e5, bool vec, bool turn, bool whole, hipStream_t s) {
-  if (e5) return vec ? launch<TYPE, SHK_FP8_E5M2, true>(p, turn, whole, s) : launch<TYPE, SHK_FP8_E5M2, false>(p, turn, whole, s);
-  return vec ? launch<TYPE, SHK_FP8_E4M3, true>(p, turn, whole, s) : launch<TYPE, SHK_FP8_E4M3, false>(p, turn, whole, s);
+hipError_t launch_kind(const Convert& p, bool e5, bool turn, bool whole, hipStream_t s) {
+  return e5 ? launch<TYPE, SHK_FP8_E5M2>(p, turn, whole, s) : launch<TYPE, SHK_FP8_E4M3>(p, turn, whole, s);
 }
 
 }  // namespace
@@ -259,14 +256,10 @@ hipError_t launch_fp8_quantize(const shk_fp8_quantize& a, hipStream_t s) {
   if (a.rows * a.cols == 0) return hipSuccess;
   const Convert p{static_cast<const uint8_t*>(a.x), a.rows, a.cols, a.x_stride, static_cast<uint8_t*>(a.codes),
                   a.code_pitch, a.scales, a.scale_row_stride, a.scale_block_stride};
-  // 16-byte loads of x, and 8-byte stores of the codes that lie as x does
-  const long size = a.type == SHK_SRC_F32 ? 4 : 2;
-  const bool vec = ((reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(size * a.x_stride)) & 15) == 0 &&
-                   (a.transpose || ((reinterpret_cast<uintptr_t>(a.codes) | (uintptr_t)a.code_pitch) & 7) == 0);
   const bool e5 = a.kind == SHK_FP8_E5M2, turn = a.transpose != 0, whole = a.block_rows == 128;
-  if (a.type == SHK_SRC_F32) return launch_type<SHK_SRC_F32>(p, e5, vec, turn, whole, s);
-  if (a.type == SHK_SRC_F16) return launch_type<SHK_SRC_F16>(p, e5, vec, turn, whole, s);
-  return launch_type<SHK_SRC_BF16>(p, e5, vec, turn, whole, s);
+  if (a.type == SHK_SRC_F32) return launch_kind<SHK_SRC_F32>(p, e5, turn, whole, s);
+  if (a.type == SHK_SRC_F16) return launch_kind<SHK_SRC_F16>(p, e5, turn, whole, s);
+  return launch_kind<SHK_SRC_BF16>(p, e5, turn, whole, s);
 }
 
 }  // namespace shk

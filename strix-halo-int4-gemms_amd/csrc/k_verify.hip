@@ -14,6 +14,7 @@
 #include <cstdint>
 
 #include "shk_common.h"
+#include "shk_loads.h"
 #include "shk_step.h"
 
 namespace shk {
@@ -42,24 +43,22 @@ __device__ __forceinline__ float value_of(const void* x, long i) {
   return TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
-// Values [at, at + 8) of a row, those from `count` on as 0.  VEC: on 16 bytes.
-template <int TYPE, bool VEC>
+// Values [at, at + 8) of a row, those from `count` on as 0.  Whole ones come in
+// vectors, of any alignment.
+template <int TYPE>
 __device__ __forceinline__ void load8(const void* x, long at, long count, float (&v)[8]) {
-  if (VEC && count >= 8) {
+  if (count >= 8) {
     constexpr int SIZE = TYPE == SHK_SRC_F32 ? 4 : 2;
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * SIZE);
-    uint32_t u[SIZE * 2];
+    const any_u4* src = reinterpret_cast<const any_u4*>(static_cast<const uint8_t*>(x) + at * SIZE);
+    u4 u[SIZE / 2];
 #pragma unroll
-    for (int i = 0; i < SIZE / 2; ++i) {
-      const uint4 w = src[i];
-      u[4 * i] = w.x, u[4 * i + 1] = w.y, u[4 * i + 2] = w.z, u[4 * i + 3] = w.w;
-    }
+    for (int i = 0; i < SIZE / 2; ++i) u[i] = src[i];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (TYPE == SHK_SRC_F32) {
-        v[e] = __uint_as_float(u[e]);
+        v[e] = __uint_as_float(u[e / 4][e % 4]);
       } else {
-        const uint16_t h = (uint16_t)(u[e / 2] >> (16 * (e % 2)));
+        const uint16_t h = (uint16_t)(u[0][e / 2] >> (16 * (e % 2)));
         v[e] = TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
       }
     }
@@ -111,13 +110,13 @@ __device__ __forceinline__ Row row_of(const shk_verify& p, long b, int kept) {
 }
 
 // Weights of values [t, t + 8); NaN and negative ones count as 0.
-template <int TYPE, bool VEC>
+template <int TYPE>
 __device__ __forceinline__ void weights8(const shk_verify& p, const Row& r, long t, Sum (&w)[8]) {
   const long count = p.vocab - t;
   float have[8], gone[8];
-  load8<TYPE, VEC>(p.target, r.target + t, count, have);
+  load8<TYPE>(p.target, r.target + t, count, have);
   if (r.draft >= 0) {
-    load8<TYPE, VEC>(p.draft, r.draft + t, count, gone);
+    load8<TYPE>(p.draft, r.draft + t, count, gone);
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -132,7 +131,7 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-template <int TYPE, bool VEC>
+template <int TYPE>
 __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, const Pieces pieces) {
   __shared__ Sum parts[kThreads / 64];
   const long b = blockIdx.y;
@@ -142,7 +141,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, cons
   Sum mine{0.0, 0.0};
   for (long t = from + threadIdx.x * 8; t < to; t += kPiece) {
     Sum w[8];
-    weights8<TYPE, VEC>(p, r, t, w);
+    weights8<TYPE>(p, r, t, w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) mine.left += w[e].left, mine.all += w[e].all;
   }
@@ -173,7 +172,7 @@ __device__ __forceinline__ Sum group_inclusive(Sum v, Sum (&parts)[kThreads / 64
   return Sum{before.left + v.left, before.all + v.all};
 }
 
-template <int TYPE, bool VEC>
+template <int TYPE>
 __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, const Pieces pieces) {
   __shared__ Sum parts[2][kThreads / 64], total;
   __shared__ double before;
@@ -208,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, cons
     for (long base = from; base < to; base += kPiece) {
       const long t = base + threadIdx.x * 8;
       Sum w[8], sum{0.0, 0.0};
-      weights8<TYPE, VEC>(p, r, t, w);
+      weights8<TYPE>(p, r, t, w);
       double values[8], mass = 0.0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -251,23 +250,13 @@ Pieces pieces_of(const shk_verify& a) {
   return Pieces{(int)((steps + each - 1) / each), (int)(each * kPiece)};
 }
 
-template <int TYPE, bool VEC>
+template <int TYPE>
 hipError_t launch(const shk_verify& a, hipStream_t s) {
   const Pieces pieces = pieces_of(a);
-  hipLaunchKernelGGL((verify_sums<TYPE, VEC>), dim3(pieces.count, (unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
+  hipLaunchKernelGGL((verify_sums<TYPE>), dim3(pieces.count, (unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
   if (hipError_t e = hipGetLastError()) return e;
-  hipLaunchKernelGGL((verify_draw<TYPE, VEC>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
+  hipLaunchKernelGGL((verify_draw<TYPE>), dim3((unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
   return hipGetLastError();
-}
-
-template <int TYPE>
-hipError_t launch_type(const shk_verify& a, hipStream_t s) {
-  // 16-byte loads where every row starts on 16 bytes
-  const uintptr_t size = TYPE == SHK_SRC_F32 ? 4 : 2;
-  uintptr_t all = reinterpret_cast<uintptr_t>(a.target) | size * (uintptr_t)(a.target_batch_stride | a.target_row_stride);
-  if (a.draft != nullptr)
-    all |= reinterpret_cast<uintptr_t>(a.draft) | size * (uintptr_t)(a.draft_batch_stride | a.draft_row_stride);
-  return all % 16 == 0 ? launch<TYPE, true>(a, s) : launch<TYPE, false>(a, s);
 }
 
 }  // namespace
@@ -277,9 +266,9 @@ int64_t verify_workspace(const shk_verify& a) {
 }
 
 hipError_t launch_verify(const shk_verify& a, hipStream_t s) {
-  if (a.type == SHK_SRC_F32) return launch_type<SHK_SRC_F32>(a, s);
-  if (a.type == SHK_SRC_F16) return launch_type<SHK_SRC_F16>(a, s);
-  return launch_type<SHK_SRC_BF16>(a, s);
+  if (a.type == SHK_SRC_F32) return launch<SHK_SRC_F32>(a, s);
+  if (a.type == SHK_SRC_F16) return launch<SHK_SRC_F16>(a, s);
+  return launch<SHK_SRC_BF16>(a, s);
 }
 
 }  // namespace shk

@@ -9,6 +9,7 @@
 #include "shk_common.h"
 #include "shk_dma.h"
 #include "shk_fp8.h"
+#include "shk_loads.h"
 
 namespace shk {
 
@@ -29,7 +30,6 @@ struct Fp8Product {
   int tiles_m, tiles_n;
   int splits, per_split;  // blocks of K
   int out_type, b_shift;  // rows of b >> b_shift: its row of scales
-  int aligned;            // rows of out start on 16 bytes
 };
 
 // One block of K.  Rows of the result are b's (four of a lane group's), columns
@@ -45,22 +45,23 @@ __device__ __forceinline__ void store_value(const Fp8Product& p, long at, float 
   else static_cast<_Float16*>(p.out)[at] = (_Float16)v;
 }
 
-// Four neighbouring values of a row, whole where they lie inside and rows start
-// on 16 bytes (p.aligned).
+// Four neighbouring values of a row, in one store where they lie inside (rows of
+// out start where they will: the memory unit takes vectors of any alignment).
 __device__ __forceinline__ void store_four(const Fp8Product& p, int m, int n, const v4f& v) {
   const long at = (long)m * p.out_stride + n;
-  if (p.aligned && n + 3 < p.n) {
+  if (n + 3 < p.n) {
     if (p.out_type == SHK_SRC_F32) {
-      *reinterpret_cast<v4f*>(static_cast<float*>(p.out) + at) = v;
+      *reinterpret_cast<any_u4*>(static_cast<float*>(p.out) + at) =
+          u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
     } else {
-      uint2 u;
+      u2 u;
       if (p.out_type == SHK_SRC_BF16) {
-        u = make_uint2(pack_bf16x2_nonan(v[0], v[1]), pack_bf16x2_nonan(v[2], v[3]));
+        u = u2{pack_bf16x2_nonan(v[0], v[1]), pack_bf16x2_nonan(v[2], v[3])};
       } else {
-        u.x = __builtin_bit_cast(uint16_t, (_Float16)v[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16);
-        u.y = __builtin_bit_cast(uint16_t, (_Float16)v[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[3]) << 16);
+        u[0] = __builtin_bit_cast(uint16_t, (_Float16)v[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16);
+        u[1] = __builtin_bit_cast(uint16_t, (_Float16)v[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[3]) << 16);
       }
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = u;
+      *reinterpret_cast<any_u2*>(static_cast<uint16_t*>(p.out) + at) = u;
     }
     return;
   }
