@@ -276,7 +276,9 @@ Plan plan_of(const shk_fp8_mm& a) {
   const bool wide = a.out_type == SHK_SRC_F32;
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
   const int64_t small = tiles(64, 64);
-  if (a.m <= 32 || (a.m <= 64 && a.n <= 4096)) {
+  if (a.k == 0) {
+    r.kind = kTile64;  // asks for no stage
+  } else if (a.m <= 32 || (a.m <= 64 && a.n <= 4096)) {
     r.kind = kFew;
   } else if (wide) {
     r.kind = tiles(128, 128) > 128 ? kWide : kTile64;
@@ -290,7 +292,8 @@ Plan plan_of(const shk_fp8_mm& a) {
   r.per_split = std::max(1, (blocks + r.splits - 1) / r.splits);
   r.splits = std::max(1, (blocks + r.per_split - 1) / r.per_split);
   // the copies to LDS are of whole 16 bytes; loads to registers are not
-  r.copy_a = r.kind != kFew && loose(a.a, a.a_pitch, a.m), r.copy_b = r.kind != kFew && loose(a.b, a.b_pitch, a.n);
+  const bool staged = a.k > 0 && r.kind != kFew;
+  r.copy_a = staged && loose(a.a, a.a_pitch, a.m), r.copy_b = staged && loose(a.b, a.b_pitch, a.n);
   r.pitch = (a.k + 15) & ~15L;
   r.at_b = r.copy_a ? a.m * r.pitch : 0;
   r.at_partial = r.at_b + (r.copy_b ? a.n * r.pitch : 0);
