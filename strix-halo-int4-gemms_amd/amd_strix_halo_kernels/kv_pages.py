@@ -123,6 +123,8 @@ def kv_pages_step(pages: KVPages, new_tokens: Any, capacity: int, *, stream: Any
         with _on_stream(torch, table, stream):
             return kv_pages_step(pages, new_tokens, capacity)
     batch, width = table.shape
+    if pages.lengths.shape[0] != batch or pages.owned.shape[0] != batch or not table.is_contiguous():
+        pages.__post_init__()  # a tensor was given other memory: says what is wrong
     if new_tokens.dtype != torch.int32 or new_tokens.shape != (batch,) or not new_tokens.is_contiguous():
         raise ValueError(f"new_tokens must be a contiguous torch.int32 tensor of shape ({batch},); got "
                          f"{new_tokens.dtype} {tuple(new_tokens.shape)}")

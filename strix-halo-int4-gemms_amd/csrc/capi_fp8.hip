@@ -1,5 +1,6 @@
 // C ABI of the 8-bit floating-point products: argument validation and launches.
 // Declarations are in include/strix_halo_gfx950.h.
+#include <algorithm>
 #include <climits>
 #include <string>
 
@@ -29,11 +30,13 @@ int check_mm(const shk_fp8_mm* a) {
   if (!source(a->out_type)) return capi_fail("unknown output type " + std::to_string(a->out_type));
   if (a->b_rows != 1 && a->b_rows != shk::kFp8Block)
     return capi_fail("b_rows is 1 or 128; got " + std::to_string(a->b_rows));
-  if (a->m < 0 || a->n < 0 || a->k < 0 || a->m > INT_MAX / 2 || a->n > INT_MAX / 2 || a->k >= (1 << 23))
-    return capi_fail("m and n are from 0 to 1073741823, k to 8388607");
+  if (a->m < 0 || a->n < 0 || a->k < 0 || a->m > INT_MAX / 4 || a->n > INT_MAX / 4 || a->k >= (1 << 23))
+    return capi_fail("m and n are from 0 to 536870911, k to 8388607");
   if (a->m * a->n == 0) return 0;
-  // workgroups are counted in 32 bits by the smallest tile, and the join by 256 values
-  if ((__int128)a->m * a->n > (__int128)INT_MAX * 64) return capi_fail("too many outputs for one launch");
+  // a launch holds fewer than 2^32 work-items: 256 for 64 x 128 results, and one
+  // for 16 bytes of an operand that is copied
+  if ((__int128)((a->m + 63) / 64) * ((a->n + 127) / 128) > 0xFFFFFF || (a->k > 0 && std::max(a->m, a->n) > 0xFFFFFF00LL / ((a->k + 15) / 16)))
+    return capi_fail("too many outputs for one launch");
   if (a->a_pitch < a->k || a->b_pitch < a->k || a->a_pitch >= (1 << 24) || a->b_pitch >= (1 << 24))
     return capi_fail("row pitches are from k to 16777215 bytes");
   if (a->out_stride < a->n) return capi_fail("rows of out must not overlap");

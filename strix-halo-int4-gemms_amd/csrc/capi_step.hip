@@ -32,8 +32,10 @@ int check_rotate(const shk_kv_cache* c, const shk_rotate* args) {
   if (!std::isfinite((float)a.amplitude)) return capi_fail("the amplitude must be finite in 32 bits");
   if (!(a.eps >= 0.0) || !std::isfinite((float)a.eps)) return capi_fail("eps must be finite and not negative");
   if ((a.q_weight == nullptr) != (a.k_weight == nullptr)) return capi_fail("q and k have weights both or neither");
-  // rows are counted in 32 bits
-  if ((__int128)a.tokens * (a.heads + 2 * a.kv_heads) > INT_MAX - 4096) return capi_fail("too many rows for one launch");
+  // a launch holds fewer than 2^32 work-items, and rows are counted in 32 bits
+  const int64_t lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
+  if ((__int128)a.tokens * (a.heads + (c != nullptr ? 2 : 1) * a.kv_heads) > (0xFFFFFFFFLL / lanes) - 4096)
+    return capi_fail("too many rows for one launch");
   if (c != nullptr) {
     if (int rc = check_cache(c)) return rc;
     if (c->head_dim != a.head_dim || c->kv_heads != a.kv_heads)

@@ -114,3 +114,26 @@ def test_replays(device):
         for g, w in zip(got, want):
             assert torch.equal(g, w)
         assert _state(eager) == _state(captured)
+
+
+def test_refused_arguments(device):
+    pool = shk.new_kv_pages(3, 4, 12, 16, device=device)
+    new = torch.ones(3, dtype=torch.int32, device=device)
+    for bad, capacity, match in ((new.long(), 8, "new_tokens"), (new[:2], 8, "new_tokens"), (new, -1, "capacity"),
+                                 (new, 2.0, "capacity"), (new, True, "capacity"), (new, 2**31, "capacity")):
+        with pytest.raises(ValueError, match=match):
+            shk.kv_pages_step(pool, bad, capacity)
+    with pytest.raises((RuntimeError, ValueError), match="CUDA/HIP|expected"):
+        shk.kv_pages_step(pool, new.cpu(), 8)
+    assert pool.lengths.tolist() == [0, 0, 0] and int(pool.free_count) == 12
+
+
+def test_counts_past_any_capacity(device):
+    """Numbers that no table holds are refused, their sum saturates, and what fits before them is served."""
+    pool = shk.new_kv_pages(4, 4, 16, 16, device=device)
+    new = torch.tensor([20, 2**31 - 1, 2**31 - 1, 5], dtype=torch.int32, device=device)
+    step = shk.kv_pages_step(pool, new, 30)
+    assert step.taken.tolist() == [20, 0, 0, 0] and pool.lengths.tolist() == [20, 0, 0, 0]
+    assert step.slots[:20].tolist() == list(range(20)) and step.slots[20:].tolist() == [-1] * 10
+    assert step.sequences.tolist() == [0] * 20 + [1] * 10
+    assert step.starts.tolist() == [0, 20, 2**31 - 1, 2**31 - 1, 2**31 - 1]

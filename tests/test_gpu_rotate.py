@@ -175,3 +175,53 @@ def test_stream_graph_and_gradient(device):
     out = shk.rotate_qk(q, dev[:, 4:6], positions, rotary)
     with pytest.raises(RuntimeError, match="rotate_qk has no gradient"):
         out[0].float().sum().backward()
+
+
+def test_refusals(device):
+    rotary = shk.new_rotary(ref.half_turns(32), device=device)
+    x = torch.zeros((5, 6, 64), dtype=BF16, device=device)
+    q, k, v = x[:, :4], x[:, 4:5], x[:, 5:]
+    at = torch.arange(5, device=device)
+    w = torch.ones(64, dtype=BF16, device=device)
+    cache = shk.new_kv_cache(4, 16, 1, 64, device=device)
+    into = {"cache": cache, "values": v, "slots": at}
+    for args, kw, match in (
+        ((q.double(), k.double(), at, rotary), {}, "q must have dtype"), ((q, k.half(), at, rotary), {}, "dtype of q"),
+        ((q[0], k, at, rotary), {}, "q must have shape"), ((q, k[:4], at, rotary), {}, "k must have shape"),
+        ((q, k[..., :32], at, rotary), {}, "k must have shape"),
+        ((x.transpose(1, 2), k, at, rotary), {}, "contiguous along head_dim"),
+        ((q[..., :32], k[..., :32], at, rotary), {}, "rotary turns 64"),
+        ((q, k, at.float(), rotary), {}, "positions must have dtype"),
+        ((q, k, at[:4], rotary), {}, "positions must be contiguous"),
+        ((q, k, at, rotary), {"q_weight": w}, "both or neither"),
+        ((q, k, at, rotary), {"q_weight": w, "k_weight": w.float()}, "both the same"),
+        ((q, k, at, rotary), {"q_weight": w.half(), "k_weight": w.half()}, "must have dtype"),
+        ((q, k, at, rotary), {"q_weight": w[:32], "k_weight": w[:32]}, "q_weight must be contiguous"),
+        ((q, k, at, rotary), {"eps": -1.0}, "eps"), ((q, k, at, rotary), {"eps": math.nan}, "eps"),
+        ((q, k, at, rotary), {"values": v}, "need a cache"), ((q, k, at, rotary), {"slots": at}, "need a cache"),
+        ((q, k, at, rotary), {"q_out": q.float()}, "q_out must have dtype"),
+        ((q, k, at, rotary), {"k_out": q}, "k_out must have shape"),
+        ((q, k, at, rotary), into | {"k_out": k}, "no other result"),
+        ((q, k, at, rotary), into | {"values": None}, "needs values and slots"),
+        ((q, k, at, rotary), into | {"values": v.float()}, "values must have the dtype"),
+        ((q, k, at, rotary), into | {"slots": at[:3]}, "slots must have shape"),
+        ((q, x[:, 4:], at, rotary), into, "k must have shape"),
+    ):
+        with pytest.raises(ValueError, match=match):
+            shk.rotate_qk(*args, **kw)
+    with pytest.raises((RuntimeError, ValueError), match="CUDA/HIP|expected"):
+        shk.rotate_qk(q, k, at.cpu(), rotary)
+
+
+def test_offsets_past_32_bits(device):
+    """Tokens 18 MB apart."""
+    store = torch.zeros((300, 9_000_000), dtype=BF16, device=device)
+    x = torch.randn((300, 3, 128), generator=torch.Generator().manual_seed(1)).to(BF16)
+    far = store.as_strided((300, 3, 128), (9_000_000, 128, 1), 8_999_000)
+    far.copy_(x)
+    rotary = shk.new_rotary(ref.half_turns(64), device=device)
+    at = torch.arange(300, device=device)
+    near = x.to(device)
+    want = shk.rotate_qk(near[:, :2], near[:, 2:], at, rotary)
+    got = shk.rotate_qk(far[:, :2], far[:, 2:], at, rotary)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -156,3 +156,39 @@ def test_kept_tokens_are_distributed_as_the_targets(device):
                               torch.rand((n, 2), generator=g).to(device))
     share = torch.bincount(out[:, 0].cpu(), minlength=5).double() / n
     assert ((share - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all()
+
+
+def test_refusals(device):
+    target, draft = torch.zeros((2, 4, 50), device=device), torch.zeros((2, 3, 50), device=device)
+    tokens, u = torch.zeros((2, 3), dtype=torch.int64, device=device), torch.zeros((2, 4), device=device)
+    counts = torch.zeros(2, dtype=torch.int32, device=device)
+    for args, kw, match in (((target.double(), None, tokens, u), {}, "target must have dtype"),
+                            ((target[:, :3], None, tokens, u), {}, "target must have shape"),
+                            ((target[..., ::2], None, tokens, u), {}, "target must be contiguous"),
+                            ((target, draft.half(), tokens, u), {}, "draft must have shape"),
+                            ((target, draft[..., :49], tokens, u), {}, "draft must have shape"),
+                            ((target, draft, tokens.float(), u), {}, "tokens must have dtype"),
+                            ((target, draft, tokens[0], u), {}, "tokens must be contiguous"),
+                            ((target, draft, tokens, u[:, :3]), {}, "uniforms must be contiguous"),
+                            ((target, draft, tokens, u.half()), {}, "uniforms must be contiguous"),
+                            ((target, draft, tokens, u), {"counts": counts.long()}, "counts must be"),
+                            ((target, draft, tokens, u), {"lengths": counts[:1]}, "lengths must be"),
+                            ((torch.zeros((1, 65, 4), device=device), None, torch.zeros((1, 64), dtype=torch.int64, device=device),
+                              torch.zeros((1, 65), device=device)), {}, "up to 63 drafts")):
+        with pytest.raises(ValueError, match=match):
+            shk.verify_draft(*args, **kw)
+    with pytest.raises((RuntimeError, ValueError), match="CUDA/HIP|expected"):
+        shk.verify_draft(target, draft, tokens.cpu(), u)
+
+
+@pytest.mark.parametrize("vocab", [524288, 600001])
+def test_vocabularies_of_several_steps_a_piece(device, vocab):
+    """Weights that are whole multiples of 2^-20, so that the order of adding does not show."""
+    g = torch.Generator().manual_seed(vocab)
+    target = (torch.randint(0, 9, (2, 1, vocab), generator=g).float() * 2.0**-20)
+    target[1, 0, : vocab - 3] = 0.0
+    uniforms = torch.tensor([[0.734375], [0.5]])
+    out, _ = shk.verify_draft(target.to(device), None, torch.empty((2, 0), dtype=torch.int64, device=device),
+                              uniforms.to(device))
+    run = target[:, 0].double().cumsum(-1)
+    assert out[:, 0].tolist() == [int((run[b] <= float(uniforms[b, 0]) * float(run[b, -1])).sum()) for b in range(2)]
