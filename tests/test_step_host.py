@@ -166,7 +166,7 @@ MM = {"a": FAKE, "a_pitch": 256, "a_kind": 0, "b": FAKE, "b_pitch": 256, "b_kind
                                        ({"out_stride": 127}, b"out must not overlap"),
                                        ({"a_scale_row": -1}, b"not negative"), ({"b_scale_block": 2**30}, b"span less"),
                                        ({"out": 0}, b"non-null"), ({"a_scale": 0}, b"non-null"),
-                                       ({"out": FAKE + 1}, b"aligned"), ({"a": FAKE + 8}, b"workspace must hold"),
+                                       ({"out": FAKE + 1}, b"aligned"), ({"a": FAKE + 8, "m": 100}, b"workspace must hold"),
                                        ({"m": 2**28, "n": 2**28, "out_stride": 2**28}, b"too many outputs"),
                                        ({"m": 2**29}, b"m and n")])
 def test_product_refusals(lib, bad, match):
