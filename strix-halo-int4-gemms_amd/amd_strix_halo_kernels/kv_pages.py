@@ -132,7 +132,8 @@ def kv_pages_step(pages: KVPages, new_tokens: Any, capacity: int, *, stream: Any
         raise ValueError(f"capacity must be an int from 0 to {2**31 - 1}; got {capacity!r}")
     # one allocation, the 8-byte slots first
     work = torch.empty(4 * capacity + 2 * batch + 1, dtype=torch.int32, device=table.device)
-    slots, positions, sequences, starts, taken = work.split((2 * capacity, capacity, capacity, batch + 1, batch))
+    slots, positions, sequences, starts, taken = work.split_with_sizes(
+        (2 * capacity, capacity, capacity, batch + 1, batch))
     step = KVStep(slots.view(torch.int64), positions, sequences, starts, taken)
     lib = _verified_library()
     _check(lib, lib.amd_strix_halo_kernels_kv_plan(

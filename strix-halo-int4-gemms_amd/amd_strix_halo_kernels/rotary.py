@@ -104,13 +104,11 @@ def new_rotary(frequencies: Sequence[float], *, amplitude: float = 1.0, interlea
     return Rotary(torch.tensor(turns, dtype=torch.float64, device=device), float(amplitude), bool(interleaved))
 
 
-def _heads(name: str, t: Any, tokens: int, heads: int | None, dim: int) -> int:
-    if t.ndim != 3 or t.shape[0] != tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        want = (tokens, "heads" if heads is None else heads, dim)
-        raise ValueError(f"{name} must have shape {want} == (tokens, heads, head_dim); got {tuple(t.shape)}")
-    if t.stride(2) != 1:
+def _heads(name: str, t: Any, shape: tuple, strides: tuple) -> None:
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape} == (tokens, heads, head_dim); got {tuple(t.shape)}")
+    if strides[2] != 1:
         raise ValueError(f"{name} must be contiguous along head_dim")
-    return int(t.shape[1])
 
 
 def rotate_qk(
@@ -159,14 +157,19 @@ def rotate_qk(
             return rotate_qk(q, k, positions, rotary, q_weight=q_weight, k_weight=k_weight, eps=eps, cache=cache,
                              values=values, slots=slots, q_out=q_out, k_out=k_out)
     native = None if cache is None else cache._native
-    kind = _row_type(torch, "q", q.dtype)
-    if k.dtype != q.dtype:
-        raise ValueError(f"k must have the dtype of q, {q.dtype}; got {k.dtype}")
+    dtype = q.dtype
+    kind = _row_type(torch, "q", dtype)
+    if k.dtype != dtype:
+        raise ValueError(f"k must have the dtype of q, {dtype}; got {k.dtype}")
     if q.ndim != 3:
         raise ValueError(f"q must have shape (tokens, heads, head_dim); got {tuple(q.shape)}")
-    tokens, dim = int(q.shape[0]), int(q.shape[2])
-    heads = _heads("q", q, tokens, None, dim)
-    kv_heads = _heads("k", k, tokens, None if cache is None else cache.kv_heads, dim)
+    if k.ndim != 3:
+        raise ValueError(f"k must have shape (tokens, heads, head_dim); got {tuple(k.shape)}")
+    tokens, heads, dim = q.shape
+    kv_heads = k.shape[1] if cache is None else cache.kv_heads
+    q_strides, k_strides, k_shape = q.stride(), k.stride(), (tokens, kv_heads, dim)
+    _heads("q", q, (tokens, heads, dim), q_strides)
+    _heads("k", k, k_shape, k_strides)
     if dim % 2 or not 2 <= dim <= 256:
         raise ValueError(f"head_dim must be even, from 2 to 256; got {dim}")
     if rotary.rotated > dim:
@@ -190,24 +193,27 @@ def rotate_qk(
     if not 0.0 <= eps < 3e38:
         raise ValueError(f"eps must be finite and not negative; got {eps}")
     if q_out is None:
-        q_out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        q_out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
+        qo_strides = (heads * dim, dim)
     else:
-        _heads("q_out", q_out, tokens, heads, dim)
-        if q_out.dtype != q.dtype:
-            raise ValueError(f"q_out must have dtype {q.dtype}; got {q_out.dtype}")
-    given = (q, k) if q_weight is None else (q, k, q_weight, k_weight)
+        qo_strides = q_out.stride()
+        _heads("q_out", q_out, (tokens, heads, dim), qo_strides)
+        if q_out.dtype != dtype:
+            raise ValueError(f"q_out must have dtype {dtype}; got {q_out.dtype}")
     k_at = v_at = (0, 0, 0)
     slots_at = (0, 4)
     if cache is None:
         if values is not None or slots is not None:
             raise ValueError("values and slots need a cache")
         if k_out is None:
-            k_out = torch.empty((tokens, kv_heads, dim), dtype=q.dtype, device=q.device)
+            k_out = torch.empty(k_shape, dtype=dtype, device=q.device)
+            k_at = (k_out.data_ptr(), kv_heads * dim, dim)
         else:
-            _heads("k_out", k_out, tokens, kv_heads, dim)
-            if k_out.dtype != q.dtype:
-                raise ValueError(f"k_out must have dtype {q.dtype}; got {k_out.dtype}")
-        k_at = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+            strides = k_out.stride()
+            _heads("k_out", k_out, k_shape, strides)
+            if k_out.dtype != dtype:
+                raise ValueError(f"k_out must have dtype {dtype}; got {k_out.dtype}")
+            k_at = (k_out.data_ptr(), strides[0], strides[1])
     else:
         if k_out is not None:
             raise ValueError("with a cache the keys have no other result")
@@ -215,11 +221,14 @@ def rotate_qk(
             raise ValueError("a cache needs values and slots")
         if dim != cache.head_dim:
             raise ValueError(f"head_dim must be the cache's, {cache.head_dim}; got {dim}")
-        _heads("values", values, tokens, kv_heads, dim)
-        if values.dtype != q.dtype:
-            raise ValueError(f"values must have the dtype of q, {q.dtype}; got {values.dtype}")
+        if values.ndim != 3:
+            raise ValueError(f"values must have shape {k_shape}; got {tuple(values.shape)}")
+        strides = values.stride()
+        _heads("values", values, k_shape, strides)
+        if values.dtype != dtype:
+            raise ValueError(f"values must have the dtype of q, {dtype}; got {values.dtype}")
         _check_slots(torch, slots, tokens)
-        v_at = (values.data_ptr(), values.stride(0), values.stride(1))
+        v_at = (values.data_ptr(), strides[0], strides[1])
         slots_at = (slots.data_ptr(), slots.element_size())
     if tokens:
         if heads < 1 or kv_heads < 1:
@@ -227,13 +236,14 @@ def rotate_qk(
         lib = _verified_library()
         _check(lib, lib.amd_strix_halo_kernels_rotate(
             index, _current_stream(torch, index), native,
-            _ROTATE.pack(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), kind, tokens,
-                         heads, kv_heads, dim, rotary.rotated, rotary.interleaved, positions.data_ptr(),
+            _ROTATE.pack(q.data_ptr(), q_strides[0], q_strides[1], k.data_ptr(), k_strides[0], k_strides[1], kind,
+                         tokens, heads, kv_heads, dim, rotary.rotated, rotary.interleaved, positions.data_ptr(),
                          positions.element_size(), rotary.turns.data_ptr(), rotary.amplitude,
                          0 if q_weight is None else q_weight.data_ptr(),
                          0 if k_weight is None else k_weight.data_ptr(), weight_kind, eps, q_out.data_ptr(),
-                         q_out.stride(0), q_out.stride(1), *k_at, *v_at, *slots_at)))
-    if any(t.requires_grad for t in given):
+                         qo_strides[0], qo_strides[1], *k_at, *v_at, *slots_at)))
+    if q.requires_grad or k.requires_grad or (q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad)):
+        given = (q, k) if q_weight is None else (q, k, q_weight, k_weight)
         q_out = _no_gradient(torch, "rotate_qk", q_out, *given)
         k_out = None if cache is not None else _no_gradient(torch, "rotate_qk", k_out, *given)
     return q_out if cache is not None else (q_out, k_out)
