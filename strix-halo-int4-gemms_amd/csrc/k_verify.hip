@@ -157,14 +157,31 @@ __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, cons
   }
 }
 
+// v plus the value that CTRL moves to this lane, in the rows of ROWS (else plus 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double plus_moved(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+
+// Inclusive sum over a wave's lanes: within rows of 16 by 1, 2, 4 and 8 lanes up,
+// then the last lane of rows 0 and 2 to the rows above them, and lane 31 to both
+// rows behind it.
+__device__ __forceinline__ double wave_inclusive(double v) {
+  v = plus_moved<0x111, 0xF>(v);
+  v = plus_moved<0x112, 0xF>(v);
+  v = plus_moved<0x114, 0xF>(v);
+  v = plus_moved<0x118, 0xF>(v);
+  v = plus_moved<0x142, 0xA>(v);
+  return plus_moved<0x143, 0xC>(v);
+}
+
 // Inclusive sums over the workgroup's threads, of both weights.
 __device__ __forceinline__ Sum group_inclusive(Sum v, Sum (&parts)[kThreads / 64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const Sum o{__shfl_up(v.left, d, 64), __shfl_up(v.all, d, 64)};
-    if (lane >= d) v.left += o.left, v.all += o.all;
-  }
+  v.left = wave_inclusive(v.left), v.all = wave_inclusive(v.all);
   if (lane == 63) parts[wave] = v;
   __syncthreads();
   Sum before{0.0, 0.0};
@@ -183,12 +200,16 @@ __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, cons
   const Row r = row_of(p, b, kept);
   const Sum* sums = reinterpret_cast<const Sum*>(work + kept_bytes(p.batch)) + b * pieces.count;
   const Sum mine = (int)threadIdx.x < pieces.count ? sums[threadIdx.x] : Sum{0.0, 0.0};
+  // what is needed at the end, asked for now
+  const double uniform = p.uniforms[b * (p.drafts + 1) + p.drafts];
+  const long drafted = (int)threadIdx.x < (int)p.drafts ? token_of(p, b * p.drafts + threadIdx.x) : -1;
+  const int lost = drafts_of(p, b) - kept, length = p.lengths != nullptr ? p.lengths[b] : 0;
   const Sum upto = group_inclusive(mine, parts[0]);
   if (threadIdx.x == 0) piece = passes = INT_MAX, holds = holds_here = -1;
   if (threadIdx.x == kThreads - 1) total = upto;
   __syncthreads();
   const bool rest = total.left > 0.0;
-  const double share = (double)p.uniforms[b * (p.drafts + 1) + p.drafts] * (rest ? total.left : total.all);
+  const double share = uniform * (rest ? total.left : total.all);
   const double run = rest ? upto.left : upto.all, own = rest ? mine.left : mine.all;
   // the first piece whose running sum passes the share; the last that holds
   // anything where a share of the whole sum, or more, was asked for
@@ -236,11 +257,11 @@ __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, cons
     // rounding can leave the running sum of a piece just below its own sum
     token = from + (passes != INT_MAX ? passes : holds_here);
   }
-  for (int i = threadIdx.x; i <= (int)p.drafts; i += kThreads)
-    p.out[b * (p.drafts + 1) + i] = i < kept ? token_of(p, b * p.drafts + i) : i == kept ? token : -1;
-  if (threadIdx.x == 0) {
+  const int i = threadIdx.x;  // there are fewer drafts than threads
+  if (i <= (int)p.drafts) p.out[b * (p.drafts + 1) + i] = i < kept ? drafted : i == kept ? token : -1;
+  if (i == 0) {
     p.kept[b] = kept;
-    if (p.lengths != nullptr) p.lengths[b] -= drafts_of(p, b) - kept;
+    if (p.lengths != nullptr) p.lengths[b] = length - lost;
   }
 }
 
