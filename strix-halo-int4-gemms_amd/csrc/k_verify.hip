@@ -7,7 +7,8 @@
 // is cut into pieces, verify_sums adds each piece, and verify_draw finds the
 // piece and then the token in it.  Sums are 64 bits: over a vocabulary f32 would
 // move the place by whole tokens, and the order of adding would show.
-// Bound by the one row of each kind that a sequence reads, or by two launches.
+// Bound by the one row of each kind that a sequence reads, or by two launches:
+// 1 x 32000 3.8 and 7 us, 61 x 131072 (61 MB) 14 (4.2 TB/s) and 12 us.
 #include <hip/hip_runtime.h>
 
 #include <climits>

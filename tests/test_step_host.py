@@ -168,6 +168,7 @@ MM = {"a": FAKE, "a_pitch": 256, "a_kind": 0, "b": FAKE, "b_pitch": 256, "b_kind
                                        ({"out": 0}, b"non-null"), ({"a_scale": 0}, b"non-null"),
                                        ({"out": FAKE + 1}, b"aligned"), ({"a": FAKE + 8, "m": 100}, b"workspace must hold"),
                                        ({"m": 2**28, "n": 2**28, "out_stride": 2**28}, b"too many outputs"),
+                                       ({"m": 1, "n": 2**29 - 1, "k": 1, "out_stride": 2**29}, b"too many outputs"),
                                        ({"m": 2**29}, b"m and n")])
 def test_product_refusals(lib, bad, match):
     packed = fp8._MM.pack(*(MM | bad).values())
