@@ -762,7 +762,7 @@ int amd_strix_halo_kernels_kv_plan(int device_index, uintptr_t stream, const shk
  * then -1; kept [batch].  Where lengths is not null, lengths[b] loses the drafts
  * that were not kept.  Draft tokens outside the vocabulary are not kept.
  * workspace: at least amd_strix_halo_kernels_verify_workspace bytes, on 16 bytes,
- * not read before it is written. */
+ * not read before it is written; null where that is 0 (up to 32768 tokens). */
 typedef struct shk_verify {
   const void* target;
   int64_t target_batch_stride;
@@ -772,7 +772,7 @@ typedef struct shk_verify {
   int64_t draft_row_stride;
   int64_t type; /* SHK_SRC_F32, SHK_SRC_F16 or SHK_SRC_BF16 */
   int64_t batch;
-  int64_t drafts; /* up to 64 */
+  int64_t drafts; /* up to 63 */
   int64_t vocab;
   const void* tokens;
   int64_t token_bytes; /* 4 or 8 */

@@ -112,7 +112,7 @@ def verify_draft(
                 _check(lib, 1)
             if len(_WORKSPACES) < 4096:
                 _WORKSPACES[batch, vocab] = nbytes
-        work = torch.empty(nbytes, dtype=torch.uint8, device=target.device)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=target.device) if nbytes else None
         _check(lib, lib.amd_strix_halo_kernels_verify(index, _current_stream(torch, index),
-                                                      args(work.data_ptr(), nbytes)))
+                                                      args(work.data_ptr() if nbytes else 0, nbytes)))
     return out, kept

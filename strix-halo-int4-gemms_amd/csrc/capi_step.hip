@@ -135,7 +135,7 @@ int amd_strix_halo_kernels_verify(int device_index, uintptr_t stream, const shk_
         !on(a.counts, 4) || !on(a.out, 8) || !on(a.kept, 4) || !on(a.lengths, 4))
       return capi_fail("tensors must be aligned to their elements");
     const int64_t need = shk::verify_workspace(a);
-    if (a.workspace == nullptr || a.workspace_bytes < need || !on(a.workspace, 16))
+    if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need || !on(a.workspace, 16)))
       return capi_fail("the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
     shk::DeviceGuard guard(device_index);
     if (guard.error() != hipSuccess) return capi_fail_hip("hipSetDevice", guard.error());

@@ -2,13 +2,19 @@
 // token that follows them, drawn from what the draft left of the target.
 //
 // The kept drafts are a handful of gathers, which a wave tests at once; every
-// workgroup does so for itself.  The draw needs the sum of one row's weights
-// before the place where the running sum passes its share u of it: the vocabulary
-// is cut into pieces, verify_sums adds each piece, and verify_draw finds the
-// piece and then the token in it.  Sums are 64 bits: over a vocabulary f32 would
-// move the place by whole tokens, and the order of adding would show.
-// Bound by the one row of each kind that a sequence reads, or by two launches:
-// 1 x 32000 3.8 and 7 us, 61 x 131072 (61 MB) 14 (4.2 TB/s) and 12 us.
+// wave does so for itself.  The draw needs the sum of one row's weights before the
+// place where the running sum passes its share u of it.  Sums are 64 bits: over a
+// vocabulary f32 would move the place by whole tokens, and the order of adding
+// would show.
+//  * verify_whole, up to 32768 tokens: a workgroup has a sequence's rows in its
+//    registers, one launch.  Bound by latency (tokens, gathers, rows, each asked
+//    for with what came before), and by what one CU can read.
+//  * verify_sums and verify_draw: the vocabulary is cut into pieces over all CUs,
+//    added first, then the piece and the token in it are found.  Bound by the one
+//    row of each kind that a sequence reads, and by the second launch: 61 x 131072
+//    f32 (61 MB) 14 us (4.2 TB/s) and 12.
+// f32, replayed, whole and in pieces: 1 x 2048 3.7 and 13.5 us, 128 x 16384 9 and
+// 24, 1 x 32768 8.5 and 11.2, 128 x 32768 12 and 19.5.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -110,26 +116,59 @@ __device__ __forceinline__ Row row_of(const shk_verify& p, long b, int kept) {
   return r;
 }
 
-// Weights of values [t, t + 8); NaN and negative ones count as 0.
+// Target and draft at values [t, t + 8); of a draft without probabilities the
+// token that it was certain of takes everything.
 template <int TYPE>
-__device__ __forceinline__ void weights8(const shk_verify& p, const Row& r, long t, Sum (&w)[8]) {
+__device__ __forceinline__ void values8(const shk_verify& p, const Row& r, long t, float (&have)[8], float (&gone)[8]) {
   const long count = p.vocab - t;
-  float have[8], gone[8];
   load8<TYPE>(p.target, r.target + t, count, have);
   if (r.draft >= 0) {
     load8<TYPE>(p.draft, r.draft + t, count, gone);
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    w[e].all = __builtin_fmaxf(have[e], 0.f);
-    w[e].left = r.draft >= 0 ? __builtin_fmax(w[e].all - (double)gone[e], 0.0) : t + e == r.certain ? 0.0 : w[e].all;
+    for (int e = 0; e < 8; ++e) gone[e] = t + e == r.certain ? __builtin_inff() : 0.f;
   }
+}
+
+// The weights of a value; NaN and negative ones count as 0.
+__device__ __forceinline__ Sum weight_of(float have, float gone) {
+  const double all = __builtin_fmaxf(have, 0.f);
+  return Sum{__builtin_fmax(all - (double)gone, 0.0), all};
+}
+
+template <int TYPE>
+__device__ __forceinline__ void weights8(const shk_verify& p, const Row& r, long t, Sum (&w)[8]) {
+  float have[8], gone[8];
+  values8<TYPE>(p, r, t, have, gone);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = weight_of(have[e], gone[e]);
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
   return v;
+}
+
+// v plus the value that CTRL moves to this lane, in the rows of ROWS (else plus 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double plus_moved(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+
+// Inclusive sum over a wave's lanes: within rows of 16 by 1, 2, 4 and 8 lanes up,
+// then the last lane of rows 0 and 2 to the rows above them, and lane 31 to both
+// rows behind it.
+__device__ __forceinline__ double wave_inclusive(double v) {
+  v = plus_moved<0x111, 0xF>(v);
+  v = plus_moved<0x112, 0xF>(v);
+  v = plus_moved<0x114, 0xF>(v);
+  v = plus_moved<0x118, 0xF>(v);
+  v = plus_moved<0x142, 0xA>(v);
+  return plus_moved<0x143, 0xC>(v);
 }
 
 template <int TYPE>
@@ -156,27 +195,6 @@ __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, cons
     reinterpret_cast<Sum*>(work + kept_bytes(p.batch))[b * pieces.count + blockIdx.x] = s;
     if (blockIdx.x == 0) reinterpret_cast<int32_t*>(work)[b] = kept;
   }
-}
-
-// v plus the value that CTRL moves to this lane, in the rows of ROWS (else plus 0).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double plus_moved(double v) {
-  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
-  return v + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
-}
-
-// Inclusive sum over a wave's lanes: within rows of 16 by 1, 2, 4 and 8 lanes up,
-// then the last lane of rows 0 and 2 to the rows above them, and lane 31 to both
-// rows behind it.
-__device__ __forceinline__ double wave_inclusive(double v) {
-  v = plus_moved<0x111, 0xF>(v);
-  v = plus_moved<0x112, 0xF>(v);
-  v = plus_moved<0x114, 0xF>(v);
-  v = plus_moved<0x118, 0xF>(v);
-  v = plus_moved<0x142, 0xA>(v);
-  return plus_moved<0x143, 0xC>(v);
 }
 
 // Inclusive sums over the workgroup's threads, of both weights.
@@ -266,6 +284,103 @@ __global__ __launch_bounds__(kThreads) void verify_draw(const shk_verify p, cons
   }
 }
 
+// A whole sequence in a workgroup: wave w has the values [w, w + 1) * 512 * STEPS,
+// a lane 8 of each 512.  The waves' sums say which of them holds the place, and
+// that one goes through its values again, which are still in its registers.
+template <int TYPE, int WAVES, int STEPS>
+__global__ __launch_bounds__(64 * WAVES) void verify_whole(const shk_verify p) {
+  __shared__ Sum parts[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long b = blockIdx.x;
+  const double uniform = p.uniforms[b * (p.drafts + 1) + p.drafts];
+  const long drafted = lane < (int)p.drafts ? token_of(p, b * p.drafts + lane) : -1;
+  const int length = p.lengths != nullptr ? p.lengths[b] : 0;
+  const int kept = kept_of<TYPE>(p, b);
+  const Row r = row_of(p, b, kept);
+  const long from = (long)wave * 512 * STEPS + lane * 8;
+  float have[STEPS][8], gone[STEPS][8];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) values8<TYPE>(p, r, from + i * 512, have[i], gone[i]);
+  Sum mine{0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const Sum w = weight_of(have[i][e], gone[i][e]);
+      mine.left += w.left, mine.all += w.all;
+    }
+  // what was read stays, not the weights made of it, which are twice as large
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(have[i][e]), "+v"(gone[i][e]));
+  mine.left = wave_inclusive(mine.left), mine.all = wave_inclusive(mine.all);
+  if (lane == 63) parts[wave] = mine;
+  __syncthreads();
+  Sum total{0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) total.left += parts[i].left, total.all += parts[i].all;
+  const bool rest = total.left > 0.0;
+  const double share = uniform * (rest ? total.left : total.all);
+  // the first wave whose running sum passes the share; the last that holds
+  // anything where a share of the whole sum, or more, was asked for
+  int at = -1;
+  bool passed = false;
+  double run = 0.0, carry = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    const double own = rest ? parts[i].left : parts[i].all;
+    if (own > 0.0 && !passed) at = i, carry = run, passed = run + own > share;
+    run += own;
+  }
+  if (wave != max(at, 0)) return;
+  long token = -1;
+  if (at >= 0) {
+    passed = false;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (passed) continue;
+      double values[8], mass = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Sum w = weight_of(have[i][e], gone[i][e]);
+        values[e] = rest ? w.left : w.all;
+        mass += values[e];
+      }
+      const double through = carry + wave_inclusive(mass);
+      double upto = through - mass;
+      int first = -1, last = -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        upto += values[e];
+        if (values[e] > 0.0) {
+          last = e;
+          if (first < 0 && upto > share) first = e;
+        }
+      }
+      // rounding can leave the running sum of a wave just below its own sum: the
+      // last value that holds anything, then
+      const unsigned long long passes = __ballot(first >= 0), holds = __ballot(last >= 0);
+      passed = passes != 0;
+      if (passed) {
+        const int l = __builtin_ctzll(passes);
+        token = ((long)at * STEPS + i) * 512 + l * 8 + __builtin_amdgcn_readlane(first, l);
+      } else if (holds != 0) {
+        const int l = 63 - __builtin_clzll(holds);
+        token = ((long)at * STEPS + i) * 512 + l * 8 + __builtin_amdgcn_readlane(last, l);
+      }
+      carry = __shfl(through, 63, 64);
+    }
+  }
+  if (lane <= (int)p.drafts) p.out[b * (p.drafts + 1) + lane] = lane < kept ? drafted : lane == kept ? token : -1;
+  if (lane == 0) {
+    p.kept[b] = kept;
+    if (p.lengths != nullptr) p.lengths[b] = length - (drafts_of(p, b) - kept);
+  }
+}
+
+constexpr long kWhole = 16 * 512 * 4;  // values that a workgroup's registers hold
+
 Pieces pieces_of(const shk_verify& a) {
   // one step each, more where a row has more steps than a workgroup threads
   const long steps = (a.vocab + kPiece - 1) / kPiece, each = (steps + kPieces - 1) / kPieces;
@@ -274,6 +389,12 @@ Pieces pieces_of(const shk_verify& a) {
 
 template <int TYPE>
 hipError_t launch(const shk_verify& a, hipStream_t s) {
+  const dim3 one((unsigned)a.batch);
+  if (a.vocab <= 4 * 512) hipLaunchKernelGGL((verify_whole<TYPE, 4, 1>), one, dim3(256), 0, s, a);
+  else if (a.vocab <= 16 * 512) hipLaunchKernelGGL((verify_whole<TYPE, 16, 1>), one, dim3(1024), 0, s, a);
+  else if (a.vocab <= 16 * 512 * 2) hipLaunchKernelGGL((verify_whole<TYPE, 16, 2>), one, dim3(1024), 0, s, a);
+  else if (a.vocab <= kWhole) hipLaunchKernelGGL((verify_whole<TYPE, 16, 4>), one, dim3(1024), 0, s, a);
+  if (a.vocab <= kWhole) return hipGetLastError();
   const Pieces pieces = pieces_of(a);
   hipLaunchKernelGGL((verify_sums<TYPE>), dim3(pieces.count, (unsigned)a.batch), dim3(kThreads), 0, s, a, pieces);
   if (hipError_t e = hipGetLastError()) return e;
@@ -284,6 +405,7 @@ hipError_t launch(const shk_verify& a, hipStream_t s) {
 }  // namespace
 
 int64_t verify_workspace(const shk_verify& a) {
+  if (a.vocab <= kWhole) return 0;
   return kept_bytes(a.batch) + a.batch * pieces_of(a).count * (int64_t)sizeof(Sum);
 }
 

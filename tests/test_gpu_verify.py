@@ -56,6 +56,22 @@ def test_coarse(device, batch, drafts, vocab, dtype, greedy):
     _check(device, target, draft, tokens.to(torch.int32), uniforms, counts)
 
 
+@pytest.mark.parametrize("greedy", [False, True])
+@pytest.mark.parametrize("vocab", [2047, 2048, 2049, 8192, 8193, 16384, 16385, 24001, 32767, 32768, 32769, 65537])
+def test_sizes_around_a_workgroup(device, vocab, greedy):
+    """Where another form of the kernel begins: shares at the start, on running sums, and at the end."""
+    g = torch.Generator().manual_seed(stable_seed("around", vocab, greedy))
+    target = _coarse(g, 5, 2, vocab)
+    draft = None if greedy else _coarse(g, 5, 1, vocab)
+    target[3, :, : vocab - 1] = 0.0  # one weight, the last
+    target[3, :, vocab - 1] = 0.25
+    target[4, :, 1:] = 0.0  # one, the first
+    target[4, :, 0] = 0.25
+    tokens = torch.randint(0, vocab, (5, 1), generator=g)
+    uniforms = torch.tensor([[1.0, 0.0], [1.0, 0.5], [1.0, 255 / 256], [1.0, 0.75], [1.0, 0.75]])
+    _check(device, target, draft, tokens, uniforms)
+
+
 @pytest.mark.parametrize("batch,vocab", [(3, 131072), (70, 32001)])
 def test_fine(device, batch, vocab):
     """Real probabilities: the drawn token's running sum passes the share, the one before does not, to

@@ -232,7 +232,8 @@ VERIFY = {"target": FAKE, "tb": 400, "tr": 100, "draft": FAKE, "db": 300, "dr": 
                                        ({"drafts": 64}, b"63 drafts"), ({"vocab": 0}, b"vocabulary"),
                                        ({"token_bytes": 2}, b"int32 or int64"), ({"target": 0}, b"non-null"),
                                        ({"tokens": 0}, b"non-null"), ({"out": FAKE + 4}, b"aligned"),
-                                       ({"work_bytes": 8}, b"workspace must hold"), ({"work": 0}, b"workspace must hold")])
+                                       ({"vocab": 10**6, "work_bytes": 8}, b"workspace must hold"),
+                                       ({"vocab": 10**6, "work": 0}, b"workspace must hold")])
 def test_verify_refusals(lib, bad, match):
     packed = verify._VERIFY.pack(*(VERIFY | bad).values())
     _refuses(lib, lib.amd_strix_halo_kernels_verify, (packed,), match)
