@@ -49,22 +49,28 @@ _QUANTIZE = struct.Struct("=13q")
 _MM = struct.Struct("=21q")
 
 
-def _kind(torch: Any, name: str, dtype: Any) -> int:
-    if dtype == torch.float8_e4m3fn:
-        return kt.FP8_E4M3
-    if dtype == torch.float8_e5m2:
-        return kt.FP8_E5M2
-    raise ValueError(f"{name} must have dtype torch.float8_e4m3fn or torch.float8_e5m2; got {dtype}")
+# of dtypes, filled at the first call
+_KINDS: dict[Any, int] = {}
+_SOURCES: dict[Any, int] = {}
 
 
-def _value_type(torch: Any, name: str, dtype: Any) -> int:
-    if dtype == torch.bfloat16:
-        return kt.SRC_BF16
-    if dtype == torch.float16:
-        return kt.SRC_F16
-    if dtype == torch.float32:
-        return kt.SRC_F32
-    raise ValueError(f"{name} must have dtype torch.bfloat16, torch.float16 or torch.float32; got {dtype}")
+def _fill(torch: Any) -> None:
+    _SOURCES.update({torch.bfloat16: kt.SRC_BF16, torch.float16: kt.SRC_F16, torch.float32: kt.SRC_F32})
+    _KINDS.update({torch.float8_e4m3fn: kt.FP8_E4M3, torch.float8_e5m2: kt.FP8_E5M2})
+
+
+def _kind(name: str, dtype: Any) -> int:
+    kind = _KINDS.get(dtype)
+    if kind is None:
+        raise ValueError(f"{name} must have dtype torch.float8_e4m3fn or torch.float8_e5m2; got {dtype}")
+    return kind
+
+
+def _value_type(name: str, dtype: Any) -> int:
+    source = _SOURCES.get(dtype)
+    if source is None:
+        raise ValueError(f"{name} must have dtype torch.bfloat16, torch.float16 or torch.float32; got {dtype}")
+    return source
 
 
 def quantize_fp8(x: Any, *, block_rows: int = 1, transpose: bool = False, dtype: Any = None,
@@ -81,37 +87,41 @@ def quantize_fp8(x: Any, *, block_rows: int = 1, transpose: bool = False, dtype:
     zero codes, so that what it is multiplied with becomes NaN.
     """
     torch = _torch()
-    if x.get_device() < 0:
+    index = x.get_device()
+    if index < 0:
         _require_device(torch, {"x": x})
     if stream is not None:
         with _on_stream(torch, x, stream):
             return quantize_fp8(x, block_rows=block_rows, transpose=transpose, dtype=dtype)
+    if not _KINDS:
+        _fill(torch)
     dtype = torch.float8_e4m3fn if dtype is None else dtype
-    kind, source = _kind(torch, "the result", dtype), _value_type(torch, "x", x.dtype)
+    kind, source = _kind("the result", dtype), _value_type("x", x.dtype)
     if block_rows not in (1, FP8_BLOCK):
         raise ValueError(f"block_rows must be 1 or {FP8_BLOCK}; got {block_rows}")
     if x.ndim != 2:
         raise ValueError(f"x must have shape (rows, cols); got {tuple(x.shape)}")
-    rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape  # of the operand
-    turn, given = bool(transpose), x
-    if x.stride(1) != 1 and x.shape[1] > 1:
-        if x.stride(0) != 1 and x.shape[0] > 1:
+    (m, n), (m_stride, n_stride) = x.shape, x.stride()
+    rows, cols = (n, m) if transpose else (m, n)  # of the operand
+    turn = bool(transpose)
+    if n_stride != 1 and n > 1:
+        if m_stride != 1 and m > 1:
             raise ValueError("x must be contiguous along rows or columns")
-        x, turn = x.t(), not turn
+        m, n, m_stride, turn = n, m, n_stride, not turn
     pitch = -(-cols // 16) * 16
-    codes = torch.empty((rows, pitch), dtype=dtype, device=x.device)
-    scales = torch.empty((-(-cols // FP8_BLOCK), -(-rows // block_rows)), dtype=torch.float32, device=x.device)
+    groups = rows if block_rows == 1 else -(-rows // FP8_BLOCK)
+    codes = x.new_empty((rows, pitch), dtype=dtype)
+    scales = x.new_empty_strided((groups, -(-cols // FP8_BLOCK)), (1, groups), dtype=torch.float32)
     if rows and cols:
-        stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
         lib = _verified_library()
-        index = x.get_device()
         _check(lib, lib.amd_strix_halo_kernels_fp8_quantize(
             index, _current_stream(torch, index),
-            _QUANTIZE.pack(x.data_ptr(), source, x.shape[0], x.shape[1], stride, turn, block_rows, kind,
-                           codes.data_ptr(), pitch, scales.data_ptr(), 1, scales.shape[1])))
-    codes, scales = codes if pitch == cols else codes[:, :cols], scales.t()
-    if given.requires_grad:
-        scales = _no_gradient(torch, "quantize_fp8", scales, given)
+            _QUANTIZE.pack(x.data_ptr(), source, m, n, m_stride if m > 1 else n, turn, block_rows, kind,
+                           codes.data_ptr(), pitch, scales.data_ptr(), 1, groups)))
+    if pitch != cols:
+        codes = codes[:, :cols]
+    if x.requires_grad:
+        scales = _no_gradient(torch, "quantize_fp8", scales, x)
     return codes, scales
 
 
@@ -138,17 +148,19 @@ def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None,
     if stream is not None:
         with _on_stream(torch, a, stream):
             return mm_fp8(a, b, a_scale=a_scale, b_scale=b_scale, out_dtype=out_dtype, out=out)
-    a_kind, b_kind = _kind(torch, "a", a.dtype), _kind(torch, "b", b.dtype)
+    if not _KINDS:
+        _fill(torch)
+    a_kind, b_kind = _kind("a", a.dtype), _kind("b", b.dtype)
     if a.ndim != 2 or b.ndim != 2 or a.shape[1] != b.shape[1]:
         raise ValueError(f"a and b must have shapes (M, K) and (N, K); got {tuple(a.shape)} and {tuple(b.shape)}")
-    m, k = a.shape
-    n = b.shape[0]
-    if k > 1 and (a.stride(1) != 1 or b.stride(1) != 1):
+    (m, k), n = a.shape, b.shape[0]
+    (a_pitch, a_step), (b_pitch, b_step) = a.stride(), b.stride()
+    if k > 1 and (a_step != 1 or b_step != 1):
         raise ValueError("rows of a and b must be contiguous")
     blocks = -(-k // FP8_BLOCK)
-    for name, t in (("a_scale", a_scale), ("b_scale", b_scale)):
-        if t.dtype != torch.float32:
-            raise ValueError(f"{name} must have dtype torch.float32; got {t.dtype}")
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        name, t = ("a_scale", a_scale) if a_scale.dtype != torch.float32 else ("b_scale", b_scale)
+        raise ValueError(f"{name} must have dtype torch.float32; got {t.dtype}")
     if a_scale.shape != (m, blocks):
         raise ValueError(f"a_scale must have shape {(m, blocks)} == (M, ceil(K/128)); got {tuple(a_scale.shape)}")
     if b_scale.shape == (-(-n // FP8_BLOCK), blocks):
@@ -160,36 +172,35 @@ def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None,
                          f"{(n, blocks)} == (N, ceil(K/128)); got {tuple(b_scale.shape)}")
     if out is None:
         out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
-        out_type = _value_type(torch, "the result", out_dtype)
+        out_type, out_stride = _value_type("the result", out_dtype), n
         out = a.new_empty((m, n), dtype=out_dtype)
     else:
-        out_type = _value_type(torch, "out", out.dtype)
+        out_type, out_stride = _value_type("out", out.dtype), out.stride(0) if m > 1 else n
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out must have dtype {out_dtype}; got {out.dtype}")
-        if out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        if out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or out_stride < n:
             raise ValueError(f"out must have shape {(m, n)} and contiguous rows; got {tuple(out.shape)}")
     if m and n:
-        a_pitch, b_pitch = a.stride(0) if m > 1 else k, b.stride(0) if n > 1 else k
+        if m == 1:
+            a_pitch = k
+        if n == 1:
+            b_pitch = k
         a_at, b_at = a.data_ptr(), b.data_ptr()
         lib = _verified_library()
-
-        def args(at: int, nbytes: int) -> bytes:
-            return _MM.pack(a_at, a_pitch, a_kind, b_at, b_pitch, b_kind, a_scale.data_ptr(), *a_scale.stride(),
-                            b_scale.data_ptr(), *b_scale.stride(), b_rows, m, n, k, out.data_ptr(),
-                            out.stride(0) if m > 1 else n, out_type, at, nbytes)
-
+        given = (a_at, a_pitch, a_kind, b_at, b_pitch, b_kind, a_scale.data_ptr(), *a_scale.stride(),
+                 b_scale.data_ptr(), *b_scale.stride(), b_rows, m, n, k, out.data_ptr(), out_stride, out_type)
         key = (m, n, k, out_type, (a_at | (a_pitch if m > 1 else 0)) % 16 == 0,
                (b_at | (b_pitch if n > 1 else 0)) % 16 == 0)
         nbytes = _WORKSPACES.get(key)
         if nbytes is None:
-            nbytes = lib.amd_strix_halo_kernels_fp8_mm_workspace(args(0, 0))
+            nbytes = lib.amd_strix_halo_kernels_fp8_mm_workspace(_MM.pack(*given, 0, 0))
             if nbytes < 0:
                 _check(lib, 1)
             if len(_WORKSPACES) < 4096:
                 _WORKSPACES[key] = nbytes
         work = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _check(lib, lib.amd_strix_halo_kernels_fp8_mm(index, _current_stream(torch, index),
-                                                      args(work.data_ptr() if nbytes else 0, nbytes)))
+        _check(lib, lib.amd_strix_halo_kernels_fp8_mm(
+            index, _current_stream(torch, index), _MM.pack(*given, 0 if work is None else work.data_ptr(), nbytes)))
     if a_scale.requires_grad or b_scale.requires_grad:
         return _no_gradient(torch, "mm_fp8", out, a_scale, b_scale)
     return out
