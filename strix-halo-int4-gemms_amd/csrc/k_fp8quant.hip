@@ -3,15 +3,17 @@
 // L = 448 (e4m3) or 57344 (e5m2).  One pass over memory: a block's values stay
 // in registers between the maximum and the codes.
 //
-// fp8_rows: blocks of one row by 128 columns; 16 lanes hold one, 8 values each.
+// fp8_rows: blocks of one row by 128 columns; 16 lanes hold one, 8 values each (of
+// ROWS rows).
 // fp8_tile: a workgroup holds 128 rows by 128 columns, a thread 8 rows by 8
 // columns; for blocks of 128 x 128, and for the operand x^T, whose blocks of one
 // row are x's columns.  Transposed codes pass through LDS in units of 8 bytes
 // (8 rows of one column), unit u of column c at c * 128 + 8 * (u ^ (c / 8)): both
 // sides are spread over the banks (18% of the LDS's cycles are conflicts, and it is
 // busy 11% of the time).
-// Bound by memory.  11008 x 4096 bf16 (135 MB): rows 31 us, 4.4 TB/s; tiles with
-// the transpose 35 to 38, whose stores are runs of 128 bytes a column.
+// Bound by memory.  11008 x 4096 bf16 (135 MB): rows 27 us, 5 TB/s; tiles 26 to 29,
+// transposed too.  16-bit values wait in registers as they are: as f32 they take
+// twice as many, a third of the tiles waits for the others, and it was 35 to 38.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,35 +38,37 @@ struct Convert {
 template <int TYPE>
 constexpr int kSize = TYPE == SHK_SRC_F32 ? 4 : 2;
 
+// Eight values as they are in memory.
 template <int TYPE>
-__device__ __forceinline__ float value_of(const uint8_t* x, long i) {
-  if constexpr (TYPE == SHK_SRC_F32) return reinterpret_cast<const float*>(x)[i];
-  const uint16_t h = reinterpret_cast<const uint16_t*>(x)[i];
-  return TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-}
+struct Eight {
+  u4 u[kSize<TYPE> / 2];
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (TYPE == SHK_SRC_F32) return __uint_as_float(u[e / 4][e % 4]);
+    const uint16_t h = (uint16_t)(u[0][e / 2] >> (16 * (e % 2)));
+    return TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+  }
+};
 
-// x[at .. at + 8); `count` of them lie inside.  Whole ones come in vectors, of any
-// alignment.
+// x[at .. at + 8), zeros behind the `count` of them that lie inside.  Whole ones
+// come in vectors, of any alignment.
 template <int TYPE>
-__device__ __forceinline__ void load8(const uint8_t* x, long at, long count, float (&v)[8]) {
+__device__ __forceinline__ Eight<TYPE> load8(const uint8_t* x, long at, long count) {
+  Eight<TYPE> v;
   if (count >= 8) {
     const any_u4* src = reinterpret_cast<const any_u4*>(x + at * kSize<TYPE>);
-    u4 u[kSize<TYPE> / 2];
 #pragma unroll
-    for (int i = 0; i < kSize<TYPE> / 2; ++i) u[i] = src[i];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (TYPE == SHK_SRC_F32) {
-        v[e] = __uint_as_float(u[e / 4][e % 4]);
-      } else {
-        const uint16_t h = (uint16_t)(u[0][e / 2] >> (16 * (e % 2)));
-        v[e] = TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-      }
-    }
-    return;
+    for (int i = 0; i < kSize<TYPE> / 2; ++i) v.u[i] = src[i];
+    return v;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = e < count ? value_of<TYPE>(x, at + e) : 0.f;
+  for (int i = 0; i < kSize<TYPE> / 2; ++i) v.u[i] = u4{0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < count) {
+      if constexpr (TYPE == SHK_SRC_F32) v.u[e / 4][e % 4] = reinterpret_cast<const uint32_t*>(x)[at + e];
+      else v.u[0][e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[at + e] << (16 * (e % 2));
+    }
+  return v;
 }
 
 // Magnitudes compare as integers: a NaN is larger than an infinity, and stays.
@@ -121,26 +125,32 @@ __device__ __forceinline__ void store8(uint8_t* to, const uint32_t (&w)[2], long
     if (e < count) to[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
 }
 
-template <int TYPE, int KIND>
+template <int TYPE, int KIND, int ROWS>
 __global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
   const long blocks = (p.cols + 127) / 128;
   const long unit = (long)blockIdx.x * 16 + threadIdx.x / 16;
   const int part = threadIdx.x % 16;
-  if (unit >= p.rows * blocks) return;  // all 16 lanes of a block
-  const long row = unit / blocks, block = unit - row * blocks;
+  const long group = unit / blocks, block = unit - group * blocks, row = group * ROWS;
+  if (row >= p.rows) return;  // all 16 lanes of a block
   const long at = block * 128 + part * 8;
-  float v[8];
-  load8<TYPE>(p.x, row * p.stride + at, p.cols - at, v);
-  uint32_t most = 0;
+  Eight<TYPE> x[ROWS];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e]));
+  for (int i = 0; i < ROWS; ++i) x[i] = load8<TYPE>(p.x, (row + i) * p.stride + at, row + i < p.rows ? p.cols - at : 0);
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
-  const float s = scale_of<KIND>(most);
-  uint32_t w[2];
-  codes8<KIND>(v, s, 1.f / s, normal_scale(s), w);
-  if (at < p.cols) store8(p.codes + row * p.pitch + at, w, p.cols - at);
-  if (part == 0) p.scales[row * p.s_row + block * p.s_block] = s;
+  for (int i = 0; i < ROWS; ++i) {
+    const float v[8] = {x[i][0], x[i][1], x[i][2], x[i][3], x[i][4], x[i][5], x[i][6], x[i][7]};
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e]));
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+    const float s = scale_of<KIND>(most);
+    uint32_t w[2];
+    codes8<KIND>(v, s, 1.f / s, normal_scale(s), w);
+    if (row + i >= p.rows) break;
+    if (at < p.cols) store8(p.codes + (row + i) * p.pitch + at, w, p.cols - at);
+    if (part == 0) p.scales[(row + i) * p.s_row + block * p.s_block] = s;
+  }
 }
 
 template <int TYPE, int KIND, bool TURN, bool WHOLE>  // WHOLE: one scale for the tile
@@ -150,11 +160,11 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int cg = threadIdx.x % 16, rg = threadIdx.x / 16;
   const long c0 = (long)blockIdx.x * 128, r0 = (long)blockIdx.y * 128;
-  float v[8][8];
+  Eight<TYPE> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const long row = r0 + rg * 8 + i, at = c0 + cg * 8;
-    load8<TYPE>(p.x, row * p.stride + at, row < p.rows ? p.cols - at : 0, v[i]);
+    v[i] = load8<TYPE>(p.x, row * p.stride + at, row < p.rows ? p.cols - at : 0);
   }
   uint32_t top[8];
 #pragma unroll
@@ -165,6 +175,10 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
     top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 16, 64));
     top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 32, 64));
   }
+  // values of 16 bits stay as they came, not as twice the registers of f32
+  if constexpr (TYPE != SHK_SRC_F32)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(v[i].u[0]));
   if constexpr (WHOLE) {
 #pragma unroll
     for (int e = 1; e < 8; ++e) top[0] = max(top[0], top[e]);
@@ -200,8 +214,9 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long row = r0 + rg * 8 + i, at = c0 + cg * 8;
+      const float line[8] = {v[i][0], v[i][1], v[i][2], v[i][3], v[i][4], v[i][5], v[i][6], v[i][7]};
       uint32_t w[2];
-      codes8<KIND>(v[i], s[0], inv[0], plain, w);
+      codes8<KIND>(line, s[0], inv[0], plain, w);
       if (row < p.rows && at < p.cols) store8(p.codes + row * p.pitch + at, w, p.cols - at);
     }
   } else {
@@ -237,8 +252,15 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
 template <int TYPE, int KIND>
 hipError_t launch(const Convert& p, bool turn, bool whole, hipStream_t s) {
   if (!turn && !whole) {
-    const long units = p.rows * ((p.cols + 127) / 128);
-    hipLaunchKernelGGL((fp8_rows<TYPE, KIND>), dim3((unsigned)((units + 15) / 16)), dim3(256), 0, s, p);
+    // two rows a lane of 16-bit values where there are blocks for several rounds of
+    // the chip: 8192 x 4096 bf16 21.4 us and 24.7 with one, 4096 x 4096 12.9 and
+    // 13.2, but 1024 x 4096 6.1 and 5.5; f32 gains nothing (29.5 and 29.3)
+    const long blocks = (p.cols + 127) / 128;
+    const bool two = TYPE != SHK_SRC_F32 && p.rows * blocks >= 1 << 17;
+    const long units = (two ? (p.rows + 1) / 2 : p.rows) * blocks;
+    const dim3 grid((unsigned)((units + 15) / 16));
+    if (two) hipLaunchKernelGGL((fp8_rows<TYPE, KIND, TYPE == SHK_SRC_F32 ? 1 : 2>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((fp8_rows<TYPE, KIND, 1>), grid, dim3(256), 0, s, p);
   } else {
     const dim3 grid((unsigned)((p.cols + 127) / 128), (unsigned)((p.rows + 127) / 128));
     if (!turn) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, false, true>), grid, dim3(256), 0, s, p);

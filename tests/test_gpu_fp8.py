@@ -133,6 +133,18 @@ def test_quantize(device, rows, cols, kind, dtype):
 # Values that are no numbers, layouts, streams
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(131075, 100), (70001, 203)])
+def test_quantize_rows_in_pairs(device, rows, cols, dtype):
+    """Many blocks are taken two rows at a time: the same codes and scales as those of parts of the rows."""
+    x = torch.randn((rows, cols), generator=_gen("pairs", rows, cols, dtype)).to(dtype).to(device)
+    codes, scales = shk.quantize_fp8(x)
+    for at in range(0, rows, 40000):
+        want, want_scales = shk.quantize_fp8(x[at : at + 40000])
+        assert torch.equal(codes[at : at + 40000].view(torch.uint8), want.view(torch.uint8))
+        assert torch.equal(scales[at : at + 40000], want_scales)
+
+
 @pytest.mark.parametrize("kind", [E4M3, E5M2])
 def test_quantize_bad_blocks(device, kind):
     """A block with an infinity or a NaN has that as its scale and zero codes; its neighbours do not see it;
