@@ -135,8 +135,8 @@ def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None,
     ceil(K / 128)] and ``b_scale`` [ceil(N / 128), ceil(K / 128)] (a weight's
     blocks) or [N, ceil(K / 128)], f32 of any strides.  Returns [M, N] in
     ``out_dtype`` (bf16, the default, f16 or f32).  Sums are f32: inside a
-    block of K by the matrix unit, over the blocks in order of K, or, where few
-    tiles share a long K, in order of its parts; rounded once at the end.
+    block of K by the matrix unit, over the blocks in an order that follows from
+    the sizes (the same call has the same bits); rounded once at the end.
     Operands whose rows do not all start on 16 bytes are copied first; the codes
     of ``quantize_fp8`` do.
     """

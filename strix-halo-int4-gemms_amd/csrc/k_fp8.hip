@@ -28,10 +28,12 @@ namespace shk {
 namespace {
 
 
-template <int BM_, int BN_, int WM_, int WN_, int P_>
+// KG groups of WM x WN waves, each with a ring of P stages, take the blocks of K
+// in turn.
+template <int BM_, int BN_, int WM_, int WN_, int P_, int KG_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, P = P_;
-  static constexpr int NW = WM * WN, THREADS = 64 * NW;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, P = P_, KG = KG_;
+  static constexpr int NW = WM * WN, THREADS = 64 * NW * KG;
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // MFMA tiles of a wave
   static constexpr int SA = (BM + 63) / 64 * 64;              // scales of a stage, whole DMAs
   static constexpr int DATA = (BM + BN) * 128;
@@ -41,7 +43,9 @@ struct Tile {
   static constexpr int SCALES = (SA + BN) / 64;               // 256-byte DMAs of a stage
   static constexpr int SCALES_PER_WAVE = (SCALES + NW - 1) / NW;
   static constexpr int ISSUED = PER_WAVE + SCALES_PER_WAVE;   // by a wave and stage
-  static_assert(BM % 16 == 0 && BN % 64 == 0 && P * STAGE <= 160 * 1024, "");
+  static constexpr int RING = P * STAGE;
+  static_assert(BM % 16 == 0 && BN % 64 == 0 && KG * RING <= 160 * 1024, "");
+  static_assert((KG - 1) * BM * BN * 4 <= KG * RING, "sums of the other groups");
 };
 
 __device__ __forceinline__ void stage_barrier() {
@@ -50,14 +54,17 @@ __device__ __forceinline__ void stage_barrier() {
 
 template <class T, int KIND_A, int KIND_B, bool BROW, bool WIDE>
 __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Product p) {
-  __shared__ __align__(16) uint8_t lds[T::P * T::STAGE];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __align__(16) uint8_t lds[T::KG * T::RING];
+  const int lane = threadIdx.x & 63, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = T::KG == 1 ? 0 : wave_id / T::NW, wave = wave_id - kg * T::NW;
+  uint8_t* ring = lds + kg * T::RING;
   int tm, tn;
   tile_of(p, 1024 / T::BM, tm, tn);
   const int m0 = tm * T::BM, n0 = tn * T::BN;
   const int first = blockIdx.y * p.per_split;
   const int blocks = (p.k + 127) >> 7;
-  const int count = min(p.per_split, blocks - first);
+  const int all = min(p.per_split, blocks - first);
+  const int steps = (all + T::KG - 1) / T::KG, count = (all - kg + T::KG - 1) / T::KG;  // of all groups, of this one
 
   // where this wave's pieces of a stage come from
   const int rows_a = min(T::BM, p.m - m0), rows_b = min(T::BN, p.n - n0);
@@ -90,8 +97,9 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Produc
                           : (uint32_t)((((n0 + min(row, rows_b - 1)) >> p.b_shift) - s0) * p.sb_row * 4);
     to_s[c] = T::DATA + piece * 256;
   }
-  const uint32_t base = lds_address(lds);
-  auto issue = [&](int kb, int slot) {
+  const uint32_t base = lds_address(ring);
+  auto issue = [&](int i, int slot) {
+    const int kb = first + i * T::KG + kg;
     const uint32_t at = base + slot * T::STAGE;
 #pragma unroll
     for (int c = 0; c < T::PER_WAVE; ++c)
@@ -122,7 +130,7 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Produc
     v4f sb[BROW ? T::NT : 1];
   };
   auto read = [&](int slot, Stage& f) {
-    const uint8_t* st = lds + slot * T::STAGE;
+    const uint8_t* st = ring + slot * T::STAGE;
     auto fragment = [&](uint32_t at) {
       return __builtin_shufflevector(*reinterpret_cast<const v4i*>(st + at), *reinterpret_cast<const v4i*>(st + (at ^ 64u)),
                                      0, 1, 2, 3, 4, 5, 6, 7);
@@ -154,12 +162,12 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Produc
       }
     }
   };
-  // zeros behind K in its last stage
+  // zeros behind K in its last stage, which one group has
   auto clear_tail = [&](int i, int slot) {
-    const int left = p.k - (first + i) * 128;
-    if (left >= 128) return;
-    uint8_t* st = lds + slot * T::STAGE;
-    for (int u = threadIdx.x; u < (T::BM + T::BN) * 8; u += T::THREADS) {
+    if (i + 1 < steps || p.k - (first + all) * 128 >= 0) return;
+    const int left = i + 1 == count && (all - 1) % T::KG == kg ? p.k - (first + all - 1) * 128 : 128;
+    uint8_t* st = ring + slot * T::STAGE;
+    for (int u = wave * 64 + lane; u < (T::BM + T::BN) * 8; u += 64 * T::NW) {
       const int row = u >> 3, unit = (u & 7) ^ (row & 7), keep = left - unit * 16;
       if (keep >= 16) continue;
       uint32_t* w = reinterpret_cast<uint32_t*>(st + u * 16);
@@ -174,8 +182,8 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Produc
 
 #pragma unroll
   for (int s = 0; s < T::P; ++s)
-    if (s < count) issue(first + s, s);
-  if (count > 0) {
+    if (s < count) issue(s, s);
+  if (steps > 0) {
     if (T::P <= count) wait_vmcnt<(T::P - 1) * T::ISSUED>();
     else wait_vmcnt<0>();
     stage_barrier();
@@ -183,27 +191,45 @@ __global__ __launch_bounds__(T::THREADS) void fp8_product_kernel(const Fp8Produc
   }
   // Stage i + 1 is read while stage i is multiplied.  The barrier of a stage says
   // that stage i + 1 has come and that every wave has read stage i, whose slot
-  // then takes stage i + P.
+  // then takes stage i + P.  A group whose stages are fewer than the others' takes
+  // part in the barriers.
   Stage even, odd;
   int slot = 0;
   auto step = [&](int i, const Stage& now, Stage& next) {
-    if (i + 1 < count) {
+    if (i + 1 < steps) {
       if (i + T::P - 1 < count) wait_vmcnt<(T::P - 2) * T::ISSUED>();
       else wait_vmcnt<0>();
       stage_barrier();
-      if (i + T::P < count) issue(first + i + T::P, slot);
+      if (i + T::P < count) issue(i + T::P, slot);
       slot = slot == T::P - 1 ? 0 : slot + 1;
       clear_tail(i + 1, slot);
-      read(slot, next);
+      if (T::KG == 1 || i + 1 < count) read(slot, next);
     }
-    multiply(now);
+    if (T::KG == 1 || i < count) multiply(now);
   };
   if (count > 0) read(0, even);
-  for (int i = 0; i < count; i += 2) {
+  for (int i = 0; i < steps; i += 2) {
     step(i, even, odd);
-    if (i + 1 < count) step(i + 1, odd, even);
+    if (i + 1 < steps) step(i + 1, odd, even);
   }
 
+  if constexpr (T::KG > 1) {  // the groups' sums, in their order
+    stage_barrier();
+    v4f* sums = reinterpret_cast<v4f*>(lds) + (wave * T::MT * T::NT) * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < T::MT; ++x)
+#pragma unroll
+      for (int j = 0; j < T::NT; ++j)
+        if (kg > 0) sums[((kg - 1) * T::NW * T::MT * T::NT + x * T::NT + j) * 64] = acc[x][j];
+    stage_barrier();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 1; g < T::KG; ++g)
+#pragma unroll
+      for (int x = 0; x < T::MT; ++x)
+#pragma unroll
+        for (int j = 0; j < T::NT; ++j) acc[x][j] += sums[((g - 1) * T::NW * T::MT * T::NT + x * T::NT + j) * 64];
+  }
 #pragma unroll
   for (int x = 0; x < T::MT; ++x) {
     const int m = m0 + (wm * T::MT + x) * 16 + row_in;
@@ -248,7 +274,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* src, long 
   *reinterpret_cast<u4*>(dst + row * to + c) = v;
 }
 
-enum Kind { kFew, kTile64, kTile128, kBig, kWide };
+enum Kind { kFew, kTile64, kTile64Two, kTile128, kBig, kWide };
 
 struct Plan {
   Kind kind;
@@ -266,16 +292,22 @@ bool loose(const void* x, int64_t pitch, int64_t rows) {
 // with all CUs busy, measured: 64 x 64 tiles 0.62 us for 512 workgroups, 64 x 128
 // 0.95 us for 512, 256 x 256 1.45 us for 256.  f32 results: 64 x 64 0.8 to 0.95,
 // 128 x 128 1.4 for 256 workgroups and 2.2 for 512.
-//  * Up to 32 rows b is streamed past them: 16 x 11008 x 4096 in 11.7 us, by 64 x
-//    64 tiles in 18.  Up to 64 rows where 16 columns a workgroup leave each CU one:
-//    64 x 4096 x 4096 in 12.6 us (tiles: 15.9), but 64 x 11008 x 4096 in 20.3 (17.5).
-//  * One round of 64 x 64 tiles: 333 x 1408 x 2048 in 9.8 us, by 64 x 128 in 13.5;
-//    512 x 4096 x 4096 in 20.7 and 24.4.
+//  * Few rows: b is streamed past them.  A CU takes in what it multiplies at 35 to
+//    41 GB/s, a's rows for every 16 to 64 columns with it, so this is for short K:
+//    16 rows 512 x 4096 5.8 us (tiles 8.3), 512 x 14336 14.9 (11.9), 4096 x 14336
+//    15.8 (16.8), 11008 x 14336 36 (41); 32 rows 4096 x 4096 8.4 (11.1), 4096 x
+//    14336 22 (17.5), 11008 x 4096 15.1 (14.1); 64 rows 4096 x 1024 5.5 (6.3), 512 x
+//    4096 12.3 (9.8).
+//  * One round of 64 x 64 tiles: 333 x 1408 x 2048 in 8.4 us, by 64 x 128 in 13.5;
+//    512 x 4096 x 4096 in 20.7 and 24.4.  Where each has a CU, by two groups of
+//    waves that share K: 256 x 4096 x 4096 in 13.0 us (one group: 17.4), 333 x 1408
+//    x 2048 in 8.4 (10.2), 500 x 512 x 512 in 4.9 (4.8).
 //  * Else the cheaper of the larger ones: 1024 x 4096 x 4096 in 30.5 by 64 x 128 and
 //    43 by 256 x 256, 4096 x 4096 x 4096 in 110 and 65.  f32: 128 x 128 from more
 //    than half a workgroup a CU on, 1024 x 4096 x 4096 in 49 us (64 x 64: 61).
-// K is cut where tiles leave half the CUs idle, into parts of at least 8 stages, so
-// that the join (about 4 us) is less than what it saves: 64 x 512 x 14336.
+// K is cut where tiles leave half the CUs idle, into parts of at least 8 stages and
+// from 24 on, so that the join (about 4 us) is less than what it saves: 128 x 512 x
+// 4096 in 10.1 us (whole 11.8), but 128 x 512 x 2048 in 9.2 (7.9).
 Plan plan_of(const shk_fp8_mm& a) {
   Plan r{};
   const int blocks = (int)((a.k + 127) / 128);
@@ -284,7 +316,9 @@ Plan plan_of(const shk_fp8_mm& a) {
   const int64_t small = tiles(64, 64);
   if (a.k == 0) {
     r.kind = kTile64;  // asks for no stage
-  } else if (a.m <= 32 || (a.m <= 64 && a.n <= 4096)) {
+  } else if (a.m <= 16   ? a.n > 2048 || blocks <= 80
+             : a.m <= 32 ? blocks <= (a.n <= 8192 ? 40 : 16)
+                         : a.m <= 64 && a.n <= 4096 && blocks <= 16) {
     r.kind = kFew;
   } else if (wide) {
     r.kind = tiles(128, 128) > 128 ? kWide : kTile64;
@@ -294,7 +328,8 @@ Plan plan_of(const shk_fp8_mm& a) {
     const double tile128 = 0.95 * ((tiles(64, 128) + 511) / 512), big = 1.45 * ((tiles(256, 256) + 255) / 256);
     r.kind = big < tile128 ? kBig : kTile128;
   }
-  r.splits = r.kind == kTile64 && small <= 128 ? (int)std::max<int64_t>(1, std::min<int64_t>(256 / small, blocks / 8)) : 1;
+  r.splits = r.kind == kTile64 && small <= 128 && blocks >= 24 ? (int)std::max<int64_t>(1, std::min<int64_t>(256 / small, blocks / 8)) : 1;
+  if (r.kind == kTile64 && small * r.splits <= 256 && blocks > 1) r.kind = kTile64Two;
   r.per_split = std::max(1, (blocks + r.splits - 1) / r.splits);
   r.splits = std::max(1, (blocks + r.per_split - 1) / r.per_split);
   // the copies to LDS are of whole 16 bytes; loads to registers are not
@@ -316,8 +351,9 @@ hipError_t launch(Fp8Product& p, hipStream_t s) {
 }
 
 // 64 x 64 tiles take f32 results too.
-typedef Tile<64, 64, 2, 2, 4> Tile64;
-typedef Tile<64, 128, 2, 2, 3> Tile128;
+typedef Tile<64, 64, 2, 2, 4, 1> Tile64;
+typedef Tile<64, 64, 2, 2, 4, 2> Tile64Two;
+typedef Tile<64, 128, 2, 2, 3, 1> Tile128;
 
 template <class T, int KIND_A, int KIND_B>
 hipError_t launch_rows(Fp8Product& p, hipStream_t s) {
@@ -371,6 +407,7 @@ hipError_t launch_fp8_mm(const shk_fp8_mm& a, hipStream_t s) {
   const bool e5_a = a.a_kind == SHK_FP8_E5M2, e5_b = a.b_kind == SHK_FP8_E5M2;
   hipError_t e;
   if (r.kind == kFew) e = launch_fp8_few(p, e5_a, e5_b, s);
+  else if (r.kind == kTile64Two) e = launch_kinds<Tile64Two>(p, e5_a, e5_b, s);
   else if (r.kind == kTile64) e = launch_kinds<Tile64>(p, e5_a, e5_b, s);
   else if (r.kind == kTile128) e = launch_kinds<Tile128>(p, e5_a, e5_b, s);
   else if (r.kind == kBig) e = launch_fp8_big(p, e5_a, e5_b, s);

@@ -60,6 +60,26 @@ def test_product(device, m, n, k, b_rows):
     _check(got, a, b, sa, sb)
 
 
+# 64 x 64 tiles by one group of waves, by two (an odd and an even number of blocks,
+# with and without an end, K whole and in parts, the last of one block), and both
+# sides of where few rows give way to tiles
+GROUPS = [(700, 1900, 100), (700, 1900, 900), (65, 200, 129), (65, 200, 256), (65, 200, 300), (130, 70, 384), (66, 200, 640),
+          (65, 200, 2944), (65, 200, 3100), (65, 200, 9324), (16, 600, 10240), (16, 600, 10300), (32, 600, 5120),
+          (32, 600, 5200), (20, 8300, 2048), (20, 8300, 2100), (60, 300, 2048), (60, 300, 2060)]
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", GROUPS)
+def test_groups_of_waves(device, m, n, k, out_dtype):
+    a, b, sa, sb = _case(_gen("groups", m, n, k), m, n, k, 1)
+    dev = [t.to(device) for t in (a, b, sa, sb)]
+    got = shk.mm_fp8(*dev[:2], a_scale=dev[2], b_scale=dev[3], out_dtype=out_dtype)
+    rows = torch.arange(0, m, 1 if m < 100 else 7)
+    _check(got[rows.to(device)], a[rows], b, sa[rows], sb)
+    again = shk.mm_fp8(*dev[:2], a_scale=dev[2], b_scale=dev[3], out_dtype=out_dtype)
+    assert torch.equal(got, again)
+
+
 # tiles of 64 x 128, of 256 x 256 (K of no whole block, one, an odd and an even
 # number, with and without an end), and the f32 results' own of 128 x 128
 LARGE = [(1000, 3000, 200), (2500, 2700, 100), (2600, 2560, 128), (2500, 2505, 384), (2304, 2568, 300),
