@@ -10,8 +10,10 @@
 // vector unit: conversions and, where every row of b has its own scale, two
 // operations a value and block make as many cycles as the MFMAs, and by power.
 // 4096 x 4096 x 8064: 258 to 313 us from box to box, 1050 TFLOP/s at most, clock
-// 1.75 GHz, matrix unit 48%.  Dropped: widening or folding between the MFMAs (269
-// to 281 us), copies spread over the stage (no gain).
+// 1.75 GHz, matrix unit 48%.  Power is what holds it: with operands of one value
+// 204 to 218 us, and an order fixed step by step, folds and conversions under the
+// next MFMAs, took those to 193 but random ones from 246 to 250 only, and spilled
+// where rows of b have scales.  Dropped too: copies spread over the stage.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
