@@ -80,7 +80,8 @@ def quantize_fp8(x: Any, *, block_rows: int = 1, transpose: bool = False, dtype:
 
     Returns ``(codes, scales)`` of the operand, x or x^T, [R, C]: codes [R, C]
     in ``dtype`` (``torch.float8_e4m3fn``, the default, or
-    ``torch.float8_e5m2``), each row on 16 bytes, and f32 scales
+    ``torch.float8_e5m2``), each row on 16 bytes, on 128 where C is above 1024
+    (what lies between two rows is not written), and f32 scales
     [ceil(R / block_rows), ceil(C / 128)] (stored with the blocks of one row
     ``ceil(R / block_rows)`` apart), ``block_rows`` 1 or 128.  A block of zeros
     has scale 0; one that holds an infinity or a NaN has that as its scale and
@@ -108,7 +109,9 @@ def quantize_fp8(x: Any, *, block_rows: int = 1, transpose: bool = False, dtype:
         if m_stride != 1 and m > 1:
             raise ValueError("x must be contiguous along rows or columns")
         m, n, m_stride, turn = n, m, n_stride, not turn
-    pitch = -(-cols // 16) * 16
+    # rows on whole lines where that adds little: a product with K of 8111 takes 278 us
+    # instead of 292, with 2064 180 instead of 190
+    pitch = -(-cols // 128) * 128 if cols > 1024 else -(-cols // 16) * 16
     groups = rows if block_rows == 1 else -(-rows // FP8_BLOCK)
     codes = x.new_empty((rows, pitch), dtype=dtype)
     scales = x.new_empty_strided((groups, -(-cols // FP8_BLOCK)), (1, groups), dtype=torch.float32)

@@ -153,6 +153,24 @@ __global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
   }
 }
 
+// Transposed codes of column c of a tile, 16 rows of it, from LDS.
+__device__ __forceinline__ void store_turned(const Convert& p, const uint8_t* lds, int c, int piece, long c0, long r0) {
+  const int g = c / 8;
+  uint4 w = *reinterpret_cast<const uint4*>(lds + c * 128 + 16 * (piece ^ (g >> 1)));
+  if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+  const long out = c0 + c, at = r0 + piece * 16, count = p.rows - at;
+  if (out >= p.cols || count <= 0) return;
+  uint8_t* to = p.codes + out * p.pitch + at;
+  if (count >= 16) {
+    *reinterpret_cast<any_u4*>(to) = u4{w.x, w.y, w.z, w.w};
+    return;
+  }
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (e < count) to[e] = (uint8_t)(u[e / 4] >> (8 * (e % 4)));
+}
+
 template <int TYPE, int KIND, bool TURN, bool WHOLE>  // WHOLE: one scale for the tile
 __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
   __shared__ __align__(16) uint8_t lds[TURN ? 128 * 128 : 16];
@@ -230,22 +248,95 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
     }
     __syncthreads();
 #pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-      const int c = pass * 32 + threadIdx.x / 8, piece = threadIdx.x % 8, g = c / 8;
-      uint4 w = *reinterpret_cast<const uint4*>(lds + c * 128 + 16 * (piece ^ (g >> 1)));
-      if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
-      const long out = c0 + c, at = r0 + piece * 16, count = p.rows - at;
-      if (out >= p.cols || count <= 0) continue;
-      uint8_t* to = p.codes + out * p.pitch + at;
-      if (count >= 16) {
-        *reinterpret_cast<any_u4*>(to) = u4{w.x, w.y, w.z, w.w};
-      } else {
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    for (int pass = 0; pass < 4; ++pass) store_turned(p, lds, pass * 32 + threadIdx.x / 8, threadIdx.x % 8, c0, r0);
+  }
+}
+
+// The same with 16 waves, a thread 8 rows by 2 columns, for few tiles: a CU then has
+// one or two, whose loads and conversions are what takes the time.
+template <int TYPE, int KIND, bool TURN, bool WHOLE>
+__global__ __launch_bounds__(1024) void fp8_tile_thin(const Convert p) {
+  __shared__ __align__(16) uint8_t lds[TURN ? 128 * 128 : 16];
+  __shared__ __align__(16) uint32_t tops[16][WHOLE ? 4 : 128];
+  const int lane = threadIdx.x & 63, rg = threadIdx.x >> 6, col = 2 * lane;
+  const long c0 = (long)blockIdx.x * 128, r0 = (long)blockIdx.y * 128, count = p.cols - c0 - col;
+  float v[2][8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (e < count) to[e] = (uint8_t)(u[e / 4] >> (8 * (e % 4)));
+  for (int i = 0; i < 8; ++i) {
+    const long row = r0 + rg * 8 + i;
+    const uint8_t* at = p.x + (row * p.stride + c0 + col) * kSize<TYPE>;
+    uint32_t u[2] = {0, 0};
+    if (row < p.rows && count > 0) {
+      if constexpr (TYPE == SHK_SRC_F32) {
+        if (count > 1) {
+          const u2 w = *reinterpret_cast<const any_u2*>(at);
+          u[0] = w[0], u[1] = w[1];
+        } else {
+          u[0] = *reinterpret_cast<const uint32_t*>(at);
+        }
+      } else {
+        const uint32_t w = count > 1 ? *reinterpret_cast<const any_u32*>(at) : *reinterpret_cast<const uint16_t*>(at);
+        u[0] = w & 0xFFFFu, u[1] = w >> 16;
       }
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      v[e][i] = TYPE == SHK_SRC_F32    ? __uint_as_float(u[e])
+                : TYPE == SHK_SRC_BF16 ? bf16_bits_to_f32((uint16_t)u[e])
+                                       : (float)__builtin_bit_cast(_Float16, (uint16_t)u[e]);
+  }
+  uint32_t top[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) top[e] = max(top[e], magnitude(v[e][i]));
+  if constexpr (WHOLE) {
+    top[0] = max(top[0], top[1]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], d, 64));
+    if (lane == 0) tops[rg][0] = top[0];
+  } else {
+    *reinterpret_cast<uint2*>(&tops[rg][col]) = make_uint2(top[0], top[1]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if constexpr (WHOLE) {
+      top[0] = max(top[0], tops[w][0]);
+    } else {
+      const uint2 t = *reinterpret_cast<const uint2*>(&tops[w][col]);
+      top[0] = max(top[0], t.x), top[1] = max(top[1], t.y);
+    }
+  }
+  uint32_t w[2][2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float s = scale_of<KIND>(top[WHOLE ? 0 : e]);
+    codes8<KIND>(v[e], s, 1.f / s, normal_scale(s), w[e]);
+    if constexpr (WHOLE) {
+      if (threadIdx.x == 0 && e == 0)
+        p.scales[TURN ? blockIdx.x * p.s_row + blockIdx.y * p.s_block : blockIdx.y * p.s_row + blockIdx.x * p.s_block] = s;
+    } else {
+      if (rg == 0 && count > e) p.scales[(c0 + col + e) * p.s_row + blockIdx.y * p.s_block] = s;
+    }
+  }
+  if constexpr (!TURN) {
+    static_assert(TURN || WHOLE, "blocks of one row are fp8_rows'");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long row = r0 + rg * 8 + i;
+      uint8_t* to = p.codes + row * p.pitch + c0 + col;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (row < p.rows && count > e) to[e] = (uint8_t)(w[e][i / 4] >> (8 * (i % 4)));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<uint2*>(lds + (col + e) * 128 + 8 * (rg ^ (col / 8))) = make_uint2(w[e][0], w[e][1]);
+    __syncthreads();
+    const int c = threadIdx.x / 8, piece = threadIdx.x % 8;
+    store_turned(p, lds, c, piece, c0, r0);
   }
 }
 
@@ -263,7 +354,14 @@ hipError_t launch(const Convert& p, bool turn, bool whole, hipStream_t s) {
     else hipLaunchKernelGGL((fp8_rows<TYPE, KIND, 1>), grid, dim3(256), 0, s, p);
   } else {
     const dim3 grid((unsigned)((p.cols + 127) / 128), (unsigned)((p.rows + 127) / 128));
-    if (!turn) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, false, true>), grid, dim3(256), 0, s, p);
+    // few tiles: 300 x 600 transposed 6.8 us and 9.6 by whole vectors, 1000 x 1040 7.0
+    // and 9.2, 2048 x 4096 10.1 and 11.1, but 4096 x 4096 17.0 and 15.7; with one scale
+    // a tile 1000 x 1040 6.1 and 7.9, but 2048 x 2048 7.5 and 7.0
+    if ((long)grid.x * grid.y <= (turn && !whole ? 512 : 128)) {
+      if (!turn) hipLaunchKernelGGL((fp8_tile_thin<TYPE, KIND, false, true>), grid, dim3(1024), 0, s, p);
+      else if (whole) hipLaunchKernelGGL((fp8_tile_thin<TYPE, KIND, true, true>), grid, dim3(1024), 0, s, p);
+      else hipLaunchKernelGGL((fp8_tile_thin<TYPE, KIND, true, false>), grid, dim3(1024), 0, s, p);
+    } else if (!turn) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, false, true>), grid, dim3(256), 0, s, p);
     else if (whole) hipLaunchKernelGGL((fp8_tile<TYPE, KIND, true, true>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((fp8_tile<TYPE, KIND, true, false>), grid, dim3(256), 0, s, p);
   }

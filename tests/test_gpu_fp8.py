@@ -165,6 +165,25 @@ def test_quantize_rows_in_pairs(device, rows, cols, dtype):
         assert torch.equal(scales[at : at + 40000], want_scales)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("block_rows,transpose", [(128, False), (128, True), (1, True)])
+def test_quantize_many_tiles(device, block_rows, transpose, dtype):
+    """Many tiles take another form than few: the same codes and scales as those of parts of the rows, blocks of
+    zeros and with infinities and NaN among them."""
+    x = torch.randn((3001, 3003), generator=_gen("tiles", block_rows, transpose, dtype)).to(dtype)
+    x[256:384] = 0
+    x[500, 700], x[2999, 3002], x[700, 128:256] = math.inf, math.nan, -math.inf
+    x = x.to(device)
+    codes, scales = shk.quantize_fp8(x, block_rows=block_rows, transpose=transpose)
+    for at in range(0, 3001, 512):
+        want, want_scales = shk.quantize_fp8(x[at : at + 512], block_rows=block_rows, transpose=transpose)
+        got, got_scales = codes[at : at + 512], scales[at // 128 : at // 128 + 4]
+        if transpose:
+            got, got_scales = codes[:, at : at + 512], scales[:, at // 128 : at // 128 + 4]
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+        assert torch.equal(got_scales.contiguous().view(torch.int32), want_scales.contiguous().view(torch.int32))
+
+
 @pytest.mark.parametrize("kind", [E4M3, E5M2])
 def test_quantize_bad_blocks(device, kind):
     """A block with an infinity or a NaN has that as its scale and zero codes; its neighbours do not see it;
