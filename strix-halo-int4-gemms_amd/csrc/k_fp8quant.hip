@@ -21,6 +21,7 @@
 
 #include "shk_common.h"
 #include "shk_fp8.h"
+#include "shk_lanes.h"
 #include "shk_loads.h"
 
 namespace shk {
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(256) void fp8_rows(const Convert p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e]));
 #pragma unroll
-    for (int d = 1; d < 16; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+    for (int d = 1; d < 16; d *= 2) most = max(most, across(most, d));
     const float s = scale_of<KIND>(most);
     uint32_t w[2];
     codes8<KIND>(v, s, 1.f / s, normal_scale(s), w);
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256) void fp8_tile(const Convert p) {
 #pragma unroll
     for (int e = 1; e < 8; ++e) top[0] = max(top[0], top[e]);
 #pragma unroll
-    for (int d = 1; d < 16; d *= 2) top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], d, 64));
+    for (int d = 1; d < 16; d *= 2) top[0] = max(top[0], across(top[0], d));
     if (lane == 0) tops[wave][0] = top[0];
   } else if (lane < 16) {
 #pragma unroll
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(1024) void fp8_tile_thin(const Convert p) {
   if constexpr (WHOLE) {
     top[0] = max(top[0], top[1]);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) top[0] = max(top[0], (uint32_t)__shfl_xor((int)top[0], d, 64));
+    for (int d = 1; d < 64; d *= 2) top[0] = max(top[0], across(top[0], d));
     if (lane == 0) tops[rg][0] = top[0];
   } else {
     *reinterpret_cast<uint2*>(&tops[rg][col]) = make_uint2(top[0], top[1]);

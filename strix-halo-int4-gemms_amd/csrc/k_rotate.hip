@@ -10,7 +10,8 @@
 // what is left is at most an eighth of a turn, exact in f32 to 2^-24 of itself.
 //
 // Bound by memory, and by latency for a few tokens.  8191 tokens of 40 heads of 128
-// (168 MB): 40 to 44 us, 3.9 TB/s, with stores that pass the caches by, 51 without.
+// (168 MB): 35 us, 4.8 TB/s.  The vector unit is near: 44 us before addresses took
+// products of 32 bits and sums over lanes moves, 38 without stores past the caches.
 // 24 tokens, with norm and cache, 4.7 us.
 #include <hip/hip_runtime.h>
 
@@ -19,6 +20,7 @@
 
 #include "shk_common.h"
 #include "shk_kvrows.h"
+#include "shk_lanes.h"
 #include "shk_loads.h"
 #include "shk_step.h"
 
@@ -36,7 +38,8 @@ struct Rotate {
   float amplitude, eps;
   unsigned rows, per_token;  // per_token: heads + kv_heads, and kv_heads more with a cache
   unsigned inverse[2];       // floor(2^64 / per_token) + 1, low half first
-  float per_dim;             // 1 / dim
+  float per_dim, per_half;   // 1 / dim, 1 / half
+  unsigned token_bytes[3], head_bytes[3], out_token_bytes[2], out_head_bytes[2];  // the strides, where these hold them
   unsigned heads, kv_heads;
   int dim, half, rotated;
   int position8, weight_type;
@@ -116,14 +119,20 @@ __device__ __forceinline__ double position_of(const Rotate& p, long token) {
                      : (double)static_cast<const int32_t*>(p.positions)[token];
 }
 
+// i / half: i is below 2^15, and i + 1/2 is nowhere near a multiple of half.
+__device__ __forceinline__ int quotient(const Rotate& p, int i) { return (int)(((float)i + 0.5f) * p.per_half); }
+
 __device__ __forceinline__ Asked ask_shared(const Rotate& p, unsigned token0, unsigned tokens) {
   Asked r{0.0, 0.0, 0.f, (int)tokens * p.half, (int)threadIdx.x, p.weight[0] != nullptr ? 2 * p.dim : 0};
   if (r.angle < r.angles) {
-    const int t = r.angle / p.half;
+    const int t = quotient(p, r.angle);
     r.position = position_of(p, (long)token0 + t);
     r.turns = p.turns[r.angle - t * p.half];
   }
-  if ((int)threadIdx.x < r.weights) r.weight = weight_of(p, (int)threadIdx.x >= p.dim, (int)threadIdx.x % p.dim);
+  if ((int)threadIdx.x < r.weights) {
+    const bool key = (int)threadIdx.x >= p.dim;
+    r.weight = weight_of(p, key, (int)threadIdx.x - (key ? p.dim : 0));
+  }
   return r;
 }
 
@@ -131,7 +140,7 @@ __device__ __forceinline__ void fill_shared(const Shared& s, const Rotate& p, un
   for (int i = r.angle; i < r.angles; i += 256) {
     double angle = r.position * r.turns;
     if (i != r.angle) {
-      const int t = i / p.half;
+      const int t = quotient(p, i);
       angle = position_of(p, (long)token0 + t) * p.turns[i - t * p.half];
     }
     const float2 cs = turned(angle);
@@ -166,6 +175,12 @@ __device__ __forceinline__ Place place_of(const Rotate& p, unsigned row, bool in
   return r;
 }
 
+// One of three arguments: a choice, where an index would be a load.
+template <class T>
+__device__ __forceinline__ T pick(int kind, T query, T key, T value) {
+  return kind == 0 ? query : kind == 1 ? key : value;
+}
+
 // The quantized row of a key or value, as kv_write_kernel makes it: a NaN is
 // larger than an infinity, and both stay.
 template <int TYPE, int LANES>
@@ -177,7 +192,7 @@ __device__ __forceinline__ void into_cache(const Rotate& p, const Place& r, int 
     most = max(most, __float_as_uint(v[e]) & 0x7FFFFFFFu);
   }
 #pragma unroll
-  for (int d = 1; d < LANES; d *= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+  for (int d = 1; d < LANES; d *= 2) most = max(most, across(most, d));
   const long slot = p.slot8 ? static_cast<const int64_t*>(p.slots)[r.token] : static_cast<const int32_t*>(p.slots)[r.token];
   if (slot < 0 || slot >= p.slots_total) return;
   const uint32_t sb = f32_to_bf16_rne(__uint_as_float(most) / (p.bits == 4 ? 7.0f : 127.0f));
@@ -214,7 +229,7 @@ __device__ __forceinline__ void store16(uint8_t* to, u4 v) {
   else *reinterpret_cast<u4*>(to) = v;
 }
 
-// Rows on 16 bytes whose values, turning ones and (APART) half of them are whole
+// Rows on 16 bytes, strides of 32 bits, whose values, turning ones and (APART) half of them are whole
 // 8s: a lane turns with all its values or none, and its partners are one load.
 template <int TYPE, int LANES, bool APART, int ROUNDS>
 __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
@@ -236,8 +251,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
     if (r.kind < 0) continue;
-    const uint8_t* x = p.x[r.kind] + ((long)r.token * p.token_stride[r.kind] + (long)r.head * p.head_stride[r.kind]) *
-                                         kSize<TYPE>;
+    const uint8_t* x = pick(r.kind, p.x[0], p.x[1], p.x[2]) +
+                       (unsigned long long)r.token * pick(r.kind, p.token_bytes[0], p.token_bytes[1], p.token_bytes[2]) +
+                       (unsigned long long)r.head * pick(r.kind, p.head_bytes[0], p.head_bytes[1], p.head_bytes[2]);
     load8<TYPE, true>(x + first * kSize<TYPE>, v[i]);
     if constexpr (APART)
       if (r.kind < 2 && turning) load8<TYPE, true>(x + partner * kSize<TYPE>, w[i]);
@@ -256,7 +272,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[i][e], v[i][e], sum);
 #pragma unroll
-      for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d, 64);
+      for (int d = 1; d < LANES; d *= 2) sum += __uint_as_float(across(__float_as_uint(sum), d));
       scale = norm_of(p, sum);
       if (head) {
         float weight[8];
@@ -299,8 +315,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(const Rotate p) {
     if (r.kind >= 1 && p.bits != 0) {
       into_cache<TYPE, LANES>(p, r, part, v[i]);
     } else if (r.kind >= 0) {
-      uint8_t* out = p.out[r.kind] + ((long)r.token * p.out_token_stride[r.kind] +
-                                      (long)r.head * p.out_head_stride[r.kind] + first) * kSize<TYPE>;
+      uint8_t* out = (r.kind == 0 ? p.out[0] : p.out[1]) +
+                     (unsigned long long)r.token * (r.kind == 0 ? p.out_token_bytes[0] : p.out_token_bytes[1]) +
+                     (unsigned long long)r.head * (r.kind == 0 ? p.out_head_bytes[0] : p.out_head_bytes[1]) + first * kSize<TYPE>;
       if constexpr (TYPE == SHK_SRC_F32) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -345,7 +362,7 @@ __global__ __launch_bounds__(256) void rotate_any_kernel(const Rotate p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
 #pragma unroll
-    for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d, 64);
+    for (int d = 1; d < LANES; d *= 2) sum += __uint_as_float(across(__float_as_uint(sum), d));
     scale = norm_of(p, sum);
   }
   if (head) {
@@ -407,8 +424,8 @@ hipError_t launch_pairs(const Rotate& p, bool vec, hipStream_t s) {
     return hipGetLastError();
   }
   // one round while that leaves CUs idle, else two, whose loads go out together
-  // (8191 tokens of 40 heads of 128: 51 us with two, 55 with one, 60 with four,
-  // whose registers halve the waves; 43 with stores past the caches)
+  // (8191 tokens of 40 heads of 128: 35 us with two, 39 with four, whose registers
+  // halve the waves, 43 with one; two without stores past the caches 38)
   return p.rows <= 256 * PER * 4 ? launch<TYPE, LANES, APART, 1>(p, s) : launch<TYPE, LANES, APART, 2>(p, s);
 }
 
@@ -446,6 +463,7 @@ hipError_t launch_rotate(const shk_kv_cache* c, const shk_rotate& a, hipStream_t
   const unsigned long long inverse = ~0ULL / p.per_token + 1;  // per_token is 2 or more, 2^64 - 1 divides alike
   p.inverse[0] = (unsigned)inverse, p.inverse[1] = (unsigned)(inverse >> 32);
   p.per_dim = 1.f / (float)a.head_dim;
+  p.per_half = a.rotated > 0 ? 2.f / (float)a.rotated : 0.f;
   p.dim = (int)a.head_dim, p.rotated = (int)a.rotated, p.half = p.rotated / 2;
   uintptr_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
                   reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_out) |
@@ -462,8 +480,18 @@ hipError_t launch_rotate(const shk_kv_cache* c, const shk_rotate& a, hipStream_t
   } else {
     all |= (uintptr_t)(size * (a.k_out_token_stride | a.k_out_head_stride));
   }
+  unsigned long long widest = 0;  // a negative stride is wide, too
+  for (int i = 0; i < 3; ++i) {
+    widest |= (unsigned long long)p.token_stride[i] * size | (unsigned long long)p.head_stride[i] * size;
+    p.token_bytes[i] = (unsigned)(p.token_stride[i] * size), p.head_bytes[i] = (unsigned)(p.head_stride[i] * size);
+  }
+  for (int i = 0; i < 2; ++i) {
+    widest |= (unsigned long long)p.out_token_stride[i] * size | (unsigned long long)p.out_head_stride[i] * size;
+    p.out_token_bytes[i] = (unsigned)(p.out_token_stride[i] * size);
+    p.out_head_bytes[i] = (unsigned)(p.out_head_stride[i] * size);
+  }
   const bool apart = a.interleaved == 0;
-  const bool vec = (all & 15) == 0 && a.head_dim % 8 == 0 && a.rotated % (apart ? 16 : 8) == 0;
+  const bool vec = (all & 15) == 0 && widest >> 32 == 0 && a.head_dim % 8 == 0 && a.rotated % (apart ? 16 : 8) == 0;
   if (a.type == SHK_SRC_F32) return launch_type<SHK_SRC_F32>(p, vec, apart, s);
   if (a.type == SHK_SRC_F16) return launch_type<SHK_SRC_F16>(p, vec, apart, s);
   return launch_type<SHK_SRC_BF16>(p, vec, apart, s);
