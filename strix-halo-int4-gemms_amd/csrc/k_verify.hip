@@ -12,7 +12,7 @@
 //  * verify_sums and verify_draw: the vocabulary is cut into pieces over all CUs,
 //    added first, then the piece and the token in it are found.  Bound by the one
 //    row of each kind that a sequence reads, and by the second launch: 61 x 131072
-//    f32 (61 MB) 14 us (4.2 TB/s) and 12.
+//    f32 (61 MB) 13 us (4.6 TB/s) and 11.5.
 // f32, replayed, whole and in pieces: 1 x 2048 3.7 and 13.5 us, 128 x 16384 9 and
 // 24, 1 x 32768 8.5 and 11.2, 128 x 32768 12 and 19.5.
 #include <hip/hip_runtime.h>
@@ -21,6 +21,7 @@
 #include <cstdint>
 
 #include "shk_common.h"
+#include "shk_lanes.h"
 #include "shk_loads.h"
 #include "shk_step.h"
 
@@ -144,33 +145,6 @@ __device__ __forceinline__ void weights8(const shk_verify& p, const Row& r, long
   for (int e = 0; e < 8; ++e) w[e] = weight_of(have[e], gone[e]);
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
-  return v;
-}
-
-// v plus the value that CTRL moves to this lane, in the rows of ROWS (else plus 0).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double plus_moved(double v) {
-  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
-  return v + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
-}
-
-// Inclusive sum over a wave's lanes: within rows of 16 by 1, 2, 4 and 8 lanes up,
-// then the last lane of rows 0 and 2 to the rows above them, and lane 31 to both
-// rows behind it.
-__device__ __forceinline__ double wave_inclusive(double v) {
-  v = plus_moved<0x111, 0xF>(v);
-  v = plus_moved<0x112, 0xF>(v);
-  v = plus_moved<0x114, 0xF>(v);
-  v = plus_moved<0x118, 0xF>(v);
-  v = plus_moved<0x142, 0xA>(v);
-  return plus_moved<0x143, 0xC>(v);
-}
-
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, const Pieces pieces) {
   __shared__ Sum parts[kThreads / 64];
@@ -185,8 +159,8 @@ __global__ __launch_bounds__(kThreads) void verify_sums(const shk_verify p, cons
 #pragma unroll
     for (int e = 0; e < 8; ++e) mine.left += w[e].left, mine.all += w[e].all;
   }
-  mine.left = wave_sum(mine.left), mine.all = wave_sum(mine.all);
-  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = mine;
+  mine.left = wave_inclusive(mine.left), mine.all = wave_inclusive(mine.all);
+  if ((threadIdx.x & 63) == 63) parts[threadIdx.x >> 6] = mine;
   __syncthreads();
   if (threadIdx.x == 0) {
     Sum s = parts[0];

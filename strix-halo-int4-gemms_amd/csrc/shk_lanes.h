@@ -20,4 +20,28 @@ __device__ __forceinline__ uint32_t across(uint32_t v, int d) {
   }
 }
 
+// v plus the value of 8 bytes that CTRL moves to this lane, in the rows of ROWS (else
+// plus 0).
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T plus_moved(T v) {
+  static_assert(sizeof(T) == 8, "");
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(T, ((unsigned long long)hi << 32) | lo);
+}
+
+// Inclusive sum over a wave's lanes, all of them active: within rows of 16 by 1, 2, 4
+// and 8 lanes up, then the last lane of rows 0 and 2 to the rows above them, and lane
+// 31 to both rows behind it.
+template <class T>
+__device__ __forceinline__ T wave_inclusive(T v) {
+  v = plus_moved<0x111, 0xF>(v);
+  v = plus_moved<0x112, 0xF>(v);
+  v = plus_moved<0x114, 0xF>(v);
+  v = plus_moved<0x118, 0xF>(v);
+  v = plus_moved<0x142, 0xA>(v);
+  return plus_moved<0x143, 0xC>(v);
+}
+
 }  // namespace shk
