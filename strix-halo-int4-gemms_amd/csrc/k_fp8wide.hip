@@ -37,7 +37,7 @@ __device__ __forceinline__ int swizzle(int row) { return (row ^ (row >> 3)) & 7;
 
 template <int KIND_A, int KIND_B, bool BROW>
 __global__ __launch_bounds__(256, 2) void fp8_wide_kernel(const Fp8Product p) {
-  __shared__ __align__(16) uint8_t lds[2 * kStage];
+  __shared__ __align__(16) uint8_t lds[2 * kStage];  // 64 KiB of it for the results, too
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
   tile_of(p, 8, tm, tn);
@@ -140,17 +140,27 @@ __global__ __launch_bounds__(256, 2) void fp8_wide_kernel(const Fp8Product p) {
         }
     }
   }
+  // Through LDS, so that a store is four runs of 256 bytes and not 32 of 32 (5489 x
+  // 13153 x 300: 126 us, 138 without): unit u of row r of a wave's 64 x 64 lies at
+  // r * 256 + 16 * (u ^ (r % 16)).
+  __syncthreads();
+  uint8_t* own = lds + wave * 16384;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int m = m0 + wm * 64 + x * 32 + row_in;
-    if (m >= p.m) continue;
+  for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const v16f& v = acc[x][j];
-        store_four(p, m, n0 + wn * 64 + j * 32 + q * 8 + half * 4, v4f{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]});
+        *reinterpret_cast<v4f*>(own + (x * 32 + row_in) * 256 + 16 * ((j * 8 + q * 2 + half) ^ (row_in & 15))) =
+            v4f{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
       }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int r = 0; r < 64; r += 4) {
+    const int row = r + lane / 16, unit = lane & 15, m = m0 + wm * 64 + row;
+    const v4f v = *reinterpret_cast<const v4f*>(own + row * 256 + 16 * (unit ^ (row & 15)));
+    if (m < p.m) store_four(p, m, n0 + wn * 64 + unit * 4, v);
   }
 }
 
