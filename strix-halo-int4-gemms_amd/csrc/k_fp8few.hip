@@ -5,11 +5,15 @@
 // Its eight waves take K's blocks in turn, so that together they read runs of 1
 // KiB of each row of b, and nothing is shared while they do: a wave loads both
 // operands' fragments straight into registers, one block ahead, multiplies a block
-// with one MFMA for each 16 x 16 results, and folds it into its own f32 sums.
-// Behind the loop the eight sums are added in LDS, in order of the waves.
+// for each 16 x 16 results, and folds it into its own f32 sums.  Behind the loop the
+// eight sums are added in LDS, in order of the waves.
+// Results of all types go through the f16 matrix unit, whose sums are f32 ones
+// (k_fp8.hip says what the 8-bit one keeps): widening the codes hides behind b, 16 x
+// 11008 x 4096 in 11.1 us where the 8-bit unit takes 10.9, 32 x 4096 x 4096 in 9.8
+// and 9.6.
 // K is not cut over workgroups: 16 rows of b keep a CU's share of the memory rate
 // busy, and a sum over workgroups would be another launch.
-// Bound by that share: 16 x 11008 x 4096 in 11 to 12 us, b at 3.9 TB/s.
+// Bound by that share: b at 4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -48,7 +52,7 @@ __device__ __forceinline__ v8i load_end(const uint8_t* at, int left) {
   return v;
 }
 
-template <int MT, int NT, int KIND_A, int KIND_B, bool BROW, bool WIDE>
+template <int MT, int NT, int KIND_A, int KIND_B, bool BROW>
 __global__ __launch_bounds__(64 * kWaves) void fp8_few_kernel(const Fp8Product p) {
   __shared__ v4f sums[kWaves][MT * NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_few_kernel(const Fp8Product p
     for (int x = 0; x < MT; ++x)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const v4f t = product128<KIND_A, KIND_B, WIDE>(f.b[j], f.a[x]);
+        const v4f t = product128<KIND_A, KIND_B, true>(f.b[j], f.a[x]);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           acc[x][j][r] = __builtin_fmaf(t[r], f.sa[x] * f.sb[j][BROW ? r : 0], acc[x][j][r]);
@@ -135,23 +139,18 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_few_kernel(const Fp8Product p
   }
 }
 
-template <int MT, int NT, int KIND_A, int KIND_B, bool WIDE>
+template <int MT, int NT, int KIND_A, int KIND_B>
 hipError_t launch(const Fp8Product& p, hipStream_t s) {
   const dim3 grid((p.n + 16 * NT - 1) / (16 * NT)), group(64 * kWaves);
-  if (p.b_shift == 0) hipLaunchKernelGGL((fp8_few_kernel<MT, NT, KIND_A, KIND_B, true, WIDE>), grid, group, 0, s, p);
-  else hipLaunchKernelGGL((fp8_few_kernel<MT, NT, KIND_A, KIND_B, false, WIDE>), grid, group, 0, s, p);
+  if (p.b_shift == 0) hipLaunchKernelGGL((fp8_few_kernel<MT, NT, KIND_A, KIND_B, true>), grid, group, 0, s, p);
+  else hipLaunchKernelGGL((fp8_few_kernel<MT, NT, KIND_A, KIND_B, false>), grid, group, 0, s, p);
   return hipGetLastError();
-}
-
-template <int MT, int NT, int KIND_A, int KIND_B>
-hipError_t launch_wide(const Fp8Product& p, hipStream_t s) {
-  return p.out_type == SHK_SRC_F32 ? launch<MT, NT, KIND_A, KIND_B, true>(p, s) : launch<MT, NT, KIND_A, KIND_B, false>(p, s);
 }
 
 template <int MT, int NT>
 hipError_t launch_columns(const Fp8Product& p, bool e5_a, bool e5_b, hipStream_t s) {
-  if (e5_a) return e5_b ? launch_wide<MT, NT, 1, 1>(p, s) : launch_wide<MT, NT, 1, 0>(p, s);
-  return e5_b ? launch_wide<MT, NT, 0, 1>(p, s) : launch_wide<MT, NT, 0, 0>(p, s);
+  if (e5_a) return e5_b ? launch<MT, NT, 1, 1>(p, s) : launch<MT, NT, 1, 0>(p, s);
+  return e5_b ? launch<MT, NT, 0, 1>(p, s) : launch<MT, NT, 0, 0>(p, s);
 }
 
 // As many columns a workgroup as leave each CU one, four times 16 at most: what a

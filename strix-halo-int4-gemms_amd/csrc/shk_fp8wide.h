@@ -1,4 +1,4 @@
-// A block of K through the f16 matrix unit, for f32 results.
+// A block of K through the f16 matrix unit, whose sums are f32 ones.
 #pragma once
 
 #include "shk_fp8product.h"
