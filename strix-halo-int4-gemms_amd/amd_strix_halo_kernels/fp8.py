@@ -139,9 +139,18 @@ def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None,
     blocks) or [N, ceil(K / 128)], f32 of any strides.  Returns [M, N] in
     ``out_dtype`` (bf16, the default, f16 or f32).  Sums are f32: inside a
     block of K by the matrix unit, over the blocks in an order that follows from
-    the sizes (the same call has the same bits); rounded once at the end.  For
-    bf16 and f16 results the 8-bit unit multiplies, whose sums hold to about 2e-5;
-    for f32 results the 16-bit one, whose sums are as f32 ones.
+    the sizes (the same call has the same bits); rounded once at the end.
+
+    f32 results, and results of a decode step's few rows, go through the 16-bit
+    unit, whose sums are as f32 ones.  Other bf16 and f16 results go through the
+    8-bit unit, which keeps the products of eight neighbours along K to 2^-13 of
+    the power of two of the largest of them, cut towards zero.  That is 2e-5 of the
+    results' rms where channels are alike, 8e-5 where some are hundreds of times
+    the others, and up to 1.5e-4, nearly all of it towards zero, where the
+    operands are of one sign besides (at worst 8.5e-4 of the largest products added
+    up).  A bf16 result's own rounding is 1.7e-3; an f16 one's 2.1e-4 is no longer
+    well above it.  ``out_dtype=torch.float32`` is the way around.
+
     Operands whose rows do not all start on 16 bytes are copied first; the codes
     of ``quantize_fp8`` do.
     """
