@@ -1,9 +1,9 @@
 // 8-bit floating-point products on tiles of 256 x 256: the matrix unit kept fed.
 //
-// A stage is one block of K (128): 256 rows of each operand, 64 KiB, and their
-// scales, in one of two LDS slots.  Eight waves hold 128 x 64 of the tile each:
-// per stage 32 MFMAs (32 cycles of a SIMD each), whose results are folded into
-// the f32 sums with four multiply-adds (16 cycles) while the next ones run: the
+// A stage is one block of K (128): 256 rows of each operand, 64 KiB, in one of two
+// LDS slots, and their scales, in one of three.  Eight waves hold 128 x 64 of the
+// tile each: per stage 32 MFMAs (32 cycles of a SIMD each), whose results are folded
+// into the f32 sums with four multiply-adds (16 cycles) while the next ones run: the
 // sums have to lie where the vector unit reaches them, and 128 of them with both
 // operands' fragments fill a wave's 256 registers.
 //
@@ -13,13 +13,19 @@
 // Three quarters through, when the last fragment of the stage is in registers,
 // the waves meet: behind that barrier the next stage is complete (its copy was
 // issued a whole stage ago), so its first fragments are read under the last
-// MFMAs, and this stage's slot is free.  The copies of the stage after next are
-// spread over the following steps; in one burst they cost 500 cycles a stage.
+// MFMAs, and this stage's rows are all in registers: their slot is free.  The copies
+// of the stage after next are spread over the following steps; in one burst they
+// cost 500 cycles a stage.  Scales of b's rows are read by the folds, behind that
+// barrier too, and those of the stage after next are copied before the next one, so
+// that a wave may still read the ones while another's copy brings the others: they
+// have three slots, and the barrier between a slot's last reads and its next copy is
+// the following stage's.
 //
 // Bound by power, then by the matrix unit: at 8192^3 a stage takes 2600 cycles
 // (2048 of MFMAs) at 1.6 GHz; with operands of one value it runs at 2.3 GHz.
-// 8192^3 437 to 449 us (2500 TFLOP/s), 556 where each row of b has its own scales;
-// 4096 x 11008 x 4096 172 to 179 (three rounds of workgroups for 2.7 of work).
+// 8192^3 428 to 449 us (2500 TFLOP/s), 573 to 589 where each row of b has its own
+// scales; 4096 x 11008 x 4096 160 to 179, 221 with those (three rounds of workgroups
+// for 2.7 of work).
 // Measured and dropped: fragments of b straight from memory (the 16 rows of a
 // load cost the vector memory path 5600 cycles a stage), folds grouped by row.
 #include <hip/hip_runtime.h>
@@ -38,8 +44,11 @@ typedef __attribute__((address_space(3))) const v4f lds_v4f;
 typedef __attribute__((address_space(3))) const float lds_float;
 
 constexpr int kB = 256 * 128;            // where b lies in a stage
-constexpr int kScales = 512 * 128;       // 256 of a's, 256 of b's
-constexpr int kStage = kScales + 2048;
+constexpr int kStage = 512 * 128;
+constexpr int kScales = 2 * kStage;      // behind both slots of rows
+constexpr int kScaleSlots = 3, kScaleSlot = 2048;  // 256 of a's, 256 of b's
+constexpr int kRead = 23;                // the step behind which a stage's barrier is
+constexpr int kCopyScales = 8;           // the step that copies the next stage's scales
 
 // What is behind K in the last stage is whatever follows the rows: zeros instead,
 // `left` of 128 values stay.
@@ -58,7 +67,7 @@ __device__ __forceinline__ void clear_tail(uint8_t* st, int left) {
 
 template <int KIND_A, int KIND_B, bool BROW>
 __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
-  __shared__ __align__(16) uint8_t lds[2 * kStage];
+  __shared__ __align__(16) uint8_t lds[kScales + kScaleSlots * kScaleSlot];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
   tile_of(p, 4, tm, tn);
@@ -84,10 +93,10 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
   const uint32_t off = (uint32_t)(((wave & 3) * 64 + lane / 8) * pitch) + 16 * ((lane & 7) ^ (lane / 8));
   const uint32_t step8 = (uint32_t)(8 * pitch), base = lds_address(lds);
   const uint32_t to = base + (of_a ? 0 : kB) + (wave & 3) * 8192, s_to = base + kScales + wave * 256;
-  auto piece = [&](int kb, int slot, int c) {  // 8 of a wave's rows, and the scales of them all
-    if (c < 8) lds_dma16(rows, off, (uint32_t)kb * 128u + c * step8, to + slot * kStage + c * 1024);
-    else lds_dma4(scales, s_off, (uint32_t)kb * s_step, s_to + slot * kStage);
+  auto piece = [&](int kb, int slot, int c) {  // 8 of a wave's rows
+    lds_dma16(rows, off, (uint32_t)kb * 128u + c * step8, to + slot * kStage + c * 1024);
   };
+  auto piece_scales = [&](int kb, uint32_t at) { lds_dma4(scales, s_off, (uint32_t)kb * s_step, s_to + at); };
 
   const int wm = wave & 1, wn = wave >> 1, row_in = lane & 15, group = lane >> 4;
   v4f acc[8][4];
@@ -108,7 +117,8 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
   auto scale = [&](uint32_t at, int off) { return *(lds_float*)(uintptr_t)(at + off); };
 
 #pragma unroll
-  for (int c = 0; c < 9; ++c) piece(0, 0, c);
+  for (int c = 0; c < 8; ++c) piece(0, 0, c);
+  piece_scales(0, 0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   asm volatile("s_barrier" ::: "memory");
 #pragma unroll
@@ -118,10 +128,12 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) fb[0][j] = fragment(b_lo, b_hi, j * 2048);
   fa[0] = fragment(a_lo, a_hi, 0), fa[1] = fragment(a_lo, a_hi, 2048);
+  uint32_t s_at = 0;  // the slot of the stage's scales
 
   auto stage = [&](int i, auto slot_of, v8i (&now)[4], v8i (&next)[4]) {
     constexpr int slot = decltype(slot_of)::value, turn = slot ? -kStage : kStage;
     const int soon = min(i + 1, count - 1), later = min(i + 2, count - 1);
+    const uint32_t s_next = s_at == (kScaleSlots - 1) * kScaleSlot ? 0 : s_at + kScaleSlot, s_turn = s_next - s_at;
     v4f t[3], row_scales;
     float s_now = 0.f, s_old = 0.f, sb_next = 0.f;
     v8i f[10] = {fa[0], fa[1]};  // this stage's eight row tiles, the next one's first two
@@ -140,7 +152,8 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
         if (x == 6) next[j] = fragment(b_lo, b_hi, j * 2048);
         t[step % 3] = mfma128<KIND_A, KIND_B>(now[j], f[x]);
         if (step >= 24 && step % 2 == 0) piece(later, slot, (step - 24) / 2);
-        if (step < 10 && step % 2 == 0) piece(soon, slot ^ 1, 4 + step / 2);
+        if (step < 8 && step % 2 == 0) piece(soon, slot ^ 1, 4 + step / 2);
+        if (step == kCopyScales) piece_scales(soon, s_next);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (step >= 2) {
@@ -152,19 +165,20 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
           acc[fx][fj][r] = __builtin_fmaf(t[(step - 2) % 3][r], BROW ? s * row_scales[r] : s, acc[fx][fj][r]);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (step == 23) {
+      if (step == kRead) {
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
         asm volatile("s_barrier" ::: "memory");
-        a_lo += turn, a_hi += turn, b_lo += turn, b_hi += turn, sa_at += turn;
-        if constexpr (!BROW) sb_at += turn;
+        a_lo += turn, a_hi += turn, b_lo += turn, b_hi += turn, sa_at += s_turn;
+        if constexpr (!BROW) sb_at += s_turn;
         asm volatile("" : "+v"(a_lo), "+v"(a_hi), "+v"(b_lo), "+v"(b_hi), "+v"(sa_at), "+v"(sb_at));
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     if constexpr (BROW) {
-      sb_at += turn;
+      sb_at += s_turn;
       asm volatile("" : "+v"(sb_at));
     }
+    s_at = s_next;
     fa[0] = f[8], fa[1] = f[9], sa[0] = q[8], sa[1] = q[9], sb = sb_next;
   };
   int i = 0;
@@ -179,7 +193,8 @@ __global__ __launch_bounds__(512) void fp8_big_kernel(const Fp8Product p) {
   asm volatile("s_barrier" ::: "memory");
   if (left != 0) {
 #pragma unroll
-    for (int c = 0; c < 9; ++c) piece(count, 0, c);
+    for (int c = 0; c < 8; ++c) piece(count, 0, c);
+    piece_scales(count, 0);
     __builtin_amdgcn_s_waitcnt(0x0F70);
     asm volatile("s_barrier" ::: "memory");
     clear_tail(lds, left);
