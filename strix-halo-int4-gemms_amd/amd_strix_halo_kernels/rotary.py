@@ -45,8 +45,9 @@ def rotary_frequencies(rotated: int, *, base: float = 10000.0, scaling: str = "n
       slows the slowest pair by ``factor`` and the fastest not at all;
     * ``yarn``: pairs that turn more than ``fast`` times over the ``trained``
       positions stay, those that turn less than ``slow`` times are slowed by
-      ``factor``, those between in proportion to their index; the amplitude is
-      ``0.1 ln(factor) + 1``.
+      ``factor``, those between in proportion to their index (both ends in whole
+      pairs, the second at most ``rotated - 1``); the amplitude is ``0.1
+      ln(factor) + 1``, 1 for factors below 1.
     """
     if isinstance(rotated, bool) or not isinstance(rotated, int) or rotated < 2 or rotated % 2:
         raise ValueError(f"rotated must be a positive even int; got {rotated!r}")
@@ -68,9 +69,9 @@ def rotary_frequencies(rotated: int, *, base: float = 10000.0, scaling: str = "n
     def pair(turns: float) -> float:  # the pair that turns so often over the trained positions
         return half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)
 
-    low, high = max(0, math.floor(pair(fast))), min(half - 1, math.ceil(pair(slow)))
+    low, high = max(0, math.floor(pair(fast))), min(rotated - 1, math.ceil(pair(slow)))
     share = [min(1.0, max(0.0, (i - low) / max(1e-3, high - low))) for i in range(half)]
-    return [f * (1 - s) + f / factor * s for f, s in zip(plain, share)], 0.1 * math.log(factor) + 1.0
+    return [f * (1 - s) + f / factor * s for f, s in zip(plain, share)], 0.1 * math.log(max(1.0, factor)) + 1.0
 
 
 @dataclass(frozen=True, eq=False)
