@@ -205,7 +205,7 @@ def _frequencies(case):
     def pair(turns):  # the pair that turns so often over the trained context
         return half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)
 
-    low, high = max(0, math.floor(pair(32.0))), min(half - 1, math.ceil(pair(1.0)))
+    low, high = max(0, math.floor(pair(32.0))), min(case["rotated"] - 1, math.ceil(pair(1.0)))
     slow = [min(1.0, max(0.0, (i - low) / max(1e-3, high - low))) for i in range(half)]
     return [f * (1 - s) + f / factor * s for f, s in zip(plain, slow)], 0.1 * math.log(factor) + 1.0
 
