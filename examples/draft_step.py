@@ -14,7 +14,8 @@ A step runs, for all of them at once,
     the lengths without the others                   verify_draft
 
 Weights are random, and the drafts are the layer's own likeliest tokens with
-some noise.  Nothing of a step is read back to the host.  ``python
+some noise.  Nothing of a step is read back to the host.  A sequence that gets no
+places (the pool or its row of the table is full) sits the step out.  ``python
 examples/draft_step.py`` runs steps of 16 sequences with five drafts each and
 prints the time of a step, called one by one and replayed from a HIP graph, and
 how many drafts were kept.
@@ -69,7 +70,8 @@ class DraftLayer:
 
     def step(self, tokens, draft, uniforms):
         """tokens [batch, 1 + drafts]: each sequence's last token and its drafts, which draft [batch, drafts,
-        vocab] gave; returns verify_draft's result, and what went into and came out of the operators."""
+        vocab] gave; returns verify_draft's result, and what went into and came out of the operators.  A sequence
+        that got no places keeps its length and has no token: its row is -1 and none of its drafts is kept."""
         count = self.batch * (1 + self.drafts)
         at = shk.kv_pages_step(self.pages, self.new, count)
         x = self.embedding[tokens.flatten()]
@@ -83,7 +85,10 @@ class DraftLayer:
         y = x + self.project(seen.reshape(count, -1))
         logits = self.head(_norm(y), torch.float32)
         target = torch.softmax(logits, dim=-1).view(self.batch, 1 + self.drafts, -1)
-        out, kept = shk.verify_draft(target, draft, tokens[:, 1:].contiguous(), uniforms, lengths=self.pages.lengths)
+        # only drafts that got places are in the cache, and counted in the lengths
+        out, kept = shk.verify_draft(target, draft, tokens[:, 1:].contiguous(), uniforms,
+                                     counts=(at.taken - 1).clamp(min=0), lengths=self.pages.lengths)
+        out = torch.where(at.taken[:, None] > 0, out, -1)
         return out, kept, {"step": at, "q": q, "qkv": qkv, "lengths": lengths, "seen": seen, "y": y, "logits": logits,
                            "target": target}
 

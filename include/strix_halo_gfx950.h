@@ -762,7 +762,8 @@ int amd_strix_halo_kernels_kv_plan(int device_index, uintptr_t stream, const shk
  * weights count as 0, and where no weight is left the token is -1.  Sums are 64
  * bits.  out [batch, drafts + 1] (int64) holds the kept drafts, the next token,
  * then -1; kept [batch].  Where lengths is not null, lengths[b] loses the drafts
- * that were not kept.  Draft tokens outside the vocabulary are not kept.
+ * that were not kept (of counts[b], which is 0 for a sequence whose drafts
+ * amd_strix_halo_kernels_kv_plan gave no places).  Draft tokens outside the vocabulary are not kept.
  * workspace: at least amd_strix_halo_kernels_verify_workspace bytes, on 16 bytes,
  * not read before it is written; null where that is 0 (up to 32768 tokens). */
 typedef struct shk_verify {

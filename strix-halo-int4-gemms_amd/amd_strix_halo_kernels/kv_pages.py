@@ -109,7 +109,8 @@ def kv_pages_step(pages: KVPages, new_tokens: Any, capacity: int, *, stream: Any
     for in order of the sequences: a sequence that asks for any behind the first
     one that cannot be served is not served either) is refused: its slots are
     -1, its length and pages stay, and ``taken[b]`` is 0 instead of
-    ``new_tokens[b]``.
+    ``new_tokens[b]``.  Nothing of it is in the cache then: what a later call takes
+    off the lengths (``verify_draft``) is to leave it out.
 
     Updates ``pages`` in place: lengths, owned, page_table and the free stack.
     Steps of one pool must follow each other.

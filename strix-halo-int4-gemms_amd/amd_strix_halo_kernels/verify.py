@@ -56,6 +56,9 @@ def verify_draft(
     has only its first ``counts[b]`` drafts.  ``lengths`` (int32 [batch]) is
     changed in place where given: ``lengths[b]`` loses the drafts that were not
     kept, which is what is then left of the cached tokens (``KVPages.lengths``).
+    It has to hold them before: of a sequence that ``kv_pages_step`` refused no
+    draft is in the cache, which ``counts=(step.taken - 1).clamp(min=0)`` says
+    where a step takes a token and its drafts; its row of ``out`` is to be ignored.
     """
     torch = _torch()
     index = target.get_device()
