@@ -708,7 +708,8 @@ int amd_strix_halo_kernels_rotate(int device_index, uintptr_t stream, const shk_
 /* ---- pages of a step ---------------------------------------------------------
  * No counterpart in the reference.  Sequence b holds lengths[b] tokens and owns
  * the first owned[b] pages of its row of page_table [batch, width] (contiguous);
- * free_pages[0 .. *free_count) is a stack of unused pages, of free_total places.
+ * free_pages[0 .. *free_count) is a stack of unused pages, of free_total places (up to
+ * 2147483646).
  * A step takes new_tokens[b] tokens of each sequence, in order of b:
  *  1. A negative number ends the sequence: its pages go onto the stack, sequence
  *     after sequence, and its length and pages become 0.

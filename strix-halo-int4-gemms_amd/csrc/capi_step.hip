@@ -96,7 +96,7 @@ int amd_strix_halo_kernels_kv_plan(int device_index, uintptr_t stream, const shk
       return capi_fail("page_size must be a power of two from 16 to 1024; got " + std::to_string(a.page_size));
     if (a.width < 1 || a.width > INT_MAX / a.page_size)
       return capi_fail("a sequence holds at most 2147483647 tokens, in at least one page");
-    if (a.free_total < 0 || a.free_total > INT_MAX) return capi_fail("0 to 2147483647 places for free pages");
+    if (a.free_total < 0 || a.free_total >= INT_MAX) return capi_fail("0 to 2147483646 places for free pages");
     if (a.capacity < 0 || a.capacity > INT_MAX) return capi_fail("capacity must be from 0 to 2147483647");
     if (!a.page_table || !a.lengths || !a.owned || !a.free_count || !a.new_tokens || !a.starts || !a.taken || !a.ticket ||
         (a.free_total > 0 && !a.free_pages) || (a.capacity > 0 && (!a.slots || !a.positions || !a.sequences)))

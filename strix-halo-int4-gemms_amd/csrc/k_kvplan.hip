@@ -124,10 +124,12 @@ __global__ __launch_bounds__(kThreads) void kv_plan_kernel(const shk_kv_plan p, 
     const int place = top - 1 - j;
     return place < had ? p.free_pages[place] : returned(place - had);
   };
-  // whether the new tokens of a sequence have places
+  // whether the new tokens of a sequence have places; sums of pages that saturated
+  // are larger than any stack, and say nothing of what one sequence asks for
   auto fits = [&](int b) {
-    return s.fresh[b] >= 0 && (((long)s.length[b] + s.fresh[b] + (1L << shift) - 1) >> shift) <= width &&
-           s.start[b] + (long)s.fresh[b] <= p.capacity && (s.ask[b + 1] == s.ask[b] || s.ask[b + 1] <= top);
+    const long pages = ((long)s.length[b] + s.fresh[b] + (1L << shift) - 1) >> shift;
+    return s.fresh[b] >= 0 && pages <= width && s.start[b] + (long)s.fresh[b] <= p.capacity &&
+           (pages <= s.owned[b] || s.ask[b + 1] <= top);
   };
 
   const long mine = blockIdx.x * (long)kThreads + threadIdx.x, all = (long)gridDim.x * kThreads;

@@ -57,3 +57,27 @@ def test_pages_for_sequences_without_tokens_run_out(device):
     now = _step(pool, [0, 0, 0, 0], 8, device)
     assert now["owned"] == [3, 3, 0, 0] and now["free"] == []
     assert sorted(now["page_table"][0][:3] + now["page_table"][1][:3]) == [0, 1, 2, 3, 4, 5]
+
+
+def test_sums_of_pages_past_32_bits(device):
+    """Sequences behind 2^31 pages that are asked for and not there are refused, with and without new tokens."""
+    batch, width = 4096, 2**19 + 1024  # 8.6 GB of table, of which nothing is read
+    table = torch.empty((batch, width), dtype=torch.int32, device=device)
+    zeros = lambda n: torch.zeros(n, dtype=torch.int32, device=device)  # noqa: E731
+    pool = shk.KVPages(table, zeros(batch), zeros(batch), torch.arange(8, dtype=torch.int32, device=device),
+                       torch.full((1,), 8, dtype=torch.int32, device=device), 16)
+    pool.lengths.fill_(16 * width - 1)
+    pool.lengths[0] = pool.lengths[-1] = 20
+    pool.owned[-1] = 2  # the last one's new token asks for no page
+    table[-1, :2] = torch.tensor([50, 51], dtype=torch.int32)
+    new = torch.ones(batch, dtype=torch.int32, device=device)
+    new[1::2] = 0
+    new[-1] = 1
+    step = shk.kv_pages_step(pool, new, batch)
+    taken = step.taken.tolist()
+    assert taken[0] == taken[-1] == 1 and not any(taken[1:-1])
+    assert pool.lengths.tolist() == [21] + [16 * width - 1] * (batch - 2) + [21]
+    assert pool.owned.tolist() == [2] + [0] * (batch - 2) + [2] and pool.free_count.item() == 6
+    slots, total = step.slots.tolist(), int(new.sum())
+    assert slots[0] == 6 * 16 + 4 and slots[total - 1] == 51 * 16 + 4
+    assert set(slots[1:total - 1]) == {-1} and set(slots[total:]) == {-1}
