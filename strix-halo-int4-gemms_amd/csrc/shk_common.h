@@ -76,8 +76,8 @@ __device__ __forceinline__ uint32_t f32_to_bf16_rne(float f) {
 }
 
 // Two fp32 values -> packed bf16 pair with v_cvt_pk_bf16_f32 (round to
-// nearest even, subnormals kept).  Only for values that are not NaN: the
-// instruction keeps a NaN's payload where torch writes 0x7FC0.
+// nearest even, subnormals kept).  Only for values that are not NaN, or where any
+// NaN will do: the instruction keeps its payload where torch writes 0x7FC0.
 typedef float shk_f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 shk_bf2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16x2_nonan(float a, float b) {

@@ -39,9 +39,10 @@ __device__ __forceinline__ v4f mfma128(const v8i& b, const v8i& a) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, v4f{0.f, 0.f, 0.f, 0.f}, KIND_B, KIND_A, 0, 0, 0, 0);
 }
 
+// (A NaN keeps its payload, in whichever of these forms a column is stored.)
 __device__ __forceinline__ void store_value(const Fp8Product& p, long at, float v) {
   if (p.out_type == SHK_SRC_F32) static_cast<float*>(p.out)[at] = v;
-  else if (p.out_type == SHK_SRC_BF16) static_cast<uint16_t*>(p.out)[at] = (uint16_t)f32_to_bf16_rne(v);
+  else if (p.out_type == SHK_SRC_BF16) static_cast<uint16_t*>(p.out)[at] = (uint16_t)pack_bf16x2_nonan(v, 0.f);
   else static_cast<_Float16*>(p.out)[at] = (_Float16)v;
 }
 

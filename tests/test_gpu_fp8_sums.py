@@ -91,3 +91,14 @@ def test_tiles(device, m, n, k, large, one_sign, gain):
         got = _multiplied(device, a, b, sa, sb, out_dtype).cpu().double()[rows]
         part = (a[rows], b, sa[rows], sb)
         _within(got, *(_bounds(*part, F32) if out_dtype == F32 else ref.product(*part, out_dtype)), out_dtype)
+
+
+# few rows, tiles of 64 x 64 whole and with K cut, of 64 x 128 and of 256 x 256
+@pytest.mark.parametrize("m,n,k", [(5, 301, 300), (100, 503, 300), (65, 203, 3100), (1000, 3003, 200), (2500, 2703, 300)])
+@pytest.mark.parametrize("out_dtype", [BF16, F16])
+def test_a_nan_has_the_same_bits_in_every_column(device, m, n, k, out_dtype):
+    a, b, sa, sb = _operands("nan", m, n, k, m=m, n=n, k=k, large=1.0, one_sign=False)
+    sa.view(torch.int32)[3, 0] = 0x7FD23456
+    got = _multiplied(device, a, b, sa * 2.0**-9, sb, out_dtype)
+    assert got[3].isnan().all() and torch.isfinite(got[:3]).all() and torch.isfinite(got[4:]).all()
+    assert got[3].view(torch.int16).unique().numel() == 1
