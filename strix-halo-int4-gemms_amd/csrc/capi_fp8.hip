@@ -33,9 +33,11 @@ int check_mm(const shk_fp8_mm* a) {
   if (a->m < 0 || a->n < 0 || a->k < 0 || a->m > INT_MAX / 4 || a->n > INT_MAX / 4 || a->k >= (1 << 23))
     return capi_fail("m and n are from 0 to 536870911, k to 8388607");
   if (a->m * a->n == 0) return 0;
-  // a launch holds fewer than 2^32 work-items: 256 for 64 x 128 results, 512 for 64
-  // columns of few rows, and one for 16 bytes of an operand that is copied
-  if ((__int128)((a->m + 63) / 64) * ((a->n + 127) / 128) > 0xFFFFFF || (a->m <= 32 && a->n > (1LL << 29) - 64) ||
+  // a launch holds fewer than 2^32 work-items: 256 for 64 x 128 results (64 x 64 where
+  // K has no values), 512 for 64 columns of few rows, and one for 16 bytes of an
+  // operand that is copied
+  const int64_t columns = a->k == 0 ? 64 : 128;
+  if ((__int128)((a->m + 63) / 64) * ((a->n + columns - 1) / columns) > 0xFFFFFF || (a->m <= 32 && a->n > (1LL << 29) - 64) ||
       (a->k > 0 && std::max(a->m, a->n) > 0xFFFFFF00LL / ((a->k + 15) / 16)))
     return capi_fail("too many outputs for one launch");
   if (a->a_pitch < a->k || a->b_pitch < a->k || a->a_pitch >= (1 << 24) || a->b_pitch >= (1 << 24))

@@ -6,8 +6,8 @@ import pytest
 
 pytest.importorskip("torch")
 
-from amd_strix_halo_kernels import kv_pages, native  # noqa: E402
-from tests.test_step_host import PLAN  # noqa: E402
+from amd_strix_halo_kernels import fp8, kv_pages, native  # noqa: E402
+from tests.test_step_host import MM, PLAN  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -20,3 +20,19 @@ def test_stacks_of_pages(lib):
     packed = kv_pages._PLAN.pack(*(PLAN | {"free_total": 2**31 - 1}).values())
     assert lib.amd_strix_halo_kernels_kv_plan(0, 0, packed) == 1
     assert b"2147483646 places" in lib.amd_strix_halo_kernels_last_error()
+
+
+@pytest.mark.parametrize("k", [0, 1, 256])
+@pytest.mark.parametrize("out_type", [0, 1, 2])
+def test_products_hold_their_launch(lib, k, out_type):
+    """Fewer than 2^32 work-items of 64 x 64 results where K has no values, of 64 x 128 where it has."""
+    tiles = 0xFFFFFF
+    columns = 64 if k == 0 else 128
+    fits = MM | {"m": 64 * 4095, "n": columns * (tiles // 4095), "k": k, "out_type": out_type}
+    for args, good in ((fits, True), (fits | {"n": fits["n"] + columns}, False)):
+        args = args | {"out_stride": args["n"], "b_rows": 128, "a_scale_row": 1, "a_scale_block": 0, "b_scale_row": 1,
+                       "b_scale_block": 0}
+        nbytes = lib.amd_strix_halo_kernels_fp8_mm_workspace(fp8._MM.pack(*args.values()))
+        assert (nbytes >= 0) == good, (k, args["n"])
+        if not good:
+            assert b"too many outputs" in lib.amd_strix_halo_kernels_last_error()
