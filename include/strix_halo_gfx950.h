@@ -661,7 +661,8 @@ int amd_strix_halo_kernels_fp8_mm(int device_index, uintptr_t stream, const shk_
  * and, with c_i + j s_i = amplitude * exp(j * positions[t] * 2 pi * turns[i]),
  * pair i of the first `rotated` values becomes (a c_i - b s_i, b c_i + a s_i):
  * its values are 2i and 2i + 1 (interleaved) or i and i + rotated / 2.  The other
- * values stay n.  Angles are reduced in 64 bits; the rest is f32, rounded once.
+ * values stay n.  Angles are formed and reduced in 64 bits (to 2^-53 of the whole
+ * angle); the rest is f32, rounded once.
  * Outputs go to q_out and k_out (which may be q and k with their strides).  With
  * a cache, k_out is null and the keys, rounded to their type, go with `values`
  * [tokens, kv_heads, head_dim] into slots[t], as amd_strix_halo_kernels_kv_write

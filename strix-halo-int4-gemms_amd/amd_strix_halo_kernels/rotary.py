@@ -4,9 +4,10 @@ No counterpart in the reference.  ``rotary_frequencies`` gives how fast each
 pair of a head turns with the position, plain or for a context longer than the
 trained one; ``new_rotary`` puts that on a device, and ``rotate_qk`` norms and
 turns the heads of new tokens in one pass, the keys, with their values, straight
-into a quantized cache if there is one.  Angles are reduced in 64 bits, so a far
-position turns as exactly as a near one.  There is no CPU path, and asking a
-result for a gradient raises.
+into a quantized cache if there is one.  Angles are formed and reduced in 64
+bits: off by at most 2^-52 of the whole angle, which up to 10^8 radians is less
+than 32 bits lose of what is left of it.  There is no CPU path, and asking a result
+for a gradient raises.
 """
 
 from __future__ import annotations
@@ -16,7 +17,6 @@ import struct
 from dataclasses import dataclass
 from typing import Any, Sequence
 
-from . import kernel_table as kt
 from .kv_cache import KVCache, _check_slots, _row_type
 from .native import (
     _check,
@@ -136,7 +136,8 @@ def rotate_qk(
     With ``q_weight`` and ``k_weight`` [head_dim] (q's dtype or f32) each head is
     first normed, ``x / sqrt(mean(x^2) + eps) * weight``.  Then the first
     ``rotary.rotated`` of its values turn by ``positions`` [tokens] (int64 or
-    int32, any value); the others stay.  Sums and products are f32, rounded once.
+    int32, any value; above 2^53 rounded to 53 bits); the others stay.  Sums and
+    products are f32, rounded once.
 
     Returns ``(q, k)`` of the inputs' dtype, in ``q_out`` and ``k_out`` if given
     (``q`` and ``k`` themselves for a result in place).  With a ``cache``, the

@@ -7,7 +7,9 @@
 // lanes.  A workgroup takes whole rounds of rows, first all its loads; while they
 // are on their way its threads compute the angles of the tokens that it meets
 // into LDS.  An angle is positions * turns in 64 bits, less its nearest quarter:
-// what is left is at most an eighth of a turn, exact in f32 to 2^-24 of itself.
+// what is left is at most an eighth of a turn, held in f32 to 2^-24 of itself beside
+// the 2^-53 of the whole angle that the product loses, and as much that `turns` did
+// (together less, up to 2^27 radians).
 //
 // Bound by memory, and by latency for a few tokens.  8191 tokens of 40 heads of 128
 // (168 MB): 35 us, 4.8 TB/s.  The vector unit is near: 44 us before addresses took
