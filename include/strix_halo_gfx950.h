@@ -663,10 +663,11 @@ int amd_strix_halo_kernels_fp8_mm(int device_index, uintptr_t stream, const shk_
  * its values are 2i and 2i + 1 (interleaved) or i and i + rotated / 2.  The other
  * values stay n.  Angles are formed and reduced in 64 bits (to 2^-53 of the whole
  * angle); the rest is f32, rounded once.
- * Outputs go to q_out and k_out (which may be q and k with their strides).  With
- * a cache, k_out is null and the keys, rounded to their type, go with `values`
- * [tokens, kv_heads, head_dim] into slots[t], as amd_strix_halo_kernels_kv_write
- * puts them there; head_dim and kv_heads are then the cache's. */
+ * Outputs go to q_out and k_out (which may be q and k with their strides; rows must
+ * not overlap).  With a cache, k_out is null and the keys, rounded to their type, go
+ * with `values` [tokens, kv_heads, head_dim] into slots[t], as
+ * amd_strix_halo_kernels_kv_write puts them there; head_dim and kv_heads are then the
+ * cache's. */
 typedef struct shk_rotate {
   const void* q;
   int64_t q_token_stride;

@@ -140,7 +140,7 @@ def rotate_qk(
     products are f32, rounded once.
 
     Returns ``(q, k)`` of the inputs' dtype, in ``q_out`` and ``k_out`` if given
-    (``q`` and ``k`` themselves for a result in place).  With a ``cache``, the
+    (``q`` and ``k`` themselves for a result in place; rows that overlap raise).  With a ``cache``, the
     keys and ``values`` [tokens, kv_heads, head_dim] go into ``slots`` as
     ``kv_cache_write`` puts them there, without the keys' way through memory,
     and q alone is returned.

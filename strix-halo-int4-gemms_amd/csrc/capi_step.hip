@@ -2,6 +2,7 @@
 // and launches.  Declarations are in include/strix_halo_gfx950.h.
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <string>
 
 #include "shk_capi.h"
@@ -43,6 +44,13 @@ int check_rotate(const shk_kv_cache* c, const shk_rotate* args) {
                        std::to_string(c->kv_heads));
     if (a.slot_bytes != 4 && a.slot_bytes != 8) return capi_fail("slots are int32 or int64");
   }
+  const auto apart = [&](int64_t token_stride, int64_t head_stride, int64_t heads) {
+    return (a.tokens <= 1 || std::llabs(token_stride) >= a.head_dim) &&
+           (heads <= 1 || std::llabs(head_stride) >= a.head_dim);
+  };
+  if (!apart(a.q_out_token_stride, a.q_out_head_stride, a.heads) ||
+      (c == nullptr && !apart(a.k_out_token_stride, a.k_out_head_stride, a.kv_heads)))
+    return capi_fail("rows of q_out and k_out must not overlap");
   return 0;
 }
 

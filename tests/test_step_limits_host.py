@@ -6,8 +6,8 @@ import pytest
 
 pytest.importorskip("torch")
 
-from amd_strix_halo_kernels import fp8, kv_pages, native  # noqa: E402
-from tests.test_step_host import MM, PLAN  # noqa: E402
+from amd_strix_halo_kernels import fp8, kv_pages, native, rotary  # noqa: E402
+from tests.test_step_host import MM, PLAN, ROTATE  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -36,3 +36,17 @@ def test_products_hold_their_launch(lib, k, out_type):
         assert (nbytes >= 0) == good, (k, args["n"])
         if not good:
             assert b"too many outputs" in lib.amd_strix_halo_kernels_last_error()
+
+
+@pytest.mark.parametrize("bad", [{"qot": 0}, {"qoh": 0}, {"kot": 0}, {"koh": 0}, {"qoh": 63}, {"kot": 63}])
+def test_rotated_rows_lie_apart(lib, bad):
+    """Expanded outputs would be written by several rows at once."""
+    assert lib.amd_strix_halo_kernels_rotate(0, 0, None, rotary._ROTATE.pack(*(ROTATE | bad).values())) == 1
+    assert b"must not overlap" in lib.amd_strix_halo_kernels_last_error()
+
+
+def test_strides_of_one_row_may_be_anything(lib):
+    """One token's, or one head's: the call fails for its missing q alone."""
+    one = ROTATE | {"tokens": 1, "heads": 1, "kv_heads": 1, "qot": 0, "qoh": 0, "kot": 0, "koh": 0, "q": 0}
+    assert lib.amd_strix_halo_kernels_rotate(0, 0, None, rotary._ROTATE.pack(*one.values())) == 1
+    assert b"non-null" in lib.amd_strix_halo_kernels_last_error()
