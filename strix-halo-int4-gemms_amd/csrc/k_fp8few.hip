@@ -8,9 +8,9 @@
 // for each 16 x 16 results, and folds it into its own f32 sums.  Behind the loop the
 // eight sums are added in LDS, in order of the waves.
 // Results of all types go through the f16 matrix unit, whose sums are f32 ones
-// (k_fp8.hip says what the 8-bit one keeps): widening the codes hides behind b, 16 x
-// 11008 x 4096 in 11.1 us where the 8-bit unit takes 10.9, 32 x 4096 x 4096 in 9.8
-// and 9.6.
+// (k_fp8.hip says what the 8-bit one keeps): widening the codes hides behind b but
+// for 1 to 3%, 16 x 11008 x 4096 in 11.1 us where the 8-bit unit takes 10.9, 32 x
+// 4096 x 4096 in 9.8 and 9.6, 64 x 4096 x 1024 in 6.0 and 5.8.
 // K is not cut over workgroups: 16 rows of b keep a CU's share of the memory rate
 // busy, and a sum over workgroups would be another launch.
 // Bound by that share: b at 4 TB/s.
