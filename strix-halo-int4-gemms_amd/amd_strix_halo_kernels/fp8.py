@@ -215,6 +215,6 @@ def mm_fp8(a: Any, b: Any, *, a_scale: Any, b_scale: Any, out_dtype: Any = None,
         work = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _check(lib, lib.amd_strix_halo_kernels_fp8_mm(
             index, _current_stream(torch, index), _MM.pack(*given, 0 if work is None else work.data_ptr(), nbytes)))
-    if a_scale.requires_grad or b_scale.requires_grad:
-        return _no_gradient(torch, "mm_fp8", out, a_scale, b_scale)
+    if a_scale.requires_grad or b_scale.requires_grad or a.requires_grad or b.requires_grad:
+        return _no_gradient(torch, "mm_fp8", out, a, b, a_scale, b_scale)
     return out
